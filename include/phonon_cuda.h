@@ -433,6 +433,110 @@ int phonon_cuda_mimi_set_tensor_min(PhononCudaMimi *mimi, uint32_t min_states, i
 int phonon_cuda_mimi_process(PhononCudaMimi *mimi, uint32_t state, const float *latents, size_t frames,
                              float *features, size_t capacity);
 
+/* ---- 8-bit paged K/V cache: write, read back, attend ----
+ * A cache of any head layout beside the context's fixed 8 x 64, at one byte an
+ * element. A page holds 16 positions of every K/V head; the 16 x head_dim keys
+ * of a head in a page share one power-of-two scale 2^e, and so do the values:
+ * e is the smallest integer in [-48, 64] for which no element of the block
+ * exceeds 127 * 2^e, and an element x is held as the integer nearest x / 2^e
+ * (ties to even, at most 127 in magnitude). Rows appended to a page that holds
+ * earlier positions of the sequence can raise its scale, never lower it; the
+ * integers that are there are then divided by the ratio of the scales and
+ * rounded again. Reading back is exact.
+ *
+ * The caller owns the page tables. A call works on a batch of sequences,
+ * described by arrays in device memory; position p of sequence i lies in page
+ * pages[i * page_stride + p / 16]. Sequence i holds lengths[i] positions, and
+ * the call's rows [row_begin[i], row_begin[i + 1]) are its LAST positions
+ * (append writes them, read fetches them, attention has a query for each).
+ * max_rows and max_length bound every sequence's rows and length; the host
+ * picks the launch by them, so tight bounds are faster.
+ *
+ * Calls enqueue on `cuda_stream` (a cudaStream_t, may be 0) of the cache's
+ * device, allocate nothing, do not synchronise and can be captured; the
+ * calling thread's current device is left as it was. status_dev (device,
+ * [sequences], optional, zeroed by the caller) is raised to a PhononCudaStatus
+ * for a sequence whose
+ *   - length is negative or above max_length (CAPACITY): it counts as empty;
+ *   - rows lie outside [0, rows) or exceed max_rows (INVALID_ARGUMENT): none
+ *     of its rows is read or written;
+ *   - page id lies outside the pool (INVALID_ARGUMENT): that page is not
+ *     written, reads as zeros, and no query sees it;
+ *   - rows hold a non-finite value (NON_FINITE): append holds such an element
+ *     as 0, and a query row with one gets NaN.
+ * The largest code stays. A page that a call appends to belongs to one
+ * sequence of the batch; pages that are only read may be shared. Calls on one
+ * cache may run at the same time as long as none writes a page that another
+ * uses. */
+typedef enum { PHONON_CUDA_ROWS_F32 = 0, PHONON_CUDA_ROWS_BF16 = 1 } PhononCudaRowType;
+
+typedef struct {
+    int device;          /* CUDA ordinal */
+    uint32_t layers;     /* 1..1024; every layer has pool_pages pages */
+    uint32_t kv_heads;   /* 1..1024 */
+    uint32_t head_dim;   /* 32, 64 or 128 */
+    uint32_t pool_pages; /* pages per layer */
+} PhononCudaKv8Config;
+
+typedef struct {
+    uint32_t sequences;       /* at least 1 */
+    uint32_t rows;            /* rows of the call's row arrays; 0 does nothing */
+    const int32_t *row_begin; /* device [sequences + 1], or NULL: one row per sequence */
+    const int32_t *lengths;   /* device [sequences], the call's rows included */
+    const int32_t *pages;     /* device [sequences][page_stride] */
+    uint32_t page_stride;
+    uint32_t max_rows;        /* at least 1 */
+    uint32_t max_length;      /* at most page_stride * 16 */
+} PhononCudaKv8Batch;
+
+/* Key and value rows [rows][kv_heads][head_dim], `stride` elements from row to
+ * row (0: packed). Pointers are 16-byte aligned, strides multiples of 8. */
+typedef struct {
+    uint32_t type; /* PhononCudaRowType */
+    uint64_t stride;
+    void *keys, *values; /* append only reads them */
+} PhononCudaKv8Rows;
+
+typedef struct PhononCudaKv8 PhononCudaKv8;
+int phonon_cuda_kv8_create(const PhononCudaKv8Config *config, PhononCudaKv8 **out);
+/* No call on the cache may be running. */
+void phonon_cuda_kv8_destroy(PhononCudaKv8 *cache);
+/* Bytes of device memory: 2 * head_dim + 1/8 per position and head. */
+size_t phonon_cuda_kv8_bytes(const PhononCudaKv8 *cache);
+/* Quantise rows as they are written. A sequence whose rows start a page drops
+ * what the page held; positions behind the new length are unspecified. Rows
+ * that would lie before position 0 (more rows than length) are not written. */
+int phonon_cuda_kv8_append_device(PhononCudaKv8 *cache, uint32_t layer, const PhononCudaKv8Batch *batch,
+                                  const PhononCudaKv8Rows *rows, int32_t *status_dev, void *cuda_stream);
+/* Read positions back; rows before position 0 become 0. */
+int phonon_cuda_kv8_read_device(PhononCudaKv8 *cache, uint32_t layer, const PhononCudaKv8Batch *batch,
+                                const PhononCudaKv8Rows *rows, int32_t *status_dev, void *cuda_stream);
+
+/* Scratch of the attention calls on a cache's device (about 22 MB). Calls that
+ * may run at the same time, captured ones included, need one each. */
+typedef struct PhononCudaKv8Workspace PhononCudaKv8Workspace;
+int phonon_cuda_kv8_workspace_create(PhononCudaKv8 *cache, PhononCudaKv8Workspace **out);
+void phonon_cuda_kv8_workspace_destroy(PhononCudaKv8Workspace *workspace);
+
+/* Causal attention of query rows over the cache (flow_attention,
+ * src/phonon_transformer.c:340-404, for any head layout and any number of
+ * rows): the row at position p sees positions (p - window, p], or [0, p] where
+ * window is 0. q and out are [rows][heads][head_dim], heads a multiple of
+ * kv_heads (query head h reads K/V head h / (heads / kv_heads)); out may be q.
+ * A row that sees nothing gets 0. */
+typedef struct {
+    uint32_t type;   /* PhononCudaRowType of q and out */
+    uint32_t heads;
+    uint32_t window; /* 0: none */
+    float scale;     /* of the scores; 0: 1 / sqrt(head_dim) */
+    const void *q;
+    void *out;
+    uint64_t q_stride, out_stride; /* elements from row to row (0: packed) */
+} PhononCudaKv8Query;
+int phonon_cuda_kv8_attention_device(PhononCudaKv8 *cache, uint32_t layer, const PhononCudaKv8Batch *batch,
+                                     const PhononCudaKv8Query *query, PhononCudaKv8Workspace *workspace,
+                                     int32_t *status_dev, void *cuda_stream);
+
 const char *phonon_cuda_status_string(int status);
 
 #ifdef __cplusplus

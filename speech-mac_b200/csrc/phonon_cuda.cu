@@ -8,6 +8,7 @@
 #include "phonon_persist.cuh"
 #include "phonon_head.cuh"
 #include "phonon_mimi.cuh"
+#include "phonon_kv8.cuh"
 
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -47,6 +48,9 @@ constexpr uint32_t kClusterMaxPosBf16 = 1248;  // ... bf16 K/V
 constexpr int kTicketMinChunk = 8;   // pages per guided chunk, at least
 constexpr int kMaxChunks = 8192;     // chunks per plan, at most
 constexpr int kSplitMinBatch = 96;   // from here a step runs as two concurrent half batches
+constexpr int kKv8Ctas = 8;          // 8-bit attention: CTAs per SM that a split call aims at
+constexpr int kKv8MinPages = 8;      // ... pages per split, at least (two a warp)
+constexpr int kKv8TileFloats = 2048; // ... outputs of a row tile, at most
 
 #define CUDA_TRY(expr)                                                                       \
     do {                                                                                     \
@@ -419,6 +423,181 @@ cudaError_t launch_digits(const float* x, int ldx, const float* ln_w, const floa
         constexpr int rows_per_cta = 256 / (kCols / 8);
         return launch_pdl(digits_kernel<kCols>, dim3((Bpad + rows_per_cta - 1) / rows_per_cta), dim3(256), 0, s, x,
                           ldx, B, Bpad, digits, exps, status);
+    }
+}
+
+// ---------------------------------------------------------- 8-bit K/V cache
+// The device memory of a cache (phonon_kv8.cuh): every integer 0 and every
+// scale the smallest until rows are written.
+struct Kv8Pool {
+    uint8_t* pool = nullptr;
+    int8_t* exps = nullptr;
+    uint32_t layers = 0, pages = 0, heads = 0, dim = 0;
+    size_t layer_bytes() const { return static_cast<size_t>(pages) * heads * 2 * kKv8Block * dim; }
+    size_t layer_exps() const { return static_cast<size_t>(pages) * heads * 2; }
+    size_t bytes() const { return layers * (layer_bytes() + layer_exps()); }
+    Kv8View view(uint32_t layer) const {
+        return Kv8View{pool + layer * layer_bytes(), exps + layer * layer_exps(), static_cast<int>(pages),
+                       static_cast<int>(heads)};
+    }
+    int alloc(uint32_t n_layers, uint32_t n_pages, uint32_t n_heads, uint32_t head_dim) {
+        layers = n_layers;
+        pages = n_pages;
+        heads = n_heads;
+        dim = head_dim;
+        if (cudaMalloc(&pool, layers * layer_bytes()) != cudaSuccess ||
+            cudaMalloc(&exps, layers * layer_exps()) != cudaSuccess) {
+            cudaGetLastError();
+            release();
+            return PHONON_CUDA_OUT_OF_MEMORY;
+        }
+        CUDA_TRY(cudaMemset(pool, 128, layers * layer_bytes()));
+        CUDA_TRY(cudaMemset(exps, kKv8MinExp & 0xff, layers * layer_exps()));
+        CUDA_TRY(cudaStreamSynchronize(nullptr));  // callers' streams do not wait for the legacy stream
+        return PHONON_CUDA_OK;
+    }
+    void release() {
+        if (pool) cudaFree(pool);
+        if (exps) cudaFree(exps);
+        pool = nullptr;
+        exps = nullptr;
+    }
+};
+
+// Where split attention calls leave their partial results. One call in
+// flight uses it at a time; the arrival counters are back at zero when a call
+// has ended.
+struct Kv8Scratch {
+    float* part = nullptr;
+    float2* ml = nullptr;
+    unsigned* arrived = nullptr;
+    int max_splits = 0;  // CTAs of a split call, at most
+    int alloc(int sms) {
+        // A call is split only while its (sequence, tile, head) items are
+        // fewer than the CTAs that it aims at, and into no more of them than
+        // that plus one per item (kv8_enqueue_attention).
+        max_splits = 2 * kKv8Ctas * sms;
+        if (cudaMalloc(&part, static_cast<size_t>(max_splits) * kKv8TileFloats * 4) != cudaSuccess ||
+            cudaMalloc(&ml, static_cast<size_t>(max_splits) * 32 * sizeof(float2)) != cudaSuccess ||
+            cudaMalloc(&arrived, static_cast<size_t>(max_splits) * 4) != cudaSuccess) {
+            cudaGetLastError();
+            release();
+            return PHONON_CUDA_OUT_OF_MEMORY;
+        }
+        CUDA_TRY(cudaMemset(arrived, 0, static_cast<size_t>(max_splits) * 4));
+        CUDA_TRY(cudaStreamSynchronize(nullptr));
+        return PHONON_CUDA_OK;
+    }
+    void release() {
+        if (part) cudaFree(part);
+        if (ml) cudaFree(ml);
+        if (arrived) cudaFree(arrived);
+        part = nullptr;
+        ml = nullptr;
+        arrived = nullptr;
+    }
+};
+
+// Blocks that `rows` consecutive positions touch, at most.
+int kv8_blocks(int rows) { return (rows + kKv8Block - 2) / kKv8Block + 1; }
+
+template <typename Params, typename Kernel>
+int kv8_launch_rows(Kernel kernel, const Params& p, cudaStream_t s) {
+    const long long warps = static_cast<long long>(p.seqs.n) * p.blocks * p.cache.heads * 2;
+    const long long ctas = (warps + 3) / 4;
+    if (ctas > INT32_MAX) return PHONON_CUDA_CAPACITY;
+    CUDA_TRY(launch_pdl(kernel, dim3(static_cast<unsigned>(ctas)), dim3(128), 0, s, p));
+    return PHONON_CUDA_OK;
+}
+
+int kv8_enqueue_append(const Kv8Pool& c, uint32_t layer, const Kv8Seqs& seqs, bool bf16, const void* keys,
+                       const void* values, long long stride, cudaStream_t s) {
+    Kv8AppendParams p{c.view(layer), seqs, {keys, values}, stride, kv8_blocks(seqs.max_rows)};
+    switch (c.dim) {
+        case 32: return kv8_launch_rows(bf16 ? kv8_append_kernel<32, true> : kv8_append_kernel<32, false>, p, s);
+        case 64: return kv8_launch_rows(bf16 ? kv8_append_kernel<64, true> : kv8_append_kernel<64, false>, p, s);
+        default: return kv8_launch_rows(bf16 ? kv8_append_kernel<128, true> : kv8_append_kernel<128, false>, p, s);
+    }
+}
+
+int kv8_enqueue_read(const Kv8Pool& c, uint32_t layer, const Kv8Seqs& seqs, bool bf16, void* keys, void* values,
+                     long long stride, cudaStream_t s) {
+    Kv8ReadParams p{c.view(layer), seqs, {keys, values}, stride, kv8_blocks(seqs.max_rows)};
+    switch (c.dim) {
+        case 32: return kv8_launch_rows(bf16 ? kv8_read_kernel<32, true> : kv8_read_kernel<32, false>, p, s);
+        case 64: return kv8_launch_rows(bf16 ? kv8_read_kernel<64, true> : kv8_read_kernel<64, false>, p, s);
+        default: return kv8_launch_rows(bf16 ? kv8_read_kernel<128, true> : kv8_read_kernel<128, false>, p, s);
+    }
+}
+
+struct Kv8Attend {
+    const void* q;
+    void* out;
+    long long q_stride, out_stride;
+    int group;
+    float scale;
+    int window;
+    bool bf16;
+};
+
+template <int D, int NT, int PB, bool kBf16>
+int kv8_launch_attention(const Kv8Pool& c, uint32_t layer, const Kv8Seqs& seqs, const Kv8Attend& a,
+                         const Kv8Scratch& w, int sms, cudaStream_t s) {
+    static_assert(8 * NT * D <= kKv8TileFloats, "a partial result outgrows its scratch");
+    Kv8AttnParams p{};
+    p.cache = c.view(layer);
+    p.seqs = seqs;
+    p.q = a.q;
+    p.out = a.out;
+    p.q_stride = a.q_stride;
+    p.out_stride = a.out_stride;
+    p.group = a.group;
+    p.scale = a.scale * 1.44269504088896340736f;
+    p.window = a.window;
+    const long long rows = static_cast<long long>(seqs.max_rows) * a.group;
+    p.tiles = static_cast<int>((rows + 8 * NT - 1) / (8 * NT));
+    const long long items = static_cast<long long>(seqs.n) * p.tiles * c.heads;
+    // pages that a row tile can see
+    long long span = seqs.max_length;
+    if (a.window) span = std::min<long long>(span, static_cast<long long>(a.window) + (8 * NT - 1) / a.group + kKv8Block);
+    const long long pages = std::max<long long>(1, (span + kKv8Block - 1) / kKv8Block);
+    const long long want = static_cast<long long>(kKv8Ctas) * sms;
+    long long splits = items >= want ? 1 : (want + items - 1) / items;
+    splits = std::max<long long>(1, std::min(splits, (pages + kKv8MinPages - 1) / kKv8MinPages));
+    if (items * splits > INT32_MAX) return PHONON_CUDA_CAPACITY;
+    if (splits > 1 && items * splits > w.max_splits) return PHONON_CUDA_CAPACITY;
+    p.splits = static_cast<int>(splits);
+    p.split_pages = static_cast<int>((pages + splits - 1) / splits);
+    p.part = w.part;
+    p.part_ml = w.ml;
+    p.arrived = w.arrived;
+    CUDA_TRY(launch_pdl(kv8_attention_kernel<D, NT, PB, kBf16>, dim3(static_cast<unsigned>(items * splits)),
+                        dim3(32 * kKv8Warps), 0, s, p));
+    return PHONON_CUDA_OK;
+}
+
+template <int D, int PB, bool kBf16>
+int kv8_attention_rows(const Kv8Pool& c, uint32_t layer, const Kv8Seqs& seqs, const Kv8Attend& a, const Kv8Scratch& w,
+                       int sms, cudaStream_t s) {
+    const long long rows = static_cast<long long>(seqs.max_rows) * a.group;
+    if (rows <= 8) return kv8_launch_attention<D, 1, PB, kBf16>(c, layer, seqs, a, w, sms, s);
+    if (rows <= 16 || D == 128) return kv8_launch_attention<D, 2, PB / 2, kBf16>(c, layer, seqs, a, w, sms, s);
+    if constexpr (D < 128) return kv8_launch_attention<D, 4, PB / 4, kBf16>(c, layer, seqs, a, w, sms, s);
+    return PHONON_CUDA_INVALID_ARGUMENT;
+}
+
+int kv8_enqueue_attention(const Kv8Pool& c, uint32_t layer, const Kv8Seqs& seqs, const Kv8Attend& a,
+                          const Kv8Scratch& w, int sms, cudaStream_t s) {
+    switch (c.dim) {
+        case 32:
+            return a.bf16 ? kv8_attention_rows<32, 4, true>(c, layer, seqs, a, w, sms, s)
+                          : kv8_attention_rows<32, 4, false>(c, layer, seqs, a, w, sms, s);
+        case 64:
+            return a.bf16 ? kv8_attention_rows<64, 4, true>(c, layer, seqs, a, w, sms, s)
+                          : kv8_attention_rows<64, 4, false>(c, layer, seqs, a, w, sms, s);
+        default:
+            return a.bf16 ? kv8_attention_rows<128, 2, true>(c, layer, seqs, a, w, sms, s)
+                          : kv8_attention_rows<128, 2, false>(c, layer, seqs, a, w, sms, s);
     }
 }
 
@@ -4062,6 +4241,187 @@ int phonon_cuda_mimi_process(PhononCudaMimi* m, uint32_t state, const float* lat
         if (st_row) return st_row;
     }
     return PHONON_CUDA_OK;
+}
+
+}  // extern "C"
+
+// ====================================================== 8-bit paged K/V cache
+struct PhononCudaKv8 {
+    int device = 0, sms = 0;
+    Kv8Pool pool;
+};
+
+struct PhononCudaKv8Workspace {
+    int device = 0;
+    Kv8Scratch scratch;
+};
+
+namespace {
+
+// The calling thread's current device, put back on the way out.
+struct DeviceGuard {
+    int before = -1;
+    bool ok = false;
+    explicit DeviceGuard(int device) {
+        if (cudaGetDevice(&before) != cudaSuccess) {
+            cudaGetLastError();
+            before = -1;
+            return;
+        }
+        ok = before == device || cudaSetDevice(device) == cudaSuccess;
+        if (!ok) cudaGetLastError();
+        if (before == device) before = -1;
+    }
+    ~DeviceGuard() {
+        if (before >= 0) cudaSetDevice(before);
+    }
+    DeviceGuard(const DeviceGuard&) = delete;
+    DeviceGuard& operator=(const DeviceGuard&) = delete;
+};
+
+bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+
+// Rows of `width` elements, `stride` apart (0: packed), that are read and
+// written four elements (16 or 8 bytes) at a time.
+bool kv8_stride(uint64_t stride, uint64_t width, long long* out) {
+    if (stride == 0) stride = width;
+    if (stride < width || stride % 8 || stride > (1ull << 40)) return false;
+    *out = static_cast<long long>(stride);
+    return true;
+}
+
+bool kv8_seqs(const PhononCudaKv8Batch* b, int32_t* status, Kv8Seqs* out) {
+    if (!b || !b->lengths || !b->pages || b->sequences == 0 || b->sequences > (1u << 24) || b->rows > (1u << 30) ||
+        b->max_rows == 0 || b->max_rows > (1u << 30) || b->page_stride == 0 || b->page_stride > (1u << 26) ||
+        b->max_length > (1u << 30) || b->max_length > static_cast<uint64_t>(b->page_stride) * kKv8Block)
+        return false;
+    if (!b->row_begin && b->rows != b->sequences) return false;
+    *out = Kv8Seqs{static_cast<int>(b->sequences), static_cast<int>(b->rows), 1, b->row_begin, b->lengths, 0, nullptr,
+                   b->pages, static_cast<int>(b->page_stride), static_cast<int>(b->max_rows),
+                   static_cast<int>(b->max_length), status};
+    return true;
+}
+
+bool kv8_rows_ok(const PhononCudaKv8* c, const PhononCudaKv8Rows* r, long long* stride) {
+    return r && r->keys && r->values && r->type <= PHONON_CUDA_ROWS_BF16 && aligned16(r->keys) && aligned16(r->values) &&
+           kv8_stride(r->stride, static_cast<uint64_t>(c->pool.heads) * c->pool.dim, stride);
+}
+
+}  // namespace
+
+extern "C" {
+
+int phonon_cuda_kv8_create(const PhononCudaKv8Config* cfg, PhononCudaKv8** out) {
+    if (!out) return PHONON_CUDA_INVALID_ARGUMENT;
+    *out = nullptr;
+    if (!cfg || cfg->layers < 1 || cfg->layers > 1024 || cfg->kv_heads < 1 || cfg->kv_heads > 1024 ||
+        (cfg->head_dim != 32 && cfg->head_dim != 64 && cfg->head_dim != 128) || cfg->pool_pages < 1 ||
+        cfg->pool_pages > (1u << 30))
+        return PHONON_CUDA_INVALID_ARGUMENT;
+    DeviceGuard guard(cfg->device);
+    if (!guard.ok) return PHONON_CUDA_DEVICE_ERROR;
+    PhononCudaKv8* c = new (std::nothrow) PhononCudaKv8();
+    if (!c) return PHONON_CUDA_OUT_OF_MEMORY;
+    c->device = cfg->device;
+    int st = cudaDeviceGetAttribute(&c->sms, cudaDevAttrMultiProcessorCount, cfg->device) == cudaSuccess
+                 ? c->pool.alloc(cfg->layers, cfg->pool_pages, cfg->kv_heads, cfg->head_dim)
+                 : PHONON_CUDA_DEVICE_ERROR;
+    if (st) {
+        c->pool.release();
+        delete c;
+        return st;
+    }
+    *out = c;
+    return PHONON_CUDA_OK;
+}
+
+void phonon_cuda_kv8_destroy(PhononCudaKv8* c) {
+    if (!c) return;
+    DeviceGuard guard(c->device);
+    c->pool.release();
+    delete c;
+}
+
+size_t phonon_cuda_kv8_bytes(const PhononCudaKv8* c) { return c ? c->pool.bytes() : 0; }
+
+int phonon_cuda_kv8_append_device(PhononCudaKv8* c, uint32_t layer, const PhononCudaKv8Batch* batch,
+                                  const PhononCudaKv8Rows* rows, int32_t* status_dev, void* cuda_stream) {
+    Kv8Seqs seqs;
+    long long stride;
+    if (!c || layer >= c->pool.layers || !kv8_seqs(batch, status_dev, &seqs) || !kv8_rows_ok(c, rows, &stride))
+        return PHONON_CUDA_INVALID_ARGUMENT;
+    if (seqs.rows == 0) return PHONON_CUDA_OK;
+    DeviceGuard guard(c->device);
+    if (!guard.ok) return PHONON_CUDA_DEVICE_ERROR;
+    return kv8_enqueue_append(c->pool, layer, seqs, rows->type == PHONON_CUDA_ROWS_BF16, rows->keys, rows->values,
+                              stride, static_cast<cudaStream_t>(cuda_stream));
+}
+
+int phonon_cuda_kv8_read_device(PhononCudaKv8* c, uint32_t layer, const PhononCudaKv8Batch* batch,
+                                const PhononCudaKv8Rows* rows, int32_t* status_dev, void* cuda_stream) {
+    Kv8Seqs seqs;
+    long long stride;
+    if (!c || layer >= c->pool.layers || !kv8_seqs(batch, status_dev, &seqs) || !kv8_rows_ok(c, rows, &stride))
+        return PHONON_CUDA_INVALID_ARGUMENT;
+    if (seqs.rows == 0) return PHONON_CUDA_OK;
+    DeviceGuard guard(c->device);
+    if (!guard.ok) return PHONON_CUDA_DEVICE_ERROR;
+    return kv8_enqueue_read(c->pool, layer, seqs, rows->type == PHONON_CUDA_ROWS_BF16, rows->keys, rows->values, stride,
+                            static_cast<cudaStream_t>(cuda_stream));
+}
+
+int phonon_cuda_kv8_workspace_create(PhononCudaKv8* c, PhononCudaKv8Workspace** out) {
+    if (!out) return PHONON_CUDA_INVALID_ARGUMENT;
+    *out = nullptr;
+    if (!c) return PHONON_CUDA_INVALID_ARGUMENT;
+    DeviceGuard guard(c->device);
+    if (!guard.ok) return PHONON_CUDA_DEVICE_ERROR;
+    PhononCudaKv8Workspace* w = new (std::nothrow) PhononCudaKv8Workspace();
+    if (!w) return PHONON_CUDA_OUT_OF_MEMORY;
+    w->device = c->device;
+    const int st = w->scratch.alloc(c->sms);
+    if (st) {
+        w->scratch.release();
+        delete w;
+        return st;
+    }
+    *out = w;
+    return PHONON_CUDA_OK;
+}
+
+void phonon_cuda_kv8_workspace_destroy(PhononCudaKv8Workspace* w) {
+    if (!w) return;
+    DeviceGuard guard(w->device);
+    w->scratch.release();
+    delete w;
+}
+
+int phonon_cuda_kv8_attention_device(PhononCudaKv8* c, uint32_t layer, const PhononCudaKv8Batch* batch,
+                                     const PhononCudaKv8Query* query, PhononCudaKv8Workspace* workspace,
+                                     int32_t* status_dev, void* cuda_stream) {
+    Kv8Seqs seqs;
+    if (!c || layer >= c->pool.layers || !workspace || workspace->device != c->device ||
+        !kv8_seqs(batch, status_dev, &seqs) || !query || !query->q || !query->out ||
+        query->type > PHONON_CUDA_ROWS_BF16 || !aligned16(query->q) || !aligned16(query->out) || query->heads == 0 ||
+        query->heads % c->pool.heads || query->heads > (1u << 16) || query->window > (1u << 30) ||
+        !std::isfinite(query->scale) || query->scale < 0.0f)
+        return PHONON_CUDA_INVALID_ARGUMENT;
+    Kv8Attend a{};
+    const uint64_t width = static_cast<uint64_t>(query->heads) * c->pool.dim;
+    if (!kv8_stride(query->q_stride, width, &a.q_stride) || !kv8_stride(query->out_stride, width, &a.out_stride))
+        return PHONON_CUDA_INVALID_ARGUMENT;
+    if (seqs.rows == 0) return PHONON_CUDA_OK;
+    a.q = query->q;
+    a.out = query->out;
+    a.group = static_cast<int>(query->heads / c->pool.heads);
+    a.scale = query->scale > 0.0f ? query->scale : static_cast<float>(1.0 / std::sqrt(static_cast<double>(c->pool.dim)));
+    a.window = static_cast<int>(query->window);
+    a.bf16 = query->type == PHONON_CUDA_ROWS_BF16;
+    if (static_cast<long long>(seqs.max_rows) * a.group > (1 << 30)) return PHONON_CUDA_CAPACITY;
+    DeviceGuard guard(c->device);
+    if (!guard.ok) return PHONON_CUDA_DEVICE_ERROR;
+    return kv8_enqueue_attention(c->pool, layer, seqs, a, workspace->scratch, c->sms,
+                                 static_cast<cudaStream_t>(cuda_stream));
 }
 
 }  // extern "C"

@@ -1,0 +1,813 @@
+// The 8-bit paged K/V cache (sm_100a): rows quantised as they are written,
+// read back, and attended over.
+//
+// Format. A block is 16 positions of one K/V head; its keys and its values
+// each share one scale 2^e with e the smallest integer in [kKv8MinExp,
+// kKv8MaxExp] for which |x| <= 127 * 2^e over the block, and an element is
+// held as the integer nearest x / 2^e, at most 127 in magnitude, plus 128.
+// The scale is a power of two so that quantising, raising the scale of a
+// partly filled block (the held integers divided by a power of two and
+// rounded again) and reading back are exact but for the one rounding each
+// names, in any order of operations; it costs at most one of the eight bits
+// against a free scale. A block that fills position by position is rounded
+// again only when its maximum crosses a power of two: the roundings' errors
+// (1/2 unit of each scale, each scale at least twice the one before) sum to
+// less than one unit of the last scale.
+//
+// Layout. pool: [layer][page][head][keys 16*D | values 16*D] bytes, exponents
+// [layer][page][head][2]. Keys lie [position][dim]. Values lie in the order in
+// which the attention's lanes hold them: the 16 bytes of lane 4g + t in chunk
+// j are dims 32j + 4g + w (w = byte / 4) of positions 2t, 2t + 1, 2t + 8,
+// 2t + 9, so that a lane's 16-byte loads of either are matrix fragments as
+// they stand: no shared memory, no transposition between the cache and the
+// tensor cores.
+#pragma once
+
+#include "phonon_kernels.cuh"
+
+#include <cuda_fp16.h>
+
+namespace phonon {
+
+constexpr int kKv8Block = kPage;  // positions that share a scale (a page)
+constexpr int kKv8MinExp = -48, kKv8MaxExp = 64;
+constexpr int kStatusInvalid = 1;   // PHONON_CUDA_INVALID_ARGUMENT
+constexpr int kStatusCapacity = 5;  // PHONON_CUDA_CAPACITY
+
+// One layer of a cache.
+struct Kv8View {
+    uint8_t* pool;
+    int8_t* exps;
+    int pool_pages;
+    int heads;  // K/V heads
+};
+
+// The sequences of a call. Sequence i holds lengths[i] + length_bias
+// positions, the last of which are its rows [row_begin[i], row_begin[i + 1])
+// of the call (rows_per_seq each where row_begin is null); position p lies in
+// page pages[slot * page_stride + p / 16], slot = slots ? slots[i] : i.
+struct Kv8Seqs {
+    int n, rows, rows_per_seq;
+    const int32_t* row_begin;
+    const int32_t* lengths;
+    int length_bias;
+    const int32_t* slots;
+    const int32_t* pages;
+    int page_stride;
+    int max_rows, max_length;
+    int32_t* status;  // [n] or null
+};
+
+// The largest code wins: a sequence's status is set by many warps.
+__device__ __forceinline__ void kv8_flag(const Kv8Seqs& s, int i, int code) {
+    if (s.status) atomicMax(s.status + i, code);
+}
+
+struct Kv8Seq {
+    int row0, count, length;
+    const int32_t* pages;
+};
+
+// Sequence i's extent, checked against what the host launched for: rows
+// outside the call's are refused (no row), lengths past the page table's or
+// the launch's bound count as empty.
+__device__ __forceinline__ Kv8Seq kv8_seq(const Kv8Seqs& s, int i) {
+    Kv8Seq q;
+    const int b = s.row_begin ? __ldg(s.row_begin + i) : i * s.rows_per_seq;
+    const int e = s.row_begin ? __ldg(s.row_begin + i + 1) : b + s.rows_per_seq;
+    q.length = __ldg(s.lengths + i) + s.length_bias;
+    q.row0 = b;
+    q.count = e - b;
+    if (b < 0 || e < b || e > s.rows || e - b > s.max_rows) {
+        kv8_flag(s, i, kStatusInvalid);
+        q.row0 = q.count = 0;
+    }
+    if (q.length < 0 || q.length > s.max_length) {
+        kv8_flag(s, i, kStatusCapacity);
+        q.length = 0;
+    }
+    q.pages = s.pages + static_cast<long long>(s.slots ? __ldg(s.slots + i) : i) * s.page_stride;
+    return q;
+}
+
+template <int D>
+__device__ __forceinline__ uint8_t* kv8_block(const Kv8View& c, int page, int head, int which) {
+    return c.pool + (static_cast<size_t>(page) * c.heads + head) * (2 * kKv8Block * D) + which * (kKv8Block * D);
+}
+
+__device__ __forceinline__ int8_t* kv8_exp(const Kv8View& c, int page, int head) {
+    return c.exps + (static_cast<size_t>(page) * c.heads + head) * 2;
+}
+
+__device__ __forceinline__ float pow2i(int e) { return __int_as_float((e + 127) << 23); }  // e in [-126, 127]
+
+// The smallest e with amax <= 127 * 2^e, 127 = 1.984375 * 2^6.
+__device__ __forceinline__ int kv8_exponent(float amax) {
+    const uint32_t u = __float_as_uint(amax);
+    const int e = static_cast<int>(u >> 23) - 127 - 6 + ((u & 0x7fffffu) > 0x7e0000u ? 1 : 0);
+    return min(max(e, kKv8MinExp), kKv8MaxExp);
+}
+
+__device__ __forceinline__ uint32_t kv8_code(float x, float inverse) {
+    return static_cast<uint32_t>(min(max(__float2int_rn(__fmul_rn(x, inverse)), -127), 127) + 128);
+}
+
+// A held byte of a scale 2^k times smaller (shrink = 2^-k) in the new one.
+__device__ __forceinline__ uint32_t kv8_shrink(uint32_t byte, float shrink) {
+    return static_cast<uint32_t>(__float2int_rn(__fmul_rn(static_cast<float>(static_cast<int>(byte) - 128), shrink)) + 128);
+}
+
+template <bool kBf16>
+__device__ __forceinline__ float4 load_row4(const void* base, size_t at) {
+    if constexpr (kBf16) {
+        const uint2 w = __ldg(reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(base) + at));
+        return make_float4(__uint_as_float(w.x << 16), __uint_as_float(w.x & 0xffff0000u), __uint_as_float(w.y << 16),
+                           __uint_as_float(w.y & 0xffff0000u));
+    } else {
+        return __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(base) + at));
+    }
+}
+
+template <bool kBf16>
+__device__ __forceinline__ void store_row4(void* base, size_t at, float4 v) {
+    if constexpr (kBf16) {
+        const uint2 w = make_uint2(f32_to_bf16(v.x) | static_cast<uint32_t>(f32_to_bf16(v.y)) << 16,
+                                   f32_to_bf16(v.z) | static_cast<uint32_t>(f32_to_bf16(v.w)) << 16);
+        *reinterpret_cast<uint2*>(static_cast<uint16_t*>(base) + at) = w;
+    } else {
+        *reinterpret_cast<float4*>(static_cast<float*>(base) + at) = v;
+    }
+}
+
+// ------------------------------------------------------------------- append
+struct Kv8AppendParams {
+    Kv8View cache;
+    Kv8Seqs seqs;
+    const void* rows[2];  // keys, values: [rows][heads][D], rows `stride` elements apart
+    long long stride;
+    int blocks;  // blocks of a sequence that its rows can touch, at most
+};
+
+// Position of lane 4g + t's k-th byte of a value word (the layout above).
+__device__ __forceinline__ int kv8_value_pos(int t, int k) { return 2 * t + (k & 1) + 8 * (k >> 1); }
+
+// One warp writes one block's keys (which = 0) or values (1): the new rows'
+// maximum, the scale, then the integers. A block's bytes are all owned by one
+// warp; a partly filled block is read again only where its scale rises or a
+// value word mixes old and new positions. Lane layout: keys, 4 dims of a row
+// a lane (4-byte stores, rows coalesced); values, the lane's own chunks.
+template <int D, bool kBf16>
+__global__ void __launch_bounds__(128) kv8_append_kernel(Kv8AppendParams p) {
+    constexpr int kLanesPerRow = D / 4, kRowsPerPass = 32 / kLanesPerRow, kPasses = kKv8Block / kRowsPerPass;
+    constexpr int kChunks = D / 32;
+    pdl_wait();
+    pdl_trigger();
+    const int lane = threadIdx.x & 31;
+    const long long item = (static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x) >> 5;
+    const int which = static_cast<int>(item & 1);
+    long long rest = item >> 1;
+    const int head = static_cast<int>(rest % p.cache.heads);
+    rest /= p.cache.heads;
+    const int bi = static_cast<int>(rest % p.blocks);
+    rest /= p.blocks;
+    if (rest >= p.seqs.n) return;
+    const int i = static_cast<int>(rest);
+    const Kv8Seq q = kv8_seq(p.seqs, i);
+    const int start = max(q.length - q.count, 0);  // rows before position 0 go nowhere
+    const int row0 = q.row0 + q.count - q.length;  // row of position 0
+    const int block = start / kKv8Block + bi;
+    const int p0 = block * kKv8Block;
+    if (p0 >= q.length || q.count == 0) return;
+    const int page = __ldg(q.pages + block);
+    if (static_cast<unsigned>(page) >= static_cast<unsigned>(p.cache.pool_pages)) {
+        if (lane == 0) kv8_flag(p.seqs, i, kStatusInvalid);
+        return;
+    }
+    const int lo = max(start - p0, 0), hi = min(q.length - p0, kKv8Block);  // new slots [lo, hi), kept [0, lo)
+    int8_t* ep = kv8_exp(p.cache, page, head) + which;
+    const int held = lo > 0 ? *ep : kKv8MinExp;
+    uint8_t* dst = kv8_block<D>(p.cache, page, head, which);
+    const void* src = p.rows[which];
+
+    float4 x[16 * D / 128];
+    float amax = 0.0f;
+    bool finite = true;
+    auto take = [&](float4& v, int slot, int dim) {
+        v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (slot < lo || slot >= hi) return;
+        v = load_row4<kBf16>(src, static_cast<size_t>(row0 + p0 + slot) * p.stride + head * D + dim);
+        float* f = &v.x;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            if (!isfinite(f[k])) {  // held as 0 and flagged
+                finite = false;
+                f[k] = 0.0f;
+            }
+            amax = fmaxf(amax, fabsf(f[k]));
+        }
+    };
+    const int g = lane >> 2, t = lane & 3;
+    if (which == 0) {
+#pragma unroll
+        for (int a = 0; a < kPasses; ++a) take(x[a], a * kRowsPerPass + lane / kLanesPerRow, (lane % kLanesPerRow) * 4);
+    } else {
+#pragma unroll
+        for (int j = 0; j < kChunks; ++j)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) take(x[j * 4 + k], kv8_value_pos(t, k), 32 * j + 4 * g);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(kFull, amax, o));
+    if (!__all_sync(kFull, finite) && lane == 0) kv8_flag(p.seqs, i, kStatusNonFinite);
+    const int e = max(kv8_exponent(amax), held);
+    const float inverse = pow2i(-e), shrink = pow2i(held - e);
+    const bool raised = lo > 0 && e > held;
+    if (lane == 0) *ep = static_cast<int8_t>(e);
+
+    if (which == 0) {
+#pragma unroll
+        for (int a = 0; a < kPasses; ++a) {
+            const int slot = a * kRowsPerPass + lane / kLanesPerRow;
+            uint32_t* at = reinterpret_cast<uint32_t*>(dst + slot * D) + lane % kLanesPerRow;
+            if (slot >= lo && slot < hi) {
+                *at = kv8_code(x[a].x, inverse) | kv8_code(x[a].y, inverse) << 8 | kv8_code(x[a].z, inverse) << 16 |
+                      kv8_code(x[a].w, inverse) << 24;
+            } else if (raised && slot < lo) {
+                const uint32_t w = *at;
+                uint32_t r = 0;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) r |= kv8_shrink((w >> (8 * k)) & 0xffu, shrink) << (8 * k);
+                *at = r;
+            }
+        }
+    } else {
+        bool any_new = false, any_old = false, any_raise = false;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int slot = kv8_value_pos(t, k);
+            const bool fresh = slot >= lo && slot < hi;
+            any_new |= fresh;
+            any_old |= !fresh;
+            any_raise |= raised && slot < lo;
+        }
+        if (!any_new && !any_raise) return;
+#pragma unroll
+        for (int j = 0; j < kChunks; ++j) {
+            uint4* at = reinterpret_cast<uint4*>(dst + j * 512) + lane;
+            uint4 w4 = make_uint4(0, 0, 0, 0);
+            if (any_old) w4 = *at;
+            uint32_t* w = &w4.x;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int slot = kv8_value_pos(t, k);
+                const float* f = &x[j * 4 + k].x;
+#pragma unroll
+                for (int d = 0; d < 4; ++d) {
+                    const uint32_t old = (w[d] >> (8 * k)) & 0xffu;
+                    uint32_t b = old;
+                    if (slot >= lo && slot < hi) b = kv8_code(f[d], inverse);
+                    else if (raised && slot < lo) b = kv8_shrink(old, shrink);
+                    w[d] = (w[d] & ~(0xffu << (8 * k))) | (b << (8 * k));
+                }
+            }
+            *at = w4;
+        }
+    }
+}
+
+// --------------------------------------------------------------------- read
+struct Kv8ReadParams {
+    Kv8View cache;
+    Kv8Seqs seqs;
+    void* rows[2];
+    long long stride;
+    int blocks;
+};
+
+// One warp reads one block's keys or values back: held byte - 128 times 2^e,
+// exact in fp32. Rows of positions before 0, of empty and of bad pages are 0.
+template <int D, bool kBf16>
+__global__ void __launch_bounds__(128) kv8_read_kernel(Kv8ReadParams p) {
+    constexpr int kLanesPerRow = D / 4, kRowsPerPass = 32 / kLanesPerRow, kPasses = kKv8Block / kRowsPerPass;
+    constexpr int kChunks = D / 32;
+    pdl_wait();
+    pdl_trigger();
+    const int lane = threadIdx.x & 31;
+    const long long item = (static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x) >> 5;
+    const int which = static_cast<int>(item & 1);
+    long long rest = item >> 1;
+    const int head = static_cast<int>(rest % p.cache.heads);
+    rest /= p.cache.heads;
+    const int bi = static_cast<int>(rest % p.blocks);
+    rest /= p.blocks;
+    if (rest >= p.seqs.n) return;
+    const int i = static_cast<int>(rest);
+    const Kv8Seq q = kv8_seq(p.seqs, i);
+    // positions [length - count, length), counted from the block of the first (negative ones included)
+    const int start = q.length - q.count;
+    const int block = (start >= 0 ? start / kKv8Block : -((kKv8Block - 1 - start) / kKv8Block)) + bi;
+    const int p0 = block * kKv8Block;
+    if (p0 >= q.length || q.count == 0) return;
+    const int row0 = q.row0 - start;
+    int page = block >= 0 ? __ldg(q.pages + block) : -1;
+    if (block >= 0 && static_cast<unsigned>(page) >= static_cast<unsigned>(p.cache.pool_pages)) {
+        if (lane == 0) kv8_flag(p.seqs, i, kStatusInvalid);
+        page = -1;
+    }
+    const int lo = max(start - p0, 0), hi = min(q.length - p0, kKv8Block);
+    const uint8_t* src = page >= 0 ? kv8_block<D>(p.cache, page, head, which) : nullptr;
+    const float unit = page >= 0 ? pow2i(kv8_exp(p.cache, page, head)[which]) : 0.0f;
+    void* dst = p.rows[which];
+    auto value = [&](uint32_t w, int k) {
+        return static_cast<float>(static_cast<int>((w >> (8 * k)) & 0xffu) - 128) * unit;
+    };
+    const int g = lane >> 2, t = lane & 3;
+    if (which == 0) {
+        uint32_t w[kPasses];
+#pragma unroll
+        for (int a = 0; a < kPasses; ++a) {
+            const int slot = a * kRowsPerPass + lane / kLanesPerRow;
+            w[a] = src && slot >= lo && slot < hi
+                       ? __ldg(reinterpret_cast<const uint32_t*>(src + slot * D) + lane % kLanesPerRow)
+                       : 0x80808080u;
+        }
+#pragma unroll
+        for (int a = 0; a < kPasses; ++a) {
+            const int slot = a * kRowsPerPass + lane / kLanesPerRow;
+            if (slot >= lo && slot < hi)
+                store_row4<kBf16>(dst, static_cast<size_t>(row0 + p0 + slot) * p.stride + head * D + (lane % kLanesPerRow) * 4,
+                                  make_float4(value(w[a], 0), value(w[a], 1), value(w[a], 2), value(w[a], 3)));
+        }
+    } else {
+        uint4 w[kChunks];
+#pragma unroll
+        for (int j = 0; j < kChunks; ++j)
+            w[j] = src ? __ldg(reinterpret_cast<const uint4*>(src + j * 512) + lane)
+                       : make_uint4(0x80808080u, 0x80808080u, 0x80808080u, 0x80808080u);
+#pragma unroll
+        for (int j = 0; j < kChunks; ++j)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int slot = kv8_value_pos(t, k);
+                if (slot >= lo && slot < hi)
+                    store_row4<kBf16>(dst, static_cast<size_t>(row0 + p0 + slot) * p.stride + head * D + 32 * j + 4 * g,
+                                      make_float4(value(w[j].x, k), value(w[j].y, k), value(w[j].z, k), value(w[j].w, k)));
+            }
+    }
+}
+
+// ---------------------------------------------------------------- attention
+// out[r] = sum_k softmax_k(scale q_r . K_k) V_k over the positions k that row
+// r (at position p_r) sees: k <= p_r, and k > p_r - window where a window is
+// set. Rows that see nothing get 0.
+//
+// Per block the tensor cores compute S^T = K q^T (16 positions x 8 rows) and
+// O^T += V^T P^T (16 dims x 8 rows) with the cache's integers as the A
+// operand: byte | 0x6400 is the half 1024 + byte, minus 1152 the signed
+// integer, exactly, one PRMT and one HSUB2 for two elements. Rows are the N
+// operand: a decode step's single row (times the grouped heads) costs half
+// the instructions that it would as M. A block's scales enter in fp32: with s
+// = scale log2(e) 2^eK (q.K) + eV, the weight 2^(s - M) is the softmax weight
+// times the block's value scale, so that O needs no scaling of its own, and the
+// sum of weights takes 2^(s - M - eV). M is the running maximum of s. eV spans
+// [-48, 64], so weights that matter stay inside fp32's range.
+//
+// Rounding: the 8-bit integers and their products with a half are exact in
+// the fp32 accumulators. fp32 rows: q (scaled by a power of two to a row
+// maximum near 2^12) and the weights enter as two halves each, 22 bits. bf16
+// rows: q fits one half (8 bits), a weight is rounded to one half (11 bits,
+// under the output's 8).
+struct Kv8AttnParams {
+    Kv8View cache;
+    Kv8Seqs seqs;
+    const void* q;
+    void* out;
+    long long q_stride, out_stride;  // elements between rows; a row is [heads][D]
+    int group;                       // query heads per K/V head
+    float scale;                     // softmax scale times log2(e)
+    int window;                      // 0: none
+    int tiles, splits, split_pages;  // row tiles of a sequence, splits and their pages, at most
+    float* part;                     // [items * splits][rows of a tile][D]
+    float2* part_ml;                 // [items * splits][rows of a tile]: M, sum
+    unsigned* arrived;               // [items], zero between launches
+};
+
+constexpr int kKv8Warps = 4;
+constexpr float kKv8WeightBits = 14.0f;  // weights are held times 2^14: a half keeps 11 bits down to 2^-28
+
+__device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                         uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ uint32_t movmatrix_trans(uint32_t v) {
+    uint32_t r;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+    return r;
+}
+
+__device__ __forceinline__ float ex2(float x) {
+    float r;
+    asm("ex2.approx.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+
+// Bytes 0, 1 (kHigh: 2, 3) of a cache word as the halves byte - 128.
+template <bool kHigh>
+__device__ __forceinline__ uint32_t kv8_halves(uint32_t w) {
+    uint32_t u = __byte_perm(w, 0x64646464u, kHigh ? 0x4342 : 0x4140);
+    const __half2 bias = __halves2half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480));  // 1152
+    const __half2 h = __hsub2(*reinterpret_cast<__half2*>(&u), bias);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+__device__ __forceinline__ uint32_t half2_bits(float a, float b) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+__device__ __forceinline__ float2 half2_floats(uint32_t u) { return __half22float2(*reinterpret_cast<__half2*>(&u)); }
+
+__device__ __forceinline__ uint4 ld_stream16(const uint8_t* p) {
+    uint4 v;
+    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                 : "l"(p));
+    return v;
+}
+
+__device__ __forceinline__ uint2 ld_stream8(const uint8_t* p) {
+    uint2 v;
+    asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
+    return v;
+}
+
+// A lane's share of a block's keys: word [half][c] is dims 4c.. of the lane's
+// D/4 (the t-th 16 bytes of each 64, 8 of 32) of positions g, g + 8.
+template <int D>
+__device__ __forceinline__ void kv8_load_keys(uint32_t (&w)[2][D / 16], const uint8_t* block, int lane) {
+    const int g = lane >> 2, t = lane & 3;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const uint8_t* row = block + (g + 8 * h) * D;
+        if constexpr (D == 32) {
+            const uint2 v = ld_stream8(row + t * 8);
+            w[h][0] = v.x;
+            w[h][1] = v.y;
+        } else {
+#pragma unroll
+            for (int c = 0; c < D / 64; ++c) {
+                const uint4 v = ld_stream16(row + c * 64 + t * 16);
+                w[h][4 * c] = v.x;
+                w[h][4 * c + 1] = v.y;
+                w[h][4 * c + 2] = v.z;
+                w[h][4 * c + 3] = v.w;
+            }
+        }
+    }
+}
+
+// The first dim of word c above.
+template <int D>
+__device__ __forceinline__ int kv8_key_dim(int t, int c) {
+    return D == 32 ? t * 8 + c * 4 : (c >> 2) * 64 + t * 16 + (c & 3) * 4;
+}
+
+template <int D>
+__device__ __forceinline__ void kv8_load_values(uint32_t (&w)[D / 8], const uint8_t* block, int lane) {
+#pragma unroll
+    for (int j = 0; j < D / 32; ++j) {
+        const uint4 v = ld_stream16(block + j * 512 + lane * 16);
+        w[4 * j] = v.x;
+        w[4 * j + 1] = v.y;
+        w[4 * j + 2] = v.z;
+        w[4 * j + 3] = v.w;
+    }
+}
+
+// One CTA: one (sequence, row tile, K/V head, split). Its warps take the
+// split's pages PB at a time in turn, each with an online softmax of its own,
+// and meet in shared memory; the last split to arrive merges them in order.
+// The next pages' keys are loaded when the current ones have been multiplied,
+// the next values after the current: a warp always has PB pages of either in
+// flight (2 to 8 KB), without shared memory.
+template <int D, int NT, int PB, bool kBf16>
+__global__ void __launch_bounds__(32 * kKv8Warps) kv8_attention_kernel(Kv8AttnParams p) {
+    constexpr int kRows = 8 * NT;
+    constexpr bool kFine = !kBf16;  // two halves for q and the weights
+    constexpr int KS = D / 16;      // 16-dim steps of a score, and 16-dim tiles of an output
+    __shared__ float s_o[kKv8Warps][kRows][D];
+    __shared__ float2 s_ml[kKv8Warps][kRows];
+    __shared__ int s_last;
+    pdl_wait();
+    pdl_trigger();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const int split = static_cast<int>(blockIdx.x % p.splits);
+    const unsigned item = blockIdx.x / p.splits;
+    const int head = static_cast<int>(item % p.cache.heads);
+    const int tile = static_cast<int>(item / p.cache.heads % p.tiles);
+    const int i = static_cast<int>(item / p.cache.heads / p.tiles);
+    const Kv8Seq sq = kv8_seq(p.seqs, i);
+    const int rows = sq.count * p.group - tile * kRows;  // rows left from this tile on
+    if (rows <= 0) return;
+    const int n_rows = min(rows, kRows), rho0 = tile * kRows;
+    const int at0 = sq.length - sq.count;  // position of the sequence's first row
+    const int pos_lo = at0 + rho0 / p.group, pos_hi = at0 + (rho0 + n_rows - 1) / p.group;
+    const int key_end = min(pos_hi + 1, sq.length);
+    const int page_begin = p.window ? max(pos_lo - p.window + 1, 0) / kKv8Block : 0;
+    const int pages = key_end > 0 ? (key_end + kKv8Block - 1) / kKv8Block - page_begin : 0;
+    const int active = max(1, min(p.splits, (pages + p.split_pages - 1) / p.split_pages));
+    if (split >= active) return;
+    const int per = (pages + active - 1) / active;
+    const int first = page_begin + min(pages, split * per), last = page_begin + min(pages, (split + 1) * per);
+
+    // q as B fragments, scaled to a row maximum in [2^12, 2^13)
+    uint32_t qh[NT][KS][2], ql[NT][kFine ? KS : 1][2];
+    float f0[NT], f1[NT];  // scale * 2^(row exponent) of rows 2t, 2t + 1
+    int pos0[NT], pos1[NT];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+        const int r = n * 8 + g, rho = rho0 + min(r, n_rows - 1);
+        const size_t row = static_cast<size_t>(sq.row0 + rho / p.group) * p.q_stride +
+                           static_cast<size_t>(head * p.group + rho % p.group) * D;
+        float4 v[KS];
+        float amax = 0.0f;
+        bool finite = true;
+#pragma unroll
+        for (int c = 0; c < KS; ++c) {
+            v[c] = load_row4<kBf16>(p.q, row + kv8_key_dim<D>(t, c));
+            finite &= isfinite(v[c].x) & isfinite(v[c].y) & isfinite(v[c].z) & isfinite(v[c].w);
+            amax = fmaxf(amax, fmaxf(fmaxf(fabsf(v[c].x), fabsf(v[c].y)), fmaxf(fabsf(v[c].z), fabsf(v[c].w))));
+        }
+        amax = fmaxf(amax, __shfl_xor_sync(kFull, amax, 1));
+        amax = fmaxf(amax, __shfl_xor_sync(kFull, amax, 2));
+        const unsigned bad = __ballot_sync(kFull, !finite);
+        const bool row_bad = (bad >> (lane & ~3) & 0xfu) != 0;
+        if (row_bad && t == 0 && r < n_rows) kv8_flag(p.seqs, i, kStatusNonFinite);
+        // exponent of the maximum, kept where both powers below are normal
+        const int ex = min(max(static_cast<int>(__float_as_uint(amax) >> 23) - 127, -110), 126);
+        const float up = pow2i(min(12 - ex, 122)), back = pow2i(ex - 12);
+#pragma unroll
+        for (int c = 0; c < KS; ++c) {
+            const float a = v[c].x * up, b = v[c].y * up, cc = v[c].z * up, d = v[c].w * up;
+            qh[n][c][0] = half2_bits(a, b);
+            qh[n][c][1] = half2_bits(cc, d);
+            if constexpr (kFine) {
+                const float2 h0 = half2_floats(qh[n][c][0]), h1 = half2_floats(qh[n][c][1]);
+                ql[n][c][0] = half2_bits(a - h0.x, b - h0.y);
+                ql[n][c][1] = half2_bits(cc - h1.x, d - h1.y);
+            }
+        }
+        const float f = row_bad ? __int_as_float(0x7fc00000) : p.scale * back;  // a bad row's output is NaN
+        f0[n] = __shfl_sync(kFull, f, 8 * t);
+        f1[n] = __shfl_sync(kFull, f, 8 * t + 4);
+        pos0[n] = at0 + (rho0 + min(n * 8 + 2 * t, n_rows - 1)) / p.group;
+        pos1[n] = at0 + (rho0 + min(n * 8 + 2 * t + 1, n_rows - 1)) / p.group;
+    }
+
+    float o[KS][NT][4];
+    float m0[NT], m1[NT], l0[NT], l1[NT];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+        m0[n] = m1[n] = -INFINITY;
+        l0[n] = l1[n] = 0.0f;
+#pragma unroll
+        for (int k = 0; k < KS; ++k) o[k][n][0] = o[k][n][1] = o[k][n][2] = o[k][n][3] = 0.0f;
+    }
+
+    uint32_t kw[PB][2][D / 16], vw[PB][D / 8];
+    int page[PB];   // page ids of the batch whose keys are in kw; -1: none
+    int ek[PB], ev[PB];
+    auto load_ids = [&](int from, int (&id)[PB]) {
+#pragma unroll
+        for (int b = 0; b < PB; ++b) {
+            id[b] = from + b < last ? __ldg(sq.pages + from + b) : -1;
+            if (from + b < last && static_cast<unsigned>(id[b]) >= static_cast<unsigned>(p.cache.pool_pages)) {
+                if (lane == 0) kv8_flag(p.seqs, i, kStatusInvalid);
+                id[b] = -1;  // its keys are not seen
+            }
+        }
+    };
+    auto load_keys = [&](const int (&id)[PB]) {
+#pragma unroll
+        for (int b = 0; b < PB; ++b) {
+            const int pg = max(id[b], 0);
+            if (id[b] >= 0) kv8_load_keys<D>(kw[b], kv8_block<D>(p.cache, pg, head, 0), lane);
+            const short e2 = __ldg(reinterpret_cast<const short*>(kv8_exp(p.cache, pg, head)));
+            ek[b] = static_cast<int8_t>(e2 & 0xff);
+            ev[b] = e2 >> 8;
+        }
+    };
+    auto load_values = [&](const int (&id)[PB]) {
+#pragma unroll
+        for (int b = 0; b < PB; ++b)
+            if (id[b] >= 0) kv8_load_values<D>(vw[b], kv8_block<D>(p.cache, id[b], head, 1), lane);
+    };
+#pragma unroll
+    for (int b = 0; b < PB; ++b) {
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k) kw[b][0][k] = kw[b][1][k] = 0x80808080u;
+#pragma unroll
+        for (int k = 0; k < D / 8; ++k) vw[b][k] = 0x80808080u;
+    }
+    const int step = kKv8Warps * PB;
+    int at = first + warp * PB;
+    load_ids(at, page);
+    load_keys(page);
+    load_values(page);
+    for (; at < last; at += step) {
+        int next[PB];
+        load_ids(at + step, next);
+        float s[PB][NT][4];
+        float add[PB], less[PB];  // eV, 2^-eV
+#pragma unroll
+        for (int b = 0; b < PB; ++b) {
+#pragma unroll
+            for (int n = 0; n < NT; ++n) s[b][n][0] = s[b][n][1] = s[b][n][2] = s[b][n][3] = 0.0f;
+#pragma unroll
+            for (int c = 0; c < KS; ++c) {
+                const uint32_t a0 = kv8_halves<false>(kw[b][0][c]), a1 = kv8_halves<false>(kw[b][1][c]);
+                const uint32_t a2 = kv8_halves<true>(kw[b][0][c]), a3 = kv8_halves<true>(kw[b][1][c]);
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    mma16816(s[b][n], a0, a1, a2, a3, qh[n][c][0], qh[n][c][1]);
+                    if constexpr (kFine) mma16816(s[b][n], a0, a1, a2, a3, ql[n][c][0], ql[n][c][1]);
+                }
+            }
+            const float uk = pow2i(ek[b]);
+            add[b] = static_cast<float>(ev[b]);
+            less[b] = pow2i(-ev[b]);
+            const int key = (at + b) * kKv8Block + g;
+            // every row of the tile sees the whole page
+            const bool whole = page[b] >= 0 && (at + b + 1) * kKv8Block <= pos_lo + 1 &&
+                               (!p.window || (at + b) * kKv8Block > pos_hi - p.window);
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                const float u0 = f0[n] * uk, u1 = f1[n] * uk;
+                s[b][n][0] = fmaf(s[b][n][0], u0, add[b]);
+                s[b][n][1] = fmaf(s[b][n][1], u1, add[b]);
+                s[b][n][2] = fmaf(s[b][n][2], u0, add[b]);
+                s[b][n][3] = fmaf(s[b][n][3], u1, add[b]);
+                if (!whole) {
+                    const int w0 = p.window ? pos0[n] - p.window : -1, w1 = p.window ? pos1[n] - p.window : -1;
+                    if (page[b] < 0 || key > pos0[n] || key <= w0) s[b][n][0] = -INFINITY;
+                    if (page[b] < 0 || key > pos1[n] || key <= w1) s[b][n][1] = -INFINITY;
+                    if (page[b] < 0 || key + 8 > pos0[n] || key + 8 <= w0) s[b][n][2] = -INFINITY;
+                    if (page[b] < 0 || key + 8 > pos1[n] || key + 8 <= w1) s[b][n][3] = -INFINITY;
+                }
+            }
+        }
+        load_keys(next);
+        uint32_t ph[PB][NT][2], pl[PB][kFine ? NT : 1][2];
+        bool moved = false;
+        float c0[NT], c1[NT];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            float x0 = m0[n], x1 = m1[n];
+#pragma unroll
+            for (int b = 0; b < PB; ++b) {
+                x0 = fmaxf(x0, fmaxf(s[b][n][0], s[b][n][2]));
+                x1 = fmaxf(x1, fmaxf(s[b][n][1], s[b][n][3]));
+            }
+#pragma unroll
+            for (int w = 4; w < 32; w <<= 1) {
+                x0 = fmaxf(x0, __shfl_xor_sync(kFull, x0, w));
+                x1 = fmaxf(x1, __shfl_xor_sync(kFull, x1, w));
+            }
+            c0[n] = m0[n] == x0 ? 1.0f : ex2(m0[n] - x0);
+            c1[n] = m1[n] == x1 ? 1.0f : ex2(m1[n] - x1);
+            moved |= m0[n] != x0 || m1[n] != x1;
+            m0[n] = x0;
+            m1[n] = x1;
+            // rows that have seen nothing yet keep weight 0: -inf - 0
+            const float b0 = x0 == -INFINITY ? 0.0f : x0 - kKv8WeightBits, b1 = x1 == -INFINITY ? 0.0f : x1 - kKv8WeightBits;
+            l0[n] *= c0[n];
+            l1[n] *= c1[n];
+#pragma unroll
+            for (int b = 0; b < PB; ++b) {
+                const float p0 = ex2(s[b][n][0] - b0), p1 = ex2(s[b][n][1] - b1);
+                const float p2 = ex2(s[b][n][2] - b0), p3 = ex2(s[b][n][3] - b1);
+                l0[n] = fmaf(p0 + p2, less[b], l0[n]);
+                l1[n] = fmaf(p1 + p3, less[b], l1[n]);
+                const uint32_t h0 = half2_bits(p0, p1), h1 = half2_bits(p2, p3);
+                ph[b][n][0] = movmatrix_trans(h0);
+                ph[b][n][1] = movmatrix_trans(h1);
+                if constexpr (kFine) {
+                    const float2 r0 = half2_floats(h0), r1 = half2_floats(h1);
+                    pl[b][n][0] = movmatrix_trans(half2_bits(p0 - r0.x, p1 - r0.y));
+                    pl[b][n][1] = movmatrix_trans(half2_bits(p2 - r1.x, p3 - r1.y));
+                }
+            }
+        }
+        if (__any_sync(kFull, moved)) {
+#pragma unroll
+            for (int k = 0; k < KS; ++k)
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    o[k][n][0] *= c0[n];
+                    o[k][n][1] *= c1[n];
+                    o[k][n][2] *= c0[n];
+                    o[k][n][3] *= c1[n];
+                }
+        }
+#pragma unroll
+        for (int b = 0; b < PB; ++b)
+#pragma unroll
+            for (int k = 0; k < KS; ++k) {
+                const uint32_t wa = vw[b][2 * k], wb = vw[b][2 * k + 1];
+                const uint32_t a0 = kv8_halves<false>(wa), a1 = kv8_halves<false>(wb);
+                const uint32_t a2 = kv8_halves<true>(wa), a3 = kv8_halves<true>(wb);
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    mma16816(o[k][n], a0, a1, a2, a3, ph[b][n][0], ph[b][n][1]);
+                    if constexpr (kFine) mma16816(o[k][n], a0, a1, a2, a3, pl[b][n][0], pl[b][n][1]);
+                }
+            }
+        load_values(next);
+#pragma unroll
+        for (int b = 0; b < PB; ++b) page[b] = next[b];
+    }
+
+    // the warps' shares meet
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+#pragma unroll
+        for (int w = 4; w < 32; w <<= 1) {
+            l0[n] += __shfl_xor_sync(kFull, l0[n], w);
+            l1[n] += __shfl_xor_sync(kFull, l1[n], w);
+        }
+        const int r = n * 8 + 2 * t;
+        if (g == 0) {
+            s_ml[warp][r] = make_float2(m0[n], l0[n]);
+            s_ml[warp][r + 1] = make_float2(m1[n], l1[n]);
+        }
+#pragma unroll
+        for (int j = 0; j < D / 32; ++j) {
+            if (r < n_rows)
+                *reinterpret_cast<float4*>(&s_o[warp][r][32 * j + 4 * g]) =
+                    make_float4(o[2 * j][n][0], o[2 * j][n][2], o[2 * j + 1][n][0], o[2 * j + 1][n][2]);
+            if (r + 1 < n_rows)
+                *reinterpret_cast<float4*>(&s_o[warp][r + 1][32 * j + 4 * g]) =
+                    make_float4(o[2 * j][n][1], o[2 * j][n][3], o[2 * j + 1][n][1], o[2 * j + 1][n][3]);
+        }
+    }
+    __syncthreads();
+    constexpr int kQuads = D / 4;
+    auto finish = [&](int r, int d, float total, float4 a) {
+        const float inv = total > 0.0f || isnan(total) ? __fdiv_rn(1.0f, total) : 0.0f;
+        const int rho = rho0 + r;
+        store_row4<kBf16>(p.out,
+                          static_cast<size_t>(sq.row0 + rho / p.group) * p.out_stride +
+                              static_cast<size_t>(head * p.group + rho % p.group) * D + d,
+                          make_float4(a.x * inv, a.y * inv, a.z * inv, a.w * inv));
+    };
+    auto fold = [](float& m, float& l, float4& a, float m2, float l2, float4 b) {
+        const float x = fmaxf(m, m2);
+        const float wa = m == -INFINITY ? 0.0f : ex2(m - x), wb = m2 == -INFINITY ? 0.0f : ex2(m2 - x);
+        m = x;
+        l = l * wa + l2 * wb;
+        a = make_float4(a.x * wa + b.x * wb, a.y * wa + b.y * wb, a.z * wa + b.z * wb, a.w * wa + b.w * wb);
+    };
+    const size_t slot = static_cast<size_t>(item) * p.splits;
+    for (int x = threadIdx.x; x < n_rows * kQuads; x += blockDim.x) {
+        const int r = x / kQuads, d = x % kQuads * 4;
+        float m = -INFINITY, l = 0.0f;
+        float4 a = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+        for (int w = 0; w < kKv8Warps; ++w)
+            fold(m, l, a, s_ml[w][r].x, s_ml[w][r].y, *reinterpret_cast<const float4*>(&s_o[w][r][d]));
+        if (active == 1) {
+            finish(r, d, l, a);
+        } else {
+            const size_t at_part = (slot + split) * kRows + r;
+            *reinterpret_cast<float4*>(p.part + at_part * D + d) = a;
+            if (d == 0) p.part_ml[at_part] = make_float2(m, l);
+        }
+    }
+    if (active == 1) return;
+    __threadfence();
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        const unsigned n = atomicAdd(p.arrived + item, 1u);
+        s_last = n + 1 == static_cast<unsigned>(active);
+        if (s_last) p.arrived[item] = 0;
+    }
+    __syncthreads();
+    if (!s_last) return;
+    __threadfence();
+    for (int x = threadIdx.x; x < n_rows * kQuads; x += blockDim.x) {
+        const int r = x / kQuads, d = x % kQuads * 4;
+        float m = -INFINITY, l = 0.0f;
+        float4 a = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        for (int k = 0; k < active; ++k) {
+            const size_t at_part = (slot + k) * kRows + r;
+            const float2 ml = __ldcg(p.part_ml + at_part);
+            fold(m, l, a, ml.x, ml.y, __ldcg(reinterpret_cast<const float4*>(p.part + at_part * D + d)));
+        }
+        finish(r, d, l, a);
+    }
+}
+
+}  // namespace phonon

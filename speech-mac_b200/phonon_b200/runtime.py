@@ -14,6 +14,7 @@ KERNEL_CLASSES = ("qkv", "attention", "combine", "out", "up", "down", "other", "
 OK, INVALID, NON_FINITE, OOM, POOL_EXHAUSTED, CAPACITY, BAD_POSITION, CANCELLED, DEVICE_ERROR = range(9)
 Q8_0, BF16 = 1, 2
 KV_F32, KV_BF16 = 0, 1
+ROWS_F32, ROWS_BF16 = 0, 1  # PhononCudaRowType
 FUSED_MAX_BATCH = 64  # PHONON_CUDA_FUSED_MAX_BATCH
 MAX_POSITIONS = 8192  # PHONON_CUDA_MAX_POSITIONS
 WIDTH = 512
@@ -57,6 +58,26 @@ class MimiWeights(C.Structure):
                 ("out_proj", C.c_void_p * 2), ("linear1", C.c_void_p * 2), ("linear2", C.c_void_p * 2),
                 ("norm1_w", C.c_void_p * 2), ("norm1_b", C.c_void_p * 2), ("norm2_w", C.c_void_p * 2),
                 ("norm2_b", C.c_void_p * 2), ("scale1", C.c_void_p * 2), ("scale2", C.c_void_p * 2)]
+
+
+class Kv8Config(C.Structure):
+    _fields_ = [("device", C.c_int), ("layers", C.c_uint32), ("kv_heads", C.c_uint32), ("head_dim", C.c_uint32),
+                ("pool_pages", C.c_uint32)]
+
+
+class Kv8Batch(C.Structure):
+    _fields_ = [("sequences", C.c_uint32), ("rows", C.c_uint32), ("row_begin", C.c_void_p), ("lengths", C.c_void_p),
+                ("pages", C.c_void_p), ("page_stride", C.c_uint32), ("max_rows", C.c_uint32),
+                ("max_length", C.c_uint32)]
+
+
+class Kv8Rows(C.Structure):
+    _fields_ = [("type", C.c_uint32), ("stride", C.c_uint64), ("keys", C.c_void_p), ("values", C.c_void_p)]
+
+
+class Kv8Query(C.Structure):
+    _fields_ = [("type", C.c_uint32), ("heads", C.c_uint32), ("window", C.c_uint32), ("scale", C.c_float),
+                ("q", C.c_void_p), ("out", C.c_void_p), ("q_stride", C.c_uint64), ("out_stride", C.c_uint64)]
 
 
 class CudaError(RuntimeError):
@@ -120,6 +141,11 @@ def lib():
         "phonon_cuda_mimi_step": [P, U32, P, P, P, P],
         "phonon_cuda_mimi_set_tensor_min": [P, U32, C.POINTER(C.c_int)],
         "phonon_cuda_mimi_process": [P, U32, P, SZ, P, SZ],
+        "phonon_cuda_kv8_create": [C.POINTER(Kv8Config), C.POINTER(P)],
+        "phonon_cuda_kv8_append_device": [P, U32, C.POINTER(Kv8Batch), C.POINTER(Kv8Rows), P, P],
+        "phonon_cuda_kv8_read_device": [P, U32, C.POINTER(Kv8Batch), C.POINTER(Kv8Rows), P, P],
+        "phonon_cuda_kv8_workspace_create": [P, C.POINTER(P)],
+        "phonon_cuda_kv8_attention_device": [P, U32, C.POINTER(Kv8Batch), C.POINTER(Kv8Query), P, P, P],
     }
     for name, args in sig.items():
         fn = getattr(L, name)
@@ -127,6 +153,11 @@ def lib():
         fn.restype = C.c_int
     L.phonon_cuda_mimi_destroy.argtypes = [P]
     L.phonon_cuda_mimi_destroy.restype = None
+    for name in ("phonon_cuda_kv8_destroy", "phonon_cuda_kv8_workspace_destroy"):
+        getattr(L, name).argtypes = [P]
+        getattr(L, name).restype = None
+    L.phonon_cuda_kv8_bytes.argtypes = [P]
+    L.phonon_cuda_kv8_bytes.restype = SZ
     L.phonon_cuda_head_free.argtypes = [P]
     L.phonon_cuda_head_free.restype = None
     L.phonon_cuda_destroy.argtypes = [P]
@@ -583,3 +614,84 @@ class Mimi:
         check(self.L.phonon_cuda_mimi_process(self.h, s, _p(latents), latents.shape[0], _p(feats), feats.shape[0]),
               "mimi_process")
         return feats
+
+
+def kv8_batch(sequences, lengths_ptr, pages_ptr, page_stride, max_length, rows=None, row_begin_ptr=None, max_rows=1):
+    """PhononCudaKv8Batch over device arrays (addresses; the arrays must
+    outlive the calls): lengths [sequences], pages [sequences][page_stride],
+    row_begin [sequences + 1] or none for one row per sequence."""
+    return Kv8Batch(sequences, sequences if rows is None else rows, row_begin_ptr, lengths_ptr, pages_ptr, page_stride,
+                    max_rows, max_length)
+
+
+def kv8_rows(keys_ptr, values_ptr, type=ROWS_F32, stride=0):
+    """PhononCudaKv8Rows: key and value rows in device memory."""
+    return Kv8Rows(type, stride, keys_ptr, values_ptr)
+
+
+def kv8_query(q_ptr, out_ptr, type=ROWS_F32, heads=8, window=0, scale=0.0, q_stride=0, out_stride=0):
+    """PhononCudaKv8Query: query and output rows in device memory."""
+    return Kv8Query(type, heads, window, scale, q_ptr, out_ptr, q_stride, out_stride)
+
+
+class Kv8Cache:
+    """An 8-bit paged K/V cache (phonon_cuda_kv8_*). Its calls take the
+    structures that kv8_batch, kv8_rows and kv8_query build, which a serving
+    loop keeps from step to step, and enqueue on a CUDA stream."""
+
+    def __init__(self, kv_heads, head_dim, pool_pages, layers=1, device=0):
+        self.h = None
+        self.L = lib()
+        h = C.c_void_p()
+        cfg = Kv8Config(device, layers, kv_heads, head_dim, pool_pages)
+        check(self.L.phonon_cuda_kv8_create(C.byref(cfg), C.byref(h)), "kv8_create")
+        self.h = h
+        self._append = self.L.phonon_cuda_kv8_append_device
+        self._read = self.L.phonon_cuda_kv8_read_device
+        self._attention = self.L.phonon_cuda_kv8_attention_device
+
+    def bytes(self):
+        return self.L.phonon_cuda_kv8_bytes(self.h)
+
+    def append(self, batch, rows, layer=0, status_ptr=None, stream_ptr=0):
+        check(self._append(self.h, layer, batch, rows, status_ptr, stream_ptr), "kv8_append_device")
+
+    def read(self, batch, rows, layer=0, status_ptr=None, stream_ptr=0):
+        check(self._read(self.h, layer, batch, rows, status_ptr, stream_ptr), "kv8_read_device")
+
+    def attention(self, batch, query, workspace, layer=0, status_ptr=None, stream_ptr=0):
+        check(self._attention(self.h, layer, batch, query, workspace.h, status_ptr, stream_ptr), "kv8_attention_device")
+
+    def close(self):
+        if self.h:
+            self.L.phonon_cuda_kv8_destroy(self.h)
+            self.h = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+class Kv8Workspace:
+    """Scratch of attention calls on a cache's device; calls that may run at
+    the same time need one each."""
+
+    def __init__(self, cache):
+        self.h = None
+        self.L = cache.L
+        h = C.c_void_p()
+        check(self.L.phonon_cuda_kv8_workspace_create(cache.h, C.byref(h)), "kv8_workspace_create")
+        self.h = h
+
+    def close(self):
+        if self.h:
+            self.L.phonon_cuda_kv8_workspace_destroy(self.h)
+            self.h = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
