@@ -537,6 +537,34 @@ int phonon_cuda_kv8_attention_device(PhononCudaKv8 *cache, uint32_t layer, const
                                      const PhononCudaKv8Query *query, PhononCudaKv8Workspace *workspace,
                                      int32_t *status_dev, void *cuda_stream);
 
+/* ---- norms of queries and keys per head, with the position rotation ----
+ * For every row and head, on device rows: the RMS norm x / sqrt(mean(x^2) +
+ * epsilon) * weight (phonon_rms_norm's formula, src/phonon_transformer.c:66-85,
+ * per head; a side without weights is not normed), then the rotation of the
+ * head's first rotary_dim values by position * theta^(-2i / rotary_dim), pairs
+ * (2i, 2i + 1) as in phonon_cuda_rope_interleaved, or (i, i + rotary_dim / 2)
+ * with `halves`. Angles are reduced in 64 bits, so far positions keep 32-bit
+ * sines (the one-row primitive keeps the reference's 32-bit phases instead).
+ * q is [rows][heads][head_dim], k [rows][kv_heads][head_dim]; either may be
+ * absent (0 heads). Outputs may be the inputs. Enqueued on `cuda_stream` of
+ * `device`, like the cache's calls; status_dev (device, [rows], optional) is
+ * set to PHONON_CUDA_NON_FINITE for a row with a non-finite output. */
+typedef struct {
+    uint32_t type; /* PhononCudaRowType of q, k and the outputs */
+    uint32_t rows, heads, kv_heads;
+    uint32_t head_dim;   /* 32, 64 or 128 */
+    uint32_t rotary_dim; /* 2..head_dim, a multiple of 2 (of 8 with halves) */
+    uint32_t halves;
+    float epsilon, theta;
+    const void *q, *k; /* 16-byte aligned */
+    void *q_out, *k_out;
+    uint64_t q_stride, k_stride, q_out_stride, k_out_stride; /* elements from row to row, multiples of 8 (0: packed) */
+    const int32_t *positions;                                /* device [rows] */
+    const float *q_weight, *k_weight;                        /* device [head_dim], or NULL */
+} PhononCudaQkNormRope;
+int phonon_cuda_qk_norm_rope_device(int device, const PhononCudaQkNormRope *args, int32_t *status_dev,
+                                    void *cuda_stream);
+
 const char *phonon_cuda_status_string(int status);
 
 #ifdef __cplusplus

@@ -9,6 +9,7 @@
 #include "phonon_head.cuh"
 #include "phonon_mimi.cuh"
 #include "phonon_kv8.cuh"
+#include "phonon_qk.cuh"
 
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -4422,6 +4423,73 @@ int phonon_cuda_kv8_attention_device(PhononCudaKv8* c, uint32_t layer, const Pho
     if (!guard.ok) return PHONON_CUDA_DEVICE_ERROR;
     return kv8_enqueue_attention(c->pool, layer, seqs, a, workspace->scratch, c->sms,
                                  static_cast<cudaStream_t>(cuda_stream));
+}
+
+}  // extern "C"
+
+// =================================== per-head norm and rotation on device rows
+namespace {
+
+template <int D, bool kBf16>
+int qk_launch(QkParams& p, bool halves, int sms, cudaStream_t s) {
+    // Warps: a row each, or a slice of its heads while rows are few; at most
+    // 32 warps per SM, each of which computes its frequencies once.
+    const int passes = (p.heads[0] + p.heads[1] + 128 / D - 1) / (128 / D);
+    const long long resident = 32ll * sms;
+    p.slices = static_cast<int>(std::max<long long>(1, std::min<long long>(passes, 2 * resident / p.rows)));
+    const long long ctas = std::min((static_cast<long long>(p.rows) * p.slices + 3) / 4, resident / 4);
+    CUDA_TRY(launch_pdl(halves ? qk_norm_rope_kernel<D, kBf16, true> : qk_norm_rope_kernel<D, kBf16, false>,
+                        dim3(static_cast<unsigned>(ctas)), dim3(128), 0, s, p));
+    return PHONON_CUDA_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int phonon_cuda_qk_norm_rope_device(int device, const PhononCudaQkNormRope* a, int32_t* status_dev, void* cuda_stream) {
+    if (!a || a->type > PHONON_CUDA_ROWS_BF16 || a->rows > (1u << 30) || a->heads > (1u << 16) ||
+        a->kv_heads > (1u << 16) || a->heads + a->kv_heads == 0 ||
+        (a->head_dim != 32 && a->head_dim != 64 && a->head_dim != 128) || a->rotary_dim == 0 ||
+        a->rotary_dim > a->head_dim || a->rotary_dim % (a->halves ? 8 : 2) || !a->positions ||
+        !(a->epsilon >= 0.0f) || !std::isfinite(a->epsilon) || !(a->theta > 0.0f) || !std::isfinite(a->theta) ||
+        !aligned16(a->q_weight) || !aligned16(a->k_weight))
+        return PHONON_CUDA_INVALID_ARGUMENT;
+    QkParams p{};
+    const void* in[2] = {a->q, a->k};
+    void* out[2] = {a->q_out, a->k_out};
+    const uint64_t in_stride[2] = {a->q_stride, a->k_stride}, out_stride[2] = {a->q_out_stride, a->k_out_stride};
+    const uint32_t heads[2] = {a->heads, a->kv_heads};
+    for (int s = 0; s < 2; ++s) {
+        p.heads[s] = static_cast<int>(heads[s]);
+        if (heads[s] == 0) continue;
+        const uint64_t width = static_cast<uint64_t>(heads[s]) * a->head_dim;
+        if (!in[s] || !out[s] || !aligned16(in[s]) || !aligned16(out[s]) ||
+            !kv8_stride(in_stride[s], width, &p.in_stride[s]) || !kv8_stride(out_stride[s], width, &p.out_stride[s]))
+            return PHONON_CUDA_INVALID_ARGUMENT;
+        p.in[s] = in[s];
+        p.out[s] = out[s];
+    }
+    if (a->rows == 0) return PHONON_CUDA_OK;
+    p.weight[0] = a->q_weight;
+    p.weight[1] = a->k_weight;
+    p.positions = a->positions;
+    p.status = status_dev;
+    p.rows = static_cast<int>(a->rows);
+    p.rotary = static_cast<int>(a->rotary_dim);
+    p.epsilon = a->epsilon;
+    p.log2_theta = std::log2(static_cast<double>(a->theta));
+    DeviceGuard guard(device);
+    int sms = 0;
+    if (!guard.ok || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device) != cudaSuccess)
+        return PHONON_CUDA_DEVICE_ERROR;
+    cudaStream_t s = static_cast<cudaStream_t>(cuda_stream);
+    const bool bf16 = a->type == PHONON_CUDA_ROWS_BF16, halves = a->halves != 0;
+    switch (a->head_dim) {
+        case 32: return bf16 ? qk_launch<32, true>(p, halves, sms, s) : qk_launch<32, false>(p, halves, sms, s);
+        case 64: return bf16 ? qk_launch<64, true>(p, halves, sms, s) : qk_launch<64, false>(p, halves, sms, s);
+        default: return bf16 ? qk_launch<128, true>(p, halves, sms, s) : qk_launch<128, false>(p, halves, sms, s);
+    }
 }
 
 }  // extern "C"

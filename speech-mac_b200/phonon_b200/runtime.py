@@ -80,6 +80,15 @@ class Kv8Query(C.Structure):
                 ("q", C.c_void_p), ("out", C.c_void_p), ("q_stride", C.c_uint64), ("out_stride", C.c_uint64)]
 
 
+class QkNormRopeArgs(C.Structure):
+    _fields_ = [("type", C.c_uint32), ("rows", C.c_uint32), ("heads", C.c_uint32), ("kv_heads", C.c_uint32),
+                ("head_dim", C.c_uint32), ("rotary_dim", C.c_uint32), ("halves", C.c_uint32), ("epsilon", C.c_float),
+                ("theta", C.c_float), ("q", C.c_void_p), ("k", C.c_void_p), ("q_out", C.c_void_p),
+                ("k_out", C.c_void_p), ("q_stride", C.c_uint64), ("k_stride", C.c_uint64),
+                ("q_out_stride", C.c_uint64), ("k_out_stride", C.c_uint64), ("positions", C.c_void_p),
+                ("q_weight", C.c_void_p), ("k_weight", C.c_void_p)]
+
+
 class CudaError(RuntimeError):
     def __init__(self, status, what):
         self.status = status
@@ -145,6 +154,7 @@ def lib():
         "phonon_cuda_kv8_append_device": [P, U32, C.POINTER(Kv8Batch), C.POINTER(Kv8Rows), P, P],
         "phonon_cuda_kv8_read_device": [P, U32, C.POINTER(Kv8Batch), C.POINTER(Kv8Rows), P, P],
         "phonon_cuda_kv8_workspace_create": [P, C.POINTER(P)],
+        "phonon_cuda_qk_norm_rope_device": [C.c_int, C.POINTER(QkNormRopeArgs), P, P],
         "phonon_cuda_kv8_attention_device": [P, U32, C.POINTER(Kv8Batch), C.POINTER(Kv8Query), P, P, P],
     }
     for name, args in sig.items():
@@ -695,3 +705,22 @@ class Kv8Workspace:
             self.close()
         except Exception:
             pass
+
+
+class QkNormRope:
+    """phonon_cuda_qk_norm_rope_device over rows at fixed addresses: RMS norm
+    of every query and key head (sides with weights), then the rotation.
+    Calling it enqueues one pass."""
+
+    def __init__(self, q_ptr, k_ptr, q_out_ptr, k_out_ptr, rows, heads, kv_heads, head_dim, positions_ptr,
+                 type=ROWS_F32, q_stride=0, k_stride=0, q_out_stride=0, k_out_stride=0, q_weight_ptr=None,
+                 k_weight_ptr=None, epsilon=1e-6, theta=10000.0, rotary_dim=None, halves=False, device=0):
+        self.device = device
+        self.args = QkNormRopeArgs(type, rows, heads, kv_heads, head_dim,
+                                   head_dim if rotary_dim is None else rotary_dim, int(halves), epsilon, theta, q_ptr,
+                                   k_ptr, q_out_ptr, k_out_ptr, q_stride, k_stride, q_out_stride, k_out_stride,
+                                   positions_ptr, q_weight_ptr, k_weight_ptr)
+        self._fn = lib().phonon_cuda_qk_norm_rope_device
+
+    def __call__(self, status_ptr=None, stream_ptr=0):
+        check(self._fn(self.device, self.args, status_ptr, stream_ptr), "qk_norm_rope_device")
