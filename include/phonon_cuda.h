@@ -42,7 +42,12 @@ typedef enum {
 } PhononCudaStatus;
 
 typedef enum { PHONON_CUDA_LINEAR_Q8_0 = 1, PHONON_CUDA_LINEAR_BF16 = 2 } PhononCudaLinearKind;
-typedef enum { PHONON_CUDA_KV_F32 = 0, PHONON_CUDA_KV_BF16 = 1 } PhononCudaKvType;
+/* PHONON_CUDA_KV_Q8: 8-bit pages with a scale per page and head (the format of
+ * the 8-bit paged K/V cache below), half of bf16's bytes. Every entry point of
+ * the context works on them; steps run per stage (no persistent or cluster
+ * step). kv_write at a position drops what the stream held behind the written
+ * range in its last page. */
+typedef enum { PHONON_CUDA_KV_F32 = 0, PHONON_CUDA_KV_BF16 = 1, PHONON_CUDA_KV_Q8 = 2 } PhononCudaKvType;
 
 #define PHONON_CUDA_WIDTH 512
 #define PHONON_CUDA_PAGE_POSITIONS 16

@@ -630,6 +630,8 @@ struct Lane {
     float2* rope = nullptr;
     cudaEvent_t ready = nullptr;  // recorded when the lane's share of a step is enqueued
     int32_t* chunk_ctr = nullptr;  // [n_layers] attention chunk tickets, zeroed at step start
+    float* kv_stage = nullptr;     // 8-bit K/V: the layer's key and value rows [rows][2][512] before they are quantised
+    Kv8Scratch kv8;                //   and the attention's scratch
     std::vector<long long> h_cuts;  // host scratch of the split planner: chunk boundaries
     std::vector<int32_t> h_pages;   //   page ids in split order
     std::vector<int32_t> h_first_split;  //   first split of each chunk
@@ -642,6 +644,9 @@ struct PhononCuda {
     std::vector<DevLayer> layers;
     void* kv_pool = nullptr;
     long long page_elems = 0;
+    // PHONON_CUDA_KV_Q8: the pages live here instead of in kv_pool
+    Kv8Pool kv8;
+    int32_t* d_kv8_length = nullptr;  // length of the stream that kv_read / kv_write work on
     int32_t* d_table = nullptr;
     std::vector<int32_t> free_pages;
     std::vector<StreamSlot> streams;
@@ -782,8 +787,14 @@ KvView kv_view(const PhononCuda* c) {
     kv.bf16 = c->cfg.kv_type == PHONON_CUDA_KV_BF16;
     kv.table = c->d_table;
     kv.max_pages = kMaxPagesPerStream;
+    kv.stage = nullptr;
     return kv;
 }
+
+bool kv_is_q8(const PhononCuda* c) { return c->cfg.kv_type == PHONON_CUDA_KV_Q8; }
+
+// Bytes of a K/V element in the pages.
+double kv_esize(const PhononCuda* c) { return kv_is_q8(c) ? 1.0 : c->cfg.kv_type == PHONON_CUDA_KV_BF16 ? 2.0 : 4.0; }
 
 bool valid_stream(const PhononCuda* c, uint32_t s) { return s < c->streams.size() && c->streams[s].used; }
 
@@ -846,6 +857,8 @@ struct Batch {
     bool persist = false;  // whole step in step_persist_kernel
     bool split = false;    // one lane's share of a step split over two lanes
     int row0 = 0;          // first row of this batch within the step (the second lane's half)
+    int seq_rows = 1;      // consecutive entries that are rows of one stream (prefill: all of them)
+    int kv8_length = 0;    // 8-bit K/V: bound of the positions attended, coarse so that step graphs repeat
     Lane* lane = nullptr;
     int32_t* d_status = nullptr;  // status words of this batch's entries
     double keys = 0;  // sum over entries of (position + 1)
@@ -1092,6 +1105,20 @@ int upload_batch(PhononCuda* c, const std::vector<int32_t>& slot, const std::vec
     b.attn_grid = guided ? grid : C;
     b.d_rope = lane->rope;
     b.persist = !device_prep;
+    if (kv_is_q8(c)) {
+        // rounded up to an eighth of its octave
+        const int longest = *std::max_element(pos.begin(), pos.end()) + 1;
+        int unit = kPage;
+        while (unit * 8 < longest) unit *= 2;
+        b.kv8_length = (longest + unit - 1) / unit * unit;
+        if (U > 0) {
+            LaunchScope ls(c, PHONON_CUDA_K_OTHER, U * c->cfg.n_layers * 2.0 * kHeads, b.lane->stream);
+            const long long bytes = static_cast<long long>(U) * c->cfg.n_layers * 2 * kHeads;
+            kv8_reset_kernel<<<static_cast<unsigned>(std::min<long long>((bytes + 255) / 256, 1024)), 256, 0, lane->stream>>>(
+                c->kv8.exps, static_cast<int>(c->cfg.n_layers), static_cast<int>(c->cfg.pool_pages), kHeads, b.d_updates, U);
+            CUDA_TRY(cudaGetLastError());
+        }
+    }
     if (!device_prep) {
         *out = b;
         return PHONON_CUDA_OK;
@@ -1112,6 +1139,36 @@ int upload_batch(PhononCuda* c, const std::vector<int32_t>& slot, const std::vec
 // Enqueue layer `l` for the batch: in -> out (out != in).
 int enqueue_attention(PhononCuda* c, const Batch& b, int l, bool digits_out = false, bool no_merge = false);
 
+// 8-bit K/V: the staged key and value rows of the layer into the pages, then
+// attention over them into the lane's fp32 rows.
+int enqueue_kv8(PhononCuda* c, const Batch& b, int l) {
+    cudaStream_t s = b.lane->stream;
+    Kv8Seqs seqs{};
+    seqs.n = b.R / b.seq_rows;
+    seqs.rows = b.R;
+    seqs.rows_per_seq = b.seq_rows;
+    seqs.lengths = b.d_pos + (b.seq_rows - 1);  // (one stream if seq_rows > 1) its last position ...
+    seqs.length_bias = 1;                       // ... plus one
+    seqs.slots = b.d_slot;
+    seqs.pages = c->d_table;
+    seqs.page_stride = kMaxPagesPerStream;
+    seqs.max_rows = b.seq_rows;
+    seqs.max_length = b.kv8_length;
+    seqs.status = b.d_status;
+    const double act = 4.0 * b.R * kWidth;
+    int st;
+    {
+        LaunchScope ls(c, PHONON_CUDA_K_OTHER, 2.0 * act + b.R * 2.0 * kWidth, s);
+        if ((st = kv8_enqueue_append(c->kv8, static_cast<uint32_t>(l), seqs, false, b.lane->kv_stage,
+                                     b.lane->kv_stage + kWidth, 2 * kWidth, s)))
+            return st;
+    }
+    LaunchScope ls(c, PHONON_CUDA_K_ATTENTION, b.keys * 2.0 * kWidth + 2.0 * act, s);
+    return kv8_enqueue_attention(c->kv8, static_cast<uint32_t>(l), seqs,
+                                 Kv8Attend{b.lane->q, b.lane->a, kWidth, kWidth, 1, 0.125f, 0, false}, b.lane->kv8,
+                                 c->sms, s);
+}
+
 // Split-K attention then the split merge. With digits_out the merge writes
 // the digit rows of the attention output (tensor-core path) instead of fp32;
 // with no_merge the consumer merges the partials itself.
@@ -1119,7 +1176,7 @@ int enqueue_attention(PhononCuda* c, const Batch& b, int l, bool digits_out, boo
     cudaStream_t s = b.lane->stream;
     const KvView kv = kv_view(c);
     const double act = 4.0 * b.R;
-    const double esize = kv.bf16 ? 2.0 : 4.0;
+    const double esize = kv_esize(c);
     AttnParams ap{};
     ap.q = b.lane->q;
     ap.slot = b.d_slot;
@@ -1171,9 +1228,10 @@ int enqueue_attention(PhononCuda* c, const Batch& b, int l, bool digits_out, boo
 int enqueue_layer_tensor(PhononCuda* c, const Batch& b, int l, const float* in, float* out) {
     const DevLayer& L = c->layers[l];
     cudaStream_t s = b.lane->stream;
-    const KvView kv = kv_view(c);
+    KvView kv = kv_view(c);
+    kv.stage = b.lane->kv_stage;
     const int B = b.R, Bpad = (b.R + 31) / 32 * 32, nd = kDigits * Bpad;
-    const double act = 4.0 * B, esize = kv.bf16 ? 2.0 : 4.0, dig = kDigits * Bpad;
+    const double act = 4.0 * B, esize = kv_esize(c), dig = kDigits * Bpad;
     GemmParams g{};
     g.B = B;
     g.exps = b.lane->exps;
@@ -1199,8 +1257,13 @@ int enqueue_layer_tensor(PhononCuda* c, const Batch& b, int l, const float* in, 
         CUDA_TRY(launch_linear_gemm<GEPI_QKV>(L.qkv, b.lane->tm_dig512, nd, g, s));
     }
     // 2. attention; the combine writes the digit rows of the attention output
-    int st = enqueue_attention(c, b, l, true);
+    int st = kv_is_q8(c) ? enqueue_kv8(c, b, l) : enqueue_attention(c, b, l, true);
     if (st) return st;
+    if (kv_is_q8(c)) {
+        LaunchScope ls(c, PHONON_CUDA_K_COMBINE, act * kWidth + dig * 512, b.lane->stream);
+        CUDA_TRY((launch_digits<512, false>(b.lane->a, kWidth, nullptr, nullptr, B, Bpad, b.lane->dig512, b.lane->exps,
+                                            b.d_status, s)));
+    }
     // 3. h = x + attn Wout^T
     GemmParams go = g;
     go.rows = 512;
@@ -1257,7 +1320,8 @@ int enqueue_layer(PhononCuda* c, const Batch& b, int l, const float* in, float* 
         return enqueue_layer_tensor(c, b, l, in, out);
     const bool q8 = L.q8;
     cudaStream_t s = b.lane->stream;
-    const KvView kv = kv_view(c);
+    KvView kv = kv_view(c);
+    kv.stage = b.lane->kv_stage;
     GemvParams p{};
     p.B = b.R;
     p.status = b.d_status;
@@ -1277,17 +1341,17 @@ int enqueue_layer(PhononCuda* c, const Batch& b, int l, const float* in, float* 
     p.kv = kv;
     p.layer = l;
     const double act = 4.0 * b.R;  // bytes per activation element across the batch
-    const double esize = kv.bf16 ? 2.0 : 4.0;
+    const double esize = kv_esize(c);
     {
         LaunchScope ls(c, PHONON_CUDA_K_QKV, linear_bytes(L.qkv) + act * (kWidth + kWidth) + b.R * 2.0 * kWidth * esize, b.lane->stream);
         CUDA_TRY((launch_gemv<1, SRC_LN, EPI_QKV>(q8, p, s)));
     }
     // 2. split-K attention (the out projection merges the splits)
     {
-        int st = enqueue_attention(c, b, l, false, true);
+        int st = kv_is_q8(c) ? enqueue_kv8(c, b, l) : enqueue_attention(c, b, l, false, true);
         if (st) return st;
     }
-    // 3. h = x + attn Wout^T, attn merged from the split partials
+    // 3. h = x + attn Wout^T, attn merged from the split partials (8-bit K/V: merged already)
     GemvParams po{};
     po.B = b.R;
     po.status = b.d_status;
@@ -1298,6 +1362,7 @@ int enqueue_layer(PhononCuda* c, const Batch& b, int l, const float* in, float* 
     po.part = b.lane->part;
     po.first = b.d_first;
     po.count = b.d_count;
+    po.x = b.lane->a;
     po.ldx = kWidth;
     po.res = in;
     po.ldres = kWidth;
@@ -1305,7 +1370,8 @@ int enqueue_layer(PhononCuda* c, const Batch& b, int l, const float* in, float* 
     po.ldy = kWidth;
     {
         LaunchScope ls(c, PHONON_CUDA_K_OUT, linear_bytes(L.out) + act * 3 * kWidth, b.lane->stream);
-        CUDA_TRY((launch_gemv<1, SRC_MERGE, EPI_RESID>(q8, po, s)));
+        if (kv_is_q8(c)) CUDA_TRY((launch_gemv<1, SRC_X, EPI_RESID>(q8, po, s)));
+        else CUDA_TRY((launch_gemv<1, SRC_MERGE, EPI_RESID>(q8, po, s)));
     }
     // 4. g = GELU(LN2(h) Wup^T)
     GemvParams pu{};
@@ -1385,8 +1451,8 @@ int enqueue_layers_graphed(PhononCuda* c, const Batch& b, const float* in, float
     shape.R = b.R;
     // Kernels read S and the chunk tables through the plan header; the TMA
     // attention grid is fixed except for small (static) plans.
-    shape.S = c->attn_tma ? 0 : b.S;
-    shape.chunks = b.attn_grid;
+    shape.S = kv_is_q8(c) ? b.kv8_length : c->attn_tma ? 0 : b.S;
+    shape.chunks = kv_is_q8(c) ? 0 : b.attn_grid;
     shape.in = in;
     shape.out = final_out;
     if (c->graph_exec && c->graph_shape == shape) {
@@ -1773,9 +1839,11 @@ void destroy_context(PhononCuda* c) {
     void* dev[] = {c->kv_pool, c->d_table, c->d_freq, c->d_x0, c->d_x1, c->d_y, c->d_q, c->d_a,
                    c->d_h, c->d_g, c->d_part, c->d_stage, c->d_meta, c->d_status,
                    c->d_dig512, c->d_dig2048, c->d_exps, c->d_err, c->d_rope,
-                   c->d_players, c->d_bar, c->d_cltc};
+                   c->d_players, c->d_bar, c->d_cltc, c->d_kv8_length, c->lanes[0].kv_stage, c->lanes[1].kv_stage};
     for (void* p : dev)
         if (p) cudaFree(p);
+    c->kv8.release();
+    for (Lane& lane : c->lanes) lane.kv8.release();
     void* host[] = {c->h_meta, c->h_x, c->h_y, c->h_stage, c->h_status};
     for (void* p : host)
         if (p) cudaFreeHost(p);
@@ -1847,7 +1915,7 @@ int phonon_cuda_create(const PhononCudaConfig* config, const PhononCudaLayer* la
     *out = nullptr;
     const PhononCudaConfig& cfg = *config;
     if (cfg.n_layers < 1 || cfg.n_layers > kMaxLayers || cfg.max_streams < 1 || cfg.max_batch < 1 ||
-        cfg.max_batch > 65536 || cfg.pool_pages < 1 || cfg.kv_type > PHONON_CUDA_KV_BF16 ||
+        cfg.max_batch > 65536 || cfg.pool_pages < 1 || cfg.kv_type > PHONON_CUDA_KV_Q8 ||
         !(cfg.theta > 0.0f) || !std::isfinite(cfg.theta))
         return PHONON_CUDA_INVALID_ARGUMENT;
     int st = set_device(cfg.device);
@@ -1870,6 +1938,7 @@ int phonon_cuda_create(const PhononCudaConfig* config, const PhononCudaLayer* la
         if ((st = load_layer(&c->layers[l], layers[l]))) return fail(st);
     float freq[32];
     rope_frequencies(cfg.theta, kHeadDim, freq);
+    const bool q8_kv = cfg.kv_type == PHONON_CUDA_KV_Q8;
     const size_t esize = cfg.kv_type == PHONON_CUDA_KV_BF16 ? 2 : 4;
     c->page_elems = static_cast<long long>(cfg.n_layers) * 2 * kHeads * kPage * kHeadDim;
     c->cap_rows = static_cast<int>(std::max<uint32_t>(cfg.max_batch, kPrefillChunk));
@@ -1881,7 +1950,17 @@ int phonon_cuda_create(const PhononCudaConfig* config, const PhononCudaLayer* la
     c->meta_ints = static_cast<int>(4 * c->cap_rows + kPlanHeader + 4 * c->max_splits +
                                     2 * (std::max(kMaxChunks, kMaxSms) + 1) + batch_pages + 3 * U_max);
     const size_t rows = static_cast<size_t>(c->cap_rows);
-    bool ok = cudaMalloc(&c->kv_pool, static_cast<size_t>(cfg.pool_pages) * c->page_elems * esize) == cudaSuccess &&
+    if (cudaDeviceGetAttribute(&c->sms, cudaDevAttrMultiProcessorCount, cfg.device) != cudaSuccess)
+        return fail(PHONON_CUDA_DEVICE_ERROR);
+    if (q8_kv) {
+        st = c->kv8.alloc(cfg.n_layers, cfg.pool_pages, kHeads, kHeadDim);
+        if (st == PHONON_CUDA_OK) st = c->lanes[0].kv8.alloc(c->sms);
+        if (st == PHONON_CUDA_OK && cfg.max_batch >= 96) st = c->lanes[1].kv8.alloc(c->sms);
+        if (st) return fail(st);
+    }
+    bool ok = (q8_kv ? cudaMalloc(&c->lanes[0].kv_stage, rows * 2 * kWidth * 4) == cudaSuccess &&
+                           cudaMalloc(&c->d_kv8_length, 4) == cudaSuccess
+                     : cudaMalloc(&c->kv_pool, static_cast<size_t>(cfg.pool_pages) * c->page_elems * esize) == cudaSuccess) &&
               cudaMalloc(&c->d_table, static_cast<size_t>(cfg.max_streams) * kMaxPagesPerStream * 4) == cudaSuccess &&
               cudaMalloc(&c->d_freq, sizeof(freq)) == cudaSuccess &&
               cudaMalloc(&c->d_x0, rows * kWidth * 4) == cudaSuccess &&
@@ -1947,13 +2026,14 @@ int phonon_cuda_create(const PhononCudaConfig* config, const PhononCudaLayer* la
                 cudaMalloc(&L1.exps, rows_pad * 4) == cudaSuccess &&
                 cudaMalloc(&L1.rope, rows * 32 * sizeof(float2)) == cudaSuccess &&
                 cudaMalloc(&L1.chunk_ctr, ctr_bytes) == cudaSuccess &&
+                (!q8_kv || cudaMalloc(&L1.kv_stage, rows * 2 * kWidth * 4) == cudaSuccess) &&
                 cudaMemset(L1.chunk_ctr, 0, ctr_bytes) == cudaSuccess;
             if (!ok1) return fail(PHONON_CUDA_OUT_OF_MEMORY);
             c->lane1_ok = c->tensor_ok && make_i8_map(&L1.tm_dig512, L1.dig512, rows_pad * kDigits, 512) &&
                           make_i8_map(&L1.tm_dig2048, L1.dig2048, rows_pad * kDigits, 2048);
         }
     }
-    {
+    if (!q8_kv) {
         // Row r of the pool = 64 dims of (layer, page, k|v, head, slot); a
         // layer-page K block is rows [(layer*pool_pages + page)*256, +128).
         const uint64_t kv_rows = static_cast<uint64_t>(cfg.pool_pages) * cfg.n_layers * 256;
@@ -2406,6 +2486,7 @@ int phonon_cuda_append(PhononCuda* c, uint32_t stream, const float* rows, uint32
         Batch b;
         result = upload_batch(c, slot, pos, p0 == 0 ? updates : std::vector<int32_t>{}, &b);
         if (result != PHONON_CUDA_OK) break;
+        b.seq_rows = R;
         std::memcpy(c->h_x, rows + static_cast<size_t>(p0) * kWidth, static_cast<size_t>(R) * kWidth * 4);
         cudaMemcpyAsync(c->d_x0, c->h_x, static_cast<size_t>(R) * kWidth * 4, cudaMemcpyHostToDevice, c->stream);
         cudaMemsetAsync(c->d_status, 0, R * 4, c->stream);
@@ -2452,6 +2533,31 @@ static int check_kv_range(PhononCuda* c, uint32_t stream, uint32_t layer_begin, 
     return PHONON_CUDA_OK;
 }
 
+// 8-bit K/V: positions [position, position + count) of a stream between the
+// pages of its layers and the device staging rows ([layer][count][512] keys,
+// then the values).
+static int kv8_transfer(PhononCuda* c, uint32_t stream, uint32_t layer_begin, uint32_t layer_count, uint32_t position,
+                        uint32_t count, bool write) {
+    const int32_t length = static_cast<int32_t>(position + count);
+    CUDA_TRY(cudaMemcpyAsync(c->d_kv8_length, &length, 4, cudaMemcpyHostToDevice, c->stream));
+    Kv8Seqs seqs{};
+    seqs.n = 1;
+    seqs.rows = seqs.rows_per_seq = seqs.max_rows = static_cast<int>(count);
+    seqs.lengths = c->d_kv8_length;
+    seqs.pages = c->d_table + static_cast<size_t>(stream) * kMaxPagesPerStream;
+    seqs.page_stride = kMaxPagesPerStream;
+    seqs.max_length = PHONON_CUDA_MAX_POSITIONS;
+    const size_t per_layer = static_cast<size_t>(count) * kWidth;
+    for (uint32_t l = 0; l < layer_count; ++l) {
+        float* keys = c->d_stage + l * per_layer;
+        float* values = c->d_stage + (layer_count + l) * per_layer;
+        const int st = write ? kv8_enqueue_append(c->kv8, layer_begin + l, seqs, false, keys, values, kWidth, c->stream)
+                             : kv8_enqueue_read(c->kv8, layer_begin + l, seqs, false, keys, values, kWidth, c->stream);
+        if (st) return st;
+    }
+    return PHONON_CUDA_OK;
+}
+
 int phonon_cuda_kv_write(PhononCuda* c, uint32_t stream, uint32_t layer_begin, uint32_t layer_count,
                          uint32_t position, uint32_t count, const float* keys, const float* values) {
     if (!c || !keys || !values) return PHONON_CUDA_INVALID_ARGUMENT;
@@ -2479,9 +2585,13 @@ int phonon_cuda_kv_write(PhononCuda* c, uint32_t stream, uint32_t layer_begin, u
     std::memcpy(c->h_stage, keys, n * 4);
     std::memcpy(c->h_stage + n, values, n * 4);
     CUDA_TRY(cudaMemcpyAsync(c->d_stage, c->h_stage, 2 * n * 4, cudaMemcpyHostToDevice, c->stream));
-    kv_rows_kernel<<<static_cast<unsigned>(std::min<size_t>((2 * n + 255) / 256, 4096)), 256, 0, c->stream>>>(
-        kv_view(c), static_cast<int>(stream), static_cast<int>(layer_begin), static_cast<int>(layer_count),
-        static_cast<int>(position), static_cast<int>(count), c->d_stage, 1);
+    if (kv_is_q8(c)) {
+        if ((st = kv8_transfer(c, stream, layer_begin, layer_count, position, count, true))) return st;
+    } else {
+        kv_rows_kernel<<<static_cast<unsigned>(std::min<size_t>((2 * n + 255) / 256, 4096)), 256, 0, c->stream>>>(
+            kv_view(c), static_cast<int>(stream), static_cast<int>(layer_begin), static_cast<int>(layer_count),
+            static_cast<int>(position), static_cast<int>(count), c->d_stage, 1);
+    }
     CUDA_TRY(cudaGetLastError());
     CUDA_TRY(cudaStreamSynchronize(c->stream));
     return PHONON_CUDA_OK;
@@ -2504,9 +2614,13 @@ int phonon_cuda_kv_read(PhononCuda* c, uint32_t stream, uint32_t layer_begin, ui
     }
     if (readable == 0) return PHONON_CUDA_OK;
     if ((st = set_device(c->cfg.device)) || (st = reserve_stage(c, 2 * n))) return st;
-    kv_rows_kernel<<<static_cast<unsigned>(std::min<size_t>((2 * n + 255) / 256, 4096)), 256, 0, c->stream>>>(
-        kv_view(c), static_cast<int>(stream), static_cast<int>(layer_begin), static_cast<int>(layer_count),
-        static_cast<int>(position), static_cast<int>(readable), c->d_stage, 0);
+    if (kv_is_q8(c)) {
+        if ((st = kv8_transfer(c, stream, layer_begin, layer_count, position, readable, false))) return st;
+    } else {
+        kv_rows_kernel<<<static_cast<unsigned>(std::min<size_t>((2 * n + 255) / 256, 4096)), 256, 0, c->stream>>>(
+            kv_view(c), static_cast<int>(stream), static_cast<int>(layer_begin), static_cast<int>(layer_count),
+            static_cast<int>(position), static_cast<int>(readable), c->d_stage, 0);
+    }
     CUDA_TRY(cudaGetLastError());
     const size_t nr = static_cast<size_t>(layer_count) * readable * kWidth;
     CUDA_TRY(cudaMemcpyAsync(c->h_stage, c->d_stage, 2 * nr * 4, cudaMemcpyDeviceToHost, c->stream));
@@ -2542,10 +2656,14 @@ int phonon_cuda_stream_fill_synthetic(PhononCuda* c, uint32_t stream, uint32_t l
         return st;
     }
     {
-        LaunchScope ls(c, PHONON_CUDA_K_OTHER, static_cast<double>(length) * c->page_elems / kPage *
-                                                   (c->cfg.kv_type == PHONON_CUDA_KV_BF16 ? 2 : 4));
-        kv_fill_kernel<<<296, 256, 0, c->stream>>>(kv_view(c), static_cast<int>(stream),
-                                                   static_cast<int>(c->cfg.n_layers), static_cast<int>(length), seed);
+        LaunchScope ls(c, PHONON_CUDA_K_OTHER, static_cast<double>(length) * c->page_elems / kPage * kv_esize(c));
+        if (kv_is_q8(c))
+            kv8_fill_kernel<<<296, 256, 0, c->stream>>>(c->kv8.pool, c->kv8.exps, static_cast<int>(c->cfg.pool_pages),
+                                                        c->d_table + static_cast<size_t>(stream) * kMaxPagesPerStream,
+                                                        static_cast<int>(c->cfg.n_layers), static_cast<int>(length), seed);
+        else
+            kv_fill_kernel<<<296, 256, 0, c->stream>>>(kv_view(c), static_cast<int>(stream),
+                                                       static_cast<int>(c->cfg.n_layers), static_cast<int>(length), seed);
         CUDA_TRY(cudaGetLastError());
     }
     CUDA_TRY(cudaStreamSynchronize(c->stream));

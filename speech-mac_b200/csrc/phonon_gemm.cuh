@@ -441,6 +441,8 @@ __global__ void __launch_bounds__(kGemmThreads, kWD == 1 ? 2 : 1)
                                 if (!isfinite(v[t])) flag_nonfinite(p.status, b);
                                 if (region == 0) {
                                     p.q[static_cast<size_t>(b) * kWidth + within] = v[t];
+                                } else if (p.kv.stage) {
+                                    p.kv.stage[(static_cast<size_t>(b) * 2 + region - 1) * kWidth + within] = v[t];
                                 } else {
                                     const long long off = kv_offset(p.kv, meta->page[tt], p.layer, region - 1, within >> 6,
                                                                     meta->pos[tt] % kPage) + (within & 63);

@@ -263,6 +263,8 @@ struct KvView {
     int bf16;               // 1: bf16 elements, 0: fp32
     const int32_t* table;   // [stream slot][max_pages]
     int max_pages;
+    float* stage;           // 8-bit K/V: the step's key and value rows [batch row][k|v][512], quantised by the
+                            // append launch that follows; null otherwise
 };
 
 __device__ __forceinline__ long long kv_offset(const KvView& kv, int page, int layer, int which,
@@ -592,6 +594,9 @@ __global__ void __launch_bounds__(kGemvWarps * 32) gemv_kernel(GemvParams p) {
                 if (!isfinite(v0) || !isfinite(v1)) flag_nonfinite(p.status, b);
                 if (region == 0) {
                     *reinterpret_cast<float2*>(p.q + static_cast<size_t>(b) * kWidth + within) =
+                        make_float2(v0, v1);
+                } else if (p.kv.stage) {
+                    *reinterpret_cast<float2*>(p.kv.stage + (static_cast<size_t>(b) * 2 + region - 1) * kWidth + within) =
                         make_float2(v0, v1);
                 } else {
                     const int page = p.kv.table[static_cast<size_t>(p.slot[b]) * p.kv.max_pages + pos / kPage];

@@ -275,6 +275,53 @@ __global__ void __launch_bounds__(128) kv8_append_kernel(Kv8AppendParams p) {
     }
 }
 
+// ------------------------------------------- pages of a decode context (8 x 64)
+// Where a block holds dim `dim` of position `slot` of its page.
+template <int D>
+__device__ __forceinline__ int kv8_byte(int which, int slot, int dim) {
+    if (which == 0) return slot * D + dim;
+    const int t = (slot & 7) >> 1, k = (slot & 1) + 2 * (slot >> 3);
+    return (dim >> 5) * 512 + (((dim & 31) >> 2) * 4 + t) * 16 + (dim & 3) * 4 + k;
+}
+
+// Pages that a stream has just received (the step's (slot, index, page)
+// updates) forget their scales in every layer: a stream may write its first
+// row of a page at any slot.
+__global__ void kv8_reset_kernel(int8_t* exps, int layers, int pool_pages, int heads, const int32_t* updates, int n) {
+    const int bytes = heads * 2;
+    const long long total = static_cast<long long>(n) * layers * bytes;
+    for (long long i = static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x; i < total;
+         i += static_cast<long long>(gridDim.x) * blockDim.x) {
+        const int b = static_cast<int>(i % bytes), layer = static_cast<int>(i / bytes % layers);
+        const int page = updates[3 * (i / bytes / layers) + 2];
+        exps[(static_cast<size_t>(layer) * pool_pages + page) * bytes + b] = kKv8MinExp;
+    }
+}
+
+// kv_fill_kernel's values in 8 bits: below 2.449 in magnitude, so every block
+// has the scale 2^-5.
+__global__ void kv8_fill_kernel(uint8_t* pool, int8_t* exps, int pool_pages, const int32_t* table, int n_layers, int length,
+                                uint64_t seed) {
+    constexpr int kBlockBytes = kKv8Block * kHeadDim;
+    const long long per_pos = static_cast<long long>(n_layers) * 2 * kWidth;
+    const long long total = per_pos * length;
+    for (long long i = static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x; i < total;
+         i += static_cast<long long>(gridDim.x) * blockDim.x) {
+        const int position = static_cast<int>(i / per_pos);
+        const long long r = i % per_pos;
+        const int layer = static_cast<int>(r / (2 * kWidth));
+        const int which = static_cast<int>((r / kWidth) & 1);
+        const int d = static_cast<int>(r % kWidth);
+        const uint32_t h = hash32(seed * 0x9E3779B97F4A7C15ull + static_cast<uint64_t>(i));
+        const float u = (static_cast<float>(h & 0xffff) + static_cast<float>(h >> 16)) * (1.0f / 65536.0f);
+        const float v = (u - 1.0f) * 2.449f;
+        const size_t block = (static_cast<size_t>(layer) * pool_pages + table[position / kPage]) * kHeads + (d >> 6);
+        pool[(block * 2 + which) * kBlockBytes + kv8_byte<kHeadDim>(which, position % kPage, d & 63)] =
+            static_cast<uint8_t>(kv8_code(v, 32.0f));
+        if ((d & 63) == 0 && position % kPage == 0) exps[block * 2 + which] = -5;
+    }
+}
+
 // --------------------------------------------------------------------- read
 struct Kv8ReadParams {
     Kv8View cache;

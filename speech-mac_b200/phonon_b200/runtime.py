@@ -13,7 +13,7 @@ from ._libs import load_cuda
 KERNEL_CLASSES = ("qkv", "attention", "combine", "out", "up", "down", "other", "fused", "head")
 OK, INVALID, NON_FINITE, OOM, POOL_EXHAUSTED, CAPACITY, BAD_POSITION, CANCELLED, DEVICE_ERROR = range(9)
 Q8_0, BF16 = 1, 2
-KV_F32, KV_BF16 = 0, 1
+KV_F32, KV_BF16, KV_Q8 = 0, 1, 2
 ROWS_F32, ROWS_BF16 = 0, 1  # PhononCudaRowType
 FUSED_MAX_BATCH = 64  # PHONON_CUDA_FUSED_MAX_BATCH
 MAX_POSITIONS = 8192  # PHONON_CUDA_MAX_POSITIONS
