@@ -432,7 +432,7 @@ cudaError_t launch_digits(const float* x, int ldx, const float* ln_w, const floa
 // scale the smallest until rows are written.
 struct Kv8Pool {
     uint8_t* pool = nullptr;
-    int8_t* exps = nullptr;
+    uint8_t* exps = nullptr;
     uint32_t layers = 0, pages = 0, heads = 0, dim = 0;
     size_t layer_bytes() const { return static_cast<size_t>(pages) * heads * 2 * kKv8Block * dim; }
     size_t layer_exps() const { return static_cast<size_t>(pages) * heads * 2; }
@@ -453,7 +453,7 @@ struct Kv8Pool {
             return PHONON_CUDA_OUT_OF_MEMORY;
         }
         CUDA_TRY(cudaMemset(pool, 128, layers * layer_bytes()));
-        CUDA_TRY(cudaMemset(exps, kKv8MinExp & 0xff, layers * layer_exps()));
+        CUDA_TRY(cudaMemset(exps, kKv8MinExp + 127, layers * layer_exps()));
         CUDA_TRY(cudaStreamSynchronize(nullptr));  // callers' streams do not wait for the legacy stream
         return PHONON_CUDA_OK;
     }
@@ -541,10 +541,11 @@ struct Kv8Attend {
     bool bf16;
 };
 
-template <int D, int NT, int PB, bool kBf16>
+template <int D, int NT, int PB, int kMode, int kWarps>
 int kv8_launch_attention(const Kv8Pool& c, uint32_t layer, const Kv8Seqs& seqs, const Kv8Attend& a,
                          const Kv8Scratch& w, int sms, cudaStream_t s) {
-    static_assert(8 * NT * D <= kKv8TileFloats, "a partial result outgrows its scratch");
+    constexpr int kRows = kMode == KV8_F32_PACKED ? 4 : 8 * NT;
+    static_assert(kRows * D <= kKv8TileFloats, "a partial result outgrows its scratch");
     Kv8AttnParams p{};
     p.cache = c.view(layer);
     p.seqs = seqs;
@@ -556,11 +557,11 @@ int kv8_launch_attention(const Kv8Pool& c, uint32_t layer, const Kv8Seqs& seqs, 
     p.scale = a.scale * 1.44269504088896340736f;
     p.window = a.window;
     const long long rows = static_cast<long long>(seqs.max_rows) * a.group;
-    p.tiles = static_cast<int>((rows + 8 * NT - 1) / (8 * NT));
+    p.tiles = static_cast<int>((rows + kRows - 1) / kRows);
     const long long items = static_cast<long long>(seqs.n) * p.tiles * c.heads;
     // pages that a row tile can see
     long long span = seqs.max_length;
-    if (a.window) span = std::min<long long>(span, static_cast<long long>(a.window) + (8 * NT - 1) / a.group + kKv8Block);
+    if (a.window) span = std::min<long long>(span, static_cast<long long>(a.window) + (kRows - 1) / a.group + kKv8Block);
     const long long pages = std::max<long long>(1, (span + kKv8Block - 1) / kKv8Block);
     const long long want = static_cast<long long>(kKv8Ctas) * sms;
     long long splits = items >= want ? 1 : (want + items - 1) / items;
@@ -572,33 +573,37 @@ int kv8_launch_attention(const Kv8Pool& c, uint32_t layer, const Kv8Seqs& seqs, 
     p.part = w.part;
     p.part_ml = w.ml;
     p.arrived = w.arrived;
-    CUDA_TRY(launch_pdl(kv8_attention_kernel<D, NT, PB, kBf16>, dim3(static_cast<unsigned>(items * splits)),
-                        dim3(32 * kKv8Warps), 0, s, p));
+    CUDA_TRY(launch_pdl(kv8_attention_kernel<D, NT, PB, kMode, kWarps>, dim3(static_cast<unsigned>(items * splits)),
+                        dim3(32 * kWarps), 0, s, p));
     return PHONON_CUDA_OK;
 }
 
-template <int D, int PB, bool kBf16>
+// By the rows that share a K/V head of a sequence: what they need of the
+// column tiles (four fp32 rows or eight bf16 rows fill one).
+template <int D>
 int kv8_attention_rows(const Kv8Pool& c, uint32_t layer, const Kv8Seqs& seqs, const Kv8Attend& a, const Kv8Scratch& w,
                        int sms, cudaStream_t s) {
     const long long rows = static_cast<long long>(seqs.max_rows) * a.group;
-    if (rows <= 8) return kv8_launch_attention<D, 1, PB, kBf16>(c, layer, seqs, a, w, sms, s);
-    if (rows <= 16 || D == 128) return kv8_launch_attention<D, 2, PB / 2, kBf16>(c, layer, seqs, a, w, sms, s);
-    if constexpr (D < 128) return kv8_launch_attention<D, 4, PB / 4, kBf16>(c, layer, seqs, a, w, sms, s);
+    constexpr int PB = D == 128 ? 2 : 4, W = 4;
+    if (a.bf16) {
+        if (rows <= 8) return kv8_launch_attention<D, 1, PB, KV8_BF16, W>(c, layer, seqs, a, w, sms, s);
+        if (rows <= 16 || D == 128)
+            return kv8_launch_attention<D, 2, PB / 2, KV8_BF16, W>(c, layer, seqs, a, w, sms, s);
+        if constexpr (D < 128) return kv8_launch_attention<D, 4, PB / 4, KV8_BF16, W>(c, layer, seqs, a, w, sms, s);
+    }
+    if (rows <= 4) return kv8_launch_attention<D, 1, PB, KV8_F32_PACKED, W>(c, layer, seqs, a, w, sms, s);
+    if (rows <= 8) return kv8_launch_attention<D, 1, PB, KV8_F32, W>(c, layer, seqs, a, w, sms, s);
+    if (rows <= 16 || D == 128) return kv8_launch_attention<D, 2, PB / 2, KV8_F32, W>(c, layer, seqs, a, w, sms, s);
+    if constexpr (D < 128) return kv8_launch_attention<D, 4, PB / 4, KV8_F32, W>(c, layer, seqs, a, w, sms, s);
     return PHONON_CUDA_INVALID_ARGUMENT;
 }
 
 int kv8_enqueue_attention(const Kv8Pool& c, uint32_t layer, const Kv8Seqs& seqs, const Kv8Attend& a,
                           const Kv8Scratch& w, int sms, cudaStream_t s) {
     switch (c.dim) {
-        case 32:
-            return a.bf16 ? kv8_attention_rows<32, 4, true>(c, layer, seqs, a, w, sms, s)
-                          : kv8_attention_rows<32, 4, false>(c, layer, seqs, a, w, sms, s);
-        case 64:
-            return a.bf16 ? kv8_attention_rows<64, 4, true>(c, layer, seqs, a, w, sms, s)
-                          : kv8_attention_rows<64, 4, false>(c, layer, seqs, a, w, sms, s);
-        default:
-            return a.bf16 ? kv8_attention_rows<128, 2, true>(c, layer, seqs, a, w, sms, s)
-                          : kv8_attention_rows<128, 2, false>(c, layer, seqs, a, w, sms, s);
+        case 32: return kv8_attention_rows<32>(c, layer, seqs, a, w, sms, s);
+        case 64: return kv8_attention_rows<64>(c, layer, seqs, a, w, sms, s);
+        default: return kv8_attention_rows<128>(c, layer, seqs, a, w, sms, s);
     }
 }
 

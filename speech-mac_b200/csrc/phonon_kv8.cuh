@@ -15,7 +15,7 @@
 // less than one unit of the last scale.
 //
 // Layout. pool: [layer][page][head][keys 16*D | values 16*D] bytes, exponents
-// [layer][page][head][2]. Keys lie [position][dim]. Values lie in the order in
+// [layer][page][head][2], e + 127 in a byte. Keys lie [position][dim]. Values lie in the order in
 // which the attention's lanes hold them: the 16 bytes of lane 4g + t in chunk
 // j are dims 32j + 4g + w (w = byte / 4) of positions 2t, 2t + 1, 2t + 8,
 // 2t + 9, so that a lane's 16-byte loads of either are matrix fragments as
@@ -37,7 +37,7 @@ constexpr int kStatusCapacity = 5;  // PHONON_CUDA_CAPACITY
 // One layer of a cache.
 struct Kv8View {
     uint8_t* pool;
-    int8_t* exps;
+    uint8_t* exps;
     int pool_pages;
     int heads;  // K/V heads
 };
@@ -95,7 +95,7 @@ __device__ __forceinline__ uint8_t* kv8_block(const Kv8View& c, int page, int he
     return c.pool + (static_cast<size_t>(page) * c.heads + head) * (2 * kKv8Block * D) + which * (kKv8Block * D);
 }
 
-__device__ __forceinline__ int8_t* kv8_exp(const Kv8View& c, int page, int head) {
+__device__ __forceinline__ uint8_t* kv8_exp(const Kv8View& c, int page, int head) {
     return c.exps + (static_cast<size_t>(page) * c.heads + head) * 2;
 }
 
@@ -184,8 +184,8 @@ __global__ void __launch_bounds__(128) kv8_append_kernel(Kv8AppendParams p) {
         return;
     }
     const int lo = max(start - p0, 0), hi = min(q.length - p0, kKv8Block);  // new slots [lo, hi), kept [0, lo)
-    int8_t* ep = kv8_exp(p.cache, page, head) + which;
-    const int held = lo > 0 ? *ep : kKv8MinExp;
+    uint8_t* ep = kv8_exp(p.cache, page, head) + which;
+    const int held = lo > 0 ? *ep - 127 : kKv8MinExp;
     uint8_t* dst = kv8_block<D>(p.cache, page, head, which);
     const void* src = p.rows[which];
 
@@ -222,7 +222,7 @@ __global__ void __launch_bounds__(128) kv8_append_kernel(Kv8AppendParams p) {
     const int e = max(kv8_exponent(amax), held);
     const float inverse = pow2i(-e), shrink = pow2i(held - e);
     const bool raised = lo > 0 && e > held;
-    if (lane == 0) *ep = static_cast<int8_t>(e);
+    if (lane == 0) *ep = static_cast<uint8_t>(e + 127);
 
     if (which == 0) {
 #pragma unroll
@@ -287,20 +287,20 @@ __device__ __forceinline__ int kv8_byte(int which, int slot, int dim) {
 // Pages that a stream has just received (the step's (slot, index, page)
 // updates) forget their scales in every layer: a stream may write its first
 // row of a page at any slot.
-__global__ void kv8_reset_kernel(int8_t* exps, int layers, int pool_pages, int heads, const int32_t* updates, int n) {
+__global__ void kv8_reset_kernel(uint8_t* exps, int layers, int pool_pages, int heads, const int32_t* updates, int n) {
     const int bytes = heads * 2;
     const long long total = static_cast<long long>(n) * layers * bytes;
     for (long long i = static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x; i < total;
          i += static_cast<long long>(gridDim.x) * blockDim.x) {
         const int b = static_cast<int>(i % bytes), layer = static_cast<int>(i / bytes % layers);
         const int page = updates[3 * (i / bytes / layers) + 2];
-        exps[(static_cast<size_t>(layer) * pool_pages + page) * bytes + b] = kKv8MinExp;
+        exps[(static_cast<size_t>(layer) * pool_pages + page) * bytes + b] = kKv8MinExp + 127;
     }
 }
 
 // kv_fill_kernel's values in 8 bits: below 2.449 in magnitude, so every block
 // has the scale 2^-5.
-__global__ void kv8_fill_kernel(uint8_t* pool, int8_t* exps, int pool_pages, const int32_t* table, int n_layers, int length,
+__global__ void kv8_fill_kernel(uint8_t* pool, uint8_t* exps, int pool_pages, const int32_t* table, int n_layers, int length,
                                 uint64_t seed) {
     constexpr int kBlockBytes = kKv8Block * kHeadDim;
     const long long per_pos = static_cast<long long>(n_layers) * 2 * kWidth;
@@ -318,7 +318,7 @@ __global__ void kv8_fill_kernel(uint8_t* pool, int8_t* exps, int pool_pages, con
         const size_t block = (static_cast<size_t>(layer) * pool_pages + table[position / kPage]) * kHeads + (d >> 6);
         pool[(block * 2 + which) * kBlockBytes + kv8_byte<kHeadDim>(which, position % kPage, d & 63)] =
             static_cast<uint8_t>(kv8_code(v, 32.0f));
-        if ((d & 63) == 0 && position % kPage == 0) exps[block * 2 + which] = -5;
+        if ((d & 63) == 0 && position % kPage == 0) exps[block * 2 + which] = 127 - 5;
     }
 }
 
@@ -363,7 +363,7 @@ __global__ void __launch_bounds__(128) kv8_read_kernel(Kv8ReadParams p) {
     }
     const int lo = max(start - p0, 0), hi = min(q.length - p0, kKv8Block);
     const uint8_t* src = page >= 0 ? kv8_block<D>(p.cache, page, head, which) : nullptr;
-    const float unit = page >= 0 ? pow2i(kv8_exp(p.cache, page, head)[which]) : 0.0f;
+    const float unit = page >= 0 ? pow2i(kv8_exp(p.cache, page, head)[which] - 127) : 0.0f;
     void* dst = p.rows[which];
     auto value = [&](uint32_t w, int k) {
         return static_cast<float>(static_cast<int>((w >> (8 * k)) & 0xffu) - 128) * unit;
@@ -408,22 +408,27 @@ __global__ void __launch_bounds__(128) kv8_read_kernel(Kv8ReadParams p) {
 // r (at position p_r) sees: k <= p_r, and k > p_r - window where a window is
 // set. Rows that see nothing get 0.
 //
-// Per block the tensor cores compute S^T = K q^T (16 positions x 8 rows) and
-// O^T += V^T P^T (16 dims x 8 rows) with the cache's integers as the A
+// Per block the tensor cores compute S^T = K q^T (16 positions x 8 columns)
+// and O^T += V^T P^T (16 dims x 8 columns) with the cache's integers as the A
 // operand: byte | 0x6400 is the half 1024 + byte, minus 1152 the signed
 // integer, exactly, one PRMT and one HSUB2 for two elements. Rows are the N
 // operand: a decode step's single row (times the grouped heads) costs half
 // the instructions that it would as M. A block's scales enter in fp32: with s
 // = scale log2(e) 2^eK (q.K) + eV, the weight 2^(s - M) is the softmax weight
 // times the block's value scale, so that O needs no scaling of its own, and the
-// sum of weights takes 2^(s - M - eV). M is the running maximum of s. eV spans
-// [-48, 64], so weights that matter stay inside fp32's range.
+// sum of weights takes 2^(s - M - eV). M is the running maximum of s; eV is
+// taken relative to the first visible page's, so that s keeps its precision
+// whatever the values' size. eV spans 112 at most, so weights that matter stay
+// inside fp32's range.
 //
 // Rounding: the 8-bit integers and their products with a half are exact in
 // the fp32 accumulators. fp32 rows: q (scaled by a power of two to a row
-// maximum near 2^12) and the weights enter as two halves each, 22 bits. bf16
-// rows: q fits one half (8 bits), a weight is rounded to one half (11 bits,
-// under the output's 8).
+// maximum near 2^12) and the weights enter as two halves each, 22 bits. Up to
+// four rows are packed: columns 2r and 2r + 1 are the two halves of row r, one
+// product for both, summed by the lane that holds both (half the products and
+// half the softmax work a lane); more rows take two products each. bf16 rows:
+// q fits one half (8 bits), a weight is rounded to one half (11 bits, under
+// the output's 8).
 struct Kv8AttnParams {
     Kv8View cache;
     Kv8Seqs seqs;
@@ -439,8 +444,9 @@ struct Kv8AttnParams {
     unsigned* arrived;               // [items], zero between launches
 };
 
-constexpr int kKv8Warps = 4;
 constexpr float kKv8WeightBits = 14.0f;  // weights are held times 2^14: a half keeps 11 bits down to 2^-28
+
+enum Kv8Mode : int { KV8_BF16 = 0, KV8_F32 = 1, KV8_F32_PACKED = 2 };
 
 __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                          uint32_t b1) {
@@ -455,9 +461,10 @@ __device__ __forceinline__ uint32_t movmatrix_trans(uint32_t v) {
     return r;
 }
 
+// 2^x, results below 2^-126 are 0 (weights are at most 2^14).
 __device__ __forceinline__ float ex2(float x) {
     float r;
-    asm("ex2.approx.f32 %0, %1;" : "=f"(r) : "f"(x));
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
     return r;
 }
 
@@ -492,21 +499,26 @@ __device__ __forceinline__ uint2 ld_stream8(const uint8_t* p) {
 }
 
 // A lane's share of a block's keys: word [half][c] is dims 4c.. of the lane's
-// D/4 (the t-th 16 bytes of each 64, 8 of 32) of positions g, g + 8.
+// D/4 (the t-th 16 bytes of each 64, 8 of 32) of positions g, g + 8. `block`
+// is the block's address plus kv8_key_lane.
 template <int D>
-__device__ __forceinline__ void kv8_load_keys(uint32_t (&w)[2][D / 16], const uint8_t* block, int lane) {
-    const int g = lane >> 2, t = lane & 3;
+__device__ __forceinline__ int kv8_key_lane(int g, int t) {
+    return g * D + (D == 32 ? t * 8 : t * 16);
+}
+
+template <int D>
+__device__ __forceinline__ void kv8_load_keys(uint32_t (&w)[2][D / 16], const uint8_t* block) {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-        const uint8_t* row = block + (g + 8 * h) * D;
+        const uint8_t* row = block + 8 * h * D;
         if constexpr (D == 32) {
-            const uint2 v = ld_stream8(row + t * 8);
+            const uint2 v = ld_stream8(row);
             w[h][0] = v.x;
             w[h][1] = v.y;
         } else {
 #pragma unroll
             for (int c = 0; c < D / 64; ++c) {
-                const uint4 v = ld_stream16(row + c * 64 + t * 16);
+                const uint4 v = ld_stream16(row + c * 64);
                 w[h][4 * c] = v.x;
                 w[h][4 * c + 1] = v.y;
                 w[h][4 * c + 2] = v.z;
@@ -522,11 +534,12 @@ __device__ __forceinline__ int kv8_key_dim(int t, int c) {
     return D == 32 ? t * 8 + c * 4 : (c >> 2) * 64 + t * 16 + (c & 3) * 4;
 }
 
+// ... and of its values: `block` is the address of the values plus lane * 16.
 template <int D>
-__device__ __forceinline__ void kv8_load_values(uint32_t (&w)[D / 8], const uint8_t* block, int lane) {
+__device__ __forceinline__ void kv8_load_values(uint32_t (&w)[D / 8], const uint8_t* block) {
 #pragma unroll
     for (int j = 0; j < D / 32; ++j) {
-        const uint4 v = ld_stream16(block + j * 512 + lane * 16);
+        const uint4 v = ld_stream16(block + j * 512);
         w[4 * j] = v.x;
         w[4 * j + 1] = v.y;
         w[4 * j + 2] = v.z;
@@ -539,14 +552,18 @@ __device__ __forceinline__ void kv8_load_values(uint32_t (&w)[D / 8], const uint
 // and meet in shared memory; the last split to arrive merges them in order.
 // The next pages' keys are loaded when the current ones have been multiplied,
 // the next values after the current: a warp always has PB pages of either in
-// flight (2 to 8 KB), without shared memory.
-template <int D, int NT, int PB, bool kBf16>
-__global__ void __launch_bounds__(32 * kKv8Warps) kv8_attention_kernel(Kv8AttnParams p) {
-    constexpr int kRows = 8 * NT;
-    constexpr bool kFine = !kBf16;  // two halves for q and the weights
-    constexpr int KS = D / 16;      // 16-dim steps of a score, and 16-dim tiles of an output
-    __shared__ float s_o[kKv8Warps][kRows][D];
-    __shared__ float2 s_ml[kKv8Warps][kRows];
+// flight (2 to 8 KB), without shared memory. Page ids and scales are fetched a
+// lane each, 32 / PB turns at a time.
+template <int D, int NT, int PB, int kMode, int kWarps>
+__global__ void __launch_bounds__(32 * kWarps) kv8_attention_kernel(Kv8AttnParams p) {
+    constexpr bool kBf16 = kMode == KV8_BF16, kFine = kMode == KV8_F32, kPack = kMode == KV8_F32_PACKED;
+    static_assert(!kPack || NT == 1, "packed rows fill one column tile");
+    constexpr int kRows = kPack ? 4 : 8 * NT;
+    constexpr int RT = kPack ? 1 : 2;  // rows of a column tile that a lane holds scores of
+    constexpr int KS = D / 16;         // 16-dim steps of a score, and 16-dim tiles of an output
+    constexpr int kTurns = 32 / PB;
+    __shared__ float s_o[kWarps][kRows][D];
+    __shared__ float2 s_ml[kWarps][kRows];
     __shared__ int s_last;
     pdl_wait();
     pdl_trigger();
@@ -569,14 +586,73 @@ __global__ void __launch_bounds__(32 * kKv8Warps) kv8_attention_kernel(Kv8AttnPa
     if (split >= active) return;
     const int per = (pages + active - 1) / active;
     const int first = page_begin + min(pages, split * per), last = page_begin + min(pages, (split + 1) * per);
+    // pages that every row of the tile sees whole: [whole_first, whole_last)
+    const int whole_last = max(pos_lo + 1, 0) / kKv8Block;
+    const int whole_first = p.window && pos_hi >= p.window ? (pos_hi - p.window) / kKv8Block + 1 : 0;
 
-    // q as B fragments, scaled to a row maximum in [2^12, 2^13)
+    // this lane's page of the next kTurns turns: its id (-1: none) and scales
+    constexpr int kStep = kWarps * PB;
+    const int own = first + warp * PB + lane / PB * kStep + lane % PB;
+    const uint8_t* exps = p.cache.exps + head * 2;
+    int my_id, my_exps;
+    auto fetch = [&](int turn) {
+        const int at = own + turn * kStep;
+        my_id = at < last ? __ldg(sq.pages + at) : -1;
+        if (at < last && static_cast<unsigned>(my_id) >= static_cast<unsigned>(p.cache.pool_pages)) {
+            kv8_flag(p.seqs, i, kStatusInvalid);
+            my_id = -1;  // its positions are not seen
+        }
+        my_exps = my_id >= 0 ? __ldg(reinterpret_cast<const unsigned short*>(exps + static_cast<size_t>(my_id) * p.cache.heads * 2))
+                             : 127 | 127 << 8;
+    };
+    uint32_t kw[PB][2][D / 16], vw[PB][D / 8];
+    int id[PB], next[PB], ex[PB], next_ex[PB];
+    const size_t page_bytes = static_cast<size_t>(p.cache.heads) * (2 * kKv8Block * D);
+    const uint8_t* key_base = p.cache.pool + static_cast<size_t>(head) * (2 * kKv8Block * D) + kv8_key_lane<D>(g, t);
+    const uint8_t* value_base = p.cache.pool + static_cast<size_t>(head) * (2 * kKv8Block * D) + kKv8Block * D + lane * 16;
+    auto take = [&](int turn) {
+        if (turn % kTurns == 0) fetch(turn);
+#pragma unroll
+        for (int b = 0; b < PB; ++b) {
+            next[b] = __shfl_sync(kFull, my_id, turn % kTurns * PB + b);
+            next_ex[b] = __shfl_sync(kFull, my_exps, turn % kTurns * PB + b);
+        }
+    };
+    auto load_keys = [&]() {
+#pragma unroll
+        for (int b = 0; b < PB; ++b)
+            if (next[b] >= 0) kv8_load_keys<D>(kw[b], key_base + next[b] * page_bytes);
+    };
+    auto load_values = [&]() {
+#pragma unroll
+        for (int b = 0; b < PB; ++b)
+            if (next[b] >= 0) kv8_load_values<D>(vw[b], value_base + next[b] * page_bytes);
+    };
+#pragma unroll
+    for (int b = 0; b < PB; ++b) {
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k) kw[b][0][k] = kw[b][1][k] = 0x80808080u;
+#pragma unroll
+        for (int k = 0; k < D / 8; ++k) vw[b][k] = 0x80808080u;
+    }
+    take(0);
+    load_keys();
+    load_values();
+    int ref = 127;  // the value scale that eV is relative to, the same for all warps and splits
+    if (pages > 0) {
+        const int id0 = __ldg(sq.pages + page_begin);
+        if (static_cast<unsigned>(id0) < static_cast<unsigned>(p.cache.pool_pages))
+            ref = __ldg(exps + static_cast<size_t>(id0) * p.cache.heads * 2 + 1);
+    }
+
+    // q as B fragments, scaled to a row maximum in [2^12, 2^13); column g is
+    // row g, or one half of row g / 2
     uint32_t qh[NT][KS][2], ql[NT][kFine ? KS : 1][2];
-    float f0[NT], f1[NT];  // scale * 2^(row exponent) of rows 2t, 2t + 1
-    int pos0[NT], pos1[NT];
+    float f[NT][RT];  // scale * 2^(row exponent) of the lane's rows
+    int pos[NT][RT];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-        const int r = n * 8 + g, rho = rho0 + min(r, n_rows - 1);
+        const int r = kPack ? g >> 1 : n * 8 + g, rho = rho0 + min(r, n_rows - 1);
         const size_t row = static_cast<size_t>(sq.row0 + rho / p.group) * p.q_stride +
                            static_cast<size_t>(head * p.group + rho % p.group) * D;
         float4 v[KS];
@@ -594,157 +670,141 @@ __global__ void __launch_bounds__(32 * kKv8Warps) kv8_attention_kernel(Kv8AttnPa
         const bool row_bad = (bad >> (lane & ~3) & 0xfu) != 0;
         if (row_bad && t == 0 && r < n_rows) kv8_flag(p.seqs, i, kStatusNonFinite);
         // exponent of the maximum, kept where both powers below are normal
-        const int ex = min(max(static_cast<int>(__float_as_uint(amax) >> 23) - 127, -110), 126);
-        const float up = pow2i(min(12 - ex, 122)), back = pow2i(ex - 12);
+        const int e = min(max(static_cast<int>(__float_as_uint(amax) >> 23) - 127, -110), 126);
+        const float up = pow2i(12 - e), back = pow2i(e - 12);
 #pragma unroll
         for (int c = 0; c < KS; ++c) {
-            const float a = v[c].x * up, b = v[c].y * up, cc = v[c].z * up, d = v[c].w * up;
-            qh[n][c][0] = half2_bits(a, b);
-            qh[n][c][1] = half2_bits(cc, d);
-            if constexpr (kFine) {
+            const float x[4] = {v[c].x * up, v[c].y * up, v[c].z * up, v[c].w * up};
+            qh[n][c][0] = half2_bits(x[0], x[1]);
+            qh[n][c][1] = half2_bits(x[2], x[3]);
+            if constexpr (!kBf16) {
                 const float2 h0 = half2_floats(qh[n][c][0]), h1 = half2_floats(qh[n][c][1]);
-                ql[n][c][0] = half2_bits(a - h0.x, b - h0.y);
-                ql[n][c][1] = half2_bits(cc - h1.x, d - h1.y);
+                const uint32_t l0 = half2_bits(x[0] - h0.x, x[1] - h0.y), l1 = half2_bits(x[2] - h1.x, x[3] - h1.y);
+                if constexpr (kFine) {
+                    ql[n][c][0] = l0;
+                    ql[n][c][1] = l1;
+                } else if (g & 1) {
+                    qh[n][c][0] = l0;
+                    qh[n][c][1] = l1;
+                }
             }
         }
-        const float f = row_bad ? __int_as_float(0x7fc00000) : p.scale * back;  // a bad row's output is NaN
-        f0[n] = __shfl_sync(kFull, f, 8 * t);
-        f1[n] = __shfl_sync(kFull, f, 8 * t + 4);
-        pos0[n] = at0 + (rho0 + min(n * 8 + 2 * t, n_rows - 1)) / p.group;
-        pos1[n] = at0 + (rho0 + min(n * 8 + 2 * t + 1, n_rows - 1)) / p.group;
+        const float fr = row_bad ? __int_as_float(0x7fc00000) : p.scale * back;  // a bad row's output is NaN
+#pragma unroll
+        for (int k = 0; k < RT; ++k) {
+            f[n][k] = __shfl_sync(kFull, fr, 8 * t + 4 * k);
+            const int lane_row = kPack ? t : n * 8 + 2 * t + k;
+            pos[n][k] = at0 + (rho0 + min(lane_row, n_rows - 1)) / p.group;
+        }
     }
 
-    float o[KS][NT][4];
-    float m0[NT], m1[NT], l0[NT], l1[NT];
+    float o[KS][NT][4], m[NT][RT], l[NT][RT];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-        m0[n] = m1[n] = -INFINITY;
-        l0[n] = l1[n] = 0.0f;
+#pragma unroll
+        for (int k = 0; k < RT; ++k) {
+            m[n][k] = -INFINITY;
+            l[n][k] = 0.0f;
+        }
 #pragma unroll
         for (int k = 0; k < KS; ++k) o[k][n][0] = o[k][n][1] = o[k][n][2] = o[k][n][3] = 0.0f;
     }
 
-    uint32_t kw[PB][2][D / 16], vw[PB][D / 8];
-    int page[PB];   // page ids of the batch whose keys are in kw; -1: none
-    int ek[PB], ev[PB];
-    auto load_ids = [&](int from, int (&id)[PB]) {
+    int turn = 0;
+    for (int at = first + warp * PB; at < last; at += kStep) {
 #pragma unroll
         for (int b = 0; b < PB; ++b) {
-            id[b] = from + b < last ? __ldg(sq.pages + from + b) : -1;
-            if (from + b < last && static_cast<unsigned>(id[b]) >= static_cast<unsigned>(p.cache.pool_pages)) {
-                if (lane == 0) kv8_flag(p.seqs, i, kStatusInvalid);
-                id[b] = -1;  // its keys are not seen
-            }
+            id[b] = next[b];
+            ex[b] = next_ex[b];
         }
-    };
-    auto load_keys = [&](const int (&id)[PB]) {
+        take(++turn);
+        float s[PB][NT][2][RT];  // positions g, g + 8
+        float less[PB];          // 2^-eV
 #pragma unroll
         for (int b = 0; b < PB; ++b) {
-            const int pg = max(id[b], 0);
-            if (id[b] >= 0) kv8_load_keys<D>(kw[b], kv8_block<D>(p.cache, pg, head, 0), lane);
-            const short e2 = __ldg(reinterpret_cast<const short*>(kv8_exp(p.cache, pg, head)));
-            ek[b] = static_cast<int8_t>(e2 & 0xff);
-            ev[b] = e2 >> 8;
-        }
-    };
-    auto load_values = [&](const int (&id)[PB]) {
+            float c4[NT][4];
 #pragma unroll
-        for (int b = 0; b < PB; ++b)
-            if (id[b] >= 0) kv8_load_values<D>(vw[b], kv8_block<D>(p.cache, id[b], head, 1), lane);
-    };
-#pragma unroll
-    for (int b = 0; b < PB; ++b) {
-#pragma unroll
-        for (int k = 0; k < D / 16; ++k) kw[b][0][k] = kw[b][1][k] = 0x80808080u;
-#pragma unroll
-        for (int k = 0; k < D / 8; ++k) vw[b][k] = 0x80808080u;
-    }
-    const int step = kKv8Warps * PB;
-    int at = first + warp * PB;
-    load_ids(at, page);
-    load_keys(page);
-    load_values(page);
-    for (; at < last; at += step) {
-        int next[PB];
-        load_ids(at + step, next);
-        float s[PB][NT][4];
-        float add[PB], less[PB];  // eV, 2^-eV
-#pragma unroll
-        for (int b = 0; b < PB; ++b) {
-#pragma unroll
-            for (int n = 0; n < NT; ++n) s[b][n][0] = s[b][n][1] = s[b][n][2] = s[b][n][3] = 0.0f;
+            for (int n = 0; n < NT; ++n) c4[n][0] = c4[n][1] = c4[n][2] = c4[n][3] = 0.0f;
 #pragma unroll
             for (int c = 0; c < KS; ++c) {
                 const uint32_t a0 = kv8_halves<false>(kw[b][0][c]), a1 = kv8_halves<false>(kw[b][1][c]);
                 const uint32_t a2 = kv8_halves<true>(kw[b][0][c]), a3 = kv8_halves<true>(kw[b][1][c]);
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
-                    mma16816(s[b][n], a0, a1, a2, a3, qh[n][c][0], qh[n][c][1]);
-                    if constexpr (kFine) mma16816(s[b][n], a0, a1, a2, a3, ql[n][c][0], ql[n][c][1]);
+                    mma16816(c4[n], a0, a1, a2, a3, qh[n][c][0], qh[n][c][1]);
+                    if constexpr (kFine) mma16816(c4[n], a0, a1, a2, a3, ql[n][c][0], ql[n][c][1]);
                 }
             }
-            const float uk = pow2i(ek[b]);
-            add[b] = static_cast<float>(ev[b]);
-            less[b] = pow2i(-ev[b]);
-            const int key = (at + b) * kKv8Block + g;
-            // every row of the tile sees the whole page
-            const bool whole = page[b] >= 0 && (at + b + 1) * kKv8Block <= pos_lo + 1 &&
-                               (!p.window || (at + b) * kKv8Block > pos_hi - p.window);
+            const float uk = __int_as_float((ex[b] & 0xff) << 23);
+            const int ev = (ex[b] >> 8) - ref;
+            const float add = static_cast<float>(ev);
+            less[b] = pow2i(-ev);
 #pragma unroll
-            for (int n = 0; n < NT; ++n) {
-                const float u0 = f0[n] * uk, u1 = f1[n] * uk;
-                s[b][n][0] = fmaf(s[b][n][0], u0, add[b]);
-                s[b][n][1] = fmaf(s[b][n][1], u1, add[b]);
-                s[b][n][2] = fmaf(s[b][n][2], u0, add[b]);
-                s[b][n][3] = fmaf(s[b][n][3], u1, add[b]);
-                if (!whole) {
-                    const int w0 = p.window ? pos0[n] - p.window : -1, w1 = p.window ? pos1[n] - p.window : -1;
-                    if (page[b] < 0 || key > pos0[n] || key <= w0) s[b][n][0] = -INFINITY;
-                    if (page[b] < 0 || key > pos1[n] || key <= w1) s[b][n][1] = -INFINITY;
-                    if (page[b] < 0 || key + 8 > pos0[n] || key + 8 <= w0) s[b][n][2] = -INFINITY;
-                    if (page[b] < 0 || key + 8 > pos1[n] || key + 8 <= w1) s[b][n][3] = -INFINITY;
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int k = 0; k < RT; ++k) {
+                    const float u = f[n][k] * uk;
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+                        s[b][n][h][k] = fmaf(kPack ? c4[n][2 * h] + c4[n][2 * h + 1] : c4[n][2 * h + k], u, add);
                 }
+            const int page = at + b;
+            if (id[b] < 0 || page < whole_first || page >= whole_last) {
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int k = 0; k < RT; ++k) {
+                        const int low = p.window ? pos[n][k] - p.window : -1;
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            const int key = page * kKv8Block + g + 8 * h;
+                            if (id[b] < 0 || key > pos[n][k] || key <= low) s[b][n][h][k] = -INFINITY;
+                        }
+                    }
             }
         }
-        load_keys(next);
+        load_keys();
         uint32_t ph[PB][NT][2], pl[PB][kFine ? NT : 1][2];
         bool moved = false;
-        float c0[NT], c1[NT];
+        float c[NT][RT];
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-            float x0 = m0[n], x1 = m1[n];
+            float base[RT];
 #pragma unroll
-            for (int b = 0; b < PB; ++b) {
-                x0 = fmaxf(x0, fmaxf(s[b][n][0], s[b][n][2]));
-                x1 = fmaxf(x1, fmaxf(s[b][n][1], s[b][n][3]));
+            for (int k = 0; k < RT; ++k) {
+                float x = m[n][k];
+#pragma unroll
+                for (int b = 0; b < PB; ++b) x = fmaxf(x, fmaxf(s[b][n][0][k], s[b][n][1][k]));
+#pragma unroll
+                for (int w = 4; w < 32; w <<= 1) x = fmaxf(x, __shfl_xor_sync(kFull, x, w));
+                c[n][k] = m[n][k] == x ? 1.0f : ex2(m[n][k] - x);
+                moved |= m[n][k] != x;
+                m[n][k] = x;
+                base[k] = x == -INFINITY ? 0.0f : x - kKv8WeightBits;  // nothing seen yet: weights 2^(-inf - 0)
+                l[n][k] *= c[n][k];
             }
 #pragma unroll
-            for (int w = 4; w < 32; w <<= 1) {
-                x0 = fmaxf(x0, __shfl_xor_sync(kFull, x0, w));
-                x1 = fmaxf(x1, __shfl_xor_sync(kFull, x1, w));
-            }
-            c0[n] = m0[n] == x0 ? 1.0f : ex2(m0[n] - x0);
-            c1[n] = m1[n] == x1 ? 1.0f : ex2(m1[n] - x1);
-            moved |= m0[n] != x0 || m1[n] != x1;
-            m0[n] = x0;
-            m1[n] = x1;
-            // rows that have seen nothing yet keep weight 0: -inf - 0
-            const float b0 = x0 == -INFINITY ? 0.0f : x0 - kKv8WeightBits, b1 = x1 == -INFINITY ? 0.0f : x1 - kKv8WeightBits;
-            l0[n] *= c0[n];
-            l1[n] *= c1[n];
-#pragma unroll
             for (int b = 0; b < PB; ++b) {
-                const float p0 = ex2(s[b][n][0] - b0), p1 = ex2(s[b][n][1] - b1);
-                const float p2 = ex2(s[b][n][2] - b0), p3 = ex2(s[b][n][3] - b1);
-                l0[n] = fmaf(p0 + p2, less[b], l0[n]);
-                l1[n] = fmaf(p1 + p3, less[b], l1[n]);
-                const uint32_t h0 = half2_bits(p0, p1), h1 = half2_bits(p2, p3);
-                ph[b][n][0] = movmatrix_trans(h0);
-                ph[b][n][1] = movmatrix_trans(h1);
-                if constexpr (kFine) {
-                    const float2 r0 = half2_floats(h0), r1 = half2_floats(h1);
-                    pl[b][n][0] = movmatrix_trans(half2_bits(p0 - r0.x, p1 - r0.y));
-                    pl[b][n][1] = movmatrix_trans(half2_bits(p2 - r1.x, p3 - r1.y));
+                float w[2][RT];
+#pragma unroll
+                for (int k = 0; k < RT; ++k) {
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) w[h][k] = ex2(s[b][n][h][k] - base[k]);
+                    l[n][k] = fmaf(w[0][k] + w[1][k], less[b], l[n][k]);
+                }
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    if constexpr (kPack) {
+                        const float high = __half2float(__float2half_rn(w[h][0]));
+                        ph[b][n][h] = movmatrix_trans(half2_bits(w[h][0], w[h][0] - high));
+                    } else {
+                        const uint32_t high = half2_bits(w[h][0], w[h][RT - 1]);
+                        ph[b][n][h] = movmatrix_trans(high);
+                        if constexpr (kFine) {
+                            const float2 r = half2_floats(high);
+                            pl[b][n][h] = movmatrix_trans(half2_bits(w[h][0] - r.x, w[h][RT - 1] - r.y));
+                        }
+                    }
                 }
             }
         }
@@ -752,12 +812,9 @@ __global__ void __launch_bounds__(32 * kKv8Warps) kv8_attention_kernel(Kv8AttnPa
 #pragma unroll
             for (int k = 0; k < KS; ++k)
 #pragma unroll
-                for (int n = 0; n < NT; ++n) {
-                    o[k][n][0] *= c0[n];
-                    o[k][n][1] *= c1[n];
-                    o[k][n][2] *= c0[n];
-                    o[k][n][3] *= c1[n];
-                }
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) o[k][n][j] *= c[n][kPack ? 0 : j & 1];
         }
 #pragma unroll
         for (int b = 0; b < PB; ++b)
@@ -772,38 +829,33 @@ __global__ void __launch_bounds__(32 * kKv8Warps) kv8_attention_kernel(Kv8AttnPa
                     if constexpr (kFine) mma16816(o[k][n], a0, a1, a2, a3, pl[b][n][0], pl[b][n][1]);
                 }
             }
-        load_values(next);
-#pragma unroll
-        for (int b = 0; b < PB; ++b) page[b] = next[b];
+        load_values();
     }
 
     // the warps' shares meet
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
+    for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int w = 4; w < 32; w <<= 1) {
-            l0[n] += __shfl_xor_sync(kFull, l0[n], w);
-            l1[n] += __shfl_xor_sync(kFull, l1[n], w);
-        }
-        const int r = n * 8 + 2 * t;
-        if (g == 0) {
-            s_ml[warp][r] = make_float2(m0[n], l0[n]);
-            s_ml[warp][r + 1] = make_float2(m1[n], l1[n]);
-        }
+        for (int k = 0; k < RT; ++k) {
 #pragma unroll
-        for (int j = 0; j < D / 32; ++j) {
-            if (r < n_rows)
+            for (int w = 4; w < 32; w <<= 1) l[n][k] += __shfl_xor_sync(kFull, l[n][k], w);
+            const int r = kPack ? t : n * 8 + 2 * t + k;
+            if (g == 0) s_ml[warp][r] = make_float2(m[n][k], l[n][k]);
+            if (r >= n_rows) continue;
+#pragma unroll
+            for (int j = 0; j < D / 32; ++j) {
+                const float* x = o[2 * j][n];
+                const float* y = o[2 * j + 1][n];
                 *reinterpret_cast<float4*>(&s_o[warp][r][32 * j + 4 * g]) =
-                    make_float4(o[2 * j][n][0], o[2 * j][n][2], o[2 * j + 1][n][0], o[2 * j + 1][n][2]);
-            if (r + 1 < n_rows)
-                *reinterpret_cast<float4*>(&s_o[warp][r + 1][32 * j + 4 * g]) =
-                    make_float4(o[2 * j][n][1], o[2 * j][n][3], o[2 * j + 1][n][1], o[2 * j + 1][n][3]);
+                    kPack ? make_float4(x[0] + x[1], x[2] + x[3], y[0] + y[1], y[2] + y[3])
+                          : make_float4(x[k], x[2 + k], y[k], y[2 + k]);
+            }
         }
-    }
     __syncthreads();
     constexpr int kQuads = D / 4;
+    const float unit = pow2i(ref - 127);
     auto finish = [&](int r, int d, float total, float4 a) {
-        const float inv = total > 0.0f || isnan(total) ? __fdiv_rn(1.0f, total) : 0.0f;
+        const float inv = total > 0.0f || isnan(total) ? __fdiv_rn(unit, total) : 0.0f;
         const int rho = rho0 + r;
         store_row4<kBf16>(p.out,
                           static_cast<size_t>(sq.row0 + rho / p.group) * p.out_stride +
@@ -820,17 +872,17 @@ __global__ void __launch_bounds__(32 * kKv8Warps) kv8_attention_kernel(Kv8AttnPa
     const size_t slot = static_cast<size_t>(item) * p.splits;
     for (int x = threadIdx.x; x < n_rows * kQuads; x += blockDim.x) {
         const int r = x / kQuads, d = x % kQuads * 4;
-        float m = -INFINITY, l = 0.0f;
+        float mm = -INFINITY, ll = 0.0f;
         float4 a = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
-        for (int w = 0; w < kKv8Warps; ++w)
-            fold(m, l, a, s_ml[w][r].x, s_ml[w][r].y, *reinterpret_cast<const float4*>(&s_o[w][r][d]));
+        for (int w = 0; w < kWarps; ++w)
+            fold(mm, ll, a, s_ml[w][r].x, s_ml[w][r].y, *reinterpret_cast<const float4*>(&s_o[w][r][d]));
         if (active == 1) {
-            finish(r, d, l, a);
+            finish(r, d, ll, a);
         } else {
             const size_t at_part = (slot + split) * kRows + r;
             *reinterpret_cast<float4*>(p.part + at_part * D + d) = a;
-            if (d == 0) p.part_ml[at_part] = make_float2(m, l);
+            if (d == 0) p.part_ml[at_part] = make_float2(mm, ll);
         }
     }
     if (active == 1) return;
@@ -846,14 +898,15 @@ __global__ void __launch_bounds__(32 * kKv8Warps) kv8_attention_kernel(Kv8AttnPa
     __threadfence();
     for (int x = threadIdx.x; x < n_rows * kQuads; x += blockDim.x) {
         const int r = x / kQuads, d = x % kQuads * 4;
-        float m = -INFINITY, l = 0.0f;
+        float mm = -INFINITY, ll = 0.0f;
         float4 a = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
         for (int k = 0; k < active; ++k) {
             const size_t at_part = (slot + k) * kRows + r;
             const float2 ml = __ldcg(p.part_ml + at_part);
-            fold(m, l, a, ml.x, ml.y, __ldcg(reinterpret_cast<const float4*>(p.part + at_part * D + d)));
+            fold(mm, ll, a, ml.x, ml.y, __ldcg(reinterpret_cast<const float4*>(p.part + at_part * D + d)));
         }
-        finish(r, d, l, a);
+        finish(r, d, ll, a);
     }
 }
 
