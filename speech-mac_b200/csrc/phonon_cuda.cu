@@ -541,7 +541,14 @@ struct Kv8Attend {
     bool bf16;
 };
 
-template <int D, int NT, int PB, int kMode, int kWarps>
+Kv8Div kv8_divisor(uint32_t d) {
+    uint32_t log = 0;
+    while ((1ull << log) < d) ++log;
+    // ceil(2^(31 + log) / d) < 2^32, exact for n < 2^31
+    return Kv8Div{d, d == 1 ? 0 : static_cast<uint32_t>(((1ull << (31 + log)) + d - 1) / d), log ? log - 1 : 0};
+}
+
+template <int D, int NT, int PB, int kStages, int kMode, int kWarps, int kCtas>
 int kv8_launch_attention(const Kv8Pool& c, uint32_t layer, const Kv8Seqs& seqs, const Kv8Attend& a,
                          const Kv8Scratch& w, int sms, cudaStream_t s) {
     constexpr int kRows = kMode == KV8_F32_PACKED ? 4 : 8 * NT;
@@ -557,8 +564,8 @@ int kv8_launch_attention(const Kv8Pool& c, uint32_t layer, const Kv8Seqs& seqs, 
     p.scale = a.scale * 1.44269504088896340736f;
     p.window = a.window;
     const long long rows = static_cast<long long>(seqs.max_rows) * a.group;
-    p.tiles = static_cast<int>((rows + kRows - 1) / kRows);
-    const long long items = static_cast<long long>(seqs.n) * p.tiles * c.heads;
+    const long long tiles = (rows + kRows - 1) / kRows;
+    const long long items = seqs.n * tiles * c.heads;
     // pages that a row tile can see
     long long span = seqs.max_length;
     if (a.window) span = std::min<long long>(span, static_cast<long long>(a.window) + (kRows - 1) / a.group + kKv8Block);
@@ -568,13 +575,20 @@ int kv8_launch_attention(const Kv8Pool& c, uint32_t layer, const Kv8Seqs& seqs, 
     splits = std::max<long long>(1, std::min(splits, (pages + kKv8MinPages - 1) / kKv8MinPages));
     if (items * splits > INT32_MAX) return PHONON_CUDA_CAPACITY;
     if (splits > 1 && items * splits > w.max_splits) return PHONON_CUDA_CAPACITY;
-    p.splits = static_cast<int>(splits);
+    p.by_heads = kv8_divisor(c.heads);
+    p.by_splits = kv8_divisor(static_cast<uint32_t>(splits));
+    p.by_tiles = kv8_divisor(static_cast<uint32_t>(tiles));
     p.split_pages = static_cast<int>((pages + splits - 1) / splits);
     p.part = w.part;
     p.part_ml = w.ml;
     p.arrived = w.arrived;
-    CUDA_TRY(launch_pdl(kv8_attention_kernel<D, NT, PB, kMode, kWarps>, dim3(static_cast<unsigned>(items * splits)),
-                        dim3(32 * kWarps), 0, s, p));
+    constexpr int smem = kWarps * std::max(kStages * PB * 2 * kKv8Block * D, kRows * D * 4);
+    auto kernel = kv8_attention_kernel<D, NT, PB, kStages, kMode, kWarps, kCtas>;
+    if constexpr (smem > 46 * 1024) {  // 48 KB with the kernel's static arrays
+        static std::atomic<uint64_t> configured{0};
+        CUDA_TRY(opt_in_smem(reinterpret_cast<const void*>(kernel), smem, configured));
+    }
+    CUDA_TRY(launch_pdl(kernel, dim3(static_cast<unsigned>(items * splits)), dim3(32 * kWarps), smem, s, p));
     return PHONON_CUDA_OK;
 }
 
@@ -584,17 +598,16 @@ template <int D>
 int kv8_attention_rows(const Kv8Pool& c, uint32_t layer, const Kv8Seqs& seqs, const Kv8Attend& a, const Kv8Scratch& w,
                        int sms, cudaStream_t s) {
     const long long rows = static_cast<long long>(seqs.max_rows) * a.group;
-    constexpr int PB = D == 128 ? 2 : 4, W = 4;
+    constexpr int PB = D == 128 ? 1 : 2;
     if (a.bf16) {
-        if (rows <= 8) return kv8_launch_attention<D, 1, PB, KV8_BF16, W>(c, layer, seqs, a, w, sms, s);
-        if (rows <= 16 || D == 128)
-            return kv8_launch_attention<D, 2, PB / 2, KV8_BF16, W>(c, layer, seqs, a, w, sms, s);
-        if constexpr (D < 128) return kv8_launch_attention<D, 4, PB / 4, KV8_BF16, W>(c, layer, seqs, a, w, sms, s);
+        if (rows <= 8) return kv8_launch_attention<D, 1, PB, 3, KV8_BF16, 4, 4>(c, layer, seqs, a, w, sms, s);
+        if (rows <= 16 || D == 128) return kv8_launch_attention<D, 2, 1, 3, KV8_BF16, 4, 4>(c, layer, seqs, a, w, sms, s);
+        if constexpr (D < 128) return kv8_launch_attention<D, 4, 1, 3, KV8_BF16, 4, 2>(c, layer, seqs, a, w, sms, s);
     }
-    if (rows <= 4) return kv8_launch_attention<D, 1, PB, KV8_F32_PACKED, W>(c, layer, seqs, a, w, sms, s);
-    if (rows <= 8) return kv8_launch_attention<D, 1, PB, KV8_F32, W>(c, layer, seqs, a, w, sms, s);
-    if (rows <= 16 || D == 128) return kv8_launch_attention<D, 2, PB / 2, KV8_F32, W>(c, layer, seqs, a, w, sms, s);
-    if constexpr (D < 128) return kv8_launch_attention<D, 4, PB / 4, KV8_F32, W>(c, layer, seqs, a, w, sms, s);
+    if (rows <= 4) return kv8_launch_attention<D, 1, PB, 3, KV8_F32_PACKED, 4, 4>(c, layer, seqs, a, w, sms, s);
+    if (rows <= 8) return kv8_launch_attention<D, 1, PB, 3, KV8_F32, 4, 4>(c, layer, seqs, a, w, sms, s);
+    if (rows <= 16 || D == 128) return kv8_launch_attention<D, 2, 1, 3, KV8_F32, 4, 3>(c, layer, seqs, a, w, sms, s);
+    if constexpr (D < 128) return kv8_launch_attention<D, 4, 1, 3, KV8_F32, 4, 2>(c, layer, seqs, a, w, sms, s);
     return PHONON_CUDA_INVALID_ARGUMENT;
 }
 

@@ -403,6 +403,15 @@ __global__ void __launch_bounds__(128) kv8_read_kernel(Kv8ReadParams p) {
     }
 }
 
+// n / d and n % d of a launch's block index for a d that the host knows:
+// multiply and shift (Granlund and Montgomery's division by invariants, for
+// n < 2^31, where the multiplier fits 32 bits).
+struct Kv8Div {
+    uint32_t d, mul, shift;
+};
+
+__device__ __forceinline__ uint32_t kv8_div(uint32_t n, Kv8Div d) { return d.d == 1 ? n : __umulhi(n, d.mul) >> d.shift; }
+
 // ---------------------------------------------------------------- attention
 // out[r] = sum_k softmax_k(scale q_r . K_k) V_k over the positions k that row
 // r (at position p_r) sees: k <= p_r, and k > p_r - window where a window is
@@ -438,7 +447,8 @@ struct Kv8AttnParams {
     int group;                       // query heads per K/V head
     float scale;                     // softmax scale times log2(e)
     int window;                      // 0: none
-    int tiles, splits, split_pages;  // row tiles of a sequence, splits and their pages, at most
+    Kv8Div by_heads, by_splits, by_tiles;  // K/V heads; splits of an item, at most; row tiles of a sequence
+    int split_pages;                       // pages of a split
     float* part;                     // [items * splits][rows of a tile][D]
     float2* part_ml;                 // [items * splits][rows of a tile]: M, sum
     unsigned* arrived;               // [items], zero between launches
@@ -484,41 +494,49 @@ __device__ __forceinline__ uint32_t half2_bits(float a, float b) {
 
 __device__ __forceinline__ float2 half2_floats(uint32_t u) { return __half22float2(*reinterpret_cast<__half2*>(&u)); }
 
-__device__ __forceinline__ uint4 ld_stream16(const uint8_t* p) {
-    uint4 v;
-    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
-                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-                 : "l"(p));
-    return v;
+// A lane's share of a block: its keys are D/4 dims of positions g, g + 8 (the
+// t-th 16 bytes of each 64; 8 of 32 where D is 32), its values D/32 chunks of
+// 16 bytes. The lane copies them into its warp's ring in shared memory and
+// reads them back itself, so no other thread is waited for: 16 bytes of lane
+// 0, of lane 1, ... per chunk, without bank conflicts.
+__device__ __forceinline__ void copy16(uint32_t dst, const uint8_t* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
 
-__device__ __forceinline__ uint2 ld_stream8(const uint8_t* p) {
-    uint2 v;
-    asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
-    return v;
-}
-
-// A lane's share of a block's keys: word [half][c] is dims 4c.. of the lane's
-// D/4 (the t-th 16 bytes of each 64, 8 of 32) of positions g, g + 8. `block`
-// is the block's address plus kv8_key_lane.
-template <int D>
-__device__ __forceinline__ int kv8_key_lane(int g, int t) {
-    return g * D + (D == 32 ? t * 8 : t * 16);
+__device__ __forceinline__ void copy8(uint32_t dst, const uint8_t* src) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst), "l"(src) : "memory");
 }
 
 template <int D>
-__device__ __forceinline__ void kv8_load_keys(uint32_t (&w)[2][D / 16], const uint8_t* block) {
+__device__ __forceinline__ void kv8_copy(uint32_t dst, const uint8_t* block, int lane) {
+    const int g = lane >> 2, t = lane & 3;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-        const uint8_t* row = block + 8 * h * D;
         if constexpr (D == 32) {
-            const uint2 v = ld_stream8(row);
+            copy8(dst + h * 256 + lane * 8, block + (g + 8 * h) * D + t * 8);
+        } else {
+#pragma unroll
+            for (int c = 0; c < D / 64; ++c)
+                copy16(dst + (h * (D / 64) + c) * 512 + lane * 16, block + (g + 8 * h) * D + c * 64 + t * 16);
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < D / 32; ++j) copy16(dst + kKv8Block * D + j * 512 + lane * 16, block + kKv8Block * D + j * 512 + lane * 16);
+}
+
+// Key words [position g, g + 8][4 dims each], value words [2 x 16-dim tiles].
+template <int D>
+__device__ __forceinline__ void kv8_key_words(uint32_t (&w)[2][D / 16], const uint8_t* page, int lane) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        if constexpr (D == 32) {
+            const uint2 v = *reinterpret_cast<const uint2*>(page + h * 256 + lane * 8);
             w[h][0] = v.x;
             w[h][1] = v.y;
         } else {
 #pragma unroll
             for (int c = 0; c < D / 64; ++c) {
-                const uint4 v = ld_stream16(row + c * 64);
+                const uint4 v = *reinterpret_cast<const uint4*>(page + (h * (D / 64) + c) * 512 + lane * 16);
                 w[h][4 * c] = v.x;
                 w[h][4 * c + 1] = v.y;
                 w[h][4 * c + 2] = v.z;
@@ -528,51 +546,41 @@ __device__ __forceinline__ void kv8_load_keys(uint32_t (&w)[2][D / 16], const ui
     }
 }
 
-// The first dim of word c above.
+// The first dim of key word c.
 template <int D>
 __device__ __forceinline__ int kv8_key_dim(int t, int c) {
     return D == 32 ? t * 8 + c * 4 : (c >> 2) * 64 + t * 16 + (c & 3) * 4;
 }
 
-// ... and of its values: `block` is the address of the values plus lane * 16.
-template <int D>
-__device__ __forceinline__ void kv8_load_values(uint32_t (&w)[D / 8], const uint8_t* block) {
-#pragma unroll
-    for (int j = 0; j < D / 32; ++j) {
-        const uint4 v = ld_stream16(block + j * 512);
-        w[4 * j] = v.x;
-        w[4 * j + 1] = v.y;
-        w[4 * j + 2] = v.z;
-        w[4 * j + 3] = v.w;
-    }
-}
-
 // One CTA: one (sequence, row tile, K/V head, split). Its warps take the
 // split's pages PB at a time in turn, each with an online softmax of its own,
 // and meet in shared memory; the last split to arrive merges them in order.
-// The next pages' keys are loaded when the current ones have been multiplied,
-// the next values after the current: a warp always has PB pages of either in
-// flight (2 to 8 KB), without shared memory. Page ids and scales are fetched a
-// lane each, 32 / PB turns at a time.
-template <int D, int NT, int PB, int kMode, int kWarps>
-__global__ void __launch_bounds__(32 * kWarps) kv8_attention_kernel(Kv8AttnParams p) {
+// Pages come by asynchronous copies, kStages - 1 turns ahead, in a ring that a
+// warp has to itself: the copies, not registers, hold what is in flight, which
+// leaves room for 16 to 20 warps an SM. Page ids and scales are fetched a lane
+// each, 32 / PB turns at a time.
+template <int D, int NT, int PB, int kStages, int kMode, int kWarps, int kCtas>
+__global__ void __launch_bounds__(32 * kWarps, kCtas) kv8_attention_kernel(Kv8AttnParams p) {
     constexpr bool kBf16 = kMode == KV8_BF16, kFine = kMode == KV8_F32, kPack = kMode == KV8_F32_PACKED;
     static_assert(!kPack || NT == 1, "packed rows fill one column tile");
     constexpr int kRows = kPack ? 4 : 8 * NT;
     constexpr int RT = kPack ? 1 : 2;  // rows of a column tile that a lane holds scores of
     constexpr int KS = D / 16;         // 16-dim steps of a score, and 16-dim tiles of an output
-    constexpr int kTurns = 32 / PB;
-    __shared__ float s_o[kWarps][kRows][D];
+    constexpr int kTurns = 32 / PB, kPageBytes = 2 * kKv8Block * D;
+    extern __shared__ __align__(16) uint8_t s_ring[];  // [kWarps][kStages][PB][kPageBytes], then the warps' results
+    float(*s_o)[kRows][D] = reinterpret_cast<float(*)[kRows][D]>(s_ring);
     __shared__ float2 s_ml[kWarps][kRows];
     __shared__ int s_last;
     pdl_wait();
     pdl_trigger();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const int split = static_cast<int>(blockIdx.x % p.splits);
-    const unsigned item = blockIdx.x / p.splits;
-    const int head = static_cast<int>(item % p.cache.heads);
-    const int tile = static_cast<int>(item / p.cache.heads % p.tiles);
-    const int i = static_cast<int>(item / p.cache.heads / p.tiles);
+    // block index: heads fastest (a page's heads are neighbours), then splits, row tiles, sequences
+    const uint32_t rest = kv8_div(blockIdx.x, p.by_heads), rest2 = kv8_div(rest, p.by_splits);
+    const int head = static_cast<int>(blockIdx.x - rest * p.by_heads.d);
+    const int split = static_cast<int>(rest - rest2 * p.by_splits.d);
+    const int i = static_cast<int>(kv8_div(rest2, p.by_tiles));
+    const int tile = static_cast<int>(rest2 - i * p.by_tiles.d);
+    const uint32_t item = rest2 * p.by_heads.d + head;
     const Kv8Seq sq = kv8_seq(p.seqs, i);
     const int rows = sq.count * p.group - tile * kRows;  // rows left from this tile on
     if (rows <= 0) return;
@@ -582,7 +590,7 @@ __global__ void __launch_bounds__(32 * kWarps) kv8_attention_kernel(Kv8AttnParam
     const int key_end = min(pos_hi + 1, sq.length);
     const int page_begin = p.window ? max(pos_lo - p.window + 1, 0) / kKv8Block : 0;
     const int pages = key_end > 0 ? (key_end + kKv8Block - 1) / kKv8Block - page_begin : 0;
-    const int active = max(1, min(p.splits, (pages + p.split_pages - 1) / p.split_pages));
+    const int active = max(1, min(static_cast<int>(p.by_splits.d), (pages + p.split_pages - 1) / p.split_pages));
     if (split >= active) return;
     const int per = (pages + active - 1) / active;
     const int first = page_begin + min(pages, split * per), last = page_begin + min(pages, (split + 1) * per);
@@ -590,54 +598,38 @@ __global__ void __launch_bounds__(32 * kWarps) kv8_attention_kernel(Kv8AttnParam
     const int whole_last = max(pos_lo + 1, 0) / kKv8Block;
     const int whole_first = p.window && pos_hi >= p.window ? (pos_hi - p.window) / kKv8Block + 1 : 0;
 
-    // this lane's page of the next kTurns turns: its id (-1: none) and scales
+    // this lane's page of kTurns turns of the warp, and of the kTurns after them: its id (-1: none) and scales
     constexpr int kStep = kWarps * PB;
     const int own = first + warp * PB + lane / PB * kStep + lane % PB;
     const uint8_t* exps = p.cache.exps + head * 2;
-    int my_id, my_exps;
-    auto fetch = [&](int turn) {
+    int ids[2], scales[2];
+    auto fetch = [&](int half, int turn) {
         const int at = own + turn * kStep;
-        my_id = at < last ? __ldg(sq.pages + at) : -1;
-        if (at < last && static_cast<unsigned>(my_id) >= static_cast<unsigned>(p.cache.pool_pages)) {
+        ids[half] = at < last ? __ldg(sq.pages + at) : -1;
+        if (at < last && static_cast<unsigned>(ids[half]) >= static_cast<unsigned>(p.cache.pool_pages)) {
             kv8_flag(p.seqs, i, kStatusInvalid);
-            my_id = -1;  // its positions are not seen
+            ids[half] = -1;  // its positions are not seen
         }
-        my_exps = my_id >= 0 ? __ldg(reinterpret_cast<const unsigned short*>(exps + static_cast<size_t>(my_id) * p.cache.heads * 2))
-                             : 127 | 127 << 8;
+        scales[half] = ids[half] >= 0
+                           ? __ldg(reinterpret_cast<const unsigned short*>(exps + static_cast<size_t>(ids[half]) * p.cache.heads * 2))
+                           : 127 | 127 << 8;
     };
-    uint32_t kw[PB][2][D / 16], vw[PB][D / 8];
-    int id[PB], next[PB], ex[PB], next_ex[PB];
-    const size_t page_bytes = static_cast<size_t>(p.cache.heads) * (2 * kKv8Block * D);
-    const uint8_t* key_base = p.cache.pool + static_cast<size_t>(head) * (2 * kKv8Block * D) + kv8_key_lane<D>(g, t);
-    const uint8_t* value_base = p.cache.pool + static_cast<size_t>(head) * (2 * kKv8Block * D) + kKv8Block * D + lane * 16;
-    auto take = [&](int turn) {
-        if (turn % kTurns == 0) fetch(turn);
+    const uint8_t* base = p.cache.pool + static_cast<size_t>(head) * kPageBytes;
+    const size_t page_bytes = static_cast<size_t>(p.cache.heads) * kPageBytes;
+    const uint8_t* ring = s_ring + warp * (kStages * PB * kPageBytes);
+    const uint32_t ring_addr = static_cast<uint32_t>(__cvta_generic_to_shared(ring));
+    auto copy = [&](int half, int turn, int stage) {  // turn's pages into the stage; always one group
 #pragma unroll
         for (int b = 0; b < PB; ++b) {
-            next[b] = __shfl_sync(kFull, my_id, turn % kTurns * PB + b);
-            next_ex[b] = __shfl_sync(kFull, my_exps, turn % kTurns * PB + b);
+            const int id = __shfl_sync(kFull, ids[half], turn % kTurns * PB + b);
+            if (id >= 0) kv8_copy<D>(ring_addr + (stage * PB + b) * kPageBytes, base + id * page_bytes, lane);
         }
+        asm volatile("cp.async.commit_group;" ::: "memory");
     };
-    auto load_keys = [&]() {
+    fetch(0, 0);
 #pragma unroll
-        for (int b = 0; b < PB; ++b)
-            if (next[b] >= 0) kv8_load_keys<D>(kw[b], key_base + next[b] * page_bytes);
-    };
-    auto load_values = [&]() {
-#pragma unroll
-        for (int b = 0; b < PB; ++b)
-            if (next[b] >= 0) kv8_load_values<D>(vw[b], value_base + next[b] * page_bytes);
-    };
-#pragma unroll
-    for (int b = 0; b < PB; ++b) {
-#pragma unroll
-        for (int k = 0; k < D / 16; ++k) kw[b][0][k] = kw[b][1][k] = 0x80808080u;
-#pragma unroll
-        for (int k = 0; k < D / 8; ++k) vw[b][k] = 0x80808080u;
-    }
-    take(0);
-    load_keys();
-    load_values();
+    for (int s = 0; s < kStages - 1; ++s) copy(0, s, s);
+    fetch(1, kTurns);
     int ref = 127;  // the value scale that eV is relative to, the same for all warps and splits
     if (pages > 0) {
         const int id0 = __ldg(sq.pages + page_begin);
@@ -710,14 +702,26 @@ __global__ void __launch_bounds__(32 * kWarps) kv8_attention_kernel(Kv8AttnParam
         for (int k = 0; k < KS; ++k) o[k][n][0] = o[k][n][1] = o[k][n][2] = o[k][n][3] = 0.0f;
     }
 
-    int turn = 0;
-    for (int at = first + warp * PB; at < last; at += kStep) {
+    int turn = 0, stage = 0;
+    for (int at = first + warp * PB; at < last; at += kStep, ++turn, stage = stage + 1 == kStages ? 0 : stage + 1) {
+        if (turn && turn % kTurns == 0) {
+            ids[0] = ids[1];
+            scales[0] = scales[1];
+            fetch(1, turn + kTurns);
+        }
+        asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
+        {
+            const int ahead = turn + kStages - 1, slot = stage == 0 ? kStages - 1 : stage - 1;
+            if (turn % kTurns + kStages - 1 < kTurns) copy(0, ahead, slot);
+            else copy(1, ahead, slot);
+        }
+        const uint8_t* pages_at = ring + stage * (PB * kPageBytes);
+        int id[PB], ex[PB];
 #pragma unroll
         for (int b = 0; b < PB; ++b) {
-            id[b] = next[b];
-            ex[b] = next_ex[b];
+            id[b] = __shfl_sync(kFull, ids[0], turn % kTurns * PB + b);
+            ex[b] = __shfl_sync(kFull, scales[0], turn % kTurns * PB + b);
         }
-        take(++turn);
         float s[PB][NT][2][RT];  // positions g, g + 8
         float less[PB];          // 2^-eV
 #pragma unroll
@@ -725,10 +729,12 @@ __global__ void __launch_bounds__(32 * kWarps) kv8_attention_kernel(Kv8AttnParam
             float c4[NT][4];
 #pragma unroll
             for (int n = 0; n < NT; ++n) c4[n][0] = c4[n][1] = c4[n][2] = c4[n][3] = 0.0f;
+            uint32_t kw[2][D / 16];
+            kv8_key_words<D>(kw, pages_at + b * kPageBytes, lane);
 #pragma unroll
             for (int c = 0; c < KS; ++c) {
-                const uint32_t a0 = kv8_halves<false>(kw[b][0][c]), a1 = kv8_halves<false>(kw[b][1][c]);
-                const uint32_t a2 = kv8_halves<true>(kw[b][0][c]), a3 = kv8_halves<true>(kw[b][1][c]);
+                const uint32_t a0 = kv8_halves<false>(kw[0][c]), a1 = kv8_halves<false>(kw[1][c]);
+                const uint32_t a2 = kv8_halves<true>(kw[0][c]), a3 = kv8_halves<true>(kw[1][c]);
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
                     mma16816(c4[n], a0, a1, a2, a3, qh[n][c][0], qh[n][c][1]);
@@ -763,7 +769,6 @@ __global__ void __launch_bounds__(32 * kWarps) kv8_attention_kernel(Kv8AttnParam
                     }
             }
         }
-        load_keys();
         uint32_t ph[PB][NT][2], pl[PB][kFine ? NT : 1][2];
         bool moved = false;
         float c[NT][RT];
@@ -819,18 +824,23 @@ __global__ void __launch_bounds__(32 * kWarps) kv8_attention_kernel(Kv8AttnParam
 #pragma unroll
         for (int b = 0; b < PB; ++b)
 #pragma unroll
-            for (int k = 0; k < KS; ++k) {
-                const uint32_t wa = vw[b][2 * k], wb = vw[b][2 * k + 1];
-                const uint32_t a0 = kv8_halves<false>(wa), a1 = kv8_halves<false>(wb);
-                const uint32_t a2 = kv8_halves<true>(wa), a3 = kv8_halves<true>(wb);
+            for (int j = 0; j < D / 32; ++j) {
+                const uint4 w4 = *reinterpret_cast<const uint4*>(pages_at + b * kPageBytes + kKv8Block * D + j * 512 + lane * 16);
+                const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
 #pragma unroll
-                for (int n = 0; n < NT; ++n) {
-                    mma16816(o[k][n], a0, a1, a2, a3, ph[b][n][0], ph[b][n][1]);
-                    if constexpr (kFine) mma16816(o[k][n], a0, a1, a2, a3, pl[b][n][0], pl[b][n][1]);
+                for (int k = 0; k < 2; ++k) {
+                    const uint32_t a0 = kv8_halves<false>(w[2 * k]), a1 = kv8_halves<false>(w[2 * k + 1]);
+                    const uint32_t a2 = kv8_halves<true>(w[2 * k]), a3 = kv8_halves<true>(w[2 * k + 1]);
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) {
+                        mma16816(o[2 * j + k][n], a0, a1, a2, a3, ph[b][n][0], ph[b][n][1]);
+                        if constexpr (kFine) mma16816(o[2 * j + k][n], a0, a1, a2, a3, pl[b][n][0], pl[b][n][1]);
+                    }
                 }
             }
-        load_values();
     }
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    __syncthreads();  // the ring becomes the warps' results
 
     // the warps' shares meet
 #pragma unroll
@@ -869,7 +879,7 @@ __global__ void __launch_bounds__(32 * kWarps) kv8_attention_kernel(Kv8AttnParam
         l = l * wa + l2 * wb;
         a = make_float4(a.x * wa + b.x * wb, a.y * wa + b.y * wb, a.z * wa + b.z * wb, a.w * wa + b.w * wb);
     };
-    const size_t slot = static_cast<size_t>(item) * p.splits;
+    const size_t slot = static_cast<size_t>(item) * p.by_splits.d;
     for (int x = threadIdx.x; x < n_rows * kQuads; x += blockDim.x) {
         const int r = x / kQuads, d = x % kQuads * 4;
         float mm = -INFINITY, ll = 0.0f;
