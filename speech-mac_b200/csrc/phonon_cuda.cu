@@ -452,7 +452,7 @@ struct Kv8Pool {
             release();
             return PHONON_CUDA_OUT_OF_MEMORY;
         }
-        CUDA_TRY(cudaMemset(pool, 128, layers * layer_bytes()));
+        CUDA_TRY(cudaMemset(pool, 0, layers * layer_bytes()));
         CUDA_TRY(cudaMemset(exps, kKv8MinExp + 127, layers * layer_exps()));
         CUDA_TRY(cudaStreamSynchronize(nullptr));  // callers' streams do not wait for the legacy stream
         return PHONON_CUDA_OK;
@@ -551,7 +551,7 @@ Kv8Div kv8_divisor(uint32_t d) {
 template <int D, int NT, int PB, int kStages, int kMode, int kWarps, int kCtas>
 int kv8_launch_attention(const Kv8Pool& c, uint32_t layer, const Kv8Seqs& seqs, const Kv8Attend& a,
                          const Kv8Scratch& w, int sms, cudaStream_t s) {
-    constexpr int kRows = kMode == KV8_F32_PACKED ? 4 : 8 * NT;
+    constexpr int kRows = kMode == KV8_INT_BF16 || kMode == KV8_INT_F32 ? 4 : 8 * NT;
     static_assert(kRows * D <= kKv8TileFloats, "a partial result outgrows its scratch");
     Kv8AttnParams p{};
     p.cache = c.view(layer);
@@ -592,22 +592,23 @@ int kv8_launch_attention(const Kv8Pool& c, uint32_t layer, const Kv8Seqs& seqs, 
     return PHONON_CUDA_OK;
 }
 
-// By the rows that share a K/V head of a sequence: what they need of the
-// column tiles (four fp32 rows or eight bf16 rows fill one).
+// By the rows that share a K/V head of a sequence: up to four multiply as
+// bytes, more as halves, 8 to 32 at a time.
 template <int D>
 int kv8_attention_rows(const Kv8Pool& c, uint32_t layer, const Kv8Seqs& seqs, const Kv8Attend& a, const Kv8Scratch& w,
                        int sms, cudaStream_t s) {
     const long long rows = static_cast<long long>(seqs.max_rows) * a.group;
-    constexpr int PB = D == 128 ? 1 : 2;
+    constexpr int PB = D == 128 ? 1 : 2, PI = D == 128 ? 2 : 4;
     if (a.bf16) {
-        if (rows <= 8) return kv8_launch_attention<D, 1, PB, 3, KV8_BF16, 4, 4>(c, layer, seqs, a, w, sms, s);
-        if (rows <= 16 || D == 128) return kv8_launch_attention<D, 2, 1, 3, KV8_BF16, 4, 4>(c, layer, seqs, a, w, sms, s);
-        if constexpr (D < 128) return kv8_launch_attention<D, 4, 1, 3, KV8_BF16, 4, 2>(c, layer, seqs, a, w, sms, s);
+        if (rows <= 4) return kv8_launch_attention<D, 1, PI, 2, KV8_INT_BF16, 4, 3>(c, layer, seqs, a, w, sms, s);
+        if (rows <= 8) return kv8_launch_attention<D, 1, PB, 3, KV8_HALF_BF16, 4, 4>(c, layer, seqs, a, w, sms, s);
+        if (rows <= 16 || D == 128) return kv8_launch_attention<D, 2, 1, 3, KV8_HALF_BF16, 4, 4>(c, layer, seqs, a, w, sms, s);
+        if constexpr (D < 128) return kv8_launch_attention<D, 4, 1, 3, KV8_HALF_BF16, 4, 2>(c, layer, seqs, a, w, sms, s);
     }
-    if (rows <= 4) return kv8_launch_attention<D, 1, PB, 3, KV8_F32_PACKED, 4, 4>(c, layer, seqs, a, w, sms, s);
-    if (rows <= 8) return kv8_launch_attention<D, 1, PB, 3, KV8_F32, 4, 4>(c, layer, seqs, a, w, sms, s);
-    if (rows <= 16 || D == 128) return kv8_launch_attention<D, 2, 1, 3, KV8_F32, 4, 3>(c, layer, seqs, a, w, sms, s);
-    if constexpr (D < 128) return kv8_launch_attention<D, 4, 1, 3, KV8_F32, 4, 2>(c, layer, seqs, a, w, sms, s);
+    if (rows <= 4) return kv8_launch_attention<D, 1, PI, 2, KV8_INT_F32, 4, 3>(c, layer, seqs, a, w, sms, s);
+    if (rows <= 8) return kv8_launch_attention<D, 1, PB, 3, KV8_HALF_F32, 4, 4>(c, layer, seqs, a, w, sms, s);
+    if (rows <= 16 || D == 128) return kv8_launch_attention<D, 2, 1, 3, KV8_HALF_F32, 4, 3>(c, layer, seqs, a, w, sms, s);
+    if constexpr (D < 128) return kv8_launch_attention<D, 4, 1, 3, KV8_HALF_F32, 4, 2>(c, layer, seqs, a, w, sms, s);
     return PHONON_CUDA_INVALID_ARGUMENT;
 }
 

@@ -4,7 +4,7 @@
 // Format. A block is 16 positions of one K/V head; its keys and its values
 // each share one scale 2^e with e the smallest integer in [kKv8MinExp,
 // kKv8MaxExp] for which |x| <= 127 * 2^e over the block, and an element is
-// held as the integer nearest x / 2^e, at most 127 in magnitude, plus 128.
+// held as the integer nearest x / 2^e, at most 127 in magnitude.
 // The scale is a power of two so that quantising, raising the scale of a
 // partly filled block (the held integers divided by a power of two and
 // rounded again) and reading back are exact but for the one rounding each
@@ -109,12 +109,12 @@ __device__ __forceinline__ int kv8_exponent(float amax) {
 }
 
 __device__ __forceinline__ uint32_t kv8_code(float x, float inverse) {
-    return static_cast<uint32_t>(min(max(__float2int_rn(__fmul_rn(x, inverse)), -127), 127) + 128);
+    return static_cast<uint32_t>(min(max(__float2int_rn(__fmul_rn(x, inverse)), -127), 127)) & 0xffu;
 }
 
 // A held byte of a scale 2^k times smaller (shrink = 2^-k) in the new one.
 __device__ __forceinline__ uint32_t kv8_shrink(uint32_t byte, float shrink) {
-    return static_cast<uint32_t>(__float2int_rn(__fmul_rn(static_cast<float>(static_cast<int>(byte) - 128), shrink)) + 128);
+    return static_cast<uint32_t>(__float2int_rn(__fmul_rn(static_cast<float>(static_cast<int8_t>(byte)), shrink))) & 0xffu;
 }
 
 template <bool kBf16>
@@ -331,7 +331,7 @@ struct Kv8ReadParams {
     int blocks;
 };
 
-// One warp reads one block's keys or values back: held byte - 128 times 2^e,
+// One warp reads one block's keys or values back: the held integer times 2^e,
 // exact in fp32. Rows of positions before 0, of empty and of bad pages are 0.
 template <int D, bool kBf16>
 __global__ void __launch_bounds__(128) kv8_read_kernel(Kv8ReadParams p) {
@@ -366,7 +366,7 @@ __global__ void __launch_bounds__(128) kv8_read_kernel(Kv8ReadParams p) {
     const float unit = page >= 0 ? pow2i(kv8_exp(p.cache, page, head)[which] - 127) : 0.0f;
     void* dst = p.rows[which];
     auto value = [&](uint32_t w, int k) {
-        return static_cast<float>(static_cast<int>((w >> (8 * k)) & 0xffu) - 128) * unit;
+        return static_cast<float>(static_cast<int8_t>(w >> (8 * k))) * unit;
     };
     const int g = lane >> 2, t = lane & 3;
     if (which == 0) {
@@ -376,7 +376,7 @@ __global__ void __launch_bounds__(128) kv8_read_kernel(Kv8ReadParams p) {
             const int slot = a * kRowsPerPass + lane / kLanesPerRow;
             w[a] = src && slot >= lo && slot < hi
                        ? __ldg(reinterpret_cast<const uint32_t*>(src + slot * D) + lane % kLanesPerRow)
-                       : 0x80808080u;
+                       : 0u;
         }
 #pragma unroll
         for (int a = 0; a < kPasses; ++a) {
@@ -390,7 +390,7 @@ __global__ void __launch_bounds__(128) kv8_read_kernel(Kv8ReadParams p) {
 #pragma unroll
         for (int j = 0; j < kChunks; ++j)
             w[j] = src ? __ldg(reinterpret_cast<const uint4*>(src + j * 512) + lane)
-                       : make_uint4(0x80808080u, 0x80808080u, 0x80808080u, 0x80808080u);
+                       : make_uint4(0u, 0u, 0u, 0u);
 #pragma unroll
         for (int j = 0; j < kChunks; ++j)
 #pragma unroll
@@ -418,26 +418,31 @@ __device__ __forceinline__ uint32_t kv8_div(uint32_t n, Kv8Div d) { return d.d =
 // set. Rows that see nothing get 0.
 //
 // Per block the tensor cores compute S^T = K q^T (16 positions x 8 columns)
-// and O^T += V^T P^T (16 dims x 8 columns) with the cache's integers as the A
-// operand: byte | 0x6400 is the half 1024 + byte, minus 1152 the signed
-// integer, exactly, one PRMT and one HSUB2 for two elements. Rows are the N
-// operand: a decode step's single row (times the grouped heads) costs half
-// the instructions that it would as M. A block's scales enter in fp32: with s
-// = scale log2(e) 2^eK (q.K) + eV, the weight 2^(s - M) is the softmax weight
-// times the block's value scale, so that O needs no scaling of its own, and the
-// sum of weights takes 2^(s - M - eV). M is the running maximum of s; eV is
-// taken relative to the first visible page's, so that s keeps its precision
-// whatever the values' size. eV spans 112 at most, so weights that matter stay
-// inside fp32's range.
+// and O^T += V^T P^T (16 dims x 8 columns): the cache is the A operand, rows
+// are columns, so that a decode step's single row (times the grouped heads)
+// costs half the instructions that it would as M. A block's scales enter in
+// fp32: with s = scale log2(e) 2^eK (q.K) + eV, the weight 2^(s - M) is the
+// softmax weight times the block's value scale, so that O needs no scaling of
+// its own, and the sum of weights takes 2^(s - M - eV). M is the running
+// maximum of s; eV is taken relative to the first visible page's, so that s
+// keeps its precision whatever the values' size. eV spans 112 at most, so
+// weights that matter stay inside fp32's range.
 //
-// Rounding: the 8-bit integers and their products with a half are exact in
-// the fp32 accumulators. fp32 rows: q (scaled by a power of two to a row
-// maximum near 2^12) and the weights enter as two halves each, 22 bits. Up to
-// four rows are packed: columns 2r and 2r + 1 are the two halves of row r, one
-// product for both, summed by the lane that holds both (half the products and
-// half the softmax work a lane); more rows take two products each. bf16 rows:
-// q fits one half (8 bits), a weight is rounded to one half (11 bits, under
-// the output's 8).
+// Up to four rows that share a head (a decode step): 8-bit integer products,
+// the cache's bytes as they lie. q is held as an integer of 22 bits (14 in
+// bf16 rows, whose own 8 it keeps) relative to the row's maximum, split into
+// signed bytes: columns 2r, 2r + 1 are the first two of row r and a second
+// column tile has the third. A score's sums are exact; so are those of the
+// output per turn, with weights of 23 bits (2 + 2 weight as a float has them
+// as its mantissa: its bytes are the columns). Only the weights' rounding
+// (2^-24 of the largest) and the turns' fp32 sums are left.
+//
+// More rows: products of halves, the conversion of a block's bytes shared by
+// the rows. Byte ^ 0x80 | 0x6400 is the half 1152 + integer, minus 1152 the
+// integer, exactly. The products are exact in the fp32 accumulators. fp32 rows:
+// q (scaled by a power of two to a row maximum near 2^12) and the weights
+// enter as two halves each, 22 bits. bf16 rows: q fits one half (8 bits), a
+// weight is rounded to one half (11 bits, under the output's 8).
 struct Kv8AttnParams {
     Kv8View cache;
     Kv8Seqs seqs;
@@ -456,13 +461,31 @@ struct Kv8AttnParams {
 
 constexpr float kKv8WeightBits = 14.0f;  // weights are held times 2^14: a half keeps 11 bits down to 2^-28
 
-enum Kv8Mode : int { KV8_BF16 = 0, KV8_F32 = 1, KV8_F32_PACKED = 2 };
+// Weights as integers: the mantissa of 2 + 2 (1 - 2^-22) w, that is w in units
+// of 2^-23, short of the next power of two where w is 1 and an ulp.
+constexpr float kKv8FixedScale = 2.0f - 0x1p-21f;
+
+enum Kv8Mode : int { KV8_HALF_BF16 = 0, KV8_HALF_F32 = 1, KV8_INT_BF16 = 2, KV8_INT_F32 = 3 };
 
 __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                          uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// 16 x 32 signed bytes by 32 x 8 signed (kSigned) or unsigned bytes.
+template <bool kSigned>
+__device__ __forceinline__ void imma16832(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                          uint32_t b1) {
+    if constexpr (kSigned)
+        asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
+                     : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    else
+        asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.u8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
+                     : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
 __device__ __forceinline__ uint32_t movmatrix_trans(uint32_t v) {
@@ -478,7 +501,7 @@ __device__ __forceinline__ float ex2(float x) {
     return r;
 }
 
-// Bytes 0, 1 (kHigh: 2, 3) of a cache word as the halves byte - 128.
+// Bytes 0, 1 (kHigh: 2, 3) of a cache word, sign bits flipped, as halves.
 template <bool kHigh>
 __device__ __forceinline__ uint32_t kv8_halves(uint32_t w) {
     uint32_t u = __byte_perm(w, 0x64646464u, kHigh ? 0x4342 : 0x4140);
@@ -499,29 +522,31 @@ __device__ __forceinline__ float2 half2_floats(uint32_t u) { return __half22floa
 // 16 bytes. The lane copies them into its warp's ring in shared memory and
 // reads them back itself, so no other thread is waited for: 16 bytes of lane
 // 0, of lane 1, ... per chunk, without bank conflicts.
-__device__ __forceinline__ void copy16(uint32_t dst, const uint8_t* src) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+// (0 of `bytes` read: zeros are written and the source is not touched)
+__device__ __forceinline__ void copy16(uint32_t dst, const uint8_t* src, int bytes) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
 
-__device__ __forceinline__ void copy8(uint32_t dst, const uint8_t* src) {
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst), "l"(src) : "memory");
+__device__ __forceinline__ void copy8(uint32_t dst, const uint8_t* src, int bytes) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(dst), "l"(src), "r"(bytes / 2) : "memory");
 }
 
 template <int D>
-__device__ __forceinline__ void kv8_copy(uint32_t dst, const uint8_t* block, int lane) {
+__device__ __forceinline__ void kv8_copy(uint32_t dst, const uint8_t* block, int lane, int bytes) {
     const int g = lane >> 2, t = lane & 3;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
         if constexpr (D == 32) {
-            copy8(dst + h * 256 + lane * 8, block + (g + 8 * h) * D + t * 8);
+            copy8(dst + h * 256 + lane * 8, block + (g + 8 * h) * D + t * 8, bytes);
         } else {
 #pragma unroll
             for (int c = 0; c < D / 64; ++c)
-                copy16(dst + (h * (D / 64) + c) * 512 + lane * 16, block + (g + 8 * h) * D + c * 64 + t * 16);
+                copy16(dst + (h * (D / 64) + c) * 512 + lane * 16, block + (g + 8 * h) * D + c * 64 + t * 16, bytes);
         }
     }
 #pragma unroll
-    for (int j = 0; j < D / 32; ++j) copy16(dst + kKv8Block * D + j * 512 + lane * 16, block + kKv8Block * D + j * 512 + lane * 16);
+    for (int j = 0; j < D / 32; ++j)
+        copy16(dst + kKv8Block * D + j * 512 + lane * 16, block + kKv8Block * D + j * 512 + lane * 16, bytes);
 }
 
 // Key words [position g, g + 8][4 dims each], value words [2 x 16-dim tiles].
@@ -561,10 +586,11 @@ __device__ __forceinline__ int kv8_key_dim(int t, int c) {
 // each, 32 / PB turns at a time.
 template <int D, int NT, int PB, int kStages, int kMode, int kWarps, int kCtas>
 __global__ void __launch_bounds__(32 * kWarps, kCtas) kv8_attention_kernel(Kv8AttnParams p) {
-    constexpr bool kBf16 = kMode == KV8_BF16, kFine = kMode == KV8_F32, kPack = kMode == KV8_F32_PACKED;
-    static_assert(!kPack || NT == 1, "packed rows fill one column tile");
-    constexpr int kRows = kPack ? 4 : 8 * NT;
-    constexpr int RT = kPack ? 1 : 2;  // rows of a column tile that a lane holds scores of
+    constexpr bool kBf16 = kMode == KV8_HALF_BF16 || kMode == KV8_INT_BF16, kFine = kMode == KV8_HALF_F32;
+    constexpr bool kInt = kMode == KV8_INT_BF16 || kMode == KV8_INT_F32;
+    static_assert(!kInt || (NT == 1 && PB % 2 == 0), "four rows, values multiplied two pages at a time");
+    constexpr int kRows = kInt ? 4 : 8 * NT;
+    constexpr int RT = kInt ? 1 : 2;  // rows of a column tile that a lane holds scores of
     constexpr int KS = D / 16;         // 16-dim steps of a score, and 16-dim tiles of an output
     constexpr int kTurns = 32 / PB, kPageBytes = 2 * kKv8Block * D;
     extern __shared__ __align__(16) uint8_t s_ring[];  // [kWarps][kStages][PB][kPageBytes], then the warps' results
@@ -622,7 +648,7 @@ __global__ void __launch_bounds__(32 * kWarps, kCtas) kv8_attention_kernel(Kv8At
 #pragma unroll
         for (int b = 0; b < PB; ++b) {
             const int id = __shfl_sync(kFull, ids[half], turn % kTurns * PB + b);
-            if (id >= 0) kv8_copy<D>(ring_addr + (stage * PB + b) * kPageBytes, base + id * page_bytes, lane);
+            kv8_copy<D>(ring_addr + (stage * PB + b) * kPageBytes, base + max(id, 0) * page_bytes, lane, id >= 0 ? 16 : 0);
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
     };
@@ -637,14 +663,14 @@ __global__ void __launch_bounds__(32 * kWarps, kCtas) kv8_attention_kernel(Kv8At
             ref = __ldg(exps + static_cast<size_t>(id0) * p.cache.heads * 2 + 1);
     }
 
-    // q as B fragments, scaled to a row maximum in [2^12, 2^13); column g is
-    // row g, or one half of row g / 2
-    uint32_t qh[NT][KS][2], ql[NT][kFine ? KS : 1][2];
+    // q as B fragments; column g is row g (halves), or byte g % 2 of row g / 2 (qh) and its third byte (ql)
+    constexpr int QS = kInt ? D / 32 : KS;  // steps of a score
+    uint32_t qh[NT][QS][2], ql[NT][kFine || kMode == KV8_INT_F32 ? QS : 1][2];
     float f[NT][RT];  // scale * 2^(row exponent) of the lane's rows
     int pos[NT][RT];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-        const int r = kPack ? g >> 1 : n * 8 + g, rho = rho0 + min(r, n_rows - 1);
+        const int r = kInt ? g >> 1 : n * 8 + g, rho = rho0 + min(r, n_rows - 1);
         const size_t row = static_cast<size_t>(sq.row0 + rho / p.group) * p.q_stride +
                            static_cast<size_t>(head * p.group + rho % p.group) * D;
         float4 v[KS];
@@ -662,22 +688,34 @@ __global__ void __launch_bounds__(32 * kWarps, kCtas) kv8_attention_kernel(Kv8At
         const bool row_bad = (bad >> (lane & ~3) & 0xfu) != 0;
         if (row_bad && t == 0 && r < n_rows) kv8_flag(p.seqs, i, kStatusNonFinite);
         // exponent of the maximum, kept where both powers below are normal
-        const int e = min(max(static_cast<int>(__float_as_uint(amax) >> 23) - 127, -110), 126);
-        const float up = pow2i(12 - e), back = pow2i(e - 12);
+        constexpr int kTop = kMode == KV8_INT_F32 ? 21 : kMode == KV8_INT_BF16 ? 13 : 12;
+        const int e = min(max(static_cast<int>(__float_as_uint(amax) >> 23) - 127, -105), 126);
+        const float up = pow2i(kTop - e), back = pow2i(e - kTop);
 #pragma unroll
         for (int c = 0; c < KS; ++c) {
             const float x[4] = {v[c].x * up, v[c].y * up, v[c].z * up, v[c].w * up};
-            qh[n][c][0] = half2_bits(x[0], x[1]);
-            qh[n][c][1] = half2_bits(x[2], x[3]);
-            if constexpr (!kBf16) {
-                const float2 h0 = half2_floats(qh[n][c][0]), h1 = half2_floats(qh[n][c][1]);
-                const uint32_t l0 = half2_bits(x[0] - h0.x, x[1] - h0.y), l1 = half2_bits(x[2] - h1.x, x[3] - h1.y);
+            if constexpr (kInt) {
+                // |x| < 2^22 (2^14): signed bytes d0 * 65536 + d1 * 256 + d2 (d0 * 256 + d1), |d0| <= 64
+                uint32_t first = 0, third = 0;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    int y = __float2int_rn(x[k]);
+                    if constexpr (kMode == KV8_INT_F32) {
+                        third |= (static_cast<uint32_t>(y) & 0xffu) << (8 * k);
+                        y = (y + 128) >> 8;
+                    }
+                    const int d1 = static_cast<int8_t>(y), d0 = (y - d1) >> 8;
+                    first |= (static_cast<uint32_t>(g & 1 ? d1 : d0) & 0xffu) << (8 * k);
+                }
+                qh[n][c / 2][c % 2] = first;
+                if constexpr (kMode == KV8_INT_F32) ql[n][c / 2][c % 2] = third;
+            } else {
+                qh[n][c][0] = half2_bits(x[0], x[1]);
+                qh[n][c][1] = half2_bits(x[2], x[3]);
                 if constexpr (kFine) {
-                    ql[n][c][0] = l0;
-                    ql[n][c][1] = l1;
-                } else if (g & 1) {
-                    qh[n][c][0] = l0;
-                    qh[n][c][1] = l1;
+                    const float2 h0 = half2_floats(qh[n][c][0]), h1 = half2_floats(qh[n][c][1]);
+                    ql[n][c][0] = half2_bits(x[0] - h0.x, x[1] - h0.y);
+                    ql[n][c][1] = half2_bits(x[2] - h1.x, x[3] - h1.y);
                 }
             }
         }
@@ -685,12 +723,14 @@ __global__ void __launch_bounds__(32 * kWarps, kCtas) kv8_attention_kernel(Kv8At
 #pragma unroll
         for (int k = 0; k < RT; ++k) {
             f[n][k] = __shfl_sync(kFull, fr, 8 * t + 4 * k);
-            const int lane_row = kPack ? t : n * 8 + 2 * t + k;
+            const int lane_row = kInt ? t : n * 8 + 2 * t + k;
             pos[n][k] = at0 + (rho0 + min(lane_row, n_rows - 1)) / p.group;
         }
     }
 
-    float o[KS][NT][4], m[NT][RT], l[NT][RT];
+    // O: [16-dim tile][column tile][accumulators] (halves), or the lane's row of dims g, g + 8 of a tile
+    constexpr int OT = kInt ? 2 : 4;
+    float o[KS][NT][OT], m[NT][RT], l[NT][RT];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
 #pragma unroll
@@ -699,8 +739,12 @@ __global__ void __launch_bounds__(32 * kWarps, kCtas) kv8_attention_kernel(Kv8At
             l[n][k] = 0.0f;
         }
 #pragma unroll
-        for (int k = 0; k < KS; ++k) o[k][n][0] = o[k][n][1] = o[k][n][2] = o[k][n][3] = 0.0f;
+        for (int k = 0; k < KS; ++k)
+#pragma unroll
+            for (int j = 0; j < OT; ++j) o[k][n][j] = 0.0f;
     }
+    const int from0 = 8 * t + (g >> 1), from1 = from0 + 4;   // lanes with the weights of positions 2t, 2t + 1 of row g / 2
+    const uint32_t pick = g & 1 ? 0x6240u : 0x7351u;         // the weight byte that column g multiplies
 
     int turn = 0, stage = 0;
     for (int at = first + warp * PB; at < last; at += kStep, ++turn, stage = stage + 1 == kStages ? 0 : stage + 1) {
@@ -726,19 +770,35 @@ __global__ void __launch_bounds__(32 * kWarps, kCtas) kv8_attention_kernel(Kv8At
         float less[PB];          // 2^-eV
 #pragma unroll
         for (int b = 0; b < PB; ++b) {
-            float c4[NT][4];
-#pragma unroll
-            for (int n = 0; n < NT; ++n) c4[n][0] = c4[n][1] = c4[n][2] = c4[n][3] = 0.0f;
+            float c4[NT][4];  // q.K: positions g, g + 8 of the lane's rows
             uint32_t kw[2][D / 16];
             kv8_key_words<D>(kw, pages_at + b * kPageBytes, lane);
+            if constexpr (kInt) {
+                int x[4] = {0, 0, 0, 0}, y[4] = {0, 0, 0, 0};
 #pragma unroll
-            for (int c = 0; c < KS; ++c) {
-                const uint32_t a0 = kv8_halves<false>(kw[0][c]), a1 = kv8_halves<false>(kw[1][c]);
-                const uint32_t a2 = kv8_halves<true>(kw[0][c]), a3 = kv8_halves<true>(kw[1][c]);
+                for (int c = 0; c < QS; ++c) {
+                    imma16832<true>(x, kw[0][2 * c], kw[1][2 * c], kw[0][2 * c + 1], kw[1][2 * c + 1], qh[0][c][0], qh[0][c][1]);
+                    if constexpr (kMode == KV8_INT_F32)
+                        imma16832<true>(y, kw[0][2 * c], kw[1][2 * c], kw[0][2 * c + 1], kw[1][2 * c + 1], ql[0][c][0], ql[0][c][1]);
+                }
 #pragma unroll
-                for (int n = 0; n < NT; ++n) {
-                    mma16816(c4[n], a0, a1, a2, a3, qh[n][c][0], qh[n][c][1]);
-                    if constexpr (kFine) mma16816(c4[n], a0, a1, a2, a3, ql[n][c][0], ql[n][c][1]);
+                for (int h = 0; h < 2; ++h)
+                    c4[0][2 * h] = kMode == KV8_INT_F32 ? fmaf(static_cast<float>(x[2 * h]), 65536.0f,
+                                                               static_cast<float>(x[2 * h + 1] * 256 + y[2 * h]))
+                                                        : static_cast<float>(x[2 * h] * 256 + x[2 * h + 1]);
+            } else {
+#pragma unroll
+                for (int n = 0; n < NT; ++n) c4[n][0] = c4[n][1] = c4[n][2] = c4[n][3] = 0.0f;
+#pragma unroll
+                for (int c = 0; c < KS; ++c) {
+                    const uint32_t wa = kw[0][c] ^ 0x80808080u, wb = kw[1][c] ^ 0x80808080u;
+                    const uint32_t a0 = kv8_halves<false>(wa), a1 = kv8_halves<false>(wb);
+                    const uint32_t a2 = kv8_halves<true>(wa), a3 = kv8_halves<true>(wb);
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) {
+                        mma16816(c4[n], a0, a1, a2, a3, qh[n][c][0], qh[n][c][1]);
+                        if constexpr (kFine) mma16816(c4[n], a0, a1, a2, a3, ql[n][c][0], ql[n][c][1]);
+                    }
                 }
             }
             const float uk = __int_as_float((ex[b] & 0xff) << 23);
@@ -752,7 +812,7 @@ __global__ void __launch_bounds__(32 * kWarps, kCtas) kv8_attention_kernel(Kv8At
                     const float u = f[n][k] * uk;
 #pragma unroll
                     for (int h = 0; h < 2; ++h)
-                        s[b][n][h][k] = fmaf(kPack ? c4[n][2 * h] + c4[n][2 * h + 1] : c4[n][2 * h + k], u, add);
+                        s[b][n][h][k] = fmaf(c4[n][2 * h + k], u, add);
                 }
             const int page = at + b;
             if (id[b] < 0 || page < whole_first || page >= whole_last) {
@@ -769,12 +829,10 @@ __global__ void __launch_bounds__(32 * kWarps, kCtas) kv8_attention_kernel(Kv8At
                     }
             }
         }
-        uint32_t ph[PB][NT][2], pl[PB][kFine ? NT : 1][2];
         bool moved = false;
-        float c[NT][RT];
+        float c[NT][RT], top[NT][RT];
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-            float base[RT];
+        for (int n = 0; n < NT; ++n)
 #pragma unroll
             for (int k = 0; k < RT; ++k) {
                 float x = m[n][k];
@@ -785,24 +843,71 @@ __global__ void __launch_bounds__(32 * kWarps, kCtas) kv8_attention_kernel(Kv8At
                 c[n][k] = m[n][k] == x ? 1.0f : ex2(m[n][k] - x);
                 moved |= m[n][k] != x;
                 m[n][k] = x;
-                base[k] = x == -INFINITY ? 0.0f : x - kKv8WeightBits;  // nothing seen yet: weights 2^(-inf - 0)
+                top[n][k] = x == -INFINITY ? 0.0f : kInt ? x : x - kKv8WeightBits;  // nothing seen yet: weights 2^(-inf - 0)
                 l[n][k] *= c[n][k];
             }
+        if constexpr (kInt) {
+            uint32_t high[PB], low[PB];  // B fragments: the weights' bytes of column g, four positions a page
+            uint32_t w[PB][2];
 #pragma unroll
             for (int b = 0; b < PB; ++b) {
-                float w[2][RT];
-#pragma unroll
-                for (int k = 0; k < RT; ++k) {
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) w[h][k] = ex2(s[b][n][h][k] - base[k]);
-                    l[n][k] = fmaf(w[0][k] + w[1][k], less[b], l[n][k]);
-                }
+                float sum = 0.0f;
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    if constexpr (kPack) {
-                        const float high = __half2float(__float2half_rn(w[h][0]));
-                        ph[b][n][h] = movmatrix_trans(half2_bits(w[h][0], w[h][0] - high));
-                    } else {
+                    const float weight = ex2(s[b][0][h][0] - top[0][0]);
+                    sum += weight;
+                    w[b][h] = __float_as_uint(fmaf(weight, kKv8FixedScale, 2.0f));
+                }
+                l[0][0] = fmaf(sum, less[b], l[0][0]);
+                const uint32_t both = __byte_perm(w[b][0], w[b][1], 0x6521);  // bytes 1, 2 of position g, of g + 8
+                high[b] = __byte_perm(__shfl_sync(kFull, both, from0), __shfl_sync(kFull, both, from1), pick);
+            }
+#pragma unroll
+            for (int b = 0; b < PB; b += 2) {
+                const uint32_t both = __byte_perm(__byte_perm(w[b][0], w[b][1], 0x0040),
+                                                  __byte_perm(w[b + 1][0], w[b + 1][1], 0x0040), 0x5410);
+                const uint32_t x = __shfl_sync(kFull, both, from0), y = __shfl_sync(kFull, both, from1);
+                low[b] = __byte_perm(x, y, 0x5140);
+                low[b + 1] = __byte_perm(x, y, 0x7362);
+            }
+#pragma unroll
+            for (int j = 0; j < D / 32; ++j) {
+                uint4 v[PB];
+#pragma unroll
+                for (int b = 0; b < PB; ++b)
+                    v[b] = *reinterpret_cast<const uint4*>(pages_at + b * kPageBytes + kKv8Block * D + j * 512 + lane * 16);
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    int x[4] = {0, 0, 0, 0}, y[4] = {0, 0, 0, 0};
+#pragma unroll
+                    for (int b = 0; b < PB; b += 2) {
+                        const uint32_t a0 = k ? v[b].z : v[b].x, a1 = k ? v[b].w : v[b].y;
+                        const uint32_t a2 = k ? v[b + 1].z : v[b + 1].x, a3 = k ? v[b + 1].w : v[b + 1].y;
+                        imma16832<false>(x, a0, a1, a2, a3, high[b], high[b + 1]);
+                        imma16832<false>(y, a0, a1, a2, a3, low[b], low[b + 1]);
+                    }
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+                        o[2 * j + k][0][h] =
+                            fmaf(o[2 * j + k][0][h], c[0][0],
+                                 fmaf(static_cast<float>(x[2 * h]), 65536.0f, static_cast<float>(x[2 * h + 1] * 256 + y[2 * h])));
+                }
+            }
+        } else {
+            uint32_t ph[PB][NT][2], pl[PB][kFine ? NT : 1][2];
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int b = 0; b < PB; ++b) {
+                    float w[2][RT];
+#pragma unroll
+                    for (int k = 0; k < RT; ++k) {
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) w[h][k] = ex2(s[b][n][h][k] - top[n][k]);
+                        l[n][k] = fmaf(w[0][k] + w[1][k], less[b], l[n][k]);
+                    }
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
                         const uint32_t high = half2_bits(w[h][0], w[h][RT - 1]);
                         ph[b][n][h] = movmatrix_trans(high);
                         if constexpr (kFine) {
@@ -811,33 +916,34 @@ __global__ void __launch_bounds__(32 * kWarps, kCtas) kv8_attention_kernel(Kv8At
                         }
                     }
                 }
+            if (__any_sync(kFull, moved)) {
+#pragma unroll
+                for (int k = 0; k < KS; ++k)
+#pragma unroll
+                    for (int n = 0; n < NT; ++n)
+#pragma unroll
+                        for (int j = 0; j < OT; ++j) o[k][n][j] *= c[n][j % RT];
             }
-        }
-        if (__any_sync(kFull, moved)) {
+            if constexpr (!kInt) {
 #pragma unroll
-            for (int k = 0; k < KS; ++k)
+                for (int b = 0; b < PB; ++b)
 #pragma unroll
-                for (int n = 0; n < NT; ++n)
+                    for (int j = 0; j < D / 32; ++j) {
+                        const uint4 w4 = *reinterpret_cast<const uint4*>(pages_at + b * kPageBytes + kKv8Block * D + j * 512 + lane * 16);
+                        const uint32_t w[4] = {w4.x ^ 0x80808080u, w4.y ^ 0x80808080u, w4.z ^ 0x80808080u, w4.w ^ 0x80808080u};
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) o[k][n][j] *= c[n][kPack ? 0 : j & 1];
-        }
+                        for (int k = 0; k < 2; ++k) {
+                            const uint32_t a0 = kv8_halves<false>(w[2 * k]), a1 = kv8_halves<false>(w[2 * k + 1]);
+                            const uint32_t a2 = kv8_halves<true>(w[2 * k]), a3 = kv8_halves<true>(w[2 * k + 1]);
 #pragma unroll
-        for (int b = 0; b < PB; ++b)
-#pragma unroll
-            for (int j = 0; j < D / 32; ++j) {
-                const uint4 w4 = *reinterpret_cast<const uint4*>(pages_at + b * kPageBytes + kKv8Block * D + j * 512 + lane * 16);
-                const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
-#pragma unroll
-                for (int k = 0; k < 2; ++k) {
-                    const uint32_t a0 = kv8_halves<false>(w[2 * k]), a1 = kv8_halves<false>(w[2 * k + 1]);
-                    const uint32_t a2 = kv8_halves<true>(w[2 * k]), a3 = kv8_halves<true>(w[2 * k + 1]);
-#pragma unroll
-                    for (int n = 0; n < NT; ++n) {
-                        mma16816(o[2 * j + k][n], a0, a1, a2, a3, ph[b][n][0], ph[b][n][1]);
-                        if constexpr (kFine) mma16816(o[2 * j + k][n], a0, a1, a2, a3, pl[b][n][0], pl[b][n][1]);
+                            for (int n = 0; n < NT; ++n) {
+                                mma16816(o[2 * j + k][n], a0, a1, a2, a3, ph[b][n][0], ph[b][n][1]);
+                                if constexpr (kFine) mma16816(o[2 * j + k][n], a0, a1, a2, a3, pl[b][n][0], pl[b][n][1]);
+                            }
+                        }
                     }
-                }
             }
+        }
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
     __syncthreads();  // the ring becomes the warps' results
@@ -849,7 +955,7 @@ __global__ void __launch_bounds__(32 * kWarps, kCtas) kv8_attention_kernel(Kv8At
         for (int k = 0; k < RT; ++k) {
 #pragma unroll
             for (int w = 4; w < 32; w <<= 1) l[n][k] += __shfl_xor_sync(kFull, l[n][k], w);
-            const int r = kPack ? t : n * 8 + 2 * t + k;
+            const int r = kInt ? t : n * 8 + 2 * t + k;
             if (g == 0) s_ml[warp][r] = make_float2(m[n][k], l[n][k]);
             if (r >= n_rows) continue;
 #pragma unroll
@@ -857,13 +963,12 @@ __global__ void __launch_bounds__(32 * kWarps, kCtas) kv8_attention_kernel(Kv8At
                 const float* x = o[2 * j][n];
                 const float* y = o[2 * j + 1][n];
                 *reinterpret_cast<float4*>(&s_o[warp][r][32 * j + 4 * g]) =
-                    kPack ? make_float4(x[0] + x[1], x[2] + x[3], y[0] + y[1], y[2] + y[3])
-                          : make_float4(x[k], x[2 + k], y[k], y[2 + k]);
+                    kInt ? make_float4(x[0], x[1], y[0], y[1]) : make_float4(x[k], x[OT - 2 + k], y[k], y[OT - 2 + k]);
             }
         }
     __syncthreads();
     constexpr int kQuads = D / 4;
-    const float unit = pow2i(ref - 127);
+    const float unit = pow2i(ref - 127) * (kInt ? 2.0f / 8388608.0f / kKv8FixedScale : 1.0f);  // of the held weights
     auto finish = [&](int r, int d, float total, float4 a) {
         const float inv = total > 0.0f || isnan(total) ? __fdiv_rn(unit, total) : 0.0f;
         const int rho = rho0 + r;
