@@ -49,8 +49,9 @@ constexpr uint32_t kClusterMaxPosBf16 = 1248;  // ... bf16 K/V
 constexpr int kTicketMinChunk = 8;   // pages per guided chunk, at least
 constexpr int kMaxChunks = 8192;     // chunks per plan, at most
 constexpr int kSplitMinBatch = 96;   // from here a step runs as two concurrent half batches
-constexpr int kKv8Ctas = 8;          // 8-bit attention: CTAs per SM that a split call aims at
+constexpr int kKv8Ctas = 5;          // 8-bit attention: resident CTAs per SM, at most
 constexpr int kKv8MinPages = 8;      // ... pages per split, at least (two a warp)
+constexpr int kKv8LongPages = 64;    // ... of a call whose CTAs are not all resident
 constexpr int kKv8TileFloats = 2048; // ... outputs of a row tile, at most
 
 #define CUDA_TRY(expr)                                                                       \
@@ -470,16 +471,13 @@ struct Kv8Pool {
 // has ended.
 struct Kv8Scratch {
     float* part = nullptr;
-    float2* ml = nullptr;
+    float4* ml = nullptr;
     unsigned* arrived = nullptr;
     int max_splits = 0;  // CTAs of a split call, at most
     int alloc(int sms) {
-        // A call is split only while its (sequence, tile, head) items are
-        // fewer than the CTAs that it aims at, and into no more of them than
-        // that plus one per item (kv8_enqueue_attention).
-        max_splits = 2 * kKv8Ctas * sms;
+        max_splits = 4 * kKv8Ctas * sms;  // as kv8_launch_attention splits
         if (cudaMalloc(&part, static_cast<size_t>(max_splits) * kKv8TileFloats * 4) != cudaSuccess ||
-            cudaMalloc(&ml, static_cast<size_t>(max_splits) * 32 * sizeof(float2)) != cudaSuccess ||
+            cudaMalloc(&ml, static_cast<size_t>(max_splits) * 32 * sizeof(float4)) != cudaSuccess ||
             cudaMalloc(&arrived, static_cast<size_t>(max_splits) * 4) != cudaSuccess) {
             cudaGetLastError();
             release();
@@ -552,7 +550,7 @@ template <int D, int NT, int PB, int kStages, int kMode, int kWarps, int kCtas>
 int kv8_launch_attention(const Kv8Pool& c, uint32_t layer, const Kv8Seqs& seqs, const Kv8Attend& a,
                          const Kv8Scratch& w, int sms, cudaStream_t s) {
     constexpr int kRows = kMode == KV8_INT_BF16 || kMode == KV8_INT_F32 ? 4 : 8 * NT;
-    static_assert(kRows * D <= kKv8TileFloats, "a partial result outgrows its scratch");
+    static_assert(kRows * D <= kKv8TileFloats && kCtas <= kKv8Ctas, "a partial result outgrows its scratch");
     Kv8AttnParams p{};
     p.cache = c.view(layer);
     p.seqs = seqs;
@@ -560,7 +558,7 @@ int kv8_launch_attention(const Kv8Pool& c, uint32_t layer, const Kv8Seqs& seqs, 
     p.out = a.out;
     p.q_stride = a.q_stride;
     p.out_stride = a.out_stride;
-    p.group = a.group;
+    p.group = kv8_divisor(static_cast<uint32_t>(a.group));
     p.scale = a.scale * 1.44269504088896340736f;
     p.window = a.window;
     const long long rows = static_cast<long long>(seqs.max_rows) * a.group;
@@ -570,9 +568,15 @@ int kv8_launch_attention(const Kv8Pool& c, uint32_t layer, const Kv8Seqs& seqs, 
     long long span = seqs.max_length;
     if (a.window) span = std::min<long long>(span, static_cast<long long>(a.window) + (kRows - 1) / a.group + kKv8Block);
     const long long pages = std::max<long long>(1, (span + kKv8Block - 1) / kKv8Block);
-    const long long want = static_cast<long long>(kKv8Ctas) * sms;
-    long long splits = items >= want ? 1 : (want + items - 1) / items;
-    splits = std::max<long long>(1, std::min(splits, (pages + kKv8MinPages - 1) / kKv8MinPages));
+    // Splits cost a CTA's start and end (4 to 6 us of latency) each: down to
+    // kKv8MinPages pages while all CTAs are resident at once (8 streams of 8000
+    // positions: 9 splits 21 us, 19 splits 29 us), and into kKv8LongPages or more
+    // up to four times that, where a ragged batch's longest sequence would
+    // otherwise end alone (48 sequences of up to 4096 positions: 4 splits
+    // 51 us, 2 splits 59 us).
+    const long long resident = static_cast<long long>(kCtas) * sms;
+    const long long splits = std::max<long long>(
+        1, std::max(std::min(resident / items, pages / kKv8MinPages), std::min(4 * resident / items, pages / kKv8LongPages)));
     if (items * splits > INT32_MAX) return PHONON_CUDA_CAPACITY;
     if (splits > 1 && items * splits > w.max_splits) return PHONON_CUDA_CAPACITY;
     p.by_heads = kv8_divisor(c.heads);
@@ -598,18 +602,19 @@ template <int D>
 int kv8_attention_rows(const Kv8Pool& c, uint32_t layer, const Kv8Seqs& seqs, const Kv8Attend& a, const Kv8Scratch& w,
                        int sms, cudaStream_t s) {
     const long long rows = static_cast<long long>(seqs.max_rows) * a.group;
-    constexpr int PB = D == 128 ? 1 : 2, PI = D == 128 ? 2 : 4;
+    constexpr int PB = D == 128 ? 1 : 2;
     if (a.bf16) {
-        if (rows <= 4) return kv8_launch_attention<D, 1, PI, 2, KV8_INT_BF16, 4, 3>(c, layer, seqs, a, w, sms, s);
+        if (rows <= 4)
+            return kv8_launch_attention<D, 1, 2, D == 128 ? 2 : 3, KV8_INT_BF16, 4, D == 128 ? 3 : 4>(c, layer, seqs, a, w, sms, s);
         if (rows <= 8) return kv8_launch_attention<D, 1, PB, 3, KV8_HALF_BF16, 4, 4>(c, layer, seqs, a, w, sms, s);
         if (rows <= 16 || D == 128) return kv8_launch_attention<D, 2, 1, 3, KV8_HALF_BF16, 4, 4>(c, layer, seqs, a, w, sms, s);
         if constexpr (D < 128) return kv8_launch_attention<D, 4, 1, 3, KV8_HALF_BF16, 4, 2>(c, layer, seqs, a, w, sms, s);
     }
-    if (rows <= 4) return kv8_launch_attention<D, 1, PI, 2, KV8_INT_F32, 4, 3>(c, layer, seqs, a, w, sms, s);
+    if (rows <= 4)
+        return kv8_launch_attention<D, 1, 2, D == 128 ? 2 : 3, KV8_INT_F32, 4, D == 128 ? 3 : 4>(c, layer, seqs, a, w, sms, s);
     if (rows <= 8) return kv8_launch_attention<D, 1, PB, 3, KV8_HALF_F32, 4, 4>(c, layer, seqs, a, w, sms, s);
-    if (rows <= 16 || D == 128) return kv8_launch_attention<D, 2, 1, 3, KV8_HALF_F32, 4, 3>(c, layer, seqs, a, w, sms, s);
-    if constexpr (D < 128) return kv8_launch_attention<D, 4, 1, 3, KV8_HALF_F32, 4, 2>(c, layer, seqs, a, w, sms, s);
-    return PHONON_CUDA_INVALID_ARGUMENT;
+    if constexpr (D == 128) return kv8_launch_attention<D, 2, 1, 3, KV8_HALF_F32, 4, 3>(c, layer, seqs, a, w, sms, s);
+    else return kv8_launch_attention<D, 2, 2, 2, KV8_HALF_F32, 4, 3>(c, layer, seqs, a, w, sms, s);
 }
 
 int kv8_enqueue_attention(const Kv8Pool& c, uint32_t layer, const Kv8Seqs& seqs, const Kv8Attend& a,

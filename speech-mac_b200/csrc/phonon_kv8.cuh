@@ -424,8 +424,8 @@ __device__ __forceinline__ uint32_t kv8_div(uint32_t n, Kv8Div d) { return d.d =
 // fp32: with s = scale log2(e) 2^eK (q.K) + eV, the weight 2^(s - M) is the
 // softmax weight times the block's value scale, so that O needs no scaling of
 // its own, and the sum of weights takes 2^(s - M - eV). M is the running
-// maximum of s; eV is taken relative to the first visible page's, so that s
-// keeps its precision whatever the values' size. eV spans 112 at most, so
+// maximum of s; eV is taken relative to a warp's first page's, so that s keeps
+// its precision whatever the values' size. eV spans 112 at most, so
 // weights that matter stay inside fp32's range.
 //
 // Up to four rows that share a head (a decode step): 8-bit integer products,
@@ -449,13 +449,13 @@ struct Kv8AttnParams {
     const void* q;
     void* out;
     long long q_stride, out_stride;  // elements between rows; a row is [heads][D]
-    int group;                       // query heads per K/V head
+    Kv8Div group;                    // query heads per K/V head
     float scale;                     // softmax scale times log2(e)
     int window;                      // 0: none
     Kv8Div by_heads, by_splits, by_tiles;  // K/V heads; splits of an item, at most; row tiles of a sequence
     int split_pages;                       // pages of a split
     float* part;                     // [items * splits][rows of a tile][D]
-    float2* part_ml;                 // [items * splits][rows of a tile]: M, sum
+    float4* part_ml;                 // [items * splits][rows of a tile]: M, sum, eV's reference
     unsigned* arrived;               // [items], zero between launches
 };
 
@@ -595,7 +595,7 @@ __global__ void __launch_bounds__(32 * kWarps, kCtas) kv8_attention_kernel(Kv8At
     constexpr int kTurns = 32 / PB, kPageBytes = 2 * kKv8Block * D;
     extern __shared__ __align__(16) uint8_t s_ring[];  // [kWarps][kStages][PB][kPageBytes], then the warps' results
     float(*s_o)[kRows][D] = reinterpret_cast<float(*)[kRows][D]>(s_ring);
-    __shared__ float2 s_ml[kWarps][kRows];
+    __shared__ float4 s_ml[kWarps][kRows];  // M, sum, eV's reference
     __shared__ int s_last;
     pdl_wait();
     pdl_trigger();
@@ -608,11 +608,12 @@ __global__ void __launch_bounds__(32 * kWarps, kCtas) kv8_attention_kernel(Kv8At
     const int tile = static_cast<int>(rest2 - i * p.by_tiles.d);
     const uint32_t item = rest2 * p.by_heads.d + head;
     const Kv8Seq sq = kv8_seq(p.seqs, i);
-    const int rows = sq.count * p.group - tile * kRows;  // rows left from this tile on
+    const int rows = sq.count * static_cast<int>(p.group.d) - tile * kRows;  // rows left from this tile on
     if (rows <= 0) return;
     const int n_rows = min(rows, kRows), rho0 = tile * kRows;
     const int at0 = sq.length - sq.count;  // position of the sequence's first row
-    const int pos_lo = at0 + rho0 / p.group, pos_hi = at0 + (rho0 + n_rows - 1) / p.group;
+    auto token = [&](int rho) { return static_cast<int>(kv8_div(rho, p.group)); };
+    const int pos_lo = at0 + token(rho0), pos_hi = at0 + token(rho0 + n_rows - 1);
     const int key_end = min(pos_hi + 1, sq.length);
     const int page_begin = p.window ? max(pos_lo - p.window + 1, 0) / kKv8Block : 0;
     const int pages = key_end > 0 ? (key_end + kKv8Block - 1) / kKv8Block - page_begin : 0;
@@ -652,17 +653,20 @@ __global__ void __launch_bounds__(32 * kWarps, kCtas) kv8_attention_kernel(Kv8At
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
     };
+    // the rows of q on their way before the page ids are waited for
+    float4 q[NT][KS];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+        const int rho = rho0 + min(kInt ? g >> 1 : n * 8 + g, n_rows - 1), at = token(rho);
+        const size_t row = static_cast<size_t>(sq.row0 + at) * p.q_stride +
+                           static_cast<size_t>(head * p.group.d + rho - at * p.group.d) * D;
+#pragma unroll
+        for (int c = 0; c < KS; ++c) q[n][c] = load_row4<kBf16>(p.q, row + kv8_key_dim<D>(t, c));
+    }
     fetch(0, 0);
 #pragma unroll
     for (int s = 0; s < kStages - 1; ++s) copy(0, s, s);
     fetch(1, kTurns);
-    int ref = 127;  // the value scale that eV is relative to, the same for all warps and splits
-    if (pages > 0) {
-        const int id0 = __ldg(sq.pages + page_begin);
-        if (static_cast<unsigned>(id0) < static_cast<unsigned>(p.cache.pool_pages))
-            ref = __ldg(exps + static_cast<size_t>(id0) * p.cache.heads * 2 + 1);
-    }
-
     // q as B fragments; column g is row g (halves), or byte g % 2 of row g / 2 (qh) and its third byte (ql)
     constexpr int QS = kInt ? D / 32 : KS;  // steps of a score
     uint32_t qh[NT][QS][2], ql[NT][kFine || kMode == KV8_INT_F32 ? QS : 1][2];
@@ -670,15 +674,12 @@ __global__ void __launch_bounds__(32 * kWarps, kCtas) kv8_attention_kernel(Kv8At
     int pos[NT][RT];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-        const int r = kInt ? g >> 1 : n * 8 + g, rho = rho0 + min(r, n_rows - 1);
-        const size_t row = static_cast<size_t>(sq.row0 + rho / p.group) * p.q_stride +
-                           static_cast<size_t>(head * p.group + rho % p.group) * D;
-        float4 v[KS];
+        const int r = kInt ? g >> 1 : n * 8 + g;
+        const float4(&v)[KS] = q[n];
         float amax = 0.0f;
         bool finite = true;
 #pragma unroll
         for (int c = 0; c < KS; ++c) {
-            v[c] = load_row4<kBf16>(p.q, row + kv8_key_dim<D>(t, c));
             finite &= isfinite(v[c].x) & isfinite(v[c].y) & isfinite(v[c].z) & isfinite(v[c].w);
             amax = fmaxf(amax, fmaxf(fmaxf(fabsf(v[c].x), fabsf(v[c].y)), fmaxf(fabsf(v[c].z), fabsf(v[c].w))));
         }
@@ -724,7 +725,7 @@ __global__ void __launch_bounds__(32 * kWarps, kCtas) kv8_attention_kernel(Kv8At
         for (int k = 0; k < RT; ++k) {
             f[n][k] = __shfl_sync(kFull, fr, 8 * t + 4 * k);
             const int lane_row = kInt ? t : n * 8 + 2 * t + k;
-            pos[n][k] = at0 + (rho0 + min(lane_row, n_rows - 1)) / p.group;
+            pos[n][k] = at0 + token(rho0 + min(lane_row, n_rows - 1));
         }
     }
 
@@ -746,6 +747,7 @@ __global__ void __launch_bounds__(32 * kWarps, kCtas) kv8_attention_kernel(Kv8At
     const int from0 = 8 * t + (g >> 1), from1 = from0 + 4;   // lanes with the weights of positions 2t, 2t + 1 of row g / 2
     const uint32_t pick = g & 1 ? 0x6240u : 0x7351u;         // the weight byte that column g multiplies
 
+    const int ref = __shfl_sync(kFull, scales[0], 0) >> 8;  // the value scale that eV is relative to in this warp
     int turn = 0, stage = 0;
     for (int at = first + warp * PB; at < last; at += kStep, ++turn, stage = stage + 1 == kStages ? 0 : stage + 1) {
         if (turn && turn % kTurns == 0) {
@@ -956,7 +958,7 @@ __global__ void __launch_bounds__(32 * kWarps, kCtas) kv8_attention_kernel(Kv8At
 #pragma unroll
             for (int w = 4; w < 32; w <<= 1) l[n][k] += __shfl_xor_sync(kFull, l[n][k], w);
             const int r = kInt ? t : n * 8 + 2 * t + k;
-            if (g == 0) s_ml[warp][r] = make_float2(m[n][k], l[n][k]);
+            if (g == 0) s_ml[warp][r] = make_float4(m[n][k], l[n][k], __int_as_float(ref), 0.0f);
             if (r >= n_rows) continue;
 #pragma unroll
             for (int j = 0; j < D / 32; ++j) {
@@ -968,60 +970,87 @@ __global__ void __launch_bounds__(32 * kWarps, kCtas) kv8_attention_kernel(Kv8At
         }
     __syncthreads();
     constexpr int kQuads = D / 4;
-    const float unit = pow2i(ref - 127) * (kInt ? 2.0f / 8388608.0f / kKv8FixedScale : 1.0f);  // of the held weights
-    auto finish = [&](int r, int d, float total, float4 a) {
-        const float inv = total > 0.0f || isnan(total) ? __fdiv_rn(unit, total) : 0.0f;
-        const int rho = rho0 + r;
-        store_row4<kBf16>(p.out,
-                          static_cast<size_t>(sq.row0 + rho / p.group) * p.out_stride +
-                              static_cast<size_t>(head * p.group + rho % p.group) * D + d,
-                          make_float4(a.x * inv, a.y * inv, a.z * inv, a.w * inv));
+    constexpr float kUnit = kInt ? 2.0f / 8388608.0f / kKv8FixedScale : 1.0f;  // of the held weights
+    struct Share {  // M, sum, reference and four dims of a row
+        float m, l;
+        int ref;
+        float4 a;
     };
-    auto fold = [](float& m, float& l, float4& a, float m2, float l2, float4 b) {
-        const float x = fmaxf(m, m2);
-        const float wa = m == -INFINITY ? 0.0f : ex2(m - x), wb = m2 == -INFINITY ? 0.0f : ex2(m2 - x);
-        m = x;
-        l = l * wa + l2 * wb;
-        a = make_float4(a.x * wa + b.x * wb, a.y * wa + b.y * wb, a.z * wa + b.z * wb, a.w * wa + b.w * wb);
+    auto nothing = [] { return Share{-INFINITY, 0.0f, 127, make_float4(0.0f, 0.0f, 0.0f, 0.0f)}; };
+    auto fold = [](Share& s, float4 ml, float4 b) {
+        if (s.m == -INFINITY && !isnan(s.l)) s.ref = __float_as_int(ml.z);  // nothing yet: as it comes
+        // into s's reference (an exact power of two, and 0 to add where the references agree), then the larger maximum
+        const int shift = __float_as_int(ml.z) - s.ref;
+        const float m2 = ml.x + static_cast<float>(shift), x = fmaxf(s.m, m2);
+        const float wa = s.m == -INFINITY ? 0.0f : ex2(s.m - x), wb = m2 == -INFINITY ? 0.0f : ex2(m2 - x);
+        s.m = x;
+        s.l = s.l * wa + ml.y * (pow2i(min(max(-shift, -126), 126)) * wb);
+        s.a = make_float4(s.a.x * wa + b.x * wb, s.a.y * wa + b.y * wb, s.a.z * wa + b.z * wb, s.a.w * wa + b.w * wb);
+    };
+    auto finish = [&](int r, int d, const Share& s) {
+        const float inv = s.l > 0.0f || isnan(s.l) ? __fdiv_rn(pow2i(s.ref - 127) * kUnit, s.l) : 0.0f;
+        const int rho = rho0 + r, at = token(rho);
+        store_row4<kBf16>(p.out,
+                          static_cast<size_t>(sq.row0 + at) * p.out_stride +
+                              static_cast<size_t>(head * p.group.d + rho - at * p.group.d) * D + d,
+                          make_float4(s.a.x * inv, s.a.y * inv, s.a.z * inv, s.a.w * inv));
     };
     const size_t slot = static_cast<size_t>(item) * p.by_splits.d;
     for (int x = threadIdx.x; x < n_rows * kQuads; x += blockDim.x) {
         const int r = x / kQuads, d = x % kQuads * 4;
-        float mm = -INFINITY, ll = 0.0f;
-        float4 a = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        Share s = nothing();
 #pragma unroll
-        for (int w = 0; w < kWarps; ++w)
-            fold(mm, ll, a, s_ml[w][r].x, s_ml[w][r].y, *reinterpret_cast<const float4*>(&s_o[w][r][d]));
+        for (int w = 0; w < kWarps; ++w) fold(s, s_ml[w][r], *reinterpret_cast<const float4*>(&s_o[w][r][d]));
         if (active == 1) {
-            finish(r, d, ll, a);
+            finish(r, d, s);
         } else {
             const size_t at_part = (slot + split) * kRows + r;
-            *reinterpret_cast<float4*>(p.part + at_part * D + d) = a;
-            if (d == 0) p.part_ml[at_part] = make_float2(mm, ll);
+            *reinterpret_cast<float4*>(p.part + at_part * D + d) = s.a;
+            if (d == 0) p.part_ml[at_part] = make_float4(s.m, s.l, __int_as_float(s.ref), 0.0f);
         }
     }
     if (active == 1) return;
-    __threadfence();
     __syncthreads();
     if (threadIdx.x == 0) {
-        const unsigned n = atomicAdd(p.arrived + item, 1u);
+        unsigned n;  // releases the CTA's partial results (ordered before by the barrier), acquires the others'
+        asm volatile("atom.acq_rel.gpu.global.add.u32 %0, [%1], 1;" : "=r"(n) : "l"(p.arrived + item) : "memory");
         s_last = n + 1 == static_cast<unsigned>(active);
         if (s_last) p.arrived[item] = 0;
     }
     __syncthreads();
     if (!s_last) return;
-    __threadfence();
-    for (int x = threadIdx.x; x < n_rows * kQuads; x += blockDim.x) {
-        const int r = x / kQuads, d = x % kQuads * 4;
-        float mm = -INFINITY, ll = 0.0f;
-        float4 a = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 4
-        for (int k = 0; k < active; ++k) {
-            const size_t at_part = (slot + k) * kRows + r;
-            const float2 ml = __ldcg(p.part_ml + at_part);
-            fold(mm, ll, a, ml.x, ml.y, __ldcg(reinterpret_cast<const float4*>(p.part + at_part * D + d)));
+    // Few rows: the threads share a row's splits, each every subs-th, and the
+    // subs meet in shared memory; four splits are loaded at a time.
+    const int cells = n_rows * kQuads, subs = max(1, min(active, 32 * kWarps / cells));
+    float4* s_a = reinterpret_cast<float4*>(s_ring);  // [subs][cells]; the warps' results have been read
+    for (int x = threadIdx.x; x < cells * subs; x += blockDim.x) {
+        const int sub = x / cells, cell = x - sub * cells, r = cell / kQuads, d = cell % kQuads * 4;
+        Share s = nothing();
+        for (int k0 = sub; k0 < active; k0 += 4 * subs) {
+            float4 ml[4], a[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const size_t at_part = (slot + min(k0 + k * subs, active - 1)) * kRows + r;
+                ml[k] = __ldcg(p.part_ml + at_part);
+                a[k] = __ldcg(reinterpret_cast<const float4*>(p.part + at_part * D + d));
+            }
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                if (k0 + k * subs < active) fold(s, ml[k], a[k]);
         }
-        finish(r, d, ll, a);
+        if (subs == 1) {
+            finish(r, d, s);
+        } else {
+            s_a[x] = s.a;
+            s_a[cells * subs + x] = make_float4(s.m, s.l, __int_as_float(s.ref), 0.0f);
+        }
+    }
+    if (subs == 1) return;
+    __syncthreads();
+    for (int cell = threadIdx.x; cell < cells; cell += blockDim.x) {
+        Share s = nothing();
+        for (int sub = 0; sub < subs; ++sub) fold(s, s_a[cells * subs + sub * cells + cell], s_a[sub * cells + cell]);
+        finish(cell / kQuads, cell % kQuads * 4, s);
     }
 }
 
