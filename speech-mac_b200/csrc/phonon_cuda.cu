@@ -4574,13 +4574,15 @@ namespace {
 
 template <int D, bool kBf16>
 int qk_launch(QkParams& p, bool halves, int sms, cudaStream_t s) {
-    // Warps: a row each, or a slice of its heads while rows are few; at most
-    // 32 warps per SM, each of which computes its frequencies once.
-    const int passes = (p.heads[0] + p.heads[1] + 128 / D - 1) / (128 / D);
-    const long long resident = 32ll * sms;
-    p.slices = static_cast<int>(std::max<long long>(1, std::min<long long>(passes, 2 * resident / p.rows)));
+    // As many warps as are resident at once; a row each in turn, or a slice of
+    // its heads while rows are fewer.
+    constexpr int kAhead = kBf16 ? 4 : 2, kCtas = kBf16 ? 4 : 5, kHeads = 256 / D;
+    const int passes = (p.heads[0] + kHeads - 1) / kHeads + (p.heads[1] + kHeads - 1) / kHeads;
+    const long long resident = 4ll * kCtas * sms;
+    p.slices = static_cast<int>(std::max<long long>(1, std::min<long long>(passes, resident / p.rows)));
     const long long ctas = std::min((static_cast<long long>(p.rows) * p.slices + 3) / 4, resident / 4);
-    CUDA_TRY(launch_pdl(halves ? qk_norm_rope_kernel<D, kBf16, true> : qk_norm_rope_kernel<D, kBf16, false>,
+    CUDA_TRY(launch_pdl(halves ? qk_norm_rope_kernel<D, kBf16, true, kAhead, kCtas>
+                               : qk_norm_rope_kernel<D, kBf16, false, kAhead, kCtas>,
                         dim3(static_cast<unsigned>(ctas)), dim3(128), 0, s, p));
     return PHONON_CUDA_OK;
 }

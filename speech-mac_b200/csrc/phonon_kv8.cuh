@@ -25,6 +25,7 @@
 
 #include "phonon_kernels.cuh"
 
+#include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
 namespace phonon {
@@ -131,9 +132,9 @@ __device__ __forceinline__ float4 load_row4(const void* base, size_t at) {
 template <bool kBf16>
 __device__ __forceinline__ void store_row4(void* base, size_t at, float4 v) {
     if constexpr (kBf16) {
-        const uint2 w = make_uint2(f32_to_bf16(v.x) | static_cast<uint32_t>(f32_to_bf16(v.y)) << 16,
-                                   f32_to_bf16(v.z) | static_cast<uint32_t>(f32_to_bf16(v.w)) << 16);
-        *reinterpret_cast<uint2*>(static_cast<uint16_t*>(base) + at) = w;
+        const __nv_bfloat162 a = __floats2bfloat162_rn(v.x, v.y), b = __floats2bfloat162_rn(v.z, v.w);
+        *reinterpret_cast<uint2*>(static_cast<uint16_t*>(base) + at) =
+            make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
     } else {
         *reinterpret_cast<float4*>(static_cast<float*>(base) + at) = v;
     }

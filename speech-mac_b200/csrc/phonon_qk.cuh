@@ -6,13 +6,17 @@
 //
 // for the rotary_dim / 2 pairs of a head: (2i, 2i + 1), or (i, i + rotary_dim
 // / 2). Bound by the bytes of the rows, read once and written once. A warp
-// takes one row's heads (or a slice of them) in turn: a lane owns 4 dims of a
-// head, so its angles, weights and frequencies stay in registers for all
-// heads of the row, and the two halves of a pair meet by a shuffle.
+// takes rows (or slices of a row's heads, where rows are few) in turn; a lane
+// owns 8 dims of a head in two chunks of 4, both values of every pair among
+// them, so that the rotation needs no exchange and the row's four sines and
+// the weights stay in registers for all its heads. The next kAhead passes, of the next row if need be, are
+// on their way while kAhead are worked on side by side.
 //
-// The angle is reduced in turns: position * theta^(...) / 2 pi and its nearest
-// integer in 64 bits, the remainder (within half a turn) rounded to 32, an
-// error below 2^-25 turns at any position; sine and cosine are sincospif's.
+// The angle in turns is position * theta^(...) / 2 pi modulo 1. The frequency
+// is held as a 64-bit fraction of a turn (rounded once from double), so that
+// the product with the position wraps at whole turns by itself: an error below
+// 2^-33 turns for any position of 31 bits; its upper 32 bits, signed, go to
+// fp32 (2^-25 turns) and sincospif.
 #pragma once
 
 #include "phonon_kv8.cuh"
@@ -31,84 +35,147 @@ struct QkParams {
     double log2_theta;
 };
 
-template <int D, bool kBf16, bool kHalves>
-__global__ void __launch_bounds__(128) qk_norm_rope_kernel(QkParams p) {
-    constexpr int kLanes = D / 4, kPerWarp = 32 / kLanes;  // lanes of a head, heads of a warp pass
-    constexpr int kAngles = kHalves ? 4 : 2;
-    const int lane = threadIdx.x & 31, sub = lane / kLanes, d = (lane % kLanes) * 4;
+template <int D, bool kBf16, bool kHalves, int kAhead, int kCtas>
+__global__ void __launch_bounds__(128, kCtas) qk_norm_rope_kernel(QkParams p) {
+    constexpr int kLanes = D / 8, kPerWarp = 32 / kLanes;  // lanes of a head, heads of a warp pass
+    constexpr int kSize = kBf16 ? 2 : 4;
+    using Raw = std::conditional_t<kBf16, uint2, uint4>;
+    const int lane = threadIdx.x & 31, sub = lane / kLanes, l = lane % kLanes;
+    // dims [chunk[0], + 4) and [chunk[1], + 4): halves are paired across the chunks, neighbours within
     const int half = p.rotary / 2;
-    // the lane's frequencies, in turns per position
-    double turns[kAngles];
+    const bool turned = kHalves && l < p.rotary / 8;
+    const int chunk[2] = {turned ? 4 * l : 8 * l, turned ? half + 4 * l : 8 * l + 4};
+    unsigned long long turns[4];  // per position, 2^-64 of a turn
 #pragma unroll
-    for (int k = 0; k < kAngles; ++k) {
-        const int i = kHalves ? (d < half ? d + k : d + k - half) : d / 2 + k;
-        turns[k] = exp2(-2.0 * i / p.rotary * p.log2_theta) * 0.15915494309189533577;
+    for (int k = 0; k < 4; ++k) {
+        const int i = kHalves ? chunk[0] + k : chunk[0] / 2 + k;
+        turns[k] = __double2ull_rn(exp2(64.0 - 2.0 * i / p.rotary * p.log2_theta) * 0.15915494309189533577);
     }
     pdl_wait();
     pdl_trigger();
-    float4 w[2];
+    float w[2][8];
 #pragma unroll
     for (int s = 0; s < 2; ++s)
-        w[s] = p.weight[s] ? __ldg(reinterpret_cast<const float4*>(p.weight[s] + d)) : make_float4(1.0f, 1.0f, 1.0f, 1.0f);
-    const int total = p.heads[0] + p.heads[1];
-    const int passes = (total + kPerWarp - 1) / kPerWarp, per = (passes + p.slices - 1) / p.slices;
-    const long long items = static_cast<long long>(p.rows) * p.slices;
-    const long long stride = static_cast<long long>(gridDim.x) * (blockDim.x >> 5);
-    for (long long item = static_cast<long long>(blockIdx.x) * (blockDim.x >> 5) + (threadIdx.x >> 5); item < items;
-         item += stride) {
-        const int row = static_cast<int>(item / p.slices), slice = static_cast<int>(item % p.slices);
-        const int position = __ldg(p.positions + row);
-        float sn[kAngles], cs[kAngles];
 #pragma unroll
-        for (int k = 0; k < kAngles; ++k) {
-            const double t = position * turns[k];
-            sincospif(2.0f * static_cast<float>(t - rint(t)), &sn[k], &cs[k]);
+        for (int c = 0; c < 2; ++c) {
+            const float4 v = p.weight[s] ? __ldg(reinterpret_cast<const float4*>(p.weight[s] + chunk[c])) : make_float4(1.0f, 1.0f, 1.0f, 1.0f);
+            w[s][4 * c] = v.x, w[s][4 * c + 1] = v.y, w[s][4 * c + 2] = v.z, w[s][4 * c + 3] = v.w;
         }
-        bool finite = true;
-        for (int u = slice * per; u < min(passes, (slice + 1) * per); ++u) {
-            const int h = u * kPerWarp + sub;
-            const bool live = h < total;
-            const int side = live && h >= p.heads[0] ? 1 : 0;
-            const size_t at = static_cast<size_t>(side ? h - p.heads[0] : h) * D + d;
-            float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            if (live) x = load_row4<kBf16>(p.in[side], row * static_cast<size_t>(p.in_stride[side]) + at);
-            // every lane takes part in the shuffles: a pass can hold normed and plain heads
-            float sq = fmaf(x.x, x.x, fmaf(x.y, x.y, fmaf(x.z, x.z, x.w * x.w)));
+    // passes of the queries, then of the keys: a pass has one side
+    const int pass_q = (p.heads[0] + kPerWarp - 1) / kPerWarp, passes = pass_q + (p.heads[1] + kPerWarp - 1) / kPerWarp;
+    const int per = (passes + p.slices - 1) / p.slices;
+    const int items = p.rows * p.slices, stride = gridDim.x * (blockDim.x >> 5);
+    int item = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
+    if (item >= items) return;  // the whole warp
+    Raw raw[kAhead][2];
+    // the passes [u, min(u + kAhead, the side's end, stop)) of a row
+    auto load = [&](int row, int u, int stop) {
+        const bool side = u >= pass_q;
+        const int h0 = (u - (side ? pass_q : 0)) * kPerWarp + sub, heads = side ? p.heads[1] : p.heads[0];
+        const char* in = static_cast<const char*>(side ? p.in[1] : p.in[0]) +
+                         row * (side ? p.in_stride[1] : p.in_stride[0]) * kSize + h0 * (D * kSize);
 #pragma unroll
-            for (int o = kLanes / 2; o > 0; o >>= 1) sq += __shfl_xor_sync(kFull, sq, o);
-            if (p.weight[side]) {
-                const float r = __fdiv_rn(1.0f, __fsqrt_rn(fmaf(sq, 1.0f / D, p.epsilon)));
-                const float4 v = side ? w[1] : w[0];
-                x = make_float4(x.x * r * v.x, x.y * r * v.y, x.z * r * v.z, x.w * r * v.w);
+        for (int a = 0; a < kAhead; ++a)
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                raw[a][c] = Raw{};
+                if (u + a < stop && h0 + a * kPerWarp < heads)
+                    raw[a][c] = __ldg(reinterpret_cast<const Raw*>(in + a * (kPerWarp * D * kSize) + chunk[c] * kSize));
             }
-            if constexpr (kHalves) {
-                const int from = d < half ? lane + half / 4 : lane - half / 4;
-                const float4 o = make_float4(__shfl_sync(kFull, x.x, from), __shfl_sync(kFull, x.y, from),
-                                             __shfl_sync(kFull, x.z, from), __shfl_sync(kFull, x.w, from));
-                if (d < half)
-                    x = make_float4(x.x * cs[0] - o.x * sn[0], x.y * cs[1] - o.y * sn[1], x.z * cs[2] - o.z * sn[2],
-                                    x.w * cs[3] - o.w * sn[3]);
-                else if (d < p.rotary)
-                    x = make_float4(o.x * sn[0] + x.x * cs[0], o.y * sn[1] + x.y * cs[1], o.z * sn[2] + x.z * cs[2],
-                                    o.w * sn[3] + x.w * cs[3]);
-            } else {
-                if (d < p.rotary) {
-                    const float a = x.x, b = x.y;
-                    x.x = a * cs[0] - b * sn[0];
-                    x.y = a * sn[0] + b * cs[0];
-                }
-                if (d + 2 < p.rotary) {
-                    const float a = x.z, b = x.w;
-                    x.z = a * cs[1] - b * sn[1];
-                    x.w = a * sn[1] + b * cs[1];
-                }
-            }
-            if (live) {
-                finite &= isfinite(x.x) & isfinite(x.y) & isfinite(x.z) & isfinite(x.w);
-                store_row4<kBf16>(p.out[side], row * static_cast<size_t>(p.out_stride[side]) + at, x);
-            }
+    };
+    auto end_of = [&](int u, int stop) { return min(min(u + kAhead, stop), u < pass_q ? pass_q : passes); };
+    int row = item / p.slices, first = (item - row * p.slices) * per;
+    int position = __ldg(p.positions + row);
+    if (first < passes) load(row, first, min(passes, first + per));
+    while (true) {
+        const int stop = min(passes, first + per);
+        const int next = item + stride, next_row = next < items ? next / p.slices : row;
+        const int next_first = (next - next_row * p.slices) * per;
+        const int next_position = __ldg(p.positions + next_row);
+        float sn[8], cs[8];  // of every dim, with the sign of its own term: a cos - b sin, a sin + b cos
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const unsigned long long t = static_cast<unsigned long long>(static_cast<long long>(position)) * turns[k];
+            float s, c;
+            sincospif(static_cast<float>(static_cast<int>(t >> 32)) * 0x1p-31f, &s, &c);
+            if (kHalves ? !turned : chunk[0] + 2 * k >= p.rotary) s = 0.0f, c = 1.0f;
+            const int one = kHalves ? k : 2 * k, two = kHalves ? k + 4 : 2 * k + 1;
+            sn[one] = -s;
+            sn[two] = s;
+            cs[one] = cs[two] = c;
         }
-        if (p.status && !__all_sync(kFull, finite) && lane == 0) flag_nonfinite(p.status, row);
+        float finite = 0.0f;  // NaN once an output is not
+        int u = first;
+#pragma unroll
+        for (int side = 0; side < 2; ++side) {
+            const int side_end = min(stop, side ? passes : pass_q), heads = p.heads[side];
+            if (u >= side_end) continue;
+            constexpr int kOther = kHalves ? 4 : 1;  // a dim's pair: k ^ kOther
+            float a0[8], a1[8];                      // y = r (a0 x + a1 other)
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                a0[k] = cs[k] * w[side][k];
+                a1[k] = sn[k] * w[side][k ^ kOther];
+            }
+            char* out = static_cast<char*>(p.out[side]) + row * p.out_stride[side] * kSize;
+            for (; u < side_end; u += kAhead) {
+                float x[kAhead][8], sq[kAhead];
+#pragma unroll
+                for (int a = 0; a < kAhead; ++a) {
+                    sq[a] = 0.0f;
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) {
+                        const uint32_t* words = reinterpret_cast<const uint32_t*>(&raw[a][k / 4]);
+                        x[a][k] = __uint_as_float(!kBf16 ? words[k % 4] : k % 2 ? words[k % 4 / 2] & 0xffff0000u : words[k % 4 / 2] << 16);
+                        sq[a] = fmaf(x[a][k], x[a][k], sq[a]);
+                    }
+                }
+                const int after = end_of(u, stop);
+                if (after < stop) load(row, after, stop);
+                else if (next < items && next_first < passes) load(next_row, next_first, min(passes, next_first + per));
+                // every lane takes part in the shuffles
+#pragma unroll
+                for (int o = kLanes / 2; o > 0; o >>= 1)
+#pragma unroll
+                    for (int a = 0; a < kAhead; ++a) sq[a] += __shfl_xor_sync(kFull, sq[a], o);
+                const int h0 = (u - (side ? pass_q : 0)) * kPerWarp + sub;
+#pragma unroll
+                for (int a = 0; a < kAhead; ++a) {
+                    const float r = p.weight[side] ? rsqrtf(fmaf(sq[a], 1.0f / D, p.epsilon)) : 1.0f;
+                    float y[8];
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) x[a][k] *= r;
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) {
+                        y[k] = fmaf(x[a][k], a0[k], x[a][k ^ kOther] * a1[k]);
+                        finite = fmaf(y[k], 0.0f, finite);  // (0 where the pass has no head: its x is 0)
+                    }
+                    Raw packed[2];
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) {
+                        uint32_t* words = reinterpret_cast<uint32_t*>(&packed[k / 4]);
+                        if constexpr (!kBf16) {
+                            words[k % 4] = __float_as_uint(y[k]);
+                        } else if (k % 2 == 0) {
+                            const __nv_bfloat162 b = __floats2bfloat162_rn(y[k], y[k + 1]);
+                            words[k % 4 / 2] = *reinterpret_cast<const uint32_t*>(&b);
+                        }
+                    }
+                    if (u + a < side_end && h0 + a * kPerWarp < heads) {
+                        char* to = out + (h0 + a * kPerWarp) * (D * kSize);
+                        *reinterpret_cast<Raw*>(to + chunk[0] * kSize) = packed[0];
+                        *reinterpret_cast<Raw*>(to + chunk[1] * kSize) = packed[1];
+                    }
+                }
+            }
+            u = side_end;
+        }
+        if (p.status && !__all_sync(kFull, finite == 0.0f) && lane == 0) flag_nonfinite(p.status, row);
+        if (next >= items) break;
+        item = next;
+        row = next_row;
+        first = next_first;
+        position = next_position;
     }
 }
 
