@@ -500,22 +500,39 @@ struct Kv8Scratch {
 // Blocks that `rows` consecutive positions touch, at most.
 int kv8_blocks(int rows) { return (rows + kKv8Block - 2) / kKv8Block + 1; }
 
+Kv8Div kv8_divisor(uint32_t d) {
+    uint32_t log = 0;
+    while ((1ull << log) < d) ++log;
+    // ceil(2^(31 + log) / d) < 2^32, exact for n < 2^31
+    return Kv8Div{d, d == 1 ? 0 : static_cast<uint32_t>(((1ull << (31 + log)) + d - 1) / d), log ? log - 1 : 0};
+}
+
+// `lanes` threads for each (sequence, block, head, keys or values).
 template <typename Params, typename Kernel>
-int kv8_launch_rows(Kernel kernel, const Params& p, cudaStream_t s) {
-    const long long warps = static_cast<long long>(p.seqs.n) * p.blocks * p.cache.heads * 2;
-    const long long ctas = (warps + 3) / 4;
-    if (ctas > INT32_MAX) return PHONON_CUDA_CAPACITY;
+int kv8_launch_rows(Kernel kernel, const Params& p, int lanes, cudaStream_t s) {
+    const long long items = static_cast<long long>(p.seqs.n) * p.blocks * p.cache.heads * 2;
+    const long long ctas = (items * lanes + 127) / 128;
+    if (items >= (1ll << 31) || ctas * 128 >= (1ll << 32)) return PHONON_CUDA_CAPACITY;  // the kernels' 32-bit indices
     CUDA_TRY(launch_pdl(kernel, dim3(static_cast<unsigned>(ctas)), dim3(128), 0, s, p));
     return PHONON_CUDA_OK;
 }
 
 int kv8_enqueue_append(const Kv8Pool& c, uint32_t layer, const Kv8Seqs& seqs, bool bf16, const void* keys,
                        const void* values, long long stride, cudaStream_t s) {
-    Kv8AppendParams p{c.view(layer), seqs, {keys, values}, stride, kv8_blocks(seqs.max_rows)};
+    Kv8AppendParams p{c.view(layer), seqs, {keys, values}, stride, kv8_blocks(seqs.max_rows), kv8_divisor(c.heads),
+                      kv8_divisor(static_cast<uint32_t>(kv8_blocks(seqs.max_rows)))};
+    if (seqs.max_rows == 1) {
+        const int lanes = static_cast<int>(c.dim / 4);
+        switch (c.dim) {
+            case 32: return kv8_launch_rows(bf16 ? kv8_append_one_kernel<32, true> : kv8_append_one_kernel<32, false>, p, lanes, s);
+            case 64: return kv8_launch_rows(bf16 ? kv8_append_one_kernel<64, true> : kv8_append_one_kernel<64, false>, p, lanes, s);
+            default: return kv8_launch_rows(bf16 ? kv8_append_one_kernel<128, true> : kv8_append_one_kernel<128, false>, p, lanes, s);
+        }
+    }
     switch (c.dim) {
-        case 32: return kv8_launch_rows(bf16 ? kv8_append_kernel<32, true> : kv8_append_kernel<32, false>, p, s);
-        case 64: return kv8_launch_rows(bf16 ? kv8_append_kernel<64, true> : kv8_append_kernel<64, false>, p, s);
-        default: return kv8_launch_rows(bf16 ? kv8_append_kernel<128, true> : kv8_append_kernel<128, false>, p, s);
+        case 32: return kv8_launch_rows(bf16 ? kv8_append_kernel<32, true> : kv8_append_kernel<32, false>, p, 32, s);
+        case 64: return kv8_launch_rows(bf16 ? kv8_append_kernel<64, true> : kv8_append_kernel<64, false>, p, 32, s);
+        default: return kv8_launch_rows(bf16 ? kv8_append_kernel<128, true> : kv8_append_kernel<128, false>, p, 32, s);
     }
 }
 
@@ -523,9 +540,9 @@ int kv8_enqueue_read(const Kv8Pool& c, uint32_t layer, const Kv8Seqs& seqs, bool
                      long long stride, cudaStream_t s) {
     Kv8ReadParams p{c.view(layer), seqs, {keys, values}, stride, kv8_blocks(seqs.max_rows)};
     switch (c.dim) {
-        case 32: return kv8_launch_rows(bf16 ? kv8_read_kernel<32, true> : kv8_read_kernel<32, false>, p, s);
-        case 64: return kv8_launch_rows(bf16 ? kv8_read_kernel<64, true> : kv8_read_kernel<64, false>, p, s);
-        default: return kv8_launch_rows(bf16 ? kv8_read_kernel<128, true> : kv8_read_kernel<128, false>, p, s);
+        case 32: return kv8_launch_rows(bf16 ? kv8_read_kernel<32, true> : kv8_read_kernel<32, false>, p, 32, s);
+        case 64: return kv8_launch_rows(bf16 ? kv8_read_kernel<64, true> : kv8_read_kernel<64, false>, p, 32, s);
+        default: return kv8_launch_rows(bf16 ? kv8_read_kernel<128, true> : kv8_read_kernel<128, false>, p, 32, s);
     }
 }
 
@@ -538,13 +555,6 @@ struct Kv8Attend {
     int window;
     bool bf16;
 };
-
-Kv8Div kv8_divisor(uint32_t d) {
-    uint32_t log = 0;
-    while ((1ull << log) < d) ++log;
-    // ceil(2^(31 + log) / d) < 2^32, exact for n < 2^31
-    return Kv8Div{d, d == 1 ? 0 : static_cast<uint32_t>(((1ull << (31 + log)) + d - 1) / d), log ? log - 1 : 0};
-}
 
 template <int D, int NT, int PB, int kStages, int kMode, int kWarps, int kCtas>
 int kv8_launch_attention(const Kv8Pool& c, uint32_t layer, const Kv8Seqs& seqs, const Kv8Attend& a,

@@ -109,13 +109,23 @@ __device__ __forceinline__ int kv8_exponent(float amax) {
     return min(max(e, kKv8MinExp), kKv8MaxExp);
 }
 
+// The nearest integer to x / 2^e (ties to even) in the low byte: adding 1.5 *
+// 2^23 rounds the exact quotient to an integer. |x| <= 127 * 2^e.
 __device__ __forceinline__ uint32_t kv8_code(float x, float inverse) {
-    return static_cast<uint32_t>(min(max(__float2int_rn(__fmul_rn(x, inverse)), -127), 127)) & 0xffu;
+    return __float_as_uint(__fmaf_rn(x, inverse, 12582912.0f));
 }
 
-// A held byte of a scale 2^k times smaller (shrink = 2^-k) in the new one.
-__device__ __forceinline__ uint32_t kv8_shrink(uint32_t byte, float shrink) {
-    return static_cast<uint32_t>(__float2int_rn(__fmul_rn(static_cast<float>(static_cast<int8_t>(byte)), shrink))) & 0xffu;
+// The low bytes of four words.
+__device__ __forceinline__ uint32_t kv8_pack(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
+}
+
+// Four held bytes of a scale 2^k times smaller (shrink = 2^-k) in the new one.
+__device__ __forceinline__ uint32_t kv8_shrink(uint32_t w, float shrink) {
+    uint32_t r[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) r[k] = kv8_code(static_cast<float>(static_cast<int8_t>(w >> (8 * k))), shrink);
+    return kv8_pack(r[0], r[1], r[2], r[3]);
 }
 
 template <bool kBf16>
@@ -141,16 +151,41 @@ __device__ __forceinline__ void store_row4(void* base, size_t at, float4 v) {
 }
 
 // ------------------------------------------------------------------- append
+// n / d and n % d of a launch's block index for a d that the host knows:
+// multiply and shift (Granlund and Montgomery's division by invariants, for
+// n < 2^31, where the multiplier fits 32 bits).
+struct Kv8Div {
+    uint32_t d, mul, shift;
+};
+
+__device__ __forceinline__ uint32_t kv8_div(uint32_t n, Kv8Div d) { return d.d == 1 ? n : __umulhi(n, d.mul) >> d.shift; }
+
 struct Kv8AppendParams {
     Kv8View cache;
     Kv8Seqs seqs;
     const void* rows[2];  // keys, values: [rows][heads][D], rows `stride` elements apart
     long long stride;
     int blocks;  // blocks of a sequence that its rows can touch, at most
+    Kv8Div by_heads, by_blocks;
 };
 
 // Position of lane 4g + t's k-th byte of a value word (the layout above).
 __device__ __forceinline__ int kv8_value_pos(int t, int k) { return 2 * t + (k & 1) + 8 * (k >> 1); }
+
+// The values to quantise: non-finite ones count as 0, and none exceeds the
+// largest that can be held.
+__device__ __forceinline__ float4 kv8_sane(float4 v) {
+    constexpr float kMost = 127.0f * 18446744073709551616.0f;  // 127 * 2^kKv8MaxExp
+    float* f = &v.x;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) f[k] = isfinite(f[k]) ? fminf(fmaxf(f[k], -kMost), kMost) : 0.0f;
+    return v;
+}
+
+__device__ __forceinline__ float kv8_amax(float4 v) { return fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w))); }
+
+// Above this the values are looked at one by one (kv8_sane).
+constexpr float kKv8Tame = 1e20f;
 
 // One warp writes one block's keys (which = 0) or values (1): the new rows'
 // maximum, the scale, then the integers. A block's bytes are all owned by one
@@ -164,15 +199,12 @@ __global__ void __launch_bounds__(128) kv8_append_kernel(Kv8AppendParams p) {
     pdl_wait();
     pdl_trigger();
     const int lane = threadIdx.x & 31;
-    const long long item = (static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x) >> 5;
-    const int which = static_cast<int>(item & 1);
-    long long rest = item >> 1;
-    const int head = static_cast<int>(rest % p.cache.heads);
-    rest /= p.cache.heads;
-    const int bi = static_cast<int>(rest % p.blocks);
-    rest /= p.blocks;
-    if (rest >= p.seqs.n) return;
-    const int i = static_cast<int>(rest);
+    const uint32_t item = (blockIdx.x * blockDim.x + threadIdx.x) >> 5;
+    const int which = item & 1;
+    const uint32_t rest = kv8_div(item >> 1, p.by_heads);
+    const int head = static_cast<int>((item >> 1) - rest * p.by_heads.d);
+    const int i = static_cast<int>(kv8_div(rest, p.by_blocks)), bi = static_cast<int>(rest - i * p.by_blocks.d);
+    if (i >= p.seqs.n) return;
     const Kv8Seq q = kv8_seq(p.seqs, i);
     const int start = max(q.length - q.count, 0);  // rows before position 0 go nowhere
     const int row0 = q.row0 + q.count - q.length;  // row of position 0
@@ -180,46 +212,43 @@ __global__ void __launch_bounds__(128) kv8_append_kernel(Kv8AppendParams p) {
     const int p0 = block * kKv8Block;
     if (p0 >= q.length || q.count == 0) return;
     const int page = __ldg(q.pages + block);
+    const int lo = max(start - p0, 0), hi = min(q.length - p0, kKv8Block);  // new slots [lo, hi), kept [0, lo)
+    const void* src = p.rows[which];
+    const int g = lane >> 2, t = lane & 3;
+
+    float4 x[kPasses];  // keys: rows of the passes; values: positions k of chunk j at 4j + k
+    float amax = 0.0f, clean = 0.0f;
+#pragma unroll
+    for (int a = 0; a < kPasses; ++a) {
+        const int slot = which == 0 ? a * kRowsPerPass + lane / kLanesPerRow : kv8_value_pos(t, a & 3);
+        const int dim = which == 0 ? (lane % kLanesPerRow) * 4 : 32 * (a >> 2) + 4 * g;
+        x[a] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (slot >= lo && slot < hi)
+            x[a] = load_row4<kBf16>(src, static_cast<size_t>(row0 + p0 + slot) * p.stride + head * D + dim);
+    }
     if (static_cast<unsigned>(page) >= static_cast<unsigned>(p.cache.pool_pages)) {
         if (lane == 0) kv8_flag(p.seqs, i, kStatusInvalid);
         return;
     }
-    const int lo = max(start - p0, 0), hi = min(q.length - p0, kKv8Block);  // new slots [lo, hi), kept [0, lo)
     uint8_t* ep = kv8_exp(p.cache, page, head) + which;
     const int held = lo > 0 ? *ep - 127 : kKv8MinExp;
     uint8_t* dst = kv8_block<D>(p.cache, page, head, which);
-    const void* src = p.rows[which];
-
-    float4 x[16 * D / 128];
-    float amax = 0.0f;
-    bool finite = true;
-    auto take = [&](float4& v, int slot, int dim) {
-        v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        if (slot < lo || slot >= hi) return;
-        v = load_row4<kBf16>(src, static_cast<size_t>(row0 + p0 + slot) * p.stride + head * D + dim);
-        float* f = &v.x;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            if (!isfinite(f[k])) {  // held as 0 and flagged
-                finite = false;
-                f[k] = 0.0f;
-            }
-            amax = fmaxf(amax, fabsf(f[k]));
+    for (int a = 0; a < kPasses; ++a) {
+        amax = fmaxf(amax, kv8_amax(x[a]));
+        clean = fmaf(x[a].x, 0.0f, fmaf(x[a].y, 0.0f, fmaf(x[a].z, 0.0f, fmaf(x[a].w, 0.0f, clean))));  // NaN once a value is not finite
+    }
+    if (!__all_sync(kFull, amax < kKv8Tame && clean == 0.0f)) {
+        if (!__all_sync(kFull, clean == 0.0f) && lane == 0) kv8_flag(p.seqs, i, kStatusNonFinite);
+        amax = 0.0f;
+#pragma unroll
+        for (int a = 0; a < kPasses; ++a) {
+            x[a] = kv8_sane(x[a]);
+            amax = fmaxf(amax, kv8_amax(x[a]));
         }
-    };
-    const int g = lane >> 2, t = lane & 3;
-    if (which == 0) {
-#pragma unroll
-        for (int a = 0; a < kPasses; ++a) take(x[a], a * kRowsPerPass + lane / kLanesPerRow, (lane % kLanesPerRow) * 4);
-    } else {
-#pragma unroll
-        for (int j = 0; j < kChunks; ++j)
-#pragma unroll
-            for (int k = 0; k < 4; ++k) take(x[j * 4 + k], kv8_value_pos(t, k), 32 * j + 4 * g);
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(kFull, amax, o));
-    if (!__all_sync(kFull, finite) && lane == 0) kv8_flag(p.seqs, i, kStatusNonFinite);
     const int e = max(kv8_exponent(amax), held);
     const float inverse = pow2i(-e), shrink = pow2i(held - e);
     const bool raised = lo > 0 && e > held;
@@ -230,49 +259,102 @@ __global__ void __launch_bounds__(128) kv8_append_kernel(Kv8AppendParams p) {
         for (int a = 0; a < kPasses; ++a) {
             const int slot = a * kRowsPerPass + lane / kLanesPerRow;
             uint32_t* at = reinterpret_cast<uint32_t*>(dst + slot * D) + lane % kLanesPerRow;
-            if (slot >= lo && slot < hi) {
-                *at = kv8_code(x[a].x, inverse) | kv8_code(x[a].y, inverse) << 8 | kv8_code(x[a].z, inverse) << 16 |
-                      kv8_code(x[a].w, inverse) << 24;
-            } else if (raised && slot < lo) {
-                const uint32_t w = *at;
-                uint32_t r = 0;
-#pragma unroll
-                for (int k = 0; k < 4; ++k) r |= kv8_shrink((w >> (8 * k)) & 0xffu, shrink) << (8 * k);
-                *at = r;
-            }
+            if (slot >= lo && slot < hi)
+                *at = kv8_pack(kv8_code(x[a].x, inverse), kv8_code(x[a].y, inverse), kv8_code(x[a].z, inverse),
+                               kv8_code(x[a].w, inverse));
         }
+        if (raised)
+            for (int slot = lane / kLanesPerRow; slot < lo; slot += kRowsPerPass) {
+                uint32_t* at = reinterpret_cast<uint32_t*>(dst + slot * D) + lane % kLanesPerRow;
+                *at = kv8_shrink(*at, shrink);
+            }
     } else {
-        bool any_new = false, any_old = false, any_raise = false;
+        uint32_t fresh = 0;  // the new positions' bytes of a word
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
             const int slot = kv8_value_pos(t, k);
-            const bool fresh = slot >= lo && slot < hi;
-            any_new |= fresh;
-            any_old |= !fresh;
-            any_raise |= raised && slot < lo;
+            if (slot >= lo && slot < hi) fresh |= 0xffu << (8 * k);
         }
-        if (!any_new && !any_raise) return;
+        if (fresh == 0 && !raised) return;
 #pragma unroll
         for (int j = 0; j < kChunks; ++j) {
             uint4* at = reinterpret_cast<uint4*>(dst + j * 512) + lane;
-            uint4 w4 = make_uint4(0, 0, 0, 0);
-            if (any_old) w4 = *at;
-            uint32_t* w = &w4.x;
+            uint4 old = make_uint4(0, 0, 0, 0);
+            if (fresh != 0xffffffffu) old = *at;
+            uint32_t* w = &old.x;
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const int slot = kv8_value_pos(t, k);
-                const float* f = &x[j * 4 + k].x;
-#pragma unroll
-                for (int d = 0; d < 4; ++d) {
-                    const uint32_t old = (w[d] >> (8 * k)) & 0xffu;
-                    uint32_t b = old;
-                    if (slot >= lo && slot < hi) b = kv8_code(f[d], inverse);
-                    else if (raised && slot < lo) b = kv8_shrink(old, shrink);
-                    w[d] = (w[d] & ~(0xffu << (8 * k))) | (b << (8 * k));
-                }
+            for (int d = 0; d < 4; ++d) {
+                const float* f[4] = {&x[4 * j].x, &x[4 * j + 1].x, &x[4 * j + 2].x, &x[4 * j + 3].x};
+                const uint32_t mine = kv8_pack(kv8_code(f[0][d], inverse), kv8_code(f[1][d], inverse),
+                                               kv8_code(f[2][d], inverse), kv8_code(f[3][d], inverse));
+                // (bytes of positions behind the rows are shrunk too: they hold nothing)
+                if (raised) w[d] = kv8_shrink(w[d], shrink);
+                w[d] = (mine & fresh) | (w[d] & ~fresh);
             }
-            *at = w4;
+            *at = old;
         }
+    }
+}
+
+// One new row a sequence (a decode step): D / 4 lanes per (sequence, head, keys
+// or values), 4 dims a lane; nothing of the block is read unless the scale
+// rises.
+template <int D, bool kBf16>
+__global__ void __launch_bounds__(128) kv8_append_one_kernel(Kv8AppendParams p) {
+    constexpr int kLanes = D / 4;
+    pdl_wait();
+    pdl_trigger();
+    const int lane = threadIdx.x & 31, l = lane % kLanes;
+    const uint32_t item = (blockIdx.x * blockDim.x + threadIdx.x) / kLanes;
+    const int which = item & 1;
+    const uint32_t rest = kv8_div(item >> 1, p.by_heads);
+    const int head = static_cast<int>((item >> 1) - rest * p.by_heads.d), i = static_cast<int>(min(rest, p.seqs.n - 1u));
+    const Kv8Seq q = kv8_seq(p.seqs, i);
+    const bool real = rest < static_cast<uint32_t>(p.seqs.n) && q.count == 1 && q.length > 0;
+    const int position = max(q.length - 1, 0), slot = position % kKv8Block;
+    int page = -1;
+    float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    if (real) {
+        page = __ldg(q.pages + position / kKv8Block);
+        x = load_row4<kBf16>(p.rows[which], static_cast<size_t>(q.row0) * p.stride + head * D + 4 * l);
+        if (static_cast<unsigned>(page) >= static_cast<unsigned>(p.cache.pool_pages)) {
+            if (l == 0) kv8_flag(p.seqs, i, kStatusInvalid);
+            page = -1;
+        }
+    }
+    uint8_t* ep = kv8_exp(p.cache, max(page, 0), head) + which;
+    const int held = page >= 0 && slot > 0 ? *ep - 127 : kKv8MinExp;
+    float amax = kv8_amax(x);
+    const bool finite = isfinite(x.x) && isfinite(x.y) && isfinite(x.z) && isfinite(x.w);
+    if (!finite && page >= 0) kv8_flag(p.seqs, i, kStatusNonFinite);
+    if (!finite || amax >= kKv8Tame) {
+        x = kv8_sane(x);
+        amax = kv8_amax(x);
+    }
+#pragma unroll
+    for (int o = kLanes / 2; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(kFull, amax, o));
+    if (page < 0) return;
+    const int e = max(kv8_exponent(amax), held);
+    const float inverse = pow2i(-e), shrink = pow2i(held - e);
+    if (l == 0) *ep = static_cast<uint8_t>(e + 127);
+    const uint32_t c[4] = {kv8_code(x.x, inverse), kv8_code(x.y, inverse), kv8_code(x.z, inverse), kv8_code(x.w, inverse)};
+    uint8_t* dst = kv8_block<D>(p.cache, page, head, which);
+    if (which == 0) {
+        uint32_t* at = reinterpret_cast<uint32_t*>(dst) + l;
+        if (slot > 0 && e > held)
+            for (int s = 0; s < slot; ++s) at[s * (D / 4)] = kv8_shrink(at[s * (D / 4)], shrink);
+        at[slot * (D / 4)] = kv8_pack(c[0], c[1], c[2], c[3]);
+    } else {
+        // dims 4l.. are chunk l / 8, lanes 4 (l % 8) + t: four words of each t
+        uint8_t* words = dst + (l >> 3) * 512 + (l & 7) * 64;
+        if (slot > 0 && e > held)
+            for (int w = 0; w < 16; ++w) {
+                uint32_t* at = reinterpret_cast<uint32_t*>(words) + w;
+                *at = kv8_shrink(*at, shrink);
+            }
+        const int t = (slot & 7) >> 1, k = (slot & 1) + 2 * (slot >> 3);
+#pragma unroll
+        for (int d = 0; d < 4; ++d) words[t * 16 + d * 4 + k] = static_cast<uint8_t>(c[d]);
     }
 }
 
@@ -403,15 +485,6 @@ __global__ void __launch_bounds__(128) kv8_read_kernel(Kv8ReadParams p) {
             }
     }
 }
-
-// n / d and n % d of a launch's block index for a d that the host knows:
-// multiply and shift (Granlund and Montgomery's division by invariants, for
-// n < 2^31, where the multiplier fits 32 bits).
-struct Kv8Div {
-    uint32_t d, mul, shift;
-};
-
-__device__ __forceinline__ uint32_t kv8_div(uint32_t n, Kv8Div d) { return d.d == 1 ? n : __umulhi(n, d.mul) >> d.shift; }
 
 // ---------------------------------------------------------------- attention
 // out[r] = sum_k softmax_k(scale q_r . K_k) V_k over the positions k that row
