@@ -551,7 +551,7 @@ struct Kv8Attend {
     void* out;
     long long q_stride, out_stride;
     int group;
-    float scale;
+    double scale;
     int window;
     bool bf16;
 };
@@ -569,7 +569,9 @@ int kv8_launch_attention(const Kv8Pool& c, uint32_t layer, const Kv8Seqs& seqs, 
     p.q_stride = a.q_stride;
     p.out_stride = a.out_stride;
     p.group = kv8_divisor(static_cast<uint32_t>(a.group));
-    p.scale = a.scale * 1.44269504088896340736f;
+    const double scale = a.scale * 1.4426950408889634074;
+    p.scale = static_cast<float>(scale);
+    p.scale_low = static_cast<float>(scale - p.scale);
     p.window = a.window;
     const long long rows = static_cast<long long>(seqs.max_rows) * a.group;
     const long long tiles = (rows + kRows - 1) / kRows;
@@ -1199,7 +1201,7 @@ int enqueue_kv8(PhononCuda* c, const Batch& b, int l) {
     }
     LaunchScope ls(c, PHONON_CUDA_K_ATTENTION, b.keys * 2.0 * kWidth + 2.0 * act, s);
     return kv8_enqueue_attention(c->kv8, static_cast<uint32_t>(l), seqs,
-                                 Kv8Attend{b.lane->q, b.lane->a, kWidth, kWidth, 1, 0.125f, 0, false}, b.lane->kv8,
+                                 Kv8Attend{b.lane->q, b.lane->a, kWidth, kWidth, 1, 0.125, 0, false}, b.lane->kv8,
                                  c->sms, s);
 }
 
@@ -4567,7 +4569,7 @@ int phonon_cuda_kv8_attention_device(PhononCudaKv8* c, uint32_t layer, const Pho
     a.q = query->q;
     a.out = query->out;
     a.group = static_cast<int>(query->heads / c->pool.heads);
-    a.scale = query->scale > 0.0f ? query->scale : static_cast<float>(1.0 / std::sqrt(static_cast<double>(c->pool.dim)));
+    a.scale = query->scale > 0.0f ? static_cast<double>(query->scale) : 1.0 / std::sqrt(static_cast<double>(c->pool.dim));
     a.window = static_cast<int>(query->window);
     a.bf16 = query->type == PHONON_CUDA_ROWS_BF16;
     if (static_cast<long long>(seqs.max_rows) * a.group > (1 << 30)) return PHONON_CUDA_CAPACITY;

@@ -503,13 +503,13 @@ __global__ void __launch_bounds__(128) kv8_read_kernel(Kv8ReadParams p) {
 // weights that matter stay inside fp32's range.
 //
 // Up to four rows that share a head (a decode step): 8-bit integer products,
-// the cache's bytes as they lie. q is held as an integer of 22 bits (14 in
+// the cache's bytes as they lie. q is held as an integer of 23 bits (15 in
 // bf16 rows, whose own 8 it keeps) relative to the row's maximum, split into
 // signed bytes: columns 2r, 2r + 1 are the first two of row r and a second
 // column tile has the third. A score's sums are exact; so are those of the
-// output per turn, with weights of 23 bits (2 + 2 weight as a float has them
-// as its mantissa: its bytes are the columns). Only the weights' rounding
-// (2^-24 of the largest) and the turns' fp32 sums are left.
+// output per turn, with the weights as integers of 32 bits, a byte a column.
+// What is left are q's and the weights' own roundings (2^-24 of a row's
+// largest; 2^-33 of the largest weight, or its fp32's) and the turns' fp32 sums.
 //
 // More rows: products of halves, the conversion of a block's bytes shared by
 // the rows. Byte ^ 0x80 | 0x6400 is the half 1152 + integer, minus 1152 the
@@ -524,7 +524,7 @@ struct Kv8AttnParams {
     void* out;
     long long q_stride, out_stride;  // elements between rows; a row is [heads][D]
     Kv8Div group;                    // query heads per K/V head
-    float scale;                     // softmax scale times log2(e)
+    float scale, scale_low;          // softmax scale times log2(e), and what its rounding left
     int window;                      // 0: none
     Kv8Div by_heads, by_splits, by_tiles;  // K/V heads; splits of an item, at most; row tiles of a sequence
     int split_pages;                       // pages of a split
@@ -535,9 +535,8 @@ struct Kv8AttnParams {
 
 constexpr float kKv8WeightBits = 14.0f;  // weights are held times 2^14: a half keeps 11 bits down to 2^-28
 
-// Weights as integers: the mantissa of 2 + 2 (1 - 2^-22) w, that is w in units
-// of 2^-23, short of the next power of two where w is 1 and an ulp.
-constexpr float kKv8FixedScale = 2.0f - 0x1p-21f;
+// Weights as integers of 32 bits: 1 is the largest float below 2^32.
+constexpr float kKv8FixedScale = 4294967040.0f;
 
 enum Kv8Mode : int { KV8_HALF_BF16 = 0, KV8_HALF_F32 = 1, KV8_INT_BF16 = 2, KV8_INT_F32 = 3 };
 
@@ -744,7 +743,7 @@ __global__ void __launch_bounds__(32 * kWarps, kCtas) kv8_attention_kernel(Kv8At
     // q as B fragments; column g is row g (halves), or byte g % 2 of row g / 2 (qh) and its third byte (ql)
     constexpr int QS = kInt ? D / 32 : KS;  // steps of a score
     uint32_t qh[NT][QS][2], ql[NT][kFine || kMode == KV8_INT_F32 ? QS : 1][2];
-    float f[NT][RT];  // scale * 2^(row exponent) of the lane's rows
+    float f[NT][RT];  // 2^(row exponent) of the lane's rows
     int pos[NT][RT];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
@@ -763,14 +762,17 @@ __global__ void __launch_bounds__(32 * kWarps, kCtas) kv8_attention_kernel(Kv8At
         const bool row_bad = (bad >> (lane & ~3) & 0xfu) != 0;
         if (row_bad && t == 0 && r < n_rows) kv8_flag(p.seqs, i, kStatusNonFinite);
         // exponent of the maximum, kept where both powers below are normal
-        constexpr int kTop = kMode == KV8_INT_F32 ? 21 : kMode == KV8_INT_BF16 ? 13 : 12;
-        const int e = min(max(static_cast<int>(__float_as_uint(amax) >> 23) - 127, -105), 126);
+        // (integers: the maximum times 2^(kTop - e) is at most 1.984375 * 2^kTop, whose bytes fit)
+        constexpr int kTop = kMode == KV8_INT_F32 ? 22 : kMode == KV8_INT_BF16 ? 14 : 12;
+        const uint32_t top_bits = __float_as_uint(amax);
+        const int above = kInt && (top_bits & 0x7fffffu) > 0x7e0000u ? 1 : 0;
+        const int e = min(max(static_cast<int>(top_bits >> 23) - 127 + above, -104), 126);
         const float up = pow2i(kTop - e), back = pow2i(e - kTop);
 #pragma unroll
         for (int c = 0; c < KS; ++c) {
             const float x[4] = {v[c].x * up, v[c].y * up, v[c].z * up, v[c].w * up};
             if constexpr (kInt) {
-                // |x| < 2^22 (2^14): signed bytes d0 * 65536 + d1 * 256 + d2 (d0 * 256 + d1), |d0| <= 64
+                // signed bytes d0 * 65536 + d1 * 256 + d2 (d0 * 256 + d1), |d0| <= 127
                 uint32_t first = 0, third = 0;
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
@@ -794,7 +796,7 @@ __global__ void __launch_bounds__(32 * kWarps, kCtas) kv8_attention_kernel(Kv8At
                 }
             }
         }
-        const float fr = row_bad ? __int_as_float(0x7fc00000) : p.scale * back;  // a bad row's output is NaN
+        const float fr = row_bad ? __int_as_float(0x7fc00000) : back;  // a bad row's output is NaN
 #pragma unroll
         for (int k = 0; k < RT; ++k) {
             f[n][k] = __shfl_sync(kFull, fr, 8 * t + 4 * k);
@@ -885,10 +887,10 @@ __global__ void __launch_bounds__(32 * kWarps, kCtas) kv8_attention_kernel(Kv8At
             for (int n = 0; n < NT; ++n)
 #pragma unroll
                 for (int k = 0; k < RT; ++k) {
-                    const float u = f[n][k] * uk;
+                    const float u = f[n][k] * uk, u_high = u * p.scale, u_low = u * p.scale_low;
 #pragma unroll
                     for (int h = 0; h < 2; ++h)
-                        s[b][n][h][k] = fmaf(c4[n][2 * h + k], u, add);
+                        s[b][n][h][k] = fmaf(c4[n][2 * h + k], u_high, fmaf(c4[n][2 * h + k], u_low, add));
                 }
             const int page = at + b;
             if (id[b] < 0 || page < whole_first || page >= whole_last) {
@@ -924,27 +926,21 @@ __global__ void __launch_bounds__(32 * kWarps, kCtas) kv8_attention_kernel(Kv8At
             }
         if constexpr (kInt) {
             uint32_t high[PB], low[PB];  // B fragments: the weights' bytes of column g, four positions a page
-            uint32_t w[PB][2];
 #pragma unroll
             for (int b = 0; b < PB; ++b) {
+                uint32_t w[2];
                 float sum = 0.0f;
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     const float weight = ex2(s[b][0][h][0] - top[0][0]);
                     sum += weight;
-                    w[b][h] = __float_as_uint(fmaf(weight, kKv8FixedScale, 2.0f));
+                    w[h] = __float2uint_rn(weight * kKv8FixedScale);
                 }
                 l[0][0] = fmaf(sum, less[b], l[0][0]);
-                const uint32_t both = __byte_perm(w[b][0], w[b][1], 0x6521);  // bytes 1, 2 of position g, of g + 8
-                high[b] = __byte_perm(__shfl_sync(kFull, both, from0), __shfl_sync(kFull, both, from1), pick);
-            }
-#pragma unroll
-            for (int b = 0; b < PB; b += 2) {
-                const uint32_t both = __byte_perm(__byte_perm(w[b][0], w[b][1], 0x0040),
-                                                  __byte_perm(w[b + 1][0], w[b + 1][1], 0x0040), 0x5410);
-                const uint32_t x = __shfl_sync(kFull, both, from0), y = __shfl_sync(kFull, both, from1);
-                low[b] = __byte_perm(x, y, 0x5140);
-                low[b + 1] = __byte_perm(x, y, 0x7362);
+                // bytes 2, 3 and 0, 1 of positions g and g + 8 to the lanes that multiply them
+                const uint32_t upper = __byte_perm(w[0], w[1], 0x7632), lower = __byte_perm(w[0], w[1], 0x5410);
+                high[b] = __byte_perm(__shfl_sync(kFull, upper, from0), __shfl_sync(kFull, upper, from1), pick);
+                low[b] = __byte_perm(__shfl_sync(kFull, lower, from0), __shfl_sync(kFull, lower, from1), pick);
             }
 #pragma unroll
             for (int j = 0; j < D / 32; ++j) {
@@ -966,7 +962,8 @@ __global__ void __launch_bounds__(32 * kWarps, kCtas) kv8_attention_kernel(Kv8At
                     for (int h = 0; h < 2; ++h)
                         o[2 * j + k][0][h] =
                             fmaf(o[2 * j + k][0][h], c[0][0],
-                                 fmaf(static_cast<float>(x[2 * h]), 65536.0f, static_cast<float>(x[2 * h + 1] * 256 + y[2 * h])));
+                                 fmaf(static_cast<float>(x[2 * h] * 256 + x[2 * h + 1]), 65536.0f,
+                                      static_cast<float>(y[2 * h] * 256 + y[2 * h + 1])));
                 }
             }
         } else {
@@ -1044,7 +1041,7 @@ __global__ void __launch_bounds__(32 * kWarps, kCtas) kv8_attention_kernel(Kv8At
         }
     __syncthreads();
     constexpr int kQuads = D / 4;
-    constexpr float kUnit = kInt ? 2.0f / 8388608.0f / kKv8FixedScale : 1.0f;  // of the held weights
+    constexpr float kUnit = kInt ? 1.0f / kKv8FixedScale : 1.0f;  // of the held weights
     struct Share {  // M, sum, reference and four dims of a row
         float m, l;
         int ref;
