@@ -453,7 +453,7 @@ struct Kv8Pool {
             release();
             return PHONON_CUDA_OUT_OF_MEMORY;
         }
-        CUDA_TRY(cudaMemset(pool, 0, layers * layer_bytes()));
+        CUDA_TRY(cudaMemset(pool, 128, layers * layer_bytes()));
         CUDA_TRY(cudaMemset(exps, kKv8MinExp + 127, layers * layer_exps()));
         CUDA_TRY(cudaStreamSynchronize(nullptr));  // callers' streams do not wait for the legacy stream
         return PHONON_CUDA_OK;

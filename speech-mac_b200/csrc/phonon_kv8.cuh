@@ -4,7 +4,7 @@
 // Format. A block is 16 positions of one K/V head; its keys and its values
 // each share one scale 2^e with e the smallest integer in [kKv8MinExp,
 // kKv8MaxExp] for which |x| <= 127 * 2^e over the block, and an element is
-// held as the integer nearest x / 2^e, at most 127 in magnitude.
+// held as the integer nearest x / 2^e, at most 127 in magnitude, plus 128.
 // The scale is a power of two so that quantising, raising the scale of a
 // partly filled block (the held integers divided by a power of two and
 // rounded again) and reading back are exact but for the one rounding each
@@ -109,10 +109,11 @@ __device__ __forceinline__ int kv8_exponent(float amax) {
     return min(max(e, kKv8MinExp), kKv8MaxExp);
 }
 
-// The nearest integer to x / 2^e (ties to even) in the low byte: adding 1.5 *
-// 2^23 rounds the exact quotient to an integer. |x| <= 127 * 2^e.
+// The nearest integer to x / 2^e (ties to even) plus 128 in the low byte:
+// adding 1.5 * 2^23 + 128 rounds the exact quotient to an integer. |x| <= 127
+// * 2^e.
 __device__ __forceinline__ uint32_t kv8_code(float x, float inverse) {
-    return __float_as_uint(__fmaf_rn(x, inverse, 12582912.0f));
+    return __float_as_uint(__fmaf_rn(x, inverse, 12583040.0f));
 }
 
 // The low bytes of four words.
@@ -124,7 +125,7 @@ __device__ __forceinline__ uint32_t kv8_pack(uint32_t a, uint32_t b, uint32_t c,
 __device__ __forceinline__ uint32_t kv8_shrink(uint32_t w, float shrink) {
     uint32_t r[4];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) r[k] = kv8_code(static_cast<float>(static_cast<int8_t>(w >> (8 * k))), shrink);
+    for (int k = 0; k < 4; ++k) r[k] = kv8_code(static_cast<float>(static_cast<int>((w >> (8 * k)) & 0xffu) - 128), shrink);
     return kv8_pack(r[0], r[1], r[2], r[3]);
 }
 
@@ -414,7 +415,7 @@ struct Kv8ReadParams {
     int blocks;
 };
 
-// One warp reads one block's keys or values back: the held integer times 2^e,
+// One warp reads one block's keys or values back: held byte - 128 times 2^e,
 // exact in fp32. Rows of positions before 0, of empty and of bad pages are 0.
 template <int D, bool kBf16>
 __global__ void __launch_bounds__(128) kv8_read_kernel(Kv8ReadParams p) {
@@ -449,7 +450,7 @@ __global__ void __launch_bounds__(128) kv8_read_kernel(Kv8ReadParams p) {
     const float unit = page >= 0 ? pow2i(kv8_exp(p.cache, page, head)[which] - 127) : 0.0f;
     void* dst = p.rows[which];
     auto value = [&](uint32_t w, int k) {
-        return static_cast<float>(static_cast<int8_t>(w >> (8 * k))) * unit;
+        return (static_cast<float>((w >> (8 * k)) & 0xffu) - 128.0f) * unit;
     };
     const int g = lane >> 2, t = lane & 3;
     if (which == 0) {
@@ -459,7 +460,7 @@ __global__ void __launch_bounds__(128) kv8_read_kernel(Kv8ReadParams p) {
             const int slot = a * kRowsPerPass + lane / kLanesPerRow;
             w[a] = src && slot >= lo && slot < hi
                        ? __ldg(reinterpret_cast<const uint32_t*>(src + slot * D) + lane % kLanesPerRow)
-                       : 0u;
+                       : 0x80808080u;
         }
 #pragma unroll
         for (int a = 0; a < kPasses; ++a) {
@@ -473,7 +474,7 @@ __global__ void __launch_bounds__(128) kv8_read_kernel(Kv8ReadParams p) {
 #pragma unroll
         for (int j = 0; j < kChunks; ++j)
             w[j] = src ? __ldg(reinterpret_cast<const uint4*>(src + j * 512) + lane)
-                       : make_uint4(0u, 0u, 0u, 0u);
+                       : make_uint4(0x80808080u, 0x80808080u, 0x80808080u, 0x80808080u);
 #pragma unroll
         for (int j = 0; j < kChunks; ++j)
 #pragma unroll
@@ -508,12 +509,13 @@ __global__ void __launch_bounds__(128) kv8_read_kernel(Kv8ReadParams p) {
 // signed bytes: columns 2r, 2r + 1 are the first two of row r and a second
 // column tile has the third. A score's sums are exact; so are those of the
 // output per turn, with the weights as integers of 32 bits, a byte a column.
-// What is left are q's and the weights' own roundings (2^-24 of a row's
+// (The cache's bytes are unsigned, 128 too large: products with a constant -128
+// in their place start the sums.) What is left are q's and the weights' own roundings (2^-24 of a row's
 // largest; 2^-33 of the largest weight, or its fp32's) and the turns' fp32 sums.
 //
 // More rows: products of halves, the conversion of a block's bytes shared by
-// the rows. Byte ^ 0x80 | 0x6400 is the half 1152 + integer, minus 1152 the
-// integer, exactly. The products are exact in the fp32 accumulators. fp32 rows:
+// the rows. Byte | 0x6400 is the half 1152 + integer, minus 1152 the integer,
+// exactly, one PRMT and one HSUB2 for two. The products are exact in the fp32 accumulators. fp32 rows:
 // q (scaled by a power of two to a row maximum near 2^12) and the weights
 // enter as two halves each, 22 bits. bf16 rows: q fits one half (8 bits), a
 // weight is rounded to one half (11 bits, under the output's 8).
@@ -547,18 +549,44 @@ __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// 16 x 32 signed bytes by 32 x 8 signed (kSigned) or unsigned bytes.
-template <bool kSigned>
-__device__ __forceinline__ void imma16832(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
-                                          uint32_t b1) {
-    if constexpr (kSigned)
-        asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                     : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
-                     : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-    else
-        asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.u8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                     : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
-                     : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+// d = c + 16 x 32 bytes by 32 x 8 bytes; kKinds: "u8.s8", "u8.u8", "s8.s8" or
+// "s8.u8".
+#define KV8_IMMA(NAME, KINDS)                                                                                        \
+    __device__ __forceinline__ void NAME(int (&d)[4], const int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2,      \
+                                         uint32_t a3, uint32_t b0, uint32_t b1) {                                    \
+        asm volatile("mma.sync.aligned.m16n8k32.row.col.s32." KINDS                                                  \
+                     ".s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"                                \
+                     : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])                                                \
+                     : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "r"(c[0]), "r"(c[1]), "r"(c[2]), "r"(c[3])); \
+    }
+KV8_IMMA(imma_u8_s8, "u8.s8")
+KV8_IMMA(imma_u8_u8, "u8.u8")
+KV8_IMMA(imma_s8_s8, "s8.s8")
+KV8_IMMA(imma_s8_u8, "s8.u8")
+#undef KV8_IMMA
+constexpr uint32_t kKv8Minus128 = 0x80808080u;  // four signed bytes
+
+// Two fp32 operations an instruction.
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+    float2 d;
+    asm("{.reg .b64 x, y, z; mov.b64 x, {%2, %3}; mov.b64 y, {%4, %5}; mul.rn.f32x2 z, x, y; mov.b64 {%0, %1}, z;}"
+        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    float2 d;
+    asm("{.reg .b64 x, y, z; mov.b64 x, {%2, %3}; mov.b64 y, {%4, %5}; add.rn.f32x2 z, x, y; mov.b64 {%0, %1}, z;}"
+        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 d;
+    asm("{.reg .b64 x, y, z, w; mov.b64 x, {%2, %3}; mov.b64 y, {%4, %5}; mov.b64 z, {%6, %7}; fma.rn.f32x2 w, x, y, z; "
+        "mov.b64 {%0, %1}, w;}"
+        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return d;
 }
 
 __device__ __forceinline__ uint32_t movmatrix_trans(uint32_t v) {
@@ -574,7 +602,7 @@ __device__ __forceinline__ float ex2(float x) {
     return r;
 }
 
-// Bytes 0, 1 (kHigh: 2, 3) of a cache word, sign bits flipped, as halves.
+// Bytes 0, 1 (kHigh: 2, 3) of a cache word as the halves byte - 128.
 template <bool kHigh>
 __device__ __forceinline__ uint32_t kv8_halves(uint32_t w) {
     uint32_t u = __byte_perm(w, 0x64646464u, kHigh ? 0x4342 : 0x4140);
@@ -805,6 +833,17 @@ __global__ void __launch_bounds__(32 * kWarps, kCtas) kv8_attention_kernel(Kv8At
         }
     }
 
+    // what a score's sums start from: -128 times those of q's bytes
+    int q_base[4] = {0, 0, 0, 0}, q_base3[4] = {0, 0, 0, 0};
+    if constexpr (kInt) {
+#pragma unroll
+        for (int c = 0; c < QS; ++c) {
+            imma_s8_s8(q_base, q_base, kKv8Minus128, kKv8Minus128, kKv8Minus128, kKv8Minus128, qh[0][c][0], qh[0][c][1]);
+            if constexpr (kMode == KV8_INT_F32)
+                imma_s8_s8(q_base3, q_base3, kKv8Minus128, kKv8Minus128, kKv8Minus128, kKv8Minus128, ql[0][c][0], ql[0][c][1]);
+        }
+    }
+
     // O: [16-dim tile][column tile][accumulators] (halves), or the lane's row of dims g, g + 8 of a tile
     constexpr int OT = kInt ? 2 : 4;
     float o[KS][NT][OT], m[NT][RT], l[NT][RT];
@@ -852,12 +891,12 @@ __global__ void __launch_bounds__(32 * kWarps, kCtas) kv8_attention_kernel(Kv8At
             uint32_t kw[2][D / 16];
             kv8_key_words<D>(kw, pages_at + b * kPageBytes, lane);
             if constexpr (kInt) {
-                int x[4] = {0, 0, 0, 0}, y[4] = {0, 0, 0, 0};
+                int x[4], y[4];
 #pragma unroll
                 for (int c = 0; c < QS; ++c) {
-                    imma16832<true>(x, kw[0][2 * c], kw[1][2 * c], kw[0][2 * c + 1], kw[1][2 * c + 1], qh[0][c][0], qh[0][c][1]);
+                    imma_u8_s8(x, c ? x : q_base, kw[0][2 * c], kw[1][2 * c], kw[0][2 * c + 1], kw[1][2 * c + 1], qh[0][c][0], qh[0][c][1]);
                     if constexpr (kMode == KV8_INT_F32)
-                        imma16832<true>(y, kw[0][2 * c], kw[1][2 * c], kw[0][2 * c + 1], kw[1][2 * c + 1], ql[0][c][0], ql[0][c][1]);
+                        imma_u8_s8(y, c ? y : q_base3, kw[0][2 * c], kw[1][2 * c], kw[0][2 * c + 1], kw[1][2 * c + 1], ql[0][c][0], ql[0][c][1]);
                 }
 #pragma unroll
                 for (int h = 0; h < 2; ++h)
@@ -869,7 +908,7 @@ __global__ void __launch_bounds__(32 * kWarps, kCtas) kv8_attention_kernel(Kv8At
                 for (int n = 0; n < NT; ++n) c4[n][0] = c4[n][1] = c4[n][2] = c4[n][3] = 0.0f;
 #pragma unroll
                 for (int c = 0; c < KS; ++c) {
-                    const uint32_t wa = kw[0][c] ^ 0x80808080u, wb = kw[1][c] ^ 0x80808080u;
+                    const uint32_t wa = kw[0][c], wb = kw[1][c];
                     const uint32_t a0 = kv8_halves<false>(wa), a1 = kv8_halves<false>(wb);
                     const uint32_t a2 = kv8_halves<true>(wa), a3 = kv8_halves<true>(wb);
 #pragma unroll
@@ -885,13 +924,23 @@ __global__ void __launch_bounds__(32 * kWarps, kCtas) kv8_attention_kernel(Kv8At
             less[b] = pow2i(-ev);
 #pragma unroll
             for (int n = 0; n < NT; ++n)
+            {
+                // both positions of a row (integers), both rows of a position (halves), at a time
+                const float2 u = make_float2(f[n][0] * uk, f[n][RT - 1] * uk), both = make_float2(add, add);
+                const float2 u_high = mul2(u, make_float2(p.scale, p.scale)), u_low = mul2(u, make_float2(p.scale_low, p.scale_low));
+                if constexpr (kInt) {
+                    const float2 x = make_float2(c4[n][0], c4[n][2]), z = fma2(x, u_high, fma2(x, u_low, both));
+                    s[b][n][0][0] = z.x;
+                    s[b][n][1][0] = z.y;
+                } else {
 #pragma unroll
-                for (int k = 0; k < RT; ++k) {
-                    const float u = f[n][k] * uk, u_high = u * p.scale, u_low = u * p.scale_low;
-#pragma unroll
-                    for (int h = 0; h < 2; ++h)
-                        s[b][n][h][k] = fmaf(c4[n][2 * h + k], u_high, fmaf(c4[n][2 * h + k], u_low, add));
+                    for (int h = 0; h < 2; ++h) {
+                        const float2 x = make_float2(c4[n][2 * h], c4[n][2 * h + 1]), z = fma2(x, u_high, fma2(x, u_low, both));
+                        s[b][n][h][0] = z.x;
+                        s[b][n][h][RT - 1] = z.y;
+                    }
                 }
+            }
             const int page = at + b;
             if (id[b] < 0 || page < whole_first || page >= whole_last) {
 #pragma unroll
@@ -942,6 +991,12 @@ __global__ void __launch_bounds__(32 * kWarps, kCtas) kv8_attention_kernel(Kv8At
                 high[b] = __byte_perm(__shfl_sync(kFull, upper, from0), __shfl_sync(kFull, upper, from1), pick);
                 low[b] = __byte_perm(__shfl_sync(kFull, lower, from0), __shfl_sync(kFull, lower, from1), pick);
             }
+            int base[4] = {0, 0, 0, 0}, base_low[4] = {0, 0, 0, 0};  // of the output's sums
+#pragma unroll
+            for (int b = 0; b < PB; b += 2) {
+                imma_s8_u8(base, base, kKv8Minus128, kKv8Minus128, kKv8Minus128, kKv8Minus128, high[b], high[b + 1]);
+                imma_s8_u8(base_low, base_low, kKv8Minus128, kKv8Minus128, kKv8Minus128, kKv8Minus128, low[b], low[b + 1]);
+            }
 #pragma unroll
             for (int j = 0; j < D / 32; ++j) {
                 uint4 v[PB];
@@ -950,20 +1005,20 @@ __global__ void __launch_bounds__(32 * kWarps, kCtas) kv8_attention_kernel(Kv8At
                     v[b] = *reinterpret_cast<const uint4*>(pages_at + b * kPageBytes + kKv8Block * D + j * 512 + lane * 16);
 #pragma unroll
                 for (int k = 0; k < 2; ++k) {
-                    int x[4] = {0, 0, 0, 0}, y[4] = {0, 0, 0, 0};
+                    int x[4], y[4];
 #pragma unroll
                     for (int b = 0; b < PB; b += 2) {
                         const uint32_t a0 = k ? v[b].z : v[b].x, a1 = k ? v[b].w : v[b].y;
                         const uint32_t a2 = k ? v[b + 1].z : v[b + 1].x, a3 = k ? v[b + 1].w : v[b + 1].y;
-                        imma16832<false>(x, a0, a1, a2, a3, high[b], high[b + 1]);
-                        imma16832<false>(y, a0, a1, a2, a3, low[b], low[b + 1]);
+                        imma_u8_u8(x, b ? x : base, a0, a1, a2, a3, high[b], high[b + 1]);
+                        imma_u8_u8(y, b ? y : base_low, a0, a1, a2, a3, low[b], low[b + 1]);
                     }
-#pragma unroll
-                    for (int h = 0; h < 2; ++h)
-                        o[2 * j + k][0][h] =
-                            fmaf(o[2 * j + k][0][h], c[0][0],
-                                 fmaf(static_cast<float>(x[2 * h] * 256 + x[2 * h + 1]), 65536.0f,
-                                      static_cast<float>(y[2 * h] * 256 + y[2 * h + 1])));
+                    const float2 upper = make_float2(static_cast<float>(x[0] * 256 + x[1]), static_cast<float>(x[2] * 256 + x[3]));
+                    const float2 lower = make_float2(static_cast<float>(y[0] * 256 + y[1]), static_cast<float>(y[2] * 256 + y[3]));
+                    const float2 z = fma2(make_float2(o[2 * j + k][0][0], o[2 * j + k][0][1]), make_float2(c[0][0], c[0][0]),
+                                          fma2(upper, make_float2(65536.0f, 65536.0f), lower));
+                    o[2 * j + k][0][0] = z.x;
+                    o[2 * j + k][0][1] = z.y;
                 }
             }
         } else {
@@ -974,18 +1029,23 @@ __global__ void __launch_bounds__(32 * kWarps, kCtas) kv8_attention_kernel(Kv8At
                 for (int b = 0; b < PB; ++b) {
                     float w[2][RT];
 #pragma unroll
-                    for (int k = 0; k < RT; ++k) {
-#pragma unroll
-                        for (int h = 0; h < 2; ++h) w[h][k] = ex2(s[b][n][h][k] - top[n][k]);
-                        l[n][k] = fmaf(w[0][k] + w[1][k], less[b], l[n][k]);
+                    for (int h = 0; h < 2; ++h) {
+                        const float2 z = add2(make_float2(s[b][n][h][0], s[b][n][h][RT - 1]), make_float2(-top[n][0], -top[n][RT - 1]));
+                        w[h][0] = ex2(z.x);
+                        w[h][RT - 1] = ex2(z.y);
                     }
+                    const float2 sum = fma2(add2(make_float2(w[0][0], w[0][RT - 1]), make_float2(w[1][0], w[1][RT - 1])),
+                                            make_float2(less[b], less[b]), make_float2(l[n][0], l[n][RT - 1]));
+                    l[n][0] = sum.x;
+                    l[n][RT - 1] = sum.y;
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
                         const uint32_t high = half2_bits(w[h][0], w[h][RT - 1]);
                         ph[b][n][h] = movmatrix_trans(high);
                         if constexpr (kFine) {
-                            const float2 r = half2_floats(high);
-                            pl[b][n][h] = movmatrix_trans(half2_bits(w[h][0] - r.x, w[h][RT - 1] - r.y));
+                            const float2 r = half2_floats(high ^ 0x80008000u);
+                            const float2 rest = add2(make_float2(w[h][0], w[h][RT - 1]), r);
+                            pl[b][n][h] = movmatrix_trans(half2_bits(rest.x, rest.y));
                         }
                     }
                 }
@@ -995,7 +1055,11 @@ __global__ void __launch_bounds__(32 * kWarps, kCtas) kv8_attention_kernel(Kv8At
 #pragma unroll
                     for (int n = 0; n < NT; ++n)
 #pragma unroll
-                        for (int j = 0; j < OT; ++j) o[k][n][j] *= c[n][j % RT];
+                        for (int j = 0; j < OT; j += 2) {
+                            const float2 z = mul2(make_float2(o[k][n][j], o[k][n][j + 1]), make_float2(c[n][0], c[n][RT - 1]));
+                            o[k][n][j] = z.x;
+                            o[k][n][j + 1] = z.y;
+                        }
             }
             if constexpr (!kInt) {
 #pragma unroll
@@ -1003,7 +1067,7 @@ __global__ void __launch_bounds__(32 * kWarps, kCtas) kv8_attention_kernel(Kv8At
 #pragma unroll
                     for (int j = 0; j < D / 32; ++j) {
                         const uint4 w4 = *reinterpret_cast<const uint4*>(pages_at + b * kPageBytes + kKv8Block * D + j * 512 + lane * 16);
-                        const uint32_t w[4] = {w4.x ^ 0x80808080u, w4.y ^ 0x80808080u, w4.z ^ 0x80808080u, w4.w ^ 0x80808080u};
+                        const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
 #pragma unroll
                         for (int k = 0; k < 2; ++k) {
                             const uint32_t a0 = kv8_halves<false>(w[2 * k]), a1 = kv8_halves<false>(w[2 * k + 1]);
