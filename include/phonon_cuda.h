@@ -503,6 +503,7 @@ typedef struct {
 } PhononCudaKv8Rows;
 
 typedef struct PhononCudaKv8 PhononCudaKv8;
+/* Create, destroy and workspace calls allocate and wait: not during a capture. */
 int phonon_cuda_kv8_create(const PhononCudaKv8Config *config, PhononCudaKv8 **out);
 /* No call on the cache may be running. */
 void phonon_cuda_kv8_destroy(PhononCudaKv8 *cache);
@@ -517,7 +518,7 @@ int phonon_cuda_kv8_append_device(PhononCudaKv8 *cache, uint32_t layer, const Ph
 int phonon_cuda_kv8_read_device(PhononCudaKv8 *cache, uint32_t layer, const PhononCudaKv8Batch *batch,
                                 const PhononCudaKv8Rows *rows, int32_t *status_dev, void *cuda_stream);
 
-/* Scratch of the attention calls on a cache's device (about 22 MB). Calls that
+/* Scratch of the attention calls on a cache's device (about 26 MB). Calls that
  * may run at the same time, captured ones included, need one each. */
 typedef struct PhononCudaKv8Workspace PhononCudaKv8Workspace;
 int phonon_cuda_kv8_workspace_create(PhononCudaKv8 *cache, PhononCudaKv8Workspace **out);
@@ -527,7 +528,8 @@ void phonon_cuda_kv8_workspace_destroy(PhononCudaKv8Workspace *workspace);
  * src/phonon_transformer.c:340-404, for any head layout and any number of
  * rows): the row at position p sees positions (p - window, p], or [0, p] where
  * window is 0. q and out are [rows][heads][head_dim], heads a multiple of
- * kv_heads (query head h reads K/V head h / (heads / kv_heads)); out may be q.
+ * kv_heads (query head h reads K/V head h / (heads / kv_heads)); out may be q
+ * with q's stride.
  * A row that sees nothing gets 0. */
 typedef struct {
     uint32_t type;   /* PhononCudaRowType of q and out */

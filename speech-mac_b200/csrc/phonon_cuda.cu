@@ -447,12 +447,12 @@ struct Kv8Pool {
         pages = n_pages;
         heads = n_heads;
         dim = head_dim;
-        if (cudaMalloc(&pool, layers * layer_bytes()) != cudaSuccess ||
-            cudaMalloc(&exps, layers * layer_exps()) != cudaSuccess) {
+        if (cudaMalloc(&pool, bytes()) != cudaSuccess) {
             cudaGetLastError();
-            release();
+            pool = nullptr;
             return PHONON_CUDA_OUT_OF_MEMORY;
         }
+        exps = pool + layers * layer_bytes();
         CUDA_TRY(cudaMemset(pool, 128, layers * layer_bytes()));
         CUDA_TRY(cudaMemset(exps, kKv8MinExp + 127, layers * layer_exps()));
         CUDA_TRY(cudaStreamSynchronize(nullptr));  // callers' streams do not wait for the legacy stream
@@ -460,9 +460,7 @@ struct Kv8Pool {
     }
     void release() {
         if (pool) cudaFree(pool);
-        if (exps) cudaFree(exps);
-        pool = nullptr;
-        exps = nullptr;
+        pool = exps = nullptr;
     }
 };
 
@@ -476,21 +474,20 @@ struct Kv8Scratch {
     int max_splits = 0;  // CTAs of a split call, at most
     int alloc(int sms) {
         max_splits = 4 * kKv8Ctas * sms;  // as kv8_launch_attention splits
-        if (cudaMalloc(&part, static_cast<size_t>(max_splits) * kKv8TileFloats * 4) != cudaSuccess ||
-            cudaMalloc(&ml, static_cast<size_t>(max_splits) * 32 * sizeof(float4)) != cudaSuccess ||
-            cudaMalloc(&arrived, static_cast<size_t>(max_splits) * 4) != cudaSuccess) {
+        const size_t n = static_cast<size_t>(max_splits), floats = n * kKv8TileFloats;
+        if (cudaMalloc(&part, (floats + n * 32 * 4 + n) * 4) != cudaSuccess) {
             cudaGetLastError();
-            release();
+            part = nullptr;
             return PHONON_CUDA_OUT_OF_MEMORY;
         }
+        ml = reinterpret_cast<float4*>(part + floats);
+        arrived = reinterpret_cast<unsigned*>(ml + n * 32);
         CUDA_TRY(cudaMemset(arrived, 0, static_cast<size_t>(max_splits) * 4));
         CUDA_TRY(cudaStreamSynchronize(nullptr));
         return PHONON_CUDA_OK;
     }
     void release() {
         if (part) cudaFree(part);
-        if (ml) cudaFree(ml);
-        if (arrived) cudaFree(arrived);
         part = nullptr;
         ml = nullptr;
         arrived = nullptr;
@@ -592,7 +589,8 @@ int kv8_launch_attention(const Kv8Pool& c, uint32_t layer, const Kv8Seqs& seqs, 
     if (items * splits > INT32_MAX) return PHONON_CUDA_CAPACITY;
     if (splits > 1 && items * splits > w.max_splits) return PHONON_CUDA_CAPACITY;
     p.by_heads = kv8_divisor(c.heads);
-    p.by_splits = kv8_divisor(static_cast<uint32_t>(splits));
+    p.by_items = kv8_divisor(static_cast<uint32_t>(items));
+    p.splits = static_cast<int>(splits);
     p.by_tiles = kv8_divisor(static_cast<uint32_t>(tiles));
     p.split_pages = static_cast<int>((pages + splits - 1) / splits);
     p.part = w.part;

@@ -528,7 +528,8 @@ struct Kv8AttnParams {
     Kv8Div group;                    // query heads per K/V head
     float scale, scale_low;          // softmax scale times log2(e), and what its rounding left
     int window;                      // 0: none
-    Kv8Div by_heads, by_splits, by_tiles;  // K/V heads; splits of an item, at most; row tiles of a sequence
+    Kv8Div by_items, by_heads, by_tiles;  // (sequence, row tile, K/V head) items; K/V heads; row tiles of a sequence
+    int splits;                            // of an item, at most
     int split_pages;                       // pages of a split
     float* part;                     // [items * splits][rows of a tile][D]
     float4* part_ml;                 // [items * splits][rows of a tile]: M, sum, eV's reference
@@ -701,13 +702,15 @@ __global__ void __launch_bounds__(32 * kWarps, kCtas) kv8_attention_kernel(Kv8At
     pdl_wait();
     pdl_trigger();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    // block index: heads fastest (a page's heads are neighbours), then splits, row tiles, sequences
-    const uint32_t rest = kv8_div(blockIdx.x, p.by_heads), rest2 = kv8_div(rest, p.by_splits);
-    const int head = static_cast<int>(blockIdx.x - rest * p.by_heads.d);
-    const int split = static_cast<int>(rest - rest2 * p.by_splits.d);
-    const int i = static_cast<int>(kv8_div(rest2, p.by_tiles));
-    const int tile = static_cast<int>(rest2 - i * p.by_tiles.d);
-    const uint32_t item = rest2 * p.by_heads.d + head;
+    // block index: heads fastest (a page's heads are neighbours), then row
+    // tiles, sequences and, last to first, splits: the splits that only long
+    // sequences have start first, the short sequences' work ends the launch
+    const uint32_t later = kv8_div(blockIdx.x, p.by_items), item = blockIdx.x - later * p.by_items.d;
+    const uint32_t entry = kv8_div(item, p.by_heads);
+    const int head = static_cast<int>(item - entry * p.by_heads.d);
+    const int split = p.splits - 1 - static_cast<int>(later);
+    const int i = static_cast<int>(kv8_div(entry, p.by_tiles));
+    const int tile = static_cast<int>(entry - i * p.by_tiles.d);
     const Kv8Seq sq = kv8_seq(p.seqs, i);
     const int rows = sq.count * static_cast<int>(p.group.d) - tile * kRows;  // rows left from this tile on
     if (rows <= 0) return;
@@ -718,7 +721,7 @@ __global__ void __launch_bounds__(32 * kWarps, kCtas) kv8_attention_kernel(Kv8At
     const int key_end = min(pos_hi + 1, sq.length);
     const int page_begin = p.window ? max(pos_lo - p.window + 1, 0) / kKv8Block : 0;
     const int pages = key_end > 0 ? (key_end + kKv8Block - 1) / kKv8Block - page_begin : 0;
-    const int active = max(1, min(static_cast<int>(p.by_splits.d), (pages + p.split_pages - 1) / p.split_pages));
+    const int active = max(1, min(p.splits, (pages + p.split_pages - 1) / p.split_pages));
     if (split >= active) return;
     const int per = (pages + active - 1) / active;
     const int first = page_begin + min(pages, split * per), last = page_begin + min(pages, (split + 1) * per);
@@ -1130,7 +1133,7 @@ __global__ void __launch_bounds__(32 * kWarps, kCtas) kv8_attention_kernel(Kv8At
                               static_cast<size_t>(head * p.group.d + rho - at * p.group.d) * D + d,
                           make_float4(s.a.x * inv, s.a.y * inv, s.a.z * inv, s.a.w * inv));
     };
-    const size_t slot = static_cast<size_t>(item) * p.by_splits.d;
+    const size_t slot = static_cast<size_t>(item) * p.splits;
     for (int x = threadIdx.x; x < n_rows * kQuads; x += blockDim.x) {
         const int r = x / kQuads, d = x % kQuads * 4;
         Share s = nothing();

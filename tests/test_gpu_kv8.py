@@ -438,3 +438,108 @@ def test_repeated_calls_are_bit_identical(cuda_ok):
         outs.append(out)
     torch.cuda.synchronize()
     assert all(torch.equal(o, outs[0]) for o in outs)
+
+
+def test_one_row_appends_refuse_and_keep(cuda_ok):
+    """The form for one row a sequence: bad pages, bad lengths, non-finite and extreme values, and what it must leave."""
+    rng = np.random.default_rng(15)
+    lengths = [17, 18, 33, 5, 1, 40]
+    c = Cache(3, 64, lengths)
+    first = [n - 1 for n in lengths]
+    old = [[rows(rng, n, 3, 64) for n in first] for _ in range(2)]
+    c.append(first, *old)
+    held = [[model.Held(3, 64) for _ in lengths] for _ in range(2)]
+    for w in range(2):
+        for h, r in zip(held[w], old[w]):
+            h.append(f64(r))
+    new = [[rows(rng, 1, 3, 64) * 50 for _ in lengths] for _ in range(2)]  # raises every scale
+    new[0][1][0, 0, 3], new[1][1][0, 2, 7] = float("nan"), float("-inf")
+    new[0][2][0, 1, :2] = torch.tensor([3e38, -3e38])
+    table = c.table.clone()
+    c.table[3, 0] = c.pool + 7
+    status = torch.zeros(len(lengths), dtype=torch.int32, device="cuda")
+    told = list(lengths)
+    told[5] = -3  # refused: nothing of sequence 5 changes
+    k, v = torch.cat(new[0]), torch.cat(new[1])
+    length = i32(told)
+    batch = rt.kv8_batch(len(lengths), length.data_ptr(), c.table.data_ptr(), c.stride, max_length=48)
+    c.kv.append(batch, rt.kv8_rows(k.data_ptr(), v.data_ptr()), status_ptr=status.data_ptr())
+    torch.cuda.synchronize()
+    assert status.tolist() == [0, rt.NON_FINITE, 0, rt.INVALID, 0, rt.CAPACITY]
+    c.table.copy_(table)
+    for w in range(2):
+        for i, h in enumerate(held[w]):
+            if i not in (3, 5):
+                h.append(f64(new[w][i]))
+    now = [n if i not in (3, 5) else n - 1 for i, n in enumerate(lengths)]
+    for got, want in zip(c.read(now), held):
+        for g, h in zip(got, want):
+            np.testing.assert_array_equal(g, h.values().astype(np.float32))
+
+
+@pytest.mark.parametrize("dim", [32, 64, 128])
+def test_single_rows_equal_one_append(cuda_ok, dim):
+    """40 one-row appends, a scale rising inside the block or not, against the definition and the many-row form."""
+    rng = np.random.default_rng(dim)
+    n = 40
+    x = rng.standard_normal((n, 2, dim)) * 4.0 ** rng.integers(-3, 4, (n, 2, 1))
+    x[16:32] = x[16:17] / (1 + np.arange(16)[:, None, None])  # never rises
+    k = dev(x, torch.float32)
+    one, many = Cache(2, dim, [n]), Cache(2, dim, [n])
+    h = model.Held(2, dim)
+    for t in range(n):
+        one.append([t + 1], [k[t:t + 1]], [-k[t:t + 1]])
+        h.append(x[t:t + 1].astype(np.float32))
+    for t in range(0, n, 2):
+        many.append([t + 2], [k[t:t + 2]], [-k[t:t + 2]])
+    got = one.read([n])
+    np.testing.assert_array_equal(got[0][0], h.values().astype(np.float32))
+    np.testing.assert_array_equal(got[1][0], -h.values().astype(np.float32))
+    pairs = model.Held(2, dim)
+    for t in range(0, n, 2):
+        pairs.append(x[t:t + 2].astype(np.float32))
+    np.testing.assert_array_equal(many.read([n])[0][0], pairs.values().astype(np.float32))
+
+
+def test_more_rows_than_positions(cuda_ok):
+    """Rows that would lie before position 0 are not written and read as 0."""
+    rng = np.random.default_rng(16)
+    c = Cache(1, 32, [3, 20])
+    k = [rows(rng, 8, 1, 32), rows(rng, 8, 1, 32)]
+    v = [rows(rng, 8, 1, 32), rows(rng, 8, 1, 32)]
+    c.append([3, 8], k, v)
+    for got, new in zip(c.read([3, 8], [5, 8]), (k, v)):
+        for g, r, n in zip(got, new, (3, 8)):
+            h = model.Held(1, 32)
+            h.append(f64(r[8 - n:]))
+            assert (g[:len(g) - n] == 0).all()
+            np.testing.assert_array_equal(g[len(g) - n:], h.values().astype(np.float32))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("group,count", [(1, 1), (1, 20)])
+def test_all_keys_alike_and_one_key_far_ahead(cuda_ok, group, count, dtype):
+    """Flat softmax over many keys, and one that a single key takes: the weights at both ends of their range."""
+    n = 2000
+    rng = np.random.default_rng(17)
+    k = np.ones((n, 1, 64), np.float32)
+    far = k.copy()
+    far[::2] *= -1
+    far[777] = 100.0
+    c = Cache(1, 64, [n, n])
+    v = rows(rng, n, 1, 64, dtype)
+    c.append([n, n], [dev(k).to(dtype), dev(far).to(dtype)], [v, v])
+    q = torch.full((2 * count, group, 64), 1.5, device="cuda").to(dtype)
+    out = torch.empty_like(q)
+    kind = rt.ROWS_BF16 if dtype == torch.bfloat16 else rt.ROWS_F32
+    ws = rt.Kv8Workspace(c.kv)
+    c.kv.attention(c.batch([n, n], [count, count]), rt.kv8_query(q.data_ptr(), out.data_ptr(), kind, heads=group), ws)
+    torch.cuda.synchronize()
+    for i, keys in enumerate((k, far)):
+        hk, hv = model.Held(1, 64), model.Held(1, 64)
+        hk.append(keys)
+        hv.append(f64(v))
+        part = f64(q[i * count:(i + 1) * count])
+        want, size = model.attention(part, hk.values(), hv.values())
+        bound = model.attention_bound(size, np.abs(hv.values()).max(), want, 64, n, dtype == torch.bfloat16)
+        assert (np.abs(f64(out[i * count:(i + 1) * count]) - want) <= bound).all()

@@ -74,6 +74,25 @@ def test_against_the_formula(cuda_ok, rows, heads, kv_heads, dim, rotary, halves
         assert (err <= bound(x, w, rotary, 1e-5, want, bf16)).all()
 
 
+@pytest.mark.parametrize("theta", [1.0, 0.01, 1e6])
+def test_frequencies_of_any_base(cuda_ok, theta):
+    """Bases below 1 turn more than once a position; far and negative positions."""
+    rng = np.random.default_rng(7)
+    x = torch.tensor(rng.standard_normal((6, 1, 64)), dtype=torch.float32, device="cuda")
+    positions = np.array([0, 1, -1, 4_000_000, -77_777, 12])
+    pos = torch.tensor(positions, dtype=torch.int32, device="cuda")
+    out = torch.empty_like(x)
+    rt.QkNormRope(x.data_ptr(), None, out.data_ptr(), None, 6, 1, 0, 64, pos.data_ptr(), theta=theta)()
+    torch.cuda.synchronize()
+    theta = float(np.float32(theta))  # the argument is a float: 0.01 is not one
+    want = formula(x.double().cpu().numpy(), None, positions, 64, False, 1e-6, theta)
+    # a frequency f is within 2^-53 of itself (the library's exp2): |position| f 2^-52 of an angle, in either form
+    freq = theta ** (-np.arange(0, 64, 2) / 64)
+    slack = np.repeat(np.abs(positions)[:, None] * freq * 2.0 ** -51, 2, -1)[:, None] * np.abs(x.cpu().numpy()).max()
+    lim = bound(x.double().cpu().numpy(), None, 64, 1e-6, want, False) + slack
+    assert (np.abs(out.double().cpu().numpy() - want) <= lim).all()
+
+
 def test_in_place_on_a_stream_and_non_finite_rows(cuda_ok):
     rng = np.random.default_rng(5)
     x = torch.tensor(rng.standard_normal((40, 6, 64)), dtype=torch.float32, device="cuda")
