@@ -553,7 +553,22 @@ struct Kv8Attend {
     bool bf16;
 };
 
+// kWarps warps a CTA share an item's pages; kCtas CTAs of four warps (twice and
+// four times as many of two and one) are resident on an SM.
 template <int D, int NT, int PB, int kStages, int kMode, int kWarps, int kCtas>
+int kv8_launch_ctas(Kv8AttnParams p, long long items, long long splits, cudaStream_t s) {
+    constexpr int kRows = kMode == KV8_INT_BF16 || kMode == KV8_INT_F32 ? 4 : 8 * NT;
+    constexpr int smem = kWarps * std::max(kStages * PB * 2 * kKv8Block * D, kRows * D * 4);
+    auto kernel = kv8_attention_kernel<D, NT, PB, kStages, kMode, kWarps, kCtas * 4 / kWarps>;
+    if constexpr (smem > 46 * 1024) {  // 48 KB with the kernel's static arrays
+        static std::atomic<uint64_t> configured{0};
+        CUDA_TRY(opt_in_smem(reinterpret_cast<const void*>(kernel), smem, configured));
+    }
+    CUDA_TRY(launch_pdl(kernel, dim3(static_cast<unsigned>(items * splits)), dim3(32 * kWarps), smem, s, p));
+    return PHONON_CUDA_OK;
+}
+
+template <int D, int NT, int PB, int kStages, int kMode, int kCtas>
 int kv8_launch_attention(const Kv8Pool& c, uint32_t layer, const Kv8Seqs& seqs, const Kv8Attend& a,
                          const Kv8Scratch& w, int sms, cudaStream_t s) {
     constexpr int kRows = kMode == KV8_INT_BF16 || kMode == KV8_INT_F32 ? 4 : 8 * NT;
@@ -577,15 +592,17 @@ int kv8_launch_attention(const Kv8Pool& c, uint32_t layer, const Kv8Seqs& seqs, 
     long long span = seqs.max_length;
     if (a.window) span = std::min<long long>(span, static_cast<long long>(a.window) + (kRows - 1) / a.group + kKv8Block);
     const long long pages = std::max<long long>(1, (span + kKv8Block - 1) / kKv8Block);
-    // Splits cost a CTA's start and end (4 to 6 us of latency) each: down to
-    // kKv8MinPages pages while all CTAs are resident at once (8 streams of 8000
-    // positions: 9 splits 21 us, 19 splits 29 us), and into kKv8LongPages or more
-    // up to four times that, where a ragged batch's longest sequence would
-    // otherwise end alone (48 sequences of up to 4096 positions: 4 splits
-    // 51 us, 2 splits 59 us).
+    // Splits cost a CTA's start and end (4 to 6 us of latency) each. Few items:
+    // as many as keep all CTAs resident at once, of kKv8MinPages pages or more
+    // (8 streams of 8000 positions: 9 splits 21 us, 19 splits 29 us; 15 x 12 heads
+    // of 3864: 2 splits in one wave, 3 in two 53 us). Where the items alone fill
+    // most of the GPU: pieces of kKv8LongPages or more, up to four times what is
+    // resident, so that a ragged batch's longest sequence does not end alone (48
+    // sequences of up to 4096 positions: 4 splits 51 us, 2 splits 59 us).
     const long long resident = static_cast<long long>(kCtas) * sms;
     const long long splits = std::max<long long>(
-        1, std::max(std::min(resident / items, pages / kKv8MinPages), std::min(4 * resident / items, pages / kKv8LongPages)));
+        1, resident / items >= 2 ? std::min(resident / items, pages / kKv8MinPages)
+                                 : std::min(4 * resident / items, pages / kKv8LongPages));
     if (items * splits > INT32_MAX) return PHONON_CUDA_CAPACITY;
     if (splits > 1 && items * splits > w.max_splits) return PHONON_CUDA_CAPACITY;
     p.by_heads = kv8_divisor(c.heads);
@@ -596,35 +613,33 @@ int kv8_launch_attention(const Kv8Pool& c, uint32_t layer, const Kv8Seqs& seqs, 
     p.part = w.part;
     p.part_ml = w.ml;
     p.arrived = w.arrived;
-    constexpr int smem = kWarps * std::max(kStages * PB * 2 * kKv8Block * D, kRows * D * 4);
-    auto kernel = kv8_attention_kernel<D, NT, PB, kStages, kMode, kWarps, kCtas>;
-    if constexpr (smem > 46 * 1024) {  // 48 KB with the kernel's static arrays
-        static std::atomic<uint64_t> configured{0};
-        CUDA_TRY(opt_in_smem(reinterpret_cast<const void*>(kernel), smem, configured));
-    }
-    CUDA_TRY(launch_pdl(kernel, dim3(static_cast<unsigned>(items * splits)), dim3(32 * kWarps), smem, s, p));
-    return PHONON_CUDA_OK;
+    // Warps of an item: four read its pages four times as fast, but all of them
+    // start and end, and where items wait for one another a short item's start
+    // and end are most of it. One page each (373 sequences of one position: 4
+    // warps 13.2 us, 2 8.1, 1 5.7), up to 12 pages (500 of up to 185
+    // positions: 30.5, 22.5, 22.3), up to 31 (512 of 170 to 500: 50.4, 41.7,
+    // 43.4), up to 94 (512 of 500 to 1500: 98.1, 97.4, 111.5).
+    if (pages <= 8 && (items > resident || pages <= 2))
+        return kv8_launch_ctas<D, NT, PB, kStages, kMode, 1, kCtas>(p, items, splits, s);
+    if (pages <= 48 && items > resident) return kv8_launch_ctas<D, NT, PB, kStages, kMode, 2, kCtas>(p, items, splits, s);
+    return kv8_launch_ctas<D, NT, PB, kStages, kMode, 4, kCtas>(p, items, splits, s);
 }
 
 // By the rows that share a K/V head of a sequence: up to four multiply as
-// bytes, more as halves, 8 to 32 at a time.
+// bytes, more as halves, 8 or 16 at a time.
 template <int D>
 int kv8_attention_rows(const Kv8Pool& c, uint32_t layer, const Kv8Seqs& seqs, const Kv8Attend& a, const Kv8Scratch& w,
                        int sms, cudaStream_t s) {
     const long long rows = static_cast<long long>(seqs.max_rows) * a.group;
-    constexpr int PB = D == 128 ? 1 : 2;
+    constexpr int PB = D == 128 ? 1 : 2, kByteStages = D == 128 ? 2 : 3, kByteCtas = D == 128 ? 3 : 4;
     if (a.bf16) {
-        if (rows <= 4)
-            return kv8_launch_attention<D, 1, 2, D == 128 ? 2 : 3, KV8_INT_BF16, 4, D == 128 ? 3 : 4>(c, layer, seqs, a, w, sms, s);
-        if (rows <= 8) return kv8_launch_attention<D, 1, PB, 3, KV8_HALF_BF16, 4, 4>(c, layer, seqs, a, w, sms, s);
-        if (rows <= 16 || D == 128) return kv8_launch_attention<D, 2, 1, 3, KV8_HALF_BF16, 4, 4>(c, layer, seqs, a, w, sms, s);
-        if constexpr (D < 128) return kv8_launch_attention<D, 4, 1, 3, KV8_HALF_BF16, 4, 2>(c, layer, seqs, a, w, sms, s);
+        if (rows <= 4) return kv8_launch_attention<D, 1, 2, kByteStages, KV8_INT_BF16, kByteCtas>(c, layer, seqs, a, w, sms, s);
+        if (rows <= 8) return kv8_launch_attention<D, 1, PB, 3, KV8_HALF_BF16, 4>(c, layer, seqs, a, w, sms, s);
+        return kv8_launch_attention<D, 2, 1, 3, KV8_HALF_BF16, D == 128 ? 3 : 4>(c, layer, seqs, a, w, sms, s);
     }
-    if (rows <= 4)
-        return kv8_launch_attention<D, 1, 2, D == 128 ? 2 : 3, KV8_INT_F32, 4, D == 128 ? 3 : 4>(c, layer, seqs, a, w, sms, s);
-    if (rows <= 8) return kv8_launch_attention<D, 1, PB, 3, KV8_HALF_F32, 4, 4>(c, layer, seqs, a, w, sms, s);
-    if constexpr (D == 128) return kv8_launch_attention<D, 2, 1, 3, KV8_HALF_F32, 4, 3>(c, layer, seqs, a, w, sms, s);
-    else return kv8_launch_attention<D, 2, 2, 2, KV8_HALF_F32, 4, 3>(c, layer, seqs, a, w, sms, s);
+    if (rows <= 4) return kv8_launch_attention<D, 1, 2, kByteStages, KV8_INT_F32, kByteCtas>(c, layer, seqs, a, w, sms, s);
+    if (rows <= 8) return kv8_launch_attention<D, 1, PB, 3, KV8_HALF_F32, D == 128 ? 3 : 4>(c, layer, seqs, a, w, sms, s);
+    return kv8_launch_attention<D, 2, PB, 2, KV8_HALF_F32, 3>(c, layer, seqs, a, w, sms, s);
 }
 
 int kv8_enqueue_attention(const Kv8Pool& c, uint32_t layer, const Kv8Seqs& seqs, const Kv8Attend& a,
