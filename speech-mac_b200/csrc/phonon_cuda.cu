@@ -9,6 +9,7 @@
 #include "phonon_head.cuh"
 #include "phonon_mimi.cuh"
 #include "phonon_kv8.cuh"
+#include "phonon_kv8_prompt.cuh"
 #include "phonon_qk.cuh"
 
 #include <cuda_fp16.h>
@@ -52,6 +53,9 @@ constexpr int kSplitMinBatch = 96;   // from here a step runs as two concurrent 
 constexpr int kKv8Ctas = 5;          // 8-bit attention: resident CTAs per SM, at most
 constexpr int kKv8MinPages = 8;      // ... pages per split, at least (two a warp)
 constexpr int kKv8LongPages = 64;    // ... of a call whose CTAs are not all resident
+constexpr int kKv8PromptRows = 64;   // the 128-row attention: rows of a K/V head of a sequence on average, at least
+constexpr int kKv8PromptWork = 6;    // ... 128-row, 128-position products per SM, at least
+constexpr int kKv8PromptMinPages = 64, kKv8PromptLongPages = 64;  // ... pages per split, at least
 constexpr int kKv8TileFloats = 2048; // ... outputs of a row tile, at most
 
 #define CUDA_TRY(expr)                                                                       \
@@ -568,12 +572,21 @@ int kv8_launch_ctas(Kv8AttnParams p, long long items, long long splits, cudaStre
     return PHONON_CUDA_OK;
 }
 
-template <int D, int NT, int PB, int kStages, int kMode, int kCtas>
-int kv8_launch_attention(const Kv8Pool& c, uint32_t layer, const Kv8Seqs& seqs, const Kv8Attend& a,
-                         const Kv8Scratch& w, int sms, cudaStream_t s) {
-    constexpr int kRows = kMode == KV8_INT_BF16 || kMode == KV8_INT_F32 ? 4 : 8 * NT;
-    static_assert(kRows * D <= kKv8TileFloats && kCtas <= kKv8Ctas, "a partial result outgrows its scratch");
-    Kv8AttnParams p{};
+// Pages that a tile of rows can see, at most.
+long long kv8_pages(const Kv8Seqs& seqs, const Kv8Attend& a, int tile_rows) {
+    long long span = seqs.max_length;
+    if (a.window) span = std::min<long long>(span, static_cast<long long>(a.window) + (tile_rows - 1) / a.group + kKv8Block);
+    return std::max<long long>(1, (span + kKv8Block - 1) / kKv8Block);
+}
+
+// Kernel parameters of a call in row tiles of `tile_rows`, with `resident`
+// CTAs on the GPU at once. *items: (sequence, row tile, K/V head); their
+// splits have few_pages pages or more where there are few items, long_pages
+// where there are many.
+int kv8_plan(const Kv8Pool& c, uint32_t layer, const Kv8Seqs& seqs, const Kv8Attend& a, const Kv8Scratch& w,
+             int tile_rows, long long resident, long long few_pages, long long long_pages, Kv8AttnParams* out,
+             long long* n_items, long long* n_pages) {
+    Kv8AttnParams& p = *out;
     p.cache = c.view(layer);
     p.seqs = seqs;
     p.q = a.q;
@@ -586,33 +599,48 @@ int kv8_launch_attention(const Kv8Pool& c, uint32_t layer, const Kv8Seqs& seqs, 
     p.scale_low = static_cast<float>(scale - p.scale);
     p.window = a.window;
     const long long rows = static_cast<long long>(seqs.max_rows) * a.group;
-    const long long tiles = (rows + kRows - 1) / kRows;
+    const long long tiles = (rows + tile_rows - 1) / tile_rows;
     const long long items = seqs.n * tiles * c.heads;
-    // pages that a row tile can see
-    long long span = seqs.max_length;
-    if (a.window) span = std::min<long long>(span, static_cast<long long>(a.window) + (kRows - 1) / a.group + kKv8Block);
-    const long long pages = std::max<long long>(1, (span + kKv8Block - 1) / kKv8Block);
-    // Splits cost a CTA's start and end (4 to 6 us of latency) each. Few items:
-    // as many as keep all CTAs resident at once, of kKv8MinPages pages or more
-    // (8 streams of 8000 positions: 9 splits 21 us, 19 splits 29 us; 15 x 12 heads
-    // of 3864: 2 splits in one wave, 3 in two 53 us). Where the items alone fill
-    // most of the GPU: pieces of kKv8LongPages or more, up to four times what is
-    // resident, so that a ragged batch's longest sequence does not end alone (48
-    // sequences of up to 4096 positions: 4 splits 51 us, 2 splits 59 us).
-    const long long resident = static_cast<long long>(kCtas) * sms;
-    const long long splits = std::max<long long>(
-        1, resident / items >= 2 ? std::min(resident / items, pages / kKv8MinPages)
-                                 : std::min(4 * resident / items, pages / kKv8LongPages));
+    const long long pages = kv8_pages(seqs, a, tile_rows);
+    long long splits = resident / items >= 2 ? std::min(resident / items, pages / few_pages)
+                                             : std::min(4 * resident / items, pages / long_pages);
+    // what the scratch holds
+    const long long most = std::min<long long>(w.max_splits, static_cast<long long>(w.max_splits) * kKv8TileFloats /
+                                                                 (static_cast<long long>(tile_rows) * c.dim));
+    splits = std::max<long long>(1, std::min(splits, std::min(most, w.max_splits * 32ll / tile_rows) / items));
     if (items * splits > INT32_MAX) return PHONON_CUDA_CAPACITY;
-    if (splits > 1 && items * splits > w.max_splits) return PHONON_CUDA_CAPACITY;
     p.by_heads = kv8_divisor(c.heads);
     p.by_items = kv8_divisor(static_cast<uint32_t>(items));
     p.splits = static_cast<int>(splits);
     p.by_tiles = kv8_divisor(static_cast<uint32_t>(tiles));
     p.split_pages = static_cast<int>((pages + splits - 1) / splits);
+    p.tile_rows = tile_rows;
     p.part = w.part;
     p.part_ml = w.ml;
     p.arrived = w.arrived;
+    *n_items = items;
+    *n_pages = pages;
+    return PHONON_CUDA_OK;
+}
+
+// Splits cost a CTA's start and end (4 to 6 us of latency) each. Few items:
+// as many as keep all CTAs resident at once, of kKv8MinPages pages or more
+// (8 streams of 8000 positions: 9 splits 21 us, 19 splits 29 us; 15 x 12 heads
+// of 3864: 2 splits in one wave 41.5 us, 3 in two 53). Where the items alone
+// fill most of the GPU: pieces of kKv8LongPages or more, up to four times what
+// is resident, so that a ragged batch's longest sequence does not end alone (48
+// sequences of up to 4096 positions: 4 splits 51 us, 2 splits 59 us).
+template <int D, int NT, int PB, int kStages, int kMode, int kCtas>
+int kv8_launch_attention(const Kv8Pool& c, uint32_t layer, const Kv8Seqs& seqs, const Kv8Attend& a,
+                         const Kv8Scratch& w, int sms, cudaStream_t s) {
+    constexpr int kRows = kMode == KV8_INT_BF16 || kMode == KV8_INT_F32 ? 4 : 8 * NT;
+    static_assert(kRows * D <= kKv8TileFloats && kCtas <= kKv8Ctas, "a partial result outgrows its scratch");
+    Kv8AttnParams p{};
+    long long items = 0, pages = 0;
+    const long long resident = static_cast<long long>(kCtas) * sms;
+    const int rc = kv8_plan(c, layer, seqs, a, w, kRows, resident, kKv8MinPages, kKv8LongPages, &p, &items, &pages);
+    if (rc != PHONON_CUDA_OK) return rc;
+    const long long splits = p.splits;
     // Warps of an item: four read its pages four times as fast, but all of them
     // start and end, and where items wait for one another a short item's start
     // and end are most of it. One page each (373 sequences of one position: 4
@@ -625,12 +653,53 @@ int kv8_launch_attention(const Kv8Pool& c, uint32_t layer, const Kv8Seqs& seqs, 
     return kv8_launch_ctas<D, NT, PB, kStages, kMode, 4, kCtas>(p, items, splits, s);
 }
 
+// Many rows: one CTA an SM.
+template <int D, bool kBf16>
+int kv8_launch_prompt(const Kv8Pool& c, uint32_t layer, const Kv8Seqs& seqs, const Kv8Attend& a, const Kv8Scratch& w,
+                      int sms, cudaStream_t s) {
+    Kv8AttnParams p{};
+    long long items = 0, pages = 0;
+    // Two row tiles in a CTA share the conversion of their keys and values (a
+    // turn of both takes 1.74 times one's), one leaves more CTAs.
+    int tile_rows = 128;
+    if constexpr (kv8_prompt_rows<D, kBf16>() == 256) {
+        const long long rows = static_cast<long long>(seqs.max_rows) * a.group, each = static_cast<long long>(seqs.n) * c.heads;
+        const long long waves = (each * ((rows + 127) / 128) + sms - 1) / sms, waves2 = (each * ((rows + 255) / 256) + sms - 1) / sms;
+        if (174 * waves2 < 100 * waves) tile_rows = 256;
+    }
+    const int rc = kv8_plan(c, layer, seqs, a, w, tile_rows, sms, kKv8PromptMinPages, kKv8PromptLongPages, &p, &items, &pages);
+    if (rc != PHONON_CUDA_OK) return rc;
+    constexpr int smem = kv8_prompt_smem<D, kBf16>();
+    auto kernel = kv8_prompt_kernel<D, kBf16>;
+    if constexpr (smem > 40 * 1024) {  // 48 KB with the kernel's static arrays
+        static std::atomic<uint64_t> configured{0};
+        CUDA_TRY(opt_in_smem(reinterpret_cast<const void*>(kernel), smem, configured));
+    }
+    CUDA_TRY(launch_pdl(kernel, dim3(static_cast<unsigned>(items * p.splits)), dim3(kKv8PromptThreads), smem, s, p));
+    return PHONON_CUDA_OK;
+}
+
 // By the rows that share a K/V head of a sequence: up to four multiply as
-// bytes, more as halves, 8 or 16 at a time.
+// bytes, more as halves, 8 or 16 at a time. From 64 rows on average, where the
+// products fill the GPU (kKv8PromptWork): 128 rows at a time on the tcgen05
+// tensor cores, whose CTA of 512 threads starts and ends in 8 us and takes 2.3
+// us a 128 x 128 product of 64 fp32 dims, however few of the rows there are. us
+// of the 128-row kernel and the other; rows x positions, K/V heads of all
+// sequences (products an SM): fp32, 64 dims: 128 x 1024, 32 heads (1.7) 25.7
+// and 19.3; 256 x 1024, 32 (3.5) 25.9 and 27.9; 1 to 256 rows of 300 to 2048
+// positions, 32 (4.1 by the longest) 30.4 and 27.7; 128 x 1024, 128 (6.9) 26.8 and 45.3; 1024
+// x 4096, 32 (55) 156 and 265; 64 x 1024, 128 25.3 and 28.9, where 1 to 64 rows
+// of 16 to 700 positions, 512 heads, take 52 and 34. bf16, 128 dims: 128 x
+// 1024, 32 30.4 and 25.8; 512 x 2048, 32 74 and 124; 1024 x 4096, 32 134 and 353.
 template <int D>
 int kv8_attention_rows(const Kv8Pool& c, uint32_t layer, const Kv8Seqs& seqs, const Kv8Attend& a, const Kv8Scratch& w,
                        int sms, cudaStream_t s) {
     const long long rows = static_cast<long long>(seqs.max_rows) * a.group;
+    const double all_rows = static_cast<double>(seqs.rows) * a.group;
+    const double products = all_rows * c.heads * kv8_pages(seqs, a, 256) / (128.0 * (kKv8PromptKeys / kKv8Block));
+    if (all_rows >= static_cast<double>(kKv8PromptRows) * seqs.n && products >= kKv8PromptWork * static_cast<double>(sms))
+        return a.bf16 ? kv8_launch_prompt<D, true>(c, layer, seqs, a, w, sms, s)
+                      : kv8_launch_prompt<D, false>(c, layer, seqs, a, w, sms, s);
     constexpr int PB = D == 128 ? 1 : 2, kByteStages = D == 128 ? 2 : 3, kByteCtas = D == 128 ? 3 : 4;
     if (a.bf16) {
         if (rows <= 4) return kv8_launch_attention<D, 1, 2, kByteStages, KV8_INT_BF16, kByteCtas>(c, layer, seqs, a, w, sms, s);

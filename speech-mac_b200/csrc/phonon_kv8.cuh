@@ -531,6 +531,7 @@ struct Kv8AttnParams {
     Kv8Div by_items, by_heads, by_tiles;  // (sequence, row tile, K/V head) items; K/V heads; row tiles of a sequence
     int splits;                            // of an item, at most
     int split_pages;                       // pages of a split
+    int tile_rows;                         // rows of a row tile
     float* part;                     // [items * splits][rows of a tile][D]
     float4* part_ml;                 // [items * splits][rows of a tile]: M, sum, eV's reference
     unsigned* arrived;               // [items], zero between launches
@@ -618,6 +619,112 @@ __device__ __forceinline__ uint32_t half2_bits(float a, float b) {
 }
 
 __device__ __forceinline__ float2 half2_floats(uint32_t u) { return __half22float2(*reinterpret_cast<__half2*>(&u)); }
+
+// M, sum, reference of eV and four dims of a row, over some of its positions.
+struct Kv8Share {
+    float m, l;
+    int ref;
+    float4 a;
+};
+
+__device__ __forceinline__ Kv8Share kv8_nothing() { return {-INFINITY, 0.0f, 127, make_float4(0.0f, 0.0f, 0.0f, 0.0f)}; }
+
+__device__ __forceinline__ void kv8_fold(Kv8Share& s, float4 ml, float4 b) {
+    if (s.m == -INFINITY && !isnan(s.l)) s.ref = __float_as_int(ml.z);  // nothing yet: as it comes
+    // into s's reference (an exact power of two, and 0 to add where the references agree), then the larger maximum
+    const int shift = __float_as_int(ml.z) - s.ref;
+    const float m2 = ml.x + static_cast<float>(shift), x = fmaxf(s.m, m2);
+    const float wa = s.m == -INFINITY ? 0.0f : ex2(s.m - x), wb = m2 == -INFINITY ? 0.0f : ex2(m2 - x);
+    s.m = x;
+    s.l = s.l * wa + ml.y * (pow2i(min(max(-shift, -126), 126)) * wb);
+    s.a = make_float4(s.a.x * wa + b.x * wb, s.a.y * wa + b.y * wb, s.a.z * wa + b.z * wb, s.a.w * wa + b.w * wb);
+}
+
+// Four dims of row rho of a K/V head's rows, to the output.
+template <int D, bool kBf16>
+__device__ __forceinline__ void kv8_store(const Kv8AttnParams& p, int row0, int rho, int head, int d, float4 v) {
+    const int at = static_cast<int>(kv8_div(rho, p.group));
+    store_row4<kBf16>(p.out, static_cast<size_t>(row0 + at) * p.out_stride + static_cast<size_t>(head * p.group.d + rho - at * p.group.d) * D + d, v);
+}
+
+// What turns a row's sums into its output; unit: what a weight of 1 is held as, inverted.
+__device__ __forceinline__ float kv8_inverse(float l, int ref, float unit) {
+    return l > 0.0f || isnan(l) ? __fdiv_rn(pow2i(ref - 127) * unit, l) : 0.0f;
+}
+
+// The end of a split item, after the CTA has written its shares to the
+// scratch: the split that arrives last merges all of them, in their order, so
+// that results do not depend on who arrives when. Threads 0 to kThreads - 1,
+// whose barrier is sync; `scratch`: 2 * kThreads float4 of shared memory.
+template <int D, bool kBf16, int kThreads, int kCells, typename Sync>
+__device__ __forceinline__ void kv8_merge(const Kv8AttnParams& p, float unit, const Sync& sync, float4* scratch, int* s_last, uint32_t item,
+                                          int active, int tile_rows, int n_rows, int row0, int rho0, int head) {
+    constexpr int kQuads = D / 4;
+    const size_t slot = static_cast<size_t>(item) * p.splits;
+    const auto finish = [&](int cell, const Kv8Share& s) {
+        const int d = cell % kQuads * 4;
+        const float inv = kv8_inverse(s.l, s.ref, unit);
+        kv8_store<D, kBf16>(p, row0, rho0 + cell / kQuads, head, d, make_float4(s.a.x * inv, s.a.y * inv, s.a.z * inv, s.a.w * inv));
+    };
+    sync();
+    if (threadIdx.x == 0) {
+        unsigned n;  // releases the CTA's partial results (ordered before by the barrier), acquires the others'
+        asm volatile("atom.acq_rel.gpu.global.add.u32 %0, [%1], 1;" : "=r"(n) : "l"(p.arrived + item) : "memory");
+        *s_last = n + 1 == static_cast<unsigned>(active);
+        if (*s_last) p.arrived[item] = 0;
+    }
+    sync();
+    if (!*s_last) return;
+    // Few rows: the threads share a row's splits, each every subs-th, and the
+    // subs meet in shared memory; four splits of kCells cells (four dims of a
+    // row) are loaded at a time.
+    const int cells = n_rows * kQuads, subs = max(1, min(active, kThreads / cells));
+    for (int x0 = threadIdx.x; x0 < cells * subs; x0 += kCells * kThreads) {
+        Kv8Share s[kCells];
+        int at[kCells], sub[kCells];
+#pragma unroll
+        for (int c = 0; c < kCells; ++c) {
+            const int x = min(x0 + c * kThreads, cells * subs - 1);
+            sub[c] = x / cells;
+            at[c] = x - sub[c] * cells;
+            s[c] = kv8_nothing();
+        }
+        for (int step = 0; step < active; step += 4 * subs) {
+            float4 ml[kCells][4], a[kCells][4];
+#pragma unroll
+            for (int c = 0; c < kCells; ++c)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const size_t at_part = (slot + min(step + sub[c] + k * subs, active - 1)) * tile_rows + at[c] / kQuads;
+                    ml[c][k] = __ldcg(p.part_ml + at_part);
+                    a[c][k] = __ldcg(reinterpret_cast<const float4*>(p.part + at_part * D + at[c] % kQuads * 4));
+                }
+#pragma unroll
+            for (int c = 0; c < kCells; ++c)
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    if (step + sub[c] + k * subs < active) kv8_fold(s[c], ml[c][k], a[c][k]);
+        }
+#pragma unroll
+        for (int c = 0; c < kCells; ++c) {
+            const int x = x0 + c * kThreads;
+            if (x >= cells * subs) break;
+            if (subs == 1) {
+                finish(at[c], s[c]);
+            } else {
+                scratch[x] = s[c].a;
+                scratch[cells * subs + x] = make_float4(s[c].m, s[c].l, __int_as_float(s[c].ref), 0.0f);
+            }
+        }
+    }
+    if (subs == 1) return;
+    sync();
+    for (int cell = threadIdx.x; cell < cells; cell += kThreads) {
+        Kv8Share s = kv8_nothing();
+        for (int sub = 0; sub < subs; ++sub) kv8_fold(s, scratch[cells * subs + sub * cells + cell], scratch[sub * cells + cell]);
+        finish(cell, s);
+    }
+}
 
 // A lane's share of a block: its keys are D/4 dims of positions g, g + 8 (the
 // t-th 16 bytes of each 64; 8 of 32 where D is 32), its values D/32 chunks of
@@ -1108,88 +1215,24 @@ __global__ void __launch_bounds__(32 * kWarps, kCtas) kv8_attention_kernel(Kv8At
         }
     __syncthreads();
     constexpr int kQuads = D / 4;
-    constexpr float kUnit = kInt ? 1.0f / kKv8FixedScale : 1.0f;  // of the held weights
-    struct Share {  // M, sum, reference and four dims of a row
-        float m, l;
-        int ref;
-        float4 a;
-    };
-    auto nothing = [] { return Share{-INFINITY, 0.0f, 127, make_float4(0.0f, 0.0f, 0.0f, 0.0f)}; };
-    auto fold = [](Share& s, float4 ml, float4 b) {
-        if (s.m == -INFINITY && !isnan(s.l)) s.ref = __float_as_int(ml.z);  // nothing yet: as it comes
-        // into s's reference (an exact power of two, and 0 to add where the references agree), then the larger maximum
-        const int shift = __float_as_int(ml.z) - s.ref;
-        const float m2 = ml.x + static_cast<float>(shift), x = fmaxf(s.m, m2);
-        const float wa = s.m == -INFINITY ? 0.0f : ex2(s.m - x), wb = m2 == -INFINITY ? 0.0f : ex2(m2 - x);
-        s.m = x;
-        s.l = s.l * wa + ml.y * (pow2i(min(max(-shift, -126), 126)) * wb);
-        s.a = make_float4(s.a.x * wa + b.x * wb, s.a.y * wa + b.y * wb, s.a.z * wa + b.z * wb, s.a.w * wa + b.w * wb);
-    };
-    auto finish = [&](int r, int d, const Share& s) {
-        const float inv = s.l > 0.0f || isnan(s.l) ? __fdiv_rn(pow2i(s.ref - 127) * kUnit, s.l) : 0.0f;
-        const int rho = rho0 + r, at = token(rho);
-        store_row4<kBf16>(p.out,
-                          static_cast<size_t>(sq.row0 + at) * p.out_stride +
-                              static_cast<size_t>(head * p.group.d + rho - at * p.group.d) * D + d,
-                          make_float4(s.a.x * inv, s.a.y * inv, s.a.z * inv, s.a.w * inv));
-    };
-    const size_t slot = static_cast<size_t>(item) * p.splits;
-    for (int x = threadIdx.x; x < n_rows * kQuads; x += blockDim.x) {
+    constexpr float kUnit = kInt ? 1.0f / kKv8FixedScale : 1.0f;
+    for (int x = threadIdx.x; x < n_rows * kQuads; x += 32 * kWarps) {
         const int r = x / kQuads, d = x % kQuads * 4;
-        Share s = nothing();
+        Kv8Share s = kv8_nothing();
 #pragma unroll
-        for (int w = 0; w < kWarps; ++w) fold(s, s_ml[w][r], *reinterpret_cast<const float4*>(&s_o[w][r][d]));
+        for (int w = 0; w < kWarps; ++w) kv8_fold(s, s_ml[w][r], *reinterpret_cast<const float4*>(&s_o[w][r][d]));
         if (active == 1) {
-            finish(r, d, s);
+            const float inv = kv8_inverse(s.l, s.ref, kUnit);
+            kv8_store<D, kBf16>(p, sq.row0, rho0 + r, head, d, make_float4(s.a.x * inv, s.a.y * inv, s.a.z * inv, s.a.w * inv));
         } else {
-            const size_t at_part = (slot + split) * kRows + r;
+            const size_t at_part = (static_cast<size_t>(item) * p.splits + split) * kRows + r;
             *reinterpret_cast<float4*>(p.part + at_part * D + d) = s.a;
             if (d == 0) p.part_ml[at_part] = make_float4(s.m, s.l, __int_as_float(s.ref), 0.0f);
         }
     }
     if (active == 1) return;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        unsigned n;  // releases the CTA's partial results (ordered before by the barrier), acquires the others'
-        asm volatile("atom.acq_rel.gpu.global.add.u32 %0, [%1], 1;" : "=r"(n) : "l"(p.arrived + item) : "memory");
-        s_last = n + 1 == static_cast<unsigned>(active);
-        if (s_last) p.arrived[item] = 0;
-    }
-    __syncthreads();
-    if (!s_last) return;
-    // Few rows: the threads share a row's splits, each every subs-th, and the
-    // subs meet in shared memory; four splits are loaded at a time.
-    const int cells = n_rows * kQuads, subs = max(1, min(active, 32 * kWarps / cells));
-    float4* s_a = reinterpret_cast<float4*>(s_ring);  // [subs][cells]; the warps' results have been read
-    for (int x = threadIdx.x; x < cells * subs; x += blockDim.x) {
-        const int sub = x / cells, cell = x - sub * cells, r = cell / kQuads, d = cell % kQuads * 4;
-        Share s = nothing();
-        for (int k0 = sub; k0 < active; k0 += 4 * subs) {
-            float4 ml[4], a[4];
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const size_t at_part = (slot + min(k0 + k * subs, active - 1)) * kRows + r;
-                ml[k] = __ldcg(p.part_ml + at_part);
-                a[k] = __ldcg(reinterpret_cast<const float4*>(p.part + at_part * D + d));
-            }
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-                if (k0 + k * subs < active) fold(s, ml[k], a[k]);
-        }
-        if (subs == 1) {
-            finish(r, d, s);
-        } else {
-            s_a[x] = s.a;
-            s_a[cells * subs + x] = make_float4(s.m, s.l, __int_as_float(s.ref), 0.0f);
-        }
-    }
-    if (subs == 1) return;
-    __syncthreads();
-    for (int cell = threadIdx.x; cell < cells; cell += blockDim.x) {
-        Share s = nothing();
-        for (int sub = 0; sub < subs; ++sub) fold(s, s_a[cells * subs + sub * cells + cell], s_a[sub * cells + cell]);
-        finish(cell / kQuads, cell % kQuads * 4, s);
-    }
+    kv8_merge<D, kBf16, 32 * kWarps, 1>(p, kUnit, [] { __syncthreads(); }, reinterpret_cast<float4*>(s_ring), &s_last, item, active, kRows,
+                                        n_rows, sq.row0, rho0, head);
 }
 
 }  // namespace phonon

@@ -543,3 +543,127 @@ def test_all_keys_alike_and_one_key_far_ahead(cuda_ok, group, count, dtype):
         want, size = model.attention(part, hk.values(), hv.values())
         bound = model.attention_bound(size, np.abs(hv.values()).max(), want, 64, n, dtype == torch.bfloat16)
         assert (np.abs(f64(out[i * count:(i + 1) * count]) - want) <= bound).all()
+
+
+# ------------------------------------------- many rows (the 128-row kernel)
+# Calls with work enough for it: all rows * query heads * pages of the longest
+# 909312 or more (148 SMs), 64 rows of a K/V head or more. Row tiles of one row, of 128 and of
+# 129 to 256 (two streams); splits; every tile edge among the lengths.
+MANY = [
+    # kv_heads, group, dim, lengths, rows, window
+    (2, 1, 64, [4100, 1, 0, 16, 17, 127, 128, 129, 300, 2048, 5, 5, 5, 31, 33], 128, 0),
+    (1, 8, 128, [2000, 20, 1, 513] * 6, 40, 0),
+    (3, 1, 32, [1500, 129, 300, 0] * 8, 129, 0),
+    (2, 3, 64, [1000, 90, 33] * 20, 43, 0),
+    (8, 2, 64, [600, 30, 599] * 14, 100, 77),
+    (1, 5, 32, [8000], 400, 0),
+    (4, 1, 128, [8190], 450, 0),
+    (8, 1, 64, [300, 17, 2] * 36, 64, 1),
+    (2, 4, 128, [260, 1100] * 16, 100, 500),
+    (4, 64, 64, [1333, 5] * 22, 1, 0),
+    (8, 1, 128, [640, 641, 255] * 16, 256, 0),
+]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("kv_heads,group,dim,lengths,count,window", MANY)
+def test_many_rows_against_the_definition(cuda_ok, kv_heads, group, dim, lengths, count, window, dtype):
+    test_attention_against_the_definition(cuda_ok, kv_heads, group, dim, lengths, count, window, dtype)
+
+
+@pytest.mark.parametrize("dim", [32, 64, 128])
+def test_many_rows_of_bad_q_and_bad_pages(cuda_ok, dim):
+    """A row of q that is not finite is NaN and flagged, alone; a page id outside the pool hides its positions."""
+    rng = np.random.default_rng(18)
+    lengths, count = [300, 420] + [1000] * 60, 130
+    c = Cache(2, dim, lengths)
+    new = [[rows(rng, n, 2, dim) for n in lengths] for _ in range(2)]
+    c.append(lengths, *new)
+    held = [[model.Held(2, dim) for _ in range(2)] for _ in range(2)]
+    for w in range(2):
+        for h, r in zip(held[w], new[w]):
+            h.append(f64(r))
+    q = rows(rng, len(lengths) * count, 2, dim)
+    q[5, 0, 3] = float("inf")
+    q[129, 1, dim - 1] = float("nan")
+    c.table[1, 2] = c.pool  # positions 32..47 of the second sequence
+    out = torch.empty_like(q)
+    status = torch.zeros(len(lengths), dtype=torch.int32, device="cuda")
+    ws = rt.Kv8Workspace(c.kv)
+    c.kv.attention(c.batch(lengths, [count] * len(lengths)), rt.kv8_query(q.data_ptr(), out.data_ptr(), heads=2), ws,
+                   status_ptr=status.data_ptr())
+    torch.cuda.synchronize()
+    assert status.tolist() == [rt.NON_FINITE, rt.INVALID] + [0] * 60
+    got = f64(out)
+    bad = np.zeros((len(got), 2), bool)
+    bad[5, 0] = bad[129, 1] = True
+    assert np.isnan(got[bad]).all() and np.isfinite(got[~bad]).all()
+    good = np.where(bad[:, :, None], 0.0, f64(q))
+    for i, n in enumerate(lengths[:2]):
+        k, v = held[0][i].values(), held[1][i].values()
+        part = good[i * count:(i + 1) * count]
+        want, size = model.attention(part, k, v)
+        if i == 1:  # every row sees position 47: without them the sequence is 16 positions shorter
+            keep = np.r_[0:32, 48:n]
+            want, _ = model.attention(part, k[keep], v[keep])
+        bound = model.attention_bound(size, np.abs(v).max(), want, dim, n, False)
+        ok = ~bad[i * count:(i + 1) * count]
+        assert (np.abs(got[i * count:(i + 1) * count] - want) <= bound)[ok].all()
+
+
+def test_many_rows_scaled_strided_and_very_different_blocks(cuda_ok):
+    """A scale, rows inside wider ones, and values and scores over a wide range."""
+    rng = np.random.default_rng(20)
+    lengths, count = [200, 77] + [1000] * 28, 256
+    c = Cache(2, 64, lengths)
+    keys = [rows(rng, n, 2, 64) for n in lengths]
+    values = [rows(rng, n, 2, 64) * torch.exp2(torch.randint(-30, 31, (n, 1, 1), device="cuda")).float() for n in lengths]
+    c.append(lengths, keys, values)
+    q = rows(rng, len(lengths) * count, 6, 64)  # 2 heads of queries, 2 of outputs, 2 untouched
+    before = q.clone()
+    ws = rt.Kv8Workspace(c.kv)
+    c.kv.attention(c.batch(lengths, [count] * len(lengths)),
+                   rt.kv8_query(q.data_ptr(), q.data_ptr() + 2 * 64 * 4, heads=2, scale=0.7, q_stride=384, out_stride=384), ws)
+    torch.cuda.synchronize()
+    assert torch.equal(q[:, :2], before[:, :2]) and torch.equal(q[:, 4:], before[:, 4:])
+    for i, n in enumerate(lengths[:3]):
+        hk, hv = model.Held(2, 64), model.Held(2, 64)
+        hk.append(f64(keys[i]))
+        hv.append(f64(values[i]))
+        want, size = model.attention(f64(before[i * count:(i + 1) * count, :2]), hk.values(), hv.values(), scale=0.7)
+        biggest = np.maximum.accumulate(np.abs(hv.values()).max((1, 2)))  # among what a row sees
+        seen = np.arange(n - count, n)
+        most = np.where(seen >= 0, biggest[np.maximum(seen, 0)], 0.0)[:, None, None]
+        bound = model.attention_bound(size, 1.0, 0 * want, 64, n, False) * most + 2.0 ** -23 * np.abs(want)
+        assert (np.abs(f64(q[i * count:(i + 1) * count, 2:4]) - want) <= bound).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_many_rows_repeat_bit_for_bit_and_in_graphs(cuda_ok, dtype):
+    """Split and unsplit calls: the same bits from every call and replay, whichever split arrives last."""
+    rng = np.random.default_rng(19)
+    kind = rt.ROWS_BF16 if dtype == torch.bfloat16 else rt.ROWS_F32
+    for kv_heads, lengths, count in ((4, [8000], 480), (8, [700, 20, 350, 900] * 8, 70)):
+        c = Cache(kv_heads, 64, lengths)
+        c.append(lengths, *[[rows(rng, n, kv_heads, 64, dtype) for n in lengths] for _ in range(2)])
+        q = rows(rng, count * len(lengths), kv_heads, 64, dtype)
+        ws = rt.Kv8Workspace(c.kv)
+        outs = [torch.empty_like(q) for _ in range(3)]
+        batch = c.batch(lengths, [count] * len(lengths))
+
+        def call(out, stream=0):
+            c.kv.attention(batch, rt.kv8_query(q.data_ptr(), out.data_ptr(), kind, heads=kv_heads), ws, stream_ptr=stream)
+
+        call(outs[0])
+        torch.cuda.synchronize()
+        stream = torch.cuda.Stream()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            call(outs[1], torch.cuda.current_stream().cuda_stream)
+            call(outs[2], torch.cuda.current_stream().cuda_stream)
+        for _ in range(5):
+            outs[1].zero_()
+            outs[2].zero_()
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(outs[0], outs[1]) and torch.equal(outs[0], outs[2])
