@@ -660,7 +660,8 @@ int kv8_launch_prompt(const Kv8Pool& c, uint32_t layer, const Kv8Seqs& seqs, con
     Kv8AttnParams p{};
     long long items = 0, pages = 0;
     // Two row tiles in a CTA share the conversion of their keys and values (a
-    // turn of both takes 1.74 times one's), one leaves more CTAs.
+    // turn of both takes 1.74 times one's), one leaves more CTAs (fp32, 64 dims,
+    // 256 x 1024, 32 heads: one a CTA 25.9 us, two 44; 1024 x 1024, 128: two 166, one 193).
     int tile_rows = 128;
     if constexpr (kv8_prompt_rows<D, kBf16>() == 256) {
         const long long rows = static_cast<long long>(seqs.max_rows) * a.group, each = static_cast<long long>(seqs.n) * c.heads;
@@ -682,21 +683,21 @@ int kv8_launch_prompt(const Kv8Pool& c, uint32_t layer, const Kv8Seqs& seqs, con
 // By the rows that share a K/V head of a sequence: up to four multiply as
 // bytes, more as halves, 8 or 16 at a time. From 64 rows on average, where the
 // products fill the GPU (kKv8PromptWork): 128 rows at a time on the tcgen05
-// tensor cores, whose CTA of 512 threads starts and ends in 8 us and takes 2.3
-// us a 128 x 128 product of 64 fp32 dims, however few of the rows there are. us
-// of the 128-row kernel and the other; rows x positions, K/V heads of all
-// sequences (products an SM): fp32, 64 dims: 128 x 1024, 32 heads (1.7) 25.7
-// and 19.3; 256 x 1024, 32 (3.5) 25.9 and 27.9; 1 to 256 rows of 300 to 2048
-// positions, 32 (4.1 by the longest) 30.4 and 27.7; 128 x 1024, 128 (6.9) 26.8 and 45.3; 1024
-// x 4096, 32 (55) 156 and 265; 64 x 1024, 128 25.3 and 28.9, where 1 to 64 rows
-// of 16 to 700 positions, 512 heads, take 52 and 34. bf16, 128 dims: 128 x
-// 1024, 32 30.4 and 25.8; 512 x 2048, 32 74 and 124; 1024 x 4096, 32 134 and 353.
+// tensor cores, whose CTA of 512 threads starts and ends in 6 us and works on
+// 128 rows however few there are. us of the 128-row kernel and the other; rows x
+// positions, K/V heads of all sequences (products an SM): fp32, 64 dims: 128 x
+// 1024, 32 heads (1.7) 25.7 and 19.3; 256 x 1024, 32 (3.5) 25.9 and 27.9; 1 to
+// 256 rows of 300 to 2048 positions, 32 (4.1 by the longest) 30.4 and 27.7; 128
+// x 1024, 128 (6.9) 22.6 and 45.3; 1024 x 4096, 32 (55) 136 and 265; 1 to 64
+// rows of 16 to 700 positions, 512 heads, 52 and 34. bf16, 128 dims: 128 x
+// 1024, 32 30.4 and 25.8; up to 1024 x 2048, 32 77 and 124; 1024 x 4096, 32 144
+// and 353.
 template <int D>
 int kv8_attention_rows(const Kv8Pool& c, uint32_t layer, const Kv8Seqs& seqs, const Kv8Attend& a, const Kv8Scratch& w,
                        int sms, cudaStream_t s) {
     const long long rows = static_cast<long long>(seqs.max_rows) * a.group;
     const double all_rows = static_cast<double>(seqs.rows) * a.group;
-    const double products = all_rows * c.heads * kv8_pages(seqs, a, 256) / (128.0 * (kKv8PromptKeys / kKv8Block));
+    const double products = all_rows * c.heads * kv8_pages(seqs, a, 256) * kKv8Block / (128.0 * 128.0);
     if (all_rows >= static_cast<double>(kKv8PromptRows) * seqs.n && products >= kKv8PromptWork * static_cast<double>(sms))
         return a.bf16 ? kv8_launch_prompt<D, true>(c, layer, seqs, a, w, sms, s)
                       : kv8_launch_prompt<D, false>(c, layer, seqs, a, w, sms, s);

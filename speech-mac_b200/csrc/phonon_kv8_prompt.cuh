@@ -4,7 +4,7 @@
 // The mathematics is kv8_attention_kernel's: S = q K^T and O = P V with the
 // held integers as halves, exact; the blocks' scales join S by columns of 16
 // keys; the weights carry the blocks' value scales. A CTA has up to 256 rows
-// of a K/V head and one split of its positions, 128 positions a turn:
+// of a K/V head and one split of its positions, 64 positions a turn:
 //
 //   warps 8-14  load the turns' bytes, a page's keys or values at a time, and
 //               write them as halves into shared memory in matrix operand
@@ -29,8 +29,19 @@
 // them one after another would not, and the maximum can move at any turn
 // without a pass over TMEM.
 //
-// fp32 rows: q and the weights as two halves each (22 bits), two products
-// each. bf16 rows: one half each (q's 8 bits are exact, weights keep 11).
+// fp32 rows: q (times the softmax scale) and the weights as two halves each (22
+// bits), two products each. bf16 rows: one half each (q's 8 bits are exact,
+// weights keep 11).
+//
+// 1024 rows a K/V head over 4096 positions, 32 heads: bf16, 128 dims 144 us
+// (475 TFLOP/s), fp32, 64 dims 136 us (253, twice that in products); the
+// mma.sync kernel 353 and 265. Bound by the softmax's instructions: of 3000
+// clocks a turn of 64 dims, 400 go to the maximum, 1300 to the weights (two
+// warps share a scheduler's exponentials, 16 clocks an element of both), 250 to
+// O, 250 to the wait for P V, 300 to barriers and loads; a start of 7500 clocks
+// (4000 of them loads one after another: lengths, page ids, q and pages) and an
+// end of 3000. Scores of 128 positions in one buffer a stream: 156 us in fp32,
+// 134 in bf16. Warps that share a row's positions: 5300 clocks for 128.
 #pragma once
 
 #include "phonon_gemm.cuh"
@@ -38,7 +49,7 @@
 
 namespace phonon {
 
-constexpr int kKv8PromptKeys = 128, kKv8PromptThreads = 512;
+constexpr int kKv8PromptKeys = 64, kKv8PromptStages = 4, kKv8PromptThreads = 512;
 constexpr int kKv8Converters = 7;  // warps
 constexpr int kStatusDevice = 8;  // PHONON_CUDA_DEVICE_ERROR
 
@@ -131,6 +142,12 @@ __device__ __forceinline__ void kv8_put8(uint32_t at, uint32_t a, uint32_t b) {
     asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(at), "r"(a), "r"(b) : "memory");
 }
 
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+
 // Row tiles of 128 that a CTA has. Two share the turns' keys and values; q of
 // fp32 rows of 128 dims takes two halves' room, where one tile fits.
 template <int D, bool kBf16>
@@ -141,21 +158,21 @@ __host__ __device__ constexpr int kv8_prompt_rows() { return 128 * kv8_prompt_ti
 
 template <int D, bool kBf16>
 __host__ __device__ constexpr int kv8_prompt_smem() {
-    return (kBf16 ? 1 : 2) * kv8_prompt_rows<D, kBf16>() * D * 2 + 4 * kKv8PromptKeys * D * 2;
+    return (kBf16 ? 1 : 2) * kv8_prompt_rows<D, kBf16>() * D * 2 + 2 * kKv8PromptStages * kKv8PromptKeys * D * 2;
 }
 
 template <int D, bool kBf16>
 __global__ void __launch_bounds__(kKv8PromptThreads, 1) kv8_prompt_kernel(Kv8AttnParams p) {
     constexpr int kTiles = kv8_prompt_tiles<D, kBf16>();
-    constexpr int kKeys = kKv8PromptKeys, kPages = kKeys / kKv8Block;
+    constexpr int kKeys = kKv8PromptKeys, kPages = kKeys / kKv8Block, kStages = kKv8PromptStages;
     constexpr int kPlanes = kBf16 ? 1 : 2, kQBytes = 128 * D * 2, kTileBytes = kKeys * D * 2;
     constexpr uint32_t kRow8 = D * 16;      // bytes of 8 rows of q, of 8 keys
     constexpr uint32_t kDim8 = kKeys * 16;  // bytes of 8 dims of the values
     constexpr int kPieces = D / 32;         // 16-byte pieces a lane of a page's keys, of its values
     constexpr int kPitch = D + 4;           // floats of a row's result: 8 rows' quads in different banks
     static_assert(2 * 128 * kPitch * 4 <= kv8_prompt_smem<D, kBf16>(), "the rows' results outgrow the operands' room");
-    extern __shared__ __align__(128) uint8_t s_mem[];  // q [tile][plane], 2 x keys, 2 x values; then the rows' results
-    __shared__ __align__(8) uint64_t s_bars[15];
+    extern __shared__ __align__(128) uint8_t s_mem[];  // q [tile][plane], kStages x keys, x values; then the rows' results
+    __shared__ __align__(8) uint64_t s_bars[4 * kKv8PromptStages + 9];
     __shared__ uint32_t s_tmem;
     __shared__ int s_failed, s_last;
     __shared__ float s_f[128 * kTiles];
@@ -188,19 +205,21 @@ __global__ void __launch_bounds__(kKv8PromptThreads, 1) kv8_prompt_kernel(Kv8Att
     auto stream_turns = [&](int stream) { return two ? turns : (turns + 1 - stream) >> 1; };
     auto turn_of = [&](int stream, int n) { return two ? n : 2 * n + stream; };
 
-    const uint32_t s_q = smem_addr(s_mem), s_k = s_q + kTiles * kPlanes * kQBytes, s_v = s_k + 2 * kTileBytes;
+    const uint32_t s_q = smem_addr(s_mem), s_k = s_q + kTiles * kPlanes * kQBytes, s_v = s_k + kStages * kTileBytes;
     const uint32_t bars = smem_addr(s_bars);
-    // by buffer of keys and values (turn & 1), and by stream
-    const uint32_t k_full = bars, v_full = bars + 16, k_empty = bars + 32, v_empty = bars + 48;
-    const uint32_t s_full = bars + 64, p_full = bars + 80, o_full = bars + 96, q_full = bars + 112;
+    // by stage of keys and values (turn % kStages), score tile (stream, turn of the stream % 2), and stream
+    const uint32_t k_full = bars, v_full = k_full + 8 * kStages, k_empty = v_full + 8 * kStages, v_empty = k_empty + 8 * kStages;
+    const uint32_t s_full = v_empty + 8 * kStages, p_full = s_full + 32, o_full = p_full + 16, q_full = o_full + 16;
     if (threadIdx.x == 0) {
-        for (int k = 0; k < 2; ++k) {
+        for (int k = 0; k < kStages; ++k) {
             mbar_init(k_full + 8 * k, kPages);  // pages converted
             mbar_init(v_full + 8 * k, kPages);
             mbar_init(k_empty + 8 * k, two ? 2 : 1);  // tcgen05.commit of the streams that read them
             mbar_init(v_empty + 8 * k, two ? 2 : 1);
             mbar_init(s_full + 8 * k, 1);  // tcgen05.commit: S is there
-            mbar_init(p_full + 8 * k, 4);  // the stream's warps: the weights are there, the output has been read
+        }
+        for (int k = 0; k < 2; ++k) {
+            mbar_init(p_full + 8 * k, 4);  // the stream's warps: the weights are there, the output before has been read
             mbar_init(o_full + 8 * k, 1);  // tcgen05.commit: the output is there, the weights are free
         }
         mbar_init(q_full, 8);
@@ -211,6 +230,7 @@ __global__ void __launch_bounds__(kKv8PromptThreads, 1) kv8_prompt_kernel(Kv8Att
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_addr(&s_tmem)) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
+    const int scale_e = min(max(static_cast<int>(__float_as_uint(p.scale) >> 23) - 127, -126), 126);
     const auto wait = [&](uint32_t bar, int use) {  // the whole warp
         const bool ok = mbar_wait(bar, use & 1, nullptr, &s_failed);
         __syncwarp();
@@ -219,13 +239,14 @@ __global__ void __launch_bounds__(kKv8PromptThreads, 1) kv8_prompt_kernel(Kv8Att
                 asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-    const uint32_t tmem = s_tmem;  // S of the streams, then their outputs
-    const uint32_t tmem_o = tmem + 2 * kKeys;
+    const uint32_t tmem = s_tmem;  // S [stream][2], then the streams' outputs
+    const uint32_t tmem_o = tmem + 4 * kKeys;
     if (warp < 8) {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
         // q: four lanes a row
         const int passes = two ? 4 : 2;
         float4 ahead[2][kPieces][2];
+        const float unit_scale = p.scale * pow2i(-scale_e), unit_scale_low = p.scale_low * pow2i(-scale_e);
         auto load_q = [&](int pass, float4 (&v)[kPieces][2]) {
             const int rho = rho0 + min((warp * passes + pass) * 8 + (lane & 7), n_rows - 1), at = token(rho);
             const size_t row = static_cast<size_t>(sq.row0 + at) * p.q_stride +
@@ -255,7 +276,8 @@ __global__ void __launch_bounds__(kKv8PromptThreads, 1) kv8_prompt_kernel(Kv8Att
             const bool row_bad = bits >= 0x7f800000u;
             if (row_bad && lane < 8 && r < n_rows) kv8_flag(p.seqs, i, kStatusNonFinite);
             const int e = min(max(static_cast<int>(bits >> 23) - 127, -104), 126);
-            const float up = pow2i(12 - e);
+            // fp32 rows: times the softmax scale (its exponent apart, so that halves hold the products)
+            const float up = pow2i(12 - e) * (kBf16 ? 1.0f : unit_scale), up_low = pow2i(12 - e) * unit_scale_low;
             if (lane < 8) s_f[r] = row_bad ? __int_as_float(0x7fc00000) : pow2i(e - 12);  // a bad row's output is NaN
             const uint32_t to = s_q + (r >> 7) * (kPlanes * kQBytes) + (r >> 3 & 15) * kRow8 + (lane >> 3) * 128 + (r & 7) * 16;
 #pragma unroll
@@ -263,13 +285,15 @@ __global__ void __launch_bounds__(kKv8PromptThreads, 1) kv8_prompt_kernel(Kv8Att
                 uint32_t high[4], low[4];
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    const float2 x[2] = {mul2(make_float2(v[k][h].x, v[k][h].y), make_float2(up, up)),
-                                         mul2(make_float2(v[k][h].z, v[k][h].w), make_float2(up, up))};
+                    const float2 x[2] = {make_float2(v[k][h].x, v[k][h].y), make_float2(v[k][h].z, v[k][h].w)};
 #pragma unroll
                     for (int c = 0; c < 2; ++c) {
-                        high[2 * h + c] = half2_bits(x[c].x, x[c].y);
-                        const float2 rest = add2(x[c], half2_floats(high[2 * h + c] ^ 0x80008000u));
-                        low[2 * h + c] = half2_bits(rest.x, rest.y);
+                        const float2 y = mul2(x[c], make_float2(up, up));
+                        high[2 * h + c] = half2_bits(y.x, y.y);
+                        // what the half leaves of the exact product
+                        const float2 rest = fma2(x[c], make_float2(up, up), half2_floats(high[2 * h + c] ^ 0x80008000u));
+                        const float2 all = fma2(x[c], make_float2(up_low, up_low), rest);
+                        low[2 * h + c] = half2_bits(all.x, all.y);
                     }
                 }
                 kv8_put16(to + k * 512, high[0], high[1], high[2], high[3]);
@@ -288,7 +312,7 @@ __global__ void __launch_bounds__(kKv8PromptThreads, 1) kv8_prompt_kernel(Kv8Att
         // pages that every row of the CTA sees whole: [whole_first, whole_last)
         const int whole_last = max(pos_lo + 1, 0) / kKv8Block;
         const int whole_first = p.window && pos_hi >= p.window ? (pos_hi - p.window) / kKv8Block + 1 : 0;
-        // id and scales of this stream's pages of 4 turns, and of the 4 after them, a lane each
+        // scales of this stream's pages of 8 turns, and of the 8 after them, a lane each
         const uint8_t* exps = p.cache.exps + head * 2;
         auto scales_of = [&](int at, bool in) {  // -1: no page
             const int id = in ? __ldg(sq.pages + at) : -1;
@@ -297,18 +321,18 @@ __global__ void __launch_bounds__(kKv8PromptThreads, 1) kv8_prompt_kernel(Kv8Att
                        : -1;
         };
         auto fetch = [&](int n) {
-            const int at = first + turn_of(stream, n + lane / 8) * kPages + lane % 8;
+            const int at = first + turn_of(stream, n + lane / kPages) * kPages + lane % kPages;
             return scales_of(at, at < last);
         };
-        int scales = fetch(0), scales_next = fetch(4);
+        int scales = fetch(0), scales_next = fetch(8);
         // the value scale that eV is relative to: the split's first page's
         const int first_scales = scales_of(first, turns > 0), ref = first_scales < 0 ? 127 : first_scales >> 8;
         wait(q_full, 0);  // every row's factor
-        const float f_high = s_f[mine] * p.scale, f_low = s_f[mine] * p.scale_low;  // scales are not negative: the largest sum is the largest score
+        const float f = s_f[mine] * (kBf16 ? p.scale : pow2i(scale_e));  // of a product of q, as a score
         const int pos = at0 + token(rho0 + mine), low = p.window ? pos - p.window : -1;
-        const uint32_t at_s = tmem + stream * kKeys + (static_cast<uint32_t>(quarter * 32) << 16);
+        const uint32_t s_tiles = tmem + stream * 2 * kKeys + (static_cast<uint32_t>(quarter * 32) << 16);
         const uint32_t at_o = tmem_o + stream * 128 + (static_cast<uint32_t>(quarter * 32) << 16);
-        const uint32_t bar_s = s_full + 8 * stream, bar_p = p_full + 8 * stream, bar_o = o_full + 8 * stream;
+        const uint32_t bar_s = s_full + 16 * stream, bar_p = p_full + 8 * stream, bar_o = o_full + 8 * stream;
         float m = -INFINITY, l = 0.0f;
         float o[D];
 #pragma unroll
@@ -333,18 +357,18 @@ __global__ void __launch_bounds__(kKv8PromptThreads, 1) kv8_prompt_kernel(Kv8Att
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
         };
         for (int n = 0; n < n_turns; ++n) {
-            if (n) add_output(n - 1);
-            if (n && n % 4 == 0) {
+            if (n && n % 8 == 0) {
                 scales = scales_next;
-                scales_next = fetch(n + 4);
+                scales_next = fetch(n + 8);
             }
-            const int page0 = first + turn_of(stream, n) * kPages;
+            const int page0 = first + turn_of(stream, n) * kPages, lane0 = n % 8 * kPages;
+            const uint32_t at_s = s_tiles + (n & 1) * kKeys;
             // pages of this turn that some row does not see whole, and those that none does: bits
-            unsigned part = __ballot_sync(kFull, scales < 0) >> (n % 4 * 8) & 0xffu;
-            const unsigned gone = part;
+            const unsigned gone = __ballot_sync(kFull, scales < 0) >> lane0 & 0xfu;
+            unsigned part = gone;
 #pragma unroll
             for (int b = 0; b < kPages; ++b) part |= (page0 + b < whole_first || page0 + b >= whole_last ? 1u : 0u) << b;
-            wait(bar_s, n);
+            wait(bar_s + 8 * (n & 1), n >> 1);
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             // positions of chunk c (two pages) that this row sees: bits
             auto seen = [&](int c) {
@@ -356,7 +380,6 @@ __global__ void __launch_bounds__(kKv8PromptThreads, 1) kv8_prompt_kernel(Kv8Att
                 return bits;
             };
             float top = m;
-            float x[32], y[32];  // a chunk, and the next on its way
             const auto largest = [&](float (&x)[32], int c) {
                 if (part >> (2 * c) & 3) {
                     const uint32_t bits = seen(c);
@@ -365,42 +388,28 @@ __global__ void __launch_bounds__(kKv8PromptThreads, 1) kv8_prompt_kernel(Kv8Att
                 }
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    const int ex = __shfl_sync(kFull, scales, n % 4 * 8 + c * 2 + h);
+                    const int ex = __shfl_sync(kFull, scales, lane0 + c * 2 + h);
                     float most = -INFINITY;
 #pragma unroll
-                    for (int k = 0; k < 16; ++k) most = fmaxf(most, x[h * 16 + k]);
+                    for (int k = h * 16; k < h * 16 + 16; k += 2) most = max3(most, x[k], x[k + 1]);
                     const float u = __int_as_float((ex & 0xff) << 23), add = static_cast<float>((ex >> 8) - ref);
-                    const float z = fmaf(most, u * f_high, kBf16 ? add : fmaf(most, u * f_low, add));
+                    const float z = fmaf(most, u * f, add);
                     top = fmaxf(top, most == -INFINITY ? -INFINITY : z);
                 }
             };
-            tmem_start(at_s, x);
-#pragma unroll 1
-            for (int c = 0; c < 4; c += 2) {
-                tmem_arrived(x);
-                tmem_start(at_s + c * 32 + 32, y);
-                largest(x, c);
-                tmem_arrived(y);
-                tmem_start(at_s + (c * 32 + 64) % 128, x);  // at last the first chunk again, for its weights
-                largest(y, c + 1);
-            }
-            shrink = m == top ? 1.0f : ex2(m - top);
-            m = top;
-            l *= shrink;
-            top = top == -INFINITY ? 0.0f : top - kKv8WeightBits;  // nothing seen yet: weights 0
             const auto weigh = [&](float (&x)[32], int c) {
                 float less[2];  // 2^-eV
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    const int ex = __shfl_sync(kFull, scales, n % 4 * 8 + c * 2 + h);
+                    const int ex = __shfl_sync(kFull, scales, lane0 + c * 2 + h);
                     const float u = __int_as_float((ex & 0xff) << 23);
                     const int ev = (ex >> 8) - ref;
                     less[h] = ex < 0 ? 0.0f : pow2i(-ev);
-                    const float2 high = make_float2(u * f_high, u * f_high), rest = make_float2(u * f_low, u * f_low);
+                    const float2 by = make_float2(u * f, u * f);
                     const float2 from = make_float2(static_cast<float>(ev) - top, static_cast<float>(ev) - top);
 #pragma unroll
                     for (int k = h * 16; k < h * 16 + 16; k += 2) {
-                        const float2 s = make_float2(x[k], x[k + 1]), z = fma2(s, high, kBf16 ? from : fma2(s, rest, from));
+                        const float2 s = make_float2(x[k], x[k + 1]), z = fma2(s, by, from);
                         x[k] = z.x;
                         x[k + 1] = z.y;
                     }
@@ -419,10 +428,12 @@ __global__ void __launch_bounds__(kKv8PromptThreads, 1) kv8_prompt_kernel(Kv8Att
                         const int at = h * 16 + (k & 1) * 8 + (k >> 1) * 2;  // the cache's order of positions
                         float2 w = make_float2(ex2(x[at]), ex2(x[at + 1]));
                         sum = add2(sum, w);
-                        w_high[k] = half2_bits(w.x, w.y);
-                        if constexpr (!kBf16) {
-                            const float2 held = half2_floats(w_high[k] ^ 0x80008000u);
-                            w = add2(w, held);
+                        if constexpr (kBf16) {
+                            w_high[k] = half2_bits(w.x, w.y);
+                        } else {  // the first 11 bits as they are, and the rest
+                            const float2 head = make_float2(__uint_as_float(__float_as_uint(w.x) & 0xffffe000u), __uint_as_float(__float_as_uint(w.y) & 0xffffe000u));
+                            w_high[k] = half2_bits(head.x, head.y);
+                            w = fma2(head, make_float2(-1.0f, -1.0f), w);
                             w_low[k] = half2_bits(w.x, w.y);
                         }
                     }
@@ -431,19 +442,47 @@ __global__ void __launch_bounds__(kKv8PromptThreads, 1) kv8_prompt_kernel(Kv8Att
                     if constexpr (!kBf16) tmem_store8(at_s + c * 32 + 16 + h * 8, w_low);
                 }
             };
-#pragma unroll 1
-            for (int c = 0; c < 4; c += 2) {
+            // A chunk (32 positions) in registers; both of them, from the maximum to the
+            // weights, where O leaves the room.
+            constexpr bool kHold = D < 128;
+            float x[32], y[kHold ? 32 : 1];
+            if constexpr (kHold) {
+                tmem_start(at_s, x);
+                tmem_start(at_s + 32, y);
                 tmem_arrived(x);
-                tmem_start(at_s + c * 32 + 32, y);
-                weigh(x, c);
                 tmem_arrived(y);
-                if (c == 0) tmem_start(at_s + 64, x);
-                weigh(y, c + 1);
+                largest(x, 0);
+                largest(y, 1);
+            } else {
+#pragma unroll 1
+                for (int c = 0; c < 2; ++c) {
+                    tmem_start(at_s + c * 32, x);
+                    tmem_arrived(x);
+                    largest(x, c);
+                }
+            }
+            if (!kHold && n) add_output(n - 1);
+            const float c = m == top ? 1.0f : ex2(m - top);
+            m = top;
+            l *= c;
+            top = top == -INFINITY ? 0.0f : top - kKv8WeightBits;  // nothing seen yet: weights 0
+            if constexpr (kHold) {
+                weigh(x, 0);
+                if (n) add_output(n - 1);
+                weigh(y, 1);
+            } else {
+#pragma unroll 1
+                for (int c = 0; c < 2; ++c) {
+                    tmem_start(at_s + c * 32, x);
+                    tmem_arrived(x);
+                    weigh(x, c);
+                }
             }
             asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
             __syncwarp();
             if (lane == 0) mbar_arrive(bar_p);
+            shrink = c;
         }
         if (n_turns) add_output(n_turns - 1);
         __syncwarp();
@@ -490,13 +529,13 @@ __global__ void __launch_bounds__(kKv8PromptThreads, 1) kv8_prompt_kernel(Kv8Att
     } else {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
         if (warp < 15) {
-            // Pages of keys (unit 16 * turn + page) and of values (unit 16 * turn + 8 + page), every seventh unit.
+            // Pages of keys (unit 8 * turn + page) and of values (unit 8 * turn + 4 + page), every seventh unit.
                         const int units = turns * 2 * kPages, converter = warp - 8;
                         const int count = units > converter ? (units - converter + kKv8Converters - 1) / kKv8Converters : 0;
                         const size_t page_bytes = static_cast<size_t>(p.cache.heads) * 2 * kKv8Block * D;
                         const uint8_t* pool = p.cache.pool + static_cast<size_t>(head) * 2 * kKv8Block * D;
                         auto fetch_ids = [&](int n) {  // page ids of this warp's units n + lane
-                            const int unit = converter + (n + lane) * kKv8Converters, at = first + unit / 16 * kPages + unit % 8;
+                            const int unit = converter + (n + lane) * kKv8Converters, at = first + unit / (2 * kPages) * kPages + unit % kPages;
                             int id = at < last ? __ldg(sq.pages + at) : -1;
                             if (at < last && static_cast<unsigned>(id) >= static_cast<unsigned>(p.cache.pool_pages)) {
                                 kv8_flag(p.seqs, i, kStatusInvalid);
@@ -510,7 +549,7 @@ __global__ void __launch_bounds__(kKv8PromptThreads, 1) kv8_prompt_kernel(Kv8Att
                         auto load = [&](uint4 (&w)[kPieces], int n, int id) {
                             const int unit = converter + n * kKv8Converters;
                             const uint8_t* src = pool + max(id, 0) * page_bytes;
-                            const bool values = unit & 8;
+                            const bool values = unit & kPages;
             #pragma unroll
                             for (int k = 0; k < kPieces; ++k) {
                                 const int row = D == 32 ? key_row : (k & 1) * 8 + key_row, piece = D == 32 ? key_piece : (k >> 1) * 4 + key_piece;
@@ -524,9 +563,9 @@ __global__ void __launch_bounds__(kKv8PromptThreads, 1) kv8_prompt_kernel(Kv8Att
             load(b, 1, __shfl_sync(kFull, ids, 1));
             int ids_next = fetch_ids(32);
             auto convert = [&](const uint4 (&w)[kPieces], int n) {
-                const int unit = converter + n * kKv8Converters, turn = unit / 16, stage = turn & 1, page = unit % 8;
-                const bool values = unit & 8;
-                if (turn >= 2) wait((values ? v_empty : k_empty) + 8 * stage, (turn >> 1) - 1);
+                const int unit = converter + n * kKv8Converters, turn = unit / (2 * kPages), stage = turn % kStages, page = unit % kPages;
+                const bool values = unit & kPages;
+                if (turn >= kStages) wait((values ? v_empty : k_empty) + 8 * stage, turn / kStages - 1);
                 if (values) {
                     const uint32_t to = s_v + stage * kTileBytes + (page * 2 + (vt >> 1)) * 128 + vg * 16 + (vt & 1) * 8;
 #pragma unroll
@@ -572,47 +611,58 @@ __global__ void __launch_bounds__(kKv8PromptThreads, 1) kv8_prompt_kernel(Kv8Att
             const auto commit = [&](uint32_t bar) {
                 if (leader) umma_commit(bar);
             };
-            // a stream's next step, if what it waits for is there: 1 if so
-            const auto step = [&](int stream, int& scored, int& summed) {
-                const int n = summed, turn = apart ? n : 2 * n + stream, stage = turn & 1;
-                if (scored == n) {  // S goes where the weights of the turn before lie
-                    if (!(n == 0 || done(o_full + 8 * stream, n - 1)) || !done(k_full + 8 * stage, turn >> 1)) return false;
-                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                    const uint64_t q = q_desc + (apart ? stream : 0) * (kPlanes * kQBytes / 16), k8 = k_desc + stage * (kTileBytes / 16);
-#pragma unroll
-                    for (int plane = kPlanes - 1; plane >= 0; --plane)
-#pragma unroll
-                        for (int k = 0; k < D / 16; ++k)
-                            umma_half<false>(leader, base + stream * kKeys, q + plane * (kQBytes / 16) + k * 16, k8 + k * 16, idesc_s,
-                                             plane != kPlanes - 1 || k != 0);
-                    commit(s_full + 8 * stream);
-                    commit(k_empty + 8 * stage);
-                    ++scored;
-                } else {
-                    if (!done(p_full + 8 * stream, n) || !done(v_full + 8 * stage, turn >> 1)) return false;
-                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                    const uint64_t v = v_desc + stage * (kTileBytes / 16);
-#pragma unroll
-                    for (int plane = kPlanes - 1; plane >= 0; --plane)
-#pragma unroll
-                        for (int k = 0; k < kPages; ++k)
-                            umma_half<true>(leader, base + 2 * kKeys + stream * 128,
-                                            base + stream * kKeys + (k >> 1) * 32 + plane * 16 + (k & 1) * 8, v + k * 16, idesc_o,
-                                            plane != kPlanes - 1 || k != 0);
-                    commit(o_full + 8 * stream);
-                    commit(v_empty + 8 * stage);
-                    ++summed;
-                }
-                return true;
+            // A stream's next steps, if what they wait for is there: turns whose S and P V
+            // have been issued, and whose P V is known to be done.
+            struct Stream {
+                int scored, summed, done;
             };
-            bool ok = __all_sync(kFull, wait(q_full, 0));
-            int scored0 = 0, scored1 = 0, summed0 = 0, summed1 = 0;  // turns of a stream whose S, P V have been issued
-            long long since = clock64();
-            while (ok && (summed0 < turns0 || summed1 < turns1)) {
+            const auto step = [&](int stream, int n_turns, Stream& at) {
                 bool moved = false;
-                if (summed0 < turns0) moved |= step(0, scored0, summed0);
-                // the second stream half a turn behind: one's softmax beside the other's products
-                if (summed1 < turns1 && (summed0 > 0 || turns0 <= 2)) moved |= step(1, scored1, summed1);
+                if (at.done < at.summed && done(o_full + 8 * stream, at.done)) ++at.done;
+                if (at.scored < n_turns && at.scored < at.done + 2) {  // S goes where the weights of two turns before lie
+                    const int n = at.scored, turn = apart ? n : 2 * n + stream, stage = turn % kStages;
+                    if (done(k_full + 8 * stage, turn / kStages)) {
+                        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                        const uint64_t q = q_desc + (apart ? stream : 0) * (kPlanes * kQBytes / 16), k8 = k_desc + stage * (kTileBytes / 16);
+#pragma unroll
+                        for (int plane = kPlanes - 1; plane >= 0; --plane)
+#pragma unroll
+                            for (int k = 0; k < D / 16; ++k)
+                                umma_half<false>(leader, base + (stream * 2 + (n & 1)) * kKeys, q + plane * (kQBytes / 16) + k * 16, k8 + k * 16,
+                                                 idesc_s, plane != kPlanes - 1 || k != 0);
+                        commit(s_full + 16 * stream + 8 * (n & 1));
+                        commit(k_empty + 8 * stage);
+                        ++at.scored;
+                        moved = true;
+                    }
+                }
+                if (at.summed < at.scored) {
+                    const int n = at.summed, turn = apart ? n : 2 * n + stream, stage = turn % kStages;
+                    if (done(p_full + 8 * stream, n) && done(v_full + 8 * stage, turn / kStages)) {
+                        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                        const uint64_t v = v_desc + stage * (kTileBytes / 16);
+                        at.done = n;  // the stream has read the output before
+#pragma unroll
+                        for (int plane = kPlanes - 1; plane >= 0; --plane)
+#pragma unroll
+                            for (int k = 0; k < kPages; ++k)
+                                umma_half<true>(leader, base + 4 * kKeys + stream * 128,
+                                                base + (stream * 2 + (n & 1)) * kKeys + (k >> 1) * 32 + plane * 16 + (k & 1) * 8, v + k * 16, idesc_o,
+                                                plane != kPlanes - 1 || k != 0);
+                        commit(o_full + 8 * stream);
+                        commit(v_empty + 8 * stage);
+                        ++at.summed;
+                        moved = true;
+                    }
+                }
+                return moved;
+            };
+            Stream s0{0, 0, 0}, s1{0, 0, 0};
+            bool ok = __all_sync(kFull, wait(q_full, 0));
+            long long since = clock64();
+            while (ok && (s0.summed < turns0 || s1.summed < turns1)) {
+                bool moved = step(0, turns0, s0);
+                moved |= step(1, turns1, s1);
                 if (moved) {
                     since = clock64();
                 } else if (__any_sync(kFull, *static_cast<volatile int*>(&s_failed) || clock64() - since > kWaitBudgetCycles)) {
