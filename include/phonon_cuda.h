@@ -468,7 +468,9 @@ int phonon_cuda_mimi_process(PhononCudaMimi *mimi, uint32_t state, const float *
  *   - page id lies outside the pool (INVALID_ARGUMENT): that page is not
  *     written, reads as zeros, and no query sees it;
  *   - rows hold a non-finite value (NON_FINITE): append holds such an element
- *     as 0, and a query row with one gets NaN.
+ *     as 0, and a query row with one gets NaN;
+ *   - attention gave up a bounded wait inside its kernel (DEVICE_ERROR, about
+ *     two seconds): rows of it are NaN.
  * The largest code stays. A page that a call appends to belongs to one
  * sequence of the batch; pages that are only read may be shared. Calls on one
  * cache may run at the same time as long as none writes a page that another

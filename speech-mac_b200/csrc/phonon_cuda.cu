@@ -672,10 +672,15 @@ int kv8_launch_prompt(const Kv8Pool& c, uint32_t layer, const Kv8Seqs& seqs, con
     if (rc != PHONON_CUDA_OK) return rc;
     constexpr int smem = kv8_prompt_smem<D, kBf16>();
     auto kernel = kv8_prompt_kernel<D, kBf16>;
-    if constexpr (smem > 40 * 1024) {  // 48 KB with the kernel's static arrays
-        static std::atomic<uint64_t> configured{0};
-        CUDA_TRY(opt_in_smem(reinterpret_cast<const void*>(kernel), smem, configured));
-    }
+    // Its warps hand registers to one another: what they ask for has to be what
+    // the launch has, or they would wait for good.
+    static const int registers = [kernel] {
+        cudaFuncAttributes f{};
+        return cudaFuncGetAttributes(&f, kernel) == cudaSuccess ? (f.numRegs + 7) / 8 * 8 : 0;
+    }();
+    if (registers * kKv8PromptThreads < kKv8PromptRegisters) return PHONON_CUDA_DEVICE_ERROR;
+    static std::atomic<uint64_t> configured{0};
+    CUDA_TRY(opt_in_smem(reinterpret_cast<const void*>(kernel), smem, configured));
     CUDA_TRY(launch_pdl(kernel, dim3(static_cast<unsigned>(items * p.splits)), dim3(kKv8PromptThreads), smem, s, p));
     return PHONON_CUDA_OK;
 }
@@ -696,7 +701,7 @@ template <int D>
 int kv8_attention_rows(const Kv8Pool& c, uint32_t layer, const Kv8Seqs& seqs, const Kv8Attend& a, const Kv8Scratch& w,
                        int sms, cudaStream_t s) {
     const long long rows = static_cast<long long>(seqs.max_rows) * a.group;
-    const double all_rows = static_cast<double>(seqs.rows) * a.group;
+    const double all_rows = std::min(static_cast<double>(seqs.rows), static_cast<double>(seqs.n) * seqs.max_rows) * a.group;
     const double products = all_rows * c.heads * kv8_pages(seqs, a, 256) * kKv8Block / (128.0 * 128.0);
     if (all_rows >= static_cast<double>(kKv8PromptRows) * seqs.n && products >= kKv8PromptWork * static_cast<double>(sms))
         return a.bf16 ? kv8_launch_prompt<D, true>(c, layer, seqs, a, w, sms, s)

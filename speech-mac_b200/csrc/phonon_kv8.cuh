@@ -193,6 +193,11 @@ constexpr float kKv8Tame = 1e20f;
 // warp; a partly filled block is read again only where its scale rises or a
 // value word mixes old and new positions. Lane layout: keys, 4 dims of a row
 // a lane (4-byte stores, rows coalesced); values, the lane's own chunks.
+//
+// Bound by latency (length, page id, rows, then stores) until a call has tens
+// of megabytes: 4000 bf16 rows of 8 x 128 from the middle of a block on, 16
+// sequences, 25 MB: 7.9 us. A warp a block and not a CTA: nothing to wait for
+// but the warp's own loads, which are all in flight at once.
 template <int D, bool kBf16>
 __global__ void __launch_bounds__(128) kv8_append_kernel(Kv8AppendParams p) {
     constexpr int kLanesPerRow = D / 4, kRowsPerPass = 32 / kLanesPerRow, kPasses = kKv8Block / kRowsPerPass;
@@ -299,7 +304,8 @@ __global__ void __launch_bounds__(128) kv8_append_kernel(Kv8AppendParams p) {
 
 // One new row a sequence (a decode step): D / 4 lanes per (sequence, head, keys
 // or values), 4 dims a lane; nothing of the block is read unless the scale
-// rises.
+// rises. 512 rows of 8 x 64 in fp32, 2 MB: 4.1 us, launch and three loads one
+// after another (a warp a block, as above, takes 12.5).
 template <int D, bool kBf16>
 __global__ void __launch_bounds__(128) kv8_append_one_kernel(Kv8AppendParams p) {
     constexpr int kLanes = D / 4;
@@ -407,6 +413,10 @@ __global__ void kv8_fill_kernel(uint8_t* pool, uint8_t* exps, int pool_pages, co
 }
 
 // --------------------------------------------------------------------- read
+// (held integer) * 2^e. Bound by the bytes: 110 sequences of up to 2048
+// positions, 8 heads of 128, to bf16: 69 us, 6.0 TB/s, 93 % of the copy rate
+// (124 with the bytes of a block taken one at a time); one sequence of 8000, 8 x
+// 64, to fp32, 41 MB: 10.2 us, of which 4 are launch and latency.
 struct Kv8ReadParams {
     Kv8View cache;
     Kv8Seqs seqs;
@@ -510,15 +520,17 @@ __global__ void __launch_bounds__(128) kv8_read_kernel(Kv8ReadParams p) {
 // column tile has the third. A score's sums are exact; so are those of the
 // output per turn, with the weights as integers of 32 bits, a byte a column.
 // (The cache's bytes are unsigned, 128 too large: products with a constant -128
-// in their place start the sums.) What is left are q's and the weights' own roundings (2^-24 of a row's
-// largest; 2^-33 of the largest weight, or its fp32's) and the turns' fp32 sums.
+// in their place start the sums.) What is left are q's and the weights' own
+// roundings (2^-24 of a row's largest; 2^-33 of the largest weight, or its
+// fp32's) and the turns' fp32 sums.
 //
 // More rows: products of halves, the conversion of a block's bytes shared by
 // the rows. Byte | 0x6400 is the half 1152 + integer, minus 1152 the integer,
-// exactly, one PRMT and one HSUB2 for two. The products are exact in the fp32 accumulators. fp32 rows:
-// q (scaled by a power of two to a row maximum near 2^12) and the weights
-// enter as two halves each, 22 bits. bf16 rows: q fits one half (8 bits), a
-// weight is rounded to one half (11 bits, under the output's 8).
+// exactly, one byte permutation and one subtraction for two. The products are
+// exact in the fp32 accumulators. fp32 rows: q (scaled by a power of two to a
+// row maximum near 2^12) and the weights enter as two halves each, 22 bits.
+// bf16 rows: q fits one half (8 bits), a weight is rounded to one half (11 bits,
+// under the output's 8).
 struct Kv8AttnParams {
     Kv8View cache;
     Kv8Seqs seqs;
@@ -791,8 +803,20 @@ __device__ __forceinline__ int kv8_key_dim(int t, int c) {
 // and meet in shared memory; the last split to arrive merges them in order.
 // Pages come by asynchronous copies, kStages - 1 turns ahead, in a ring that a
 // warp has to itself: the copies, not registers, hold what is in flight, which
-// leaves room for 16 to 20 warps an SM. Page ids and scales are fetched a lane
-// each, 32 / PB turns at a time.
+// leaves room for 12 to 16 warps an SM (24 and more in single-warp CTAs). Page
+// ids and scales are fetched a lane each, 32 / PB turns at a time.
+//
+// Decode steps are bound by the cache's bytes: 512 sequences of up to 2048
+// positions, 8 x 64, 526 MB, 87 us (6.1 TB/s, 94 % of the copy rate); as halves
+// with register loads 137, with the ring 101, as bytes 95. 48 of up to 4096, 32
+// heads on 8 x 128, 225 MB, 47.5 us: a CTA's start and end (4 us) against 30 us of
+// pages, three CTAs an SM. 8 of 8000: 18 us, 5.7 of them the chain of loads
+// before the first page and 3 the merge. One of 800: 6.3 us, all latency. 64 x
+// 16 rows over 250 keys 13.8 us and 4 chunks of up to 256 rows 27 us: bound by
+// the halves' matrix rate (2.1 clocks an m16n8k16 on an SM, two of them in
+// fp32) and, in bf16 with 128 dims, by the conversion of the bytes.
+// A persistent form that cut the positions of all items into equal lines for
+// the resident CTAs: 99 us and 26 (8 of 8000), since each cut costs a merge.
 template <int D, int NT, int PB, int kStages, int kMode, int kWarps, int kCtas>
 __global__ void __launch_bounds__(32 * kWarps, kCtas) kv8_attention_kernel(Kv8AttnParams p) {
     constexpr bool kBf16 = kMode == KV8_HALF_BF16 || kMode == KV8_INT_BF16, kFine = kMode == KV8_HALF_F32;

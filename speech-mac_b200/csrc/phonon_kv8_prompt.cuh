@@ -51,6 +51,9 @@ namespace phonon {
 
 constexpr int kKv8PromptKeys = 64, kKv8PromptStages = 4, kKv8PromptThreads = 512;
 constexpr int kKv8Converters = 7;  // warps
+// A thread's registers in warps 0-7 and 8-15, together the launch's 128 each.
+constexpr int kKv8SoftmaxRegisters = 200, kKv8OtherRegisters = 56;
+constexpr int kKv8PromptRegisters = 256 * (kKv8SoftmaxRegisters + kKv8OtherRegisters);
 constexpr int kStatusDevice = 8;  // PHONON_CUDA_DEVICE_ERROR
 
 // 32 consecutive accumulator columns of the warp's 32 lanes, on their way until tmem_arrived.
@@ -242,7 +245,7 @@ __global__ void __launch_bounds__(kKv8PromptThreads, 1) kv8_prompt_kernel(Kv8Att
     const uint32_t tmem = s_tmem;  // S [stream][2], then the streams' outputs
     const uint32_t tmem_o = tmem + 4 * kKeys;
     if (warp < 8) {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kKv8SoftmaxRegisters));
         // q: four lanes a row
         const int passes = two ? 4 : 2;
         float4 ahead[2][kPieces][2];
@@ -527,7 +530,7 @@ __global__ void __launch_bounds__(kKv8PromptThreads, 1) kv8_prompt_kernel(Kv8Att
             kv8_merge<D, kBf16, 256, 4>(p, 1.0f, both_sync, reinterpret_cast<float4*>(s_mem), &s_last, item, active, p.tile_rows, n_rows,
                                         sq.row0, rho0, head);
     } else {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kKv8OtherRegisters));
         if (warp < 15) {
             // Pages of keys (unit 8 * turn + page) and of values (unit 8 * turn + 4 + page), every seventh unit.
                         const int units = turns * 2 * kPages, converter = warp - 8;

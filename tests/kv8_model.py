@@ -76,13 +76,14 @@ def attention_bound(size, biggest, out, dim, length, bf16):
     biggest: the largest |value|. u = 2^-23 is twice fp32's half step, the
     worst of a truncating addition.
 
-    A score: q in two halves (22 bits: 2u) and at most dim/8 + 8 rounded
-    additions and products of partial sums, each below the score's own bound.
-    A weight: the error of its exponent, the exponential (within 2u; the
-    library's bound is 2 ulp) and the rounding to two halves (2u). The output: a weighted
-    mean, whose numerator and denominator each take a weight's error and one
-    rounded addition per block and per merged share. Rows in bf16 add a weight's rounding to
-    one half, 2^-12 (numerator only), and the output's, 2^-8."""
+    A score: q in 22 bits (2u: two halves; as bytes it has 23 or, in bf16,
+    15, which hold its 8) and at most dim/8 + 8 rounded additions and products
+    of partial sums, each below the score's own bound. A weight: the error of
+    its exponent, the exponential (within 2u) and the rounding to two halves
+    (2u; as bytes 32 bits of the largest). The output: a weighted mean, whose
+    numerator and denominator each take a weight's error and one rounded
+    addition per block and per merged share. Rows in bf16 add a weight's
+    rounding to one half, 2^-12 (numerator only), and the output's, 2^-8."""
     u = 2.0 ** -23
     score = size * (dim / 8 + 10) * u
     weight = score + 4 * u
