@@ -537,7 +537,7 @@ typedef struct {
     uint32_t type;   /* PhononCudaRowType of q and out */
     uint32_t heads;
     uint32_t window; /* 0: none */
-    float scale;     /* of the scores; 0: 1 / sqrt(head_dim) */
+    float scale;     /* of the scores, at most 1e30; 0: 1 / sqrt(head_dim) */
     const void *q;
     void *out;
     uint64_t q_stride, out_stride; /* elements from row to row (0: packed) */

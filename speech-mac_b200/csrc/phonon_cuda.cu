@@ -4647,7 +4647,7 @@ int phonon_cuda_kv8_attention_device(PhononCudaKv8* c, uint32_t layer, const Pho
         !kv8_seqs(batch, status_dev, &seqs) || !query || !query->q || !query->out ||
         query->type > PHONON_CUDA_ROWS_BF16 || !aligned16(query->q) || !aligned16(query->out) || query->heads == 0 ||
         query->heads % c->pool.heads || query->heads > (1u << 16) || query->window > (1u << 30) ||
-        !std::isfinite(query->scale) || query->scale < 0.0f)
+        !(query->scale >= 0.0f && query->scale <= 1e30f))
         return PHONON_CUDA_INVALID_ARGUMENT;
     Kv8Attend a{};
     const uint64_t width = static_cast<uint64_t>(query->heads) * c->pool.dim;

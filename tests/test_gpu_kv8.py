@@ -667,3 +667,17 @@ def test_many_rows_repeat_bit_for_bit_and_in_graphs(cuda_ok, dtype):
             graph.replay()
             torch.cuda.synchronize()
             assert torch.equal(outs[0], outs[1]) and torch.equal(outs[0], outs[2])
+
+
+def test_scales_past_the_bound_are_refused(cuda_ok):
+    c = Cache(1, 64, [4])
+    q = torch.zeros(1, 1, 64, device="cuda")
+    ws = rt.Kv8Workspace(c.kv)
+    for scale, fine in ((1e30, True), (2e30, False), (float("inf"), False)):
+        query = rt.kv8_query(q.data_ptr(), q.data_ptr(), heads=1, scale=scale)
+        if fine:
+            c.kv.attention(c.batch([4], [1]), query, ws)
+        else:
+            with pytest.raises(rt.CudaError):
+                c.kv.attention(c.batch([4], [1]), query, ws)
+    torch.cuda.synchronize()

@@ -214,3 +214,24 @@ def test_frame_loop(cuda_ok, weights12):
     np.testing.assert_array_equal(outs[0][0], outs[1][0])
     np.testing.assert_array_equal(outs[0][1], outs[1][1])
     assert np.isfinite(outs[1][2]).all()
+
+
+def test_prefill_of_a_long_context(cuda_ok, oracle, weights12):
+    """7400 positions, 256 rows a pass: the last passes are work enough for the 128-row attention in every layer."""
+    length = 7400
+    weights = weights12[:2]
+    ctx = context(weights, 1, 256 * (length // 16 + 1))  # a pass lists its rows' pages, as many as the pool has
+    s = ctx.stream_alloc(length)
+    rows = synth.Generator(7).normal(length * 512).reshape(length, 512)
+    last = ctx.append(s, rows)
+    k, v = ctx.kv_read(s, 0, length)
+    om = oracle.model(weights)
+    cache = om.new_stream(length)
+    om.load_kv(cache, k, v)
+    x = rows[-1]
+    for layer in range(2):
+        ok, x, _, _ = om.layer_step_forced(cache, layer, length - 1, x)
+        assert ok
+    om.free_stream(cache)
+    ctx.close()
+    assert rt.rel_err(last, x) < FINAL_TOL
