@@ -54,7 +54,7 @@ constexpr int kKv8Ctas = 5;          // 8-bit attention: resident CTAs per SM, a
 constexpr int kKv8MinPages = 8;      // ... pages per split, at least (two a warp)
 constexpr int kKv8LongPages = 64;    // ... of a call whose CTAs are not all resident
 constexpr int kKv8PromptRows = 64;   // the 128-row attention: rows of a K/V head of a sequence on average, at least
-constexpr int kKv8PromptWork = 6;    // ... 128-row, 128-position products per SM, at least
+constexpr int kKv8PromptWork = 3;    // ... 128-row, 128-position products per SM, at least
 constexpr int kKv8PromptMinPages = 64, kKv8PromptLongPages = 64;  // ... pages per split, at least
 constexpr int kKv8TileFloats = 2048; // ... outputs of a row tile, at most
 
@@ -660,8 +660,11 @@ int kv8_launch_prompt(const Kv8Pool& c, uint32_t layer, const Kv8Seqs& seqs, con
     Kv8AttnParams p{};
     long long items = 0, pages = 0;
     // Two row tiles in a CTA share the conversion of their keys and values (a
-    // turn of both takes 1.74 times one's), one leaves more CTAs (fp32, 64 dims,
-    // 256 x 1024, 32 heads: one a CTA 25.9 us, two 44; 1024 x 1024, 128: two 166, one 193).
+    // turn of both takes 1.74 times one's), one leaves more CTAs. us with one and
+    // with two, fp32, 64 dims: 256 x 1024, 32 heads 21.7 and 37.5, 128 heads 42.7
+    // and 39.6; 256 x 2048, 160 heads 101 and 127; 1024 x 4096, 32 heads 140 and
+    // 135. bf16, 128 dims: 256 x 1024, 128 heads 60.5 and 49.8; 1024 x 4096, 32 165
+    // and 147.
     int tile_rows = 128;
     if constexpr (kv8_prompt_rows<D, kBf16>() == 256) {
         const long long rows = static_cast<long long>(seqs.max_rows) * a.group, each = static_cast<long long>(seqs.n) * c.heads;
@@ -690,13 +693,13 @@ int kv8_launch_prompt(const Kv8Pool& c, uint32_t layer, const Kv8Seqs& seqs, con
 // products fill the GPU (kKv8PromptWork): 128 rows at a time on the tcgen05
 // tensor cores, whose CTA of 512 threads starts and ends in 6 us and works on
 // 128 rows however few there are. us of the 128-row kernel and the other; rows x
-// positions, K/V heads of all sequences (products an SM): fp32, 64 dims: 128 x
-// 1024, 32 heads (1.7) 25.7 and 19.3; 256 x 1024, 32 (3.5) 25.9 and 27.9; 1 to
-// 256 rows of 300 to 2048 positions, 32 (4.1 by the longest) 30.4 and 27.7; 128
-// x 1024, 128 (6.9) 22.6 and 45.3; 1024 x 4096, 32 (55) 136 and 265; 1 to 64
-// rows of 16 to 700 positions, 512 heads, 52 and 34. bf16, 128 dims: 128 x
-// 1024, 32 30.4 and 25.8; up to 1024 x 2048, 32 77 and 124; 1024 x 4096, 32 144
-// and 353.
+// positions, K/V heads of all sequences (products an SM). fp32, 64 dims: 128 x
+// 1024, 32 heads (1.7) 21.4 and 19.4; 128 x 4096, 8 (1.7) 27.1 and 19.9; 256 x
+// 1024, 32 (3.5) 21.6 and 27.8; 1 to 256 rows of 300 to 2048 positions, 32 (4.1
+// by the longest) 26.8 and 27.3; 128 x 1024, 128 (6.9) 22.7 and 45.3; 1024 x
+// 4096, 32 (55) 136 and 265; 1 to 64 rows of 16 to 700 positions, 512 heads, 52
+// and 34. bf16, 128 dims: 128 x 1024, 32 (1.7) 28.4 and 25.9; 256 x 1024, 32
+// (3.5) 28.7 and 39.7; 1024 x 4096, 32 144 and 353.
 template <int D>
 int kv8_attention_rows(const Kv8Pool& c, uint32_t layer, const Kv8Seqs& seqs, const Kv8Attend& a, const Kv8Scratch& w,
                        int sms, cudaStream_t s) {

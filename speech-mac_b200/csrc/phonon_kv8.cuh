@@ -812,7 +812,7 @@ __device__ __forceinline__ int kv8_key_dim(int t, int c) {
 // heads on 8 x 128, 225 MB, 47.5 us: a CTA's start and end (4 us) against 30 us of
 // pages, three CTAs an SM. 8 of 8000: 18 us, 5.7 of them the chain of loads
 // before the first page and 3 the merge. One of 800: 6.3 us, all latency. 64 x
-// 16 rows over 250 keys 13.8 us and 4 chunks of up to 256 rows 27 us: bound by
+// 16 rows over 250 keys 13.8 us, 4 chunks of up to 256 rows 27.3 us: bound by
 // the halves' matrix rate (2.1 clocks an m16n8k16 on an SM, two of them in
 // fp32) and, in bf16 with 128 dims, by the conversion of the bytes.
 // A persistent form that cut the positions of all items into equal lines for

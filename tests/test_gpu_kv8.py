@@ -547,7 +547,7 @@ def test_all_keys_alike_and_one_key_far_ahead(cuda_ok, group, count, dtype):
 
 # ------------------------------------------- many rows (the 128-row kernel)
 # Calls with work enough for it: all rows * query heads * pages of the longest
-# 909312 or more (148 SMs), 64 rows of a K/V head or more. Row tiles of one row, of 128 and of
+# 454656 or more (148 SMs), 64 rows of a K/V head or more. Row tiles of one row, of 128 and of
 # 129 to 256 (two streams); splits; every tile edge among the lengths.
 MANY = [
     # kv_heads, group, dim, lengths, rows, window
