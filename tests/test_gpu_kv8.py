@@ -681,3 +681,38 @@ def test_scales_past_the_bound_are_refused(cuda_ok):
             with pytest.raises(rt.CudaError):
                 c.kv.attention(c.batch([4], [1]), query, ws)
     torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_many_rows_padded_and_on_two_streams_at_once(cuda_ok, dtype):
+    """Row and length bounds far above the batch's own, a sequence without rows, rows behind the last one left as they
+    were; and calls of two streams at once, a workspace each, give the bits of a call alone."""
+    rng = np.random.default_rng(23)
+    kind = rt.ROWS_BF16 if dtype == torch.bfloat16 else rt.ROWS_F32
+    lengths, counts = [1500, 40, 900, 1500, 700, 1200] * 4, [200, 0, 129, 128, 256, 70] * 4
+    c = Cache(4, 64, lengths)
+    c.append(lengths, *[[rows(rng, n, 4, 64, dtype) for n in lengths] for _ in range(2)])
+    q = rows(rng, sum(counts) + 5, 8, 64, dtype)
+    ws = [rt.Kv8Workspace(c.kv) for _ in range(2)]
+    tight, loose = c.batch(lengths, counts), c.batch(lengths, counts, max_rows=1000)
+    outs = [torch.full_like(q, 3.0) for _ in range(6)]
+
+    def call(batch, out, w, stream=0):
+        c.kv.attention(batch, rt.kv8_query(q.data_ptr(), out.data_ptr(), kind, heads=8), ws[w], stream_ptr=stream)
+
+    call(tight, outs[0], 0)
+    call(loose, outs[1], 0)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for k in range(2):
+        for w in range(2):
+            call(tight, outs[2 + 2 * k + w], w, streams[w].cuda_stream)
+    torch.cuda.synchronize()
+    for out in outs:
+        assert torch.isfinite(out.float()).all() and (out[sum(counts):] == 3).all()
+    for out in outs[2:]:
+        assert torch.equal(outs[0], out)
+    # Other bounds may split the positions elsewhere: the same up to both calls' roundings. bf16: the outputs' own, 2^-8
+    # each. fp32: 24 turns of 64 positions, a sum of 16 truncated steps a turn, 2^-23 each: 2 * 40 * 2^-23.
+    close = 2.0 ** -7 if dtype == torch.bfloat16 else 1e-5
+    assert (outs[0] - outs[1]).float().norm() <= close * outs[0].float().norm()
