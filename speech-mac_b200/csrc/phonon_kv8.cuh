@@ -514,15 +514,15 @@ __global__ void __launch_bounds__(128) kv8_read_kernel(Kv8ReadParams p) {
 // weights that matter stay inside fp32's range.
 //
 // Up to four rows that share a head (a decode step): 8-bit integer products,
-// the cache's bytes as they lie. q is held as an integer of 23 bits (15 in
-// bf16 rows, whose own 8 it keeps) relative to the row's maximum, split into
-// signed bytes: columns 2r, 2r + 1 are the first two of row r and a second
-// column tile has the third. A score's sums are exact; so are those of the
-// output per turn, with the weights as integers of 32 bits, a byte a column.
-// (The cache's bytes are unsigned, 128 too large: products with a constant -128
-// in their place start the sums.) What is left are q's and the weights' own
-// roundings (2^-24 of a row's largest; 2^-33 of the largest weight, or its
-// fp32's) and the turns' fp32 sums.
+// the cache's bytes as they lie. q is held as an integer of 31 bits relative
+// to the row's maximum (an element keeps fp32's 24 bits down to 2^-7 of it,
+// bf16's 8 down to 2^-23), split into signed bytes: columns 2r, 2r + 1 are the
+// first two of row r and a second column tile has the others. A score's sums
+// are exact; so are those of the output per turn, with the weights as integers
+// of 32 bits, a byte a column. (The cache's bytes are unsigned, 128 too large:
+// products with a constant -128 in their place start the sums.) What is left
+// are q's and the weights' own roundings (2^-32 of a row's largest; 2^-33 of
+// the largest weight, or its fp32's) and the turns' fp32 sums.
 //
 // More rows: products of halves, the conversion of a block's bytes shared by
 // the rows. Byte | 0x6400 is the half 1152 + integer, minus 1152 the integer,
@@ -902,9 +902,9 @@ __global__ void __launch_bounds__(32 * kWarps, kCtas) kv8_attention_kernel(Kv8At
 #pragma unroll
     for (int s = 0; s < kStages - 1; ++s) copy(0, s, s);
     fetch(1, kTurns);
-    // q as B fragments; column g is row g (halves), or byte g % 2 of row g / 2 (qh) and its third byte (ql)
+    // q as B fragments; column g is row g (halves), or byte g % 2 of row g / 2 (qh) and byte 2 + g % 2 (ql)
     constexpr int QS = kInt ? D / 32 : KS;  // steps of a score
-    uint32_t qh[NT][QS][2], ql[NT][kFine || kMode == KV8_INT_F32 ? QS : 1][2];
+    uint32_t qh[NT][QS][2], ql[NT][kFine || kInt ? QS : 1][2];
     float f[NT][RT];  // 2^(row exponent) of the lane's rows
     int pos[NT][RT];
 #pragma unroll
@@ -925,29 +925,26 @@ __global__ void __launch_bounds__(32 * kWarps, kCtas) kv8_attention_kernel(Kv8At
         if (row_bad && t == 0 && r < n_rows) kv8_flag(p.seqs, i, kStatusNonFinite);
         // exponent of the maximum, kept where both powers below are normal
         // (integers: the maximum times 2^(kTop - e) is at most 1.984375 * 2^kTop, whose bytes fit)
-        constexpr int kTop = kMode == KV8_INT_F32 ? 22 : kMode == KV8_INT_BF16 ? 14 : 12;
+        constexpr int kTop = kInt ? 30 : 12;
         const uint32_t top_bits = __float_as_uint(amax);
         const int above = kInt && (top_bits & 0x7fffffu) > 0x7e0000u ? 1 : 0;
-        const int e = min(max(static_cast<int>(top_bits >> 23) - 127 + above, -104), 126);
+        const int e = min(max(static_cast<int>(top_bits >> 23) - 127 + above, kTop - 126), 126);
         const float up = pow2i(kTop - e), back = pow2i(e - kTop);
 #pragma unroll
         for (int c = 0; c < KS; ++c) {
             const float x[4] = {v[c].x * up, v[c].y * up, v[c].z * up, v[c].w * up};
             if constexpr (kInt) {
-                // signed bytes d0 * 65536 + d1 * 256 + d2 (d0 * 256 + d1), |d0| <= 127
-                uint32_t first = 0, third = 0;
+                // signed bytes ((d0 * 256 + d1) * 256 + d2) * 256 + d3, |d0| <= 127 (unsigned: a row that is not finite wraps)
+                uint32_t first = 0, rest = 0;
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
-                    int y = __float2int_rn(x[k]);
-                    if constexpr (kMode == KV8_INT_F32) {
-                        third |= (static_cast<uint32_t>(y) & 0xffu) << (8 * k);
-                        y = (y + 128) >> 8;
-                    }
-                    const int d1 = static_cast<int8_t>(y), d0 = (y - d1) >> 8;
-                    first |= (static_cast<uint32_t>(g & 1 ? d1 : d0) & 0xffu) << (8 * k);
+                    const uint32_t y3 = static_cast<uint32_t>(__float2int_rn(x[k]));
+                    const int y2 = static_cast<int>(y3 + 128) >> 8, y1 = (y2 + 128) >> 8, y0 = (y1 + 128) >> 8;
+                    first |= (static_cast<uint32_t>(g & 1 ? y1 : y0) & 0xffu) << (8 * k);
+                    rest |= ((g & 1 ? y3 : static_cast<uint32_t>(y2)) & 0xffu) << (8 * k);
                 }
                 qh[n][c / 2][c % 2] = first;
-                if constexpr (kMode == KV8_INT_F32) ql[n][c / 2][c % 2] = third;
+                ql[n][c / 2][c % 2] = rest;
             } else {
                 qh[n][c][0] = half2_bits(x[0], x[1]);
                 qh[n][c][1] = half2_bits(x[2], x[3]);
@@ -968,13 +965,12 @@ __global__ void __launch_bounds__(32 * kWarps, kCtas) kv8_attention_kernel(Kv8At
     }
 
     // what a score's sums start from: -128 times those of q's bytes
-    int q_base[4] = {0, 0, 0, 0}, q_base3[4] = {0, 0, 0, 0};
+    int q_base[4] = {0, 0, 0, 0}, q_base2[4] = {0, 0, 0, 0};
     if constexpr (kInt) {
 #pragma unroll
         for (int c = 0; c < QS; ++c) {
             imma_s8_s8(q_base, q_base, kKv8Minus128, kKv8Minus128, kKv8Minus128, kKv8Minus128, qh[0][c][0], qh[0][c][1]);
-            if constexpr (kMode == KV8_INT_F32)
-                imma_s8_s8(q_base3, q_base3, kKv8Minus128, kKv8Minus128, kKv8Minus128, kKv8Minus128, ql[0][c][0], ql[0][c][1]);
+            imma_s8_s8(q_base2, q_base2, kKv8Minus128, kKv8Minus128, kKv8Minus128, kKv8Minus128, ql[0][c][0], ql[0][c][1]);
         }
     }
 
@@ -1029,14 +1025,12 @@ __global__ void __launch_bounds__(32 * kWarps, kCtas) kv8_attention_kernel(Kv8At
 #pragma unroll
                 for (int c = 0; c < QS; ++c) {
                     imma_u8_s8(x, c ? x : q_base, kw[0][2 * c], kw[1][2 * c], kw[0][2 * c + 1], kw[1][2 * c + 1], qh[0][c][0], qh[0][c][1]);
-                    if constexpr (kMode == KV8_INT_F32)
-                        imma_u8_s8(y, c ? y : q_base3, kw[0][2 * c], kw[1][2 * c], kw[0][2 * c + 1], kw[1][2 * c + 1], ql[0][c][0], ql[0][c][1]);
+                    imma_u8_s8(y, c ? y : q_base2, kw[0][2 * c], kw[1][2 * c], kw[0][2 * c + 1], kw[1][2 * c + 1], ql[0][c][0], ql[0][c][1]);
                 }
 #pragma unroll
                 for (int h = 0; h < 2; ++h)
-                    c4[0][2 * h] = kMode == KV8_INT_F32 ? fmaf(static_cast<float>(x[2 * h]), 65536.0f,
-                                                               static_cast<float>(x[2 * h + 1] * 256 + y[2 * h]))
-                                                        : static_cast<float>(x[2 * h] * 256 + x[2 * h + 1]);
+                    c4[0][2 * h] = fmaf(static_cast<float>(x[2 * h] * 256 + x[2 * h + 1]), 65536.0f,
+                                        static_cast<float>(y[2 * h] * 256 + y[2 * h + 1]));
             } else {
 #pragma unroll
                 for (int n = 0; n < NT; ++n) c4[n][0] = c4[n][1] = c4[n][2] = c4[n][3] = 0.0f;
