@@ -568,7 +568,14 @@ __global__ void __launch_bounds__(kKv8PromptThreads, 1) kv8_prompt_kernel(Kv8Att
             auto convert = [&](const uint4 (&w)[kPieces], int n) {
                 const int unit = converter + n * kKv8Converters, turn = unit / (2 * kPages), stage = turn % kStages, page = unit % kPages;
                 const bool values = unit & kPages;
-                if (turn >= kStages) wait((values ? v_empty : k_empty) + 8 * stage, turn / kStages - 1);
+                // Units of keys wait for the values' stage too: a warp has a unit of every turn but
+                // not of both kinds, and a wait that skipped a phase would take the one before for
+                // its own. (P V of the stage's last turn is behind S of this one anyway; units of
+                // values do not wait for the keys' stage, which may be two phases on.)
+                if (turn >= kStages) {
+                    wait(v_empty + 8 * stage, turn / kStages - 1);
+                    if (!values) wait(k_empty + 8 * stage, turn / kStages - 1);
+                }
                 if (values) {
                     const uint32_t to = s_v + stage * kTileBytes + (page * 2 + (vt >> 1)) * 128 + vg * 16 + (vt & 1) * 8;
 #pragma unroll
