@@ -829,10 +829,11 @@ struct PhononCuda {
     // contents: batch and split counts, attention grid, buffers.
     struct StepShape {
         int R = -1, S = -1, chunks = -1;
+        int seq_rows = 1;  // 8-bit K/V: the append and attention launches of a prefill are not a step's
         const void* in = nullptr;
         const void* out = nullptr;
         bool operator==(const StepShape& o) const {
-            return R == o.R && S == o.S && chunks == o.chunks && in == o.in && out == o.out;
+            return R == o.R && S == o.S && chunks == o.chunks && seq_rows == o.seq_rows && in == o.in && out == o.out;
         }
     };
     StepShape last_shape, graph_shape;
@@ -1582,6 +1583,7 @@ int enqueue_layers_graphed(PhononCuda* c, const Batch& b, const float* in, float
     // attention grid is fixed except for small (static) plans.
     shape.S = kv_is_q8(c) ? b.kv8_length : c->attn_tma ? 0 : b.S;
     shape.chunks = kv_is_q8(c) ? 0 : b.attn_grid;
+    if (kv_is_q8(c)) shape.seq_rows = b.seq_rows;
     shape.in = in;
     shape.out = final_out;
     if (c->graph_exec && c->graph_shape == shape) {

@@ -235,3 +235,25 @@ def test_prefill_of_a_long_context(cuda_ok, oracle, weights12):
     om.free_stream(cache)
     ctx.close()
     assert rt.rel_err(last, x) < FINAL_TOL
+
+
+@pytest.mark.parametrize("n", [6, 40])
+def test_prefills_and_steps_of_the_same_rows_take_turns(cuda_ok, weights12, n):
+    """Prompts of n rows and steps of n streams have the same row count, buffers and length class: neither may replay the
+    other's graph. Bit for bit what direct launches give."""
+    outs = []
+    for direct in (False, True):
+        ctx = context(weights12[:3], n, 8 * (n + 2))
+        ctx.profile(direct)
+        g = synth.Generator(31)
+        streams = [ctx.stream_alloc(64) for _ in range(n)]
+        got = [ctx.append(s, g.normal(n * 512).reshape(n, 512)) for s in streams]
+        got += [ctx.step(streams, [n + t] * n, g.normal(n * 512).reshape(n, 512)) for t in range(4)]
+        more = [ctx.stream_alloc(64) for _ in range(2)]
+        got += [ctx.append(s, g.normal(n * 512).reshape(n, 512)) for s in more]
+        got += [ctx.step(streams, [n + 4 + t] * n, g.normal(n * 512).reshape(n, 512)) for t in range(3)]
+        got += [x for s in streams + more for x in ctx.kv_read(s, 0, n + 7 if s in streams else n)]
+        outs.append(got)
+        ctx.close()
+    for a, b in zip(*outs):
+        np.testing.assert_array_equal(a, b)
