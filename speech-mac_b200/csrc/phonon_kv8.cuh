@@ -28,6 +28,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <type_traits>
+
 namespace phonon {
 
 constexpr int kKv8Block = kPage;  // positions that share a scale (a page)
@@ -509,9 +511,16 @@ __global__ void __launch_bounds__(128) kv8_read_kernel(Kv8ReadParams p) {
 // fp32: with s = scale log2(e) 2^eK (q.K) + eV, the weight 2^(s - M) is the
 // softmax weight times the block's value scale, so that O needs no scaling of
 // its own, and the sum of weights takes 2^(s - M - eV). M is the running
-// maximum of s; eV is taken relative to a warp's first page's, so that s keeps
-// its precision whatever the values' size. eV spans 112 at most, so
-// weights that matter stay inside fp32's range.
+// maximum of s.
+//
+// The weights are rounded to a step of the largest there can be (below), so
+// eV is taken relative to a reference of the warp's pages: their largest that
+// is at most kKv8Spread above their smallest. Blocks that do not lie within
+// kKv8Spread below it (one loud position among quiet ones raises its block's
+// scale by up to 2^112, whatever its weight) are multiplied in fp32, element
+// by element, behind the others: a step of theirs would be all that the other
+// blocks weigh, or the other way round. (512 sequences of about 1000 positions:
+// 87 us, with one position in 1000 that is 2^20 times louder 103, in 100 142.)
 //
 // Up to four rows that share a head (a decode step): 8-bit integer products,
 // the cache's bytes as they lie. q is held as an integer of 31 bits relative
@@ -550,6 +559,21 @@ struct Kv8AttnParams {
 };
 
 constexpr float kKv8WeightBits = 14.0f;  // weights are held times 2^14: a half keeps 11 bits down to 2^-28
+
+// The value scales 2^(ref - kKv8Spread) to 2^ref enter the weights; more would
+// cost as many of the smallest scale's bits (byte products keep 2^-25 of the
+// largest weight at the bottom of the range, halves 2^-31).
+constexpr int kKv8Spread = 8;
+constexpr int kKv8Above = 64;  // no block's scale is further above ref, so that sums stay inside fp32
+
+// The reference of blocks with value scales (biased exponents) from lo to hi.
+__device__ __forceinline__ int kv8_reference(int lo, int hi) { return max(min(hi, lo + kKv8Spread), hi - kKv8Above); }
+
+// Whether a block's scale, relative to the reference, enters the weights.
+__device__ __forceinline__ bool kv8_near(int ev) { return static_cast<unsigned>(ev + kKv8Spread) <= static_cast<unsigned>(kKv8Spread); }
+
+// Byte k of a cache word as a number.
+__device__ __forceinline__ float kv8_number(uint32_t w, int k) { return __uint_as_float(0x4b000000u | (w >> (8 * k) & 0xffu)) - 8388736.0f; }
 
 // Weights as integers of 32 bits: 1 is the largest float below 2^32.
 constexpr float kKv8FixedScale = 4294967040.0f;
@@ -632,7 +656,7 @@ __device__ __forceinline__ uint32_t half2_bits(float a, float b) {
 
 __device__ __forceinline__ float2 half2_floats(uint32_t u) { return __half22float2(*reinterpret_cast<__half2*>(&u)); }
 
-// M, sum, reference of eV and four dims of a row, over some of its positions.
+// M, sum of weights, reference of eV (biased) and four dims of a row, over some of its positions.
 struct Kv8Share {
     float m, l;
     int ref;
@@ -642,14 +666,17 @@ struct Kv8Share {
 __device__ __forceinline__ Kv8Share kv8_nothing() { return {-INFINITY, 0.0f, 127, make_float4(0.0f, 0.0f, 0.0f, 0.0f)}; }
 
 __device__ __forceinline__ void kv8_fold(Kv8Share& s, float4 ml, float4 b) {
-    if (s.m == -INFINITY && !isnan(s.l)) s.ref = __float_as_int(ml.z);  // nothing yet: as it comes
-    // into s's reference (an exact power of two, and 0 to add where the references agree), then the larger maximum
-    const int shift = __float_as_int(ml.z) - s.ref;
-    const float m2 = ml.x + static_cast<float>(shift), x = fmaxf(s.m, m2);
-    const float wa = s.m == -INFINITY ? 0.0f : ex2(s.m - x), wb = m2 == -INFINITY ? 0.0f : ex2(m2 - x);
+    // the sums go into the larger reference (an exact power of two), then the larger maximum
+    const int other = __float_as_int(ml.z);
+    if (s.m == -INFINITY && !isnan(s.l)) s.ref = other;  // nothing yet: as it comes
+    const int ref = ml.x == -INFINITY ? s.ref : max(s.ref, other);
+    const float x = fmaxf(s.m, ml.x);
+    const float wa = s.m == -INFINITY ? 0.0f : ex2(s.m - x), wb = ml.x == -INFINITY ? 0.0f : ex2(ml.x - x);
+    const float oa = wa * pow2i(s.ref - ref), ob = wb * pow2i(min(other - ref, 0));
     s.m = x;
-    s.l = s.l * wa + ml.y * (pow2i(min(max(-shift, -126), 126)) * wb);
-    s.a = make_float4(s.a.x * wa + b.x * wb, s.a.y * wa + b.y * wb, s.a.z * wa + b.z * wb, s.a.w * wa + b.w * wb);
+    s.ref = ref;
+    s.l = s.l * wa + ml.y * wb;
+    s.a = make_float4(s.a.x * oa + b.x * ob, s.a.y * oa + b.y * ob, s.a.z * oa + b.z * ob, s.a.w * oa + b.w * ob);
 }
 
 // Four dims of row rho of a K/V head's rows, to the output.
@@ -829,7 +856,8 @@ __global__ void __launch_bounds__(32 * kWarps, kCtas) kv8_attention_kernel(Kv8At
     extern __shared__ __align__(16) uint8_t s_ring[];  // [kWarps][kStages][PB][kPageBytes], then the warps' results
     float(*s_o)[kRows][D] = reinterpret_cast<float(*)[kRows][D]>(s_ring);
     __shared__ float4 s_ml[kWarps][kRows];  // M, sum, eV's reference
-    __shared__ int s_last;
+    __shared__ int s_last, s_lowest[kWarps];
+    __shared__ int4 s_range[kWarps];
     pdl_wait();
     pdl_trigger();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
@@ -992,13 +1020,57 @@ __global__ void __launch_bounds__(32 * kWarps, kCtas) kv8_attention_kernel(Kv8At
     const int from0 = 8 * t + (g >> 1), from1 = from0 + 4;   // lanes with the weights of positions 2t, 2t + 1 of row g / 2
     const uint32_t pick = g & 1 ? 0x6240u : 0x7351u;         // the weight byte that column g multiplies
 
-    const int ref = __shfl_sync(kFull, scales[0], 0) >> 8;  // the value scale that eV is relative to in this warp
+    // value scales, biased: the smallest of the CTA's first pages and of the warp's so far, the warp's largest up to
+    // kKv8Spread above it, the largest of all, and whether a page is hidden (kept out of the registers between windows)
+    const int lowest = __reduce_min_sync(kFull, ids[0] >= 0 ? scales[0] >> 8 : 255);
+    if (lane == 0) s_lowest[warp] = lowest;
+    if constexpr (kWarps > 1) __syncthreads();
+    else __syncwarp();
+    const auto start = [&] {
+        int lo = 255;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) lo = min(lo, s_lowest[w]);
+        return make_int4(lo, 0, 0, 0);
+    };
+    int ref = 127;  // what eV is relative to
+    // Takes a window's pages into the range and hides those whose value scale does not enter the weights: the lane's, or -1.
+    const auto look = [&](int4& range) {
+        const int ev = ids[0] >= 0 ? scales[0] >> 8 : 255;
+        range.x = min(range.x, __reduce_min_sync(kFull, ev));
+        range.y = max(range.y, __reduce_max_sync(kFull, ev <= range.x + kKv8Spread && ev < 255 ? ev : 0));
+        range.z = max(range.z, __reduce_max_sync(kFull, ev < 255 ? ev : 0));
+        if (range.z) ref = max(range.y ? min(range.y, range.x + kKv8Spread) : range.x, range.z - kKv8Above);
+        const int hidden = ids[0] >= 0 && !kv8_near(ev - ref) ? ids[0] : -1;
+        if (hidden >= 0) ids[0] = -1;
+        range.w |= __any_sync(kFull, hidden >= 0);
+        return hidden;
+    };
+    {
+        int4 range = start();
+        look(range);
+        if (lane == 0) s_range[warp] = range;
+    }
     int turn = 0, stage = 0;
     for (int at = first + warp * PB; at < last; at += kStep, ++turn, stage = stage + 1 == kStages ? 0 : stage + 1) {
         if (turn && turn % kTurns == 0) {
             ids[0] = ids[1];
             scales[0] = scales[1];
             fetch(1, turn + kTurns);
+            const int before = ref;
+            __syncwarp();
+            int4 range = s_range[warp];
+            look(range);
+            __syncwarp();
+            if (lane == 0) s_range[warp] = range;
+            if (ref != before) {  // O in the new unit: an exact power of two
+                const float by = pow2i(before - ref);
+#pragma unroll
+                for (int k = 0; k < KS; ++k)
+#pragma unroll
+                    for (int n = 0; n < NT; ++n)
+#pragma unroll
+                        for (int j = 0; j < OT; ++j) o[k][n][j] *= by;
+            }
         }
         asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
         {
@@ -1013,7 +1085,7 @@ __global__ void __launch_bounds__(32 * kWarps, kCtas) kv8_attention_kernel(Kv8At
             id[b] = __shfl_sync(kFull, ids[0], turn % kTurns * PB + b);
             ex[b] = __shfl_sync(kFull, scales[0], turn % kTurns * PB + b);
         }
-        float s[PB][NT][2][RT];  // positions g, g + 8
+        float s[PB][NT][2][RT];  // s + eV of positions g, g + 8
         float less[PB];          // 2^-eV
 #pragma unroll
         for (int b = 0; b < PB; ++b) {
@@ -1231,6 +1303,65 @@ __global__ void __launch_bounds__(32 * kWarps, kCtas) kv8_attention_kernel(Kv8At
                     kInt ? make_float4(x[0], x[1], y[0], y[1]) : make_float4(x[k], x[OT - 2 + k], y[k], y[OT - 2 + k]);
             }
         }
+    // The hidden pages in fp32, into the warp's share: the windows once more.
+    __syncwarp();
+    if (s_range[warp].w) {
+        const int unit_ref = ref;
+        int4 range = start();
+        for (int window = 0; first + warp * PB + window * kStep < last; window += kTurns) {
+            fetch(0, window);
+            const int away = look(range);
+            for (unsigned left = __ballot_sync(kFull, away >= 0); left; left &= left - 1) {
+                const int from = __ffs(left) - 1, ex = __shfl_sync(kFull, scales[0], from);
+                const int page = first + warp * PB + (window + from / PB) * kStep + from % PB;
+                const uint8_t* block = base + __shfl_sync(kFull, away, from) * page_bytes;
+                const float uk = __int_as_float((ex & 0xff) << 23);
+                const float unit = (kInt ? kKv8FixedScale : 1.0f) * pow2i((ex >> 8) - unit_ref);  // of a weight in O, and the value scale
+#pragma unroll 1
+                for (int r = 0; r < n_rows; ++r) {
+                    const int of = token(rho0 + r), position = at0 + of, key = page * kKv8Block + (lane & 15);
+                    const size_t row = static_cast<size_t>(sq.row0 + of) * p.q_stride +
+                                       static_cast<size_t>(head * p.group.d + rho0 + r - of * p.group.d) * D;
+                    // half the score of position lane % 16
+                    float dot = 0.0f;
+#pragma unroll 2
+                    for (int d = (lane >> 4) * (D / 2); d < ((lane >> 4) + 1) * (D / 2); d += 4) {
+                        const float4 x = load_row4<kBf16>(p.q, row + d);
+                        const uint32_t w = *reinterpret_cast<const uint32_t*>(block + (lane & 15) * D + d);
+                        dot = fmaf(x.x, kv8_number(w, 0), fmaf(x.y, kv8_number(w, 1), fmaf(x.z, kv8_number(w, 2), fmaf(x.w, kv8_number(w, 3), dot))));
+                    }
+                    dot = (dot + __shfl_xor_sync(kFull, dot, 16)) * uk;
+                    float z = fmaf(dot, p.scale, dot * p.scale_low);
+                    if (key > position || (p.window && key <= position - p.window)) z = -INFINITY;
+                    const float4 ml = s_ml[warp][r];
+                    float now = z;
+#pragma unroll
+                    for (int w = 1; w < 16; w <<= 1) now = fmaxf(now, __shfl_xor_sync(kFull, now, w));
+                    now = fmaxf(now, ml.x);
+                    const float by = ml.x == now ? 1.0f : ex2(ml.x - now);
+                    const float weight = ex2(z - (now == -INFINITY ? 0.0f : kInt ? now : now - kKv8WeightBits)), each = weight * unit;
+                    float sum = weight;
+#pragma unroll
+                    for (int w = 1; w < 16; w <<= 1) sum += __shfl_xor_sync(kFull, sum, w);
+#pragma unroll 1
+                    for (int j = 0; j < D / 32; ++j) {  // dim 32j + lane
+                        float& to = s_o[warp][r][j * 32 + lane];
+                        float x = to * by;
+#pragma unroll
+                        for (int w = 0; w < 4; ++w) {
+                            const uint32_t v = *reinterpret_cast<const uint32_t*>(block + kKv8Block * D + j * 512 + g * 64 + w * 16 + t * 4);
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) x = fmaf(__shfl_sync(kFull, each, kv8_value_pos(w, k)), kv8_number(v, k), x);
+                        }
+                        to = x;
+                    }
+                    __syncwarp();
+                    if (lane == 0) s_ml[warp][r] = make_float4(now, ml.y * by + sum, ml.z, 0.0f);
+                    __syncwarp();
+                }
+            }
+        }
+    }
     __syncthreads();
     constexpr int kQuads = D / 4;
     constexpr float kUnit = kInt ? 1.0f / kKv8FixedScale : 1.0f;

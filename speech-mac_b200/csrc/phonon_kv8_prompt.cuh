@@ -31,7 +31,8 @@
 //
 // fp32 rows: q (times the softmax scale) and the weights as two halves each (22
 // bits), two products each. bf16 rows: one half each (q's 8 bits are exact,
-// weights keep 11).
+// weights keep 11). Blocks whose value scale is far from the split's smallest
+// are hidden from the turns and added in fp32, a row a thread, at the end.
 //
 // 1024 rows a K/V head over 4096 positions, 32 heads: bf16, 128 dims 144 us
 // (475 TFLOP/s), fp32, 64 dims 136 us (253, twice that in products); the
@@ -177,7 +178,7 @@ __global__ void __launch_bounds__(kKv8PromptThreads, 1) kv8_prompt_kernel(Kv8Att
     extern __shared__ __align__(128) uint8_t s_mem[];  // q [tile][plane], kStages x keys, x values; then the rows' results
     __shared__ __align__(8) uint64_t s_bars[4 * kKv8PromptStages + 9];
     __shared__ uint32_t s_tmem;
-    __shared__ int s_failed, s_last;
+    __shared__ int s_failed, s_last, s_lo, s_hi;
     __shared__ float s_f[128 * kTiles];
     __shared__ float2 s_ml[2][128];  // M, sum
     pdl_wait();
@@ -227,6 +228,8 @@ __global__ void __launch_bounds__(kKv8PromptThreads, 1) kv8_prompt_kernel(Kv8Att
         }
         mbar_init(q_full, 8);
         s_failed = 0;
+        s_lo = 255;
+        s_hi = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 15) {
@@ -260,6 +263,26 @@ __global__ void __launch_bounds__(kKv8PromptThreads, 1) kv8_prompt_kernel(Kv8Att
                 for (int h = 0; h < 2; ++h) v[k][h] = load_row4<kBf16>(p.q, row + k * 32 + h * 4);
         };
         load_q(0, ahead[0]);
+        const uint8_t* exps = p.cache.exps + head * 2;
+        auto scales_of = [&](int at, bool in) {  // -1: no page
+            const int id = in ? __ldg(sq.pages + at) : -1;
+            return static_cast<unsigned>(id) < static_cast<unsigned>(p.cache.pool_pages)
+                       ? static_cast<int>(__ldg(reinterpret_cast<const unsigned short*>(exps + static_cast<size_t>(id) * p.cache.heads * 2)))
+                       : -1;
+        };
+        {  // the split's value scales
+            int lo = 255, hi = 0;
+            for (int at = first + threadIdx.x; at < last; at += 256) {
+                const int ex = scales_of(at, true);
+                if (ex >= 0) lo = min(lo, ex >> 8), hi = max(hi, ex >> 8);
+            }
+            lo = __reduce_min_sync(kFull, lo);
+            hi = __reduce_max_sync(kFull, hi);
+            if (lane == 0 && lo <= hi) {
+                atomicMin(&s_lo, lo);
+                atomicMax(&s_hi, hi);
+            }
+        }
 #pragma unroll 1
         for (int pass = 0; pass < passes; ++pass) {
             if (pass + 1 < passes) load_q(pass + 1, ahead[1]);
@@ -316,21 +339,15 @@ __global__ void __launch_bounds__(kKv8PromptThreads, 1) kv8_prompt_kernel(Kv8Att
         const int whole_last = max(pos_lo + 1, 0) / kKv8Block;
         const int whole_first = p.window && pos_hi >= p.window ? (pos_hi - p.window) / kKv8Block + 1 : 0;
         // scales of this stream's pages of 8 turns, and of the 8 after them, a lane each
-        const uint8_t* exps = p.cache.exps + head * 2;
-        auto scales_of = [&](int at, bool in) {  // -1: no page
-            const int id = in ? __ldg(sq.pages + at) : -1;
-            return static_cast<unsigned>(id) < static_cast<unsigned>(p.cache.pool_pages)
-                       ? static_cast<int>(__ldg(reinterpret_cast<const unsigned short*>(exps + static_cast<size_t>(id) * p.cache.heads * 2)))
-                       : -1;
-        };
         auto fetch = [&](int n) {
             const int at = first + turn_of(stream, n + lane / kPages) * kPages + lane % kPages;
             return scales_of(at, at < last);
         };
         int scales = fetch(0), scales_next = fetch(8);
-        // the value scale that eV is relative to: the split's first page's
-        const int first_scales = scales_of(first, turns > 0), ref = first_scales < 0 ? 127 : first_scales >> 8;
-        wait(q_full, 0);  // every row's factor
+        wait(q_full, 0);  // every row's factor, and the value scales' range
+        const int ref = s_lo <= s_hi ? kv8_reference(s_lo, s_hi) : 127;  // what eV is relative to
+        const auto hide = [&](int ex) { return ex >= 0 && kv8_near((ex >> 8) - ref) ? ex : -1; };  // pages for behind the turns
+        scales = hide(scales);
         const float f = s_f[mine] * (kBf16 ? p.scale : pow2i(scale_e));  // of a product of q, as a score
         const int pos = at0 + token(rho0 + mine), low = p.window ? pos - p.window : -1;
         const uint32_t s_tiles = tmem + stream * 2 * kKeys + (static_cast<uint32_t>(quarter * 32) << 16);
@@ -361,7 +378,7 @@ __global__ void __launch_bounds__(kKv8PromptThreads, 1) kv8_prompt_kernel(Kv8Att
         };
         for (int n = 0; n < n_turns; ++n) {
             if (n && n % 8 == 0) {
-                scales = scales_next;
+                scales = hide(scales_next);
                 scales_next = fetch(n + 8);
             }
             const int page0 = first + turn_of(stream, n) * kPages, lane0 = n % 8 * kPages;
@@ -395,7 +412,8 @@ __global__ void __launch_bounds__(kKv8PromptThreads, 1) kv8_prompt_kernel(Kv8Att
                     float most = -INFINITY;
 #pragma unroll
                     for (int k = h * 16; k < h * 16 + 16; k += 2) most = max3(most, x[k], x[k + 1]);
-                    const float u = __int_as_float((ex & 0xff) << 23), add = static_cast<float>((ex >> 8) - ref);
+                    const float u = __int_as_float((ex & 0xff) << 23);
+                    const float add = static_cast<float>((ex >> 8) - ref);
                     const float z = fmaf(most, u * f, add);
                     top = fmaxf(top, most == -INFINITY ? -INFINITY : z);
                 }
@@ -494,20 +512,84 @@ __global__ void __launch_bounds__(kKv8PromptThreads, 1) kv8_prompt_kernel(Kv8Att
         const auto both_sync = [] { asm volatile("bar.sync 1, 256;" ::: "memory"); };
         s_ml[stream][r] = make_float2(m, s_failed ? __int_as_float(0x7fc00000) : l);  // a wait that ran out: NaN
         both_sync();  // and both streams' products are done: the operands' room takes the results
-        const float2 other = s_ml[stream ^ 1][r];
-        const float most = two ? m : fmaxf(m, other.x);
-        const float mine_by = m == -INFINITY ? 0.0f : ex2(m - most), other_by = two || other.x == -INFINITY ? 0.0f : ex2(other.x - most);
-        const float sum = s_ml[stream][r].y * (isnan(s_ml[stream][r].y) ? 1.0f : mine_by) + (two ? 0.0f : other.y * (isnan(other.y) ? 1.0f : other_by));
-        const float by = active == 1 ? mine_by * kv8_inverse(sum, ref, 1.0f) : mine_by;
         float* s_o = reinterpret_cast<float*>(s_mem) + (stream * 128 + r) * kPitch;
+        float most, sum, by;
+        const auto factors = [&] {
+            const float2 own = s_ml[stream][r], other = s_ml[stream ^ 1][r];
+            most = two ? own.x : fmaxf(own.x, other.x);
+            const float mine_by = own.x == -INFINITY ? 0.0f : ex2(own.x - most), other_by = two || other.x == -INFINITY ? 0.0f : ex2(other.x - most);
+            sum = own.y * (isnan(own.y) ? 1.0f : mine_by) + (two ? 0.0f : other.y * (isnan(other.y) ? 1.0f : other_by));
+            by = active == 1 ? mine_by * kv8_inverse(sum, ref, 1.0f) : mine_by;
+        };
+        factors();
+        const bool mixed = s_hi - s_lo > kKv8Spread;  // pages that the turns left out
+        const float first_by = mixed ? 1.0f : by;
 #pragma unroll
         for (int j = 0; j < D / 32; ++j)
 #pragma unroll
             for (int g = 0; g < 8; ++g) {  // dims 4g.. of 32 are columns g, 8 + g, 16 + g, 24 + g
-                const float2 x = mul2(make_float2(o[j * 32 + g], o[j * 32 + 8 + g]), make_float2(by, by));
-                const float2 y = mul2(make_float2(o[j * 32 + 16 + g], o[j * 32 + 24 + g]), make_float2(by, by));
+                const float2 x = mul2(make_float2(o[j * 32 + g], o[j * 32 + 8 + g]), make_float2(first_by, first_by));
+                const float2 y = mul2(make_float2(o[j * 32 + 16 + g], o[j * 32 + 24 + g]), make_float2(first_by, first_by));
                 *reinterpret_cast<float4*>(s_o + j * 32 + 4 * g) = make_float4(x.x, x.y, y.x, y.y);
             }
+        if (mixed) {  // this row's scores, weights and sums of them in fp32
+            const int of = token(rho0 + mine);
+            const size_t row = static_cast<size_t>(sq.row0 + of) * p.q_stride + static_cast<size_t>(head * p.group.d + rho0 + mine - of * p.group.d) * D;
+#pragma unroll 1
+            for (int x = 0; x < n_turns * kPages; ++x) {
+                const int page = first + turn_of(stream, x / kPages) * kPages + x % kPages, ex = scales_of(page, page < last);
+                if (ex < 0 || kv8_near((ex >> 8) - ref)) continue;
+                const uint8_t* block = p.cache.pool + (static_cast<size_t>(sq.pages[page]) * p.cache.heads + head) * (2 * kKv8Block * D);
+                float w[kKv8Block];
+#pragma unroll
+                for (int k = 0; k < kKv8Block; ++k) w[k] = 0.0f;
+#pragma unroll 1
+                for (int d = 0; d < D; d += 4) {
+                    const float4 v = load_row4<kBf16>(p.q, row + d);
+#pragma unroll
+                    for (int k = 0; k < kKv8Block; ++k) {
+                        const uint32_t u = *reinterpret_cast<const uint32_t*>(block + k * D + d);
+                        w[k] = fmaf(v.x, kv8_number(u, 0), fmaf(v.y, kv8_number(u, 1), fmaf(v.z, kv8_number(u, 2), fmaf(v.w, kv8_number(u, 3), w[k]))));
+                    }
+                }
+                const float uk = __int_as_float((ex & 0xff) << 23), unit = pow2i((ex >> 8) - ref);
+                float now = m;
+#pragma unroll
+                for (int k = 0; k < kKv8Block; ++k) {
+                    const int key = page * kKv8Block + k;
+                    w[k] = key <= pos && key > low ? fmaf(w[k] * uk, p.scale, w[k] * uk * p.scale_low) : -INFINITY;
+                    now = fmaxf(now, w[k]);
+                }
+                const float by = m == now ? 1.0f : ex2(m - now), zero = now == -INFINITY ? 0.0f : now - kKv8WeightBits;
+                m = now;
+                l *= by;
+#pragma unroll
+                for (int k = 0; k < kKv8Block; ++k) {
+                    w[k] = ex2(w[k] - zero);
+                    l += w[k];
+                    w[k] *= unit;
+                }
+#pragma unroll 1
+                for (int k = 0; k < D / 4; ++k) {
+                    float4& at = *reinterpret_cast<float4*>(s_o + 4 * k);
+                    float sum[4] = {at.x * by, at.y * by, at.z * by, at.w * by};
+#pragma unroll
+                    for (int t = 0; t < 4; ++t) {  // positions 2t, 2t + 1, 2t + 8, 2t + 9
+                        const uint4 v = *reinterpret_cast<const uint4*>(block + kKv8Block * D + (k * 4 + t) * 16);
+                        const uint32_t u[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                        for (int j = 0; j < 4; ++j)
+                            sum[j] = fmaf(w[2 * t], kv8_number(u[j], 0), fmaf(w[2 * t + 1], kv8_number(u[j], 1),
+                                     fmaf(w[2 * t + 8], kv8_number(u[j], 2), fmaf(w[2 * t + 9], kv8_number(u[j], 3), sum[j]))));
+                    }
+                    at = make_float4(sum[0], sum[1], sum[2], sum[3]);
+                }
+            }
+            s_ml[stream][r] = make_float2(m, s_failed ? __int_as_float(0x7fc00000) : l);
+            both_sync();
+            factors();
+            for (int k = 0; k < D; ++k) s_o[k] *= by;
+        }
         const size_t part0 = (static_cast<size_t>(item) * p.splits + split) * p.tile_rows;
         if (active > 1 && (two || stream == 0) && stream * 128 + r < n_rows)
             p.part_ml[part0 + stream * 128 + r] = make_float4(most, sum, __int_as_float(ref), 0.0f);
