@@ -149,14 +149,16 @@ __global__ void __launch_bounds__(128, kCtas) qk_norm_rope_kernel(QkParams p) {
                 const int h0 = (u - (side ? pass_q : 0)) * kPerWarp + sub;
 #pragma unroll
                 for (int a = 0; a < kAhead; ++a) {
-                    const float r = p.weight[side] ? rsqrtf(fmaf(sq[a], 1.0f / D, p.epsilon)) : 1.0f;
+                    // (0 where the pass has no head: its x is 0, and without an epsilon so is the mean)
+                    const bool there = u + a < side_end && h0 + a * kPerWarp < heads;
+                    const float r = !there ? 0.0f : p.weight[side] ? rsqrtf(fmaf(sq[a], 1.0f / D, p.epsilon)) : 1.0f;
                     float y[8];
 #pragma unroll
                     for (int k = 0; k < 8; ++k) x[a][k] *= r;
 #pragma unroll
                     for (int k = 0; k < 8; ++k) {
                         y[k] = fmaf(x[a][k], a0[k], x[a][k ^ kOther] * a1[k]);
-                        finite = fmaf(y[k], 0.0f, finite);  // (0 where the pass has no head: its x is 0)
+                        finite = fmaf(y[k], 0.0f, finite);
                     }
                     Raw packed[2];
 #pragma unroll
@@ -169,7 +171,7 @@ __global__ void __launch_bounds__(128, kCtas) qk_norm_rope_kernel(QkParams p) {
                             words[k % 4 / 2] = *reinterpret_cast<const uint32_t*>(&b);
                         }
                     }
-                    if (u + a < side_end && h0 + a * kPerWarp < heads) {
+                    if (there) {
                         char* to = out + (h0 + a * kPerWarp) * (D * kSize);
                         *reinterpret_cast<Raw*>(to + chunk[0] * kSize) = packed[0];
                         *reinterpret_cast<Raw*>(to + chunk[1] * kSize) = packed[1];

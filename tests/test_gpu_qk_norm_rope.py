@@ -179,3 +179,26 @@ def test_a_layer_of_device_calls(cuda_ok):
         want, size = model.attention(qa, held[0].values(), vals)
         lim = model.attention_bound(size, np.abs(vals).max(), want, dim, b, False)
         assert (np.abs(out[a:b].double().cpu().numpy() - want) <= lim).all()
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("rows,heads,kv_heads,dim", [(3, 8, 8, 64), (1, 5, 0, 64), (40, 3, 1, 128), (7, 1, 9, 32), (2000, 5, 2, 32)])
+def test_no_epsilon_flags_no_fine_row(cuda_ok, rows, heads, kv_heads, dim, bf16):
+    """epsilon 0 and head counts that leave passes partly empty: outputs are finite, and so says the status."""
+    rng = np.random.default_rng(heads)
+    dtype = torch.bfloat16 if bf16 else torch.float32
+    x = torch.tensor(rng.standard_normal((rows, heads + kv_heads, dim)), dtype=torch.float32).to(dtype).cuda()
+    positions = np.arange(rows)
+    pos = torch.tensor(positions, dtype=torch.int32, device="cuda")
+    w = torch.tensor(1 + 0.3 * rng.standard_normal(dim), dtype=torch.float32, device="cuda")
+    out = torch.empty_like(x)
+    status = torch.zeros(rows, dtype=torch.int32, device="cuda")
+    wide = (heads + kv_heads) * dim
+    rt.QkNormRope(x.data_ptr(), x[:, heads:].data_ptr(), out.data_ptr(), out[:, heads:].data_ptr(), rows, heads, kv_heads, dim,
+                  pos.data_ptr(), rt.ROWS_BF16 if bf16 else rt.ROWS_F32, q_stride=wide, k_stride=wide, q_out_stride=wide,
+                  k_out_stride=wide, q_weight_ptr=w.data_ptr(), k_weight_ptr=w.data_ptr(), epsilon=0.0)(status.data_ptr())
+    torch.cuda.synchronize()
+    assert not status.any()
+    want = formula(x.double().cpu().numpy(), w.double().cpu().numpy(), positions, dim, False, 0.0, 10000.0)
+    lim = bound(x.double().cpu().numpy(), w.double().cpu().numpy(), dim, 0.0, want, bf16)
+    assert (np.abs(out.double().cpu().numpy() - want) <= lim).all()
