@@ -75,6 +75,7 @@ __global__ void __launch_bounds__(128, kCtas) qk_norm_rope_kernel(QkParams p) {
     const int items = p.rows * p.slices, stride = gridDim.x * (blockDim.x >> 5);
     int item = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
     if (item >= items) return;  // the whole warp
+    const float smallest = p.epsilon < 1e-25f ? 1e-25f : 0.0f;  // sums below lose bits that count
     Raw raw[kAhead][2];
     // the passes [u, min(u + kAhead, the side's end, stop)) of a row
     auto load = [&](int row, int u, int stop) {
@@ -112,7 +113,8 @@ __global__ void __launch_bounds__(128, kCtas) qk_norm_rope_kernel(QkParams p) {
             sn[two] = s;
             cs[one] = cs[two] = c;
         }
-        float finite = 0.0f;  // NaN once an output is not
+        float finite = 0.0f;  // NaN once an output, rounded, is not
+        __nv_bfloat162 finite2 = __floats2bfloat162_rn(0.0f, 0.0f);
         int u = first;
 #pragma unroll
         for (int side = 0; side < 2; ++side) {
@@ -147,18 +149,38 @@ __global__ void __launch_bounds__(128, kCtas) qk_norm_rope_kernel(QkParams p) {
 #pragma unroll
                     for (int a = 0; a < kAhead; ++a) sq[a] += __shfl_xor_sync(kFull, sq[a], o);
                 const int h0 = (u - (side ? pass_q : 0)) * kPerWarp + sub;
+                float inverse[kAhead], most = 0.0f, least = 1.0f;
+#pragma unroll
+                for (int a = 0; a < kAhead; ++a) {
+                    inverse[a] = rsqrtf(fmaf(sq[a], 1.0f / D, p.epsilon));
+                    most = fmaxf(most, sq[a]);
+                    least = fminf(least, sq[a]);
+                }
+                // squares outside fp32's range: of x times a power of two
+                if (__any_sync(kFull, !(most < 1e37f) || least < smallest)) {
+#pragma unroll
+                    for (int a = 0; a < kAhead; ++a) {
+                        const float by = sq[a] < 1.0f ? 0x1p+64f : 0x1p-64f;
+                        float again = 0.0f;
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) again = fmaf(x[a][k] * by, x[a][k] * by, again);
+#pragma unroll
+                        for (int o = kLanes / 2; o > 0; o >>= 1) again += __shfl_xor_sync(kFull, again, o);
+                        if (!(sq[a] < 1e37f) || sq[a] < smallest) inverse[a] = rsqrtf(fmaf(again, 1.0f / D, p.epsilon * by * by)) * by;
+                    }
+                }
 #pragma unroll
                 for (int a = 0; a < kAhead; ++a) {
                     // (0 where the pass has no head: its x is 0, and without an epsilon so is the mean)
                     const bool there = u + a < side_end && h0 + a * kPerWarp < heads;
-                    const float r = !there ? 0.0f : p.weight[side] ? rsqrtf(fmaf(sq[a], 1.0f / D, p.epsilon)) : 1.0f;
+                    const float r = !there ? 0.0f : p.weight[side] ? inverse[a] : 1.0f;
                     float y[8];
 #pragma unroll
                     for (int k = 0; k < 8; ++k) x[a][k] *= r;
 #pragma unroll
                     for (int k = 0; k < 8; ++k) {
                         y[k] = fmaf(x[a][k], a0[k], x[a][k ^ kOther] * a1[k]);
-                        finite = fmaf(y[k], 0.0f, finite);
+                        if constexpr (!kBf16) finite = fmaf(y[k], 0.0f, finite);
                     }
                     Raw packed[2];
 #pragma unroll
@@ -169,6 +191,7 @@ __global__ void __launch_bounds__(128, kCtas) qk_norm_rope_kernel(QkParams p) {
                         } else if (k % 2 == 0) {
                             const __nv_bfloat162 b = __floats2bfloat162_rn(y[k], y[k + 1]);
                             words[k % 4 / 2] = *reinterpret_cast<const uint32_t*>(&b);
+                            finite2 = __hfma2(b, __floats2bfloat162_rn(0.0f, 0.0f), finite2);
                         }
                     }
                     if (there) {
@@ -180,6 +203,7 @@ __global__ void __launch_bounds__(128, kCtas) qk_norm_rope_kernel(QkParams p) {
             }
             u = side_end;
         }
+        if constexpr (kBf16) finite = __low2float(finite2) + __high2float(finite2);
         if (p.status && !__all_sync(kFull, finite == 0.0f) && lane == 0) flag_nonfinite(p.status, row);
         if (next >= items) break;
         item = next;

@@ -202,3 +202,38 @@ def test_no_epsilon_flags_no_fine_row(cuda_ok, rows, heads, kv_heads, dim, bf16)
     want = formula(x.double().cpu().numpy(), w.double().cpu().numpy(), positions, dim, False, 0.0, 10000.0)
     lim = bound(x.double().cpu().numpy(), w.double().cpu().numpy(), dim, 0.0, want, bf16)
     assert (np.abs(out.double().cpu().numpy() - want) <= lim).all()
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("size,eps", [(1e30, 1e-6), (1e19, 1e-6), (3e37, 0.0), (1e-20, 0.0), (1e-30, 0.0), (1e-36, 1e-72), (1e-12, 1e-26)])
+def test_squares_outside_the_range_of_floats(cuda_ok, size, eps, bf16):
+    """Rows whose squares overflow or vanish in 32 bits, beside an ordinary head, have the formula's norm."""
+    rng = np.random.default_rng(int(abs(math.log10(size))))
+    dtype = torch.bfloat16 if bf16 else torch.float32
+    x = torch.tensor(rng.standard_normal((9, 5, 64)) * np.array([size, 1.0, size, 1.0, size])[None, :, None], dtype=torch.float32).to(dtype).cuda()
+    pos = torch.arange(9, dtype=torch.int32, device="cuda")
+    w = torch.tensor(1 + 0.3 * rng.standard_normal(64), dtype=torch.float32, device="cuda")
+    out = torch.empty_like(x)
+    status = torch.zeros(9, dtype=torch.int32, device="cuda")
+    rt.QkNormRope(x.data_ptr(), None, out.data_ptr(), None, 9, 5, 0, 64, pos.data_ptr(), rt.ROWS_BF16 if bf16 else rt.ROWS_F32,
+                  q_weight_ptr=w.data_ptr(), epsilon=eps)(status.data_ptr())
+    torch.cuda.synchronize()
+    assert not status.any()
+    eps = float(np.float32(eps))
+    want = formula(x.double().cpu().numpy(), w.double().cpu().numpy(), np.arange(9), 64, False, eps, 10000.0)
+    lim = bound(x.double().cpu().numpy(), w.double().cpu().numpy(), 64, eps, want, bf16)
+    assert (np.abs(out.double().cpu().numpy() - want) <= lim).all()
+
+
+def test_outputs_that_overflow_bf16_are_flagged(cuda_ok):
+    """Finite in 32 bits, infinite once rounded: values from 3.3953e38 on."""
+    x = torch.ones(3, 1, 64, dtype=torch.bfloat16, device="cuda")
+    pos = torch.zeros(3, dtype=torch.int32, device="cuda")
+    out = torch.empty_like(x)
+    for weight, flagged in ((3.4e38, True), (3.38e38, False)):
+        w = torch.full((64,), weight, device="cuda")
+        status = torch.zeros(3, dtype=torch.int32, device="cuda")
+        rt.QkNormRope(x.data_ptr(), None, out.data_ptr(), None, 3, 1, 0, 64, pos.data_ptr(), rt.ROWS_BF16, q_weight_ptr=w.data_ptr(),
+                      epsilon=0.0)(status.data_ptr())
+        torch.cuda.synchronize()
+        assert torch.isinf(out).all().item() == flagged and status.tolist() == [rt.NON_FINITE if flagged else 0] * 3
