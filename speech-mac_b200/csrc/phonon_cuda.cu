@@ -1125,7 +1125,9 @@ int upload_batch(PhononCuda* c, const std::vector<int32_t>& slot, const std::vec
     std::vector<long long>& cuts = lane->h_cuts;
     cuts.clear();
     cuts.push_back(0);
-    if (!guided) {
+    if (kv_is_q8(c)) {
+        // 8-bit attention splits by itself and reads the page tables: no plan
+    } else if (!guided) {
         const long long per_stream = std::max<long long>(
             1, std::llround(std::sqrt(2.0 * static_cast<double>(total_pages) / static_cast<double>(R))));
         const long long min_chunk =
@@ -1170,6 +1172,8 @@ int upload_batch(PhononCuda* c, const std::vector<int32_t>& slot, const std::vec
         int e = 0, pb = 0;   // cursor: page pb of entry e
         std::vector<int32_t>& first_split = lane->h_first_split;
         first_split.resize(static_cast<size_t>(G) + 1);
+        for (int k = 0; k < R && kv_is_q8(c); ++k)
+            if (static_cast<int>(c->streams[slot[k]].pages.size()) <= pos[k] / kPage) return PHONON_CUDA_INVALID_ARGUMENT;
         for (int k = 0; k < C; ++k) {
             first_split[k] = S;
             long long left = cuts[k + 1] - (done + pb);  // pages of chunk k

@@ -257,3 +257,24 @@ def test_prefills_and_steps_of_the_same_rows_take_turns(cuda_ok, weights12, n):
         ctx.close()
     for a, b in zip(*outs):
         np.testing.assert_array_equal(a, b)
+
+
+def test_a_long_prefill_needs_no_more_pages_than_its_own(cuda_ok, oracle, weights12):
+    """7000 positions in a pool of exactly their pages, in passes of 256 rows, then a step that takes none."""
+    length = 7000
+    weights = weights12[:2]
+    ctx = context(weights, 1, length // 16 + 1)
+    s = ctx.stream_alloc(length + 1)
+    rows = synth.Generator(17).normal((length + 1) * 512).reshape(length + 1, 512)
+    om = oracle.model(weights)
+    for at in (length - 1, length):
+        out = ctx.append(s, rows[:length]) if at < length else ctx.step([s], [at], rows[at][None])[0]
+        cache = om.new_stream(at + 1)
+        om.load_kv(cache, *ctx.kv_read(s, 0, at + 1))
+        x = rows[at]
+        for layer in range(2):
+            ok, x, _, _ = om.layer_step_forced(cache, layer, at, x)
+            assert ok
+        om.free_stream(cache)
+        assert rt.rel_err(out, x) < FINAL_TOL
+    ctx.close()
