@@ -76,9 +76,9 @@ struct Kv8Seq {
 // the launch's bound count as empty.
 __device__ __forceinline__ Kv8Seq kv8_seq(const Kv8Seqs& s, int i) {
     Kv8Seq q;
-    const int b = s.row_begin ? __ldg(s.row_begin + i) : i * s.rows_per_seq;
-    const int e = s.row_begin ? __ldg(s.row_begin + i + 1) : b + s.rows_per_seq;
-    q.length = __ldg(s.lengths + i) + s.length_bias;
+    const int b = s.row_begin ? s.row_begin[i] : i * s.rows_per_seq;
+    const int e = s.row_begin ? s.row_begin[i + 1] : b + s.rows_per_seq;
+    q.length = s.lengths[i] + s.length_bias;
     q.row0 = b;
     q.count = e - b;
     if (b < 0 || e < b || e > s.rows || e - b > s.max_rows) {
@@ -89,7 +89,7 @@ __device__ __forceinline__ Kv8Seq kv8_seq(const Kv8Seqs& s, int i) {
         kv8_flag(s, i, kStatusCapacity);
         q.length = 0;
     }
-    q.pages = s.pages + static_cast<long long>(s.slots ? __ldg(s.slots + i) : i) * s.page_stride;
+    q.pages = s.pages + static_cast<long long>(s.slots ? s.slots[i] : i) * s.page_stride;
     return q;
 }
 
@@ -131,14 +131,17 @@ __device__ __forceinline__ uint32_t kv8_shrink(uint32_t w, float shrink) {
     return kv8_pack(r[0], r[1], r[2], r[3]);
 }
 
+// (Plain loads here and below, of all that a caller passes: these kernels start
+// before the launch ahead of them has ended, which may still be writing it, and
+// the read-only path takes its data for constant from a grid's start on.)
 template <bool kBf16>
 __device__ __forceinline__ float4 load_row4(const void* base, size_t at) {
     if constexpr (kBf16) {
-        const uint2 w = __ldg(reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(base) + at));
+        const uint2 w = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(base) + at);
         return make_float4(__uint_as_float(w.x << 16), __uint_as_float(w.x & 0xffff0000u), __uint_as_float(w.y << 16),
                            __uint_as_float(w.y & 0xffff0000u));
     } else {
-        return __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(base) + at));
+        return *reinterpret_cast<const float4*>(static_cast<const float*>(base) + at);
     }
 }
 
@@ -219,7 +222,7 @@ __global__ void __launch_bounds__(128) kv8_append_kernel(Kv8AppendParams p) {
     const int block = start / kKv8Block + bi;
     const int p0 = block * kKv8Block;
     if (p0 >= q.length || q.count == 0) return;
-    const int page = __ldg(q.pages + block);
+    const int page = q.pages[block];
     const int lo = max(start - p0, 0), hi = min(q.length - p0, kKv8Block);  // new slots [lo, hi), kept [0, lo)
     const void* src = p.rows[which];
     const int g = lane >> 2, t = lane & 3;
@@ -324,7 +327,7 @@ __global__ void __launch_bounds__(128) kv8_append_one_kernel(Kv8AppendParams p) 
     int page = -1;
     float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     if (real) {
-        page = __ldg(q.pages + position / kKv8Block);
+        page = q.pages[position / kKv8Block];
         x = load_row4<kBf16>(p.rows[which], static_cast<size_t>(q.row0) * p.stride + head * D + 4 * l);
         if (static_cast<unsigned>(page) >= static_cast<unsigned>(p.cache.pool_pages)) {
             if (l == 0) kv8_flag(p.seqs, i, kStatusInvalid);
@@ -452,7 +455,7 @@ __global__ void __launch_bounds__(128) kv8_read_kernel(Kv8ReadParams p) {
     const int p0 = block * kKv8Block;
     if (p0 >= q.length || q.count == 0) return;
     const int row0 = q.row0 - start;
-    int page = block >= 0 ? __ldg(q.pages + block) : -1;
+    int page = block >= 0 ? q.pages[block] : -1;
     if (block >= 0 && static_cast<unsigned>(page) >= static_cast<unsigned>(p.cache.pool_pages)) {
         if (lane == 0) kv8_flag(p.seqs, i, kStatusInvalid);
         page = -1;
@@ -471,7 +474,7 @@ __global__ void __launch_bounds__(128) kv8_read_kernel(Kv8ReadParams p) {
         for (int a = 0; a < kPasses; ++a) {
             const int slot = a * kRowsPerPass + lane / kLanesPerRow;
             w[a] = src && slot >= lo && slot < hi
-                       ? __ldg(reinterpret_cast<const uint32_t*>(src + slot * D) + lane % kLanesPerRow)
+                       ? *(reinterpret_cast<const uint32_t*>(src + slot * D) + lane % kLanesPerRow)
                        : 0x80808080u;
         }
 #pragma unroll
@@ -485,7 +488,7 @@ __global__ void __launch_bounds__(128) kv8_read_kernel(Kv8ReadParams p) {
         uint4 w[kChunks];
 #pragma unroll
         for (int j = 0; j < kChunks; ++j)
-            w[j] = src ? __ldg(reinterpret_cast<const uint4*>(src + j * 512) + lane)
+            w[j] = src ? *(reinterpret_cast<const uint4*>(src + j * 512) + lane)
                        : make_uint4(0x80808080u, 0x80808080u, 0x80808080u, 0x80808080u);
 #pragma unroll
         for (int j = 0; j < kChunks; ++j)
@@ -895,13 +898,13 @@ __global__ void __launch_bounds__(32 * kWarps, kCtas) kv8_attention_kernel(Kv8At
     int ids[2], scales[2];
     auto fetch = [&](int half, int turn) {
         const int at = own + turn * kStep;
-        ids[half] = at < last ? __ldg(sq.pages + at) : -1;
+        ids[half] = at < last ? sq.pages[at] : -1;
         if (at < last && static_cast<unsigned>(ids[half]) >= static_cast<unsigned>(p.cache.pool_pages)) {
             kv8_flag(p.seqs, i, kStatusInvalid);
             ids[half] = -1;  // its positions are not seen
         }
         scales[half] = ids[half] >= 0
-                           ? __ldg(reinterpret_cast<const unsigned short*>(exps + static_cast<size_t>(ids[half]) * p.cache.heads * 2))
+                           ? *reinterpret_cast<const unsigned short*>(exps + static_cast<size_t>(ids[half]) * p.cache.heads * 2)
                            : 127 | 127 << 8;
     };
     const uint8_t* base = p.cache.pool + static_cast<size_t>(head) * kPageBytes;

@@ -265,9 +265,9 @@ __global__ void __launch_bounds__(kKv8PromptThreads, 1) kv8_prompt_kernel(Kv8Att
         load_q(0, ahead[0]);
         const uint8_t* exps = p.cache.exps + head * 2;
         auto scales_of = [&](int at, bool in) {  // -1: no page
-            const int id = in ? __ldg(sq.pages + at) : -1;
+            const int id = in ? sq.pages[at] : -1;
             return static_cast<unsigned>(id) < static_cast<unsigned>(p.cache.pool_pages)
-                       ? static_cast<int>(__ldg(reinterpret_cast<const unsigned short*>(exps + static_cast<size_t>(id) * p.cache.heads * 2)))
+                       ? static_cast<int>(*reinterpret_cast<const unsigned short*>(exps + static_cast<size_t>(id) * p.cache.heads * 2))
                        : -1;
         };
         {  // the split's value scales
@@ -621,7 +621,7 @@ __global__ void __launch_bounds__(kKv8PromptThreads, 1) kv8_prompt_kernel(Kv8Att
                         const uint8_t* pool = p.cache.pool + static_cast<size_t>(head) * 2 * kKv8Block * D;
                         auto fetch_ids = [&](int n) {  // page ids of this warp's units n + lane
                             const int unit = converter + (n + lane) * kKv8Converters, at = first + unit / (2 * kPages) * kPages + unit % kPages;
-                            int id = at < last ? __ldg(sq.pages + at) : -1;
+                            int id = at < last ? sq.pages[at] : -1;
                             if (at < last && static_cast<unsigned>(id) >= static_cast<unsigned>(p.cache.pool_pages)) {
                                 kv8_flag(p.seqs, i, kStatusInvalid);
                                 id = -1;  // its positions are not seen
@@ -639,7 +639,7 @@ __global__ void __launch_bounds__(kKv8PromptThreads, 1) kv8_prompt_kernel(Kv8Att
                             for (int k = 0; k < kPieces; ++k) {
                                 const int row = D == 32 ? key_row : (k & 1) * 8 + key_row, piece = D == 32 ? key_piece : (k >> 1) * 4 + key_piece;
                                 const int off = values ? kKv8Block * D + k * 512 + (vg * 4 + vt) * 16 : row * D + piece * 16;
-                                w[k] = id >= 0 ? __ldg(reinterpret_cast<const uint4*>(src + off)) : make_uint4(0, 0, 0, 0);
+                                w[k] = id >= 0 ? *reinterpret_cast<const uint4*>(src + off) : make_uint4(0, 0, 0, 0);
                             }
                         };
             uint4 a[kPieces], b[kPieces];  // this unit's bytes and the next's

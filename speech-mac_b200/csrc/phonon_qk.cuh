@@ -66,7 +66,7 @@ __global__ void __launch_bounds__(128, kCtas) qk_norm_rope_kernel(QkParams p) {
     for (int s = 0; s < 2; ++s)
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-            const float4 v = p.weight[s] ? __ldg(reinterpret_cast<const float4*>(p.weight[s] + chunk[c])) : make_float4(1.0f, 1.0f, 1.0f, 1.0f);
+            const float4 v = p.weight[s] ? *reinterpret_cast<const float4*>(p.weight[s] + chunk[c]) : make_float4(1.0f, 1.0f, 1.0f, 1.0f);
             w[s][4 * c] = v.x, w[s][4 * c + 1] = v.y, w[s][4 * c + 2] = v.z, w[s][4 * c + 3] = v.w;
         }
     // passes of the queries, then of the keys: a pass has one side
@@ -89,18 +89,18 @@ __global__ void __launch_bounds__(128, kCtas) qk_norm_rope_kernel(QkParams p) {
             for (int c = 0; c < 2; ++c) {
                 raw[a][c] = Raw{};
                 if (u + a < stop && h0 + a * kPerWarp < heads)
-                    raw[a][c] = __ldg(reinterpret_cast<const Raw*>(in + a * (kPerWarp * D * kSize) + chunk[c] * kSize));
+                    raw[a][c] = *reinterpret_cast<const Raw*>(in + a * (kPerWarp * D * kSize) + chunk[c] * kSize);
             }
     };
     auto end_of = [&](int u, int stop) { return min(min(u + kAhead, stop), u < pass_q ? pass_q : passes); };
     int row = item / p.slices, first = (item - row * p.slices) * per;
-    int position = __ldg(p.positions + row);
+    int position = p.positions[row];
     if (first < passes) load(row, first, min(passes, first + per));
     while (true) {
         const int stop = min(passes, first + per);
         const int next = item + stride, next_row = next < items ? next / p.slices : row;
         const int next_first = (next - next_row * p.slices) * per;
-        const int next_position = __ldg(p.positions + next_row);
+        const int next_position = p.positions[next_row];
         float sn[8], cs[8];  // of every dim, with the sign of its own term: a cos - b sin, a sin + b cos
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
