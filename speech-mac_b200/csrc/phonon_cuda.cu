@@ -4687,7 +4687,7 @@ template <int D, bool kBf16>
 int qk_launch(QkParams& p, bool halves, int sms, cudaStream_t s) {
     // As many warps as are resident at once; a row each in turn, or a slice of
     // its heads while rows are fewer.
-    constexpr int kAhead = kBf16 ? 4 : 2, kCtas = kBf16 ? 4 : 5, kHeads = 256 / D;
+    constexpr int kAhead = kBf16 ? 4 : 2, kCtas = 4, kHeads = 256 / D;  // (fp32, five CTAs: registers spill, 60 us against 57.6)
     const int passes = (p.heads[0] + kHeads - 1) / kHeads + (p.heads[1] + kHeads - 1) / kHeads;
     const long long resident = 4ll * kCtas * sms;
     p.slices = static_cast<int>(std::max<long long>(1, std::min<long long>(passes, resident / p.rows)));
