@@ -11,6 +11,7 @@
 #include "phonon_kv8.cuh"
 #include "phonon_kv8_prompt.cuh"
 #include "phonon_qk.cuh"
+#include "phonon_status.h"
 
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -2613,7 +2614,7 @@ int phonon_cuda_append(PhononCuda* c, uint32_t stream, const float* rows, uint32
     std::vector<int> later_polls(c->cfg.n_layers, 1);
     const int chunk = c->cap_rows;
     int result = PHONON_CUDA_OK;
-    bool cancelled = false, bad = false;
+    bool cancelled = false;
     for (uint32_t p0 = 0; p0 < length && result == PHONON_CUDA_OK; p0 += chunk) {
         const int R = static_cast<int>(std::min<uint32_t>(chunk, length - p0));
         std::vector<int32_t> slot(R, static_cast<int32_t>(stream)), pos(R);
@@ -2631,9 +2632,7 @@ int phonon_cuda_append(PhononCuda* c, uint32_t stream, const float* rows, uint32
                             c->stream);
         const int sync = finish_sync(c, R);
         if (result == PHONON_CUDA_OK && sync) result = sync;
-        for (int e = 0; e < R && result == PHONON_CUDA_OK; ++e)
-            if (c->h_status[e]) bad = true;
-        if (bad) result = PHONON_CUDA_NON_FINITE;
+        if (result == PHONON_CUDA_OK) result = phonon_rows_status(c->h_status, R);
     }
     if (result != PHONON_CUDA_OK) {
         release_pages(c, stream);
