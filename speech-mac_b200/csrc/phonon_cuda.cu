@@ -680,11 +680,13 @@ int kv8_launch_prompt(const Kv8Pool& c, uint32_t layer, const Kv8Seqs& seqs, con
     auto kernel = kv8_prompt_kernel<D, kBf16>;
     // Its warps hand registers to one another: what they ask for has to be what
     // the launch has, or they would wait for good.
-    static const int registers = [kernel] {
+    static std::atomic<bool> enough{false};  // kept once it is known: a query that fails fails its own call only
+    if (!enough) {
         cudaFuncAttributes f{};
-        return cudaFuncGetAttributes(&f, kernel) == cudaSuccess ? (f.numRegs + 7) / 8 * 8 : 0;
-    }();
-    if (registers * kKv8PromptThreads < kKv8PromptRegisters) return PHONON_CUDA_DEVICE_ERROR;
+        CUDA_TRY(cudaFuncGetAttributes(&f, kernel));
+        if ((f.numRegs + 7) / 8 * 8 * kKv8PromptThreads < kKv8PromptRegisters) return PHONON_CUDA_DEVICE_ERROR;
+        enough = true;
+    }
     static std::atomic<uint64_t> configured{0};
     CUDA_TRY(opt_in_smem(reinterpret_cast<const void*>(kernel), smem, configured));
     CUDA_TRY(launch_pdl(kernel, dim3(static_cast<unsigned>(items * p.splits)), dim3(kKv8PromptThreads), smem, s, p));
