@@ -557,7 +557,7 @@ int phonon_cuda_kv8_attention_device(PhononCudaKv8 *cache, uint32_t layer, const
  * q is [rows][heads][head_dim], k [rows][kv_heads][head_dim]; either may be
  * absent (0 heads). Outputs may be the inputs. Enqueued on `cuda_stream` of
  * `device`, like the cache's calls; status_dev (device, [rows], optional) is
- * set to PHONON_CUDA_NON_FINITE for a row with a non-finite output. */
+ * raised to PHONON_CUDA_NON_FINITE for a row with a non-finite output. */
 typedef struct {
     uint32_t type; /* PhononCudaRowType of q, k and the outputs */
     uint32_t rows, heads, kv_heads;

@@ -73,7 +73,7 @@ __device__ __forceinline__ float warp_sum(float v) {
 __device__ __forceinline__ float silu_f(float x) { return __fdiv_rn(x, __fadd_rn(1.0f, expf(-x))); }
 
 __device__ __forceinline__ void flag_nonfinite(int32_t* status, int b) {
-    if (status) atomicOr(status + b, kStatusNonFinite);
+    if (status) atomicMax(status + b, kStatusNonFinite);  // the largest code stays
 }
 
 // ------------------------------------------------------------------ LayerNorm

@@ -237,3 +237,14 @@ def test_outputs_that_overflow_bf16_are_flagged(cuda_ok):
                       epsilon=0.0)(status.data_ptr())
         torch.cuda.synchronize()
         assert torch.isinf(out).all().item() == flagged and status.tolist() == [rt.NON_FINITE if flagged else 0] * 3
+
+
+def test_a_larger_code_stays(cuda_ok):
+    """Status words that hold a larger code already (an expired wait, a bad length) keep it."""
+    x = torch.full((4, 1, 64), float("nan"), device="cuda")
+    x[3] = 1.0
+    pos = torch.zeros(4, dtype=torch.int32, device="cuda")
+    status = torch.tensor([rt.DEVICE_ERROR, 0, rt.CAPACITY, rt.INVALID], dtype=torch.int32, device="cuda")
+    rt.QkNormRope(x.data_ptr(), None, x.data_ptr(), None, 4, 1, 0, 64, pos.data_ptr())(status.data_ptr())
+    torch.cuda.synchronize()
+    assert status.tolist() == [rt.DEVICE_ERROR, rt.NON_FINITE, rt.CAPACITY, rt.INVALID]
