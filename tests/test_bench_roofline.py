@@ -86,3 +86,25 @@ def test_clock_sampler_without_nvml(tmp_path, monkeypatch):
     s = clocks.summary()
     assert s["samples"] == 0 and s["sm_mhz"] is None and s["source"].startswith("none")
     assert os.listdir(scratch) == []
+
+
+def missing(*_):
+    raise FileNotFoundError("part.so")
+
+
+def test_cpu_figures_that_were_measured_stay(monkeypatch):
+    parts = ("single_stream", "q8_matvec", "config2", "config4", "frame_loop", "mimi")
+    monkeypatch.setattr(bench, "cpu_baseline", lambda seconds: {"value": seconds})
+    monkeypatch.setattr(bench, "cpu_extras", missing)
+    line = {p: {} for p in parts}
+    bench.add_cpu_figures(line, 5, False)
+    assert line["cpu_baseline"] == {"value": 5} and line["cpu_extras"] == {"unavailable": "part.so"}
+    monkeypatch.setattr(bench, "cpu_baseline", missing)
+    monkeypatch.setattr(bench, "cpu_extras", lambda: {k: k for k in ("config0", "q8_matvec", "config2", "config4", "flow_head", "mimi")})
+    line = {p: {} for p in parts}
+    bench.add_cpu_figures(line, 5, False)
+    assert line["cpu_baseline"] == {"unavailable": "part.so"} and "cpu_extras" not in line
+    assert line["frame_loop"] == {"cpu_baseline_head": "flow_head"} and line["single_stream"] == {"cpu_baseline": "config0"}
+    line = {}
+    bench.add_cpu_figures(line, 5, True)
+    assert list(line) == ["cpu_baseline"]
