@@ -242,7 +242,7 @@ __global__ void __launch_bounds__(kKv8PromptThreads, 1) kv8_prompt_kernel(Kv8Att
         __syncwarp();
         return ok;
     };
-                asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const uint32_t tmem = s_tmem;  // S [stream][2], then the streams' outputs
@@ -615,33 +615,33 @@ __global__ void __launch_bounds__(kKv8PromptThreads, 1) kv8_prompt_kernel(Kv8Att
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kKv8OtherRegisters));
         if (warp < 15) {
             // Pages of keys (unit 8 * turn + page) and of values (unit 8 * turn + 4 + page), every seventh unit.
-                        const int units = turns * 2 * kPages, converter = warp - 8;
-                        const int count = units > converter ? (units - converter + kKv8Converters - 1) / kKv8Converters : 0;
-                        const size_t page_bytes = static_cast<size_t>(p.cache.heads) * 2 * kKv8Block * D;
-                        const uint8_t* pool = p.cache.pool + static_cast<size_t>(head) * 2 * kKv8Block * D;
-                        auto fetch_ids = [&](int n) {  // page ids of this warp's units n + lane
-                            const int unit = converter + (n + lane) * kKv8Converters, at = first + unit / (2 * kPages) * kPages + unit % kPages;
-                            int id = at < last ? sq.pages[at] : -1;
-                            if (at < last && static_cast<unsigned>(id) >= static_cast<unsigned>(p.cache.pool_pages)) {
-                                kv8_flag(p.seqs, i, kStatusInvalid);
-                                id = -1;  // its positions are not seen
-                            }
-                            return id;
-                        };
-                        // lane 8c + r: 16 dims of key r; lane 8t + g: the cache's piece 4g + t of values. Eight lanes fill a core matrix.
-                        const int key_row = D == 32 ? lane & 15 : lane & 7, key_piece = D == 32 ? lane >> 4 : lane >> 3;
-                        const int vg = lane & 7, vt = lane >> 3;
-                        auto load = [&](uint4 (&w)[kPieces], int n, int id) {
-                            const int unit = converter + n * kKv8Converters;
-                            const uint8_t* src = pool + max(id, 0) * page_bytes;
-                            const bool values = unit & kPages;
-            #pragma unroll
-                            for (int k = 0; k < kPieces; ++k) {
-                                const int row = D == 32 ? key_row : (k & 1) * 8 + key_row, piece = D == 32 ? key_piece : (k >> 1) * 4 + key_piece;
-                                const int off = values ? kKv8Block * D + k * 512 + (vg * 4 + vt) * 16 : row * D + piece * 16;
-                                w[k] = id >= 0 ? *reinterpret_cast<const uint4*>(src + off) : make_uint4(0, 0, 0, 0);
-                            }
-                        };
+            const int units = turns * 2 * kPages, converter = warp - 8;
+            const int count = units > converter ? (units - converter + kKv8Converters - 1) / kKv8Converters : 0;
+            const size_t page_bytes = static_cast<size_t>(p.cache.heads) * 2 * kKv8Block * D;
+            const uint8_t* pool = p.cache.pool + static_cast<size_t>(head) * 2 * kKv8Block * D;
+            auto fetch_ids = [&](int n) {  // page ids of this warp's units n + lane
+                const int unit = converter + (n + lane) * kKv8Converters, at = first + unit / (2 * kPages) * kPages + unit % kPages;
+                int id = at < last ? sq.pages[at] : -1;
+                if (at < last && static_cast<unsigned>(id) >= static_cast<unsigned>(p.cache.pool_pages)) {
+                    kv8_flag(p.seqs, i, kStatusInvalid);
+                    id = -1;  // its positions are not seen
+                }
+                return id;
+            };
+            // lane 8c + r: 16 dims of key r; lane 8t + g: the cache's piece 4g + t of values. Eight lanes fill a core matrix.
+            const int key_row = D == 32 ? lane & 15 : lane & 7, key_piece = D == 32 ? lane >> 4 : lane >> 3;
+            const int vg = lane & 7, vt = lane >> 3;
+            auto load = [&](uint4 (&w)[kPieces], int n, int id) {
+                const int unit = converter + n * kKv8Converters;
+                const uint8_t* src = pool + max(id, 0) * page_bytes;
+                const bool values = unit & kPages;
+#pragma unroll
+                for (int k = 0; k < kPieces; ++k) {
+                    const int row = D == 32 ? key_row : (k & 1) * 8 + key_row, piece = D == 32 ? key_piece : (k >> 1) * 4 + key_piece;
+                    const int off = values ? kKv8Block * D + k * 512 + (vg * 4 + vt) * 16 : row * D + piece * 16;
+                    w[k] = id >= 0 ? *reinterpret_cast<const uint4*>(src + off) : make_uint4(0, 0, 0, 0);
+                }
+            };
             uint4 a[kPieces], b[kPieces];  // this unit's bytes and the next's
             int ids = fetch_ids(0);
             load(a, 0, __shfl_sync(kFull, ids, 0));
