@@ -49,7 +49,7 @@ def test_quiet_channels_beside_a_loud_one(cuda_ok, kv_heads, group, dim, lengths
         assert (np.abs(f64(out[part]) - want) <= bound).all()
 
 
-def sums(q, keys, values, window, exps, bf16):
+def sums(q, keys, values, window, exps, bf16, reference=None):
     """The 64-bit output of rows at the last positions, and per element how far a kernel that keeps its documented
     precision may be: by the terms that the element is a sum of, and not by the largest value of the sequence.
 
@@ -74,7 +74,7 @@ def sums(q, keys, values, window, exps, bf16):
             total = p.sum()
             out[r, h] = (p @ v) / total
             each = off[:, None] + (2.0 ** -12 if bf16 else 0.0)
-            step = len(s) * 2.0 ** -33 * 127 * 2.0 ** max(exps[:, g].min() + 8, exps[:, g].max() - 64)
+            step = len(s) * 2.0 ** -33 * 127 * 2.0 ** (max(exps[:, g].min() + 8, exps[:, g].max() - 64) if reference is None else reference)
             bound[r, h] = ((p[:, None] * each * np.abs(v)).sum(0) + np.abs(out[r, h]) * (p @ off) + step) / total
             bound[r, h] *= 1 + off.max()
     return out, bound + (2.0 ** -8 if bf16 else u) * np.abs(out) + 1e-30
@@ -163,3 +163,62 @@ def test_value_scales_that_rise_and_fall(cuda_ok, kv_heads, group, dim, lengths,
         part = slice(i * count, (i + 1) * count)
         want, bound = sums(f64(q[part]), held[0].values(), held[1].values(), 0, held[1].exps, dtype == torch.bfloat16)
         assert (np.abs(f64(out[part]) - want) <= bound).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("count", [1, 9])
+def test_references_that_move_within_a_warp(cuda_ok, count, dtype):
+    """Sequences too long for one window of a warp's page ids, items enough that they are hardly split: the scales' range
+    grows upwards in the first, downwards in the second.
+
+    Splits and windows that hold loud blocks only have those for their reference, so that the step of a weight is 2^-33 of
+    the loudest scale here: next to a position with weight 1 whose integer is 0 in some dim, one of weight 2^-24 keeps 9
+    of its bits there (the whole output is 2^24 times what it adds)."""
+    kv_heads, dim, lengths = 64, 32, [8000, 8000] + [100] * 8
+    rng = np.random.default_rng(40 + count)
+    c = Cache(kv_heads, dim, lengths)
+    keys = [rows(rng, n, kv_heads, dim, dtype) for n in lengths]
+    values = [rows(rng, n, kv_heads, dim, dtype) for n in lengths]
+    at = np.arange(8000)
+    for i, steps in enumerate((np.select([at < 3000, at < 4500], [0, 20], 40), np.select([at < 3000, at < 5000], [30, 27], 0))):
+        values[i] = (values[i].float() * dev(2.0 ** steps[:, None, None].astype(np.float64), torch.float32)).to(dtype)
+    c.append(lengths, keys, values)
+    q = rows(rng, count * len(lengths), kv_heads, dim, dtype)
+    out = torch.empty_like(q)
+    ws = rt.Kv8Workspace(c.kv)
+    c.kv.attention(c.batch(lengths, [count] * len(lengths)),
+                   rt.kv8_query(q.data_ptr(), out.data_ptr(), kind(dtype), heads=kv_heads), ws)
+    torch.cuda.synchronize()
+    some = [0, 31, 63]
+    for i, n in enumerate(lengths[:2]):
+        held = [model.Held(len(some), dim) for _ in range(2)]
+        held[0].append(f64(keys[i])[:, some])
+        held[1].append(f64(values[i])[:, some])
+        part = slice(i * count, (i + 1) * count)
+        want, bound = sums(f64(q[part])[:, some], held[0].values(), held[1].values(), 0, held[1].exps, dtype == torch.bfloat16,
+                           held[1].exps.max())
+        assert (np.abs(f64(out[part])[:, some] - want) <= bound).all(), i
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("dim", [32, 64, 128])
+def test_loud_positions_in_splits_of_many_rows(cuda_ok, dim, dtype):
+    """One chunk of 480 rows over 6000 positions: its splits see different scales and meet in the merge."""
+    kv_heads, n, count = 4, 6000, 480
+    rng = np.random.default_rng(dim)
+    c = Cache(kv_heads, dim, [n])
+    keys, values = rows(rng, n, kv_heads, dim, dtype), rows(rng, n, kv_heads, dim, dtype)
+    values[::701] *= 2.0 ** 25
+    values[3200:4000] *= 2.0 ** -18
+    c.append([n], [keys], [values])
+    q = rows(rng, count, kv_heads, dim, dtype)
+    out = torch.empty_like(q)
+    ws = rt.Kv8Workspace(c.kv)
+    c.kv.attention(c.batch([n], [count]), rt.kv8_query(q.data_ptr(), out.data_ptr(), kind(dtype), heads=kv_heads), ws)
+    torch.cuda.synchronize()
+    held = [model.Held(kv_heads, dim) for _ in range(2)]
+    held[0].append(f64(keys))
+    held[1].append(f64(values))
+    last = 30
+    want, bound = sums(f64(q[-last:]), held[0].values(), held[1].values(), 0, held[1].exps, dtype == torch.bfloat16)
+    assert (np.abs(f64(out[-last:]) - want) <= bound).all()
