@@ -468,10 +468,12 @@ int phonon_cuda_mimi_process(PhononCudaMimi *mimi, uint32_t state, const float *
  *   - page id lies outside the pool (INVALID_ARGUMENT): that page is not
  *     written, reads as zeros, and no query sees it;
  *   - rows hold a non-finite value (NON_FINITE): append holds such an element
- *     as 0, and a query row with one gets NaN;
+ *     as 0, and a query row with one gets NaN (0 where it sees nothing);
  *   - attention gave up a bounded wait inside its kernel (DEVICE_ERROR, about
  *     two seconds): rows of it are NaN.
- * The largest code stays. A page that a call appends to belongs to one
+ * The largest code stays. The call itself returns CAPACITY where sequences,
+ * bounds and heads make more than 2^31 blocks of work (bounds far too loose).
+ * A page that a call appends to belongs to one
  * sequence of the batch; pages that are only read may be shared. Calls on one
  * cache may run at the same time as long as none writes a page that another
  * uses. */
@@ -532,7 +534,7 @@ void phonon_cuda_kv8_workspace_destroy(PhononCudaKv8Workspace *workspace);
  * window is 0. q and out are [rows][heads][head_dim], heads a multiple of
  * kv_heads (query head h reads K/V head h / (heads / kv_heads)); out may be q
  * with q's stride.
- * A row that sees nothing gets 0. */
+ * A row that sees nothing gets 0; one whose scores leave fp32's range NaN. */
 typedef struct {
     uint32_t type;   /* PhononCudaRowType of q and out */
     uint32_t heads;

@@ -702,9 +702,9 @@ int kv8_launch_prompt(const Kv8Pool& c, uint32_t layer, const Kv8Seqs& seqs, con
 // 1024, 32 heads (1.7) 21.4 and 19.4; 128 x 4096, 8 (1.7) 27.1 and 19.9; 256 x
 // 1024, 32 (3.5) 21.6 and 27.8; 1 to 256 rows of 300 to 2048 positions, 32 (4.1
 // by the longest) 26.8 and 27.3; 128 x 1024, 128 (6.9) 22.7 and 45.3; 1024 x
-// 4096, 32 (55) 136 and 265; 1 to 64 rows of 16 to 700 positions, 512 heads, 52
+// 4096, 32 (55) 134 and 265; 1 to 64 rows of 16 to 700 positions, 512 heads, 52
 // and 34. bf16, 128 dims: 128 x 1024, 32 (1.7) 28.4 and 25.9; 256 x 1024, 32
-// (3.5) 28.7 and 39.7; 1024 x 4096, 32 144 and 353.
+// (3.5) 28.7 and 39.7; 1024 x 4096, 32 148 and 353.
 template <int D>
 int kv8_attention_rows(const Kv8Pool& c, uint32_t layer, const Kv8Seqs& seqs, const Kv8Attend& a, const Kv8Scratch& w,
                        int sms, cudaStream_t s) {

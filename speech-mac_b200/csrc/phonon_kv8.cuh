@@ -419,7 +419,7 @@ __global__ void kv8_fill_kernel(uint8_t* pool, uint8_t* exps, int pool_pages, co
 
 // --------------------------------------------------------------------- read
 // (held integer) * 2^e. Bound by the bytes: 110 sequences of up to 2048
-// positions, 8 heads of 128, to bf16: 69 us, 6.0 TB/s, 93 % of the copy rate
+// positions, 8 heads of 128, to bf16: 69.5 us, 6.0 TB/s, 92 % of the copy rate
 // (124 with the bytes of a block taken one at a time); one sequence of 8000, 8 x
 // 64, to fp32, 41 MB: 10.2 us, of which 4 are launch and latency.
 struct Kv8ReadParams {
@@ -837,12 +837,12 @@ __device__ __forceinline__ int kv8_key_dim(int t, int c) {
 // ids and scales are fetched a lane each, 32 / PB turns at a time.
 //
 // Decode steps are bound by the cache's bytes: 512 sequences of up to 2048
-// positions, 8 x 64, 526 MB, 87 us (6.1 TB/s, 94 % of the copy rate); as halves
+// positions, 8 x 64, 526 MB, 87.7 us (6.0 TB/s, 93 % of the copy rate); as halves
 // with register loads 137, with the ring 101, as bytes 95. 48 of up to 4096, 32
-// heads on 8 x 128, 225 MB, 47.5 us: a CTA's start and end (4 us) against 30 us of
+// heads on 8 x 128, 225 MB, 49 us: a CTA's start and end (4 us) against 30 us of
 // pages, three CTAs an SM. 8 of 8000: 18 us, 5.7 of them the chain of loads
-// before the first page and 3 the merge. One of 800: 6.3 us, all latency. 64 x
-// 16 rows over 250 keys 13.8 us, 4 chunks of up to 256 rows 27.3 us: bound by
+// before the first page and 3 the merge. One of 1000: 6.5 us, all latency. 64 x
+// 16 rows over 250 keys 14.0 us, 4 chunks of up to 256 rows 27.3 us: bound by
 // the halves' matrix rate (2.1 clocks an m16n8k16 on an SM, two of them in
 // fp32) and, in bf16 with 128 dims, by the conversion of the bytes.
 // A persistent form that cut the positions of all items into equal lines for

@@ -34,9 +34,9 @@
 // weights keep 11). Blocks whose value scale is far from the split's smallest
 // are hidden from the turns and added in fp32, a row a thread, at the end.
 //
-// 1024 rows a K/V head over 4096 positions, 32 heads: bf16, 128 dims 144 us
-// (475 TFLOP/s), fp32, 64 dims 136 us (253, twice that in products); the
-// mma.sync kernel 353 and 265. Bound by the softmax's instructions: of 3000
+// 1024 rows a K/V head over 4096 positions, 32 heads: bf16, 128 dims 148 us
+// (408 TFLOP/s of what rows see), fp32, 64 dims 134 us (225, twice that in
+// products); the mma.sync kernel 353 and 265. Bound by the softmax's instructions: of 3000
 // clocks a turn of 64 dims, 400 go to the maximum, 1300 to the weights (two
 // warps share a scheduler's exponentials, 16 clocks an element of both), 250 to
 // O, 250 to the wait for P V, 300 to barriers and loads; a start of 7500 clocks

@@ -18,8 +18,8 @@
 // 2^-33 turns up to position 2^22, 2^-24 at the last position of 31 bits; its
 // upper 32 bits, signed, go to fp32 (2^-25 turns) and sincospif.
 //
-// Measured on B200 (34 us a pass, 4.9 TB/s, 77 % of the copy rate, for 8192
-// rows of 32 + 8 heads of 128 in bf16; 59 us, 5.7 TB/s in fp32): bf16 rows are
+// Measured on B200 (34 us a pass, 4.9 TB/s, 76 % of the copy rate, for 8192
+// rows of 32 + 8 heads of 128 in bf16; 57.6 us, 5.8 TB/s in fp32): bf16 rows are
 // bound by instructions (about 100 a pass of two heads), fp32 rows by the
 // DRAM. Dims of a pair in different lanes (a shuffle each, twice the sines)
 // took 43 us, one CTA a row with its sines in shared memory 94 us (their 64-bit
