@@ -557,7 +557,7 @@ int phonon_cuda_kv8_attention_device(PhononCudaKv8 *cache, uint32_t layer, const
  * with `halves`. Angles are reduced in 64 bits, so far positions keep 32-bit
  * sines (the one-row primitive keeps the reference's 32-bit phases instead).
  * q is [rows][heads][head_dim], k [rows][kv_heads][head_dim]; either may be
- * absent (0 heads). Outputs may be the inputs. Enqueued on `cuda_stream` of
+ * absent (0 heads). Outputs may be the inputs, with their strides. Enqueued on `cuda_stream` of
  * `device`, like the cache's calls; status_dev (device, [rows], optional) is
  * raised to PHONON_CUDA_NON_FINITE for a row with a non-finite output. */
 typedef struct {

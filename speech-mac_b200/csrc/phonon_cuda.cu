@@ -4545,6 +4545,11 @@ bool kv8_stride(uint64_t stride, uint64_t width, long long* out) {
     return true;
 }
 
+// Outputs in place of inputs that lie otherwise: a row would be written over one that is still to be read.
+bool rows_collide(const void* in, long long in_stride, const void* out, long long out_stride, long long rows) {
+    return in == out && in_stride != out_stride && rows > 1;
+}
+
 bool kv8_seqs(const PhononCudaKv8Batch* b, int32_t* status, Kv8Seqs* out) {
     if (!b || !b->lengths || !b->pages || b->sequences == 0 || b->sequences > (1u << 24) || b->rows > (1u << 30) ||
         b->max_rows == 0 || b->max_rows > (1u << 30) || b->page_stride == 0 || b->page_stride > (1u << 26) ||
@@ -4663,7 +4668,8 @@ int phonon_cuda_kv8_attention_device(PhononCudaKv8* c, uint32_t layer, const Pho
         return PHONON_CUDA_INVALID_ARGUMENT;
     Kv8Attend a{};
     const uint64_t width = static_cast<uint64_t>(query->heads) * c->pool.dim;
-    if (!kv8_stride(query->q_stride, width, &a.q_stride) || !kv8_stride(query->out_stride, width, &a.out_stride))
+    if (!kv8_stride(query->q_stride, width, &a.q_stride) || !kv8_stride(query->out_stride, width, &a.out_stride) ||
+        rows_collide(query->q, a.q_stride, query->out, a.out_stride, seqs.rows))
         return PHONON_CUDA_INVALID_ARGUMENT;
     if (seqs.rows == 0) return PHONON_CUDA_OK;
     a.q = query->q;
@@ -4721,7 +4727,8 @@ int phonon_cuda_qk_norm_rope_device(int device, const PhononCudaQkNormRope* a, i
         if (heads[s] == 0) continue;
         const uint64_t width = static_cast<uint64_t>(heads[s]) * a->head_dim;
         if (!in[s] || !out[s] || !aligned16(in[s]) || !aligned16(out[s]) ||
-            !kv8_stride(in_stride[s], width, &p.in_stride[s]) || !kv8_stride(out_stride[s], width, &p.out_stride[s]))
+            !kv8_stride(in_stride[s], width, &p.in_stride[s]) || !kv8_stride(out_stride[s], width, &p.out_stride[s]) ||
+            rows_collide(in[s], p.in_stride[s], out[s], p.out_stride[s], a->rows))
             return PHONON_CUDA_INVALID_ARGUMENT;
         p.in[s] = in[s];
         p.out[s] = out[s];

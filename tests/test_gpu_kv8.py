@@ -716,3 +716,14 @@ def test_many_rows_padded_and_on_two_streams_at_once(cuda_ok, dtype):
     # each. fp32: 24 turns of 64 positions, a sum of 16 truncated steps a turn, 2^-23 each: 2 * 40 * 2^-23.
     close = 2.0 ** -7 if dtype == torch.bfloat16 else 1e-5
     assert (outs[0] - outs[1]).float().norm() <= close * outs[0].float().norm()
+
+
+def test_attention_in_place_with_another_stride_is_refused(cuda_ok):
+    c = Cache(1, 64, [4, 4])
+    q = torch.zeros(4, 1, 64, device="cuda")
+    ws = rt.Kv8Workspace(c.kv)
+    with pytest.raises(rt.CudaError) as e:
+        c.kv.attention(c.batch([4, 4], [1, 1]), rt.kv8_query(q.data_ptr(), q.data_ptr(), heads=1, q_stride=128), ws)
+    assert e.value.status == rt.INVALID
+    c.kv.attention(c.batch([4, 4], [1, 1]), rt.kv8_query(q.data_ptr(), q.data_ptr(), heads=1, q_stride=128, out_stride=128), ws)
+    torch.cuda.synchronize()

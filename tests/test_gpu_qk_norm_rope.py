@@ -248,3 +248,17 @@ def test_a_larger_code_stays(cuda_ok):
     rt.QkNormRope(x.data_ptr(), None, x.data_ptr(), None, 4, 1, 0, 64, pos.data_ptr())(status.data_ptr())
     torch.cuda.synchronize()
     assert status.tolist() == [rt.DEVICE_ERROR, rt.NON_FINITE, rt.CAPACITY, rt.INVALID]
+
+
+def test_in_place_with_another_stride_is_refused(cuda_ok):
+    x = torch.zeros(4, 2, 64, device="cuda")
+    pos = torch.zeros(4, dtype=torch.int32, device="cuda")
+    for rows, refused in ((4, True), (1, False)):
+        call = rt.QkNormRope(x.data_ptr(), None, x.data_ptr(), None, rows, 1, 0, 64, pos.data_ptr(), q_stride=128)
+        if refused:
+            with pytest.raises(rt.CudaError) as e:
+                call()
+            assert e.value.status == rt.INVALID
+        else:
+            call()
+    torch.cuda.synchronize()
