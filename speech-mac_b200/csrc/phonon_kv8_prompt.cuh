@@ -176,7 +176,7 @@ __global__ void __launch_bounds__(kKv8PromptThreads, 1) kv8_prompt_kernel(Kv8Att
     constexpr int kPitch = D + 4;           // floats of a row's result: 8 rows' quads in different banks
     static_assert(2 * 128 * kPitch * 4 <= kv8_prompt_smem<D, kBf16>(), "the rows' results outgrow the operands' room");
     extern __shared__ __align__(128) uint8_t s_mem[];  // q [tile][plane], kStages x keys, x values; then the rows' results
-    __shared__ __align__(8) uint64_t s_bars[4 * kKv8PromptStages + 9];
+    __shared__ __align__(8) uint64_t s_bars[4 * kKv8PromptStages + 10];
     __shared__ uint32_t s_tmem;
     __shared__ int s_failed, s_last, s_lo, s_hi;
     __shared__ float s_f[128 * kTiles];
@@ -213,7 +213,7 @@ __global__ void __launch_bounds__(kKv8PromptThreads, 1) kv8_prompt_kernel(Kv8Att
     const uint32_t bars = smem_addr(s_bars);
     // by stage of keys and values (turn % kStages), score tile (stream, turn of the stream % 2), and stream
     const uint32_t k_full = bars, v_full = k_full + 8 * kStages, k_empty = v_full + 8 * kStages, v_empty = k_empty + 8 * kStages;
-    const uint32_t s_full = v_empty + 8 * kStages, p_full = s_full + 32, o_full = p_full + 16, q_full = o_full + 16;
+    const uint32_t s_full = v_empty + 8 * kStages, p_full = s_full + 32, o_full = p_full + 16, q_full = o_full + 16, drained = q_full + 8;
     if (threadIdx.x == 0) {
         for (int k = 0; k < kStages; ++k) {
             mbar_init(k_full + 8 * k, kPages);  // pages converted
@@ -227,6 +227,7 @@ __global__ void __launch_bounds__(kKv8PromptThreads, 1) kv8_prompt_kernel(Kv8Att
             mbar_init(o_full + 8 * k, 1);  // tcgen05.commit: the output is there, the weights are free
         }
         mbar_init(q_full, 8);
+        mbar_init(drained, 1);  // tcgen05.commit: every product that was issued is done
         s_failed = 0;
         s_lo = 255;
         s_hi = 0;
@@ -511,7 +512,11 @@ __global__ void __launch_bounds__(kKv8PromptThreads, 1) kv8_prompt_kernel(Kv8Att
         // split item, its maximum asks for. Two streams of one row add theirs.
         const auto both_sync = [] { asm volatile("bar.sync 1, 256;" ::: "memory"); };
         s_ml[stream][r] = make_float2(m, s_failed ? __int_as_float(0x7fc00000) : l);  // a wait that ran out: NaN
-        both_sync();  // and both streams' products are done: the operands' room takes the results
+        // The streams' products are done, and after a wait that ran out so are those that nobody waited for: the
+        // operands' room takes the results.
+        if (s_failed)
+            for (const long long since = clock64(); !mbar_test(drained, 0) && clock64() - since < kWaitBudgetCycles;) __nanosleep(20);
+        both_sync();
         float* s_o = reinterpret_cast<float*>(s_mem) + (stream * 128 + r) * kPitch;
         float most, sum, by;
         const auto factors = [&] {
@@ -764,6 +769,9 @@ __global__ void __launch_bounds__(kKv8PromptThreads, 1) kv8_prompt_kernel(Kv8Att
                     __nanosleep(20);  // leaves the issue slots to the softmax
                 }
             }
+            commit(drained);  // no product is on its way when the CTA gives its memory back
+            since = clock64();
+            while (!done(drained, 0) && !__any_sync(kFull, clock64() - since > kWaitBudgetCycles)) __nanosleep(20);
         }
         __syncwarp();
     }
