@@ -576,6 +576,42 @@ typedef struct {
 int phonon_cuda_qk_norm_rope_device(int device, const PhononCudaQkNormRope *args, int32_t *status_dev,
                                     void *cuda_stream);
 
+/* ---- rows in 8 bits, and their product with 8-bit weights ----
+ * A row x becomes 8-bit integers q with a scale s = max(max|x| / 127, 2^-126)
+ * in fp32: q is the integer nearest x / s, ties to even. x is [rows][cols], q
+ * [rows][cols] bytes; cols a multiple of 16. A row with a non-finite element
+ * gets the scale NaN and integers 0, and status_dev (device, [rows],
+ * optional, zeroed by the caller) is raised to PHONON_CUDA_NON_FINITE for it.
+ * Enqueued on `cuda_stream` of `device`, like the cache's calls above. */
+typedef struct {
+    uint32_t type; /* PhononCudaRowType of x */
+    uint32_t rows, cols;
+    const void *x; /* 16-byte aligned, as q is */
+    int8_t *q;
+    float *scales;              /* device [rows] */
+    uint64_t x_stride, q_stride; /* elements from row to row (0: packed), multiples of 8 and of 16 */
+} PhononCudaQuantizeRows;
+int phonon_cuda_quantize_rows_device(int device, const PhononCudaQuantizeRows *args, int32_t *status_dev,
+                                     void *cuda_stream);
+
+/* y[t][n] = x_scales[t] * w_scales[n] * sum_k x[t][k] * weights[n][k] + bias[n]:
+ * the sum is exact, then rounded to fp32, as are its products with x_scales
+ * and then (with the bias in one) with w_scales; bf16 rounds once more. x is
+ * [rows][depth], weights [channels][depth], any 8-bit integers, depth a
+ * multiple of 16 below 2^17; y is [rows][channels], any number of them.
+ * status_dev (device, [rows], optional, zeroed by the caller) is raised to
+ * NON_FINITE for a row with a non-finite result, and to DEVICE_ERROR where
+ * the kernel gave up a bounded wait (about two seconds): the row is NaN. */
+typedef struct {
+    uint32_t type; /* PhononCudaRowType of y */
+    uint32_t rows, channels, depth;
+    const int8_t *x, *weights;                /* 16-byte aligned, as y is */
+    const float *x_scales, *w_scales, *bias;  /* device [rows], [channels], [channels] or NULL */
+    void *y;
+    uint64_t x_stride, w_stride, y_stride; /* elements from row to row (0: packed); x's and w's multiples of 16 */
+} PhononCudaI8Product;
+int phonon_cuda_i8_product_device(int device, const PhononCudaI8Product *args, int32_t *status_dev, void *cuda_stream);
+
 const char *phonon_cuda_status_string(int status);
 
 #ifdef __cplusplus

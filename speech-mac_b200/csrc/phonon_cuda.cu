@@ -11,6 +11,7 @@
 #include "phonon_kv8.cuh"
 #include "phonon_kv8_prompt.cuh"
 #include "phonon_qk.cuh"
+#include "phonon_i8.cuh"
 #include "phonon_status.h"
 
 #include <cuda_fp16.h>
@@ -4753,6 +4754,118 @@ int phonon_cuda_qk_norm_rope_device(int device, const PhononCudaQkNormRope* a, i
         case 64: return bf16 ? qk_launch<64, true>(p, halves, sms, s) : qk_launch<64, false>(p, halves, sms, s);
         default: return bf16 ? qk_launch<128, true>(p, halves, sms, s) : qk_launch<128, false>(p, halves, sms, s);
     }
+}
+
+}  // extern "C"
+
+// ============================== rows in 8 bits and their product with weights
+namespace {
+
+int device_sms(int device, int* sms) {
+    return cudaDeviceGetAttribute(sms, cudaDevAttrMultiProcessorCount, device) == cudaSuccess ? PHONON_CUDA_OK
+                                                                                               : PHONON_CUDA_DEVICE_ERROR;
+}
+
+template <bool kBf16, int kThreads, int kUnits>
+int quantize_launch(const I8QuantParams& p, cudaStream_t s) {
+    constexpr int rows = 256 / kThreads;
+    CUDA_TRY(launch_pdl(i8_quantize_kernel<kBf16, kThreads, kUnits>, dim3(static_cast<unsigned>((p.rows + rows - 1) / rows)),
+                        dim3(256), 0, s, p));
+    return PHONON_CUDA_OK;
+}
+
+template <bool kBf16>
+int quantize_rows(const I8QuantParams& p, cudaStream_t s) {
+    if (p.cols <= 256) return quantize_launch<kBf16, 32, 1>(p, s);
+    if (p.cols <= 1024) return quantize_launch<kBf16, 32, 4>(p, s);
+    if (p.cols <= 4096) return quantize_launch<kBf16, 128, 4>(p, s);
+    return quantize_launch<kBf16, 256, 4>(p, s);
+}
+
+template <int NT, bool kBf16>
+int i8_rows_launch(const I8Params& p, cudaStream_t s) {
+    CUDA_TRY(launch_pdl(i8_rows_kernel<NT, kBf16>, dim3(static_cast<unsigned>((p.channels + 15) / 16)), dim3(32 * kI8Warps), 0, s, p));
+    return PHONON_CUDA_OK;
+}
+
+template <int kN, bool kBf16>
+int i8_tiles_launch(I8Params p, int sms, cudaStream_t s) {
+    static std::atomic<uint64_t> configured{0};
+    auto kernel = i8_product_kernel<kN, kBf16>;
+    constexpr int smem = i8_smem<kN>();
+    CUDA_TRY(opt_in_smem(reinterpret_cast<const void*>(kernel), smem, configured));
+    CUtensorMap tx, tw;
+    const uint64_t depth = static_cast<uint64_t>(p.depth);
+    if (!make_map_2d(&tx, CU_TENSOR_MAP_DATA_TYPE_UINT8, p.x, static_cast<uint64_t>(p.rows), depth, static_cast<uint64_t>(p.x_stride), 128, 128) ||
+        !make_map_2d(&tw, CU_TENSOR_MAP_DATA_TYPE_UINT8, p.w, static_cast<uint64_t>(p.channels), depth, static_cast<uint64_t>(p.w_stride), 128, kN))
+        return PHONON_CUDA_DEVICE_ERROR;
+    p.tiles_m = (p.rows + 127) / 128;
+    p.tiles_n = (p.channels + kN - 1) / kN;
+    const long long tiles = static_cast<long long>(p.tiles_m) * p.tiles_n;
+    if (tiles > (1 << 30)) return PHONON_CUDA_CAPACITY;
+    CUDA_TRY(launch_pdl(kernel, dim3(static_cast<unsigned>(std::min<long long>(tiles, sms))), dim3(kI8Threads), smem, s, tx, tw, p));
+    return PHONON_CUDA_OK;
+}
+
+template <bool kBf16>
+int i8_product(const I8Params& p, int sms, cudaStream_t s) {
+    if (p.rows <= 8) return i8_rows_launch<1, kBf16>(p, s);
+    if (p.rows <= 16) return i8_rows_launch<2, kBf16>(p, s);
+    if (p.rows <= 32) return i8_rows_launch<4, kBf16>(p, s);
+    const long long tiles_m = (p.rows + 127) / 128;
+    if (tiles_m * ((p.channels + 255) / 256) >= sms) return i8_tiles_launch<256, kBf16>(p, sms, s);
+    if (tiles_m * ((p.channels + 127) / 128) >= sms) return i8_tiles_launch<128, kBf16>(p, sms, s);
+    return i8_tiles_launch<64, kBf16>(p, sms, s);
+}
+
+}  // namespace
+
+extern "C" {
+
+int phonon_cuda_quantize_rows_device(int device, const PhononCudaQuantizeRows* a, int32_t* status_dev, void* cuda_stream) {
+    I8QuantParams p{};
+    if (!a || a->type > PHONON_CUDA_ROWS_BF16 || a->rows > (1u << 30) || a->cols == 0 || a->cols % 16 ||
+        a->cols > (1u << 24) || !a->x || !a->q || !a->scales || !aligned16(a->x) || !aligned16(a->q) ||
+        !kv8_stride(a->x_stride, a->cols, &p.x_stride) || !kv8_stride(a->q_stride, a->cols, &p.q_stride) || p.q_stride % 16)
+        return PHONON_CUDA_INVALID_ARGUMENT;
+    if (a->rows == 0) return PHONON_CUDA_OK;
+    p.x = a->x;
+    p.q = a->q;
+    p.scales = a->scales;
+    p.status = status_dev;
+    p.rows = static_cast<int>(a->rows);
+    p.cols = static_cast<int>(a->cols);
+    DeviceGuard guard(device);
+    if (!guard.ok) return PHONON_CUDA_DEVICE_ERROR;
+    cudaStream_t s = static_cast<cudaStream_t>(cuda_stream);
+    return a->type == PHONON_CUDA_ROWS_BF16 ? quantize_rows<true>(p, s) : quantize_rows<false>(p, s);
+}
+
+int phonon_cuda_i8_product_device(int device, const PhononCudaI8Product* a, int32_t* status_dev, void* cuda_stream) {
+    I8Params p{};
+    if (!a || a->type > PHONON_CUDA_ROWS_BF16 || a->rows > (1u << 30) || a->channels == 0 || a->channels > (1u << 30) ||
+        a->depth == 0 || a->depth % 16 || a->depth >= (1u << 17) || !a->x || !a->weights || !a->x_scales || !a->w_scales ||
+        !a->y || !aligned16(a->x) || !aligned16(a->weights) || !aligned16(a->y) ||
+        !kv8_stride(a->x_stride, a->depth, &p.x_stride) || !kv8_stride(a->w_stride, a->depth, &p.w_stride) ||
+        p.x_stride % 16 || p.w_stride % 16 || (a->y_stride && a->y_stride < a->channels) || a->y_stride > (1ull << 40))
+        return PHONON_CUDA_INVALID_ARGUMENT;
+    if (a->rows == 0) return PHONON_CUDA_OK;
+    p.x = a->x;
+    p.w = a->weights;
+    p.x_scales = a->x_scales;
+    p.w_scales = a->w_scales;
+    p.bias = a->bias;
+    p.y = a->y;
+    p.y_stride = static_cast<long long>(a->y_stride ? a->y_stride : a->channels);
+    p.status = status_dev;
+    p.rows = static_cast<int>(a->rows);
+    p.channels = static_cast<int>(a->channels);
+    p.depth = static_cast<int>(a->depth);
+    DeviceGuard guard(device);
+    int sms = 0;
+    if (!guard.ok || device_sms(device, &sms)) return PHONON_CUDA_DEVICE_ERROR;
+    cudaStream_t s = static_cast<cudaStream_t>(cuda_stream);
+    return a->type == PHONON_CUDA_ROWS_BF16 ? i8_product<true>(p, sms, s) : i8_product<false>(p, sms, s);
 }
 
 }  // extern "C"

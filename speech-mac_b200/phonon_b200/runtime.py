@@ -89,6 +89,18 @@ class QkNormRopeArgs(C.Structure):
                 ("q_weight", C.c_void_p), ("k_weight", C.c_void_p)]
 
 
+class QuantizeRowsArgs(C.Structure):
+    _fields_ = [("type", C.c_uint32), ("rows", C.c_uint32), ("cols", C.c_uint32), ("x", C.c_void_p), ("q", C.c_void_p),
+                ("scales", C.c_void_p), ("x_stride", C.c_uint64), ("q_stride", C.c_uint64)]
+
+
+class I8ProductArgs(C.Structure):
+    _fields_ = [("type", C.c_uint32), ("rows", C.c_uint32), ("channels", C.c_uint32), ("depth", C.c_uint32),
+                ("x", C.c_void_p), ("weights", C.c_void_p), ("x_scales", C.c_void_p), ("w_scales", C.c_void_p),
+                ("bias", C.c_void_p), ("y", C.c_void_p), ("x_stride", C.c_uint64), ("w_stride", C.c_uint64),
+                ("y_stride", C.c_uint64)]
+
+
 class CudaError(RuntimeError):
     def __init__(self, status, what):
         self.status = status
@@ -155,6 +167,8 @@ def lib():
         "phonon_cuda_kv8_read_device": [P, U32, C.POINTER(Kv8Batch), C.POINTER(Kv8Rows), P, P],
         "phonon_cuda_kv8_workspace_create": [P, C.POINTER(P)],
         "phonon_cuda_qk_norm_rope_device": [C.c_int, C.POINTER(QkNormRopeArgs), P, P],
+        "phonon_cuda_quantize_rows_device": [C.c_int, C.POINTER(QuantizeRowsArgs), P, P],
+        "phonon_cuda_i8_product_device": [C.c_int, C.POINTER(I8ProductArgs), P, P],
         "phonon_cuda_kv8_attention_device": [P, U32, C.POINTER(Kv8Batch), C.POINTER(Kv8Query), P, P, P],
     }
     for name, args in sig.items():
@@ -724,3 +738,32 @@ class QkNormRope:
 
     def __call__(self, status_ptr=None, stream_ptr=0):
         check(self._fn(self.device, self.args, status_ptr, stream_ptr), "qk_norm_rope_device")
+
+
+class QuantizeRows:
+    """phonon_cuda_quantize_rows_device over rows at fixed addresses: 8-bit
+    integers and a scale for each row. Calling it enqueues one pass."""
+
+    def __init__(self, x_ptr, q_ptr, scales_ptr, rows, cols, type=ROWS_F32, x_stride=0, q_stride=0, device=0):
+        self.device = device
+        self.args = QuantizeRowsArgs(type, rows, cols, x_ptr, q_ptr, scales_ptr, x_stride, q_stride)
+        self._fn = lib().phonon_cuda_quantize_rows_device
+
+    def __call__(self, status_ptr=None, stream_ptr=0):
+        check(self._fn(self.device, self.args, status_ptr, stream_ptr), "quantize_rows_device")
+
+
+class I8Product:
+    """phonon_cuda_i8_product_device over operands at fixed addresses: rows in
+    8 bits times weights in 8 bits, scales for each row and channel, an
+    optional bias. Calling it enqueues one pass."""
+
+    def __init__(self, x_ptr, x_scales_ptr, w_ptr, w_scales_ptr, y_ptr, rows, channels, depth, type=ROWS_F32,
+                 bias_ptr=None, x_stride=0, w_stride=0, y_stride=0, device=0):
+        self.device = device
+        self.args = I8ProductArgs(type, rows, channels, depth, x_ptr, w_ptr, x_scales_ptr, w_scales_ptr, bias_ptr, y_ptr,
+                                  x_stride, w_stride, y_stride)
+        self._fn = lib().phonon_cuda_i8_product_device
+
+    def __call__(self, status_ptr=None, stream_ptr=0):
+        check(self._fn(self.device, self.args, status_ptr, stream_ptr), "i8_product_device")
