@@ -612,6 +612,42 @@ typedef struct {
 } PhononCudaI8Product;
 int phonon_cuda_i8_product_device(int device, const PhononCudaI8Product *args, int32_t *status_dev, void *cuda_stream);
 
+/* ---- causal attention over packed prompts ----
+ * flow_attention (src/phonon_transformer.c:340-404) for whole prompts, before
+ * or without a cache: prompt i is the rows [row_begin[i], row_begin[i + 1]) of
+ * q and out ([rows][heads][head_dim]) and of k and v ([rows][kv_heads][head_dim]),
+ * heads a multiple of kv_heads; its row at position p sees its positions
+ * (p - window, p], or [0, p] where window is 0. Rows of no prompt, before
+ * row_begin[0] or from row_begin[prompts] on, are left as they were. max_rows
+ * bounds every prompt's rows. Sums and softmax statistics are fp32; bf16 rows:
+ * weights are rounded to bf16 (an output's error stays near its own rounding).
+ * Enqueued on `cuda_stream` of `device`, like the cache's calls; status_dev
+ * (device, [prompts], optional, zeroed by the caller) is raised for a prompt
+ *   - whose rows lie outside [0, rows), are more than max_rows or begin before
+ *     an earlier entry of row_begin (INVALID_ARGUMENT): its rows of out stay;
+ *   - with a non-finite output (NON_FINITE): a row that sees a non-finite
+ *     value, or whose scores leave fp32's range, is not finite; others are
+ *     what they are without it;
+ *   - where the kernel gave up a bounded wait (DEVICE_ERROR, about two
+ *     seconds): rows of it are NaN.
+ * The largest code stays. out may be q with q's stride, or lie apart from q, k
+ * and v. The call returns CAPACITY where rows, prompts and heads make more
+ * than 2^31 blocks of work. */
+typedef struct {
+    uint32_t type; /* PhononCudaRowType of q, k, v and out */
+    uint32_t prompts, rows, max_rows; /* prompts and max_rows at least 1 */
+    uint32_t heads, kv_heads;
+    uint32_t head_dim;         /* 32, 64 or 128 */
+    uint32_t window;           /* 0: none */
+    float scale;               /* of the scores, at most 1e30; 0: 1 / sqrt(head_dim) */
+    const int32_t *row_begin;  /* device [prompts + 1] */
+    const void *q, *k, *v;     /* 16-byte aligned, as out is */
+    void *out;
+    uint64_t q_stride, k_stride, v_stride, out_stride; /* elements from row to row, multiples of 8 (0: packed) */
+} PhononCudaPromptAttention;
+int phonon_cuda_prompt_attention_device(int device, const PhononCudaPromptAttention *args, int32_t *status_dev,
+                                        void *cuda_stream);
+
 const char *phonon_cuda_status_string(int status);
 
 #ifdef __cplusplus

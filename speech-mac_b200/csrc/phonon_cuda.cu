@@ -12,6 +12,7 @@
 #include "phonon_kv8_prompt.cuh"
 #include "phonon_qk.cuh"
 #include "phonon_i8.cuh"
+#include "phonon_prompt.cuh"
 #include "phonon_status.h"
 
 #include <cuda_fp16.h>
@@ -4866,6 +4867,67 @@ int phonon_cuda_i8_product_device(int device, const PhononCudaI8Product* a, int3
     if (!guard.ok || device_sms(device, &sms)) return PHONON_CUDA_DEVICE_ERROR;
     cudaStream_t s = static_cast<cudaStream_t>(cuda_stream);
     return a->type == PHONON_CUDA_ROWS_BF16 ? i8_product<true>(p, sms, s) : i8_product<false>(p, sms, s);
+}
+
+}  // extern "C"
+
+// ============================================ attention over packed prompts
+namespace {
+
+template <int D, bool kBf16>
+int prompt_launch(PromptParams p, cudaStream_t s) {
+    p.tokens = std::max(1, 64 / static_cast<int>(p.group.d));
+    const long long slots = std::min<long long>(p.rows / p.tokens + static_cast<long long>(p.prompts),
+                                                static_cast<long long>(p.prompts) * ((p.max_rows + p.tokens - 1) / p.tokens));
+    if (slots * p.kv_heads > INT32_MAX) return PHONON_CUDA_CAPACITY;
+    p.by_heads = kv8_divisor(static_cast<uint32_t>(p.kv_heads));
+    CUDA_TRY(launch_pdl(prompt_rows_kernel<D, kBf16>, dim3(static_cast<unsigned>(slots * p.kv_heads)), dim3(256), 0, s, p));
+    return PHONON_CUDA_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int phonon_cuda_prompt_attention_device(int device, const PhononCudaPromptAttention* a, int32_t* status_dev,
+                                        void* cuda_stream) {
+    PromptParams p{};
+    if (!a || a->type > PHONON_CUDA_ROWS_BF16 || a->prompts == 0 || a->prompts > (1u << 24) || a->rows > (1u << 30) ||
+        a->max_rows == 0 || a->max_rows > (1u << 30) || a->heads == 0 || a->kv_heads == 0 || a->heads > (1u << 16) ||
+        a->heads % a->kv_heads || (a->head_dim != 32 && a->head_dim != 64 && a->head_dim != 128) ||
+        a->window > (1u << 30) || !(a->scale >= 0.0f && a->scale <= 1e30f) || !a->row_begin || !a->q || !a->k || !a->v ||
+        !a->out || !aligned16(a->q) || !aligned16(a->k) || !aligned16(a->v) || !aligned16(a->out))
+        return PHONON_CUDA_INVALID_ARGUMENT;
+    const uint64_t width = static_cast<uint64_t>(a->heads) * a->head_dim, kv_width = static_cast<uint64_t>(a->kv_heads) * a->head_dim;
+    if (!kv8_stride(a->q_stride, width, &p.q_stride) || !kv8_stride(a->k_stride, kv_width, &p.k_stride) ||
+        !kv8_stride(a->v_stride, kv_width, &p.v_stride) || !kv8_stride(a->out_stride, width, &p.out_stride) ||
+        rows_collide(a->q, p.q_stride, a->out, p.out_stride, a->rows) || a->out == a->k || a->out == a->v)
+        return PHONON_CUDA_INVALID_ARGUMENT;
+    if (a->rows == 0) return PHONON_CUDA_OK;
+    p.q = a->q;
+    p.k = a->k;
+    p.v = a->v;
+    p.out = a->out;
+    p.begin = a->row_begin;
+    p.status = status_dev;
+    p.prompts = static_cast<int>(a->prompts);
+    p.rows = static_cast<int>(a->rows);
+    p.max_rows = static_cast<int>(std::min(a->max_rows, a->rows));
+    p.heads = static_cast<int>(a->heads);
+    p.kv_heads = static_cast<int>(a->kv_heads);
+    p.group = kv8_divisor(a->heads / a->kv_heads);
+    p.window = static_cast<int>(a->window);
+    p.scale = static_cast<float>((a->scale > 0.0f ? static_cast<double>(a->scale) : 1.0 / std::sqrt(static_cast<double>(a->head_dim))) *
+                                 1.4426950408889634074);
+    DeviceGuard guard(device);
+    if (!guard.ok) return PHONON_CUDA_DEVICE_ERROR;
+    cudaStream_t s = static_cast<cudaStream_t>(cuda_stream);
+    const bool bf16 = a->type == PHONON_CUDA_ROWS_BF16;
+    switch (a->head_dim) {
+        case 32: return bf16 ? prompt_launch<32, true>(p, s) : prompt_launch<32, false>(p, s);
+        case 64: return bf16 ? prompt_launch<64, true>(p, s) : prompt_launch<64, false>(p, s);
+        default: return bf16 ? prompt_launch<128, true>(p, s) : prompt_launch<128, false>(p, s);
+    }
 }
 
 }  // extern "C"

@@ -101,6 +101,14 @@ class I8ProductArgs(C.Structure):
                 ("y_stride", C.c_uint64)]
 
 
+class PromptAttentionArgs(C.Structure):
+    _fields_ = [("type", C.c_uint32), ("prompts", C.c_uint32), ("rows", C.c_uint32), ("max_rows", C.c_uint32),
+                ("heads", C.c_uint32), ("kv_heads", C.c_uint32), ("head_dim", C.c_uint32), ("window", C.c_uint32),
+                ("scale", C.c_float), ("row_begin", C.c_void_p), ("q", C.c_void_p), ("k", C.c_void_p), ("v", C.c_void_p),
+                ("out", C.c_void_p), ("q_stride", C.c_uint64), ("k_stride", C.c_uint64), ("v_stride", C.c_uint64),
+                ("out_stride", C.c_uint64)]
+
+
 class CudaError(RuntimeError):
     def __init__(self, status, what):
         self.status = status
@@ -169,6 +177,7 @@ def lib():
         "phonon_cuda_qk_norm_rope_device": [C.c_int, C.POINTER(QkNormRopeArgs), P, P],
         "phonon_cuda_quantize_rows_device": [C.c_int, C.POINTER(QuantizeRowsArgs), P, P],
         "phonon_cuda_i8_product_device": [C.c_int, C.POINTER(I8ProductArgs), P, P],
+        "phonon_cuda_prompt_attention_device": [C.c_int, C.POINTER(PromptAttentionArgs), P, P],
         "phonon_cuda_kv8_attention_device": [P, U32, C.POINTER(Kv8Batch), C.POINTER(Kv8Query), P, P, P],
     }
     for name, args in sig.items():
@@ -767,3 +776,20 @@ class I8Product:
 
     def __call__(self, status_ptr=None, stream_ptr=0):
         check(self._fn(self.device, self.args, status_ptr, stream_ptr), "i8_product_device")
+
+
+class PromptAttention:
+    """phonon_cuda_prompt_attention_device over rows at fixed addresses: causal
+    attention of packed prompts, prompt i in rows [row_begin[i],
+    row_begin[i + 1]) (a device array). Calling it enqueues one pass."""
+
+    def __init__(self, q_ptr, k_ptr, v_ptr, out_ptr, row_begin_ptr, prompts, rows, max_rows, heads, kv_heads, head_dim,
+                 type=ROWS_F32, window=0, scale=0.0, q_stride=0, k_stride=0, v_stride=0, out_stride=0, device=0):
+        self.device = device
+        self.args = PromptAttentionArgs(type, prompts, rows, max_rows, heads, kv_heads, head_dim, window, scale,
+                                        row_begin_ptr, q_ptr, k_ptr, v_ptr, out_ptr, q_stride, k_stride, v_stride,
+                                        out_stride)
+        self._fn = lib().phonon_cuda_prompt_attention_device
+
+    def __call__(self, status_ptr=None, stream_ptr=0):
+        check(self._fn(self.device, self.args, status_ptr, stream_ptr), "prompt_attention_device")
