@@ -4874,14 +4874,63 @@ int phonon_cuda_i8_product_device(int device, const PhononCudaI8Product* a, int3
 // ============================================ attention over packed prompts
 namespace {
 
-template <int D, bool kBf16>
-int prompt_launch(PromptParams p, cudaStream_t s) {
-    p.tokens = std::max(1, 64 / static_cast<int>(p.group.d));
+// Boxes of `box` elements x heads x positions over [rows][heads][dim] bf16 elements.
+bool make_rows_map(CUtensorMap* map, const void* base, int rows, int heads, int dim, long long stride, int box, int box_heads, int box_rows) {
+    EncodeTiledFn fn = encode_tiled();
+    const cuuint64_t dims[3] = {static_cast<cuuint64_t>(dim), static_cast<cuuint64_t>(heads), static_cast<cuuint64_t>(rows)};
+    const cuuint64_t strides[2] = {static_cast<cuuint64_t>(dim) * 2, static_cast<cuuint64_t>(stride) * 2};
+    const cuuint32_t boxes[3] = {static_cast<cuuint32_t>(box), static_cast<cuuint32_t>(box_heads), static_cast<cuuint32_t>(box_rows)};
+    const cuuint32_t each[3] = {1, 1, 1};
+    return fn && fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims, strides, boxes, each, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                    box == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                    CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// Tiles of p.tokens positions, `parts` CTAs each.
+int prompt_grid(PromptParams& p, int parts, unsigned* grid) {
     const long long slots = std::min<long long>(p.rows / p.tokens + static_cast<long long>(p.prompts),
                                                 static_cast<long long>(p.prompts) * ((p.max_rows + p.tokens - 1) / p.tokens));
-    if (slots * p.kv_heads > INT32_MAX) return PHONON_CUDA_CAPACITY;
-    p.by_heads = kv8_divisor(static_cast<uint32_t>(p.kv_heads));
-    CUDA_TRY(launch_pdl(prompt_rows_kernel<D, kBf16>, dim3(static_cast<unsigned>(slots * p.kv_heads)), dim3(256), 0, s, p));
+    if (slots * parts > INT32_MAX) return PHONON_CUDA_CAPACITY;
+    p.by_heads = kv8_divisor(static_cast<uint32_t>(parts));
+    *grid = static_cast<unsigned>(slots * parts);
+    return PHONON_CUDA_OK;
+}
+
+template <int D>
+int prompt_launch_bf16(PromptParams p, cudaStream_t s) {
+    using Shape = PromptShape<D>;
+    // Query heads of a K/V head share rows of a tile, and so its keys and values.
+    const int group = static_cast<int>(p.group.d), pack = group <= 32 ? group : 1, half = 128 / pack;
+    p.pack = kv8_divisor(static_cast<uint32_t>(pack));
+    p.tokens = 2 * half;
+    unsigned grid = 0;
+    if (const int rc = prompt_grid(p, p.heads / pack, &grid)) return rc;
+    CUtensorMap q, k, v;
+    if (!make_rows_map(&q, p.q, p.rows, p.heads, D, p.q_stride, Shape::kBox, pack, half) ||
+        !make_rows_map(&k, p.k, p.rows, p.kv_heads, D, p.k_stride, Shape::kBox, 1, kPromptKeys) ||
+        !make_rows_map(&v, p.v, p.rows, p.kv_heads, D, p.v_stride, Shape::kBox, 1, kPromptKeys))
+        return PHONON_CUDA_DEVICE_ERROR;
+    // Its warps hand registers to one another: what they ask for has to be what the launch has.
+    static std::atomic<bool> enough{false};
+    if (!enough) {
+        cudaFuncAttributes f{};
+        CUDA_TRY(cudaFuncGetAttributes(&f, prompt_bf16_kernel<D>));
+        if ((f.numRegs + 7) / 8 * 8 * kPromptThreads < kPromptRegisters) return PHONON_CUDA_DEVICE_ERROR;
+        enough = true;
+    }
+    static std::atomic<uint64_t> configured{0};
+    CUDA_TRY(opt_in_smem(reinterpret_cast<const void*>(prompt_bf16_kernel<D>), Shape::kSmem, configured));
+    CUDA_TRY(launch_pdl(prompt_bf16_kernel<D>, dim3(grid), dim3(kPromptThreads), Shape::kSmem, s, q, k, v, p));
+    return PHONON_CUDA_OK;
+}
+
+template <int D, bool kBf16>
+int prompt_launch(PromptParams p, cudaStream_t s) {
+    if constexpr (kBf16) return prompt_launch_bf16<D>(p, s);
+    p.tokens = std::max(1, 64 / static_cast<int>(p.group.d));
+    unsigned grid = 0;
+    if (const int rc = prompt_grid(p, p.kv_heads, &grid)) return rc;
+    CUDA_TRY(launch_pdl(prompt_rows_kernel<D, kBf16>, dim3(grid), dim3(256), 0, s, p));
     return PHONON_CUDA_OK;
 }
 

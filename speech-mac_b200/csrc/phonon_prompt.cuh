@@ -7,7 +7,8 @@
 // query heads are grouped on K/V heads.
 #pragma once
 
-#include "phonon_kv8_prompt.cuh"
+#include "phonon_head_gemm.cuh"
+#include "phonon_i8.cuh"
 
 namespace phonon {
 
@@ -18,10 +19,11 @@ struct PromptParams {
     const int32_t* begin;  // [prompts + 1]
     int32_t* status;       // [prompts] or null
     int prompts, rows, max_rows, heads, kv_heads;
-    Kv8Div group;  // query heads of a K/V head
-    int window;    // 0: none
-    float scale;   // times log2(e)
-    int tokens;    // positions of a tile
+    Kv8Div group;     // query heads of a K/V head
+    int window;       // 0: none
+    float scale;      // times log2(e)
+    Kv8Div pack;      // query heads that share a tile's rows: all of a K/V head's, or one
+    int tokens;       // positions of a tile
     Kv8Div by_heads;  // CTAs of a tile
 };
 
@@ -137,6 +139,405 @@ __device__ __forceinline__ void prompt_row(const PromptParams& p, const PromptTi
             static_cast<float*>(p.out)[at + d * 32 + lane] = x;
             finite &= isfinite(x);
         }
+    }
+}
+
+// ------------------------------------------------- bf16 rows on tcgen05
+// A CTA has two row tiles of 128 rows (a row is a position and one of the
+// `pack` query heads that share its K/V head), each with a softmax of four
+// warps, a row a thread: while one tile's scores become weights, the tensor
+// cores work for the other.
+//
+//   warp 8     brings q, then 128 positions of k and of v a turn by TMA
+//   warp 9     issues S = q k^T and O += P v in turn for both tiles
+//   warps 0-7  S to registers, its maximum, the weights 2^(s - M) as bf16 back
+//              over S (the A operand of P v), the sum of weights in fp32
+//
+// O stays in TMEM. M follows the maximum only where that would make weights
+// above 2^8: the tile's own warps then multiply O by 2^(M - M'), which they may
+// since S of a turn comes behind P v of the turn before in the tensor cores'
+// order.
+//
+// Positions that a row does not see get the weight 0, whose product with a v
+// that is not finite is NaN. So where an output is not finite the CTA starts
+// over, carefully: warp 8 looks at every turn's values, puts 0 in place of
+// those that are not finite, and the rows that see one become NaN. (Nothing is
+// written before: out may lie over q.)
+constexpr int kPromptThreads = 384, kPromptKeys = 128;
+// A thread's registers in warps 0-7 and 8-11, together the launch's 168 each.
+constexpr int kPromptSoftmaxRegisters = 208, kPromptOtherRegisters = 88;
+constexpr int kPromptRegisters = 256 * kPromptSoftmaxRegisters + 128 * kPromptOtherRegisters;
+constexpr float kPromptSlack = 8.0f;
+
+template <int D>
+struct PromptShape {
+    static constexpr int kBox = D < 64 ? D : 64, kBoxBytes = 2 * kBox, kBoxes = D / kBox;  // a row's piece of a tile
+    static constexpr int kStages = D == 128 ? 2 : 3;
+    static constexpr int kTile = 128 * D * 2;  // bytes of a tile of q, k or v
+    static constexpr int kSmem = 1024 + (2 + 2 * kStages) * kTile;
+};
+
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+        ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y), "r"(z)
+        : "memory");
+}
+
+// Rows of kBytes (128 or 64) in the swizzle of that width, 8 rows together. K
+// major: the operand's K runs along the rows. MN major: it runs across them,
+// blocks of kBytes of the other dimension `block` bytes apart.
+template <int kBytes>
+__device__ __forceinline__ uint64_t umma_desc_rows(uint32_t addr, uint32_t block = 16) {
+    uint64_t d = (static_cast<uint64_t>(addr) >> 4) & 0x3FFFull;
+    d |= static_cast<uint64_t>((block >> 4) & 0x3FFFu) << 16;     // leading byte offset
+    d |= static_cast<uint64_t>(8 * kBytes >> 4) << 32;            // stride byte offset
+    d |= static_cast<uint64_t>(1) << 46;                          // descriptor version (sm_100)
+    d |= static_cast<uint64_t>(kBytes == 128 ? 2 : 4) << 61;      // SWIZZLE_128B, SWIZZLE_64B
+    return d;
+}
+
+constexpr uint32_t kUmmaBMnMajor = 1u << 16;  // of an instruction descriptor
+
+// 32 packed columns of the warp's 32 lanes into TMEM.
+__device__ __forceinline__ void tmem_store32(uint32_t taddr, const uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {"
+        "%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
+        "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+        "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]),
+        "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]),
+        "r"(r[31])
+        : "memory");
+}
+
+__device__ __forceinline__ uint32_t bf16x2_bits(float a, float b) {  // a in the low half
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// Which of the 32 keys from `key` on the row at `position` sees: bits.
+__device__ __forceinline__ uint32_t prompt_seen(int position, int window, int key) {
+    const int ahead = position - key, behind = window ? ahead - window : -1;  // sees keys (behind, ahead]
+    uint32_t bits = ahead >= 31 ? kFull : ahead < 0 ? 0u : (2u << ahead) - 1;
+    if (behind >= 0) bits &= behind >= 31 ? 0u : ~((2u << behind) - 1);
+    return bits;
+}
+
+// The keys that the positions [first, end) see, in turns of kPromptKeys from key0 on: [begin, end).
+struct PromptTurns {
+    int begin, end;
+};
+__device__ __forceinline__ PromptTurns prompt_turns(int first, int end, int window, int key0) {
+    if (end <= first) return {0, 0};
+    const int low = window ? max(0, first - window + 1) : 0;
+    return {(low - key0) / kPromptKeys, (end - key0 + kPromptKeys - 1) / kPromptKeys};
+}
+
+template <int D>
+__global__ void __launch_bounds__(kPromptThreads, 1)
+    prompt_bf16_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
+                       const __grid_constant__ CUtensorMap tm_v, PromptParams p) {
+    using Shape = PromptShape<D>;
+    constexpr int kStages = Shape::kStages, kTile = Shape::kTile, kBoxes = Shape::kBoxes, kBytes = Shape::kBoxBytes;
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ __align__(8) uint64_t s_bars[4 * kStages + 9];
+    __shared__ uint32_t s_tmem;
+    __shared__ int s_failed, s_dirty;
+    __shared__ uint32_t s_bad[kStages][kPromptKeys / 32];  // careful: which of a turn's values are not finite
+    const uint32_t s_q = (smem_addr(smem_raw) + 1023) & ~1023u, s_k = s_q + 2 * kTile, s_v = s_k + kStages * kTile;
+    const uint32_t k_full = smem_addr(s_bars), k_empty = k_full + 8 * kStages, v_full = k_empty + 8 * kStages, v_empty = v_full + 8 * kStages;
+    const uint32_t s_full = v_empty + 8 * kStages, p_full = s_full + 16, o_full = p_full + 16, q_full = o_full + 16, tail = q_full + 8, idle = tail + 8;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const auto init = [&](bool again) {  // one thread
+        const auto set = [&](uint32_t bar, uint32_t count) {
+            if (again) asm volatile("mbarrier.inval.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
+            mbar_init(bar, count);
+        };
+        for (int s = 0; s < 4 * kStages; ++s) set(k_full + 8 * s, 1);
+        for (int s = 0; s < 2; ++s) {
+            set(s_full + 8 * s, 1);
+            set(p_full + 8 * s, 4);
+            set(o_full + 8 * s, 1);
+        }
+        set(q_full, 1);
+        set(tail, 1);
+        set(idle, 1);
+        s_failed = s_dirty = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    };
+    if (threadIdx.x == 0) init(false);
+    pdl_wait();
+    pdl_trigger();
+    const int slot = static_cast<int>(kv8_div(blockIdx.x, p.by_heads)), part = static_cast<int>(blockIdx.x - slot * p.by_heads.d);
+    const PromptTile t = prompt_tile<kPromptThreads>(p, slot, blockIdx.x == gridDim.x - 1);
+    if (t.index < 0) return;
+    const int pack = static_cast<int>(p.pack.d), head0 = part * pack, kv_head = static_cast<int>(kv8_div(head0, p.group));
+    const int half = p.tokens / 2, end = min(t.length, t.first + p.tokens);  // tile s: [first + s * half, min(end, first + (s + 1) * half))
+    const int key0 = p.window ? max(0, t.first - p.window + 1) : 0;
+    const PromptTurns turns0 = prompt_turns(t.first, min(end, t.first + half), p.window, key0);
+    const PromptTurns turns1 = prompt_turns(t.first + half, end, p.window, key0);
+    const int turns = max(turns0.end, turns1.end);
+    if (warp == 9) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_addr(&s_tmem)) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    const uint32_t tmem = s_tmem;  // S of both tiles, then O of both
+    const auto wait = [&](uint32_t bar, int use) {
+        const bool ok = mbar_wait(bar, use & 1, nullptr, &s_failed);
+        __syncwarp();
+        return __all_sync(kFull, ok);
+    };
+    bool careful = false;
+    const auto sync = [] { asm volatile("bar.sync 1, %0;" ::"n"(kPromptThreads) : "memory"); };
+    // Every warp, at its end: whether the CTA starts over.
+    const auto again = [&] {
+        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+        sync();
+        const bool redo = !careful && s_dirty && !s_failed;
+        if (!redo) return false;
+        sync();
+        if (threadIdx.x == 0) init(true);
+        sync();
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        return careful = true;
+    };
+    if (warp >= 8) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPromptOtherRegisters));
+        const bool two = turns1.end > 0;
+        if (warp == 8) do {
+            const auto load = [&](uint32_t to, const CUtensorMap* map, int head, int row, uint32_t bar) {
+#pragma unroll
+                for (int b = 0; b < kBoxes; ++b) tma_load_3d(to + b * 128 * kBytes, map, b * Shape::kBox, head, row, bar);
+            };
+            if (lane == 0) {
+                mbar_expect_tx(q_full, (two ? 2 : 1) * half * pack * D * 2);
+                load(s_q, &tm_q, head0, t.row0 + t.first, q_full);
+                if (two) load(s_q + kTile, &tm_q, head0, t.row0 + t.first + half, q_full);
+            }
+            int j = 0, looks = 0;
+            for (; j < turns; ++j) {
+                const int s = j % kStages, row = t.row0 + key0 + j * kPromptKeys, there = end - key0 - j * kPromptKeys;
+                if (j >= kStages && !wait(k_empty + 8 * s, j / kStages - 1)) break;
+                if (lane == 0) {
+                    mbar_expect_tx(k_full + 8 * s, kTile);
+                    load(s_k + s * kTile, &tm_k, kv_head, row, k_full + 8 * s);
+                }
+                if (j >= kStages && !wait(v_empty + 8 * s, j / kStages - 1)) break;
+                const bool look = careful || there < kPromptKeys;  // what follows the prompt may not be finite: zeros
+                const uint32_t bar = look ? tail : v_full + 8 * s;
+                if (lane == 0) {
+                    mbar_expect_tx(bar, kTile);
+                    load(s_v + s * kTile, &tm_v, kv_head, row, bar);
+                }
+                if (!look) continue;
+                if (lane < kPromptKeys / 32) s_bad[s][lane] = 0;
+                if (!wait(tail, looks++)) break;
+                for (int x = lane; x < 128 * kBoxes; x += 32) {  // a key's box each
+                    const int key = x & 127;
+                    const uint32_t at = s_v + s * kTile + x * kBytes;
+                    bool bad = false;
+                    for (int c = 0; c < kBytes; c += 16) {
+                        uint32_t w[4] = {0, 0, 0, 0};
+                        bool put = key >= there;
+                        if (!put) {
+                            asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(at + c));
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) {
+                                if ((w[k] & 0x7f80u) == 0x7f80u) w[k] &= 0xffff0000u, put = bad = true;
+                                if ((w[k] & 0x7f800000u) == 0x7f800000u) w[k] &= 0xffffu, put = bad = true;
+                            }
+                        }
+                        if (put) kv8_put16(at + c, w[0], w[1], w[2], w[3]);
+                    }
+                    if (bad) atomicOr(&s_bad[s][key >> 5], 1u << (key & 31));
+                }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) mbar_arrive(v_full + 8 * s);
+            }
+            if (j < turns && lane == 0) {  // a wait ran out: no copy is on its way when the CTA gives its memory back
+                mbar_settle(q_full, 0);
+                for (int i = max(0, j - kStages); i <= j; ++i) mbar_settle(k_full + 8 * (i % kStages), (i / kStages) & 1);
+                for (int i = max(0, j - kStages); i <= j; ++i) mbar_settle(v_full + 8 * (i % kStages), (i / kStages) & 1);
+            }
+            __syncwarp();
+        } while (again());
+        else if (warp == 9) do {
+            constexpr uint32_t idesc_s = umma_idesc_bf16(128, kPromptKeys), idesc_o = umma_idesc_bf16(128, D) | kUmmaBMnMajor;
+            uint32_t leader;
+            asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.b32 %0, 1, 0, p;\n\t}" : "=r"(leader));
+            const auto commit = [&](uint32_t bar) {
+                if (leader) umma_commit(bar);
+            };
+            bool ok = wait(q_full, 0);
+            const auto score = [&](int tile, const PromptTurns& in, int j) {
+                if (!ok || j < in.begin || j >= in.end) return;
+                const int s = j % kStages;
+                if (!(ok = wait(k_full + 8 * s, j / kStages))) return;
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    #pragma unroll
+                for (int k = 0; k < D / 16; ++k) {
+                    const uint32_t at = k / (kBytes / 32) * 128 * kBytes + k % (kBytes / 32) * 32;
+                    umma_half<false>(leader, tmem + tile * kPromptKeys, umma_desc_rows<kBytes>(s_q + tile * kTile + at),
+                                     umma_desc_rows<kBytes>(s_k + s * kTile + at), idesc_s, k != 0);
+                }
+                commit(s_full + 8 * tile);
+            };
+            const auto sum = [&](int tile, const PromptTurns& in, int j) {
+                if (!ok || j < in.begin || j >= in.end) return;
+                const int s = j % kStages;
+                if (!(ok = wait(v_full + 8 * s, j / kStages) && wait(p_full + 8 * tile, j - in.begin))) return;
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    #pragma unroll
+                for (int k = 0; k < kPromptKeys / 16; ++k)
+                    umma_half<true>(leader, tmem + 2 * kPromptKeys + tile * D, tmem + tile * kPromptKeys + k * 8,
+                                    umma_desc_rows<kBytes>(s_v + s * kTile + k * 16 * kBytes, 128 * kBytes), idesc_o, j != in.begin || k != 0);
+                if (j + 1 == in.end) commit(o_full + 8 * tile);
+            };
+            score(0, turns0, 0);
+            score(1, turns1, 0);
+            commit(k_empty);
+            for (int j = 0; ok && j < turns; ++j) {
+                sum(0, turns0, j);
+                score(0, turns0, j + 1);
+                sum(1, turns1, j);
+                commit(v_empty + 8 * (j % kStages));
+                if (j + 1 < turns) {
+                    score(1, turns1, j + 1);
+                    commit(k_empty + 8 * ((j + 1) % kStages));
+                }
+            }
+            commit(idle);  // no product is on its way when the CTA gives its memory back
+            mbar_settle(idle, 0);
+            __syncwarp();
+        } while (again());
+        else do {
+        } while (again());
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kPromptSoftmaxRegisters));
+        const int tile = warp >> 2, quarter = warp & 3, r = quarter * 32 + lane;
+        const PromptTurns in = tile ? turns1 : turns0;
+        const int first = t.first + tile * half, at = static_cast<int>(kv8_div(r, p.pack)), position = first + at;
+        const int last = min(end, first + half) - 1;  // the tile's last position
+        const uint32_t at_s = tmem + tile * kPromptKeys + (static_cast<uint32_t>(quarter * 32) << 16);
+        const uint32_t at_o = tmem + 2 * kPromptKeys + tile * D + (static_cast<uint32_t>(quarter * 32) << 16);
+        const bool mine = at < half && position <= last;
+        uint32_t w[D / 2];  // the row's output
+        bool good = true;
+        do {
+            float m = -INFINITY, l = 0.0f;
+            for (int j = in.begin; j < in.end; ++j) {
+                wait(s_full + 8 * tile, j - in.begin);
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                float s[4][32];
+#pragma unroll
+                for (int c = 0; c < 4; ++c) tmem_start(at_s + 32 * c, s[c]);
+#pragma unroll
+                for (int c = 0; c < 4; ++c) tmem_arrived(s[c]);
+                const int key = key0 + j * kPromptKeys;
+                if (key + kPromptKeys - 1 > first || (p.window && key <= last - p.window)) {  // not all of it by every row
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        const uint32_t bits = prompt_seen(position, p.window, key + 32 * c);
+#pragma unroll
+                        for (int k = 0; k < 32; ++k) s[c][k] = bits >> k & 1 ? s[c][k] : -INFINITY;
+                    }
+                }
+                float top[4];
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    top[c] = fmaxf(s[c][0], s[c][1]);
+#pragma unroll
+                    for (int k = 2; k < 32; k += 2) top[c] = max3(top[c], s[c][k], s[c][k + 1]);
+                }
+                const float now = fmaxf(max3(top[0], top[1], top[2]), top[3]) * p.scale;
+                const bool move = now > m + kPromptSlack;
+                if (__any_sync(kFull, move)) {
+                    const float to = move ? now : m;
+                    const float by = m == to ? 1.0f : ex2(m - to);
+                    m = to;
+                    l *= by;
+                    if (j != in.begin) {
+#pragma unroll 1
+                        for (int c = 0; c < D; c += 32) {
+                            float o[32];
+                            tmem_start(at_o + c, o);
+                            tmem_arrived(o);
+                            uint32_t w[32];
+#pragma unroll
+                            for (int k = 0; k < 32; ++k) w[k] = __float_as_uint(o[k] * by);
+                            tmem_store32(at_o + c, w);
+                        }
+                    }
+                }
+                const float from = m == -INFINITY ? 0.0f : -m;  // nothing seen yet: weights 2^-inf
+                const float2 scale = make_float2(p.scale, p.scale), from2 = make_float2(from, from);
+                float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    uint32_t w[32];
+#pragma unroll
+                    for (int k = 0; k < 32; ++k) {
+                        const float* x = &s[2 * h + k / 16][2 * (k % 16)];
+                        const float2 z = fma2(make_float2(x[0], x[1]), scale, from2);
+                        const float2 e = make_float2(ex2(z.x), ex2(z.y));
+                        sum[k & 1] = add2(sum[k & 1], e);
+                        w[k] = bf16x2_bits(e.x, e.y);
+                    }
+                    tmem_store32(at_s + 32 * h, w);
+                }
+                const float2 both = add2(sum[0], sum[1]);
+                l += both.x + both.y;
+                if (careful) {
+                    wait(v_full + 8 * (j % kStages), j / kStages);
+                    for (int c = 0; c < kPromptKeys / 32; ++c)
+                        if (s_bad[j % kStages][c] & prompt_seen(position, p.window, key + 32 * c)) l = __int_as_float(0x7fc00000);
+                }
+                asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+                asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) mbar_arrive(p_full + 8 * tile);
+            }
+            if (in.end > in.begin) wait(o_full + 8 * tile, 0);
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            const float inverse = *static_cast<volatile int*>(&s_failed) ? __int_as_float(0x7fc00000) : __fdiv_rn(1.0f, l);
+            const __nv_bfloat162 zero = __floats2bfloat162_rn(0.0f, 0.0f);
+            __nv_bfloat162 clean = zero;  // NaN once an output is not finite
+#pragma unroll
+            for (int c = 0; c < D; c += 32) {
+                float o[32];
+                tmem_start(at_o + c, o);
+                tmem_arrived(o);
+#pragma unroll
+                for (int k = 0; k < 16; ++k) {
+                    w[c / 2 + k] = bf16x2_bits(o[2 * k] * inverse, o[2 * k + 1] * inverse);
+                    clean = __hfma2(*reinterpret_cast<const __nv_bfloat162*>(&w[c / 2 + k]), zero, clean);
+                }
+            }
+            good = !mine || __low2float(clean) + __high2float(clean) == 0.0f;
+            if (!good) s_dirty = 1;
+            __syncwarp();
+        } while (again());
+        if (mine) {
+            const int head = head0 + r - at * pack;
+            uint4* to = reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(p.out) + static_cast<size_t>(t.row0 + position) * p.out_stride +
+                                                 static_cast<size_t>(head) * D);
+#pragma unroll
+            for (int k = 0; k < D / 8; ++k) to[k] = make_uint4(w[4 * k], w[4 * k + 1], w[4 * k + 2], w[4 * k + 3]);
+            if (!good) prompt_flag(p, t.index, s_failed ? kStatusDevice : kStatusNonFinite);
+        }
+    }
+    __syncwarp();
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    if (warp == 9) {
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
     }
 }
 
