@@ -4896,41 +4896,52 @@ int prompt_grid(PromptParams& p, int parts, unsigned* grid) {
     return PHONON_CUDA_OK;
 }
 
-template <int D>
-int prompt_launch_bf16(PromptParams p, cudaStream_t s) {
-    using Shape = PromptShape<D>;
-    // Query heads of a K/V head share rows of a tile, and so its keys and values.
-    const int group = static_cast<int>(p.group.d), pack = group <= 32 ? group : 1, half = 128 / pack;
-    p.pack = kv8_divisor(static_cast<uint32_t>(pack));
-    p.tokens = 2 * half;
-    unsigned grid = 0;
-    if (const int rc = prompt_grid(p, p.heads / pack, &grid)) return rc;
-    CUtensorMap q, k, v;
-    if (!make_rows_map(&q, p.q, p.rows, p.heads, D, p.q_stride, Shape::kBox, pack, half) ||
-        !make_rows_map(&k, p.k, p.rows, p.kv_heads, D, p.k_stride, Shape::kBox, 1, kPromptKeys) ||
-        !make_rows_map(&v, p.v, p.rows, p.kv_heads, D, p.v_stride, Shape::kBox, 1, kPromptKeys))
-        return PHONON_CUDA_DEVICE_ERROR;
-    // Its warps hand registers to one another: what they ask for has to be what the launch has.
-    static std::atomic<bool> enough{false};
-    if (!enough) {
-        cudaFuncAttributes f{};
-        CUDA_TRY(cudaFuncGetAttributes(&f, prompt_bf16_kernel<D>));
-        if ((f.numRegs + 7) / 8 * 8 * kPromptThreads < kPromptRegisters) return PHONON_CUDA_DEVICE_ERROR;
-        enough = true;
-    }
-    static std::atomic<uint64_t> configured{0};
-    CUDA_TRY(opt_in_smem(reinterpret_cast<const void*>(prompt_bf16_kernel<D>), Shape::kSmem, configured));
-    CUDA_TRY(launch_pdl(prompt_bf16_kernel<D>, dim3(grid), dim3(kPromptThreads), Shape::kSmem, s, q, k, v, p));
+// Kernels whose warps hand registers to one another: what they ask for has to
+// be what the launch has, or they would wait for good.
+int enough_registers(const void* kernel, int threads, int asked, std::atomic<bool>& known) {
+    if (known) return PHONON_CUDA_OK;
+    cudaFuncAttributes f{};
+    CUDA_TRY(cudaFuncGetAttributes(&f, kernel));
+    if ((f.numRegs + 7) / 8 * 8 * threads < asked) return PHONON_CUDA_DEVICE_ERROR;
+    known = true;
     return PHONON_CUDA_OK;
+}
+
+// Query heads of a K/V head share rows of a tile, and so its keys and values.
+int prompt_pack(PromptParams& p, int rows) {
+    const int group = static_cast<int>(p.group.d), pack = group <= 32 ? group : 1;
+    p.pack = kv8_divisor(static_cast<uint32_t>(pack));
+    p.tokens = rows / 128 * (128 / pack);
+    return pack;
 }
 
 template <int D, bool kBf16>
 int prompt_launch(PromptParams p, cudaStream_t s) {
-    if constexpr (kBf16) return prompt_launch_bf16<D>(p, s);
-    p.tokens = std::max(1, 64 / static_cast<int>(p.group.d));
+    static std::atomic<bool> enough{false};
+    static std::atomic<uint64_t> configured{0};
     unsigned grid = 0;
-    if (const int rc = prompt_grid(p, p.kv_heads, &grid)) return rc;
-    CUDA_TRY(launch_pdl(prompt_rows_kernel<D, kBf16>, dim3(grid), dim3(256), 0, s, p));
+    if constexpr (kBf16) {
+        using Shape = PromptShape<D>;
+        const void* kernel = reinterpret_cast<const void*>(prompt_bf16_kernel<D>);
+        const int pack = prompt_pack(p, 256);
+        if (const int rc = prompt_grid(p, p.heads / pack, &grid)) return rc;
+        if (const int rc = enough_registers(kernel, kPromptThreads, kPromptRegisters, enough)) return rc;
+        CUDA_TRY(opt_in_smem(kernel, Shape::kSmem, configured));
+        CUtensorMap q, k, v;
+        if (!make_rows_map(&q, p.q, p.rows, p.heads, D, p.q_stride, Shape::kBox, pack, 128 / pack) ||
+            !make_rows_map(&k, p.k, p.rows, p.kv_heads, D, p.k_stride, Shape::kBox, 1, kPromptKeys) ||
+            !make_rows_map(&v, p.v, p.rows, p.kv_heads, D, p.v_stride, Shape::kBox, 1, kPromptKeys))
+            return PHONON_CUDA_DEVICE_ERROR;
+        CUDA_TRY(launch_pdl(prompt_bf16_kernel<D>, dim3(grid), dim3(kPromptThreads), Shape::kSmem, s, q, k, v, p));
+    } else {
+        using Shape = PromptF32Shape<D>;
+        const void* kernel = reinterpret_cast<const void*>(prompt_f32_kernel<D>);
+        const int pack = prompt_pack(p, 128);
+        if (const int rc = prompt_grid(p, p.heads / pack, &grid)) return rc;
+        if (const int rc = enough_registers(kernel, kPromptF32Threads, kPromptF32Registers, enough)) return rc;
+        CUDA_TRY(opt_in_smem(kernel, Shape::kSmem, configured));
+        CUDA_TRY(launch_pdl(prompt_f32_kernel<D>, dim3(grid), dim3(kPromptF32Threads), Shape::kSmem, s, p));
+    }
     return PHONON_CUDA_OK;
 }
 

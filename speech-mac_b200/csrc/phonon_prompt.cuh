@@ -95,53 +95,6 @@ __device__ __forceinline__ PromptTile prompt_tile(const PromptParams& p, int slo
     return {s_tile[0], s_tile[1], s_tile[2], s_tile[3]};
 }
 
-// One row by a warp in fp32, position after position: D / 32 dims a lane.
-template <int D, bool kBf16>
-__device__ __forceinline__ void prompt_row(const PromptParams& p, const PromptTile& t, int position, int head, bool& finite) {
-    constexpr int kDims = D / 32;
-    const int lane = threadIdx.x & 31, kv_head = static_cast<int>(kv8_div(head, p.group));
-    auto load = [&](const void* base, size_t at, float (&x)[kDims]) {
-#pragma unroll
-        for (int d = 0; d < kDims; ++d) {
-            if constexpr (kBf16) x[d] = __uint_as_float(static_cast<uint32_t>(static_cast<const uint16_t*>(base)[at + d * 32 + lane]) << 16);
-            else x[d] = static_cast<const float*>(base)[at + d * 32 + lane];
-        }
-    };
-    float q[kDims], o[kDims], m = -INFINITY, l = 0.0f;
-    load(p.q, static_cast<size_t>(t.row0 + position) * p.q_stride + static_cast<size_t>(head) * D, q);
-#pragma unroll
-    for (int d = 0; d < kDims; ++d) o[d] = 0.0f;
-    for (int j = p.window ? max(0, position - p.window + 1) : 0; j <= position; ++j) {
-        float k[kDims], v[kDims], s = 0.0f;
-        load(p.k, static_cast<size_t>(t.row0 + j) * p.k_stride + static_cast<size_t>(kv_head) * D, k);
-        load(p.v, static_cast<size_t>(t.row0 + j) * p.v_stride + static_cast<size_t>(kv_head) * D, v);
-#pragma unroll
-        for (int d = 0; d < kDims; ++d) s = fmaf(q[d], k[d], s);
-#pragma unroll
-        for (int w = 16; w > 0; w >>= 1) s += __shfl_xor_sync(kFull, s, w);
-        s *= p.scale;
-        const float now = isnan(s) ? s : fmaxf(m, s);
-        const float by = m == now ? 1.0f : ex2(m - now), w = s == -INFINITY && now == -INFINITY ? 0.0f : ex2(s - now);
-        m = now;
-        l = fmaf(l, by, w);
-#pragma unroll
-        for (int d = 0; d < kDims; ++d) o[d] = fmaf(o[d], by, w * v[d]);
-    }
-    const size_t at = static_cast<size_t>(t.row0 + position) * p.out_stride + static_cast<size_t>(head) * D;
-#pragma unroll
-    for (int d = 0; d < kDims; ++d) {
-        const float x = __fdiv_rn(o[d], l);
-        if constexpr (kBf16) {
-            const __nv_bfloat16 b = __float2bfloat16(x);
-            static_cast<__nv_bfloat16*>(p.out)[at + d * 32 + lane] = b;
-            finite &= isfinite(__bfloat162float(b));
-        } else {
-            static_cast<float*>(p.out)[at + d * 32 + lane] = x;
-            finite &= isfinite(x);
-        }
-    }
-}
-
 // ------------------------------------------------- bf16 rows on tcgen05
 // A CTA has two row tiles of 128 rows (a row is a position and one of the
 // `pack` query heads that share its K/V head), each with a softmax of four
@@ -541,21 +494,393 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
     }
 }
 
-// One K/V head of a tile, a warp a row.
-template <int D, bool kBf16>
-__global__ void __launch_bounds__(256) prompt_rows_kernel(PromptParams p) {
+// ------------------------------------------------- fp32 rows on tcgen05
+// Every operand as three bf16 slices (8 bits each, the differences exact), and
+// a product as the six slice products that are above 2^-24 of it, the smallest
+// first: 6 times the matrix work, and fp32's precision. A CTA has one row tile
+// of 128 rows and 64 positions a turn:
+//
+//   warps 8-15  read k and v, and write their slices as matrix operands
+//   warp 4      issues S = q k^T a turn ahead, and P v
+//   warps 0-3   a row a thread: q times the softmax scale into TMEM (the A
+//               operand of S), S to weights, their slices back over S, and the
+//               sum of P v over the turns in registers (the tensor cores' own
+//               sum truncates: 24 truncations a turn stay near fp32's rounding,
+//               thousands would not)
+//
+// Bound by the tensor cores. Values that are not finite: as for bf16 rows; of
+// keys that are not, or would not be as bf16, the careful CTA computes the
+// scores one by one.
+constexpr int kPromptF32Threads = 512, kPromptF32Keys = 64;
+// A thread's registers in warps 0-3 and 4-15, together the launch's 128 each.
+constexpr int kPromptF32SoftmaxRegisters = 240, kPromptF32OtherRegisters = 88;
+constexpr int kPromptF32Registers = 128 * kPromptF32SoftmaxRegisters + 384 * kPromptF32OtherRegisters;
+
+template <int D>
+struct PromptF32Shape {
+    static constexpr int kBox = D < 64 ? D : 64, kBoxBytes = 2 * kBox, kBoxes = D / kBox;
+    static constexpr int kStages = D == 128 ? 2 : 3;
+    static constexpr int kPlane = kPromptF32Keys * D * 2;  // bytes of a slice of a turn's keys or values
+    static constexpr int kSmem = 1024 + 2 * kStages * 3 * kPlane;
+    static constexpr int kUnits = D / 32;  // of 8 elements a converting thread has, of a turn's keys and of its values
+};
+
+// The three slices of a pair, the first in the low half; exact but for the
+// last one's rounding.
+__device__ __forceinline__ void bf16x2_slices(float2 x, uint32_t (&w)[3]) {
+    w[0] = bf16x2_bits(x.x, x.y);
+    x = add2(x, make_float2(__uint_as_float(w[0] << 16 ^ 0x80000000u), __uint_as_float((w[0] & 0xffff0000u) ^ 0x80000000u)));
+    w[1] = bf16x2_bits(x.x, x.y);
+    x = add2(x, make_float2(__uint_as_float(w[1] << 16 ^ 0x80000000u), __uint_as_float((w[1] & 0xffff0000u) ^ 0x80000000u)));
+    w[2] = bf16x2_bits(x.x, x.y);
+}
+
+// Slices of a product, smallest first.
+__device__ __forceinline__ constexpr int prompt_slice_a(int i) { return i == 0 ? 2 : i == 1 || i == 3 ? 1 : 0; }
+__device__ __forceinline__ constexpr int prompt_slice_b(int i) { return i == 2 ? 2 : i == 1 || i == 4 ? 1 : 0; }
+
+constexpr float kBf16Most = 3.38953139e38f;  // the largest bf16
+
+template <int D>
+__global__ void __launch_bounds__(kPromptF32Threads, 1) prompt_f32_kernel(PromptParams p) {
+    using Shape = PromptF32Shape<D>;
+    constexpr int kStages = Shape::kStages, kPlane = Shape::kPlane, kBytes = Shape::kBoxBytes, kKeys = kPromptF32Keys, kUnits = Shape::kUnits;
+    constexpr uint32_t kTmemS = 3 * D / 2, kSCols = 96, kTmemO = kTmemS + 2 * kSCols;  // q's slices, S and the weights' slices twice, O
+    static_assert(kTmemO + D <= 512, "TMEM");
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ __align__(8) uint64_t s_bars[4 * kStages + 6];
+    __shared__ uint32_t s_tmem;
+    __shared__ int s_failed, s_dirty;
+    __shared__ unsigned long long s_bad[2][kStages];  // careful: which of a turn's keys, values are not finite
+    const uint32_t s_k = (smem_addr(smem_raw) + 1023) & ~1023u, s_v = s_k + kStages * 3 * kPlane;
+    const uint32_t k_full = smem_addr(s_bars), k_empty = k_full + 8 * kStages, v_full = k_empty + 8 * kStages, v_empty = v_full + 8 * kStages;
+    const uint32_t s_full = v_empty + 8 * kStages, p_full = s_full + 16, o_full = p_full + 8, q_full = o_full + 8, idle = q_full + 8;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const auto init = [&](bool again) {  // one thread
+        const auto set = [&](uint32_t bar, uint32_t count) {
+            if (again) asm volatile("mbarrier.inval.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
+            mbar_init(bar, count);
+        };
+        for (int s = 0; s < kStages; ++s) {
+            set(k_full + 8 * s, 8);
+            set(v_full + 8 * s, 8);
+            set(k_empty + 8 * s, 1);
+            set(v_empty + 8 * s, 1);
+        }
+        set(s_full, 1);
+        set(s_full + 8, 1);
+        set(p_full, 4);
+        set(o_full, 1);
+        set(q_full, 4);
+        set(idle, 1);
+        s_failed = s_dirty = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    };
+    if (threadIdx.x == 0) init(false);
     pdl_wait();
     pdl_trigger();
-    const int slot = static_cast<int>(kv8_div(blockIdx.x, p.by_heads)), kv_head = static_cast<int>(blockIdx.x - slot * p.by_heads.d);
-    const PromptTile t = prompt_tile<256>(p, slot, blockIdx.x == gridDim.x - 1);
+    const int slot = static_cast<int>(kv8_div(blockIdx.x, p.by_heads)), part = static_cast<int>(blockIdx.x - slot * p.by_heads.d);
+    const PromptTile t = prompt_tile<kPromptF32Threads>(p, slot, blockIdx.x == gridDim.x - 1);
     if (t.index < 0) return;
-    const int rows = min(p.tokens, t.length - t.first) * static_cast<int>(p.group.d);
-    bool finite = true;
-    for (int r = threadIdx.x >> 5; r < rows; r += 8) {
-        const int at = static_cast<int>(kv8_div(r, p.group));
-        prompt_row<D, kBf16>(p, t, t.first + at, kv_head * p.group.d + r - at * p.group.d, finite);
+    const int pack = static_cast<int>(p.pack.d), head0 = part * pack, kv_head = static_cast<int>(kv8_div(head0, p.group));
+    const int end = min(t.length, t.first + p.tokens), key0 = p.window ? max(0, t.first - p.window + 1) : 0;
+    const int turns = (end - key0 + kKeys - 1) / kKeys;
+    if (warp == 4) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_addr(&s_tmem)) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
-    if (!__all_sync(kFull, finite) && (threadIdx.x & 31) == 0) prompt_flag(p, t.index, kStatusNonFinite);
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    const uint32_t tmem = s_tmem;
+    const auto wait = [&](uint32_t bar, int use) {
+        const bool ok = mbar_wait(bar, use & 1, nullptr, &s_failed);
+        __syncwarp();
+        return __all_sync(kFull, ok);
+    };
+    bool careful = false;
+    const auto sync = [] { asm volatile("bar.sync 1, %0;" ::"n"(kPromptF32Threads) : "memory"); };
+    // Every warp, at its end: whether the CTA starts over.
+    const auto again = [&] {
+        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+        sync();
+        const bool redo = !careful && s_dirty && !s_failed;
+        if (!redo) return false;
+        sync();
+        if (threadIdx.x == 0) init(true);
+        sync();
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        return careful = true;
+    };
+    if (warp >= 4) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPromptF32OtherRegisters));
+        if (warp >= 8) do {
+            // A warp writes whole rows' pieces: unit u of a turn's keys (values) is 8 dims of a row.
+            constexpr int kChunks = D / 8;
+            const int u0 = (warp - 8) * 32 + lane;
+            const float* base[2] = {static_cast<const float*>(p.k) + static_cast<size_t>(t.row0 + key0) * p.k_stride + kv_head * D,
+                                    static_cast<const float*>(p.v) + static_cast<size_t>(t.row0 + key0) * p.v_stride + kv_head * D};
+            const auto load = [&](float4 (&x)[kUnits][2], int which, int j) {
+#pragma unroll
+                for (int i = 0; i < kUnits; ++i) {
+                    const int u = u0 + 256 * i, row = j * kKeys + u / kChunks;
+                    const float* at = base[which] + static_cast<size_t>(row) * (which ? p.v_stride : p.k_stride) + u % kChunks * 8;
+                    const bool in = j < turns && key0 + row < end;  // what follows the prompt does not count: zeros
+                    x[i][0] = in ? *reinterpret_cast<const float4*>(at) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                    x[i][1] = in ? *reinterpret_cast<const float4*>(at + 4) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                }
+            };
+            const auto put = [&](float4 (&x)[kUnits][2], int which, int j) {
+                const int s = j % kStages;
+                bool ok = j < kStages || wait((which ? v_empty : k_empty) + 8 * s, j / kStages - 1);
+                if (careful) {  // (P v of the stage's last turn is behind what its rows read of s_bad)
+                    if (j >= kStages) ok &= wait(v_empty + 8 * s, j / kStages - 1);
+                    if (u0 == 0) s_bad[which][s] = 0;
+                    asm volatile("bar.sync 2, 256;" ::: "memory");
+                }
+                if (!ok) return;  // (every warp goes on to the last turn: they meet above)
+#pragma unroll
+                for (int i = 0; i < kUnits; ++i) {
+                    const int u = u0 + 256 * i, row = u / kChunks, chunk = u % kChunks;
+                    uint32_t w[4][3];
+                    float* f = &x[i][0].x;
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) bf16x2_slices(make_float2(f[2 * k], f[2 * k + 1]), w[k]);
+                    if (careful) {
+                        bool bad = false;
+#pragma unroll 1
+                        for (int k = 0; k < 8; ++k) {
+                            const float v = k < 4 ? k < 2 ? k ? x[i][0].y : x[i][0].x : k == 2 ? x[i][0].z : x[i][0].w
+                                                  : k < 6 ? k == 4 ? x[i][1].x : x[i][1].y : k == 6 ? x[i][1].z : x[i][1].w;
+                            bad |= !(fabsf(v) <= kBf16Most) && (!which || !isfinite(v));
+                        }
+                        if (bad) atomicOr(&s_bad[which][s], 1ull << row);
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            // numbers between the largest bf16 and the largest float keep their value
+                            float2 y = make_float2(f[2 * k], f[2 * k + 1]);
+                            if (!isfinite(y.x)) y.x = 0.0f;
+                            if (!isfinite(y.y)) y.y = 0.0f;
+                            const float2 top = make_float2(fminf(fmaxf(y.x, -kBf16Most), kBf16Most), fminf(fmaxf(y.y, -kBf16Most), kBf16Most));
+                            const bool far = top.x != y.x || top.y != y.y;
+                            bf16x2_slices(far ? top : y, w[k]);
+                            if (far) {
+                                const float2 rest = make_float2(y.x - __uint_as_float(w[k][0] << 16), y.y - __uint_as_float(w[k][0] & 0xffff0000u));
+                                w[k][1] = bf16x2_bits(rest.x, rest.y);
+                                w[k][2] = bf16x2_bits(rest.x - __uint_as_float(w[k][1] << 16), rest.y - __uint_as_float(w[k][1] & 0xffff0000u));
+                            }
+                        }
+                    }
+                    const uint32_t at = (which ? s_v : s_k) + s * 3 * kPlane + chunk / (kBytes / 16) * kKeys * kBytes + row * kBytes +
+                                        ((chunk % (kBytes / 16)) ^ (kBytes == 128 ? row & 7 : row >> 1 & 3)) * 16;
+#pragma unroll
+                    for (int c = 0; c < 3; ++c) kv8_put16(at + c * kPlane, w[0][c], w[1][c], w[2][c], w[3][c]);
+                }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) mbar_arrive((which ? v_full : k_full) + 8 * s);
+            };
+            float4 a[kUnits][2], b[kUnits][2];
+            load(a, 0, 0);
+            for (int j = 0; j < turns; ++j) {
+                load(b, 1, j);
+                put(a, 0, j);
+                load(a, 0, j + 1);
+                put(b, 1, j);
+            }
+        } while (again());
+        else if (warp == 4) do {
+            constexpr uint32_t idesc_s = umma_idesc_bf16(128, kKeys), idesc_o = umma_idesc_bf16(128, D) | kUmmaBMnMajor;
+            uint32_t leader;
+            asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.b32 %0, 1, 0, p;\n\t}" : "=r"(leader));
+            const auto commit = [&](uint32_t bar) {
+                if (leader) umma_commit(bar);
+            };
+            bool ok = wait(q_full, 0);
+            const auto score = [&](int j) {
+                const int s = j % kStages;
+                if (!ok || !(ok = wait(k_full + 8 * s, j / kStages))) return;
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+#pragma unroll
+                for (int i = 0; i < 6; ++i)
+#pragma unroll
+                    for (int k = 0; k < D / 16; ++k)
+                        umma_half<true>(leader, tmem + kTmemS + (j & 1) * kSCols, tmem + prompt_slice_a(i) * (D / 2) + k * 8,
+                                        umma_desc_rows<kBytes>(s_k + (s * 3 + prompt_slice_b(i)) * kPlane + k / (kBytes / 32) * kKeys * kBytes +
+                                                               k % (kBytes / 32) * 32),
+                                        idesc_s, (i | k) != 0);
+                commit(s_full + 8 * (j & 1));
+                commit(k_empty + 8 * s);
+            };
+            score(0);
+            for (int j = 0; ok && j < turns; ++j) {
+                if (j + 1 < turns) score(j + 1);
+                const int s = j % kStages;
+                if (!ok || !(ok = wait(v_full + 8 * s, j / kStages) && wait(p_full, j))) break;
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+#pragma unroll
+                for (int i = 0; i < 6; ++i)
+#pragma unroll
+                    for (int k = 0; k < kKeys / 16; ++k)
+                        umma_half<true>(leader, tmem + kTmemO, tmem + kTmemS + (j & 1) * kSCols + prompt_slice_a(i) * (kKeys / 2) + k * 8,
+                                        umma_desc_rows<kBytes>(s_v + (s * 3 + prompt_slice_b(i)) * kPlane + k * 16 * kBytes, kKeys * kBytes), idesc_o,
+                                        (i | k) != 0);
+                commit(o_full);
+                commit(v_empty + 8 * s);
+            }
+            commit(idle);  // no product is on its way when the CTA gives its memory back
+            mbar_settle(idle, 0);
+            __syncwarp();
+        } while (again());
+        else do {
+        } while (again());
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kPromptF32SoftmaxRegisters));
+        const int r = threadIdx.x, at = static_cast<int>(kv8_div(r, p.pack)), position = t.first + at;
+        const bool mine = at < p.tokens && position < end;
+        const int head = head0 + r - at * pack;
+        const uint32_t lanes = tmem + (static_cast<uint32_t>(warp * 32) << 16);
+        const float* q = static_cast<const float*>(p.q) + static_cast<size_t>(t.row0 + position) * p.q_stride + static_cast<size_t>(head) * D;
+        float o[D];
+        bool good = true;
+        do {
+#pragma unroll 1
+            for (int c = 0; c < D; c += 16) {
+                uint32_t w[3][8];
+#pragma unroll
+                for (int k = 0; k < 8; k += 2) {
+                    const float4 x = mine ? *reinterpret_cast<const float4*>(q + c + 2 * k) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        uint32_t three[3];
+                        bf16x2_slices(h ? make_float2(x.z * p.scale, x.w * p.scale) : make_float2(x.x * p.scale, x.y * p.scale), three);
+                        w[0][k + h] = three[0], w[1][k + h] = three[1], w[2][k + h] = three[2];
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < 3; ++i) tmem_store8(lanes + i * (D / 2) + c / 2, w[i]);
+            }
+            asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) mbar_arrive(q_full);
+#pragma unroll
+            for (int k = 0; k < D; ++k) o[k] = 0.0f;
+            float m = -INFINITY, l = 0.0f, shrink = 1.0f;
+            const auto add_output = [&](int j) {
+                wait(o_full, j);
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                const float2 by = make_float2(shrink, shrink);
+#pragma unroll
+                for (int c = 0; c < D; c += 32) {
+                    float x[32];
+                    tmem_start(lanes + kTmemO + c, x);
+                    tmem_arrived(x);
+#pragma unroll
+                    for (int k = 0; k < 32; k += 2) {
+                        const float2 z = fma2(make_float2(o[c + k], o[c + k + 1]), by, make_float2(x[k], x[k + 1]));
+                        o[c + k] = z.x;
+                        o[c + k + 1] = z.y;
+                    }
+                }
+            };
+            for (int j = 0; j < turns; ++j) {
+                const uint32_t at_s = lanes + kTmemS + (j & 1) * kSCols;
+                wait(s_full + 8 * (j & 1), j >> 1);
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                float s[2][32];
+                tmem_start(at_s, s[0]);
+                tmem_start(at_s + 32, s[1]);
+                tmem_arrived(s[0]);
+                tmem_arrived(s[1]);
+                const int key = key0 + j * kKeys;
+                if (careful) {
+                    wait(k_full + 8 * (j % kStages), j / kStages);
+                    wait(v_full + 8 * (j % kStages), j / kStages);
+                    const unsigned long long seen = prompt_seen(position, p.window, key) |
+                                                    static_cast<unsigned long long>(prompt_seen(position, p.window, key + 32)) << 32;
+                    if (mine && s_bad[1][j % kStages] & seen) l = __int_as_float(0x7fc00000);
+                    for (unsigned long long left = mine ? s_bad[0][j % kStages] & seen : 0; left; left &= left - 1) {
+                        const int of = __ffsll(static_cast<long long>(left)) - 1;
+                        const float* k_row = static_cast<const float*>(p.k) + static_cast<size_t>(t.row0 + key + of) * p.k_stride + kv_head * D;
+                        float dot = 0.0f;
+                        for (int d = 0; d < D; ++d) dot = fmaf(q[d] * p.scale, k_row[d], dot);
+#pragma unroll
+                        for (int k = 0; k < 64; ++k) s[k / 32][k % 32] = k == of ? dot : s[k / 32][k % 32];
+                    }
+                    __syncwarp();
+                }
+                if (key + kKeys - 1 > t.first || (p.window && key <= end - 1 - p.window)) {  // not all of it by every row
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) {
+                        const uint32_t bits = prompt_seen(position, p.window, key + 32 * c);
+#pragma unroll
+                        for (int k = 0; k < 32; ++k) s[c][k] = bits >> k & 1 ? s[c][k] : -INFINITY;
+                    }
+                }
+                float top[2];
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    top[c] = fmaxf(s[c][0], s[c][1]);
+#pragma unroll
+                    for (int k = 2; k < 32; k += 2) top[c] = max3(top[c], s[c][k], s[c][k + 1]);
+                }
+                const float now = max3(m, top[0], top[1]), c = m == now ? 1.0f : ex2(m - now);
+                m = now;
+                l *= c;
+                const float from = now == -INFINITY ? 0.0f : -now;  // nothing seen yet: weights 2^-inf
+                float2 sum = make_float2(0.0f, 0.0f);
+#pragma unroll
+                for (int h = 0; h < 4; ++h) {
+                    uint32_t w[3][8];
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) {
+                        const float* x = &s[h / 2][16 * (h % 2) + 2 * k];
+                        const float2 z = add2(make_float2(x[0], x[1]), make_float2(from, from));
+                        const float2 e = make_float2(ex2(z.x), ex2(z.y));
+                        sum = add2(sum, e);
+                        uint32_t three[3];
+                        bf16x2_slices(e, three);
+                        w[0][k] = three[0], w[1][k] = three[1], w[2][k] = three[2];
+                    }
+#pragma unroll
+                    for (int i = 0; i < 3; ++i) tmem_store8(at_s + i * (kKeys / 2) + h * 8, w[i]);
+                }
+                l += sum.x + sum.y;
+                if (j) add_output(j - 1);
+                shrink = c;
+                asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+                asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) mbar_arrive(p_full);
+            }
+            add_output(turns - 1);
+            const float inverse = *static_cast<volatile int*>(&s_failed) ? __int_as_float(0x7fc00000) : __fdiv_rn(1.0f, l);
+            float clean = 0.0f;  // NaN once an output is not finite
+#pragma unroll
+            for (int k = 0; k < D; ++k) {
+                o[k] *= inverse;
+                clean = fmaf(o[k], 0.0f, clean);
+            }
+            good = !mine || clean == 0.0f;
+            if (!good) s_dirty = 1;
+            __syncwarp();
+        } while (again());
+        if (mine) {
+            float4* to = reinterpret_cast<float4*>(static_cast<float*>(p.out) + static_cast<size_t>(t.row0 + position) * p.out_stride +
+                                                   static_cast<size_t>(head) * D);
+#pragma unroll
+            for (int k = 0; k < D / 4; ++k) to[k] = make_float4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
+            if (!good) prompt_flag(p, t.index, s_failed ? kStatusDevice : kStatusNonFinite);
+        }
+    }
+    __syncwarp();
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    if (warp == 4) {
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+    }
 }
 
 }  // namespace phonon
