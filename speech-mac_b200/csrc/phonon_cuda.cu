@@ -4789,22 +4789,33 @@ int i8_rows_launch(const I8Params& p, cudaStream_t s) {
     return PHONON_CUDA_OK;
 }
 
-template <int kN, bool kBf16>
+// Maps of the rows in boxes of 128 and of the weights in boxes of box_w, 128 bytes of depth each.
+bool i8_maps(const I8Params& p, uint32_t box_w, CUtensorMap* x, CUtensorMap* w) {
+    const auto map = [&](CUtensorMap* m, const int8_t* base, int rows, long long stride, uint32_t box) {
+        return make_map_2d(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, base, static_cast<uint64_t>(rows), static_cast<uint64_t>(p.depth),
+                           static_cast<uint64_t>(stride), kGemmKTile, box);
+    };
+    return map(x, p.x, p.rows, p.x_stride, 128) && map(w, p.w, p.channels, p.w_stride, box_w);
+}
+
+// kN channels a tile; kPair: 256 x 256 by pairs of CTAs.
+template <int kN, bool kPair, bool kBf16>
 int i8_tiles_launch(I8Params p, int sms, cudaStream_t s) {
     static std::atomic<uint64_t> configured{0};
-    auto kernel = i8_product_kernel<kN, kBf16>;
-    constexpr int smem = i8_smem<kN>();
-    CUDA_TRY(opt_in_smem(reinterpret_cast<const void*>(kernel), smem, configured));
+    const auto kernel = [] {
+        if constexpr (kPair) return i8_pair_kernel<kBf16>;
+        else return i8_product_kernel<kN, kBf16>;
+    }();
+    constexpr int rows = kPair ? 256 : 128, smem = kPair ? kI8PairSmem : i8_smem<kN>();
     CUtensorMap tx, tw;
-    const uint64_t depth = static_cast<uint64_t>(p.depth);
-    if (!make_map_2d(&tx, CU_TENSOR_MAP_DATA_TYPE_UINT8, p.x, static_cast<uint64_t>(p.rows), depth, static_cast<uint64_t>(p.x_stride), 128, 128) ||
-        !make_map_2d(&tw, CU_TENSOR_MAP_DATA_TYPE_UINT8, p.w, static_cast<uint64_t>(p.channels), depth, static_cast<uint64_t>(p.w_stride), 128, kN))
-        return PHONON_CUDA_DEVICE_ERROR;
-    p.tiles_m = (p.rows + 127) / 128;
+    if (!i8_maps(p, kPair ? 128 : kN, &tx, &tw)) return PHONON_CUDA_DEVICE_ERROR;
+    CUDA_TRY(opt_in_smem(reinterpret_cast<const void*>(kernel), smem, configured));
+    p.tiles_m = (p.rows + rows - 1) / rows;
     p.tiles_n = (p.channels + kN - 1) / kN;
     const long long tiles = static_cast<long long>(p.tiles_m) * p.tiles_n;
-    if (tiles > (1 << 30)) return PHONON_CUDA_CAPACITY;
-    CUDA_TRY(launch_pdl(kernel, dim3(static_cast<unsigned>(std::min<long long>(tiles, sms))), dim3(kI8Threads), smem, s, tx, tw, p));
+    if (tiles > (1 << 26)) return PHONON_CUDA_CAPACITY;
+    const unsigned grid = static_cast<unsigned>(kPair ? 2 * std::min<long long>(tiles, sms / 2) : std::min<long long>(tiles, sms));
+    CUDA_TRY(launch_pdl(kernel, dim3(grid), dim3(kI8Threads), smem, s, tx, tw, p));
     return PHONON_CUDA_OK;
 }
 
@@ -4814,9 +4825,10 @@ int i8_product(const I8Params& p, int sms, cudaStream_t s) {
     if (p.rows <= 16) return i8_rows_launch<2, kBf16>(p, s);
     if (p.rows <= 32) return i8_rows_launch<4, kBf16>(p, s);
     const long long tiles_m = (p.rows + 127) / 128;
-    if (tiles_m * ((p.channels + 255) / 256) >= sms) return i8_tiles_launch<256, kBf16>(p, sms, s);
-    if (tiles_m * ((p.channels + 127) / 128) >= sms) return i8_tiles_launch<128, kBf16>(p, sms, s);
-    return i8_tiles_launch<64, kBf16>(p, sms, s);
+    if ((p.rows + 255) / 256 * ((p.channels + 255ll) / 256) >= sms / 2) return i8_tiles_launch<256, true, kBf16>(p, sms, s);
+    if (tiles_m * ((p.channels + 255) / 256) >= sms) return i8_tiles_launch<256, false, kBf16>(p, sms, s);
+    if (tiles_m * ((p.channels + 127) / 128) >= sms) return i8_tiles_launch<128, false, kBf16>(p, sms, s);
+    return i8_tiles_launch<64, false, kBf16>(p, sms, s);
 }
 
 }  // namespace

@@ -207,17 +207,130 @@ __device__ __forceinline__ void mbar_settle(uint32_t bar, uint32_t parity) {
     for (const long long since = clock64(); !mbar_test(bar, parity) && clock64() - since < kWaitBudgetCycles;) __nanosleep(20);
 }
 
-// Many rows: tiles of 128 rows x kN channels on the tcgen05 tensor cores, one
-// CTA an SM that takes tiles in turn. Warp 0 brings 128 bytes of depth a stage
-// by TMA, warp 1 issues the products into one of two accumulators in TMEM, and
-// warps 2-5 take the other one out, a row a thread.
+// Many rows: tiles on the tcgen05 tensor cores, a CTA (or a pair of them) an SM
+// that takes tiles in turn. Warp 0 brings 128 bytes of depth a stage by TMA,
+// warp 1 issues the products into one of two accumulators in TMEM, and warps
+// 2-5 take the other one out, a row a thread.
+//
+// i8_product_kernel: 128 rows x kN channels a CTA. i8_pair_kernel: 256 x 256 a
+// pair of CTAs (cta_group::2): each has 128 of the rows and 128 of the
+// channels in its shared memory and the products read both, so that a CTA's
+// copies are 32 KB for what takes 48 KB alone.
 constexpr int kI8Threads = 192;
+constexpr int kI8Staging = 4 * 32 * 128;  // bytes: 32 rows of 128 for each of warps 2-5
 
 template <int kN>
 __host__ __device__ constexpr int i8_stages() { return kN == 256 ? 4 : kN == 128 ? 6 : 8; }
 
 template <int kN>
-__host__ __device__ constexpr int i8_smem() { return 1024 + i8_stages<kN>() * (128 + kN) * 128; }
+__host__ __device__ constexpr int i8_smem() { return 1024 + i8_stages<kN>() * (128 + kN) * 128 + kI8Staging; }
+
+constexpr int kI8PairStages = 6;
+constexpr int kI8PairSmem = 1024 + kI8PairStages * 256 * 128 + kI8Staging;
+
+// Tiles in bands of kBand row tiles, so that the CTAs at work share rows and weights in the L2.
+__device__ __forceinline__ void i8_place(const I8Params& p, int tile, int& m, int& n) {
+    constexpr int kBand = 16;
+    const int band = tile / (kBand * p.tiles_n), in = tile - band * kBand * p.tiles_n;
+    const int high = min(kBand, p.tiles_m - band * kBand);
+    n = in / high;
+    m = band * kBand + in - n * high;
+}
+
+// kN accumulator columns of a warp's 32 rows (row0 + lane; channels from n0 on)
+// to y, 128 bytes of every row at a time through `staging`, so that a store
+// has whole lines whatever the row stride; `taken` is called once the columns
+// have left TMEM. scale, bias: the channels'. failed: NaN in their place.
+template <int kN, bool kBf16, typename Taken>
+__device__ __forceinline__ void i8_take(const I8Params& p, uint32_t tmem, uint32_t staging, int row0, int n0, const float* scale,
+                                        const float* bias, bool failed, const Taken& taken) {
+    constexpr int kCols = kBf16 ? 64 : 32, kSize = kBf16 ? 2 : 4;  // 128 bytes
+    const int lane = threadIdx.x & 31, row = row0 + lane;
+    const bool wide = p.y_stride * kSize % 16 == 0;
+    const float xs = failed ? __int_as_float(0x7fc00000) : row < p.rows ? p.x_scales[row] : 0.0f;
+    float finite = 0.0f;  // NaN once a value is not
+#pragma unroll 1
+    for (int c = 0; c < kN; c += kCols) {
+        uint32_t out[32];
+#pragma unroll
+        for (int h = 0; h < kCols / 32; ++h) {
+            uint32_t r[32];
+            tmem_load32(tmem + c + 32 * h, r);
+#pragma unroll
+            for (int k = 0; k < 32; k += 2) {
+                float v[2];
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const int at = c + 32 * h + k + i;
+                    v[i] = i8_value(static_cast<int>(r[k + i]), xs, scale[at], bias[at]);
+                }
+                if constexpr (kBf16) {
+                    const __nv_bfloat162 b = __floats2bfloat162_rn(v[0], v[1]);
+                    out[16 * h + k / 2] = *reinterpret_cast<const uint32_t*>(&b);
+                    v[0] = __low2float(b);
+                    v[1] = __high2float(b);
+                } else {
+                    out[k] = __float_as_uint(v[0]);
+                    out[k + 1] = __float_as_uint(v[1]);
+                }
+                finite = fmaf(v[0], 0.0f, fmaf(v[1], 0.0f, finite));  // (channels behind the last: sums 0, scale and bias 0)
+            }
+        }
+        if (c + kCols >= kN) taken();
+#pragma unroll
+        for (int k = 0; k < 8; ++k) kv8_put16(staging + lane * 128 + ((k ^ (lane & 7)) * 16), out[4 * k], out[4 * k + 1], out[4 * k + 2], out[4 * k + 3]);
+        __syncwarp();
+        if (wide && n0 + c + kCols <= p.channels) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int r = 4 * i + (lane >> 3);
+                uint4 w;
+                asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w)
+                             : "r"(staging + r * 128 + (((lane & 7) ^ (r & 7)) * 16)));
+                if (row0 + r < p.rows)
+                    *reinterpret_cast<uint4*>(static_cast<uint8_t*>(p.y) + (static_cast<size_t>(row0 + r) * p.y_stride + n0 + c) * kSize + (lane & 7) * 16) = w;
+            }
+        } else {
+            const int rows = min(32, p.rows - row0), cols = p.channels - n0 - c;
+#pragma unroll 4
+            for (int r = 0; r < rows; ++r)
+#pragma unroll
+                for (int h = 0; h < kCols / 32; ++h) {
+                    const int at = (32 * h + lane) * kSize;
+                    const uint32_t from = staging + r * 128 + ((at >> 4 ^ (r & 7)) * 16) + (at & 15);
+                    const size_t to = static_cast<size_t>(row0 + r) * p.y_stride + n0 + c + 32 * h + lane;
+                    if (32 * h + lane >= cols) continue;
+                    if constexpr (kBf16) {
+                        uint16_t w;
+                        asm volatile("ld.shared.b16 %0, [%1];" : "=h"(w) : "r"(from));
+                        static_cast<uint16_t*>(p.y)[to] = w;
+                    } else {
+                        uint32_t w;
+                        asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w) : "r"(from));
+                        static_cast<uint32_t*>(p.y)[to] = w;
+                    }
+                }
+        }
+        __syncwarp();
+    }
+    if (row < p.rows && finite != 0.0f) {
+        if (failed) {
+            if (p.status) atomicMax(p.status + row, kStatusDevice);
+        } else {
+            flag_nonfinite(p.status, row);
+        }
+    }
+}
+
+// The channels' scales and biases of a tile, by the threads of warps 2-5.
+template <int kN>
+__device__ __forceinline__ void i8_channels(const I8Params& p, int n0, float* scale, float* bias) {
+    for (int c = threadIdx.x - 64; c < kN; c += 128) {
+        scale[c] = n0 + c < p.channels ? p.w_scales[n0 + c] : 0.0f;
+        bias[c] = p.bias && n0 + c < p.channels ? p.bias[n0 + c] : 0.0f;
+    }
+    asm volatile("bar.sync 1, 128;" ::: "memory");
+}
 
 template <int kN, bool kBf16>
 __global__ void __launch_bounds__(kI8Threads, 1)
@@ -253,14 +366,6 @@ __global__ void __launch_bounds__(kI8Threads, 1)
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const uint32_t tmem = s_tmem;
     const int nk = (p.depth + 127) / 128, tiles = p.tiles_m * p.tiles_n;
-    // Tiles in bands of kBand row tiles, so that the CTAs at work share rows and weights in the L2.
-    constexpr int kBand = 16;
-    auto place = [&](int tile, int& m, int& n) {
-        const int band = tile / (kBand * p.tiles_n), in = tile - band * kBand * p.tiles_n;
-        const int high = min(kBand, p.tiles_m - band * kBand);
-        n = in / high;
-        m = band * kBand + in - n * high;
-    };
     pdl_wait();
     pdl_trigger();
     if (warp == 0 && lane == 0) {
@@ -268,7 +373,7 @@ __global__ void __launch_bounds__(kI8Threads, 1)
         bool ok = true;
         for (int tile = blockIdx.x; ok && tile < tiles; tile += gridDim.x) {
             int m, n;
-            place(tile, m, n);
+            i8_place(p, tile, m, n);
             for (int k = 0; k < nk; ++k, ++it) {
                 const int s = it % kStages;
                 if (it >= kStages && !(ok = mbar_wait(empty + 8 * s, (it / kStages - 1) & 1, nullptr, &s_failed))) break;
@@ -302,54 +407,23 @@ __global__ void __launch_bounds__(kI8Threads, 1)
         umma_commit(idle);  // nor is a product
         mbar_settle(idle, 0);
     } else if (warp >= 2) {
-        const int quarter = warp & 3, thread = (warp - 2) * 32 + lane;
+        const int quarter = warp & 3;
         int turn = 0;
-        const bool wide = p.y_stride % (kBf16 ? 8 : 4) == 0;
         for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x, ++turn) {
             int m, n;
-            place(tile, m, n);
-            const int a = turn & 1, n0 = n * kN, row = m * 128 + quarter * 32 + lane;
-            for (int c = thread; c < kN; c += 128) {
-                s_scale[a][c] = n0 + c < p.channels ? p.w_scales[n0 + c] : 0.0f;
-                s_bias[a][c] = p.bias && n0 + c < p.channels ? p.bias[n0 + c] : 0.0f;
-            }
-            float xs = row < p.rows ? p.x_scales[row] : 0.0f;
-            asm volatile("bar.sync 1, 128;" ::: "memory");
+            i8_place(p, tile, m, n);
+            const int a = turn & 1;
+            i8_channels<kN>(p, n * kN, s_scale[a], s_bias[a]);
             mbar_wait(done + 8 * a, (turn / 2) & 1, nullptr, &s_failed);
             __syncwarp();
-            const bool failed = *static_cast<volatile int*>(&s_failed);
-            if (failed) xs = __int_as_float(0x7fc00000);
+            const bool failed = __any_sync(kFull, *static_cast<volatile int*>(&s_failed));
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            const size_t out = static_cast<size_t>(row) * p.y_stride + n0;
-            float finite = 0.0f;
-#pragma unroll 1
-            for (int c = 0; c < kN; c += 32) {
-                uint32_t r[32];
-                tmem_load32(tmem + a * kN + c + (static_cast<uint32_t>(quarter * 32) << 16), r);
-                if (c + 32 >= kN) {
-                    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(drained + 8 * a);
-                }
-                if (row >= p.rows || n0 + c >= p.channels) continue;
-                float v[32];
-#pragma unroll
-                for (int k = 0; k < 32; ++k) {
-                    v[k] = i8_value(static_cast<int>(r[k]), xs, s_scale[a][c + k], s_bias[a][c + k]);
-                    if constexpr (kBf16) v[k] = __bfloat162float(__float2bfloat16(v[k]));
-                    if (n0 + c + k < p.channels) finite = fmaf(v[k], 0.0f, finite);
-                }
-                if (wide && n0 + c + 32 <= p.channels) {
-#pragma unroll
-                    for (int k = 0; k < 32; k += 4) store_row4<kBf16>(p.y, out + c + k, make_float4(v[k], v[k + 1], v[k + 2], v[k + 3]));
-                } else {
-#pragma unroll
-                    for (int k = 0; k < 32; ++k)
-                        if (n0 + c + k < p.channels) i8_store<kBf16>(p.y, out + c + k, v[k]);
-                }
-            }
-            if (row < p.rows && finite != 0.0f) flag_nonfinite(p.status, row);
-            if (failed && row < p.rows && p.status) atomicMax(p.status + row, kStatusDevice);
+            i8_take<kN, kBf16>(p, tmem + a * kN + (static_cast<uint32_t>(quarter * 32) << 16), stages + kStages * kStageBytes + (warp - 2) * 4096,
+                               m * 128 + quarter * 32, n * kN, s_scale[a], s_bias[a], failed, [&] {
+                                   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                                   __syncwarp();
+                                   if (lane == 0) mbar_arrive(drained + 8 * a);
+                               });
         }
     }
     __syncwarp();
@@ -358,6 +432,167 @@ __global__ void __launch_bounds__(kI8Threads, 1)
     if (warp == 1) {
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(2 * kN) : "memory");
+    }
+}
+
+__device__ __forceinline__ uint32_t cluster_addr(uint32_t addr, uint32_t rank) {  // the same place in a CTA of the cluster
+    uint32_t a;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(addr), "r"(rank));
+    return a;
+}
+
+__device__ __forceinline__ void cluster_meet() {
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+// mbar_wait for a barrier that the cluster's other CTA arrives at, too.
+__device__ __forceinline__ bool mbar_wait_cluster(uint32_t bar, uint32_t parity, volatile int* cta_failed) {
+    const long long start = clock64();
+    while (true) {
+        uint32_t done;
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+            "selp.b32 %0, 1, 0, p;\n\t}"
+            : "=r"(done)
+            : "r"(bar), "r"(parity)
+            : "memory");
+        if (done) return true;
+        if (*cta_failed) return false;
+        if (clock64() - start > kWaitBudgetCycles) {
+            *cta_failed = 1;
+            return false;
+        }
+    }
+}
+
+template <bool kBf16>
+__global__ void __launch_bounds__(kI8Threads, 1) __cluster_dims__(2, 1, 1)
+    i8_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_w, I8Params p) {
+    constexpr int kN = 256, kStages = kI8PairStages, kStageBytes = 256 * 128;
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ __align__(8) uint64_t s_bars[2 * kStages + 5];
+    __shared__ uint32_t s_tmem;
+    __shared__ int s_failed;
+    __shared__ __align__(16) float s_scale[2][kN], s_bias[2][kN];
+    const uint32_t stages = (smem_addr(smem_raw) + 1023) & ~1023u;
+    const uint32_t full = smem_addr(s_bars), empty = full + 8 * kStages, done = empty + 8 * kStages, drained = done + 16, idle = drained + 16;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = blockIdx.x & 1;  // 0 leads: its barriers count both CTAs' copies, its thread issues the products
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < kStages; ++s) {
+            mbar_init(full + 8 * s, 1);
+            mbar_init(empty + 8 * s, 1);
+        }
+        for (int a = 0; a < 2; ++a) {
+            mbar_init(done + 8 * a, 1);
+            mbar_init(drained + 8 * a, 8);
+        }
+        mbar_init(idle, 1);
+        s_failed = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&s_tmem)), "n"(2 * kN) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    cluster_meet();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    const uint32_t tmem = s_tmem;
+    const int nk = (p.depth + 127) / 128, tiles = p.tiles_m * p.tiles_n, first = blockIdx.x >> 1, step = gridDim.x >> 1;
+    pdl_wait();
+    pdl_trigger();
+    if (warp == 0 && lane == 0) {
+        const uint32_t lead_full = cluster_addr(full, 0);
+        int it = 0;
+        bool ok = true;
+        for (int tile = first; ok && tile < tiles; tile += step) {
+            int m, n;
+            i8_place(p, tile, m, n);
+            for (int k = 0; k < nk; ++k, ++it) {
+                const int s = it % kStages;
+                if (it >= kStages && !(ok = mbar_wait_cluster(empty + 8 * s, (it / kStages - 1) & 1, &s_failed))) break;
+                if (rank == 0) mbar_expect_tx(full + 8 * s, 2 * kStageBytes);
+                const auto copy = [&](uint32_t to, const CUtensorMap* map, int row) {
+                    asm volatile(
+                        "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%3, %4}], [%2];"
+                        ::"r"(to), "l"(reinterpret_cast<uint64_t>(map)), "r"(lead_full + 8 * s), "r"(k * 128), "r"(row)
+                        : "memory");
+                };
+                copy(stages + s * kStageBytes, &tm_x, m * 256 + rank * 128);
+                copy(stages + s * kStageBytes + 128 * 128, &tm_w, n * kN + rank * 128);
+            }
+        }
+        // A wait ran out: copies that are on their way end in much less than this.
+        if (!ok)
+            for (const long long since = clock64(); clock64() - since < kWaitBudgetCycles / 1024;) __nanosleep(1000);
+    } else if (warp == 1 && lane == 0 && rank == 0) {
+        constexpr uint32_t idesc = umma_idesc_i8(256, kN);
+        const auto commit = [&](uint32_t bar) {  // in both CTAs
+            asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
+                         "h"(static_cast<uint16_t>(3))
+                         : "memory");
+        };
+        int it = 0, turn = 0;
+        bool ok = true;
+        for (int tile = first; ok && tile < tiles; tile += step, ++turn) {
+            const int a = turn & 1;
+            if (turn >= 2 && !(ok = mbar_wait_cluster(drained + 8 * a, (turn / 2 - 1) & 1, &s_failed))) break;
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            for (int k = 0; k < nk; ++k, ++it) {
+                const int s = it % kStages;
+                if (!(ok = mbar_wait_cluster(full + 8 * s, (it / kStages) & 1, &s_failed))) break;
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                const uint32_t at = stages + s * kStageBytes;
+#pragma unroll
+                for (int kk = 0; kk < 4; ++kk)
+                    asm volatile(
+                        "{\n\t.reg .pred p;\n\t"
+                        "setp.ne.b32 p, %4, 0;\n\t"
+                        "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}"
+                        ::"r"(tmem + a * kN), "l"(umma_desc_sw128(at + kk * 32)), "l"(umma_desc_sw128(at + 128 * 128 + kk * 32)), "r"(idesc),
+                        "r"(static_cast<uint32_t>((k | kk) != 0))
+                        : "memory");
+                commit(empty + 8 * s);
+            }
+            if (ok) commit(done + 8 * a);
+        }
+        commit(idle);  // no product, and no arrival from one, is on its way when the CTAs give their memory back
+        mbar_settle(idle, 0);
+    } else if (warp == 1 && lane == 0) {
+        mbar_settle(idle, 0);
+    } else if (warp >= 2) {
+        const int quarter = warp & 3;
+        const uint32_t lead_drained = cluster_addr(drained, 0);
+        int turn = 0;
+        for (int tile = first; tile < tiles; tile += step, ++turn) {
+            int m, n;
+            i8_place(p, tile, m, n);
+            const int a = turn & 1;
+            i8_channels<kN>(p, n * kN, s_scale[a], s_bias[a]);
+            mbar_wait_cluster(done + 8 * a, (turn / 2) & 1, &s_failed);
+            __syncwarp();
+            const bool failed = __any_sync(kFull, *static_cast<volatile int*>(&s_failed));
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            i8_take<kN, kBf16>(p, tmem + a * kN + (static_cast<uint32_t>(quarter * 32) << 16), stages + kStages * kStageBytes + (warp - 2) * 4096,
+                               m * 256 + static_cast<int>(rank) * 128 + quarter * 32, n * kN, s_scale[a], s_bias[a], failed, [&] {
+                                   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                                   __syncwarp();
+                                   if (lane == 0)
+                                       asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(lead_drained + 8 * a) : "memory");
+                               });
+        }
+    }
+    __syncwarp();
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    cluster_meet();  // neither CTA's memory goes while the other may reach it
+    if (warp == 1) {
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(2 * kN) : "memory");
     }
 }
 
