@@ -4768,19 +4768,21 @@ int device_sms(int device, int* sms) {
 }
 
 template <bool kBf16, int kThreads, int kUnits>
-int quantize_launch(const I8QuantParams& p, cudaStream_t s) {
-    constexpr int rows = 256 / kThreads;
-    CUDA_TRY(launch_pdl(i8_quantize_kernel<kBf16, kThreads, kUnits>, dim3(static_cast<unsigned>((p.rows + rows - 1) / rows)),
-                        dim3(256), 0, s, p));
+int quantize_launch(const I8QuantParams& p, int sms, cudaStream_t s) {
+    // CTAs that take several rows each once they fill the GPU (bf16, 8192 x 4096: 21.5 us, a CTA for every two rows 23.9)
+    const long long ctas = (p.rows + 256ll / kThreads - 1) / (256 / kThreads), most = (kBf16 ? 6ll : 3ll) * sms;
+    CUDA_TRY(launch_pdl(i8_quantize_kernel<kBf16, kThreads, kUnits>, dim3(static_cast<unsigned>(std::min(ctas, most))), dim3(256), 0, s, p));
     return PHONON_CUDA_OK;
 }
 
 template <bool kBf16>
-int quantize_rows(const I8QuantParams& p, cudaStream_t s) {
-    if (p.cols <= 256) return quantize_launch<kBf16, 32, 1>(p, s);
-    if (p.cols <= 1024) return quantize_launch<kBf16, 32, 4>(p, s);
-    if (p.cols <= 4096) return quantize_launch<kBf16, 128, 4>(p, s);
-    return quantize_launch<kBf16, 256, 4>(p, s);
+int quantize_rows(const I8QuantParams& p, int sms, cudaStream_t s) {
+    if (p.cols <= 256) return quantize_launch<kBf16, 32, 1>(p, sms, s);
+    if (p.cols <= 512) return quantize_launch<kBf16, 32, 2>(p, sms, s);
+    if (p.cols <= 1024) return quantize_launch<kBf16, 64, 2>(p, sms, s);
+    if (p.cols <= 2048) return quantize_launch<kBf16, 128, 2>(p, sms, s);
+    if (p.cols <= 4096) return kBf16 ? quantize_launch<kBf16, 128, 4>(p, sms, s) : quantize_launch<kBf16, 256, 2>(p, sms, s);
+    return quantize_launch<kBf16, 256, 4>(p, sms, s);
 }
 
 template <int NT, bool kBf16>
@@ -4819,16 +4821,70 @@ int i8_tiles_launch(I8Params p, int sms, cudaStream_t s) {
     return PHONON_CUDA_OK;
 }
 
+// A tile of 128 rows x kN channels by a cluster of `splits` CTAs.
+template <int kN, bool kBf16>
+int i8_split_launch(I8Params p, int splits, cudaStream_t s) {
+    static std::atomic<uint64_t> configured{0};
+    const auto kernel = i8_split_kernel<kN, kBf16>;
+    constexpr int smem = 1024 + i8_split_stages<kN>() * (128 + kN) * 128;
+    CUtensorMap tx, tw;
+    if (!i8_maps(p, kN, &tx, &tw)) return PHONON_CUDA_DEVICE_ERROR;
+    CUDA_TRY(opt_in_smem(reinterpret_cast<const void*>(kernel), smem, configured));
+    p.tiles_m = (p.rows + 127) / 128;
+    p.tiles_n = (p.channels + kN - 1) / kN;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim = {static_cast<unsigned>(splits), 1, 1};
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(static_cast<unsigned>(p.tiles_m * p.tiles_n * splits));
+    cfg.blockDim = dim3(kI8Threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, tx, tw, p));
+    return PHONON_CUDA_OK;
+}
+
+// Which kernel, by what each takes in us, as fitted to sweeps of 25 shapes: a
+// start, then for every wave of tiles 128 bytes of depth at a time (0.31 us for
+// 64 channels, 0.345 for 128, 0.43 for a pair's 256 x 256), or the taking out
+// of a tile where that is longer (twice and a half as long where y's rows are
+// not 16-byte aligned); a split tile's sums take 3.3 and 4.5 us to meet. Up to
+// 16 rows always, and up to 32 where the weights are few, the rows' kernel.
+// us of the kernel chosen and of the next ones (rows x channels x depth):
+// 16 x 4096 x 4096 rows 6.2, split 9.5; 32 x 4096 x 4096 split by 4 8.9, 64
+// channels 13.7, rows 13.9; 32 x 512 x 2048 rows 4.7, split 5.0; 128 x 4096 x
+// 4096 split by 4 11.3, 64 channels 13.9; 512 x 512 x 2048 split by 4 6.9, 64
+// channels 8.1; 512 x 2048 x 512 64 channels 4.6, 128 5.4; 512 x 4096 x 4096
+// 128 channels 15.2, pairs 17.8, 64 channels 24.8; 1024 x 4096 x 4096 pairs
+// 18.5, 128 channels 26.3.
 template <bool kBf16>
 int i8_product(const I8Params& p, int sms, cudaStream_t s) {
     if (p.rows <= 8) return i8_rows_launch<1, kBf16>(p, s);
     if (p.rows <= 16) return i8_rows_launch<2, kBf16>(p, s);
-    if (p.rows <= 32) return i8_rows_launch<4, kBf16>(p, s);
-    const long long tiles_m = (p.rows + 127) / 128;
-    if ((p.rows + 255) / 256 * ((p.channels + 255ll) / 256) >= sms / 2) return i8_tiles_launch<256, true, kBf16>(p, sms, s);
-    if (tiles_m * ((p.channels + 255) / 256) >= sms) return i8_tiles_launch<256, false, kBf16>(p, sms, s);
-    if (tiles_m * ((p.channels + 127) / 128) >= sms) return i8_tiles_launch<128, false, kBf16>(p, sms, s);
-    return i8_tiles_launch<64, false, kBf16>(p, sms, s);
+    const int depths = (p.depth + 127) / 128;
+    const auto tiles = [&](int rows, int channels) {
+        return static_cast<double>((p.rows + rows - 1) / rows) * ((p.channels + channels - 1) / channels);
+    };
+    const double ragged = p.y_stride % (kBf16 ? 8 : 4) ? 2.5 : 1.0;
+    const auto whole = [&](double n, double each, double out, int resident) {
+        return std::ceil(n / resident) * std::max(depths * each, out * ragged) + 3.0;
+    };
+    const double n64 = tiles(128, 64), n128 = tiles(128, 128);
+    const double cost[6] = {whole(n64, 0.31, 1.2, sms), whole(n128, 0.345, 1.9, sms), whole(tiles(256, 256), 0.43, 4.0, sms / 2),
+                            4 * n64 > sms ? 1e30 : 6.3 + (depths + 3) / 4 * 0.31, 4 * n128 > sms ? 1e30 : 7.5 + (depths + 3) / 4 * 0.345,
+                            p.rows > 32 ? 1e30 : 2.5 + 0.68e-6 * p.channels * p.depth};
+    switch (std::min_element(cost, cost + 6) - cost) {
+        case 0: return i8_tiles_launch<64, false, kBf16>(p, sms, s);
+        case 1: return i8_tiles_launch<128, false, kBf16>(p, sms, s);
+        case 2: return i8_tiles_launch<256, true, kBf16>(p, sms, s);
+        case 3: return i8_split_launch<64, kBf16>(p, 4, s);
+        case 4: return i8_split_launch<128, kBf16>(p, 4, s);
+        default: return i8_rows_launch<4, kBf16>(p, s);
+    }
 }
 
 }  // namespace
@@ -4849,9 +4905,10 @@ int phonon_cuda_quantize_rows_device(int device, const PhononCudaQuantizeRows* a
     p.rows = static_cast<int>(a->rows);
     p.cols = static_cast<int>(a->cols);
     DeviceGuard guard(device);
-    if (!guard.ok) return PHONON_CUDA_DEVICE_ERROR;
+    int sms = 0;
+    if (!guard.ok || device_sms(device, &sms)) return PHONON_CUDA_DEVICE_ERROR;
     cudaStream_t s = static_cast<cudaStream_t>(cuda_stream);
-    return a->type == PHONON_CUDA_ROWS_BF16 ? quantize_rows<true>(p, s) : quantize_rows<false>(p, s);
+    return a->type == PHONON_CUDA_ROWS_BF16 ? quantize_rows<true>(p, sms, s) : quantize_rows<false>(p, sms, s);
 }
 
 int phonon_cuda_i8_product_device(int device, const PhononCudaI8Product* a, int32_t* status_dev, void* cuda_stream) {

@@ -36,78 +36,116 @@ __device__ __forceinline__ float i8_fix(float q, float x, float s) {
     return q;
 }
 
-// kThreads threads a row, kUnits units of 8 elements a thread in registers; a
-// row of more is read twice. Bound by the bytes.
+// Eight elements of a row as they lie.
+template <bool kBf16>
+struct I8Unit {
+    uint4 w[kBf16 ? 1 : 2];
+    __device__ __forceinline__ void load(const void* x, size_t at) {
+        const uint4* from = reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(x) + at * (kBf16 ? 2 : 4));
+        w[0] = from[0];
+        if constexpr (!kBf16) w[1] = from[1];
+    }
+    __device__ __forceinline__ void zero() {
+        w[0] = make_uint4(0, 0, 0, 0);
+        if constexpr (!kBf16) w[1] = w[0];
+    }
+    __device__ __forceinline__ uint32_t word(int i) const {
+        const uint4& v = w[i / 4];
+        return i % 4 == 0 ? v.x : i % 4 == 1 ? v.y : i % 4 == 2 ? v.z : v.w;
+    }
+    __device__ __forceinline__ float element(int k) const {
+        if constexpr (kBf16) return __uint_as_float(k % 2 ? word(k / 2) & 0xffff0000u : word(k / 2) << 16);
+        else return __uint_as_float(word(k));
+    }
+    // The largest magnitude's bits so far (of bf16 in both halves).
+    __device__ __forceinline__ uint32_t top(uint32_t most) const {
+#pragma unroll
+        for (int i = 0; i < (kBf16 ? 4 : 8); ++i)
+            most = kBf16 ? __vmaxu2(most, word(i) & 0x7fff7fffu) : max(most, word(i) & 0x7fffffffu);
+        return most;
+    }
+};
+
+// kThreads threads a row, kUnits units of 8 elements a thread in registers, as
+// they lie, the next row's on their way meanwhile; a row of more is read twice.
+// Bound by the bytes.
 template <bool kBf16, int kThreads, int kUnits>
-__global__ void __launch_bounds__(256) i8_quantize_kernel(I8QuantParams p) {
+__global__ void __launch_bounds__(256, kBf16 ? 4 : 3) i8_quantize_kernel(I8QuantParams p) {
     constexpr int kRows = 256 / kThreads, kWarps = kThreads / 32;
     constexpr float kRound = 12582912.0f;  // 1.5 * 2^23: adding it rounds to an integer
-    __shared__ uint32_t s_top[8];
+    __shared__ uint32_t s_top[2][8];
     pdl_wait();
     pdl_trigger();
-    const int t = threadIdx.x % kThreads, warp = threadIdx.x >> 5;
-    const long long row = static_cast<long long>(blockIdx.x) * kRows + threadIdx.x / kThreads;
-    const bool there = row < p.rows;
-    const int units = there ? p.cols / 8 : 0;
-    const size_t in = static_cast<size_t>(row) * p.x_stride;
-    float4 v[kUnits][2];
-    uint32_t top = 0;  // the largest magnitude's bits; not finite: 0x7f800000 or more
-    auto look = [&](float4 a) {
-        top = max(top, max(max(__float_as_uint(a.x) & 0x7fffffffu, __float_as_uint(a.y) & 0x7fffffffu),
-                           max(__float_as_uint(a.z) & 0x7fffffffu, __float_as_uint(a.w) & 0x7fffffffu)));
-    };
+    const int t = threadIdx.x % kThreads, warp = threadIdx.x >> 5, units = p.cols / 8;
+    const int step = static_cast<int>(gridDim.x) * kRows;
+    I8Unit<kBf16> v[kUnits], next[kUnits];
+    const auto load = [&](I8Unit<kBf16> (&x)[kUnits], long long row) {
 #pragma unroll
-    for (int u = 0; u < kUnits; ++u)
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-            v[u][h] = u * kThreads + t < units ? load_row4<kBf16>(p.x, in + (u * kThreads + t) * 8 + 4 * h)
-                                               : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll
-    for (int u = 0; u < kUnits; ++u) look(v[u][0]), look(v[u][1]);
-    for (int u = kUnits * kThreads + t; u < units; u += kThreads) {
-        look(load_row4<kBf16>(p.x, in + u * 8ll));
-        look(load_row4<kBf16>(p.x, in + u * 8ll + 4));
-    }
-    top = __reduce_max_sync(kFull, top);
-    if constexpr (kWarps > 1) {
-        if ((threadIdx.x & 31) == 0) s_top[warp] = top;
-        __syncthreads();
-        const int first = warp / kWarps * kWarps;
-#pragma unroll
-        for (int w = 0; w < kWarps; ++w) top = max(top, s_top[first + w]);
-    }
-    if (!there) return;
-    const bool bad = top >= 0x7f800000u;
-    const float s = fmaxf(__fdiv_rn(__uint_as_float(top), 127.0f), 0x1p-126f), inverse = bad ? 0.0f : __frcp_rn(s);
-    if (t == 0) {
-        p.scales[row] = bad ? __int_as_float(0x7fc00000) : s;
-        if (bad) flag_nonfinite(p.status, static_cast<int>(row));
-    }
-    int8_t* out = p.q + static_cast<size_t>(row) * p.q_stride;
-    auto put = [&](const float4 (&x)[2], int u) {
-        float q[8], far = 0.0f;
-        const float* f = &x[0].x;
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-            const float e = bad ? 0.0f : f[k];
-            q[k] = fmaf(e, inverse, kRound) - kRound;
-            far = fmaxf(far, fabsf(fmaf(-q[k], s, e)));
+        for (int u = 0; u < kUnits; ++u) {
+            if (row < p.rows && u * kThreads + t < units) x[u].load(p.x, static_cast<size_t>(row) * p.x_stride + (u * kThreads + t) * 8ll);
+            else x[u].zero();
         }
-        if (!bad && 2.0f * far >= s) {
-#pragma unroll
-            for (int k = 0; k < 8; ++k) q[k] = i8_fix(q[k], f[k], s);
-        }
-        uint32_t w[8];
-#pragma unroll
-        for (int k = 0; k < 8; ++k) w[k] = __float_as_uint(q[k] + kRound);  // the low byte is the integer's
-        *reinterpret_cast<uint2*>(out + u * 8ll) = make_uint2(kv8_pack(w[0], w[1], w[2], w[3]), kv8_pack(w[4], w[5], w[6], w[7]));
     };
+    const int own = threadIdx.x / kThreads;
+    load(next, blockIdx.x * static_cast<long long>(kRows) + own);
+    int parity = 0;
+    for (long long base = blockIdx.x * static_cast<long long>(kRows); base < p.rows; base += step, parity ^= 1) {
+        const long long row = base + own;
+        const bool there = row < p.rows;
+        const size_t in = static_cast<size_t>(row) * p.x_stride;
+        uint32_t top = 0;  // the largest magnitude's bits; not finite: an exponent of ones
 #pragma unroll
-    for (int u = 0; u < kUnits; ++u)
-        if (u * kThreads + t < units) put(v[u], u * kThreads + t);
-    for (int u = kUnits * kThreads + t; u < units; u += kThreads) {
-        const float4 x[2] = {load_row4<kBf16>(p.x, in + u * 8ll), load_row4<kBf16>(p.x, in + u * 8ll + 4)};
-        put(x, u);
+        for (int u = 0; u < kUnits; ++u) {
+            v[u] = next[u];
+            top = v[u].top(top);
+        }
+        load(next, row + step);
+        for (int u = kUnits * kThreads + t; there && u < units; u += kThreads) {
+            I8Unit<kBf16> x;
+            x.load(p.x, in + u * 8ll);
+            top = x.top(top);
+        }
+        if constexpr (kBf16) top = max(top & 0xffff0000u, top << 16);
+        top = __reduce_max_sync(kFull, top);
+        if constexpr (kWarps > 1) {
+            if ((threadIdx.x & 31) == 0) s_top[parity][warp] = top;
+            __syncthreads();
+            const int first = warp / kWarps * kWarps;
+#pragma unroll
+            for (int w = 0; w < kWarps; ++w) top = max(top, s_top[parity][first + w]);
+        }
+        if (!there) continue;
+        const bool bad = top >= 0x7f800000u;
+        const float s = fmaxf(__fdiv_rn(__uint_as_float(top), 127.0f), 0x1p-126f), inverse = __frcp_rn(s);
+        if (t == 0) {
+            p.scales[row] = bad ? __int_as_float(0x7fc00000) : s;
+            if (bad) flag_nonfinite(p.status, static_cast<int>(row));
+        }
+        int8_t* out = p.q + static_cast<size_t>(row) * p.q_stride;
+        auto put = [&](const I8Unit<kBf16>& x, int u) {
+            uint32_t w[8];  // the low byte is the integer's
+            float far = 0.0f;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                const float near = fmaf(x.element(k), inverse, kRound);
+                far = fmaxf(far, fabsf(fmaf(kRound - near, s, x.element(k))));
+                w[k] = __float_as_uint(near);
+            }
+            if (2.0f * far >= s) {
+#pragma unroll
+                for (int k = 0; k < 8; ++k) w[k] = __float_as_uint(i8_fix(__uint_as_float(w[k]) - kRound, x.element(k), s) + kRound);
+            }
+            *reinterpret_cast<uint2*>(out + u * 8ll) =
+                bad ? make_uint2(0, 0) : make_uint2(kv8_pack(w[0], w[1], w[2], w[3]), kv8_pack(w[4], w[5], w[6], w[7]));
+        };
+#pragma unroll
+        for (int u = 0; u < kUnits; ++u)
+            if (u * kThreads + t < units) put(v[u], u * kThreads + t);
+        for (int u = kUnits * kThreads + t; u < units; u += kThreads) {
+            I8Unit<kBf16> x;
+            x.load(p.x, in + u * 8ll);
+            put(x, u);
+        }
     }
 }
 
@@ -165,7 +203,7 @@ __global__ void __launch_bounds__(32 * kI8Warps) i8_rows_kernel(I8Params p) {
     int sum[NT][4];
 #pragma unroll
     for (int n = 0; n < NT; ++n) sum[n][0] = sum[n][1] = sum[n][2] = sum[n][3] = 0;
-    constexpr int kAhead = NT > 2 ? kI8Ahead / 2 : kI8Ahead;
+    constexpr int kAhead = kI8Ahead / NT;
     const uint4 zero = make_uint4(0, 0, 0, 0);
     for (int c0 = first; c0 < last; c0 += kAhead) {
         uint4 a[kAhead][2], b[kAhead][NT];
@@ -210,17 +248,17 @@ __device__ __forceinline__ void mbar_settle(uint32_t bar, uint32_t parity) {
 // Many rows: tiles on the tcgen05 tensor cores, a CTA (or a pair of them) an SM
 // that takes tiles in turn. Warp 0 brings 128 bytes of depth a stage by TMA,
 // warp 1 issues the products into one of two accumulators in TMEM, and warps
-// 2-5 take the other one out, a row a thread.
+// 2-9 take the other one out, a row and half of the channels a thread.
 //
 // i8_product_kernel: 128 rows x kN channels a CTA. i8_pair_kernel: 256 x 256 a
 // pair of CTAs (cta_group::2): each has 128 of the rows and 128 of the
 // channels in its shared memory and the products read both, so that a CTA's
 // copies are 32 KB for what takes 48 KB alone.
-constexpr int kI8Threads = 192;
-constexpr int kI8Staging = 4 * 32 * 128;  // bytes: 32 rows of 128 for each of warps 2-5
+constexpr int kI8Threads = 320;
+constexpr int kI8Staging = 8 * 32 * 64;  // bytes: 32 rows of 64 for each of warps 2-9
 
 template <int kN>
-__host__ __device__ constexpr int i8_stages() { return kN == 256 ? 4 : kN == 128 ? 6 : 8; }
+__host__ __device__ constexpr int i8_stages() { return kN == 128 ? 6 : 8; }
 
 template <int kN>
 __host__ __device__ constexpr int i8_smem() { return 1024 + i8_stages<kN>() * (128 + kN) * 128 + kI8Staging; }
@@ -237,81 +275,97 @@ __device__ __forceinline__ void i8_place(const I8Params& p, int tile, int& m, in
     m = band * kBand + in - n * high;
 }
 
-// kN accumulator columns of a warp's 32 rows (row0 + lane; channels from n0 on)
-// to y, 128 bytes of every row at a time through `staging`, so that a store
-// has whole lines whatever the row stride; `taken` is called once the columns
-// have left TMEM. scale, bias: the channels'. failed: NaN in their place.
-template <int kN, bool kBf16, typename Taken>
-__device__ __forceinline__ void i8_take(const I8Params& p, uint32_t tmem, uint32_t staging, int row0, int n0, const float* scale,
-                                        const float* bias, bool failed, const Taken& taken) {
-    constexpr int kCols = kBf16 ? 64 : 32, kSize = kBf16 ? 2 : 4;  // 128 bytes
+// Where a warp's staged row lies: 64 bytes, its 16-byte pieces turned so that
+// neither a piece of every row nor a row's pieces share banks.
+__device__ __forceinline__ uint32_t i8_staged(uint32_t staging, int row, int piece) {
+    return staging + row * 64 + ((piece ^ (row >> 1 & 3)) * 16);
+}
+
+// 32 staged rows to y where its rows have any alignment, two rows at a time: a
+// lane takes a word (two bf16) of what lies in a row between two word
+// boundaries, and single elements at its ends.
+template <bool kBf16>
+__device__ __forceinline__ void i8_store_ragged(const I8Params& p, uint32_t staging, int row0, int n0) {
+    constexpr int kCols = kBf16 ? 32 : 16;
+    const int lane = threadIdx.x & 31, w = lane & 15, cols = min(kCols, p.channels - n0);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        const int r = 2 * i + (lane >> 4);
+        const bool in = row0 + r < p.rows;
+        const size_t to = static_cast<size_t>(row0 + r) * p.y_stride + n0;
+        uint32_t mine;
+        asm volatile("ld.shared.b32 %0, [%1];" : "=r"(mine) : "r"(i8_staged(staging, r, w >> 2) + (w & 3) * 4));
+        if constexpr (kBf16) {
+            uint16_t* y = static_cast<uint16_t*>(p.y) + to;
+            const bool odd = to & 1;  // y + 1 is a word's
+            const uint32_t next = __shfl_down_sync(kFull, mine, 1);
+            const int at = 2 * w + odd;
+            if (in && at + 1 < cols && !(odd && w == 15)) *reinterpret_cast<uint32_t*>(y + at) = odd ? __byte_perm(mine, next, 0x5432) : mine;
+            else if (in && at < cols) y[at] = static_cast<uint16_t>(odd ? mine >> 16 : mine);
+            if (in && odd && w == 0) y[0] = static_cast<uint16_t>(mine);
+        } else {
+            if (in && w < cols) static_cast<uint32_t*>(p.y)[to + w] = mine;
+        }
+    }
+}
+
+// A tile's columns [c0, c1) of a warp's 32 rows (row0 + lane; channels from n0
+// on) to y, 64 bytes of every row at a time through `staging`, so that a store
+// has whole sectors whatever the row stride; `taken` is called once they have
+// left TMEM. scale, bias: the tile's channels'. failed: NaN.
+template <bool kBf16, typename Taken>
+__device__ __forceinline__ void i8_take(const I8Params& p, uint32_t tmem, uint32_t staging, int row0, int n0, int c0, int c1,
+                                        const float* scale, const float* bias, bool failed, const Taken& taken) {
+    constexpr int kCols = kBf16 ? 32 : 16, kSize = kBf16 ? 2 : 4;  // 64 bytes
     const int lane = threadIdx.x & 31, row = row0 + lane;
     const bool wide = p.y_stride * kSize % 16 == 0;
     const float xs = failed ? __int_as_float(0x7fc00000) : row < p.rows ? p.x_scales[row] : 0.0f;
     float finite = 0.0f;  // NaN once a value is not
 #pragma unroll 1
-    for (int c = 0; c < kN; c += kCols) {
-        uint32_t out[32];
+    for (int c = c0; c < c1; c += 32) {
+        uint32_t r[32];
+        tmem_load32(tmem + c, r);
+        if (c + 32 >= c1) taken();
 #pragma unroll
-        for (int h = 0; h < kCols / 32; ++h) {
-            uint32_t r[32];
-            tmem_load32(tmem + c + 32 * h, r);
+        for (int h = 0; h < 32; h += kCols) {
+            uint32_t out[16];
 #pragma unroll
-            for (int k = 0; k < 32; k += 2) {
-                float v[2];
+            for (int k = 0; k < kCols; k += 4) {
+                const float4 s4 = *reinterpret_cast<const float4*>(scale + c + h + k), b4 = *reinterpret_cast<const float4*>(bias + c + h + k);
+                const float v[4] = {i8_value(static_cast<int>(r[h + k]), xs, s4.x, b4.x), i8_value(static_cast<int>(r[h + k + 1]), xs, s4.y, b4.y),
+                                    i8_value(static_cast<int>(r[h + k + 2]), xs, s4.z, b4.z), i8_value(static_cast<int>(r[h + k + 3]), xs, s4.w, b4.w)};
 #pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    const int at = c + 32 * h + k + i;
-                    v[i] = i8_value(static_cast<int>(r[k + i]), xs, scale[at], bias[at]);
-                }
-                if constexpr (kBf16) {
-                    const __nv_bfloat162 b = __floats2bfloat162_rn(v[0], v[1]);
-                    out[16 * h + k / 2] = *reinterpret_cast<const uint32_t*>(&b);
-                    v[0] = __low2float(b);
-                    v[1] = __high2float(b);
-                } else {
-                    out[k] = __float_as_uint(v[0]);
-                    out[k + 1] = __float_as_uint(v[1]);
-                }
-                finite = fmaf(v[0], 0.0f, fmaf(v[1], 0.0f, finite));  // (channels behind the last: sums 0, scale and bias 0)
-            }
-        }
-        if (c + kCols >= kN) taken();
-#pragma unroll
-        for (int k = 0; k < 8; ++k) kv8_put16(staging + lane * 128 + ((k ^ (lane & 7)) * 16), out[4 * k], out[4 * k + 1], out[4 * k + 2], out[4 * k + 3]);
-        __syncwarp();
-        if (wide && n0 + c + kCols <= p.channels) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const int r = 4 * i + (lane >> 3);
-                uint4 w;
-                asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w)
-                             : "r"(staging + r * 128 + (((lane & 7) ^ (r & 7)) * 16)));
-                if (row0 + r < p.rows)
-                    *reinterpret_cast<uint4*>(static_cast<uint8_t*>(p.y) + (static_cast<size_t>(row0 + r) * p.y_stride + n0 + c) * kSize + (lane & 7) * 16) = w;
-            }
-        } else {
-            const int rows = min(32, p.rows - row0), cols = p.channels - n0 - c;
-#pragma unroll 4
-            for (int r = 0; r < rows; ++r)
-#pragma unroll
-                for (int h = 0; h < kCols / 32; ++h) {
-                    const int at = (32 * h + lane) * kSize;
-                    const uint32_t from = staging + r * 128 + ((at >> 4 ^ (r & 7)) * 16) + (at & 15);
-                    const size_t to = static_cast<size_t>(row0 + r) * p.y_stride + n0 + c + 32 * h + lane;
-                    if (32 * h + lane >= cols) continue;
+                for (int i = 0; i < 4; i += 2) {
                     if constexpr (kBf16) {
-                        uint16_t w;
-                        asm volatile("ld.shared.b16 %0, [%1];" : "=h"(w) : "r"(from));
-                        static_cast<uint16_t*>(p.y)[to] = w;
+                        const __nv_bfloat162 b = __floats2bfloat162_rn(v[i], v[i + 1]);
+                        const uint32_t w = *reinterpret_cast<const uint32_t*>(&b);
+                        out[(k + i) / 2] = w;
+                        finite = fmaf(__uint_as_float(w << 16), 0.0f, fmaf(__uint_as_float(w & 0xffff0000u), 0.0f, finite));
                     } else {
-                        uint32_t w;
-                        asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w) : "r"(from));
-                        static_cast<uint32_t*>(p.y)[to] = w;
+                        out[k + i] = __float_as_uint(v[i]);
+                        out[k + i + 1] = __float_as_uint(v[i + 1]);
+                        finite = fmaf(v[i], 0.0f, fmaf(v[i + 1], 0.0f, finite));  // (channels behind the last: sums, scale and bias 0)
                     }
                 }
+            }
+#pragma unroll
+            for (int k = 0; k < 4; ++k) kv8_put16(i8_staged(staging, lane, k), out[4 * k], out[4 * k + 1], out[4 * k + 2], out[4 * k + 3]);
+            __syncwarp();
+            if (wide && n0 + c + h + kCols <= p.channels) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int to = 8 * i + (lane >> 2);
+                    uint4 w;
+                    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w)
+                                 : "r"(i8_staged(staging, to, lane & 3)));
+                    if (row0 + to < p.rows)
+                        *reinterpret_cast<uint4*>(static_cast<uint8_t*>(p.y) + (static_cast<size_t>(row0 + to) * p.y_stride + n0 + c + h) * kSize + (lane & 3) * 16) = w;
+                }
+            } else if (n0 + c + h < p.channels) {
+                i8_store_ragged<kBf16>(p, staging, row0, n0 + c + h);
+            }
+            __syncwarp();
         }
-        __syncwarp();
     }
     if (row < p.rows && finite != 0.0f) {
         if (failed) {
@@ -322,14 +376,14 @@ __device__ __forceinline__ void i8_take(const I8Params& p, uint32_t tmem, uint32
     }
 }
 
-// The channels' scales and biases of a tile, by the threads of warps 2-5.
+// The channels' scales and biases of a tile, by the threads of warps 2-9.
 template <int kN>
 __device__ __forceinline__ void i8_channels(const I8Params& p, int n0, float* scale, float* bias) {
-    for (int c = threadIdx.x - 64; c < kN; c += 128) {
+    for (int c = threadIdx.x - 64; c < kN; c += 256) {
         scale[c] = n0 + c < p.channels ? p.w_scales[n0 + c] : 0.0f;
         bias[c] = p.bias && n0 + c < p.channels ? p.bias[n0 + c] : 0.0f;
     }
-    asm volatile("bar.sync 1, 128;" ::: "memory");
+    asm volatile("bar.sync 1, 256;" ::: "memory");
 }
 
 template <int kN, bool kBf16>
@@ -351,7 +405,7 @@ __global__ void __launch_bounds__(kI8Threads, 1)
         }
         for (int a = 0; a < 2; ++a) {
             mbar_init(done + 8 * a, 1);
-            mbar_init(drained + 8 * a, 4);
+            mbar_init(drained + 8 * a, 8);
         }
         mbar_init(idle, 1);
         s_failed = 0;
@@ -418,12 +472,13 @@ __global__ void __launch_bounds__(kI8Threads, 1)
             __syncwarp();
             const bool failed = __any_sync(kFull, *static_cast<volatile int*>(&s_failed));
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            i8_take<kN, kBf16>(p, tmem + a * kN + (static_cast<uint32_t>(quarter * 32) << 16), stages + kStages * kStageBytes + (warp - 2) * 4096,
-                               m * 128 + quarter * 32, n * kN, s_scale[a], s_bias[a], failed, [&] {
-                                   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-                                   __syncwarp();
-                                   if (lane == 0) mbar_arrive(drained + 8 * a);
-                               });
+            const int c0 = (warp - 2) / 4 * (kN / 2);
+            i8_take<kBf16>(p, tmem + a * kN + (static_cast<uint32_t>(quarter * 32) << 16), stages + kStages * kStageBytes + (warp - 2) * 2048,
+                           m * 128 + quarter * 32, n * kN, c0, c0 + kN / 2, s_scale[a], s_bias[a], failed, [&] {
+                               asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                               __syncwarp();
+                               if (lane == 0) mbar_arrive(drained + 8 * a);
+                           });
         }
     }
     __syncwarp();
@@ -444,6 +499,142 @@ __device__ __forceinline__ uint32_t cluster_addr(uint32_t addr, uint32_t rank) {
 __device__ __forceinline__ void cluster_meet() {
     asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
     asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+// Few tiles: the depth of one is split over the CTAs of a cluster, whose sums
+// meet in shared memory (integers: the result does not depend on the split).
+template <int kN>
+__host__ __device__ constexpr int i8_split_stages() { return kN == 128 ? 6 : 8; }
+
+template <int kN, bool kBf16>
+__global__ void __launch_bounds__(kI8Threads, 1)
+    i8_split_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_w, I8Params p) {
+    constexpr int kStages = i8_split_stages<kN>(), kStageBytes = (128 + kN) * 128, kPitch = kN * 4 + 16;
+    static_assert(128 * kPitch <= kStages * kStageBytes, "the sums outgrow the operands' room");
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ __align__(8) uint64_t s_bars[2 * kStages + 1];
+    __shared__ uint32_t s_tmem;
+    __shared__ int s_failed;
+    const uint32_t stages = (smem_addr(smem_raw) + 1023) & ~1023u;
+    const uint32_t full = smem_addr(s_bars), empty = full + 8 * kStages, done = empty + 8 * kStages;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    uint32_t rank, splits;
+    asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
+    asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(splits));
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < kStages; ++s) {
+            mbar_init(full + 8 * s, 1);
+            mbar_init(empty + 8 * s, 1);
+        }
+        mbar_init(done, 1);
+        s_failed = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&s_tmem)), "n"(kN) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    const uint32_t tmem = s_tmem;
+    int m, n;
+    i8_place(p, static_cast<int>(blockIdx.x / splits), m, n);
+    const int nk = (p.depth + 127) / 128, per = (nk + static_cast<int>(splits) - 1) / static_cast<int>(splits);
+    const int first = min(nk, static_cast<int>(rank) * per), turns = min(nk, first + per) - first;
+    pdl_wait();
+    pdl_trigger();
+    if (warp == 0 && lane == 0) {
+        int k = 0;
+        bool ok = true;
+        for (; k < turns; ++k) {
+            const int s = k % kStages;
+            if (k >= kStages && !(ok = mbar_wait(empty + 8 * s, (k / kStages - 1) & 1, nullptr, &s_failed))) break;
+            mbar_expect_tx(full + 8 * s, kStageBytes);
+            tma_load_2d(stages + s * kStageBytes, &tm_x, (first + k) * 128, m * 128, full + 8 * s);
+            tma_load_2d(stages + s * kStageBytes + 128 * 128, &tm_w, (first + k) * 128, n * kN, full + 8 * s);
+        }
+        if (!ok)  // a wait ran out: no copy is on its way when the CTA gives its memory back
+            for (int j = max(0, k - kStages); j < k; ++j) mbar_settle(full + 8 * (j % kStages), (j / kStages) & 1);
+    } else if (warp == 1 && lane == 0) {
+        constexpr uint32_t idesc = umma_idesc_i8(128, kN);
+        for (int k = 0; k < turns; ++k) {
+            const int s = k % kStages;
+            if (!mbar_wait(full + 8 * s, (k / kStages) & 1, nullptr, &s_failed)) break;
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            const uint32_t at = stages + s * kStageBytes;
+#pragma unroll
+            for (int kk = 0; kk < 4; ++kk)
+                umma_i8(tmem, umma_desc_sw128(at + kk * 32), umma_desc_sw128(at + 128 * 128 + kk * 32), idesc, (k | kk) != 0);
+            umma_commit(empty + 8 * s);
+        }
+        umma_commit(done);
+        mbar_settle(done, 0);  // nor is a product
+    }
+    __syncwarp();
+    mbar_wait(done, 0, nullptr, &s_failed);
+    __syncthreads();  // every copy has been multiplied: the operands' room takes the sums
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    if (warp >= 2 && warp < 6) {
+        const int quarter = warp & 3;
+        const uint32_t to = stages + (quarter * 32 + lane) * kPitch;
+#pragma unroll
+        for (int c = 0; c < kN; c += 32) {
+            uint32_t r[32];
+            tmem_load32(tmem + c + (static_cast<uint32_t>(quarter * 32) << 16), r);
+            const bool some = turns > 0;
+#pragma unroll
+            for (int k = 0; k < 32; k += 4)
+                kv8_put16(to + (c + k) * 4, some ? r[k] : 0, some ? r[k + 1] : 0, some ? r[k + 2] : 0, some ? r[k + 3] : 0);
+        }
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    cluster_meet();
+    // rows rank, rank + splits, ... of the tile; four channels a thread
+    constexpr int kQuads = kN / 4;
+    const int rows = min(128, p.rows - m * 128);
+    for (int x = threadIdx.x; x < 128 / static_cast<int>(splits) * kQuads; x += kI8Threads) {
+        const int r = x / kQuads * static_cast<int>(splits) + static_cast<int>(rank), c = x % kQuads * 4;
+        if (r >= rows) continue;
+        int4 sum = make_int4(0, 0, 0, 0);
+        int bad = 0;
+        for (uint32_t peer = 0; peer < splits; ++peer) {
+            int4 v;
+            int f;
+            asm volatile("ld.shared::cluster.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                         : "r"(cluster_addr(stages + r * kPitch + c * 4, peer)) : "memory");
+            asm volatile("ld.shared::cluster.b32 %0, [%1];" : "=r"(f) : "r"(cluster_addr(smem_addr(&s_failed), peer)) : "memory");
+            sum = make_int4(sum.x + v.x, sum.y + v.y, sum.z + v.z, sum.w + v.w);
+            bad |= f;
+        }
+        const int row = m * 128 + r, n0 = n * kN + c;
+        const float xs = bad ? __int_as_float(0x7fc00000) : p.x_scales[row];
+        const int v[4] = {sum.x, sum.y, sum.z, sum.w};
+        const size_t at = static_cast<size_t>(row) * p.y_stride + n0;
+        float y[4];
+        bool finite = true;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const bool in = n0 + k < p.channels;
+            y[k] = in ? i8_value(v[k], xs, p.w_scales[n0 + k], p.bias ? p.bias[n0 + k] : 0.0f) : 0.0f;
+            finite &= isfinite(kBf16 ? __bfloat162float(__float2bfloat16(y[k])) : y[k]);
+        }
+        if (p.y_stride % 4 == 0 && n0 + 4 <= p.channels) {
+            store_row4<kBf16>(p.y, at, make_float4(y[0], y[1], y[2], y[3]));
+        } else {
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                if (n0 + k < p.channels) i8_store<kBf16>(p.y, at + k, y[k]);
+        }
+        if (bad && p.status) atomicMax(p.status + row, kStatusDevice);
+        else if (!finite) flag_nonfinite(p.status, row);
+    }
+    cluster_meet();  // no CTA's sums go while another reads them
+    if (warp == 1) {
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(kN) : "memory");
+    }
 }
 
 // mbar_wait for a barrier that the cluster's other CTA arrives at, too.
@@ -487,7 +678,7 @@ __global__ void __launch_bounds__(kI8Threads, 1) __cluster_dims__(2, 1, 1)
         }
         for (int a = 0; a < 2; ++a) {
             mbar_init(done + 8 * a, 1);
-            mbar_init(drained + 8 * a, 8);
+            mbar_init(drained + 8 * a, 16);
         }
         mbar_init(idle, 1);
         s_failed = 0;
@@ -577,13 +768,14 @@ __global__ void __launch_bounds__(kI8Threads, 1) __cluster_dims__(2, 1, 1)
             __syncwarp();
             const bool failed = __any_sync(kFull, *static_cast<volatile int*>(&s_failed));
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            i8_take<kN, kBf16>(p, tmem + a * kN + (static_cast<uint32_t>(quarter * 32) << 16), stages + kStages * kStageBytes + (warp - 2) * 4096,
-                               m * 256 + static_cast<int>(rank) * 128 + quarter * 32, n * kN, s_scale[a], s_bias[a], failed, [&] {
-                                   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-                                   __syncwarp();
-                                   if (lane == 0)
-                                       asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(lead_drained + 8 * a) : "memory");
-                               });
+            const int c0 = (warp - 2) / 4 * (kN / 2);
+            i8_take<kBf16>(p, tmem + a * kN + (static_cast<uint32_t>(quarter * 32) << 16), stages + kStages * kStageBytes + (warp - 2) * 2048,
+                           m * 256 + static_cast<int>(rank) * 128 + quarter * 32, n * kN, c0, c0 + kN / 2, s_scale[a], s_bias[a], failed, [&] {
+                               asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                               __syncwarp();
+                               if (lane == 0)
+                                   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(lead_drained + 8 * a) : "memory");
+                           });
         }
     }
     __syncwarp();
