@@ -4769,8 +4769,8 @@ int device_sms(int device, int* sms) {
 
 template <bool kBf16, int kThreads, int kUnits>
 int quantize_launch(const I8QuantParams& p, int sms, cudaStream_t s) {
-    // CTAs that take several rows each once they fill the GPU (bf16, 8192 x 4096: 21.5 us, a CTA for every two rows 23.9)
-    const long long ctas = (p.rows + 256ll / kThreads - 1) / (256 / kThreads), most = (kBf16 ? 6ll : 3ll) * sms;
+    // CTAs that take several rows each once they fill the GPU (bf16, 8192 x 4096: 22.8 us, a CTA for every two rows 25.0)
+    const long long ctas = (p.rows + 256ll / kThreads - 1) / (256 / kThreads), most = (kBf16 ? 4ll : 3ll) * sms;
     CUDA_TRY(launch_pdl(i8_quantize_kernel<kBf16, kThreads, kUnits>, dim3(static_cast<unsigned>(std::min(ctas, most))), dim3(256), 0, s, p));
     return PHONON_CUDA_OK;
 }
@@ -4955,14 +4955,10 @@ bool make_rows_map(CUtensorMap* map, const void* base, int rows, int heads, int 
                     CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// Tiles of p.tokens positions, `parts` CTAs each.
-int prompt_grid(PromptParams& p, int parts, unsigned* grid) {
-    const long long slots = std::min<long long>(p.rows / p.tokens + static_cast<long long>(p.prompts),
-                                                static_cast<long long>(p.prompts) * ((p.max_rows + p.tokens - 1) / p.tokens));
-    if (slots * parts > INT32_MAX) return PHONON_CUDA_CAPACITY;
-    p.by_heads = kv8_divisor(static_cast<uint32_t>(parts));
-    *grid = static_cast<unsigned>(slots * parts);
-    return PHONON_CUDA_OK;
+// CTAs of p.tokens positions and one of `parts` groups of heads, at most.
+long long prompt_ctas(const PromptParams& p, int parts) {
+    return parts * std::min<long long>(p.rows / p.tokens + static_cast<long long>(p.prompts),
+                                       static_cast<long long>(p.prompts) * ((p.max_rows + p.tokens - 1) / p.tokens));
 }
 
 // Kernels whose warps hand registers to one another: what they ask for has to
@@ -4976,40 +4972,39 @@ int enough_registers(const void* kernel, int threads, int asked, std::atomic<boo
     return PHONON_CUDA_OK;
 }
 
-// Query heads of a K/V head share rows of a tile, and so its keys and values.
-int prompt_pack(PromptParams& p, int rows) {
-    const int group = static_cast<int>(p.group.d), pack = group <= 32 ? group : 1;
-    p.pack = kv8_divisor(static_cast<uint32_t>(pack));
-    p.tokens = rows / 128 * (128 / pack);
-    return pack;
-}
-
 template <int D, bool kBf16>
-int prompt_launch(PromptParams p, cudaStream_t s) {
+int prompt_launch(PromptParams p, int sms, cudaStream_t s) {
     static std::atomic<bool> enough{false};
     static std::atomic<uint64_t> configured{0};
-    unsigned grid = 0;
+    // Query heads of a K/V head share rows of a tile, and so its keys and values.
+    const int group = static_cast<int>(p.group.d), pack = group <= 32 ? group : 1, parts = p.heads / pack;
+    p.pack = kv8_divisor(static_cast<uint32_t>(pack));
+    p.half = 128 / pack;
+    p.tokens = p.half;
+    p.by_heads = kv8_divisor(static_cast<uint32_t>(parts));
     if constexpr (kBf16) {
         using Shape = PromptShape<D>;
         const void* kernel = reinterpret_cast<const void*>(prompt_bf16_kernel<D>);
-        const int pack = prompt_pack(p, 256);
-        if (const int rc = prompt_grid(p, p.heads / pack, &grid)) return rc;
-        if (const int rc = enough_registers(kernel, kPromptThreads, kPromptRegisters, enough)) return rc;
+        p.tokens *= 2;
+        if (prompt_ctas(p, parts) < static_cast<long long>(sms) * Shape::kCtas) p.tokens = p.half;
+        const long long ctas = prompt_ctas(p, parts);
+        if (ctas > INT32_MAX) return PHONON_CUDA_CAPACITY;
+        if (const int rc = enough_registers(kernel, kPromptThreads, Shape::kRegisters, enough)) return rc;
         CUDA_TRY(opt_in_smem(kernel, Shape::kSmem, configured));
         CUtensorMap q, k, v;
         if (!make_rows_map(&q, p.q, p.rows, p.heads, D, p.q_stride, Shape::kBox, pack, 128 / pack) ||
-            !make_rows_map(&k, p.k, p.rows, p.kv_heads, D, p.k_stride, Shape::kBox, 1, kPromptKeys) ||
-            !make_rows_map(&v, p.v, p.rows, p.kv_heads, D, p.v_stride, Shape::kBox, 1, kPromptKeys))
+            !make_rows_map(&k, p.k, p.rows, p.kv_heads, D, p.k_stride, Shape::kBox, 1, Shape::kKeys) ||
+            !make_rows_map(&v, p.v, p.rows, p.kv_heads, D, p.v_stride, Shape::kBox, 1, Shape::kKeys))
             return PHONON_CUDA_DEVICE_ERROR;
-        CUDA_TRY(launch_pdl(prompt_bf16_kernel<D>, dim3(grid), dim3(kPromptThreads), Shape::kSmem, s, q, k, v, p));
+        CUDA_TRY(launch_pdl(prompt_bf16_kernel<D>, dim3(static_cast<unsigned>(ctas)), dim3(kPromptThreads), Shape::kSmem, s, q, k, v, p));
     } else {
         using Shape = PromptF32Shape<D>;
         const void* kernel = reinterpret_cast<const void*>(prompt_f32_kernel<D>);
-        const int pack = prompt_pack(p, 128);
-        if (const int rc = prompt_grid(p, p.heads / pack, &grid)) return rc;
+        const long long ctas = prompt_ctas(p, parts);
+        if (ctas > INT32_MAX) return PHONON_CUDA_CAPACITY;
         if (const int rc = enough_registers(kernel, kPromptF32Threads, kPromptF32Registers, enough)) return rc;
         CUDA_TRY(opt_in_smem(kernel, Shape::kSmem, configured));
-        CUDA_TRY(launch_pdl(prompt_f32_kernel<D>, dim3(grid), dim3(kPromptF32Threads), Shape::kSmem, s, p));
+        CUDA_TRY(launch_pdl(prompt_f32_kernel<D>, dim3(static_cast<unsigned>(ctas)), dim3(kPromptF32Threads), Shape::kSmem, s, p));
     }
     return PHONON_CUDA_OK;
 }
@@ -5049,13 +5044,14 @@ int phonon_cuda_prompt_attention_device(int device, const PhononCudaPromptAttent
     p.scale = static_cast<float>((a->scale > 0.0f ? static_cast<double>(a->scale) : 1.0 / std::sqrt(static_cast<double>(a->head_dim))) *
                                  1.4426950408889634074);
     DeviceGuard guard(device);
-    if (!guard.ok) return PHONON_CUDA_DEVICE_ERROR;
+    int sms = 0;
+    if (!guard.ok || device_sms(device, &sms)) return PHONON_CUDA_DEVICE_ERROR;
     cudaStream_t s = static_cast<cudaStream_t>(cuda_stream);
     const bool bf16 = a->type == PHONON_CUDA_ROWS_BF16;
     switch (a->head_dim) {
-        case 32: return bf16 ? prompt_launch<32, true>(p, s) : prompt_launch<32, false>(p, s);
-        case 64: return bf16 ? prompt_launch<64, true>(p, s) : prompt_launch<64, false>(p, s);
-        default: return bf16 ? prompt_launch<128, true>(p, s) : prompt_launch<128, false>(p, s);
+        case 32: return bf16 ? prompt_launch<32, true>(p, sms, s) : prompt_launch<32, false>(p, sms, s);
+        case 64: return bf16 ? prompt_launch<64, true>(p, sms, s) : prompt_launch<64, false>(p, sms, s);
+        default: return bf16 ? prompt_launch<128, true>(p, sms, s) : prompt_launch<128, false>(p, sms, s);
     }
 }
 

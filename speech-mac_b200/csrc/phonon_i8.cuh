@@ -126,10 +126,16 @@ __global__ void __launch_bounds__(256, kBf16 ? 4 : 3) i8_quantize_kernel(I8Quant
             uint32_t w[8];  // the low byte is the integer's
             float far = 0.0f;
 #pragma unroll
-            for (int k = 0; k < 8; ++k) {
-                const float near = fmaf(x.element(k), inverse, kRound);
-                far = fmaxf(far, fabsf(fmaf(kRound - near, s, x.element(k))));
-                w[k] = __float_as_uint(near);
+            for (int k = 0; k < 8; k += 2) {
+                const float2 e = make_float2(x.element(k), x.element(k + 1));
+                const float2 by = make_float2(inverse, inverse), unit = make_float2(s, s), one = make_float2(-1.0f, -1.0f), round = make_float2(kRound, kRound);
+                // (the second step: quotients that are a rounding of the scale away from a border, which bf16 rows have many of)
+                float2 near = fma2(e, by, round);
+                near = fma2(fma2(fma2(near, one, round), unit, e), by, near);
+                const float2 rest = fma2(fma2(near, one, round), unit, e);
+                far = fmaxf(far, fmaxf(fabsf(rest.x), fabsf(rest.y)));
+                w[k] = __float_as_uint(near.x);
+                w[k + 1] = __float_as_uint(near.y);
             }
             if (2.0f * far >= s) {
 #pragma unroll

@@ -23,7 +23,8 @@ struct PromptParams {
     int window;       // 0: none
     float scale;      // times log2(e)
     Kv8Div pack;      // query heads that share a tile's rows: all of a K/V head's, or one
-    int tokens;       // positions of a tile
+    int tokens;       // positions of a CTA
+    int half;         // positions of a row tile: a CTA has one or two
     Kv8Div by_heads;  // CTAs of a tile
 };
 
@@ -31,8 +32,8 @@ __device__ __forceinline__ void prompt_flag(const PromptParams& p, int i, int co
     if (p.status) atomicMax(p.status + i, code);
 }
 
-// The slot-th tile of the call: `tokens` positions of a prompt, the last ones
-// first (they see most). index < 0: the call has fewer tiles.
+// The slot-th tile of the call: the `tokens` positions of a prompt that a CTA
+// works on, the last ones first (they see most). index < 0: the call has fewer.
 struct PromptTile {
     int index, row0, length, first;  // prompt, its first row and rows, the tile's first position
 };
@@ -96,13 +97,13 @@ __device__ __forceinline__ PromptTile prompt_tile(const PromptParams& p, int slo
 }
 
 // ------------------------------------------------- bf16 rows on tcgen05
-// A CTA has two row tiles of 128 rows (a row is a position and one of the
+// A CTA has two row tiles (one, where that leaves SMs without) of 128 rows (a row is a position and one of the
 // `pack` query heads that share its K/V head), each with a softmax of four
 // warps, a row a thread: while one tile's scores become weights, the tensor
-// cores work for the other.
+// cores work for another.
 //
-//   warp 8     brings q, then 128 positions of k and of v a turn by TMA
-//   warp 9     issues S = q k^T and O += P v in turn for both tiles
+//   warp 8     brings q, then 64 or 128 positions of k and of v a turn by TMA
+//   warp 9     (and 10) issues S = q k^T and O += P v of the tiles
 //   warps 0-7  S to registers, its maximum, the weights 2^(s - M) as bf16 back
 //              over S (the A operand of P v), the sum of weights in fp32
 //
@@ -116,18 +117,22 @@ __device__ __forceinline__ PromptTile prompt_tile(const PromptParams& p, int slo
 // over, carefully: warp 8 looks at every turn's values, puts 0 in place of
 // those that are not finite, and the rows that see one become NaN. (Nothing is
 // written before: out may lie over q.)
-constexpr int kPromptThreads = 384, kPromptKeys = 128;
-// A thread's registers in warps 0-7 and 8-11, together the launch's 168 each.
-constexpr int kPromptSoftmaxRegisters = 208, kPromptOtherRegisters = 88;
-constexpr int kPromptRegisters = 256 * kPromptSoftmaxRegisters + 128 * kPromptOtherRegisters;
+constexpr int kPromptThreads = 384;
 constexpr float kPromptSlack = 8.0f;
 
+// 128 dims: 128 positions a turn, TMEM and registers of an SM for one CTA. Up
+// to 64 dims the exponentials are the most of the work, and 64 positions a turn
+// leave room for two CTAs: four tiles' softmaxes to keep their unit at work.
 template <int D>
 struct PromptShape {
     static constexpr int kBox = D < 64 ? D : 64, kBoxBytes = 2 * kBox, kBoxes = D / kBox;  // a row's piece of a tile
-    static constexpr int kStages = D == 128 ? 2 : 3;
-    static constexpr int kTile = 128 * D * 2;  // bytes of a tile of q, k or v
-    static constexpr int kSmem = 1024 + (2 + 2 * kStages) * kTile;
+    static constexpr int kCtas = D == 128 ? 1 : 2, kKeys = D == 128 ? 128 : 64, kIssuers = kCtas;
+    static constexpr int kStages = D == 128 ? 2 : 4, kTmemCols = 512 / kCtas;
+    static constexpr int kQTile = 128 * D * 2, kTile = kKeys * D * 2;  // bytes of a row tile of q, of a turn's keys or values
+    static constexpr int kSmem = 1024 + 2 * kQTile + 2 * kStages * kTile;
+    // A thread's registers in warps 0-7 and 8-11, together what the launch has for each.
+    static constexpr int kSoftmaxRegisters = kCtas == 1 ? 208 : 96, kOtherRegisters = kCtas == 1 ? 88 : 48;
+    static constexpr int kRegisters = 256 * kSoftmaxRegisters + 128 * kOtherRegisters;
 };
 
 __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
@@ -152,16 +157,12 @@ __device__ __forceinline__ uint64_t umma_desc_rows(uint32_t addr, uint32_t block
 
 constexpr uint32_t kUmmaBMnMajor = 1u << 16;  // of an instruction descriptor
 
-// 32 packed columns of the warp's 32 lanes into TMEM.
-__device__ __forceinline__ void tmem_store32(uint32_t taddr, const uint32_t (&r)[32]) {
+// 16 packed columns of the warp's 32 lanes into TMEM.
+__device__ __forceinline__ void tmem_store16(uint32_t taddr, const uint32_t (&r)[16]) {
     asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {"
-        "%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
-        "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
         "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
-        "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]),
-        "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]),
-        "r"(r[31])
+        "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
         : "memory");
 }
 
@@ -178,45 +179,56 @@ __device__ __forceinline__ uint32_t prompt_seen(int position, int window, int ke
     return bits;
 }
 
-// The keys that the positions [first, end) see, in turns of kPromptKeys from key0 on: [begin, end).
+// The keys that the positions [first, end) see, in turns of kKeys from key0 on: [begin, end).
 struct PromptTurns {
     int begin, end;
 };
+template <int kKeys>
 __device__ __forceinline__ PromptTurns prompt_turns(int first, int end, int window, int key0) {
     if (end <= first) return {0, 0};
     const int low = window ? max(0, first - window + 1) : 0;
-    return {(low - key0) / kPromptKeys, (end - key0 + kPromptKeys - 1) / kPromptKeys};
+    return {(low - key0) / kKeys, (end - key0 + kKeys - 1) / kKeys};
 }
 
 template <int D>
-__global__ void __launch_bounds__(kPromptThreads, 1)
+__global__ void __launch_bounds__(kPromptThreads, PromptShape<D>::kCtas)
     prompt_bf16_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                        const __grid_constant__ CUtensorMap tm_v, PromptParams p) {
     using Shape = PromptShape<D>;
-    constexpr int kStages = Shape::kStages, kTile = Shape::kTile, kBoxes = Shape::kBoxes, kBytes = Shape::kBoxBytes;
+    constexpr int kStages = Shape::kStages, kTile = Shape::kTile, kQTile = Shape::kQTile, kBoxes = Shape::kBoxes, kBytes = Shape::kBoxBytes;
+    constexpr int kKeys = Shape::kKeys, kIssuers = Shape::kIssuers, kParts = kKeys / 64;  // the weights go off 64 positions at a time
+    constexpr uint32_t kTmemO = 2 * kKeys;  // S of both tiles, the weights over it, then O
+    static_assert(kTmemO + 2 * D <= Shape::kTmemCols, "TMEM");
     extern __shared__ uint8_t smem_raw[];
-    __shared__ __align__(8) uint64_t s_bars[4 * kStages + 9];
+    __shared__ __align__(8) uint64_t s_bars[4 * kStages + 2 * kParts + 7];
     __shared__ uint32_t s_tmem;
     __shared__ int s_failed, s_dirty;
-    __shared__ uint32_t s_bad[kStages][kPromptKeys / 32];  // careful: which of a turn's values are not finite
-    const uint32_t s_q = (smem_addr(smem_raw) + 1023) & ~1023u, s_k = s_q + 2 * kTile, s_v = s_k + kStages * kTile;
+    __shared__ uint32_t s_bad[kStages][kKeys / 32];  // careful: which of a turn's values are not finite
+    const uint32_t s_q = (smem_addr(smem_raw) + 1023) & ~1023u, s_k = s_q + 2 * kQTile, s_v = s_k + kStages * kTile;
     const uint32_t k_full = smem_addr(s_bars), k_empty = k_full + 8 * kStages, v_full = k_empty + 8 * kStages, v_empty = v_full + 8 * kStages;
-    const uint32_t s_full = v_empty + 8 * kStages, p_full = s_full + 16, o_full = p_full + 16, q_full = o_full + 16, tail = q_full + 8, idle = tail + 8;
+    // by tile: S is there; the weights are (by part); the last P v is done
+    const uint32_t s_full = v_empty + 8 * kStages, p_full = s_full + 16, o_full = p_full + 16 * kParts;
+    const uint32_t q_full = o_full + 16, tail = q_full + 8, idle = tail + 8;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const auto init = [&](bool again) {  // one thread
         const auto set = [&](uint32_t bar, uint32_t count) {
             if (again) asm volatile("mbarrier.inval.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
             mbar_init(bar, count);
         };
-        for (int s = 0; s < 4 * kStages; ++s) set(k_full + 8 * s, 1);
+        for (int s = 0; s < kStages; ++s) {
+            set(k_full + 8 * s, 1);
+            set(k_empty + 8 * s, kIssuers);
+            set(v_full + 8 * s, 1);
+            set(v_empty + 8 * s, kIssuers);
+        }
         for (int s = 0; s < 2; ++s) {
             set(s_full + 8 * s, 1);
-            set(p_full + 8 * s, 4);
             set(o_full + 8 * s, 1);
         }
+        for (int s = 0; s < 2 * kParts; ++s) set(p_full + 8 * s, 4);
         set(q_full, 1);
         set(tail, 1);
-        set(idle, 1);
+        set(idle, kIssuers);
         s_failed = s_dirty = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     };
@@ -227,23 +239,21 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
     const PromptTile t = prompt_tile<kPromptThreads>(p, slot, blockIdx.x == gridDim.x - 1);
     if (t.index < 0) return;
     const int pack = static_cast<int>(p.pack.d), head0 = part * pack, kv_head = static_cast<int>(kv8_div(head0, p.group));
-    const int half = p.tokens / 2, end = min(t.length, t.first + p.tokens);  // tile s: [first + s * half, min(end, first + (s + 1) * half))
+    const int half = p.half, end = min(t.length, t.first + p.tokens);  // tile s: [first + s * half, min(end, first + (s + 1) * half))
     const int key0 = p.window ? max(0, t.first - p.window + 1) : 0;
-    const PromptTurns turns0 = prompt_turns(t.first, min(end, t.first + half), p.window, key0);
-    const PromptTurns turns1 = prompt_turns(t.first + half, end, p.window, key0);
+    const PromptTurns turns0 = prompt_turns<kKeys>(t.first, min(end, t.first + half), p.window, key0);
+    const PromptTurns turns1 = prompt_turns<kKeys>(t.first + half, end, p.window, key0);
     const int turns = max(turns0.end, turns1.end);
     if (warp == 9) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_addr(&s_tmem)) : "memory");
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&s_tmem)), "n"(Shape::kTmemCols) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-    const uint32_t tmem = s_tmem;  // S of both tiles, then O of both
+    const uint32_t tmem = s_tmem;
     const auto wait = [&](uint32_t bar, int use) {
-        const bool ok = mbar_wait(bar, use & 1, nullptr, &s_failed);
-        __syncwarp();
-        return __all_sync(kFull, ok);
+        return __all_sync(kFull, mbar_wait(bar, use & 1, nullptr, &s_failed));
     };
     bool careful = false;
     const auto sync = [] { asm volatile("bar.sync 1, %0;" ::"n"(kPromptThreads) : "memory"); };
@@ -260,44 +270,44 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
         return careful = true;
     };
     if (warp >= 8) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPromptOtherRegisters));
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Shape::kOtherRegisters));
         const bool two = turns1.end > 0;
         if (warp == 8) do {
-            const auto load = [&](uint32_t to, const CUtensorMap* map, int head, int row, uint32_t bar) {
+            const auto load = [&](uint32_t to, const CUtensorMap* map, int rows, int head, int row, uint32_t bar) {
 #pragma unroll
-                for (int b = 0; b < kBoxes; ++b) tma_load_3d(to + b * 128 * kBytes, map, b * Shape::kBox, head, row, bar);
+                for (int b = 0; b < kBoxes; ++b) tma_load_3d(to + b * rows * kBytes, map, b * Shape::kBox, head, row, bar);
             };
             if (lane == 0) {
                 mbar_expect_tx(q_full, (two ? 2 : 1) * half * pack * D * 2);
-                load(s_q, &tm_q, head0, t.row0 + t.first, q_full);
-                if (two) load(s_q + kTile, &tm_q, head0, t.row0 + t.first + half, q_full);
+                load(s_q, &tm_q, 128, head0, t.row0 + t.first, q_full);
+                if (two) load(s_q + kQTile, &tm_q, 128, head0, t.row0 + t.first + half, q_full);
             }
             int j = 0, looks = 0;
             for (; j < turns; ++j) {
-                const int s = j % kStages, row = t.row0 + key0 + j * kPromptKeys, there = end - key0 - j * kPromptKeys;
+                const int s = j % kStages, row = t.row0 + key0 + j * kKeys, there = end - key0 - j * kKeys;
                 if (j >= kStages && !wait(k_empty + 8 * s, j / kStages - 1)) break;
                 if (lane == 0) {
                     mbar_expect_tx(k_full + 8 * s, kTile);
-                    load(s_k + s * kTile, &tm_k, kv_head, row, k_full + 8 * s);
+                    load(s_k + s * kTile, &tm_k, kKeys, kv_head, row, k_full + 8 * s);
                 }
                 if (j >= kStages && !wait(v_empty + 8 * s, j / kStages - 1)) break;
-                const bool look = careful || there < kPromptKeys;  // what follows the prompt may not be finite: zeros
+                const bool look = careful || there < kKeys;  // what follows the prompt may not be finite: zeros
                 const uint32_t bar = look ? tail : v_full + 8 * s;
                 if (lane == 0) {
                     mbar_expect_tx(bar, kTile);
-                    load(s_v + s * kTile, &tm_v, kv_head, row, bar);
+                    load(s_v + s * kTile, &tm_v, kKeys, kv_head, row, bar);
                 }
                 if (!look) continue;
-                if (lane < kPromptKeys / 32) s_bad[s][lane] = 0;
+                if (lane < kKeys / 32) s_bad[s][lane] = 0;
                 if (!wait(tail, looks++)) break;
-                for (int x = lane; x < 128 * kBoxes; x += 32) {  // a key's box each
-                    const int key = x & 127;
+                for (int x = lane; x < kKeys * kBoxes; x += 32) {  // a key's box each
+                    const int key = x % kKeys;
                     const uint32_t at = s_v + s * kTile + x * kBytes;
                     bool bad = false;
                     for (int c = 0; c < kBytes; c += 16) {
                         uint32_t w[4] = {0, 0, 0, 0};
                         bool put = key >= there;
-                        if (!put) {
+                        if (careful && !put) {
                             asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(at + c));
 #pragma unroll
                             for (int k = 0; k < 4; ++k) {
@@ -320,49 +330,72 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
             }
             __syncwarp();
         } while (again());
-        else if (warp == 9) do {
-            constexpr uint32_t idesc_s = umma_idesc_bf16(128, kPromptKeys), idesc_o = umma_idesc_bf16(128, D) | kUmmaBMnMajor;
+        else if (warp < 9 + kIssuers) do {
+            constexpr uint32_t idesc_s = umma_idesc_bf16(128, kKeys), idesc_o = umma_idesc_bf16(128, D) | kUmmaBMnMajor;
+            constexpr int kSteps = kBytes / 32;  // of 16 dims in a row of a box
+            const int own = __shfl_sync(kFull, warp - 9, 0);
             uint32_t leader;
             asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.b32 %0, 1, 0, p;\n\t}" : "=r"(leader));
             const auto commit = [&](uint32_t bar) {
                 if (leader) umma_commit(bar);
             };
+            const uint64_t q_desc = umma_desc_rows<kBytes>(s_q), k_desc = umma_desc_rows<kBytes>(s_k);
+            const uint64_t v_desc = umma_desc_rows<kBytes>(s_v, kKeys * kBytes);
             bool ok = wait(q_full, 0);
-            const auto score = [&](int tile, const PromptTurns& in, int j) {
-                if (!ok || j < in.begin || j >= in.end) return;
+            int keys = 0, values = 0;  // turns known to be there (a wait takes a hundred clocks even if it ends at once)
+            const auto score = [&](int tile, int j, bool last) {
                 const int s = j % kStages;
-                if (!(ok = wait(k_full + 8 * s, j / kStages))) return;
-                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-    #pragma unroll
-                for (int k = 0; k < D / 16; ++k) {
-                    const uint32_t at = k / (kBytes / 32) * 128 * kBytes + k % (kBytes / 32) * 32;
-                    umma_half<false>(leader, tmem + tile * kPromptKeys, umma_desc_rows<kBytes>(s_q + tile * kTile + at),
-                                     umma_desc_rows<kBytes>(s_k + s * kTile + at), idesc_s, k != 0);
+                if (!ok || (j >= keys && !(ok = wait(k_full + 8 * s, j / kStages)))) return;
+                keys = j + 1;
+                const PromptTurns in = tile ? turns1 : turns0;
+                if (j >= in.begin && j < in.end) {
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    const uint64_t q = q_desc + tile * (kQTile / 16), kk = k_desc + s * (kTile / 16);
+#pragma unroll
+                    for (int k = 0; k < D / 16; ++k)
+                        umma_half<false>(leader, tmem + tile * kKeys, q + (k / kSteps * 128 * kBytes + k % kSteps * 32) / 16,
+                                         kk + (k / kSteps * kKeys * kBytes + k % kSteps * 32) / 16, idesc_s, k != 0);
+                    commit(s_full + 8 * tile);
                 }
-                commit(s_full + 8 * tile);
+                if (last) commit(k_empty + 8 * s);
             };
-            const auto sum = [&](int tile, const PromptTurns& in, int j) {
-                if (!ok || j < in.begin || j >= in.end) return;
+            const auto sum = [&](int tile, int j, bool last) {
                 const int s = j % kStages;
-                if (!(ok = wait(v_full + 8 * s, j / kStages) && wait(p_full + 8 * tile, j - in.begin))) return;
-                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-    #pragma unroll
-                for (int k = 0; k < kPromptKeys / 16; ++k)
-                    umma_half<true>(leader, tmem + 2 * kPromptKeys + tile * D, tmem + tile * kPromptKeys + k * 8,
-                                    umma_desc_rows<kBytes>(s_v + s * kTile + k * 16 * kBytes, 128 * kBytes), idesc_o, j != in.begin || k != 0);
-                if (j + 1 == in.end) commit(o_full + 8 * tile);
+                if (!ok || (j >= values && !(ok = wait(v_full + 8 * s, j / kStages)))) return;
+                values = j + 1;
+                // (and the keys that come next)
+                if (j + 1 < turns && j + 1 >= keys && !(ok = wait(k_full + 8 * ((j + 1) % kStages), (j + 1) / kStages))) return;
+                if (j + 1 < turns) keys = j + 2;
+                const PromptTurns in = tile ? turns1 : turns0;
+                if (j >= in.begin && j < in.end) {
+                    const uint64_t v = v_desc + s * (kTile / 16);
+#pragma unroll
+                    for (int h = 0; h < kParts; ++h) {
+                        if (!(ok = wait(p_full + 8 * (tile * kParts + h), j - in.begin))) return;
+                        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+#pragma unroll
+                        for (int k = 4 * h; k < 4 * h + 4; ++k)
+                            umma_half<true>(leader, tmem + kTmemO + tile * D, tmem + tile * kKeys + k * 8, v + k * kBytes, idesc_o, j != in.begin || k != 0);
+                    }
+                    if (j + 1 == in.end) commit(o_full + 8 * tile);
+                }
+                if (last) commit(v_empty + 8 * s);
             };
-            score(0, turns0, 0);
-            score(1, turns1, 0);
-            commit(k_empty);
-            for (int j = 0; ok && j < turns; ++j) {
-                sum(0, turns0, j);
-                score(0, turns0, j + 1);
-                sum(1, turns1, j);
-                commit(v_empty + 8 * (j % kStages));
-                if (j + 1 < turns) {
-                    score(1, turns1, j + 1);
-                    commit(k_empty + 8 * ((j + 1) % kStages));
+            if constexpr (kIssuers == 2) {
+                score(own, 0, true);
+                for (int j = 0; ok && j < turns; ++j) {
+                    sum(own, j, true);
+                    if (j + 1 < turns) score(own, j + 1, true);
+                }
+            } else {
+                score(0, 0, false);
+                score(1, 0, true);
+                for (int j = 0; ok && j < turns; ++j) {
+                    const bool more = j + 1 < turns;
+                    sum(0, j, false);
+                    if (more) score(0, j + 1, false);
+                    sum(1, j, true);
+                    if (more) score(1, j + 1, true);
                 }
             }
             commit(idle);  // no product is on its way when the CTA gives its memory back
@@ -372,13 +405,13 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
         else do {
         } while (again());
     } else {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kPromptSoftmaxRegisters));
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Shape::kSoftmaxRegisters));
         const int tile = warp >> 2, quarter = warp & 3, r = quarter * 32 + lane;
         const PromptTurns in = tile ? turns1 : turns0;
         const int first = t.first + tile * half, at = static_cast<int>(kv8_div(r, p.pack)), position = first + at;
         const int last = min(end, first + half) - 1;  // the tile's last position
-        const uint32_t at_s = tmem + tile * kPromptKeys + (static_cast<uint32_t>(quarter * 32) << 16);
-        const uint32_t at_o = tmem + 2 * kPromptKeys + tile * D + (static_cast<uint32_t>(quarter * 32) << 16);
+        const uint32_t at_s = tmem + tile * kKeys + (static_cast<uint32_t>(quarter * 32) << 16);
+        const uint32_t at_o = tmem + kTmemO + tile * D + (static_cast<uint32_t>(quarter * 32) << 16);
         const bool mine = at < half && position <= last;
         uint32_t w[D / 2];  // the row's output
         bool good = true;
@@ -387,28 +420,28 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
             for (int j = in.begin; j < in.end; ++j) {
                 wait(s_full + 8 * tile, j - in.begin);
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                float s[4][32];
+                float s[kKeys / 32][32];
 #pragma unroll
-                for (int c = 0; c < 4; ++c) tmem_start(at_s + 32 * c, s[c]);
+                for (int c = 0; c < kKeys / 32; ++c) tmem_start(at_s + 32 * c, s[c]);
 #pragma unroll
-                for (int c = 0; c < 4; ++c) tmem_arrived(s[c]);
-                const int key = key0 + j * kPromptKeys;
-                if (key + kPromptKeys - 1 > first || (p.window && key <= last - p.window)) {  // not all of it by every row
+                for (int c = 0; c < kKeys / 32; ++c) tmem_arrived(s[c]);
+                const int key = key0 + j * kKeys;
+                if (key + kKeys - 1 > first || (p.window && key <= last - p.window)) {  // not all of it by every row
 #pragma unroll
-                    for (int c = 0; c < 4; ++c) {
+                    for (int c = 0; c < kKeys / 32; ++c) {
                         const uint32_t bits = prompt_seen(position, p.window, key + 32 * c);
 #pragma unroll
                         for (int k = 0; k < 32; ++k) s[c][k] = bits >> k & 1 ? s[c][k] : -INFINITY;
                     }
                 }
-                float top[4];
+                float top[kKeys / 32];
 #pragma unroll
-                for (int c = 0; c < 4; ++c) {
+                for (int c = 0; c < kKeys / 32; ++c) {
                     top[c] = fmaxf(s[c][0], s[c][1]);
 #pragma unroll
                     for (int k = 2; k < 32; k += 2) top[c] = max3(top[c], s[c][k], s[c][k + 1]);
                 }
-                const float now = fmaxf(max3(top[0], top[1], top[2]), top[3]) * p.scale;
+                const float now = (kParts == 2 ? fmaxf(max3(top[0], top[1], top[kParts]), top[2 * kParts - 1]) : fmaxf(top[0], top[1])) * p.scale;
                 const bool move = now > m + kPromptSlack;
                 if (__any_sync(kFull, move)) {
                     const float to = move ? now : m;
@@ -417,14 +450,13 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
                     l *= by;
                     if (j != in.begin) {
 #pragma unroll 1
-                        for (int c = 0; c < D; c += 32) {
-                            float o[32];
-                            tmem_start(at_o + c, o);
-                            tmem_arrived(o);
-                            uint32_t w[32];
+                        for (int c = 0; c < D; c += 8) {
+                            uint32_t o[8];
+                            tmem_ld8(at_o + c, o, 0);
+                            tmem_wait_ld();
 #pragma unroll
-                            for (int k = 0; k < 32; ++k) w[k] = __float_as_uint(o[k] * by);
-                            tmem_store32(at_o + c, w);
+                            for (int k = 0; k < 8; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * by);
+                            tmem_store8(at_o + c, o);
                         }
                     }
                 }
@@ -432,29 +464,31 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
                 const float2 scale = make_float2(p.scale, p.scale), from2 = make_float2(from, from);
                 float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    uint32_t w[32];
+                for (int h = 0; h < kParts; ++h) {
 #pragma unroll
-                    for (int k = 0; k < 32; ++k) {
-                        const float* x = &s[2 * h + k / 16][2 * (k % 16)];
-                        const float2 z = fma2(make_float2(x[0], x[1]), scale, from2);
-                        const float2 e = make_float2(ex2(z.x), ex2(z.y));
-                        sum[k & 1] = add2(sum[k & 1], e);
-                        w[k] = bf16x2_bits(e.x, e.y);
+                    for (int c = 0; c < 2; ++c) {
+                        uint32_t x[16];
+#pragma unroll
+                        for (int k = 0; k < 16; ++k) {
+                            const float2 z = fma2(make_float2(s[2 * h + c][2 * k], s[2 * h + c][2 * k + 1]), scale, from2);
+                            const float2 e = make_float2(ex2(z.x), ex2(z.y));
+                            sum[k & 1] = add2(sum[k & 1], e);
+                            x[k] = bf16x2_bits(e.x, e.y);
+                        }
+                        tmem_store16(at_s + 32 * h + 16 * c, x);
                     }
-                    tmem_store32(at_s + 32 * h, w);
+                    if (careful && h + 1 == kParts) {
+                        wait(v_full + 8 * (j % kStages), j / kStages);
+                        for (int c = 0; c < kKeys / 32; ++c)
+                            if (s_bad[j % kStages][c] & prompt_seen(position, p.window, key + 32 * c)) l = __int_as_float(0x7fc00000);
+                    }
+                    asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+                    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(p_full + 8 * (tile * kParts + h));
                 }
                 const float2 both = add2(sum[0], sum[1]);
                 l += both.x + both.y;
-                if (careful) {
-                    wait(v_full + 8 * (j % kStages), j / kStages);
-                    for (int c = 0; c < kPromptKeys / 32; ++c)
-                        if (s_bad[j % kStages][c] & prompt_seen(position, p.window, key + 32 * c)) l = __int_as_float(0x7fc00000);
-                }
-                asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-                asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-                __syncwarp();
-                if (lane == 0) mbar_arrive(p_full + 8 * tile);
             }
             if (in.end > in.begin) wait(o_full + 8 * tile, 0);
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -490,7 +524,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
     __syncthreads();
     if (warp == 9) {
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(Shape::kTmemCols) : "memory");
     }
 }
 

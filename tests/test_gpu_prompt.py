@@ -178,6 +178,25 @@ def test_what_a_row_does_not_see_does_not_matter(cuda_ok, dim, bf16):
 
 
 @pytest.mark.parametrize("bf16", [True, False])
+@pytest.mark.parametrize("dim", [32, 64, 128])
+@pytest.mark.parametrize("length", [1, 40, 70, 200])
+def test_values_that_are_not_finite_in_short_prompts(cuda_ok, length, dim, bf16):
+    """The turns that a prompt ends in: every row from the value on sees it, whatever its place."""
+    rng = np.random.default_rng(length)
+    for bad in sorted({0, length // 2, length - 1}):
+        packed, q, k, v = rows_of(rng, length, 2, 2, dim, bf16)
+        v[bad, 0, dim - 1] = float("inf")
+        k[bad, 1, 0] = float("nan")
+        out = torch.empty(length, 2, dim, dtype=packed.dtype, device="cuda")
+        status = torch.zeros(1, dtype=torch.int32, device="cuda")
+        call(q, k, v, out, [0, length], bf16=bf16)(status.data_ptr())
+        torch.cuda.synchronize()
+        assert status.tolist() == [rt.NON_FINITE]
+        broken = ~out.isfinite().all(-1)
+        assert not broken[:bad].any() and broken[bad:].all()
+
+
+@pytest.mark.parametrize("bf16", [True, False])
 def test_rows_of_bad_prompts_stay(cuda_ok, bf16):
     rng = np.random.default_rng(8)
     packed, q, k, v = rows_of(rng, 400, 2, 2, 64, bf16)
