@@ -197,6 +197,7 @@ __global__ void __launch_bounds__(kPromptThreads, PromptShape<D>::kCtas)
     using Shape = PromptShape<D>;
     constexpr int kStages = Shape::kStages, kTile = Shape::kTile, kQTile = Shape::kQTile, kBoxes = Shape::kBoxes, kBytes = Shape::kBoxBytes;
     constexpr int kKeys = Shape::kKeys, kIssuers = Shape::kIssuers, kParts = kKeys / 64;  // the weights go off 64 positions at a time
+    constexpr int kWide = Shape::kCtas == 1 ? 4 : 1;  // 8 columns of O that registers are free for
     constexpr uint32_t kTmemO = 2 * kKeys;  // S of both tiles, the weights over it, then O
     static_assert(kTmemO + 2 * D <= Shape::kTmemCols, "TMEM");
     extern __shared__ uint8_t smem_raw[];
@@ -450,13 +451,18 @@ __global__ void __launch_bounds__(kPromptThreads, PromptShape<D>::kCtas)
                     l *= by;
                     if (j != in.begin) {
 #pragma unroll 1
-                        for (int c = 0; c < D; c += 8) {
-                            uint32_t o[8];
-                            tmem_ld8(at_o + c, o, 0);
+                        for (int c = 0; c < D; c += 8 * kWide) {
+                            uint32_t o[8 * kWide];
+#pragma unroll
+                            for (int k = 0; k < 8 * kWide; k += 8) tmem_ld8(at_o + c + k, o, k);
                             tmem_wait_ld();
 #pragma unroll
-                            for (int k = 0; k < 8; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * by);
-                            tmem_store8(at_o + c, o);
+                            for (int k = 0; k < 8 * kWide; k += 8) {
+                                uint32_t x[8];
+#pragma unroll
+                                for (int i = 0; i < 8; ++i) x[i] = __float_as_uint(__uint_as_float(o[k + i]) * by);
+                                tmem_store8(at_o + c + k, x);
+                            }
                         }
                     }
                 }
@@ -535,7 +541,8 @@ __global__ void __launch_bounds__(kPromptThreads, PromptShape<D>::kCtas)
 // of 128 rows and 64 positions a turn:
 //
 //   warps 8-15  read k and v, and write their slices as matrix operands
-//   warp 4      issues S = q k^T a turn ahead, and P v
+//   warps 4, 5  issue S = q k^T a turn ahead, and P v (one warp for both was
+//               the slowest part: a wait takes it 200 clocks)
 //   warps 0-3   a row a thread: q times the softmax scale into TMEM (the A
 //               operand of S), S to weights, their slices back over S, and the
 //               sum of P v over the turns in registers (the tensor cores' own
@@ -557,6 +564,7 @@ struct PromptF32Shape {
     static constexpr int kPlane = kPromptF32Keys * D * 2;  // bytes of a slice of a turn's keys or values
     static constexpr int kSmem = 1024 + 2 * kStages * 3 * kPlane;
     static constexpr int kUnits = D / 32;  // of 8 elements a converting thread has, of a turn's keys and of its values
+    static constexpr int kBatch = kUnits < 2 ? kUnits : 2, kParts = kUnits / kBatch;  // of them at a time
 };
 
 // The three slices of a pair, the first in the low half; exact but for the
@@ -578,17 +586,17 @@ constexpr float kBf16Most = 3.38953139e38f;  // the largest bf16
 template <int D>
 __global__ void __launch_bounds__(kPromptF32Threads, 1) prompt_f32_kernel(PromptParams p) {
     using Shape = PromptF32Shape<D>;
-    constexpr int kStages = Shape::kStages, kPlane = Shape::kPlane, kBytes = Shape::kBoxBytes, kKeys = kPromptF32Keys, kUnits = Shape::kUnits;
+    constexpr int kStages = Shape::kStages, kPlane = Shape::kPlane, kBytes = Shape::kBoxBytes, kKeys = kPromptF32Keys, kBatch = Shape::kBatch, kParts = Shape::kParts;
     constexpr uint32_t kTmemS = 3 * D / 2, kSCols = 96, kTmemO = kTmemS + 2 * kSCols;  // q's slices, S and the weights' slices twice, O
     static_assert(kTmemO + D <= 512, "TMEM");
     extern __shared__ uint8_t smem_raw[];
-    __shared__ __align__(8) uint64_t s_bars[4 * kStages + 6];
+    __shared__ __align__(8) uint64_t s_bars[4 * kStages + 9];
     __shared__ uint32_t s_tmem;
     __shared__ int s_failed, s_dirty;
     __shared__ unsigned long long s_bad[2][kStages];  // careful: which of a turn's keys, values are not finite
     const uint32_t s_k = (smem_addr(smem_raw) + 1023) & ~1023u, s_v = s_k + kStages * 3 * kPlane;
     const uint32_t k_full = smem_addr(s_bars), k_empty = k_full + 8 * kStages, v_full = k_empty + 8 * kStages, v_empty = v_full + 8 * kStages;
-    const uint32_t s_full = v_empty + 8 * kStages, p_full = s_full + 16, o_full = p_full + 8, q_full = o_full + 8, idle = q_full + 8;
+    const uint32_t s_full = v_empty + 8 * kStages, p_full = s_full + 16, o_full = p_full + 8, q_full = o_full + 32, idle = q_full + 8;  // P v of a turn: by turn % 4
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const auto init = [&](bool again) {  // one thread
         const auto set = [&](uint32_t bar, uint32_t count) {
@@ -604,9 +612,9 @@ __global__ void __launch_bounds__(kPromptF32Threads, 1) prompt_f32_kernel(Prompt
         set(s_full, 1);
         set(s_full + 8, 1);
         set(p_full, 4);
-        set(o_full, 1);
+        for (int s = 0; s < 4; ++s) set(o_full + 8 * s, 1);
         set(q_full, 4);
-        set(idle, 1);
+        set(idle, 2);
         s_failed = s_dirty = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     };
@@ -654,40 +662,43 @@ __global__ void __launch_bounds__(kPromptF32Threads, 1) prompt_f32_kernel(Prompt
             const int u0 = (warp - 8) * 32 + lane;
             const float* base[2] = {static_cast<const float*>(p.k) + static_cast<size_t>(t.row0 + key0) * p.k_stride + kv_head * D,
                                     static_cast<const float*>(p.v) + static_cast<size_t>(t.row0 + key0) * p.v_stride + kv_head * D};
-            const auto load = [&](float4 (&x)[kUnits][2], int which, int j) {
+            // batch n: the n-th of kParts pieces of a turn's keys, then of its values, then of the next turn
+            const int batches = turns * 2 * kParts;
+            const auto load = [&](float4 (&x)[kBatch][2], int n) {
+                const int which = n / kParts & 1, j = n / (2 * kParts);
 #pragma unroll
-                for (int i = 0; i < kUnits; ++i) {
-                    const int u = u0 + 256 * i, row = j * kKeys + u / kChunks;
+                for (int i = 0; i < kBatch; ++i) {
+                    const int u = u0 + 256 * (n % kParts * kBatch + i), row = j * kKeys + u / kChunks;
                     const float* at = base[which] + static_cast<size_t>(row) * (which ? p.v_stride : p.k_stride) + u % kChunks * 8;
-                    const bool in = j < turns && key0 + row < end;  // what follows the prompt does not count: zeros
+                    const bool in = n < batches && key0 + row < end;  // what follows the prompt does not count: zeros
                     x[i][0] = in ? *reinterpret_cast<const float4*>(at) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
                     x[i][1] = in ? *reinterpret_cast<const float4*>(at + 4) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
                 }
             };
-            const auto put = [&](float4 (&x)[kUnits][2], int which, int j) {
-                const int s = j % kStages;
-                bool ok = j < kStages || wait((which ? v_empty : k_empty) + 8 * s, j / kStages - 1);
-                if (careful) {  // (P v of the stage's last turn is behind what its rows read of s_bad)
-                    if (j >= kStages) ok &= wait(v_empty + 8 * s, j / kStages - 1);
-                    if (u0 == 0) s_bad[which][s] = 0;
-                    asm volatile("bar.sync 2, 256;" ::: "memory");
+            bool ok = true;
+            const auto put = [&](float4 (&x)[kBatch][2], int n) {
+                const int which = n / kParts & 1, j = n / (2 * kParts), s = j % kStages;
+                if (n >= batches) return;
+                if (n % kParts == 0) {
+                    if (j >= kStages) ok &= wait((which ? v_empty : k_empty) + 8 * s, j / kStages - 1);
+                    if (careful) {  // (P v of the stage's last turn is behind what its rows read of s_bad)
+                        if (j >= kStages) ok &= wait(v_empty + 8 * s, j / kStages - 1);
+                        if (u0 == 0) s_bad[which][s] = 0;
+                        asm volatile("bar.sync 2, 256;" ::: "memory");
+                    }
                 }
-                if (!ok) return;  // (every warp goes on to the last turn: they meet above)
+                if (!ok) return;  // (every warp goes on to the last batch: they meet above)
 #pragma unroll
-                for (int i = 0; i < kUnits; ++i) {
-                    const int u = u0 + 256 * i, row = u / kChunks, chunk = u % kChunks;
+                for (int i = 0; i < kBatch; ++i) {
+                    const int u = u0 + 256 * (n % kParts * kBatch + i), row = u / kChunks, chunk = u % kChunks;
                     uint32_t w[4][3];
                     float* f = &x[i][0].x;
 #pragma unroll
                     for (int k = 0; k < 4; ++k) bf16x2_slices(make_float2(f[2 * k], f[2 * k + 1]), w[k]);
                     if (careful) {
                         bool bad = false;
-#pragma unroll 1
-                        for (int k = 0; k < 8; ++k) {
-                            const float v = k < 4 ? k < 2 ? k ? x[i][0].y : x[i][0].x : k == 2 ? x[i][0].z : x[i][0].w
-                                                  : k < 6 ? k == 4 ? x[i][1].x : x[i][1].y : k == 6 ? x[i][1].z : x[i][1].w;
-                            bad |= !(fabsf(v) <= kBf16Most) && (!which || !isfinite(v));
-                        }
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) bad |= !(fabsf(f[k]) <= kBf16Most) && (!which || !isfinite(f[k]));
                         if (bad) atomicOr(&s_bad[which][s], 1ull << row);
 #pragma unroll
                         for (int k = 0; k < 4; ++k) {
@@ -710,57 +721,62 @@ __global__ void __launch_bounds__(kPromptF32Threads, 1) prompt_f32_kernel(Prompt
 #pragma unroll
                     for (int c = 0; c < 3; ++c) kv8_put16(at + c * kPlane, w[0][c], w[1][c], w[2][c], w[3][c]);
                 }
+                if (n % kParts + 1 < kParts) return;
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
                 if (lane == 0) mbar_arrive((which ? v_full : k_full) + 8 * s);
             };
-            float4 a[kUnits][2], b[kUnits][2];
-            load(a, 0, 0);
-            for (int j = 0; j < turns; ++j) {
-                load(b, 1, j);
-                put(a, 0, j);
-                load(a, 0, j + 1);
-                put(b, 1, j);
+            float4 a[kBatch][2], b[kBatch][2], c[kBatch][2];
+            load(a, 0);
+            load(b, 1);
+            load(c, 2);
+            for (int n = 0; n < batches; n += 3) {
+                put(a, n);
+                load(a, n + 3);
+                put(b, n + 1);
+                load(b, n + 4);
+                put(c, n + 2);
+                load(c, n + 5);
             }
         } while (again());
-        else if (warp == 4) do {
+        else if (warp <= 5) do {
             constexpr uint32_t idesc_s = umma_idesc_bf16(128, kKeys), idesc_o = umma_idesc_bf16(128, D) | kUmmaBMnMajor;
             uint32_t leader;
             asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.b32 %0, 1, 0, p;\n\t}" : "=r"(leader));
             const auto commit = [&](uint32_t bar) {
                 if (leader) umma_commit(bar);
             };
-            bool ok = wait(q_full, 0);
-            const auto score = [&](int j) {
-                const int s = j % kStages;
-                if (!ok || !(ok = wait(k_full + 8 * s, j / kStages))) return;
-                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-#pragma unroll
-                for (int i = 0; i < 6; ++i)
-#pragma unroll
-                    for (int k = 0; k < D / 16; ++k)
-                        umma_half<true>(leader, tmem + kTmemS + (j & 1) * kSCols, tmem + prompt_slice_a(i) * (D / 2) + k * 8,
-                                        umma_desc_rows<kBytes>(s_k + (s * 3 + prompt_slice_b(i)) * kPlane + k / (kBytes / 32) * kKeys * kBytes +
-                                                               k % (kBytes / 32) * 32),
-                                        idesc_s, (i | k) != 0);
-                commit(s_full + 8 * (j & 1));
-                commit(k_empty + 8 * s);
-            };
-            score(0);
+            const uint64_t k_desc = umma_desc_rows<kBytes>(s_k), v_desc = umma_desc_rows<kBytes>(s_v, kKeys * kBytes);
+            constexpr int kSteps = kBytes / 32;  // of 16 dims in a row of a box
+            bool ok = warp == 5 || wait(q_full, 0);
             for (int j = 0; ok && j < turns; ++j) {
-                if (j + 1 < turns) score(j + 1);
                 const int s = j % kStages;
-                if (!ok || !(ok = wait(v_full + 8 * s, j / kStages) && wait(p_full, j))) break;
-                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                const uint32_t at_s = tmem + kTmemS + (j & 1) * kSCols;
+                if (warp == 4) {
+                    // (P v of two turns before has read the weights that S goes over)
+                    if (j >= 2) ok = wait(o_full + 8 * ((j - 2) & 3), (j - 2) >> 2);
+                    if (!ok || !(ok = wait(k_full + 8 * s, j / kStages))) break;
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll
-                for (int i = 0; i < 6; ++i)
+                    for (int i = 0; i < 6; ++i)
 #pragma unroll
-                    for (int k = 0; k < kKeys / 16; ++k)
-                        umma_half<true>(leader, tmem + kTmemO, tmem + kTmemS + (j & 1) * kSCols + prompt_slice_a(i) * (kKeys / 2) + k * 8,
-                                        umma_desc_rows<kBytes>(s_v + (s * 3 + prompt_slice_b(i)) * kPlane + k * 16 * kBytes, kKeys * kBytes), idesc_o,
-                                        (i | k) != 0);
-                commit(o_full);
-                commit(v_empty + 8 * s);
+                        for (int k = 0; k < D / 16; ++k)
+                            umma_half<true>(leader, at_s, tmem + prompt_slice_a(i) * (D / 2) + k * 8,
+                                            k_desc + ((s * 3 + prompt_slice_b(i)) * kPlane + k / kSteps * kKeys * kBytes + k % kSteps * 32) / 16, idesc_s, (i | k) != 0);
+                    commit(s_full + 8 * (j & 1));
+                    commit(k_empty + 8 * s);
+                } else {
+                    if (!(ok = wait(v_full + 8 * s, j / kStages) && wait(p_full, j))) break;
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+#pragma unroll
+                    for (int i = 0; i < 6; ++i)
+#pragma unroll
+                        for (int k = 0; k < kKeys / 16; ++k)
+                            umma_half<true>(leader, tmem + kTmemO, at_s + prompt_slice_a(i) * (kKeys / 2) + k * 8,
+                                            v_desc + ((s * 3 + prompt_slice_b(i)) * kPlane + k * 16 * kBytes) / 16, idesc_o, (i | k) != 0);
+                    commit(o_full + 8 * (j & 3));
+                    commit(v_empty + 8 * s);
+                }
             }
             commit(idle);  // no product is on its way when the CTA gives its memory back
             mbar_settle(idle, 0);
@@ -802,7 +818,7 @@ __global__ void __launch_bounds__(kPromptF32Threads, 1) prompt_f32_kernel(Prompt
             for (int k = 0; k < D; ++k) o[k] = 0.0f;
             float m = -INFINITY, l = 0.0f, shrink = 1.0f;
             const auto add_output = [&](int j) {
-                wait(o_full, j);
+                wait(o_full + 8 * (j & 3), j >> 2);
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 const float2 by = make_float2(shrink, shrink);
 #pragma unroll
