@@ -42,58 +42,99 @@ struct PromptTile {
 // before an earlier prompt's has none: tiles never share rows, and there are at
 // most rows / tokens + prompts of them, one less for every prompt without.
 // `report`: one CTA of the last slot, which reads all prompts if there is such
-// a one.
-template <int kThreads>
-__device__ __forceinline__ PromptTile prompt_tile(const PromptParams& p, int slot, bool report) {
-    constexpr int kWarps = kThreads / 32;
-    __shared__ int s_count[kWarps], s_most[kWarps], s_tile[4];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    if (threadIdx.x == 0) s_tile[0] = -1;
+// a one. One warp, 128 prompts at a time.
+__device__ __forceinline__ void prompt_find(const PromptParams& p, int slot, bool report, PromptTile* out) {
+    const int lane = threadIdx.x & 31;
+    if (lane == 0) out->index = -1;
+    __syncwarp();
     int before = 0, most = 0;  // tiles and the largest begin of the prompts so far
-    for (int base = 0; base < p.prompts; base += kThreads) {
-        const int i = base + static_cast<int>(threadIdx.x);
-        const bool there = i < p.prompts;
-        const int b = there ? p.begin[i] : 0, e = there ? p.begin[i + 1] : 0;
-        int top = b;
+    int x[5], next[5];
+    const auto load = [&](int (&y)[5], int base) {
+#pragma unroll
+        for (int k = 0; k < 5; ++k) y[k] = base < p.prompts ? p.begin[min(base + 4 * lane + k, p.prompts)] : 0;
+    };
+    load(x, 0);
+    for (int base = 0; base < p.prompts; base += 128) {
+        load(next, base + 128);
+        const int i = base + 4 * lane;
+        int top = max(max(x[0], x[1]), max(x[2], x[3]));  // (of prompts behind the last: the last's end, which is no begin of theirs)
+        int highest = top;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-            const int x = __shfl_up_sync(kFull, top, o);
-            if (lane >= o) top = max(top, x);
+            const int y = __shfl_up_sync(kFull, highest, o);
+            if (lane >= o) highest = max(highest, y);
         }
-        if (lane == 31) s_most[warp] = top;
-        __syncthreads();
-        int earlier = most;
-        for (int w = 0; w < kWarps; ++w) {
-            if (w < warp) earlier = max(earlier, s_most[w]);
-            most = max(most, s_most[w]);
+        int earlier = __shfl_up_sync(kFull, highest, 1);
+        earlier = max(most, lane ? earlier : 0);
+        int tiles[4], mine = 0;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int b = x[k], e = x[k + 1];
+            const bool good = b >= earlier && e >= b && e <= p.rows && e - b <= p.max_rows;
+            if (i + k < p.prompts && !good && report) prompt_flag(p, i + k, kStatusInvalid);
+            tiles[k] = i + k < p.prompts && good ? (e - b + p.tokens - 1) / p.tokens : 0;
+            mine += tiles[k];
+            earlier = max(earlier, b);
         }
-        const bool good = b >= max(top, earlier) && e >= b && e <= p.rows && e - b <= p.max_rows;
-        if (there && !good && report) prompt_flag(p, i, kStatusInvalid);
-        const int tiles = there && good ? (e - b + p.tokens - 1) / p.tokens : 0;
-        int sum = tiles;
+        int sum = mine;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-            const int x = __shfl_up_sync(kFull, sum, o);
-            if (lane >= o) sum += x;
+            const int y = __shfl_up_sync(kFull, sum, o);
+            if (lane >= o) sum += y;
         }
-        if (lane == 31) s_count[warp] = sum;
-        __syncthreads();
-        int ahead = before;
-        for (int w = 0; w < kWarps; ++w) {
-            if (w < warp) ahead += s_count[w];
-            before += s_count[w];
+        int at = slot - (before + sum - mine);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            if (at >= 0 && at < tiles[k]) *out = PromptTile{i + k, x[k], x[k + 1] - x[k], (tiles[k] - 1 - at) * p.tokens};
+            at -= tiles[k];
         }
-        const int at = slot - (ahead + sum - tiles);
-        if (at >= 0 && at < tiles) {
-            s_tile[0] = i;
-            s_tile[1] = b;
-            s_tile[2] = e - b;
-            s_tile[3] = (tiles - 1 - at) * p.tokens;
-        }
-        if (slot < before) break;  // the same for every thread
+        before += __shfl_sync(kFull, sum, 31);
+        most = max(most, __shfl_sync(kFull, highest, 31));
+        if (slot < before) break;
+#pragma unroll
+        for (int k = 0; k < 5; ++k) x[k] = next[k];
     }
-    __syncthreads();
-    return {s_tile[0], s_tile[1], s_tile[2], s_tile[3]};
+}
+
+// Piece `piece` (16 bytes) of a staged row of kRow bytes: pieces are turned so
+// that neither a row's nor a piece of all rows share banks.
+template <int kRow>
+__device__ __forceinline__ uint32_t prompt_staged(uint32_t staging, int row, int piece) {
+    return staging + row * kRow + ((piece ^ (kRow == 64 ? row >> 1 & 3 : row & (kRow / 16 - 1))) * 16);
+}
+
+__device__ __forceinline__ float4 prompt_get16(uint32_t at) {
+    float4 v;
+    asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(at));
+    return v;
+}
+
+// Where a row tile's rows lie in the call's: row r is head r % pack of the
+// `part`-th group of `pack` at position first + r / pack, while that is before
+// `end` and r / pack below `half`. A pointer to it, or null.
+struct PromptRows {
+    int row0, first, half, end, head0;
+    __device__ __forceinline__ const uint8_t* at(const PromptParams& p, const void* base, long long stride, int dim, int size, int r) const {
+        const int token = static_cast<int>(kv8_div(r, p.pack)), position = first + token, head = head0 + r - token * static_cast<int>(p.pack.d);
+        if (token >= half || position >= end) return nullptr;
+        return static_cast<const uint8_t*>(base) + (static_cast<size_t>(row0 + position) * stride + static_cast<size_t>(head) * dim) * size;
+    }
+};
+
+// A warp's 32 staged rows (of kRow bytes, the part of a row at byte `from`) to
+// the output, whole sectors at a time.
+template <int kRow>
+__device__ __forceinline__ void prompt_put_rows(const PromptParams& p, const PromptRows& rows, uint32_t staging, int r0, int dim, int size, int from) {
+    constexpr int kPieces = kRow / 16, kEach = 32 / kPieces;
+    const int lane = threadIdx.x & 31;
+    __syncwarp();
+#pragma unroll 4
+    for (int i = 0; i < 32; i += kEach) {
+        const int r = i + lane / kPieces;
+        uint8_t* to = const_cast<uint8_t*>(rows.at(p, p.out, p.out_stride, dim, size, r0 + r));
+        if (to) *reinterpret_cast<float4*>(to + from + lane % kPieces * 16) = prompt_get16(prompt_staged<kRow>(staging, r, lane % kPieces));
+    }
+    __syncwarp();
 }
 
 // ------------------------------------------------- bf16 rows on tcgen05
@@ -203,6 +244,7 @@ __global__ void __launch_bounds__(kPromptThreads, PromptShape<D>::kCtas)
     extern __shared__ uint8_t smem_raw[];
     __shared__ __align__(8) uint64_t s_bars[4 * kStages + 2 * kParts + 7];
     __shared__ uint32_t s_tmem;
+    __shared__ PromptTile s_tile;
     __shared__ int s_failed, s_dirty;
     __shared__ uint32_t s_bad[kStages][kKeys / 32];  // careful: which of a turn's values are not finite
     const uint32_t s_q = (smem_addr(smem_raw) + 1023) & ~1023u, s_k = s_q + 2 * kQTile, s_v = s_k + kStages * kTile;
@@ -237,14 +279,7 @@ __global__ void __launch_bounds__(kPromptThreads, PromptShape<D>::kCtas)
     pdl_wait();
     pdl_trigger();
     const int slot = static_cast<int>(kv8_div(blockIdx.x, p.by_heads)), part = static_cast<int>(blockIdx.x - slot * p.by_heads.d);
-    const PromptTile t = prompt_tile<kPromptThreads>(p, slot, blockIdx.x == gridDim.x - 1);
-    if (t.index < 0) return;
-    const int pack = static_cast<int>(p.pack.d), head0 = part * pack, kv_head = static_cast<int>(kv8_div(head0, p.group));
-    const int half = p.half, end = min(t.length, t.first + p.tokens);  // tile s: [first + s * half, min(end, first + (s + 1) * half))
-    const int key0 = p.window ? max(0, t.first - p.window + 1) : 0;
-    const PromptTurns turns0 = prompt_turns<kKeys>(t.first, min(end, t.first + half), p.window, key0);
-    const PromptTurns turns1 = prompt_turns<kKeys>(t.first + half, end, p.window, key0);
-    const int turns = max(turns0.end, turns1.end);
+    if (warp == 0) prompt_find(p, slot, blockIdx.x == gridDim.x - 1, &s_tile);
     if (warp == 9) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&s_tmem)), "n"(Shape::kTmemCols) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -252,7 +287,21 @@ __global__ void __launch_bounds__(kPromptThreads, PromptShape<D>::kCtas)
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    const PromptTile t = s_tile;
     const uint32_t tmem = s_tmem;
+    const auto free_tmem = [&] {
+        if (warp == 9) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(Shape::kTmemCols) : "memory");
+    };
+    if (t.index < 0) {
+        free_tmem();
+        return;
+    }
+    const int pack = static_cast<int>(p.pack.d), head0 = part * pack, kv_head = static_cast<int>(kv8_div(head0, p.group));
+    const int half = p.half, end = min(t.length, t.first + p.tokens);  // tile s: [first + s * half, min(end, first + (s + 1) * half))
+    const int key0 = p.window ? max(0, t.first - p.window + 1) : 0;
+    const PromptTurns turns0 = prompt_turns<kKeys>(t.first, min(end, t.first + half), p.window, key0);
+    const PromptTurns turns1 = prompt_turns<kKeys>(t.first + half, end, p.window, key0);
+    const int turns = max(turns0.end, turns1.end);
     const auto wait = [&](uint32_t bar, int use) {
         return __all_sync(kFull, mbar_wait(bar, use & 1, nullptr, &s_failed));
     };
@@ -516,22 +565,18 @@ __global__ void __launch_bounds__(kPromptThreads, PromptShape<D>::kCtas)
             if (!good) s_dirty = 1;
             __syncwarp();
         } while (again());
-        if (mine) {
-            const int head = head0 + r - at * pack;
-            uint4* to = reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(p.out) + static_cast<size_t>(t.row0 + position) * p.out_stride +
-                                                 static_cast<size_t>(head) * D);
+        // through q's room, which nothing reads any more
+        const uint32_t staging = s_q + tile * kQTile + quarter * (32 * 2 * D);
 #pragma unroll
-            for (int k = 0; k < D / 8; ++k) to[k] = make_uint4(w[4 * k], w[4 * k + 1], w[4 * k + 2], w[4 * k + 3]);
-            if (!good) prompt_flag(p, t.index, s_failed ? kStatusDevice : kStatusNonFinite);
-        }
+        for (int k = 0; k < D / 8; ++k) kv8_put16(prompt_staged<2 * D>(staging, lane, k), w[4 * k], w[4 * k + 1], w[4 * k + 2], w[4 * k + 3]);
+        prompt_put_rows<2 * D>(p, PromptRows{t.row0, first, half, end, head0}, staging, quarter * 32, D, 2, 0);
+        if (!good) prompt_flag(p, t.index, s_failed ? kStatusDevice : kStatusNonFinite);
     }
     __syncwarp();
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
-    if (warp == 9) {
-        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(Shape::kTmemCols) : "memory");
-    }
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    free_tmem();
 }
 
 // ------------------------------------------------- fp32 rows on tcgen05
@@ -541,7 +586,7 @@ __global__ void __launch_bounds__(kPromptThreads, PromptShape<D>::kCtas)
 // of 128 rows and 64 positions a turn:
 //
 //   warps 8-15  read k and v, and write their slices as matrix operands
-//   warps 4, 5  issue S = q k^T a turn ahead, and P v (one warp for both was
+//   warps 4, 5  issue S = q k^T one or two turns ahead, and P v (one warp for both was
 //               the slowest part: a wait takes it 200 clocks)
 //   warps 0-3   a row a thread: q times the softmax scale into TMEM (the A
 //               operand of S), S to weights, their slices back over S, and the
@@ -561,8 +606,10 @@ template <int D>
 struct PromptF32Shape {
     static constexpr int kBox = D < 64 ? D : 64, kBoxBytes = 2 * kBox, kBoxes = D / kBox;
     static constexpr int kStages = D == 128 ? 2 : 3;
+    static constexpr int kBuffers = D == 128 ? 2 : 3;  // of S and the weights over it
     static constexpr int kPlane = kPromptF32Keys * D * 2;  // bytes of a slice of a turn's keys or values
-    static constexpr int kSmem = 1024 + 2 * kStages * 3 * kPlane;
+    static constexpr int kChunk = D < 64 ? D : 64, kStaging = 128 * kChunk * 4;  // dims of 128 rows at a time, on their way in and out
+    static constexpr int kSmem = 1024 + 2 * kStages * 3 * kPlane + kStaging;
     static constexpr int kUnits = D / 32;  // of 8 elements a converting thread has, of a turn's keys and of its values
     static constexpr int kBatch = kUnits < 2 ? kUnits : 2, kParts = kUnits / kBatch;  // of them at a time
 };
@@ -571,9 +618,10 @@ struct PromptF32Shape {
 // last one's rounding.
 __device__ __forceinline__ void bf16x2_slices(float2 x, uint32_t (&w)[3]) {
     w[0] = bf16x2_bits(x.x, x.y);
-    x = add2(x, make_float2(__uint_as_float(w[0] << 16 ^ 0x80000000u), __uint_as_float((w[0] & 0xffff0000u) ^ 0x80000000u)));
+    const float2 minus = make_float2(-1.0f, -1.0f);
+    x = fma2(make_float2(__uint_as_float(w[0] << 16), __uint_as_float(w[0] & 0xffff0000u)), minus, x);
     w[1] = bf16x2_bits(x.x, x.y);
-    x = add2(x, make_float2(__uint_as_float(w[1] << 16 ^ 0x80000000u), __uint_as_float((w[1] & 0xffff0000u) ^ 0x80000000u)));
+    x = fma2(make_float2(__uint_as_float(w[1] << 16), __uint_as_float(w[1] & 0xffff0000u)), minus, x);
     w[2] = bf16x2_bits(x.x, x.y);
 }
 
@@ -586,17 +634,18 @@ constexpr float kBf16Most = 3.38953139e38f;  // the largest bf16
 template <int D>
 __global__ void __launch_bounds__(kPromptF32Threads, 1) prompt_f32_kernel(PromptParams p) {
     using Shape = PromptF32Shape<D>;
-    constexpr int kStages = Shape::kStages, kPlane = Shape::kPlane, kBytes = Shape::kBoxBytes, kKeys = kPromptF32Keys, kBatch = Shape::kBatch, kParts = Shape::kParts;
-    constexpr uint32_t kTmemS = 3 * D / 2, kSCols = 96, kTmemO = kTmemS + 2 * kSCols;  // q's slices, S and the weights' slices twice, O
+    constexpr int kStages = Shape::kStages, kPlane = Shape::kPlane, kBytes = Shape::kBoxBytes, kKeys = kPromptF32Keys, kBatch = Shape::kBatch, kParts = Shape::kParts, kBuffers = Shape::kBuffers;
+    constexpr uint32_t kTmemS = 3 * D / 2, kSCols = 96, kTmemO = kTmemS + kBuffers * kSCols;  // q's slices, S with the weights' slices over it, O
     static_assert(kTmemO + D <= 512, "TMEM");
     extern __shared__ uint8_t smem_raw[];
-    __shared__ __align__(8) uint64_t s_bars[4 * kStages + 9];
+    __shared__ __align__(8) uint64_t s_bars[4 * kStages + kBuffers + 7];
     __shared__ uint32_t s_tmem;
+    __shared__ PromptTile s_tile;
     __shared__ int s_failed, s_dirty;
     __shared__ unsigned long long s_bad[2][kStages];  // careful: which of a turn's keys, values are not finite
     const uint32_t s_k = (smem_addr(smem_raw) + 1023) & ~1023u, s_v = s_k + kStages * 3 * kPlane;
     const uint32_t k_full = smem_addr(s_bars), k_empty = k_full + 8 * kStages, v_full = k_empty + 8 * kStages, v_empty = v_full + 8 * kStages;
-    const uint32_t s_full = v_empty + 8 * kStages, p_full = s_full + 16, o_full = p_full + 8, q_full = o_full + 32, idle = q_full + 8;  // P v of a turn: by turn % 4
+    const uint32_t s_full = v_empty + 8 * kStages, p_full = s_full + 8 * kBuffers, o_full = p_full + 8, q_full = o_full + 32, idle = q_full + 8;  // P v of a turn: by turn % 4
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const auto init = [&](bool again) {  // one thread
         const auto set = [&](uint32_t bar, uint32_t count) {
@@ -609,8 +658,7 @@ __global__ void __launch_bounds__(kPromptF32Threads, 1) prompt_f32_kernel(Prompt
             set(k_empty + 8 * s, 1);
             set(v_empty + 8 * s, 1);
         }
-        set(s_full, 1);
-        set(s_full + 8, 1);
+        for (int s = 0; s < kBuffers; ++s) set(s_full + 8 * s, 1);
         set(p_full, 4);
         for (int s = 0; s < 4; ++s) set(o_full + 8 * s, 1);
         set(q_full, 4);
@@ -622,11 +670,7 @@ __global__ void __launch_bounds__(kPromptF32Threads, 1) prompt_f32_kernel(Prompt
     pdl_wait();
     pdl_trigger();
     const int slot = static_cast<int>(kv8_div(blockIdx.x, p.by_heads)), part = static_cast<int>(blockIdx.x - slot * p.by_heads.d);
-    const PromptTile t = prompt_tile<kPromptF32Threads>(p, slot, blockIdx.x == gridDim.x - 1);
-    if (t.index < 0) return;
-    const int pack = static_cast<int>(p.pack.d), head0 = part * pack, kv_head = static_cast<int>(kv8_div(head0, p.group));
-    const int end = min(t.length, t.first + p.tokens), key0 = p.window ? max(0, t.first - p.window + 1) : 0;
-    const int turns = (end - key0 + kKeys - 1) / kKeys;
+    if (warp == 0) prompt_find(p, slot, blockIdx.x == gridDim.x - 1, &s_tile);
     if (warp == 4) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_addr(&s_tmem)) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -634,7 +678,18 @@ __global__ void __launch_bounds__(kPromptF32Threads, 1) prompt_f32_kernel(Prompt
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    const PromptTile t = s_tile;
     const uint32_t tmem = s_tmem;
+    const auto free_tmem = [&] {
+        if (warp == 4) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+    };
+    if (t.index < 0) {
+        free_tmem();
+        return;
+    }
+    const int pack = static_cast<int>(p.pack.d), head0 = part * pack, kv_head = static_cast<int>(kv8_div(head0, p.group));
+    const int end = min(t.length, t.first + p.tokens), key0 = p.window ? max(0, t.first - p.window + 1) : 0;
+    const int turns = (end - key0 + kKeys - 1) / kKeys;
     const auto wait = [&](uint32_t bar, int use) {
         const bool ok = mbar_wait(bar, use & 1, nullptr, &s_failed);
         __syncwarp();
@@ -750,11 +805,11 @@ __global__ void __launch_bounds__(kPromptF32Threads, 1) prompt_f32_kernel(Prompt
             constexpr int kSteps = kBytes / 32;  // of 16 dims in a row of a box
             bool ok = warp == 5 || wait(q_full, 0);
             for (int j = 0; ok && j < turns; ++j) {
-                const int s = j % kStages;
-                const uint32_t at_s = tmem + kTmemS + (j & 1) * kSCols;
+                const int s = j % kStages, before = j - kBuffers;
+                const uint32_t at_s = tmem + kTmemS + j % kBuffers * kSCols;
                 if (warp == 4) {
-                    // (P v of two turns before has read the weights that S goes over)
-                    if (j >= 2) ok = wait(o_full + 8 * ((j - 2) & 3), (j - 2) >> 2);
+                    // (P v of that turn has read the weights that S goes over)
+                    if (before >= 0) ok = wait(o_full + 8 * (before & 3), before >> 2);
                     if (!ok || !(ok = wait(k_full + 8 * s, j / kStages))) break;
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll
@@ -763,7 +818,7 @@ __global__ void __launch_bounds__(kPromptF32Threads, 1) prompt_f32_kernel(Prompt
                         for (int k = 0; k < D / 16; ++k)
                             umma_half<true>(leader, at_s, tmem + prompt_slice_a(i) * (D / 2) + k * 8,
                                             k_desc + ((s * 3 + prompt_slice_b(i)) * kPlane + k / kSteps * kKeys * kBytes + k % kSteps * 32) / 16, idesc_s, (i | k) != 0);
-                    commit(s_full + 8 * (j & 1));
+                    commit(s_full + 8 * (j % kBuffers));
                     commit(k_empty + 8 * s);
                 } else {
                     if (!(ok = wait(v_full + 8 * s, j / kStages) && wait(p_full, j))) break;
@@ -791,21 +846,40 @@ __global__ void __launch_bounds__(kPromptF32Threads, 1) prompt_f32_kernel(Prompt
         const int head = head0 + r - at * pack;
         const uint32_t lanes = tmem + (static_cast<uint32_t>(warp * 32) << 16);
         const float* q = static_cast<const float*>(p.q) + static_cast<size_t>(t.row0 + position) * p.q_stride + static_cast<size_t>(head) * D;
+        const PromptRows rows{t.row0, t.first, p.tokens, end, head0};
+        constexpr int kChunk = Shape::kChunk, kRow = 4 * kChunk, kPieces = kChunk / 4, kEach = 32 / kPieces;
+        const uint32_t staging = s_v + kStages * 3 * kPlane + warp * (32 * kRow);
         float o[D];
         bool good = true;
         do {
-#pragma unroll 1
+#pragma unroll
+            for (int c = 0; c < D; c += kChunk) {  // q, to where O will be: whole sectors, then by rows
+                float4 x[32 / kEach];
+#pragma unroll
+                for (int i = 0; i < 32 / kEach; ++i) {
+                    const uint8_t* from = rows.at(p, p.q, p.q_stride, D, 4, warp * 32 + i * kEach + lane / kPieces);
+                    x[i] = from ? *reinterpret_cast<const float4*>(from + c * 4 + lane % kPieces * 16) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                }
+#pragma unroll
+                for (int i = 0; i < 32 / kEach; ++i)
+                    kv8_put16(prompt_staged<kRow>(staging, i * kEach + lane / kPieces, lane % kPieces), __float_as_uint(x[i].x), __float_as_uint(x[i].y),
+                              __float_as_uint(x[i].z), __float_as_uint(x[i].w));
+                __syncwarp();
+#pragma unroll
+                for (int k = 0; k < kPieces; ++k) {
+                    const float4 y = prompt_get16(prompt_staged<kRow>(staging, lane, k));
+                    o[c + 4 * k] = y.x, o[c + 4 * k + 1] = y.y, o[c + 4 * k + 2] = y.z, o[c + 4 * k + 3] = y.w;
+                }
+                __syncwarp();
+            }
+#pragma unroll
             for (int c = 0; c < D; c += 16) {
                 uint32_t w[3][8];
 #pragma unroll
-                for (int k = 0; k < 8; k += 2) {
-                    const float4 x = mine ? *reinterpret_cast<const float4*>(q + c + 2 * k) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        uint32_t three[3];
-                        bf16x2_slices(h ? make_float2(x.z * p.scale, x.w * p.scale) : make_float2(x.x * p.scale, x.y * p.scale), three);
-                        w[0][k + h] = three[0], w[1][k + h] = three[1], w[2][k + h] = three[2];
-                    }
+                for (int k = 0; k < 8; ++k) {
+                    uint32_t three[3];
+                    bf16x2_slices(make_float2(o[c + 2 * k] * p.scale, o[c + 2 * k + 1] * p.scale), three);
+                    w[0][k] = three[0], w[1][k] = three[1], w[2][k] = three[2];
                 }
 #pragma unroll
                 for (int i = 0; i < 3; ++i) tmem_store8(lanes + i * (D / 2) + c / 2, w[i]);
@@ -835,8 +909,8 @@ __global__ void __launch_bounds__(kPromptF32Threads, 1) prompt_f32_kernel(Prompt
                 }
             };
             for (int j = 0; j < turns; ++j) {
-                const uint32_t at_s = lanes + kTmemS + (j & 1) * kSCols;
-                wait(s_full + 8 * (j & 1), j >> 1);
+                const uint32_t at_s = lanes + kTmemS + j % kBuffers * kSCols;
+                wait(s_full + 8 * (j % kBuffers), j / kBuffers);
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 float s[2][32];
                 tmem_start(at_s, s[0]);
@@ -881,11 +955,11 @@ __global__ void __launch_bounds__(kPromptF32Threads, 1) prompt_f32_kernel(Prompt
                 const float from = now == -INFINITY ? 0.0f : -now;  // nothing seen yet: weights 2^-inf
                 float2 sum = make_float2(0.0f, 0.0f);
 #pragma unroll
-                for (int h = 0; h < 4; ++h) {
-                    uint32_t w[3][8];
+                for (int h = 0; h < 2; ++h) {
+                    uint32_t w[3][16];
 #pragma unroll
-                    for (int k = 0; k < 8; ++k) {
-                        const float* x = &s[h / 2][16 * (h % 2) + 2 * k];
+                    for (int k = 0; k < 16; ++k) {
+                        const float* x = &s[h][2 * k];
                         const float2 z = add2(make_float2(x[0], x[1]), make_float2(from, from));
                         const float2 e = make_float2(ex2(z.x), ex2(z.y));
                         sum = add2(sum, e);
@@ -894,7 +968,7 @@ __global__ void __launch_bounds__(kPromptF32Threads, 1) prompt_f32_kernel(Prompt
                         w[0][k] = three[0], w[1][k] = three[1], w[2][k] = three[2];
                     }
 #pragma unroll
-                    for (int i = 0; i < 3; ++i) tmem_store8(at_s + i * (kKeys / 2) + h * 8, w[i]);
+                    for (int i = 0; i < 3; ++i) tmem_store16(at_s + i * (kKeys / 2) + h * 16, w[i]);
                 }
                 l += sum.x + sum.y;
                 if (j) add_output(j - 1);
@@ -916,21 +990,21 @@ __global__ void __launch_bounds__(kPromptF32Threads, 1) prompt_f32_kernel(Prompt
             if (!good) s_dirty = 1;
             __syncwarp();
         } while (again());
-        if (mine) {
-            float4* to = reinterpret_cast<float4*>(static_cast<float*>(p.out) + static_cast<size_t>(t.row0 + position) * p.out_stride +
-                                                   static_cast<size_t>(head) * D);
 #pragma unroll
-            for (int k = 0; k < D / 4; ++k) to[k] = make_float4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
-            if (!good) prompt_flag(p, t.index, s_failed ? kStatusDevice : kStatusNonFinite);
+        for (int c = 0; c < D; c += kChunk) {
+#pragma unroll
+            for (int k = 0; k < kPieces; ++k)
+                kv8_put16(prompt_staged<kRow>(staging, lane, k), __float_as_uint(o[c + 4 * k]), __float_as_uint(o[c + 4 * k + 1]),
+                          __float_as_uint(o[c + 4 * k + 2]), __float_as_uint(o[c + 4 * k + 3]));
+            prompt_put_rows<kRow>(p, rows, staging, warp * 32, D, 4, c * 4);
         }
+        if (!good) prompt_flag(p, t.index, s_failed ? kStatusDevice : kStatusNonFinite);
     }
     __syncwarp();
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
-    if (warp == 4) {
-        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
-    }
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    free_tmem();
 }
 
 }  // namespace phonon
