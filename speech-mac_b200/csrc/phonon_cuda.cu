@@ -4988,6 +4988,7 @@ int prompt_launch(PromptParams p, int sms, cudaStream_t s) {
         p.tokens *= 2;
         if (prompt_ctas(p, parts) < static_cast<long long>(sms) * Shape::kCtas) p.tokens = p.half;
         const long long ctas = prompt_ctas(p, parts);
+        p.by_tokens = kv8_divisor(static_cast<uint32_t>(p.tokens));
         if (ctas > INT32_MAX) return PHONON_CUDA_CAPACITY;
         if (const int rc = enough_registers(kernel, kPromptThreads, Shape::kRegisters, enough)) return rc;
         CUDA_TRY(opt_in_smem(kernel, Shape::kSmem, configured));
@@ -5001,6 +5002,7 @@ int prompt_launch(PromptParams p, int sms, cudaStream_t s) {
         using Shape = PromptF32Shape<D>;
         const void* kernel = reinterpret_cast<const void*>(prompt_f32_kernel<D>);
         const long long ctas = prompt_ctas(p, parts);
+        p.by_tokens = kv8_divisor(static_cast<uint32_t>(p.tokens));
         if (ctas > INT32_MAX) return PHONON_CUDA_CAPACITY;
         if (const int rc = enough_registers(kernel, kPromptF32Threads, kPromptF32Registers, enough)) return rc;
         CUDA_TRY(opt_in_smem(kernel, Shape::kSmem, configured));

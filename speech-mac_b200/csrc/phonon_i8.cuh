@@ -251,6 +251,13 @@ __device__ __forceinline__ void mbar_settle(uint32_t bar, uint32_t parity) {
     for (const long long since = clock64(); !mbar_test(bar, parity) && clock64() - since < kWaitBudgetCycles;) __nanosleep(20);
 }
 
+// The last phases of a ring of `stages` barriers that was used n times, which
+// nobody has waited for: no arrival is on its way when the CTA gives its
+// memory back or sets its barriers up anew (commits arrive in any order).
+__device__ __forceinline__ void mbar_settle_ring(uint32_t bars, int stages, int n) {
+    for (int j = max(0, n - stages); j < n; ++j) mbar_settle(bars + 8 * (j % stages), (j / stages) & 1);
+}
+
 // Many rows: tiles on the tcgen05 tensor cores, a CTA (or a pair of them) an SM
 // that takes tiles in turn. Warp 0 brings 128 bytes of depth a stage by TMA,
 // warp 1 issues the products into one of two accumulators in TMEM, and warps
@@ -389,6 +396,7 @@ __device__ __forceinline__ void i8_channels(const I8Params& p, int n0, float* sc
         scale[c] = n0 + c < p.channels ? p.w_scales[n0 + c] : 0.0f;
         bias[c] = p.bias && n0 + c < p.channels ? p.bias[n0 + c] : 0.0f;
     }
+    __syncwarp();
     asm volatile("bar.sync 1, 256;" ::: "memory");
 }
 
@@ -443,7 +451,7 @@ __global__ void __launch_bounds__(kI8Threads, 1)
             }
         }
         if (!ok)  // a wait ran out: no copy is on its way when the CTA gives its memory back
-            for (int j = max(0, it - kStages); j < it; ++j) mbar_settle(full + 8 * (j % kStages), (j / kStages) & 1);
+            mbar_settle_ring(full, kStages, it);
     } else if (warp == 1 && lane == 0) {
         constexpr uint32_t idesc = umma_idesc_i8(128, kN);
         int it = 0, turn = 0;
@@ -466,6 +474,7 @@ __global__ void __launch_bounds__(kI8Threads, 1)
         }
         umma_commit(idle);  // nor is a product
         mbar_settle(idle, 0);
+        if (ok) mbar_settle_ring(empty, kStages, it);
     } else if (warp >= 2) {
         const int quarter = warp & 3;
         int turn = 0;
@@ -561,12 +570,13 @@ __global__ void __launch_bounds__(kI8Threads, 1)
             tma_load_2d(stages + s * kStageBytes + 128 * 128, &tm_w, (first + k) * 128, n * kN, full + 8 * s);
         }
         if (!ok)  // a wait ran out: no copy is on its way when the CTA gives its memory back
-            for (int j = max(0, k - kStages); j < k; ++j) mbar_settle(full + 8 * (j % kStages), (j / kStages) & 1);
+            mbar_settle_ring(full, kStages, k);
     } else if (warp == 1 && lane == 0) {
         constexpr uint32_t idesc = umma_idesc_i8(128, kN);
+        bool ok = true;
         for (int k = 0; k < turns; ++k) {
             const int s = k % kStages;
-            if (!mbar_wait(full + 8 * s, (k / kStages) & 1, nullptr, &s_failed)) break;
+            if (!(ok = mbar_wait(full + 8 * s, (k / kStages) & 1, nullptr, &s_failed))) break;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             const uint32_t at = stages + s * kStageBytes;
 #pragma unroll
@@ -576,6 +586,7 @@ __global__ void __launch_bounds__(kI8Threads, 1)
         }
         umma_commit(done);
         mbar_settle(done, 0);  // nor is a product
+        if (ok) mbar_settle_ring(empty, kStages, turns);
     }
     __syncwarp();
     mbar_wait(done, 0, nullptr, &s_failed);
@@ -757,10 +768,12 @@ __global__ void __launch_bounds__(kI8Threads, 1) __cluster_dims__(2, 1, 1)
             }
             if (ok) commit(done + 8 * a);
         }
-        commit(idle);  // no product, and no arrival from one, is on its way when the CTAs give their memory back
+        commit(idle);  // no product is on its way when the CTAs give their memory back
         mbar_settle(idle, 0);
+        if (ok) mbar_settle_ring(empty, kStages, it);
     } else if (warp == 1 && lane == 0) {
         mbar_settle(idle, 0);
+        if (!*static_cast<volatile int*>(&s_failed)) mbar_settle_ring(empty, kStages, (tiles - first + step - 1) / step * nk);
     } else if (warp >= 2) {
         const int quarter = warp & 3;
         const uint32_t lead_drained = cluster_addr(drained, 0);

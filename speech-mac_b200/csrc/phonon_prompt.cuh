@@ -24,6 +24,7 @@ struct PromptParams {
     float scale;      // times log2(e)
     Kv8Div pack;      // query heads that share a tile's rows: all of a K/V head's, or one
     int tokens;       // positions of a CTA
+    Kv8Div by_tokens;
     int half;         // positions of a row tile: a CTA has one or two
     Kv8Div by_heads;  // CTAs of a tile
 };
@@ -72,7 +73,7 @@ __device__ __forceinline__ void prompt_find(const PromptParams& p, int slot, boo
             const int b = x[k], e = x[k + 1];
             const bool good = b >= earlier && e >= b && e <= p.rows && e - b <= p.max_rows;
             if (i + k < p.prompts && !good && report) prompt_flag(p, i + k, kStatusInvalid);
-            tiles[k] = i + k < p.prompts && good ? (e - b + p.tokens - 1) / p.tokens : 0;
+            tiles[k] = i + k < p.prompts && good ? static_cast<int>(kv8_div(static_cast<uint32_t>(e - b + p.tokens - 1), p.by_tokens)) : 0;
             mine += tiles[k];
             earlier = max(earlier, b);
         }
@@ -128,7 +129,7 @@ __device__ __forceinline__ void prompt_put_rows(const PromptParams& p, const Pro
     constexpr int kPieces = kRow / 16, kEach = 32 / kPieces;
     const int lane = threadIdx.x & 31;
     __syncwarp();
-#pragma unroll 4
+#pragma unroll 2
     for (int i = 0; i < 32; i += kEach) {
         const int r = i + lane / kPieces;
         uint8_t* to = const_cast<uint8_t*>(rows.at(p, p.out, p.out_stride, dim, size, r0 + r));
@@ -242,40 +243,44 @@ __global__ void __launch_bounds__(kPromptThreads, PromptShape<D>::kCtas)
     constexpr uint32_t kTmemO = 2 * kKeys;  // S of both tiles, the weights over it, then O
     static_assert(kTmemO + 2 * D <= Shape::kTmemCols, "TMEM");
     extern __shared__ uint8_t smem_raw[];
-    __shared__ __align__(8) uint64_t s_bars[4 * kStages + 2 * kParts + 7];
+    constexpr uint32_t kBars = 4 * kStages + 2 * kParts + 7;
+    __shared__ __align__(8) uint64_t s_bars[2 * kBars];
     __shared__ uint32_t s_tmem;
     __shared__ PromptTile s_tile;
     __shared__ int s_failed, s_dirty;
     __shared__ uint32_t s_bad[kStages][kKeys / 32];  // careful: which of a turn's values are not finite
     const uint32_t s_q = (smem_addr(smem_raw) + 1023) & ~1023u, s_k = s_q + 2 * kQTile, s_v = s_k + kStages * kTile;
-    const uint32_t k_full = smem_addr(s_bars), k_empty = k_full + 8 * kStages, v_full = k_empty + 8 * kStages, v_empty = v_full + 8 * kStages;
+    uint32_t bars = smem_addr(s_bars);  // of this pass
+    const auto k_full = [&] { return bars; };
+    const auto k_empty = [&] { return bars + 8 * kStages; };
+    const auto v_full = [&] { return bars + 16 * kStages; };
+    const auto v_empty = [&] { return bars + 24 * kStages; };
     // by tile: S is there; the weights are (by part); the last P v is done
-    const uint32_t s_full = v_empty + 8 * kStages, p_full = s_full + 16, o_full = p_full + 16 * kParts;
-    const uint32_t q_full = o_full + 16, tail = q_full + 8, idle = tail + 8;
+    const auto s_full = [&] { return bars + 32 * kStages; };
+    const auto p_full = [&] { return bars + 32 * kStages + 16; };
+    const auto o_full = [&] { return bars + 32 * kStages + 16 + 16 * kParts; };
+    const auto q_full = [&] { return bars + 32 * kStages + 32 + 16 * kParts; };
+    const auto tail = [&] { return q_full() + 8; };
+    const auto idle = [&] { return q_full() + 16; };
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const auto init = [&](bool again) {  // one thread
-        const auto set = [&](uint32_t bar, uint32_t count) {
-            if (again) asm volatile("mbarrier.inval.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
-            mbar_init(bar, count);
-        };
-        for (int s = 0; s < kStages; ++s) {
-            set(k_full + 8 * s, 1);
-            set(k_empty + 8 * s, kIssuers);
-            set(v_full + 8 * s, 1);
-            set(v_empty + 8 * s, kIssuers);
+    // Two sets: one for each of the CTA's passes.
+    if (threadIdx.x == 32) {
+        for (uint32_t set = 0; set < 2; ++set) {
+            const auto init = [&](uint32_t bar, int n, uint32_t count) {
+                for (int x = 0; x < n; ++x) mbar_init(bar + 8 * (set * kBars + x), count);
+            };
+            init(k_full(), kStages, 1);
+            init(k_empty(), kStages, kIssuers);
+            init(v_full(), kStages, 1);
+            init(v_empty(), kStages, kIssuers);
+            init(s_full(), 2, 1);
+            init(p_full(), 2 * kParts, 4);
+            init(o_full(), 4, 1);  // and q_full(), tail()
+            init(idle(), 1, kIssuers);
         }
-        for (int s = 0; s < 2; ++s) {
-            set(s_full + 8 * s, 1);
-            set(o_full + 8 * s, 1);
-        }
-        for (int s = 0; s < 2 * kParts; ++s) set(p_full + 8 * s, 4);
-        set(q_full, 1);
-        set(tail, 1);
-        set(idle, kIssuers);
         s_failed = s_dirty = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    };
-    if (threadIdx.x == 0) init(false);
+    }
     pdl_wait();
     pdl_trigger();
     const int slot = static_cast<int>(kv8_div(blockIdx.x, p.by_heads)), part = static_cast<int>(blockIdx.x - slot * p.by_heads.d);
@@ -306,17 +311,17 @@ __global__ void __launch_bounds__(kPromptThreads, PromptShape<D>::kCtas)
         return __all_sync(kFull, mbar_wait(bar, use & 1, nullptr, &s_failed));
     };
     bool careful = false;
-    const auto sync = [] { asm volatile("bar.sync 1, %0;" ::"n"(kPromptThreads) : "memory"); };
+    const auto sync = [] {
+        __syncwarp();
+        asm volatile("bar.sync 1, %0;" ::"n"(kPromptThreads) : "memory");
+    };
     // Every warp, at its end: whether the CTA starts over.
     const auto again = [&] {
         asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
         sync();
-        const bool redo = !careful && s_dirty && !s_failed;
-        if (!redo) return false;
-        sync();
-        if (threadIdx.x == 0) init(true);
-        sync();
+        if (careful || !s_dirty || s_failed) return false;
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        bars += 8 * kBars;
         return careful = true;
     };
     if (warp >= 8) {
@@ -328,28 +333,28 @@ __global__ void __launch_bounds__(kPromptThreads, PromptShape<D>::kCtas)
                 for (int b = 0; b < kBoxes; ++b) tma_load_3d(to + b * rows * kBytes, map, b * Shape::kBox, head, row, bar);
             };
             if (lane == 0) {
-                mbar_expect_tx(q_full, (two ? 2 : 1) * half * pack * D * 2);
-                load(s_q, &tm_q, 128, head0, t.row0 + t.first, q_full);
-                if (two) load(s_q + kQTile, &tm_q, 128, head0, t.row0 + t.first + half, q_full);
+                mbar_expect_tx(q_full(), (two ? 2 : 1) * half * pack * D * 2);
+                load(s_q, &tm_q, 128, head0, t.row0 + t.first, q_full());
+                if (two) load(s_q + kQTile, &tm_q, 128, head0, t.row0 + t.first + half, q_full());
             }
             int j = 0, looks = 0;
             for (; j < turns; ++j) {
                 const int s = j % kStages, row = t.row0 + key0 + j * kKeys, there = end - key0 - j * kKeys;
-                if (j >= kStages && !wait(k_empty + 8 * s, j / kStages - 1)) break;
+                if (j >= kStages && !wait(k_empty() + 8 * s, j / kStages - 1)) break;
                 if (lane == 0) {
-                    mbar_expect_tx(k_full + 8 * s, kTile);
-                    load(s_k + s * kTile, &tm_k, kKeys, kv_head, row, k_full + 8 * s);
+                    mbar_expect_tx(k_full() + 8 * s, kTile);
+                    load(s_k + s * kTile, &tm_k, kKeys, kv_head, row, k_full() + 8 * s);
                 }
-                if (j >= kStages && !wait(v_empty + 8 * s, j / kStages - 1)) break;
+                if (j >= kStages && !wait(v_empty() + 8 * s, j / kStages - 1)) break;
                 const bool look = careful || there < kKeys;  // what follows the prompt may not be finite: zeros
-                const uint32_t bar = look ? tail : v_full + 8 * s;
+                const uint32_t bar = look ? tail() : v_full() + 8 * s;
                 if (lane == 0) {
                     mbar_expect_tx(bar, kTile);
                     load(s_v + s * kTile, &tm_v, kKeys, kv_head, row, bar);
                 }
                 if (!look) continue;
                 if (lane < kKeys / 32) s_bad[s][lane] = 0;
-                if (!wait(tail, looks++)) break;
+                if (!wait(tail(), looks++)) break;
                 for (int x = lane; x < kKeys * kBoxes; x += 32) {  // a key's box each
                     const int key = x % kKeys;
                     const uint32_t at = s_v + s * kTile + x * kBytes;
@@ -371,12 +376,12 @@ __global__ void __launch_bounds__(kPromptThreads, PromptShape<D>::kCtas)
                 }
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
-                if (lane == 0) mbar_arrive(v_full + 8 * s);
+                if (lane == 0) mbar_arrive(v_full() + 8 * s);
             }
             if (j < turns && lane == 0) {  // a wait ran out: no copy is on its way when the CTA gives its memory back
-                mbar_settle(q_full, 0);
-                for (int i = max(0, j - kStages); i <= j; ++i) mbar_settle(k_full + 8 * (i % kStages), (i / kStages) & 1);
-                for (int i = max(0, j - kStages); i <= j; ++i) mbar_settle(v_full + 8 * (i % kStages), (i / kStages) & 1);
+                mbar_settle(q_full(), 0);
+                mbar_settle_ring(k_full(), kStages, j + 1);
+                mbar_settle_ring(v_full(), kStages, j + 1);
             }
             __syncwarp();
         } while (again());
@@ -391,11 +396,11 @@ __global__ void __launch_bounds__(kPromptThreads, PromptShape<D>::kCtas)
             };
             const uint64_t q_desc = umma_desc_rows<kBytes>(s_q), k_desc = umma_desc_rows<kBytes>(s_k);
             const uint64_t v_desc = umma_desc_rows<kBytes>(s_v, kKeys * kBytes);
-            bool ok = wait(q_full, 0);
+            bool ok = wait(q_full(), 0);
             int keys = 0, values = 0;  // turns known to be there (a wait takes a hundred clocks even if it ends at once)
             const auto score = [&](int tile, int j, bool last) {
                 const int s = j % kStages;
-                if (!ok || (j >= keys && !(ok = wait(k_full + 8 * s, j / kStages)))) return;
+                if (!ok || (j >= keys && !(ok = wait(k_full() + 8 * s, j / kStages)))) return;
                 keys = j + 1;
                 const PromptTurns in = tile ? turns1 : turns0;
                 if (j >= in.begin && j < in.end) {
@@ -405,31 +410,31 @@ __global__ void __launch_bounds__(kPromptThreads, PromptShape<D>::kCtas)
                     for (int k = 0; k < D / 16; ++k)
                         umma_half<false>(leader, tmem + tile * kKeys, q + (k / kSteps * 128 * kBytes + k % kSteps * 32) / 16,
                                          kk + (k / kSteps * kKeys * kBytes + k % kSteps * 32) / 16, idesc_s, k != 0);
-                    commit(s_full + 8 * tile);
+                    commit(s_full() + 8 * tile);
                 }
-                if (last) commit(k_empty + 8 * s);
+                if (last) commit(k_empty() + 8 * s);
             };
             const auto sum = [&](int tile, int j, bool last) {
                 const int s = j % kStages;
-                if (!ok || (j >= values && !(ok = wait(v_full + 8 * s, j / kStages)))) return;
+                if (!ok || (j >= values && !(ok = wait(v_full() + 8 * s, j / kStages)))) return;
                 values = j + 1;
                 // (and the keys that come next)
-                if (j + 1 < turns && j + 1 >= keys && !(ok = wait(k_full + 8 * ((j + 1) % kStages), (j + 1) / kStages))) return;
+                if (j + 1 < turns && j + 1 >= keys && !(ok = wait(k_full() + 8 * ((j + 1) % kStages), (j + 1) / kStages))) return;
                 if (j + 1 < turns) keys = j + 2;
                 const PromptTurns in = tile ? turns1 : turns0;
                 if (j >= in.begin && j < in.end) {
                     const uint64_t v = v_desc + s * (kTile / 16);
 #pragma unroll
                     for (int h = 0; h < kParts; ++h) {
-                        if (!(ok = wait(p_full + 8 * (tile * kParts + h), j - in.begin))) return;
+                        if (!(ok = wait(p_full() + 8 * (tile * kParts + h), j - in.begin))) return;
                         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll
                         for (int k = 4 * h; k < 4 * h + 4; ++k)
                             umma_half<true>(leader, tmem + kTmemO + tile * D, tmem + tile * kKeys + k * 8, v + k * kBytes, idesc_o, j != in.begin || k != 0);
                     }
-                    if (j + 1 == in.end) commit(o_full + 8 * tile);
+                    if (j + 1 == in.end) commit(o_full() + 8 * tile);
                 }
-                if (last) commit(v_empty + 8 * s);
+                if (last) commit(v_empty() + 8 * s);
             };
             if constexpr (kIssuers == 2) {
                 score(own, 0, true);
@@ -448,8 +453,12 @@ __global__ void __launch_bounds__(kPromptThreads, PromptShape<D>::kCtas)
                     if (more) score(1, j + 1, true);
                 }
             }
-            commit(idle);  // no product is on its way when the CTA gives its memory back
-            mbar_settle(idle, 0);
+            commit(idle());  // no product is on its way when the CTA gives its memory back
+            mbar_settle(idle(), 0);
+            if (ok) {
+                mbar_settle_ring(k_empty(), kStages, turns);
+                mbar_settle_ring(v_empty(), kStages, turns);
+            }
             __syncwarp();
         } while (again());
         else do {
@@ -468,7 +477,7 @@ __global__ void __launch_bounds__(kPromptThreads, PromptShape<D>::kCtas)
         do {
             float m = -INFINITY, l = 0.0f;
             for (int j = in.begin; j < in.end; ++j) {
-                wait(s_full + 8 * tile, j - in.begin);
+                wait(s_full() + 8 * tile, j - in.begin);
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 float s[kKeys / 32][32];
 #pragma unroll
@@ -533,19 +542,19 @@ __global__ void __launch_bounds__(kPromptThreads, PromptShape<D>::kCtas)
                         tmem_store16(at_s + 32 * h + 16 * c, x);
                     }
                     if (careful && h + 1 == kParts) {
-                        wait(v_full + 8 * (j % kStages), j / kStages);
+                        wait(v_full() + 8 * (j % kStages), j / kStages);
                         for (int c = 0; c < kKeys / 32; ++c)
                             if (s_bad[j % kStages][c] & prompt_seen(position, p.window, key + 32 * c)) l = __int_as_float(0x7fc00000);
                     }
                     asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
                     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
                     __syncwarp();
-                    if (lane == 0) mbar_arrive(p_full + 8 * (tile * kParts + h));
+                    if (lane == 0) mbar_arrive(p_full() + 8 * (tile * kParts + h));
                 }
                 const float2 both = add2(sum[0], sum[1]);
                 l += both.x + both.y;
             }
-            if (in.end > in.begin) wait(o_full + 8 * tile, 0);
+            if (in.end > in.begin) wait(o_full() + 8 * tile, 0);
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             const float inverse = *static_cast<volatile int*>(&s_failed) ? __int_as_float(0x7fc00000) : __fdiv_rn(1.0f, l);
             const __nv_bfloat162 zero = __floats2bfloat162_rn(0.0f, 0.0f);
@@ -638,35 +647,43 @@ __global__ void __launch_bounds__(kPromptF32Threads, 1) prompt_f32_kernel(Prompt
     constexpr uint32_t kTmemS = 3 * D / 2, kSCols = 96, kTmemO = kTmemS + kBuffers * kSCols;  // q's slices, S with the weights' slices over it, O
     static_assert(kTmemO + D <= 512, "TMEM");
     extern __shared__ uint8_t smem_raw[];
-    __shared__ __align__(8) uint64_t s_bars[4 * kStages + kBuffers + 7];
+    constexpr uint32_t kBars = 4 * kStages + kBuffers + 7;
+    __shared__ __align__(8) uint64_t s_bars[2 * kBars];
     __shared__ uint32_t s_tmem;
     __shared__ PromptTile s_tile;
     __shared__ int s_failed, s_dirty;
     __shared__ unsigned long long s_bad[2][kStages];  // careful: which of a turn's keys, values are not finite
     const uint32_t s_k = (smem_addr(smem_raw) + 1023) & ~1023u, s_v = s_k + kStages * 3 * kPlane;
-    const uint32_t k_full = smem_addr(s_bars), k_empty = k_full + 8 * kStages, v_full = k_empty + 8 * kStages, v_empty = v_full + 8 * kStages;
-    const uint32_t s_full = v_empty + 8 * kStages, p_full = s_full + 8 * kBuffers, o_full = p_full + 8, q_full = o_full + 32, idle = q_full + 8;  // P v of a turn: by turn % 4
+    uint32_t bars = smem_addr(s_bars);  // of this pass
+    const auto k_full = [&] { return bars; };
+    const auto k_empty = [&] { return bars + 8 * kStages; };
+    const auto v_full = [&] { return bars + 16 * kStages; };
+    const auto v_empty = [&] { return bars + 24 * kStages; };
+    const auto s_full = [&] { return bars + 32 * kStages; };  // by buffer
+    const auto p_full = [&] { return s_full() + 8 * kBuffers; };
+    const auto o_full = [&] { return p_full() + 8; };  // P v of a turn: by turn % 4
+    const auto q_full = [&] { return p_full() + 40; };
+    const auto idle = [&] { return p_full() + 48; };
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const auto init = [&](bool again) {  // one thread
-        const auto set = [&](uint32_t bar, uint32_t count) {
-            if (again) asm volatile("mbarrier.inval.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
-            mbar_init(bar, count);
-        };
-        for (int s = 0; s < kStages; ++s) {
-            set(k_full + 8 * s, 8);
-            set(v_full + 8 * s, 8);
-            set(k_empty + 8 * s, 1);
-            set(v_empty + 8 * s, 1);
+    // Two sets: one for each of the CTA's passes.
+    if (threadIdx.x == 32) {
+        for (uint32_t set = 0; set < 2; ++set) {
+            const auto init = [&](uint32_t bar, int n, uint32_t count) {
+                for (int x = 0; x < n; ++x) mbar_init(bar + 8 * (set * kBars + x), count);
+            };
+            init(k_full(), kStages, 8);
+            init(k_empty(), kStages, 1);
+            init(v_full(), kStages, 8);
+            init(v_empty(), kStages, 1);
+            init(s_full(), kBuffers, 1);
+            init(p_full(), 1, 4);
+            init(o_full(), 4, 1);
+            init(q_full(), 1, 4);
+            init(idle(), 1, 2);
         }
-        for (int s = 0; s < kBuffers; ++s) set(s_full + 8 * s, 1);
-        set(p_full, 4);
-        for (int s = 0; s < 4; ++s) set(o_full + 8 * s, 1);
-        set(q_full, 4);
-        set(idle, 2);
         s_failed = s_dirty = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    };
-    if (threadIdx.x == 0) init(false);
+    }
     pdl_wait();
     pdl_trigger();
     const int slot = static_cast<int>(kv8_div(blockIdx.x, p.by_heads)), part = static_cast<int>(blockIdx.x - slot * p.by_heads.d);
@@ -696,17 +713,17 @@ __global__ void __launch_bounds__(kPromptF32Threads, 1) prompt_f32_kernel(Prompt
         return __all_sync(kFull, ok);
     };
     bool careful = false;
-    const auto sync = [] { asm volatile("bar.sync 1, %0;" ::"n"(kPromptF32Threads) : "memory"); };
+    const auto sync = [] {
+        __syncwarp();
+        asm volatile("bar.sync 1, %0;" ::"n"(kPromptF32Threads) : "memory");
+    };
     // Every warp, at its end: whether the CTA starts over.
     const auto again = [&] {
         asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
         sync();
-        const bool redo = !careful && s_dirty && !s_failed;
-        if (!redo) return false;
-        sync();
-        if (threadIdx.x == 0) init(true);
-        sync();
+        if (careful || !s_dirty || s_failed) return false;
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        bars += 8 * kBars;
         return careful = true;
     };
     if (warp >= 4) {
@@ -735,10 +752,11 @@ __global__ void __launch_bounds__(kPromptF32Threads, 1) prompt_f32_kernel(Prompt
                 const int which = n / kParts & 1, j = n / (2 * kParts), s = j % kStages;
                 if (n >= batches) return;
                 if (n % kParts == 0) {
-                    if (j >= kStages) ok &= wait((which ? v_empty : k_empty) + 8 * s, j / kStages - 1);
+                    if (j >= kStages) ok &= wait((which ? v_empty() : k_empty()) + 8 * s, j / kStages - 1);
                     if (careful) {  // (P v of the stage's last turn is behind what its rows read of s_bad)
-                        if (j >= kStages) ok &= wait(v_empty + 8 * s, j / kStages - 1);
+                        if (j >= kStages) ok &= wait(v_empty() + 8 * s, j / kStages - 1);
                         if (u0 == 0) s_bad[which][s] = 0;
+                        __syncwarp();
                         asm volatile("bar.sync 2, 256;" ::: "memory");
                     }
                 }
@@ -779,7 +797,7 @@ __global__ void __launch_bounds__(kPromptF32Threads, 1) prompt_f32_kernel(Prompt
                 if (n % kParts + 1 < kParts) return;
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
-                if (lane == 0) mbar_arrive((which ? v_full : k_full) + 8 * s);
+                if (lane == 0) mbar_arrive((which ? v_full() : k_full()) + 8 * s);
             };
             float4 a[kBatch][2], b[kBatch][2], c[kBatch][2];
             load(a, 0);
@@ -803,14 +821,14 @@ __global__ void __launch_bounds__(kPromptF32Threads, 1) prompt_f32_kernel(Prompt
             };
             const uint64_t k_desc = umma_desc_rows<kBytes>(s_k), v_desc = umma_desc_rows<kBytes>(s_v, kKeys * kBytes);
             constexpr int kSteps = kBytes / 32;  // of 16 dims in a row of a box
-            bool ok = warp == 5 || wait(q_full, 0);
+            bool ok = warp == 5 || wait(q_full(), 0);
             for (int j = 0; ok && j < turns; ++j) {
                 const int s = j % kStages, before = j - kBuffers;
                 const uint32_t at_s = tmem + kTmemS + j % kBuffers * kSCols;
                 if (warp == 4) {
                     // (P v of that turn has read the weights that S goes over)
-                    if (before >= 0) ok = wait(o_full + 8 * (before & 3), before >> 2);
-                    if (!ok || !(ok = wait(k_full + 8 * s, j / kStages))) break;
+                    if (before >= 0) ok = wait(o_full() + 8 * (before & 3), before >> 2);
+                    if (!ok || !(ok = wait(k_full() + 8 * s, j / kStages))) break;
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll
                     for (int i = 0; i < 6; ++i)
@@ -818,10 +836,10 @@ __global__ void __launch_bounds__(kPromptF32Threads, 1) prompt_f32_kernel(Prompt
                         for (int k = 0; k < D / 16; ++k)
                             umma_half<true>(leader, at_s, tmem + prompt_slice_a(i) * (D / 2) + k * 8,
                                             k_desc + ((s * 3 + prompt_slice_b(i)) * kPlane + k / kSteps * kKeys * kBytes + k % kSteps * 32) / 16, idesc_s, (i | k) != 0);
-                    commit(s_full + 8 * (j % kBuffers));
-                    commit(k_empty + 8 * s);
+                    commit(s_full() + 8 * (j % kBuffers));
+                    commit(k_empty() + 8 * s);
                 } else {
-                    if (!(ok = wait(v_full + 8 * s, j / kStages) && wait(p_full, j))) break;
+                    if (!(ok = wait(v_full() + 8 * s, j / kStages) && wait(p_full(), j))) break;
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll
                     for (int i = 0; i < 6; ++i)
@@ -829,12 +847,13 @@ __global__ void __launch_bounds__(kPromptF32Threads, 1) prompt_f32_kernel(Prompt
                         for (int k = 0; k < kKeys / 16; ++k)
                             umma_half<true>(leader, tmem + kTmemO, at_s + prompt_slice_a(i) * (kKeys / 2) + k * 8,
                                             v_desc + ((s * 3 + prompt_slice_b(i)) * kPlane + k * 16 * kBytes) / 16, idesc_o, (i | k) != 0);
-                    commit(o_full + 8 * (j & 3));
-                    commit(v_empty + 8 * s);
+                    commit(o_full() + 8 * (j & 3));
+                    commit(v_empty() + 8 * s);
                 }
             }
-            commit(idle);  // no product is on its way when the CTA gives its memory back
-            mbar_settle(idle, 0);
+            commit(idle());  // no product is on its way when the CTA gives its memory back
+            mbar_settle(idle(), 0);
+            if (ok) mbar_settle_ring(warp == 4 ? k_empty() : v_empty(), kStages, turns);
             __syncwarp();
         } while (again());
         else do {
@@ -852,47 +871,44 @@ __global__ void __launch_bounds__(kPromptF32Threads, 1) prompt_f32_kernel(Prompt
         float o[D];
         bool good = true;
         do {
-#pragma unroll
-            for (int c = 0; c < D; c += kChunk) {  // q, to where O will be: whole sectors, then by rows
-                float4 x[32 / kEach];
-#pragma unroll
-                for (int i = 0; i < 32 / kEach; ++i) {
-                    const uint8_t* from = rows.at(p, p.q, p.q_stride, D, 4, warp * 32 + i * kEach + lane / kPieces);
-                    x[i] = from ? *reinterpret_cast<const float4*>(from + c * 4 + lane % kPieces * 16) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            // q by whole sectors into shared memory, then its slices by rows. (Loops that are not unrolled here and
+            // below: code that runs once a CTA is bound by its own instructions' way from memory.)
+#pragma unroll 1
+            for (int c = 0; c < D; c += kChunk) {
+#pragma unroll 2
+                for (int i = 0; i < 32; i += kEach) {
+                    const uint8_t* from = rows.at(p, p.q, p.q_stride, D, 4, warp * 32 + i + lane / kPieces);
+                    copy16(prompt_staged<kRow>(staging, i + lane / kPieces, lane % kPieces),
+                           from ? from + c * 4 + lane % kPieces * 16 : static_cast<const uint8_t*>(p.q), from ? 16 : 0);
                 }
-#pragma unroll
-                for (int i = 0; i < 32 / kEach; ++i)
-                    kv8_put16(prompt_staged<kRow>(staging, i * kEach + lane / kPieces, lane % kPieces), __float_as_uint(x[i].x), __float_as_uint(x[i].y),
-                              __float_as_uint(x[i].z), __float_as_uint(x[i].w));
+                asm volatile("cp.async.wait_all;" ::: "memory");
                 __syncwarp();
+#pragma unroll 1
+                for (int k = 0; k < kPieces; k += 4) {
+                    uint32_t w[3][8];
 #pragma unroll
-                for (int k = 0; k < kPieces; ++k) {
-                    const float4 y = prompt_get16(prompt_staged<kRow>(staging, lane, k));
-                    o[c + 4 * k] = y.x, o[c + 4 * k + 1] = y.y, o[c + 4 * k + 2] = y.z, o[c + 4 * k + 3] = y.w;
+                    for (int i = 0; i < 8; i += 2) {
+                        const float4 y = prompt_get16(prompt_staged<kRow>(staging, lane, k + i / 2));
+                        uint32_t three[3];
+                        bf16x2_slices(make_float2(y.x * p.scale, y.y * p.scale), three);
+                        w[0][i] = three[0], w[1][i] = three[1], w[2][i] = three[2];
+                        bf16x2_slices(make_float2(y.z * p.scale, y.w * p.scale), three);
+                        w[0][i + 1] = three[0], w[1][i + 1] = three[1], w[2][i + 1] = three[2];
+                    }
+#pragma unroll
+                    for (int i = 0; i < 3; ++i) tmem_store8(lanes + i * (D / 2) + c / 2 + 2 * k, w[i]);
                 }
                 __syncwarp();
-            }
-#pragma unroll
-            for (int c = 0; c < D; c += 16) {
-                uint32_t w[3][8];
-#pragma unroll
-                for (int k = 0; k < 8; ++k) {
-                    uint32_t three[3];
-                    bf16x2_slices(make_float2(o[c + 2 * k] * p.scale, o[c + 2 * k + 1] * p.scale), three);
-                    w[0][k] = three[0], w[1][k] = three[1], w[2][k] = three[2];
-                }
-#pragma unroll
-                for (int i = 0; i < 3; ++i) tmem_store8(lanes + i * (D / 2) + c / 2, w[i]);
             }
             asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
             __syncwarp();
-            if (lane == 0) mbar_arrive(q_full);
+            if (lane == 0) mbar_arrive(q_full());
 #pragma unroll
             for (int k = 0; k < D; ++k) o[k] = 0.0f;
             float m = -INFINITY, l = 0.0f, shrink = 1.0f;
             const auto add_output = [&](int j) {
-                wait(o_full + 8 * (j & 3), j >> 2);
+                wait(o_full() + 8 * (j & 3), j >> 2);
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 const float2 by = make_float2(shrink, shrink);
 #pragma unroll
@@ -910,7 +926,7 @@ __global__ void __launch_bounds__(kPromptF32Threads, 1) prompt_f32_kernel(Prompt
             };
             for (int j = 0; j < turns; ++j) {
                 const uint32_t at_s = lanes + kTmemS + j % kBuffers * kSCols;
-                wait(s_full + 8 * (j % kBuffers), j / kBuffers);
+                wait(s_full() + 8 * (j % kBuffers), j / kBuffers);
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 float s[2][32];
                 tmem_start(at_s, s[0]);
@@ -919,8 +935,8 @@ __global__ void __launch_bounds__(kPromptF32Threads, 1) prompt_f32_kernel(Prompt
                 tmem_arrived(s[1]);
                 const int key = key0 + j * kKeys;
                 if (careful) {
-                    wait(k_full + 8 * (j % kStages), j / kStages);
-                    wait(v_full + 8 * (j % kStages), j / kStages);
+                    wait(k_full() + 8 * (j % kStages), j / kStages);
+                    wait(v_full() + 8 * (j % kStages), j / kStages);
                     const unsigned long long seen = prompt_seen(position, p.window, key) |
                                                     static_cast<unsigned long long>(prompt_seen(position, p.window, key + 32)) << 32;
                     if (mine && s_bad[1][j % kStages] & seen) l = __int_as_float(0x7fc00000);
@@ -976,7 +992,7 @@ __global__ void __launch_bounds__(kPromptF32Threads, 1) prompt_f32_kernel(Prompt
                 asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
                 asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
                 __syncwarp();
-                if (lane == 0) mbar_arrive(p_full);
+                if (lane == 0) mbar_arrive(p_full());
             }
             add_output(turns - 1);
             const float inverse = *static_cast<volatile int*>(&s_failed) ? __int_as_float(0x7fc00000) : __fdiv_rn(1.0f, l);
