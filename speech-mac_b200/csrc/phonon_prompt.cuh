@@ -110,30 +110,19 @@ __device__ __forceinline__ float4 prompt_get16(uint32_t at) {
     return v;
 }
 
-// Where a row tile's rows lie in the call's: row r is head r % pack of the
-// `part`-th group of `pack` at position first + r / pack, while that is before
-// `end` and r / pack below `half`. A pointer to it, or null.
-struct PromptRows {
-    int row0, first, half, end, head0;
-    __device__ __forceinline__ const uint8_t* at(const PromptParams& p, const void* base, long long stride, int dim, int size, int r) const {
-        const int token = static_cast<int>(kv8_div(r, p.pack)), position = first + token, head = head0 + r - token * static_cast<int>(p.pack.d);
-        if (token >= half || position >= end) return nullptr;
-        return static_cast<const uint8_t*>(base) + (static_cast<size_t>(row0 + position) * stride + static_cast<size_t>(head) * dim) * size;
-    }
-};
-
-// A warp's 32 staged rows (of kRow bytes, the part of a row at byte `from`) to
-// the output, whole sectors at a time.
+// A warp's 32 staged rows (of kRow bytes) to the output, whole sectors at a
+// time. own: the byte of the output that the lane's row goes to, or -1.
 template <int kRow>
-__device__ __forceinline__ void prompt_put_rows(const PromptParams& p, const PromptRows& rows, uint32_t staging, int r0, int dim, int size, int from) {
+__device__ __forceinline__ void prompt_put_rows(void* out, long long own, uint32_t staging) {
     constexpr int kPieces = kRow / 16, kEach = 32 / kPieces;
     const int lane = threadIdx.x & 31;
     __syncwarp();
-#pragma unroll 2
+#pragma unroll 4
     for (int i = 0; i < 32; i += kEach) {
         const int r = i + lane / kPieces;
-        uint8_t* to = const_cast<uint8_t*>(rows.at(p, p.out, p.out_stride, dim, size, r0 + r));
-        if (to) *reinterpret_cast<float4*>(to + from + lane % kPieces * 16) = prompt_get16(prompt_staged<kRow>(staging, r, lane % kPieces));
+        const long long at = __shfl_sync(kFull, own, r);
+        const float4 x = prompt_get16(prompt_staged<kRow>(staging, r, lane % kPieces));
+        if (at >= 0) *reinterpret_cast<float4*>(static_cast<uint8_t*>(out) + at + lane % kPieces * 16) = x;
     }
     __syncwarp();
 }
@@ -578,7 +567,7 @@ __global__ void __launch_bounds__(kPromptThreads, PromptShape<D>::kCtas)
         const uint32_t staging = s_q + tile * kQTile + quarter * (32 * 2 * D);
 #pragma unroll
         for (int k = 0; k < D / 8; ++k) kv8_put16(prompt_staged<2 * D>(staging, lane, k), w[4 * k], w[4 * k + 1], w[4 * k + 2], w[4 * k + 3]);
-        prompt_put_rows<2 * D>(p, PromptRows{t.row0, first, half, end, head0}, staging, quarter * 32, D, 2, 0);
+        prompt_put_rows<2 * D>(p.out, mine ? 2 * ((t.row0 + position) * p.out_stride + (head0 + r - at * pack) * D) : -1, staging);
         if (!good) prompt_flag(p, t.index, s_failed ? kStatusDevice : kStatusNonFinite);
     }
     __syncwarp();
@@ -865,7 +854,8 @@ __global__ void __launch_bounds__(kPromptF32Threads, 1) prompt_f32_kernel(Prompt
         const int head = head0 + r - at * pack;
         const uint32_t lanes = tmem + (static_cast<uint32_t>(warp * 32) << 16);
         const float* q = static_cast<const float*>(p.q) + static_cast<size_t>(t.row0 + position) * p.q_stride + static_cast<size_t>(head) * D;
-        const PromptRows rows{t.row0, t.first, p.tokens, end, head0};
+        const long long from_q = mine ? 4 * ((t.row0 + position) * p.q_stride + head * D) : -1;  // bytes
+        const long long to_out = mine ? 4 * ((t.row0 + position) * p.out_stride + head * D) : -1;
         constexpr int kChunk = Shape::kChunk, kRow = 4 * kChunk, kPieces = kChunk / 4, kEach = 32 / kPieces;
         const uint32_t staging = s_v + kStages * 3 * kPlane + warp * (32 * kRow);
         float o[D];
@@ -875,11 +865,12 @@ __global__ void __launch_bounds__(kPromptF32Threads, 1) prompt_f32_kernel(Prompt
             // below: code that runs once a CTA is bound by its own instructions' way from memory.)
 #pragma unroll 1
             for (int c = 0; c < D; c += kChunk) {
-#pragma unroll 2
+#pragma unroll 4
                 for (int i = 0; i < 32; i += kEach) {
-                    const uint8_t* from = rows.at(p, p.q, p.q_stride, D, 4, warp * 32 + i + lane / kPieces);
-                    copy16(prompt_staged<kRow>(staging, i + lane / kPieces, lane % kPieces),
-                           from ? from + c * 4 + lane % kPieces * 16 : static_cast<const uint8_t*>(p.q), from ? 16 : 0);
+                    const int row = i + lane / kPieces;
+                    const long long from = __shfl_sync(kFull, from_q, row);
+                    copy16(prompt_staged<kRow>(staging, row, lane % kPieces),
+                           static_cast<const uint8_t*>(p.q) + (from < 0 ? 0 : from + c * 4 + lane % kPieces * 16), from < 0 ? 0 : 16);
                 }
                 asm volatile("cp.async.wait_all;" ::: "memory");
                 __syncwarp();
@@ -1012,7 +1003,7 @@ __global__ void __launch_bounds__(kPromptF32Threads, 1) prompt_f32_kernel(Prompt
             for (int k = 0; k < kPieces; ++k)
                 kv8_put16(prompt_staged<kRow>(staging, lane, k), __float_as_uint(o[c + 4 * k]), __float_as_uint(o[c + 4 * k + 1]),
                           __float_as_uint(o[c + 4 * k + 2]), __float_as_uint(o[c + 4 * k + 3]));
-            prompt_put_rows<kRow>(p, rows, staging, warp * 32, D, 4, c * 4);
+            prompt_put_rows<kRow>(p.out, to_out < 0 ? -1 : to_out + c * 4, staging);
         }
         if (!good) prompt_flag(p, t.index, s_failed ? kStatusDevice : kStatusNonFinite);
     }
