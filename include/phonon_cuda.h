@@ -582,7 +582,8 @@ int phonon_cuda_qk_norm_rope_device(int device, const PhononCudaQkNormRope *args
  * [rows][cols] bytes; cols a multiple of 16. A row with a non-finite element
  * gets the scale NaN and integers 0, and status_dev (device, [rows],
  * optional, zeroed by the caller) is raised to PHONON_CUDA_NON_FINITE for it.
- * Enqueued on `cuda_stream` of `device`, like the cache's calls above. */
+ * q must not overlap x. Enqueued on `cuda_stream` of `device`, like the
+ * cache's calls above. */
 typedef struct {
     uint32_t type; /* PhononCudaRowType of x */
     uint32_t rows, cols;
@@ -598,7 +599,9 @@ int phonon_cuda_quantize_rows_device(int device, const PhononCudaQuantizeRows *a
  * the sum is exact, then rounded to fp32, as are its products with x_scales
  * and then (with the bias in one) with w_scales; bf16 rounds once more. x is
  * [rows][depth], weights [channels][depth], any 8-bit integers, depth a
- * multiple of 16 below 2^17; y is [rows][channels], any number of them.
+ * multiple of 16 below 2^17; y is [rows][channels], any number of them (rows
+ * that are not a multiple of 16 bytes apart take longer), and overlaps nothing
+ * that the call reads.
  * status_dev (device, [rows], optional, zeroed by the caller) is raised to
  * NON_FINITE for a row with a non-finite result, and to DEVICE_ERROR where
  * the kernel gave up a bounded wait (about two seconds): the row is NaN. */
@@ -625,14 +628,16 @@ int phonon_cuda_i8_product_device(int device, const PhononCudaI8Product *args, i
  * (device, [prompts], optional, zeroed by the caller) is raised for a prompt
  *   - whose rows lie outside [0, rows), are more than max_rows or begin before
  *     an earlier entry of row_begin (INVALID_ARGUMENT): its rows of out stay;
- *   - with a non-finite output (NON_FINITE): a row that sees a non-finite
- *     value, or whose scores leave fp32's range, is not finite; others are
- *     what they are without it;
+ *   - with a non-finite output (NON_FINITE): a row that sees a value which is
+ *     not finite, whatever its weight, or whose own query (fp32: times the
+ *     scale, beyond 2.3e38) or a score is not, but for scores of -infinity
+ *     beside others, which are weights of 0. Other rows are what they are
+ *     without it;
  *   - where the kernel gave up a bounded wait (DEVICE_ERROR, about two
  *     seconds): rows of it are NaN.
  * The largest code stays. out may be q with q's stride, or lie apart from q, k
- * and v. The call returns CAPACITY where rows, prompts and heads make more
- * than 2^31 blocks of work. */
+ * and v. The call returns CAPACITY for more than 2^18 prompts, and where rows,
+ * prompts and heads make more than 2^31 blocks of work. */
 typedef struct {
     uint32_t type; /* PhononCudaRowType of q, k, v and out */
     uint32_t prompts, rows, max_rows; /* prompts and max_rows at least 1 */

@@ -4537,6 +4537,7 @@ struct DeviceGuard {
 };
 
 bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+bool aligned4(const void* p) { return reinterpret_cast<uintptr_t>(p) % 4 == 0; }
 
 // Rows of `width` elements, `stride` apart (0: packed), that are read and
 // written four elements (16 or 8 bytes) at a time.
@@ -4895,7 +4896,7 @@ int phonon_cuda_quantize_rows_device(int device, const PhononCudaQuantizeRows* a
     I8QuantParams p{};
     if (!a || a->type > PHONON_CUDA_ROWS_BF16 || a->rows > (1u << 30) || a->cols == 0 || a->cols % 16 ||
         a->cols > (1u << 24) || !a->x || !a->q || !a->scales || !aligned16(a->x) || !aligned16(a->q) ||
-        !kv8_stride(a->x_stride, a->cols, &p.x_stride) || !kv8_stride(a->q_stride, a->cols, &p.q_stride) || p.q_stride % 16)
+        !aligned4(a->scales) || !aligned4(status_dev) || a->x == a->q || !kv8_stride(a->x_stride, a->cols, &p.x_stride) || !kv8_stride(a->q_stride, a->cols, &p.q_stride) || p.q_stride % 16)
         return PHONON_CUDA_INVALID_ARGUMENT;
     if (a->rows == 0) return PHONON_CUDA_OK;
     p.x = a->x;
@@ -4915,7 +4916,8 @@ int phonon_cuda_i8_product_device(int device, const PhononCudaI8Product* a, int3
     I8Params p{};
     if (!a || a->type > PHONON_CUDA_ROWS_BF16 || a->rows > (1u << 30) || a->channels == 0 || a->channels > (1u << 30) ||
         a->depth == 0 || a->depth % 16 || a->depth >= (1u << 17) || !a->x || !a->weights || !a->x_scales || !a->w_scales ||
-        !a->y || !aligned16(a->x) || !aligned16(a->weights) || !aligned16(a->y) ||
+        !a->y || !aligned16(a->x) || !aligned16(a->weights) || !aligned16(a->y) || !aligned4(a->x_scales) ||
+        !aligned4(a->w_scales) || !aligned4(a->bias) || !aligned4(status_dev) || a->y == a->x || a->y == a->weights ||
         !kv8_stride(a->x_stride, a->depth, &p.x_stride) || !kv8_stride(a->w_stride, a->depth, &p.w_stride) ||
         p.x_stride % 16 || p.w_stride % 16 || (a->y_stride && a->y_stride < a->channels) || a->y_stride > (1ull << 40))
         return PHONON_CUDA_INVALID_ARGUMENT;
@@ -5022,7 +5024,8 @@ int phonon_cuda_prompt_attention_device(int device, const PhononCudaPromptAttent
         a->max_rows == 0 || a->max_rows > (1u << 30) || a->heads == 0 || a->kv_heads == 0 || a->heads > (1u << 16) ||
         a->heads % a->kv_heads || (a->head_dim != 32 && a->head_dim != 64 && a->head_dim != 128) ||
         a->window > (1u << 30) || !(a->scale >= 0.0f && a->scale <= 1e30f) || !a->row_begin || !a->q || !a->k || !a->v ||
-        !a->out || !aligned16(a->q) || !aligned16(a->k) || !aligned16(a->v) || !aligned16(a->out))
+        !a->out || !aligned16(a->q) || !aligned16(a->k) || !aligned16(a->v) || !aligned16(a->out) || !aligned4(a->row_begin) ||
+        !aligned4(status_dev))
         return PHONON_CUDA_INVALID_ARGUMENT;
     const uint64_t width = static_cast<uint64_t>(a->heads) * a->head_dim, kv_width = static_cast<uint64_t>(a->kv_heads) * a->head_dim;
     if (!kv8_stride(a->q_stride, width, &p.q_stride) || !kv8_stride(a->k_stride, kv_width, &p.k_stride) ||
@@ -5030,6 +5033,7 @@ int phonon_cuda_prompt_attention_device(int device, const PhononCudaPromptAttent
         rows_collide(a->q, p.q_stride, a->out, p.out_stride, a->rows) || a->out == a->k || a->out == a->v)
         return PHONON_CUDA_INVALID_ARGUMENT;
     if (a->rows == 0) return PHONON_CUDA_OK;
+    if (a->prompts > (1u << 18)) return PHONON_CUDA_CAPACITY;  // a CTA finds its own among all of them: the work grows with their square
     p.q = a->q;
     p.k = a->k;
     p.v = a->v;
