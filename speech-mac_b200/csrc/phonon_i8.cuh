@@ -294,90 +294,161 @@ __device__ __forceinline__ uint32_t i8_staged(uint32_t staging, int row, int pie
     return staging + row * 64 + ((piece ^ (row >> 1 & 3)) * 16);
 }
 
-// 32 staged rows to y where its rows have any alignment, two rows at a time: a
-// lane takes a word (two bf16) of what lies in a row between two word
-// boundaries, and single elements at its ends.
+// The last channels of 32 staged rows that are a multiple of 16 bytes apart.
 template <bool kBf16>
-__device__ __forceinline__ void i8_store_ragged(const I8Params& p, uint32_t staging, int row0, int n0) {
-    constexpr int kCols = kBf16 ? 32 : 16;
-    const int lane = threadIdx.x & 31, w = lane & 15, cols = min(kCols, p.channels - n0);
-#pragma unroll
+__device__ __forceinline__ void i8_store_last(const I8Params& p, uint32_t staging, int row0, int n0) {
+    const int lane = threadIdx.x & 31, w = lane & 15, cols = p.channels - n0;
+#pragma unroll 4
     for (int i = 0; i < 16; ++i) {
         const int r = 2 * i + (lane >> 4);
-        const bool in = row0 + r < p.rows;
         const size_t to = static_cast<size_t>(row0 + r) * p.y_stride + n0;
         uint32_t mine;
         asm volatile("ld.shared.b32 %0, [%1];" : "=r"(mine) : "r"(i8_staged(staging, r, w >> 2) + (w & 3) * 4));
+        if (row0 + r >= p.rows) continue;
         if constexpr (kBf16) {
-            uint16_t* y = static_cast<uint16_t*>(p.y) + to;
-            const bool odd = to & 1;  // y + 1 is a word's
-            const uint32_t next = __shfl_down_sync(kFull, mine, 1);
-            const int at = 2 * w + odd;
-            if (in && at + 1 < cols && !(odd && w == 15)) *reinterpret_cast<uint32_t*>(y + at) = odd ? __byte_perm(mine, next, 0x5432) : mine;
-            else if (in && at < cols) y[at] = static_cast<uint16_t>(odd ? mine >> 16 : mine);
-            if (in && odd && w == 0) y[0] = static_cast<uint16_t>(mine);
+            uint16_t* y = static_cast<uint16_t*>(p.y) + to + 2 * w;
+            if (2 * w + 1 < cols) *reinterpret_cast<uint32_t*>(y) = mine;
+            else if (2 * w < cols) *y = static_cast<uint16_t>(mine);
         } else {
-            if (in && w < cols) static_cast<uint32_t*>(p.y)[to + w] = mine;
+            if (w < cols) static_cast<uint32_t*>(p.y)[to + w] = mine;
         }
     }
 }
 
+// `cols` of the 64 bf16 or 32 fp32 columns from n0 on of 16 rows of any
+// alignment, staged in 128 bytes each: a lane stores the word of y that holds
+// what its word of the staged row does. bf16 rows that start between two of
+// y's words are staged one element on, their first word with the last element
+// of the columns before (of the first columns: not stored).
+template <bool kBf16>
+__device__ __forceinline__ void i8_store_words(const I8Params& p, uint32_t staging, int row0, int n0, int cols, bool first) {
+    const int lane = threadIdx.x & 31;
+    const bool even = lane < (kBf16 ? cols / 2 : cols), odd = lane < (cols + 1) / 2 && !(first && lane == 0);
+    const uint32_t from = staging + lane * 4;
+    uint8_t* to = static_cast<uint8_t*>(p.y) + (static_cast<size_t>(row0) * p.y_stride + n0) * (kBf16 ? 2 : 4);
+    const long long step = p.y_stride * (kBf16 ? 2 : 4);
+#pragma unroll
+    for (int r = 0; r < 16; ++r, to += step) {
+        uint32_t mine;
+        asm volatile("ld.shared.b32 %0, [%1];" : "=r"(mine) : "r"((from ^ ((r & 7) * 16)) + r * 128));
+        const uintptr_t at = reinterpret_cast<uintptr_t>(to);
+        if (row0 + r < p.rows && (kBf16 && at & 2 ? odd : even)) reinterpret_cast<uint32_t*>(at & ~static_cast<uintptr_t>(3))[lane] = mine;
+    }
+}
+
 // A tile's columns [c0, c1) of a warp's 32 rows (row0 + lane; channels from n0
-// on) to y, 64 bytes of every row at a time through `staging`, so that a store
-// has whole sectors whatever the row stride; `taken` is called once they have
-// left TMEM. scale, bias: the tile's channels'. failed: NaN.
+// on) to y through `staging`, so that a store has whole sectors whatever the
+// row stride; `taken` is called once they have left TMEM. scale, bias: the
+// tile's channels'. failed: NaN. Rows that are a multiple of 16 bytes apart go
+// 64 bytes at a time; others 128, a row a store, since what they cost is the
+// instructions of every store.
 template <bool kBf16, typename Taken>
 __device__ __forceinline__ void i8_take(const I8Params& p, uint32_t tmem, uint32_t staging, int row0, int n0, int c0, int c1,
                                         const float* scale, const float* bias, bool failed, const Taken& taken) {
     constexpr int kCols = kBf16 ? 32 : 16, kSize = kBf16 ? 2 : 4;  // 64 bytes
     const int lane = threadIdx.x & 31, row = row0 + lane;
-    const bool wide = p.y_stride * kSize % 16 == 0;
     const float xs = failed ? __int_as_float(0x7fc00000) : row < p.rows ? p.x_scales[row] : 0.0f;
     float finite = 0.0f;  // NaN once a value is not
+    // kCols sums, the tile's from column c on, as they lie in y
+    const auto values = [&](const uint32_t* r, int c, uint32_t* out) {
+#pragma unroll
+        for (int k = 0; k < kCols; k += 4) {
+            const float4 s4 = *reinterpret_cast<const float4*>(scale + c + k), b4 = *reinterpret_cast<const float4*>(bias + c + k);
+            const float v[4] = {i8_value(static_cast<int>(r[k]), xs, s4.x, b4.x), i8_value(static_cast<int>(r[k + 1]), xs, s4.y, b4.y),
+                                i8_value(static_cast<int>(r[k + 2]), xs, s4.z, b4.z), i8_value(static_cast<int>(r[k + 3]), xs, s4.w, b4.w)};
+#pragma unroll
+            for (int i = 0; i < 4; i += 2) {
+                if constexpr (kBf16) {
+                    const __nv_bfloat162 b = __floats2bfloat162_rn(v[i], v[i + 1]);
+                    const uint32_t w = *reinterpret_cast<const uint32_t*>(&b);
+                    out[(k + i) / 2] = w;
+                    finite = fmaf(__uint_as_float(w << 16), 0.0f, fmaf(__uint_as_float(w & 0xffff0000u), 0.0f, finite));
+                } else {
+                    out[k + i] = __float_as_uint(v[i]);
+                    out[k + i + 1] = __float_as_uint(v[i + 1]);
+                    finite = fmaf(v[i], 0.0f, fmaf(v[i + 1], 0.0f, finite));  // (channels behind the last: sums, scale and bias 0)
+                }
+            }
+        }
+    };
+    if (p.y_stride * kSize % 16 == 0) {
 #pragma unroll 1
-    for (int c = c0; c < c1; c += 32) {
-        uint32_t r[32];
-        tmem_load32(tmem + c, r);
-        if (c + 32 >= c1) taken();
+        for (int c = c0; c < c1; c += 32) {
+            uint32_t r[32];
+            tmem_load32(tmem + c, r);
+            if (c + 32 >= c1) taken();
 #pragma unroll
-        for (int h = 0; h < 32; h += kCols) {
-            uint32_t out[16];
+            for (int h = 0; h < 32; h += kCols) {
+                uint32_t out[16];
+                values(r + h, c + h, out);
 #pragma unroll
-            for (int k = 0; k < kCols; k += 4) {
-                const float4 s4 = *reinterpret_cast<const float4*>(scale + c + h + k), b4 = *reinterpret_cast<const float4*>(bias + c + h + k);
-                const float v[4] = {i8_value(static_cast<int>(r[h + k]), xs, s4.x, b4.x), i8_value(static_cast<int>(r[h + k + 1]), xs, s4.y, b4.y),
-                                    i8_value(static_cast<int>(r[h + k + 2]), xs, s4.z, b4.z), i8_value(static_cast<int>(r[h + k + 3]), xs, s4.w, b4.w)};
+                for (int k = 0; k < 4; ++k) kv8_put16(i8_staged(staging, lane, k), out[4 * k], out[4 * k + 1], out[4 * k + 2], out[4 * k + 3]);
+                __syncwarp();
+                const int cols = p.channels - (n0 + c + h);
+                if (cols >= kCols) {
 #pragma unroll
-                for (int i = 0; i < 4; i += 2) {
-                    if constexpr (kBf16) {
-                        const __nv_bfloat162 b = __floats2bfloat162_rn(v[i], v[i + 1]);
-                        const uint32_t w = *reinterpret_cast<const uint32_t*>(&b);
-                        out[(k + i) / 2] = w;
-                        finite = fmaf(__uint_as_float(w << 16), 0.0f, fmaf(__uint_as_float(w & 0xffff0000u), 0.0f, finite));
-                    } else {
-                        out[k + i] = __float_as_uint(v[i]);
-                        out[k + i + 1] = __float_as_uint(v[i + 1]);
-                        finite = fmaf(v[i], 0.0f, fmaf(v[i + 1], 0.0f, finite));  // (channels behind the last: sums, scale and bias 0)
+                    for (int i = 0; i < 4; ++i) {
+                        const int to = 8 * i + (lane >> 2);
+                        uint4 w;
+                        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w)
+                                     : "r"(i8_staged(staging, to, lane & 3)));
+                        if (row0 + to < p.rows)
+                            *reinterpret_cast<uint4*>(static_cast<uint8_t*>(p.y) + (static_cast<size_t>(row0 + to) * p.y_stride + n0 + c + h) * kSize + (lane & 3) * 16) = w;
                     }
+                } else if (cols > 0) {
+                    i8_store_last<kBf16>(p, staging, row0, n0 + c + h);
+                }
+                __syncwarp();
+            }
+        }
+    } else {
+        constexpr int kUnit = 2 * kCols;
+        uint16_t* y = static_cast<uint16_t*>(p.y) + static_cast<size_t>(row) * p.y_stride + n0;
+        const bool odd = kBf16 && (row * p.y_stride + n0) & 1;
+        uint32_t before = 0;  // the last two elements
+#pragma unroll 1
+        for (int c = c0; c < c1; c += kUnit) {
+            uint32_t out[32];
+#pragma unroll
+            for (int h = 0; h < kUnit; h += 32) {
+                if (c + h < c1) {
+                    uint32_t r[32];
+                    tmem_load32(tmem + c + h, r);
+#pragma unroll
+                    for (int k = 0; k < 32; k += kCols) values(r + k, c + h + k, out + (h + k) * kSize / 4);
+                } else {
+#pragma unroll
+                    for (int k = 0; k < 16; ++k) out[16 + k] = 0;
                 }
             }
+            if (c + kUnit >= c1) taken();
+            const int cols = min(min(kUnit, c1 - c), p.channels - (n0 + c));
+            if (cols <= 0) continue;
+            const bool ends = c + kUnit >= c1 || n0 + c + kUnit >= p.channels;
+            if constexpr (kBf16) {
+                if (odd && c == c0 && row < p.rows) y[c] = static_cast<uint16_t>(out[0]);
+                const uint32_t last = out[31], pick = odd ? 0x5432 : 0x7654;
 #pragma unroll
-            for (int k = 0; k < 4; ++k) kv8_put16(i8_staged(staging, lane, k), out[4 * k], out[4 * k + 1], out[4 * k + 2], out[4 * k + 3]);
-            __syncwarp();
-            if (wide && n0 + c + h + kCols <= p.channels) {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int to = 8 * i + (lane >> 2);
-                    uint4 w;
-                    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w)
-                                 : "r"(i8_staged(staging, to, lane & 3)));
-                    if (row0 + to < p.rows)
-                        *reinterpret_cast<uint4*>(static_cast<uint8_t*>(p.y) + (static_cast<size_t>(row0 + to) * p.y_stride + n0 + c + h) * kSize + (lane & 3) * 16) = w;
-                }
-            } else if (n0 + c + h < p.channels) {
-                i8_store_ragged<kBf16>(p, staging, row0, n0 + c + h);
+                for (int k = 31; k > 0; --k) out[k] = __byte_perm(out[k - 1], out[k], pick);
+                out[0] = __byte_perm(before, out[0], pick);
+                before = last;
             }
-            __syncwarp();
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                const uint32_t own = staging + (lane & 15) * 128;
+                if (lane >> 4 == half)
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) kv8_put16(own + ((k ^ (lane & 7)) * 16), out[4 * k], out[4 * k + 1], out[4 * k + 2], out[4 * k + 3]);
+                __syncwarp();
+                i8_store_words<kBf16>(p, staging, row0 + 16 * half, n0 + c, cols, c == c0);
+                if (kBf16 && ends && lane >> 4 == half && (cols + odd) % 2 && row < p.rows) {  // half a word is left
+                    const int w = (cols + odd) / 2;
+                    uint32_t left = before >> 16;
+                    if (w < 32) asm volatile("ld.shared.b32 %0, [%1];" : "=r"(left) : "r"(own + (((w >> 2) ^ (lane & 7)) * 16) + (w & 3) * 4));
+                    y[c + cols - 1] = static_cast<uint16_t>(left);
+                }
+                __syncwarp();
+            }
         }
     }
     if (row < p.rows && finite != 0.0f) {

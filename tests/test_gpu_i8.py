@@ -221,3 +221,23 @@ def test_refusals(cuda_ok):
                dict(x_stride=16), dict(x_stride=40), dict(w_stride=24), dict(y_stride=15), dict(rows=(1 << 30) + 1)):
         assert product(**kw) == rt.INVALID, kw
     torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("bf16", [True, False])
+@pytest.mark.parametrize("rows,depth,channels", [(33, 80, (1, 2, 3, 31, 33, 63, 64, 65, 95, 97, 127, 130, 257)),
+                                                 (270, 80, (32, 96, 129, 159, 161, 193, 255, 385, 511, 513)),
+                                                 (1100, 528, (3001, 4099, 4351, 4353)), (1001, 2064, (4865, 5001, 5121))])
+def test_rows_of_every_alignment_and_width(cuda_ok, rows, depth, channels, bf16):
+    """Results whose rows start between two words or two sectors, and end in the middle of one, of a tile's half or behind it:
+    every element, and none beside them."""
+    for n in channels:
+        for pad in (0, 1, 2, 6):
+            rng = np.random.default_rng(n + pad)
+            x, w, xs, ws = product_case(rng, rows, n, depth)
+            bias = torch.tensor(rng.standard_normal(n), dtype=torch.float32, device="cuda")
+            y = torch.full((rows + 1, n + pad), 7.0, dtype=torch.bfloat16 if bf16 else torch.float32, device="cuda")
+            rt.I8Product(x.data_ptr(), xs.data_ptr(), w.data_ptr(), ws.data_ptr(), y.data_ptr(), rows, n, depth,
+                         rt.ROWS_BF16 if bf16 else rt.ROWS_F32, bias_ptr=bias.data_ptr(), y_stride=n + pad)()
+            torch.cuda.synchronize()
+            check_product(y[:rows, :n], *product_want(x, w, xs, ws, bias), bf16)
+            assert (y[rows:] == 7).all() and (y[:, n:] == 7).all()
