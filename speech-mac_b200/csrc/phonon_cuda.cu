@@ -4852,7 +4852,7 @@ int i8_split_launch(I8Params p, int splits, cudaStream_t s) {
 // Which kernel, by what each takes in us, as fitted to sweeps of 25 shapes: a
 // start, then for every wave of tiles 128 bytes of depth at a time (0.31 us for
 // 64 channels, 0.345 for 128, 0.43 for a pair's 256 x 256), or the taking out
-// of a tile where that is longer (1.4 times as long where y's rows are not
+// of a tile where that is longer (1.2 times as long where y's rows are not
 // 16-byte aligned); a split tile's sums take 3.3 and 4.5 us to meet. Up to
 // 16 rows always, and up to 32 where the weights are few, the rows' kernel.
 // us of the kernel chosen and of the next ones (rows x channels x depth):
@@ -4861,8 +4861,8 @@ int i8_split_launch(I8Params p, int splits, cudaStream_t s) {
 // 4096 split by 4 11.3, 64 channels 13.9; 512 x 512 x 2048 split by 4 6.9, 64
 // channels 8.1; 512 x 2048 x 512 64 channels 4.6, 128 5.4; 512 x 4096 x 4096
 // 128 channels 15.2, pairs 17.8, 64 channels 24.8; 1024 x 4096 x 4096 pairs
-// 18.5, 128 channels 26.3; 1001 x 5003 x 2064 pairs 25.2, 128 channels 26.8
-// (5008 channels: 20.6, 23.9); 700 x 9001 x 1040 128 channels 18.7, pairs 21.6.
+// 18.8, 128 channels 26.6; 1001 x 5003 x 2064 pairs 21.8, 128 channels 25.7
+// (5008 channels: 20.5, 24.2); 700 x 9001 x 1040 pairs 16.9, 128 channels 17.6.
 template <bool kBf16>
 int i8_product(const I8Params& p, int sms, cudaStream_t s) {
     if (p.rows <= 8) return i8_rows_launch<1, kBf16>(p, s);
@@ -4871,7 +4871,7 @@ int i8_product(const I8Params& p, int sms, cudaStream_t s) {
     const auto tiles = [&](int rows, int channels) {
         return static_cast<double>((p.rows + rows - 1) / rows) * ((p.channels + channels - 1) / channels);
     };
-    const double ragged = p.y_stride % (kBf16 ? 8 : 4) ? 1.4 : 1.0;
+    const double ragged = p.y_stride % (kBf16 ? 8 : 4) ? 1.2 : 1.0;
     const auto whole = [&](double n, double each, double out, int resident) {
         return std::ceil(n / resident) * std::max(depths * each, out * ragged) + 3.0;
     };

@@ -322,32 +322,42 @@ __device__ __forceinline__ void i8_store_last(const I8Params& p, uint32_t stagin
 // of the columns before (of the first columns: not stored).
 template <bool kBf16>
 __device__ __forceinline__ void i8_store_words(const I8Params& p, uint32_t staging, int row0, int n0, int cols, bool first) {
-    const int lane = threadIdx.x & 31;
-    const bool even = lane < (kBf16 ? cols / 2 : cols), odd = lane < (cols + 1) / 2 && !(first && lane == 0);
+    const int lane = threadIdx.x & 31, rows = p.rows - row0;
+    const bool whole = lane < (kBf16 ? cols / 2 : cols), shifted = lane < (cols + 1) / 2 && !(first && lane == 0);
     const uint32_t from = staging + lane * 4;
-    uint8_t* to = static_cast<uint8_t*>(p.y) + (static_cast<size_t>(row0) * p.y_stride + n0) * (kBf16 ? 2 : 4);
     const long long step = p.y_stride * (kBf16 ? 2 : 4);
+    const uintptr_t to = reinterpret_cast<uintptr_t>(p.y) + (static_cast<size_t>(row0) * p.y_stride + n0) * (kBf16 ? 2 : 4);
+    // every other row starts alike
+    uint32_t* at[2];
+    bool mine[2];
 #pragma unroll
-    for (int r = 0; r < 16; ++r, to += step) {
-        uint32_t mine;
-        asm volatile("ld.shared.b32 %0, [%1];" : "=r"(mine) : "r"((from ^ ((r & 7) * 16)) + r * 128));
-        const uintptr_t at = reinterpret_cast<uintptr_t>(to);
-        if (row0 + r < p.rows && (kBf16 && at & 2 ? odd : even)) reinterpret_cast<uint32_t*>(at & ~static_cast<uintptr_t>(3))[lane] = mine;
+    for (int i = 0; i < 2; ++i) {
+        const uintptr_t start = to + i * step;
+        at[i] = reinterpret_cast<uint32_t*>(start & ~static_cast<uintptr_t>(3)) + lane;
+        mine[i] = kBf16 && start & 2 ? shifted : whole;
+    }
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+        uint32_t w;
+        asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w) : "r"((from ^ ((r & 7) * 16)) + r * 128));
+        if (mine[r & 1] && r < rows) *at[r & 1] = w;
+        at[r & 1] = reinterpret_cast<uint32_t*>(reinterpret_cast<uint8_t*>(at[r & 1]) + 2 * step);
     }
 }
 
 // A tile's columns [c0, c1) of a warp's 32 rows (row0 + lane; channels from n0
 // on) to y through `staging`, so that a store has whole sectors whatever the
 // row stride; `taken` is called once they have left TMEM. scale, bias: the
-// tile's channels'. failed: NaN. Rows that are a multiple of 16 bytes apart go
+// tile's channels'; xs: the row's. failed: NaN. Rows that are a multiple of 16 bytes apart go
 // 64 bytes at a time; others 128, a row a store, since what they cost is the
-// instructions of every store.
+// instructions of every store (1001 x 5003 x 2064, bf16: 21.7 us; two rows a
+// store, with their alignment seen to there, 30.5; 5008 channels 20.5).
 template <bool kBf16, typename Taken>
 __device__ __forceinline__ void i8_take(const I8Params& p, uint32_t tmem, uint32_t staging, int row0, int n0, int c0, int c1,
-                                        const float* scale, const float* bias, bool failed, const Taken& taken) {
+                                        const float* scale, const float* bias, float xs, bool failed, const Taken& taken) {
     constexpr int kCols = kBf16 ? 32 : 16, kSize = kBf16 ? 2 : 4;  // 64 bytes
     const int lane = threadIdx.x & 31, row = row0 + lane;
-    const float xs = failed ? __int_as_float(0x7fc00000) : row < p.rows ? p.x_scales[row] : 0.0f;
+    if (failed) xs = __int_as_float(0x7fc00000);
     float finite = 0.0f;  // NaN once a value is not
     // kCols sums, the tile's from column c on, as they lie in y
     const auto values = [&](const uint32_t* r, int c, uint32_t* out) {
@@ -460,16 +470,29 @@ __device__ __forceinline__ void i8_take(const I8Params& p, uint32_t tmem, uint32
     }
 }
 
-// The channels' scales and biases of a tile, by the threads of warps 2-9.
+// What the threads of warps 2-9 read of scales and biases for a tile: each a
+// channel's and its row's, one tile ahead.
 template <int kN>
-__device__ __forceinline__ void i8_channels(const I8Params& p, int n0, float* scale, float* bias) {
-    for (int c = threadIdx.x - 64; c < kN; c += 256) {
-        scale[c] = n0 + c < p.channels ? p.w_scales[n0 + c] : 0.0f;
-        bias[c] = p.bias && n0 + c < p.channels ? p.bias[n0 + c] : 0.0f;
+struct I8Scales {
+    float channel, bias, row;
+    __device__ __forceinline__ void load(const I8Params& p, int own_row, int n0) {
+        const int n = n0 + static_cast<int>(threadIdx.x) - 64;
+        const bool in = static_cast<int>(threadIdx.x) - 64 < kN && n < p.channels;
+        channel = in ? p.w_scales[n] : 0.0f;
+        bias = in && p.bias ? p.bias[n] : 0.0f;
+        row = own_row < p.rows ? p.x_scales[own_row] : 0.0f;
     }
-    __syncwarp();
-    asm volatile("bar.sync 1, 256;" ::: "memory");
-}
+    // the channels' to all of those warps
+    __device__ __forceinline__ void share(float* scales, float* biases) const {
+        const int c = static_cast<int>(threadIdx.x) - 64;
+        if (c < kN) {
+            scales[c] = channel;
+            biases[c] = bias;
+        }
+        __syncwarp();
+        asm volatile("bar.sync 1, 256;" ::: "memory");
+    }
+};
 
 template <int kN, bool kBf16>
 __global__ void __launch_bounds__(kI8Threads, 1)
@@ -548,19 +571,25 @@ __global__ void __launch_bounds__(kI8Threads, 1)
         if (ok) mbar_settle_ring(empty, kStages, it);
     } else if (warp >= 2) {
         const int quarter = warp & 3;
-        int turn = 0;
-        for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x, ++turn) {
-            int m, n;
+        int turn = 0, m = 0, n = 0;
+        I8Scales<kN> scales{};
+        const auto ahead = [&](int tile) {
             i8_place(p, tile, m, n);
-            const int a = turn & 1;
-            i8_channels<kN>(p, n * kN, s_scale[a], s_bias[a]);
+            scales.load(p, m * 128 + quarter * 32 + lane, n * kN);
+        };
+        if (static_cast<int>(blockIdx.x) < tiles) ahead(blockIdx.x);
+        for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x, ++turn) {
+            const int a = turn & 1, row0 = m * 128 + quarter * 32, n0 = n * kN;
+            const float xs = scales.row;
+            scales.share(s_scale[a], s_bias[a]);
+            if (tile + static_cast<int>(gridDim.x) < tiles) ahead(tile + gridDim.x);
             mbar_wait(done + 8 * a, (turn / 2) & 1, nullptr, &s_failed);
             __syncwarp();
             const bool failed = __any_sync(kFull, *static_cast<volatile int*>(&s_failed));
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             const int c0 = (warp - 2) / 4 * (kN / 2);
             i8_take<kBf16>(p, tmem + a * kN + (static_cast<uint32_t>(quarter * 32) << 16), stages + kStages * kStageBytes + (warp - 2) * 2048,
-                           m * 128 + quarter * 32, n * kN, c0, c0 + kN / 2, s_scale[a], s_bias[a], failed, [&] {
+                           row0, n0, c0, c0 + kN / 2, s_scale[a], s_bias[a], xs, failed, [&] {
                                asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
                                __syncwarp();
                                if (lane == 0) mbar_arrive(drained + 8 * a);
@@ -848,19 +877,25 @@ __global__ void __launch_bounds__(kI8Threads, 1) __cluster_dims__(2, 1, 1)
     } else if (warp >= 2) {
         const int quarter = warp & 3;
         const uint32_t lead_drained = cluster_addr(drained, 0);
-        int turn = 0;
-        for (int tile = first; tile < tiles; tile += step, ++turn) {
-            int m, n;
+        int turn = 0, m = 0, n = 0;
+        I8Scales<kN> scales{};
+        const auto ahead = [&](int tile) {
             i8_place(p, tile, m, n);
-            const int a = turn & 1;
-            i8_channels<kN>(p, n * kN, s_scale[a], s_bias[a]);
+            scales.load(p, m * 256 + static_cast<int>(rank) * 128 + quarter * 32 + lane, n * kN);
+        };
+        if (first < tiles) ahead(first);
+        for (int tile = first; tile < tiles; tile += step, ++turn) {
+            const int a = turn & 1, row0 = m * 256 + static_cast<int>(rank) * 128 + quarter * 32, n0 = n * kN;
+            const float xs = scales.row;
+            scales.share(s_scale[a], s_bias[a]);
+            if (tile + step < tiles) ahead(tile + step);
             mbar_wait_cluster(done + 8 * a, (turn / 2) & 1, &s_failed);
             __syncwarp();
             const bool failed = __any_sync(kFull, *static_cast<volatile int*>(&s_failed));
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             const int c0 = (warp - 2) / 4 * (kN / 2);
             i8_take<kBf16>(p, tmem + a * kN + (static_cast<uint32_t>(quarter * 32) << 16), stages + kStages * kStageBytes + (warp - 2) * 2048,
-                           m * 256 + static_cast<int>(rank) * 128 + quarter * 32, n * kN, c0, c0 + kN / 2, s_scale[a], s_bias[a], failed, [&] {
+                           row0, n0, c0, c0 + kN / 2, s_scale[a], s_bias[a], xs, failed, [&] {
                                asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
                                __syncwarp();
                                if (lane == 0)

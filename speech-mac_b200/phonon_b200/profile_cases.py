@@ -22,7 +22,10 @@ cases:
             rings past the 250-key window, three steps
   perblock512  step512 with per-block-scale Q8_0 weights (three weight
             digit planes on the tensor cores)
-Each case runs three steps (or calls) after its set-up and prints "ok".
+  prompt8   nine launches, one each: rows to 8 bits, the 8-bit product's four
+            kernels, causal attention over packed prompts (two of the
+            engine's heads in bf16, one of 32 on 8 x 128, one in fp32)
+Each other case runs three steps (or calls) after its set-up and prints "ok".
 
   kvtypes   not for captures: ms a decode step of five batches with K/V in
             fp32, bf16 and 8 bits (20 timed steps after 6, device buffers)
@@ -117,6 +120,33 @@ def mimi64():
     m.close()
 
 
+def prompt8():
+    import torch
+    g = torch.Generator("cuda").manual_seed(1)
+    rows = torch.randn(8192, 4096, generator=g, device="cuda").bfloat16()
+    codes, scales = torch.empty(8192, 4096, dtype=torch.int8, device="cuda"), torch.empty(8192, device="cuda")
+    rt.QuantizeRows(rows.data_ptr(), codes.data_ptr(), scales.data_ptr(), 8192, 4096, rt.ROWS_BF16)()
+    weights = torch.randint(-127, 128, (4096, 4096), dtype=torch.int8, generator=g, device="cuda")
+    for n, channels, depth in ((16, 4096, 4096), (512, 512, 2048), (512, 4096, 4096), (2048, 4096, 4096)):
+        y = torch.empty(n, channels, dtype=torch.bfloat16, device="cuda")
+        rt.I8Product(codes.data_ptr(), scales.data_ptr(), weights.data_ptr(), scales.data_ptr(), y.data_ptr(), n, channels, depth,
+                     rt.ROWS_BF16)()
+    rng = np.random.default_rng(6)
+    for lengths, heads, kv_heads, dim, window, kind in (
+            (rng.integers(1, 513, 64), 8, 8, 64, 0, rt.ROWS_BF16), (rng.integers(100, 3001, 16), 8, 8, 64, 250, rt.ROWS_BF16),
+            ([4096, 4096], 32, 8, 128, 0, rt.ROWS_BF16), ([1100, 1400, 1700, 2048], 8, 8, 64, 0, rt.ROWS_F32)):
+        begin = torch.tensor(np.concatenate([[0], np.cumsum(lengths)]), dtype=torch.int32, device="cuda")
+        total = int(sum(lengths))
+        x = torch.randn(total, heads + 2 * kv_heads, dim, generator=g, device="cuda")
+        if kind == rt.ROWS_BF16:
+            x = x.bfloat16()
+        out = torch.empty(total, heads, dim, dtype=x.dtype, device="cuda")
+        rt.PromptAttention(x.data_ptr(), x[:, heads:].data_ptr(), x[:, heads + kv_heads:].data_ptr(), out.data_ptr(), begin.data_ptr(),
+                           len(lengths), total, int(max(lengths)), heads, kv_heads, dim, kind, window, q_stride=x.stride(0),
+                           k_stride=x.stride(0), v_stride=x.stride(0))()
+        torch.cuda.synchronize()
+
+
 def kvtypes():
     import torch
     w = synth.flow_weights(12, seed=0)
@@ -158,6 +188,7 @@ CASES = {
     "head512": head512,
     "frame1": frame1,
     "mimi64": mimi64,
+    "prompt8": prompt8,
     "kvtypes": kvtypes,
     "perblock512": lambda: _decode(512, [int(x) for x in np.random.default_rng(2).integers(64, 129, 512)], rt.KV_BF16,
                                    per_block=True),
