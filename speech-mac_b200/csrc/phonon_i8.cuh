@@ -26,7 +26,7 @@ struct I8QuantParams {
     int rows, cols;
 };
 
-// The nearest integer to x / s, ties to even: the nearest to x * (1 / s) is
+// The nearest integer to x / s, ties to even, of fp32 rows: the nearest to x * (1 / s) is
 // that but next to a border, and x - q s is exact (of both operands' last bits
 // and at most a step large), so that it says on which side x lies.
 __device__ __forceinline__ float i8_fix(float q, float x, float s) {
@@ -116,7 +116,15 @@ __global__ void __launch_bounds__(256, kBf16 ? 4 : 3) i8_quantize_kernel(I8Quant
         }
         if (!there) continue;
         const bool bad = top >= 0x7f800000u;
-        const float s = fmaxf(__fdiv_rn(__uint_as_float(top), 127.0f), 0x1p-126f), inverse = __frcp_rn(s);
+        const float s = fmaxf(__fdiv_rn(__uint_as_float(top), 127.0f), 0x1p-126f);
+        float inverse = __frcp_rn(s);
+        // bf16: x / s is k + 1/2 but for the rounding of s, or further from it than a few roundings (both have 8 bits
+        // but for the 127). So the product with a reciprocal that errs to the side of x / s rounds as x / s does:
+        // a step down where s is above top / 127, one up below it.
+        if constexpr (kBf16) {
+            const float over = fmaf(s, 127.0f, -__uint_as_float(top));
+            if (s > 0x1p-126f) inverse = __int_as_float(__float_as_int(inverse) - (over > 0.0f) + (over < 0.0f));
+        }
         if (t == 0) {
             p.scales[row] = bad ? __int_as_float(0x7fc00000) : s;
             if (bad) flag_nonfinite(p.status, static_cast<int>(row));
@@ -129,15 +137,15 @@ __global__ void __launch_bounds__(256, kBf16 ? 4 : 3) i8_quantize_kernel(I8Quant
             for (int k = 0; k < 8; k += 2) {
                 const float2 e = make_float2(x.element(k), x.element(k + 1));
                 const float2 by = make_float2(inverse, inverse), unit = make_float2(s, s), one = make_float2(-1.0f, -1.0f), round = make_float2(kRound, kRound);
-                // (the second step: quotients that are a rounding of the scale away from a border, which bf16 rows have many of)
-                float2 near = fma2(e, by, round);
-                near = fma2(fma2(fma2(near, one, round), unit, e), by, near);
-                const float2 rest = fma2(fma2(near, one, round), unit, e);
-                far = fmaxf(far, fmaxf(fabsf(rest.x), fabsf(rest.y)));
+                const float2 near = fma2(e, by, round);
+                if constexpr (!kBf16) {
+                    const float2 rest = fma2(fma2(near, one, round), unit, e);
+                    far = fmaxf(far, fmaxf(fabsf(rest.x), fabsf(rest.y)));
+                }
                 w[k] = __float_as_uint(near.x);
                 w[k + 1] = __float_as_uint(near.y);
             }
-            if (2.0f * far >= s) {
+            if (!kBf16 && 2.0f * far >= s) {
 #pragma unroll
                 for (int k = 0; k < 8; ++k) w[k] = __float_as_uint(i8_fix(__uint_as_float(w[k]) - kRound, x.element(k), s) + kRound);
             }
