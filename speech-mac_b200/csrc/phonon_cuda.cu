@@ -4770,8 +4770,8 @@ int device_sms(int device, int* sms) {
 
 template <bool kBf16, int kThreads, int kUnits>
 int quantize_launch(const I8QuantParams& p, int sms, cudaStream_t s) {
-    // CTAs that take several rows each once they fill the GPU (bf16, 8192 x 4096: 22.8 us, a CTA for every two rows 25.0)
-    const long long ctas = (p.rows + 256ll / kThreads - 1) / (256 / kThreads), most = (kBf16 ? 4ll : 3ll) * sms;
+    // CTAs that take several rows each once they fill the GPU: a row's loads go out while the one before is written
+    const long long ctas = (p.rows + 256ll / kThreads - 1) / (256 / kThreads), most = static_cast<long long>(i8_quantize_ctas<kBf16, kUnits>()) * sms;
     CUDA_TRY(launch_pdl(i8_quantize_kernel<kBf16, kThreads, kUnits>, dim3(static_cast<unsigned>(std::min(ctas, most))), dim3(256), 0, s, p));
     return PHONON_CUDA_OK;
 }

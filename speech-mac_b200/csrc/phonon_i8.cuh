@@ -66,11 +66,20 @@ struct I8Unit {
     }
 };
 
+// CTAs an SM: as many as registers hold without spills (rows of 256 bf16: 18.1
+// us for 100000, with 4 CTAs an SM 20.6; 20000 of 512: 6.7, 9.8).
+template <bool kBf16, int kUnits>
+__host__ __device__ constexpr int i8_quantize_ctas() {
+    return kBf16 ? kUnits == 1 ? 8 : kUnits == 2 ? 6 : 4 : kUnits == 1 ? 5 : kUnits == 2 ? 4 : 2;
+}
+
 // kThreads threads a row, kUnits units of 8 elements a thread in registers, as
 // they lie, the next row's on their way meanwhile; a row of more is read twice.
-// Bound by the bytes.
+// Bound by the bytes: 8192 x 4096 bf16 in 16.7 us (6.0 TB/s, 92 % of a plain
+// copy's rate), fp32 in 26.2 (6.4). Short rows by their first loads: 64 x 512
+// fp32 in 1.7.
 template <bool kBf16, int kThreads, int kUnits>
-__global__ void __launch_bounds__(256, kBf16 ? 4 : 3) i8_quantize_kernel(I8QuantParams p) {
+__global__ void __launch_bounds__(256, i8_quantize_ctas<kBf16, kUnits>()) i8_quantize_kernel(I8QuantParams p) {
     constexpr int kRows = 256 / kThreads, kWarps = kThreads / 32;
     constexpr float kRound = 12582912.0f;  // 1.5 * 2^23: adding it rounds to an integer
     __shared__ uint32_t s_top[2][8];
