@@ -241,3 +241,31 @@ def test_rows_of_every_alignment_and_width(cuda_ok, rows, depth, channels, bf16)
             torch.cuda.synchronize()
             check_product(y[:rows, :n], *product_want(x, w, xs, ws, bias), bf16)
             assert (y[rows:] == 7).all() and (y[:, n:] == 7).all()
+
+
+@pytest.mark.parametrize("rows", [1, 12, 40])
+def test_weights_that_the_pass_ahead_has_written(cuda_ok, rows):
+    """Weights quantised on the device, the product right behind, again and again over other weights: eager and replayed."""
+    rng = np.random.default_rng(rows)
+    channels, depth = 2000, 1040
+    x, _, xs, _ = product_case(rng, rows, 1, depth)
+    raw = torch.empty(channels, depth, device="cuda")
+    w, ws = torch.zeros(channels, depth, dtype=torch.int8, device="cuda"), torch.zeros(channels, device="cuda")
+    y = torch.empty(rows, channels, device="cuda")
+    first = rt.QuantizeRows(raw.data_ptr(), w.data_ptr(), ws.data_ptr(), channels, depth)
+    second = rt.I8Product(x.data_ptr(), xs.data_ptr(), w.data_ptr(), ws.data_ptr(), y.data_ptr(), rows, channels, depth)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        for c in (first, second):
+            c(stream_ptr=torch.cuda.current_stream().cuda_stream)
+    for turn in range(6):
+        raw.copy_(torch.tensor(rng.standard_normal((channels, depth)), dtype=torch.float32))
+        if turn % 2:
+            graph.replay()
+        else:
+            first(stream_ptr=torch.cuda.current_stream().cuda_stream)
+            second(stream_ptr=torch.cuda.current_stream().cuda_stream)
+        torch.cuda.synchronize()
+        want_q, want_s = quantized(raw.double().cpu().numpy())
+        assert np.array_equal(w.double().cpu().numpy(), want_q)
+        check_product(y, *product_want(x, torch.tensor(want_q, device="cuda"), xs, torch.tensor(want_s, device="cuda"), None), False)
