@@ -604,7 +604,8 @@ int phonon_cuda_quantize_rows_device(int device, const PhononCudaQuantizeRows *a
  * that the call reads.
  * status_dev (device, [rows], optional, zeroed by the caller) is raised to
  * NON_FINITE for a row with a non-finite result, and to DEVICE_ERROR where
- * the kernel gave up a bounded wait (about two seconds): the row is NaN. */
+ * the kernel gave up a bounded wait (about two seconds): the row is NaN. The
+ * call returns CAPACITY for a y of more than 2^26 tiles (128 x 64 to 256 x 256). */
 typedef struct {
     uint32_t type; /* PhononCudaRowType of y */
     uint32_t rows, channels, depth;

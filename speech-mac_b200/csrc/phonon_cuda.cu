@@ -4782,7 +4782,10 @@ int quantize_rows(const I8QuantParams& p, int sms, cudaStream_t s) {
     if (p.cols <= 512) return quantize_launch<kBf16, 32, 2>(p, sms, s);
     if (p.cols <= 1024) return quantize_launch<kBf16, 64, 2>(p, sms, s);
     if (p.cols <= 2048) return quantize_launch<kBf16, 128, 2>(p, sms, s);
-    if (p.cols <= 4096) return kBf16 ? quantize_launch<kBf16, 128, 4>(p, sms, s) : quantize_launch<kBf16, 256, 2>(p, sms, s);
+    if (p.cols <= 4096) {
+        if constexpr (kBf16) return quantize_launch<kBf16, 128, 4>(p, sms, s);
+        else return quantize_launch<kBf16, 256, 2>(p, sms, s);
+    }
     return quantize_launch<kBf16, 256, 4>(p, sms, s);
 }
 

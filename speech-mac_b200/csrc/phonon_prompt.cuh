@@ -147,7 +147,17 @@ __device__ __forceinline__ void prompt_put_rows(void* out, long long own, uint32
 // that is not finite is NaN. So where an output is not finite the CTA starts
 // over, carefully: warp 8 looks at every turn's values, puts 0 in place of
 // those that are not finite, and the rows that see one become NaN. (Nothing is
-// written before: out may lie over q.)
+// written before: out may lie over q. The pass has barriers of its own; none is
+// ever set up twice.)
+//
+// Measured: prompts of 8191 and 7500, 32 heads on 8 x 128, 885 us, 1.2 PFLOP/s
+// of the products that rows see (73 % of the measured matrix rate); 4 of 4096,
+// 16 heads of 128 280 us, of 64 213 (0.98 and 0.65 PFLOP/s). With 128 dims
+// matrix and exponential units are each busy half of the time, and the two
+// tiles' turns do not fill each other's gaps; with 64 the exponentials are the
+// most. 64 prompts of up to 512 take 40 us and 16 with a window of 250 61, bound
+// by a turn's chain (S, its maximum, weights, P v: 2000 clocks and more) and
+// a CTA's start and end (4000), four tiles an SM.
 constexpr int kPromptThreads = 384;
 constexpr float kPromptSlack = 8.0f;
 
@@ -592,9 +602,15 @@ __global__ void __launch_bounds__(kPromptThreads, PromptShape<D>::kCtas)
 //               sum truncates: 24 truncations a turn stay near fp32's rounding,
 //               thousands would not)
 //
-// Bound by the tensor cores. Values that are not finite: as for bf16 rows; of
-// keys that are not, or would not be as bf16, the careful CTA computes the
-// scores one by one.
+// Values that are not finite: as for bf16 rows; of keys that are not, or would
+// not be as bf16, the careful CTA computes the scores one by one.
+//
+// Measured: 2 prompts of 4096, 16 heads of 128, 700 us, 196 TFLOP/s of the
+// products that rows see, 1.2 PFLOP/s of slices (72 % of the measured matrix
+// rate); of 64 366 us; 4 of 1024 to 2048, 8 x 64, 90 us. Long prompts are bound
+// by the tensor cores; short ones by a CTA's start, end and chain of turns
+// (one of 128: 9 us). Errors stay at or below those of the plain form in fp32
+// (0.1 to 0.5e-6 of the output's norm against 0.1 to 1.2e-6).
 constexpr int kPromptF32Threads = 512, kPromptF32Keys = 64;
 // A thread's registers in warps 0-3 and 4-15, together the launch's 128 each.
 constexpr int kPromptF32SoftmaxRegisters = 240, kPromptF32OtherRegisters = 88;
