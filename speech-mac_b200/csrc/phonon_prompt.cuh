@@ -281,12 +281,12 @@ __global__ void __launch_bounds__(kPromptThreads, PromptShape<D>::kCtas)
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     pdl_wait();
-    pdl_trigger();
     const int slot = static_cast<int>(kv8_div(blockIdx.x, p.by_heads)), part = static_cast<int>(blockIdx.x - slot * p.by_heads.d);
     if (warp == 0) prompt_find(p, slot, blockIdx.x == gridDim.x - 1, &s_tile);
     if (warp == 9) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&s_tmem)), "n"(Shape::kTmemCols) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        pdl_trigger();  // (not before: the next launch's CTAs, which wait for this one's end, may take TMEM where there is any left)
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
@@ -690,12 +690,12 @@ __global__ void __launch_bounds__(kPromptF32Threads, 1) prompt_f32_kernel(Prompt
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     pdl_wait();
-    pdl_trigger();
     const int slot = static_cast<int>(kv8_div(blockIdx.x, p.by_heads)), part = static_cast<int>(blockIdx.x - slot * p.by_heads.d);
     if (warp == 0) prompt_find(p, slot, blockIdx.x == gridDim.x - 1, &s_tile);
     if (warp == 4) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_addr(&s_tmem)) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        pdl_trigger();  // (not before: the next launch's CTAs, which wait for this one's end, may take TMEM where there is any left)
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();

@@ -269,3 +269,17 @@ def test_weights_that_the_pass_ahead_has_written(cuda_ok, rows):
         want_q, want_s = quantized(raw.double().cpu().numpy())
         assert np.array_equal(w.double().cpu().numpy(), want_q)
         check_product(y, *product_want(x, torch.tensor(want_q, device="cuda"), xs, torch.tensor(want_s, device="cuda"), None), False)
+
+
+@pytest.mark.parametrize("exponent", [0, 100, -110, -119, -126, -133])
+def test_every_pair_of_bf16_mantissas(cuda_ok, exponent):
+    """A row for each mantissa of the largest element, every mantissa at twelve powers of two below: quotients of k + 1/2 but for
+    the scale's rounding among them, and (the last exponents) scales at the smallest."""
+    m = np.arange(128, 256, dtype=np.float64)
+    x = np.concatenate([m * 2.0 ** -j for j in range(12)])
+    x = np.where(x[None] <= m[:, None], x[None], m[:, None]) * np.where(np.arange(len(x)) % 2, -1.0, 1.0) * 2.0 ** exponent
+    x[:, 0] = m * 2.0 ** exponent
+    held = torch.tensor(x).to(torch.bfloat16).cuda()  # (below 2^-133 of the last ones: rounded)
+    q, scales = run_quantize(held, True)
+    want_q, want_s = quantized(held.double().cpu().numpy())
+    assert np.array_equal(scales, want_s) and np.array_equal(q, want_q)

@@ -25,3 +25,15 @@ def test_no_load_goes_to_several_ctas():
         code = re.sub(r"//.*", "", (CSRC / name).read_text())
         for text in re.findall(r'"(cp\.async\.bulk[^"]*)"', code):
             assert "multicast" not in text
+
+
+@pytest.mark.parametrize("name", ["phonon_i8.cuh", "phonon_prompt.cuh"])
+def test_the_next_launch_starts_when_tensor_memory_is_held(name):
+    """A launch that starts early waits for the end of the one ahead, with tensor memory of its own in hand: a CTA of the one
+    ahead that still had to get its own could wait for it in turn, for good."""
+    code = re.sub(r"//.*", "", (CSRC / name).read_text())
+    for k in re.split(r"__global__", code)[1:]:
+        if "tcgen05.alloc" in k:
+            assert k.count("pdl_trigger();") == 1
+            between = k[k.index("tcgen05.alloc"):k.index("pdl_trigger();")]
+            assert "\n    }" not in between or "__syncthreads();" in between  # the same warp's, or behind a barrier
