@@ -624,7 +624,8 @@ int phonon_cuda_i8_product_device(int device, const PhononCudaI8Product *args, i
  * (p - window, p], or [0, p] where window is 0. Rows of no prompt, before
  * row_begin[0] or from row_begin[prompts] on, are left as they were. max_rows
  * bounds every prompt's rows. Sums and softmax statistics are fp32; bf16 rows:
- * weights are rounded to bf16 (an output's error stays near its own rounding).
+ * weights are rounded to bf16 (an output's error stays near its own rounding);
+ * fp32 rows: parts of a query, key or value below 2^-133 count as 0.
  * Enqueued on `cuda_stream` of `device`, like the cache's calls; status_dev
  * (device, [prompts], optional, zeroed by the caller) is raised for a prompt
  *   - whose rows lie outside [0, rows), are more than max_rows or begin before

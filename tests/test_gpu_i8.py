@@ -283,3 +283,29 @@ def test_every_pair_of_bf16_mantissas(cuda_ok, exponent):
     q, scales = run_quantize(held, True)
     want_q, want_s = quantized(held.double().cpu().numpy())
     assert np.array_equal(scales, want_s) and np.array_equal(q, want_q)
+
+
+def test_calls_at_the_same_time(cuda_ok):
+    """Every kernel of the product on three streams at once, again and again: what each gives alone, bit for bit."""
+    rng = np.random.default_rng(12)
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    jobs = []
+    for rows, channels, depth in ((9, 1536, 512), (40, 512, 2048), (512, 1000, 1024), (520, 4096, 4096), (1030, 5003, 2064)):
+        x, w, xs, ws = product_case(rng, rows, channels, depth)
+        outs = [torch.empty(rows, channels, dtype=torch.bfloat16, device="cuda") for _ in range(len(streams) + 1)]
+        calls = [rt.I8Product(x.data_ptr(), xs.data_ptr(), w.data_ptr(), ws.data_ptr(), y.data_ptr(), rows, channels, depth, rt.ROWS_BF16)
+                 for y in outs]
+        jobs.append((x, w, xs, ws, outs, calls))
+    for *_, calls in jobs:
+        calls[-1]()
+    torch.cuda.synchronize()
+    for x, w, xs, ws, outs, _ in jobs:
+        check_product(outs[-1], *product_want(x, w, xs, ws, None), True)
+    for turn in range(5):
+        for i, s in enumerate(streams):
+            for j in range(len(jobs)):
+                jobs[(j + i + turn) % len(jobs)][-1][i](stream_ptr=s.cuda_stream)
+    torch.cuda.synchronize()
+    for *_, outs, _ in jobs:
+        for y in outs[:-1]:
+            assert torch.equal(y, outs[-1])
