@@ -26,9 +26,10 @@ struct I8QuantParams {
     int rows, cols;
 };
 
-// The nearest integer to x / s, ties to even, of fp32 rows: the nearest to x * (1 / s) is
-// that but next to a border, and x - q s is exact (of both operands' last bits
-// and at most a step large), so that it says on which side x lies.
+// fp32 rows: the nearest integer to x / s, ties to even. The nearest to
+// x * (1 / s) is that but next to a border, and x - q s is exact (of both
+// operands' last bits and at most a step large), so that it says on which side
+// x lies.
 __device__ __forceinline__ float i8_fix(float q, float x, float s) {
     const float rest = fmaf(-q, s, x), twice = 2.0f * fabsf(rest);  // (half the smallest scales is not a float)
     const bool odd = static_cast<int>(q) & 1;
@@ -281,7 +282,7 @@ __device__ __forceinline__ void mbar_settle(uint32_t bar, uint32_t parity) {
 
 // The last phases of a ring of `stages` barriers that was used n times, which
 // nobody has waited for: no arrival is on its way when the CTA gives its
-// memory back or sets its barriers up anew (commits arrive in any order).
+// memory back (commits arrive in any order).
 __device__ __forceinline__ void mbar_settle_ring(uint32_t bars, int stages, int n) {
     for (int j = max(0, n - stages); j < n; ++j) mbar_settle(bars + 8 * (j % stages), (j / stages) & 1);
 }
@@ -383,10 +384,11 @@ __device__ __forceinline__ void i8_store_words(const I8Params& p, uint32_t stagi
 // A tile's columns [c0, c1) of a warp's 32 rows (row0 + lane; channels from n0
 // on) to y through `staging`, so that a store has whole sectors whatever the
 // row stride; `taken` is called once they have left TMEM. scale, bias: the
-// tile's channels'; xs: the row's. failed: NaN. Rows that are a multiple of 16 bytes apart go
-// 64 bytes at a time; others 128, a row a store, since what they cost is the
-// instructions of every store (1001 x 5003 x 2064, bf16: 21.7 us; two rows a
-// store, with their alignment seen to there, 30.5; 5008 channels 20.5).
+// tile's channels'; xs: the row's. failed: NaN. Rows that are a multiple of 16
+// bytes apart go 64 bytes at a time; others 128, a row a store, since what they
+// cost is the instructions of every store (1001 x 5003 x 2064, bf16: 21.7 us;
+// two rows a store, with their alignment seen to there, 30.5; 5008 channels
+// 20.5).
 template <bool kBf16, typename Taken>
 __device__ __forceinline__ void i8_take(const I8Params& p, uint32_t tmem, uint32_t staging, int row0, int n0, int c0, int c1,
                                         const float* scale, const float* bias, float xs, bool failed, const Taken& taken) {
