@@ -787,6 +787,7 @@ __global__ void __launch_bounds__(kI8Threads, 1)
         if (bad && p.status) atomicMax(p.status + row, kStatusDevice);
         else if (!finite) flag_nonfinite(p.status, row);
     }
+    __syncwarp();  // (rows behind the last and lanes with other stores end their turns apart)
     cluster_meet();  // no CTA's sums go while another reads them
     if (warp == 1) {
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
