@@ -182,6 +182,9 @@ __global__ void __launch_bounds__(kKv8PromptThreads, 1) kv8_prompt_kernel(Kv8Att
     __shared__ float s_f[128 * kTiles];
     __shared__ float2 s_ml[2][128];  // M, sum
     pdl_wait();
+    // Ahead of this CTA's tensor memory: the next launch's CTAs, which wait for this one's end, might hold what there is, but
+    // none comes to an SM beside a CTA that has all of its registers. (Behind it, 4 x 256 rows take 26.4 us, not 25.8.)
+    static_assert(kKv8PromptRegisters == 64 * 1024, "the next launch may not start before this one holds its tensor memory");
     pdl_trigger();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t later = kv8_div(blockIdx.x, p.by_items), item = blockIdx.x - later * p.by_items.d;

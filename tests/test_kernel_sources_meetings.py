@@ -1,5 +1,5 @@
-"""Where warps of the 8-bit product's kernels have to be whole again. CPU only: what follows from a warp that is not would be
-undefined, so no run is asked."""
+"""Where a kernel's warps have to be whole again, and from where on the next launch may start. CPU only: what follows where
+that is not kept is undefined or a wait for good, so no run is asked."""
 import re
 
 from phonon_b200._libs import CSRC
@@ -15,3 +15,19 @@ def test_warps_are_whole_where_a_cluster_meets():
     meets = [i for i, x in enumerate(lines) if x == "cluster_meet();"]
     assert len(meets) >= 4
     assert all(lines[i - 1] in WHOLE for i in meets), [lines[i - 1] for i in meets]
+
+
+def test_no_kernel_lets_the_next_launch_start_before_it_holds_its_tensor_memory():
+    """The next launch waits for this one's end, and may hold tensor memory by then: CTAs of this one that still had to get
+    theirs would wait for it in turn, for good. A kernel that does it all the same states, where it is compiled, that its CTAs
+    have all registers of an SM (which the host checks before the launch), so that no other CTA is beside one."""
+    found = 0
+    for path in sorted(CSRC.glob("*.cuh")):
+        code = re.sub(r"//.*", "", path.read_text())
+        for kernel in re.split(r"__global__", code)[1:]:
+            if "tcgen05.alloc" not in kernel or "pdl_trigger();" not in kernel:
+                continue
+            found += 1
+            ahead = kernel[:kernel.index("pdl_trigger();")]
+            assert "tcgen05.alloc" in ahead or re.search(r"static_assert\(k\w+Registers == 64 \* 1024,", ahead), path.name
+    assert found >= 8
