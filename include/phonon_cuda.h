@@ -633,8 +633,9 @@ int phonon_cuda_i8_product_device(int device, const PhononCudaI8Product *args, i
  *   - with a non-finite output (NON_FINITE): a row that sees a value which is
  *     not finite, whatever its weight, or whose own query (fp32: times the
  *     scale, beyond 2.3e38) or a score is not, but for scores of -infinity
- *     beside others, which are weights of 0. Other rows are what they are
- *     without it;
+ *     beside others, which are weights of 0. Finite values give finite
+ *     outputs, up to the type's largest. Other rows are what they are without
+ *     it;
  *   - where the kernel gave up a bounded wait (DEVICE_ERROR, about two
  *     seconds): rows of it are NaN.
  * The largest code stays. out may be q with q's stride, or lie apart from q, k
