@@ -635,7 +635,7 @@ int phonon_cuda_i8_product_device(int device, const PhononCudaI8Product *args, i
  *     scale, beyond 2.3e38) or a score is not, but for scores of -infinity
  *     beside others, which are weights of 0. Finite values give finite
  *     outputs, up to the type's largest. Other rows are what they are without
- *     it;
+ *     it (near it, bits of values below 2^-60 may be lost);
  *   - where the kernel gave up a bounded wait (DEVICE_ERROR, about two
  *     seconds): rows of it are NaN.
  * The largest code stays. out may be q with q's stride, or lie apart from q, k

@@ -110,6 +110,20 @@ __device__ __forceinline__ float4 prompt_get16(uint32_t at) {
     return v;
 }
 
+// A lane's staged row of kRow bytes, fp32 or bf16: infinities become the largest
+// number of their sign. (Not unrolled: few rows come here.)
+template <int kRow, bool kBf16>
+__device__ __forceinline__ void prompt_within(uint32_t staging) {
+#pragma unroll 1
+    for (int k = 0; k < kRow; k += 4) {
+        const uint32_t at = prompt_staged<kRow>(staging, threadIdx.x & 31, k / 16) + k % 16;
+        uint32_t w;
+        asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w) : "r"(at));
+        w -= kBf16 ? __vcmpeq2(w & 0x7fff7fffu, 0x7f807f80u) & 0x00010001u : (w & 0x7fffffffu) == 0x7f800000u;
+        asm volatile("st.shared.b32 [%0], %1;" ::"r"(at), "r"(w) : "memory");
+    }
+}
+
 // A warp's 32 staged rows (of kRow bytes) to the output, whole sectors at a
 // time. own: the byte of the output that the lane's row goes to, or -1.
 template <int kRow>
@@ -149,9 +163,12 @@ __device__ __forceinline__ void prompt_put_rows(void* out, long long own, uint32
 // those that are not finite, and the rows that see one become NaN. And O, which
 // is divided by the sum of weights at the end, may leave fp32's range where the
 // mean of the values does not (weights up to 2^8 times any value, over all
-// keys): where the largest value could, that pass has the values times 2^-k.
-// (Rows whose output is finite are written before it, the others behind it: out
-// may lie over q. The pass has barriers of its own; none is ever set up twice.)
+// keys), so that pass has the values times a power of two: exact, but for
+// values below 2^-60, some of whose bits may be lost beside the others.
+// (Nothing is written before: out may lie over q. The pass has barriers of its
+// own; none is ever set up twice. Both passes are a loop over the same code, and
+// what the second adds is kept small: more of it, behind branches that are not
+// taken, took calls with 128 dims 5 % longer.)
 //
 // Measured: prompts of 8191 and 7500, 32 heads on 8 x 128, 885 us, 1.2 PFLOP/s
 // of the products that rows see (73 % of the measured matrix rate); 4 of 4096,
@@ -199,39 +216,11 @@ __device__ __forceinline__ uint64_t umma_desc_rows(uint32_t addr, uint32_t block
     return d;
 }
 
-constexpr float kBf16Most = 3.38953139e38f;  // the largest bf16
-
-// k of the 2^-k that keeps a sum over `keys` weights up to 2^over times values
-// whose largest magnitude has the bits `top` below 2^126.
-__device__ __forceinline__ int prompt_down(uint32_t top, int keys, int over) {
-    return max(0, static_cast<int>(top >> 23) - 126 + over + 32 - __clz(keys) - 126);
-}
+// k of the 2^-k that keeps a sum over `keys` weights up to 2^over times any
+// values below 2^126.
+__device__ __forceinline__ int prompt_down(int keys, int over) { return 34 - __clz(keys) + over; }
 
 __device__ __forceinline__ float prompt_pow2(int e) { return __int_as_float((127 + e) << 23); }
-
-// x between -most and most, as a mean of such values is; NaN stays.
-__device__ __forceinline__ float prompt_within(float x, float most) {
-    asm("min.NaN.f32 %0, %0, %1;" : "+f"(x) : "f"(most));
-    asm("max.NaN.f32 %0, %0, %1;" : "+f"(x) : "f"(-most));
-    return x;
-}
-
-// The bits of the largest finite magnitude of the values of rows [row0, row0 +
-// rows), D of each, raised in *top by `threads` threads.
-template <int D, bool kBf16>
-__device__ __forceinline__ void prompt_top(const PromptParams& p, long long row0, int rows, int head, int thread, int threads, uint32_t* top) {
-    uint32_t most = 0;
-#pragma unroll 1
-    for (int x = thread; x < rows * (D / 4); x += threads) {
-        const float4 v = load_row4<kBf16>(p.v, (row0 + x / (D / 4)) * p.v_stride + head * D + x % (D / 4) * 4);
-        const float each[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-            if (isfinite(each[k])) most = max(most, __float_as_uint(fabsf(each[k])));
-    }
-    most = __reduce_max_sync(kFull, most);
-    if ((threadIdx.x & 31) == 0) atomicMax(top, most);
-}
 
 constexpr uint32_t kUmmaBMnMajor = 1u << 16;  // of an instruction descriptor
 
@@ -244,8 +233,10 @@ __device__ __forceinline__ void tmem_store16(uint32_t taddr, const uint32_t (&r)
         : "memory");
 }
 
-__device__ __forceinline__ uint32_t bf16x2_times(uint32_t a, uint32_t b) {
-    const __nv_bfloat162 h = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&b));
+// Two bf16 times 2^-down.
+__device__ __forceinline__ uint32_t bf16x2_smaller(uint32_t w, int down) {
+    const uint32_t by = (127 - down) * 0x800080u;
+    const __nv_bfloat162 h = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&w), *reinterpret_cast<const __nv_bfloat162*>(&by));
     return *reinterpret_cast<const uint32_t*>(&h);
 }
 
@@ -289,7 +280,6 @@ __global__ void __launch_bounds__(kPromptThreads, PromptShape<D>::kCtas)
     __shared__ uint32_t s_tmem;
     __shared__ PromptTile s_tile;
     __shared__ int s_failed, s_dirty;
-    __shared__ uint32_t s_top;  // careful: the largest value's bits
     __shared__ uint32_t s_bad[kStages][kKeys / 32];  // careful: which of a turn's values are not finite
     const uint32_t s_q = (smem_addr(smem_raw) + 1023) & ~1023u, s_k = s_q + 2 * kQTile, s_v = s_k + kStages * kTile;
     uint32_t bars = smem_addr(s_bars);  // of this pass
@@ -320,7 +310,7 @@ __global__ void __launch_bounds__(kPromptThreads, PromptShape<D>::kCtas)
             init(o_full(), 4, 1);  // and q_full(), tail()
             init(idle(), 1, kIssuers);
         }
-        s_failed = s_dirty = s_top = 0;
+        s_failed = s_dirty = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     pdl_wait();
@@ -357,13 +347,11 @@ __global__ void __launch_bounds__(kPromptThreads, PromptShape<D>::kCtas)
         __syncwarp();
         asm volatile("bar.sync 1, %0;" ::"n"(kPromptThreads) : "memory");
     };
-    // Every warp, at its end: whether the CTA starts over. The softmax's warps meet the others once more by themselves: when
-    // the rows that are done have been written.
-    const auto again = [&](bool writes) {
+    // Every warp, at its end: whether the CTA starts over.
+    const auto again = [&] {
         asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
         sync();
         if (careful || !s_dirty || s_failed) return false;
-        if (!writes) sync();
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         bars += 8 * kBars;
         return careful = true;
@@ -382,7 +370,6 @@ __global__ void __launch_bounds__(kPromptThreads, PromptShape<D>::kCtas)
                 if (two) load(s_q + kQTile, &tm_q, 128, head0, t.row0 + t.first + half, q_full());
             }
             int j = 0, looks = 0;
-            const int down = careful ? prompt_down(s_top, end - key0, 8) : 0;
             for (; j < turns; ++j) {
                 const int s = j % kStages, row = t.row0 + key0 + j * kKeys, there = end - key0 - j * kKeys;
                 if (j >= kStages && !wait(k_empty() + 8 * s, j / kStages - 1)) break;
@@ -414,15 +401,18 @@ __global__ void __launch_bounds__(kPromptThreads, PromptShape<D>::kCtas)
                                 if ((w[k] & 0x7f80u) == 0x7f80u) w[k] &= 0xffff0000u, put = bad = true;
                                 if ((w[k] & 0x7f800000u) == 0x7f800000u) w[k] &= 0xffffu, put = bad = true;
                             }
-                            if (down) {
-                                put = true;
-#pragma unroll
-                                for (int k = 0; k < 4; ++k) w[k] = bf16x2_times(w[k], (127 - down) * 0x800080u);  // twice 2^-down
-                            }
                         }
                         if (put) kv8_put16(at + c, w[0], w[1], w[2], w[3]);
                     }
                     if (bad) atomicOr(&s_bad[s][key >> 5], 1u << (key & 31));
+                }
+                if (careful) {
+                    __syncwarp();
+                    for (int x = lane; x < kTile / 4; x += 32) {
+                        uint32_t w;
+                        asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w) : "r"(s_v + s * kTile + 4 * x));
+                        asm volatile("st.shared.b32 [%0], %1;" ::"r"(s_v + s * kTile + 4 * x), "r"(bf16x2_smaller(w, prompt_down(end - key0, 8))) : "memory");
+                    }
                 }
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
@@ -434,7 +424,7 @@ __global__ void __launch_bounds__(kPromptThreads, PromptShape<D>::kCtas)
                 mbar_settle_ring(v_full(), kStages, j + 1);
             }
             __syncwarp();
-        } while (again(false));
+        } while (again());
         else if (warp < 9 + kIssuers) do {
             constexpr uint32_t idesc_s = umma_idesc_bf16(128, kKeys), idesc_o = umma_idesc_bf16(128, D) | kUmmaBMnMajor;
             constexpr int kSteps = kBytes / 32;  // of 16 dims in a row of a box
@@ -510,9 +500,9 @@ __global__ void __launch_bounds__(kPromptThreads, PromptShape<D>::kCtas)
                 mbar_settle_ring(v_empty(), kStages, turns);
             }
             __syncwarp();
-        } while (again(false));
+        } while (again());
         else do {
-        } while (again(false));
+        } while (again());
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Shape::kSoftmaxRegisters));
         const int tile = warp >> 2, quarter = warp & 3, r = quarter * 32 + lane;
@@ -523,13 +513,7 @@ __global__ void __launch_bounds__(kPromptThreads, PromptShape<D>::kCtas)
         const uint32_t at_o = tmem + kTmemO + tile * D + (static_cast<uint32_t>(quarter * 32) << 16);
         const bool mine = at < half && position <= last;
         uint32_t w[D / 2];  // the row's output
-        bool good = true, left = mine;  // left: not written yet
-        const auto put = [&](bool rows) {  // through q's room, which nothing reads any more
-            const uint32_t staging = s_q + tile * kQTile + quarter * (32 * 2 * D);
-#pragma unroll
-            for (int k = 0; k < D / 8; ++k) kv8_put16(prompt_staged<2 * D>(staging, lane, k), w[4 * k], w[4 * k + 1], w[4 * k + 2], w[4 * k + 3]);
-            prompt_put_rows<2 * D>(p.out, rows ? 2 * ((t.row0 + position) * p.out_stride + (head0 + r - at * pack) * D) : -1, staging);
-        };
+        bool good = true;
         do {
             float m = -INFINITY, l = 0.0f;
             for (int j = in.begin; j < in.end; ++j) {
@@ -613,7 +597,7 @@ __global__ void __launch_bounds__(kPromptThreads, PromptShape<D>::kCtas)
             if (in.end > in.begin) wait(o_full() + 8 * tile, 0);
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             float inverse = *static_cast<volatile int*>(&s_failed) ? __int_as_float(0x7fc00000) : __fdiv_rn(1.0f, l);
-            if (careful) inverse *= prompt_pow2(prompt_down(s_top, end - key0, 8));
+            if (careful) inverse *= prompt_pow2(prompt_down(end - key0, 8));
             const __nv_bfloat162 zero = __floats2bfloat162_rn(0.0f, 0.0f);
             __nv_bfloat162 clean = zero;  // NaN once an output is not finite
 #pragma unroll
@@ -627,27 +611,16 @@ __global__ void __launch_bounds__(kPromptThreads, PromptShape<D>::kCtas)
                     clean = __hfma2(*reinterpret_cast<const __nv_bfloat162*>(&w[c / 2 + k]), zero, clean);
                 }
             }
-            if (careful) {
-                const __nv_bfloat162 most = __floats2bfloat162_rn(kBf16Most, kBf16Most);
-                clean = zero;
-#pragma unroll
-                for (int k = 0; k < D / 2; ++k) {  // a mean of values is no larger than they are; NaN stays
-                    __nv_bfloat162& x = reinterpret_cast<__nv_bfloat162&>(w[k]);
-                    x = __hmin2_nan(__hmax2_nan(x, __hneg2(most)), most);
-                    clean = __hfma2(x, zero, clean);
-                }
-            }
-            good = !left || __low2float(clean) + __high2float(clean) == 0.0f;
+            good = !mine || __low2float(clean) + __high2float(clean) == 0.0f || (careful && inverse < INFINITY);
             if (!good) s_dirty = 1;
             __syncwarp();
-            if (!again(true)) break;
-            put(left && good);
-            left = left && !good;
-            prompt_top<D, true>(p, t.row0 + key0, end - key0, kv_head, threadIdx.x, 256, &s_top);
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // q's room is written by TMA again
-            sync();
-        } while (true);
-        put(left);
+        } while (again());
+        // through q's room, which nothing reads any more
+        const uint32_t staging = s_q + tile * kQTile + quarter * (32 * 2 * D);
+#pragma unroll
+        for (int k = 0; k < D / 8; ++k) kv8_put16(prompt_staged<2 * D>(staging, lane, k), w[4 * k], w[4 * k + 1], w[4 * k + 2], w[4 * k + 3]);
+        if (careful) prompt_within<2 * D, true>(staging);  // (means of finite values, that roundings have carried over the end)
+        prompt_put_rows<2 * D>(p.out, mine ? 2 * ((t.row0 + position) * p.out_stride + (head0 + r - at * pack) * D) : -1, staging);
         if (!good) prompt_flag(p, t.index, s_failed ? kStatusDevice : kStatusNonFinite);
     }
     __syncwarp();
@@ -713,6 +686,8 @@ __device__ __forceinline__ void bf16x2_slices(float2 x, uint32_t (&w)[3]) {
 __device__ __forceinline__ constexpr int prompt_slice_a(int i) { return i == 0 ? 2 : i == 1 || i == 3 ? 1 : 0; }
 __device__ __forceinline__ constexpr int prompt_slice_b(int i) { return i == 2 ? 2 : i == 1 || i == 4 ? 1 : 0; }
 
+constexpr float kBf16Most = 3.38953139e38f;  // the largest bf16
+
 template <int D>
 __global__ void __launch_bounds__(kPromptF32Threads, 1) prompt_f32_kernel(PromptParams p) {
     using Shape = PromptF32Shape<D>;
@@ -725,7 +700,6 @@ __global__ void __launch_bounds__(kPromptF32Threads, 1) prompt_f32_kernel(Prompt
     __shared__ uint32_t s_tmem;
     __shared__ PromptTile s_tile;
     __shared__ int s_failed, s_dirty;
-    __shared__ uint32_t s_top;  // careful: the largest value's bits
     __shared__ unsigned long long s_bad[2][kStages];  // careful: which of a turn's keys, values are not finite
     const uint32_t s_k = (smem_addr(smem_raw) + 1023) & ~1023u, s_v = s_k + kStages * 3 * kPlane;
     uint32_t bars = smem_addr(s_bars);  // of this pass
@@ -755,7 +729,7 @@ __global__ void __launch_bounds__(kPromptF32Threads, 1) prompt_f32_kernel(Prompt
             init(q_full(), 1, 4);
             init(idle(), 1, 2);
         }
-        s_failed = s_dirty = s_top = 0;
+        s_failed = s_dirty = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     pdl_wait();
@@ -791,13 +765,11 @@ __global__ void __launch_bounds__(kPromptF32Threads, 1) prompt_f32_kernel(Prompt
         __syncwarp();
         asm volatile("bar.sync 1, %0;" ::"n"(kPromptF32Threads) : "memory");
     };
-    // Every warp, at its end: whether the CTA starts over. The softmax's warps meet the others once more by themselves: when
-    // the rows that are done have been written.
-    const auto again = [&](bool writes) {
+    // Every warp, at its end: whether the CTA starts over.
+    const auto again = [&] {
         asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
         sync();
         if (careful || !s_dirty || s_failed) return false;
-        if (!writes) sync();
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         bars += 8 * kBars;
         return careful = true;
@@ -846,7 +818,7 @@ __global__ void __launch_bounds__(kPromptF32Threads, 1) prompt_f32_kernel(Prompt
                     for (int k = 0; k < 4; ++k) bf16x2_slices(make_float2(f[2 * k], f[2 * k + 1]), w[k]);
                     if (careful) {
                         bool bad = false;
-                        const float smaller = which ? prompt_pow2(-prompt_down(s_top, end - key0, 0)) : 1.0f;
+                        const float smaller = which ? prompt_pow2(-prompt_down(end - key0, 0)) : 1.0f;
 #pragma unroll
                         for (int k = 0; k < 8; ++k) bad |= !(fabsf(f[k]) <= kBf16Most) && (!which || !isfinite(f[k]));
                         if (bad) atomicOr(&s_bad[which][s], 1ull << row);
@@ -888,7 +860,7 @@ __global__ void __launch_bounds__(kPromptF32Threads, 1) prompt_f32_kernel(Prompt
                 put(c, n + 2);
                 load(c, n + 5);
             }
-        } while (again(false));
+        } while (again());
         else if (warp <= 5) do {
             constexpr uint32_t idesc_s = umma_idesc_bf16(128, kKeys), idesc_o = umma_idesc_bf16(128, D) | kUmmaBMnMajor;
             uint32_t leader;
@@ -932,9 +904,9 @@ __global__ void __launch_bounds__(kPromptF32Threads, 1) prompt_f32_kernel(Prompt
             mbar_settle(idle(), 0);
             if (ok) mbar_settle_ring(warp == 4 ? k_empty() : v_empty(), kStages, turns);
             __syncwarp();
-        } while (again(false));
+        } while (again());
         else do {
-        } while (again(false));
+        } while (again());
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kPromptF32SoftmaxRegisters));
         const int r = threadIdx.x, at = static_cast<int>(kv8_div(r, p.pack)), position = t.first + at;
@@ -947,17 +919,7 @@ __global__ void __launch_bounds__(kPromptF32Threads, 1) prompt_f32_kernel(Prompt
         constexpr int kChunk = Shape::kChunk, kRow = 4 * kChunk, kPieces = kChunk / 4, kEach = 32 / kPieces;
         const uint32_t staging = s_v + kStages * 3 * kPlane + warp * (32 * kRow);
         float o[D];
-        bool good = true, left = mine;  // left: not written yet
-        const auto put = [&](bool rows) {
-#pragma unroll
-            for (int c = 0; c < D; c += kChunk) {
-#pragma unroll
-                for (int k = 0; k < kPieces; ++k)
-                    kv8_put16(prompt_staged<kRow>(staging, lane, k), __float_as_uint(o[c + 4 * k]), __float_as_uint(o[c + 4 * k + 1]),
-                              __float_as_uint(o[c + 4 * k + 2]), __float_as_uint(o[c + 4 * k + 3]));
-                prompt_put_rows<kRow>(p.out, rows ? to_out + c * 4 : -1, staging);
-            }
-        };
+        bool good = true;
         do {
             // q by whole sectors into shared memory, then its slices by rows. (Loops that are not unrolled here and
             // below: code that runs once a CTA is bound by its own instructions' way from memory.)
@@ -1085,31 +1047,26 @@ __global__ void __launch_bounds__(kPromptF32Threads, 1) prompt_f32_kernel(Prompt
             }
             add_output(turns - 1);
             float inverse = *static_cast<volatile int*>(&s_failed) ? __int_as_float(0x7fc00000) : __fdiv_rn(1.0f, l);
-            if (careful) inverse *= prompt_pow2(prompt_down(s_top, end - key0, 0));
+            if (careful) inverse *= prompt_pow2(prompt_down(end - key0, 0));
             float clean = 0.0f;  // NaN once an output is not finite
 #pragma unroll
             for (int k = 0; k < D; ++k) {
                 o[k] *= inverse;
                 clean = fmaf(o[k], 0.0f, clean);
             }
-            if (careful) {
-                clean = 0.0f;
-#pragma unroll
-                for (int k = 0; k < D; ++k) {
-                    o[k] = prompt_within(o[k], 3.40282347e38f);
-                    clean = fmaf(o[k], 0.0f, clean);
-                }
-            }
-            good = !left || clean == 0.0f;
+            good = !mine || clean == 0.0f || (careful && inverse < INFINITY);
             if (!good) s_dirty = 1;
             __syncwarp();
-            if (!again(true)) break;
-            put(left && good);
-            left = left && !good;
-            prompt_top<D, false>(p, t.row0 + key0, end - key0, kv_head, threadIdx.x, 128, &s_top);
-            sync();
-        } while (true);
-        put(left);
+        } while (again());
+#pragma unroll
+        for (int c = 0; c < D; c += kChunk) {
+#pragma unroll
+            for (int k = 0; k < kPieces; ++k)
+                kv8_put16(prompt_staged<kRow>(staging, lane, k), __float_as_uint(o[c + 4 * k]), __float_as_uint(o[c + 4 * k + 1]),
+                          __float_as_uint(o[c + 4 * k + 2]), __float_as_uint(o[c + 4 * k + 3]));
+            if (careful) prompt_within<kRow, false>(staging);
+            prompt_put_rows<kRow>(p.out, to_out < 0 ? -1 : to_out + c * 4, staging);
+        }
         if (!good) prompt_flag(p, t.index, s_failed ? kStatusDevice : kStatusNonFinite);
     }
     __syncwarp();

@@ -75,7 +75,7 @@ def test_rows_beside_them(cuda_ok, in_place, dim, window, bf16):
     v[300, 0, dim - 1] = float("nan")
     v[500:503, 1, 3] = most(bf16)
     want, lim = formula(q, k, torch.where(v.isnan(), torch.zeros_like(v), v), begin, window, tol=bf16)
-    if in_place:  # rows that are done are written before the others are gone over again
+    if in_place:
         out, codes = q, torch.zeros(2, dtype=torch.int32, device="cuda")
         call(q, k, v, q, begin, bf16=bf16, window=window)(codes.data_ptr())
         torch.cuda.synchronize()
