@@ -4879,8 +4879,9 @@ int i8_product(const I8Params& p, int sms, cudaStream_t s) {
         return std::ceil(n / resident) * std::max(depths * each, out * ragged) + 3.0;
     };
     const double n64 = tiles(128, 64), n128 = tiles(128, 128);
+    const bool shared = 3 * ((depths + 3) / 4) < depths;  // a depth of which each CTA of a cluster has a part
     const double cost[6] = {whole(n64, 0.31, 1.2, sms), whole(n128, 0.345, 1.9, sms), whole(tiles(256, 256), 0.43, 4.0, sms / 2),
-                            4 * n64 > sms ? 1e30 : 6.3 + (depths + 3) / 4 * 0.31, 4 * n128 > sms ? 1e30 : 7.5 + (depths + 3) / 4 * 0.345,
+                            !shared || 4 * n64 > sms ? 1e30 : 6.3 + (depths + 3) / 4 * 0.31, !shared || 4 * n128 > sms ? 1e30 : 7.5 + (depths + 3) / 4 * 0.345,
                             p.rows > 32 ? 1e30 : 2.5 + 0.68e-6 * p.channels * p.depth};
     switch (std::min_element(cost, cost + 6) - cost) {
         case 0: return i8_tiles_launch<64, false, kBf16>(p, sms, s);

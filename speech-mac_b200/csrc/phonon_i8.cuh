@@ -696,7 +696,7 @@ __global__ void __launch_bounds__(kI8Threads, 1)
     int m, n;
     i8_place(p, static_cast<int>(blockIdx.x / splits), m, n);
     const int nk = (p.depth + 127) / 128, per = (nk + static_cast<int>(splits) - 1) / static_cast<int>(splits);
-    const int first = min(nk, static_cast<int>(rank) * per), turns = min(nk, first + per) - first;
+    const int first = static_cast<int>(rank) * per, turns = min(nk, first + per) - first;  // (at least one: by the choice of this kernel)
     pdl_wait();
     pdl_trigger();
     if (warp == 0 && lane == 0) {
@@ -739,10 +739,8 @@ __global__ void __launch_bounds__(kI8Threads, 1)
         for (int c = 0; c < kN; c += 32) {
             uint32_t r[32];
             tmem_load32(tmem + c + (static_cast<uint32_t>(quarter * 32) << 16), r);
-            const bool some = turns > 0;
 #pragma unroll
-            for (int k = 0; k < 32; k += 4)
-                kv8_put16(to + (c + k) * 4, some ? r[k] : 0, some ? r[k + 1] : 0, some ? r[k + 2] : 0, some ? r[k + 3] : 0);
+            for (int k = 0; k < 32; k += 4) kv8_put16(to + (c + k) * 4, r[k], r[k + 1], r[k + 2], r[k + 3]);
         }
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
