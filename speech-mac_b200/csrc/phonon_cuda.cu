@@ -4799,7 +4799,7 @@ int i8_rows_launch(const I8Params& p, cudaStream_t s) {
 bool i8_maps(const I8Params& p, uint32_t box_w, CUtensorMap* x, CUtensorMap* w) {
     const auto map = [&](CUtensorMap* m, const int8_t* base, int rows, long long stride, uint32_t box) {
         return make_map_2d(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, base, static_cast<uint64_t>(rows), static_cast<uint64_t>(p.depth),
-                           static_cast<uint64_t>(stride), kGemmKTile, box);
+                           static_cast<uint64_t>(rows > 1 ? stride : p.depth), kGemmKTile, box);  // (one row has no stride: any may be given)
     };
     return map(x, p.x, p.rows, p.x_stride, 128) && map(w, p.w, p.channels, p.w_stride, box_w);
 }
@@ -4954,7 +4954,7 @@ namespace {
 bool make_rows_map(CUtensorMap* map, const void* base, int rows, int heads, int dim, long long stride, int box, int box_heads, int box_rows) {
     EncodeTiledFn fn = encode_tiled();
     const cuuint64_t dims[3] = {static_cast<cuuint64_t>(dim), static_cast<cuuint64_t>(heads), static_cast<cuuint64_t>(rows)};
-    const cuuint64_t strides[2] = {static_cast<cuuint64_t>(dim) * 2, static_cast<cuuint64_t>(stride) * 2};
+    const cuuint64_t strides[2] = {static_cast<cuuint64_t>(dim) * 2, static_cast<cuuint64_t>(rows > 1 ? stride : static_cast<long long>(heads) * dim) * 2};
     const cuuint32_t boxes[3] = {static_cast<cuuint32_t>(box), static_cast<cuuint32_t>(box_heads), static_cast<cuuint32_t>(box_rows)};
     const cuuint32_t each[3] = {1, 1, 1};
     return fn && fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims, strides, boxes, each, CU_TENSOR_MAP_INTERLEAVE_NONE,
