@@ -4856,19 +4856,29 @@ int i8_split_launch(I8Params p, int splits, cudaStream_t s) {
 // start, then for every wave of tiles 128 bytes of depth at a time (0.31 us for
 // 64 channels, 0.345 for 128, 0.43 for a pair's 256 x 256), or the taking out
 // of a tile where that is longer (1.2 times as long where y's rows are not
-// 16-byte aligned); a split tile's sums take 3.3 and 4.5 us to meet. Up to
-// 16 rows always, and up to 32 where the weights are few, the rows' kernel.
-// us of the kernel chosen and of the next ones (rows x channels x depth):
-// 16 x 4096 x 4096 rows 6.2, split 9.5; 32 x 4096 x 4096 split by 4 8.9, 64
-// channels 13.7, rows 13.9; 32 x 512 x 2048 rows 4.7, split 5.0; 128 x 4096 x
-// 4096 split by 4 11.3, 64 channels 13.9; 512 x 512 x 2048 split by 4 6.9, 64
-// channels 8.1; 512 x 2048 x 512 64 channels 4.6, 128 5.4; 512 x 4096 x 4096
-// 128 channels 15.2, pairs 17.8, 64 channels 24.8; 1024 x 4096 x 4096 pairs
-// 18.8, 128 channels 26.6; 1001 x 5003 x 2064 pairs 21.8, 128 channels 25.7
-// (5008 channels: 20.5, 24.2); 700 x 9001 x 1040 pairs 16.9, 128 channels 17.6.
+// 16-byte aligned); a split tile's sums take 3.3 and 4.5 us to meet.
+//
+// us of the kernel that takes least and of the next ones (rows x channels x depth,
+// bf16, in a graph, operands from DRAM). Up to 16 rows always the rows' kernel: 16
+// x 4096 x 4096 5.8, split 9.9; 16 x 14336 x 4096 17.2, 128 channels 19.8; 16 x
+// 4096 x 14336 15.1, split 15.8; 16 x 2048 x 8192 7.8, split 10.2; 16 x 512 x 2048
+// 2.3, split 5.2. Its form for 8 rows, which has twice as much of the weights on
+// the way, where channels are many and the depth is not: 8 x 14336 x 4096 14.9
+// (that for 16: 16.2), 8 x 65536 x 512 16.9 (28.0); else that for 16: 8 x 4096 x
+// 14336 14.2 (20.7), 1 x 4096 x 4096 5.1 (5.8), 1 x 1536 x 512 1.8 (1.9), 8 x 8192
+// x 14336 28.8 (32.7).
+// 32 x 512 x 2048 rows 4.7, split 5.2; 32 x 1024 x 4096 split 7.4, rows 10.6; 32 x
+// 4096 x 1024 rows 5.3, split by 4 6.2; 32 x 4096 x 4096 split by 4 9.2, 128
+// channels 13.4, rows 14.0; 128 x 4096 x 4096 split by 4 11.6, 64 channels 13.7;
+// 512 x 512 x 2048 split by 4 7.1, 64 channels 8.2; 512 x 2048 x 512 64 channels
+// 4.5, 128 5.2; 512 x 4096 x 4096 128 channels 14.3, pairs 16.9, 64 channels 23.5;
+// 1024 x 4096 x 4096 pairs 17.8, 128 channels 24.2; 1001 x 5003 x 2064 pairs 21.3,
+// 128 channels 24.9 (5008 channels: 20.0, 23.5). The model errs by up to an
+// eighth: 32 x 512 x 4096 rows 7.6, split 6.7; 700 x 9001 x 1040 128 channels
+// 16.9, pairs 16.3.
 template <bool kBf16>
 int i8_product(const I8Params& p, int sms, cudaStream_t s) {
-    if (p.rows <= 8) return i8_rows_launch<1, kBf16>(p, s);
+    if (p.rows <= 8 && p.channels > 32 * sms && p.depth <= 4096) return i8_rows_launch<1, kBf16>(p, s);
     if (p.rows <= 16) return i8_rows_launch<2, kBf16>(p, s);
     const int depths = (p.depth + 127) / 128;
     const auto tiles = [&](int rows, int channels) {
@@ -4882,7 +4892,7 @@ int i8_product(const I8Params& p, int sms, cudaStream_t s) {
     const bool shared = 3 * ((depths + 3) / 4) < depths;  // a depth of which each CTA of a cluster has a part
     const double cost[6] = {whole(n64, 0.31, 1.2, sms), whole(n128, 0.345, 1.9, sms), whole(tiles(256, 256), 0.43, 4.0, sms / 2),
                             !shared || 4 * n64 > sms ? 1e30 : 6.3 + (depths + 3) / 4 * 0.31, !shared || 4 * n128 > sms ? 1e30 : 7.5 + (depths + 3) / 4 * 0.345,
-                            p.rows > 32 ? 1e30 : 2.5 + 0.68e-6 * p.channels * p.depth};
+                            p.rows > 32 ? 1e30 : 1.7 + (1.37e-3 + 0.52e-6 * p.channels) * p.depth};
     switch (std::min_element(cost, cost + 6) - cost) {
         case 0: return i8_tiles_launch<64, false, kBf16>(p, sms, s);
         case 1: return i8_tiles_launch<128, false, kBf16>(p, sms, s);

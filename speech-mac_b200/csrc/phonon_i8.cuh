@@ -209,7 +209,7 @@ __device__ __forceinline__ bool i8_store(void* y, size_t at, float v) {  // whet
 // 64c + 16t, whose words count as the depths that the fragments' order asks
 // for, in the rows' operand alike, so that nothing is exchanged.
 //
-// 1 x 4096 x 4096 in 5.9 us (2.8 TB/s), 8 x 14336 x 4096 in 14.8 (4.0), from
+// 1 x 4096 x 4096 in 5.1 us (3.3 TB/s), 8 x 14336 x 4096 in 14.9 (4.0), from
 // DRAM; 16 x 4096 x 4096 and the pass that quantises its rows in 9.2 together
 // (10.3 without the weights' prefetch). What is left is a chain:
 // the start, two rounds of loads, the sums' meeting. All loads of a warp ahead

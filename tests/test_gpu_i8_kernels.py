@@ -13,7 +13,7 @@ torch = pytest.importorskip("torch")
 
 ROWS, WIDE, SPLIT = "i8_rows_kernelILi%dE", "i8_product_kernelILi%dE", "i8_split_kernelILi%dE"
 SIZES = [  # the kernel, and rows x channels x depth with parts of tiles, odd rows and depths among them
-    (ROWS % 1, (7, 1003, 528)), (ROWS % 2, (13, 515, 1040)), (ROWS % 4, (31, 130, 400)),
+    (ROWS % 1, (7, 5003, 528)), (ROWS % 2, (1, 1003, 528)), (ROWS % 2, (13, 515, 1040)), (ROWS % 4, (31, 130, 400)),
     (WIDE % 64, (333, 1001, 272)), (WIDE % 128, (2049, 4100, 640)), ("i8_pair_kernel", (1030, 5003, 2064)),
     (SPLIT % 64, (127, 129, 2048)), (SPLIT % 64, (40, 513, 2064)),
     (SPLIT % 128, (32, 4096, 4096)), (SPLIT % 128, (100, 2501, 3088)), (SPLIT % 128, (40, 4099, 4112)), (SPLIT % 128, (200, 2047, 4080)),
