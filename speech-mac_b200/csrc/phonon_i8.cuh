@@ -910,9 +910,6 @@ __global__ void __launch_bounds__(kI8Threads, 1) __cluster_dims__(2, 1, 1)
         commit(idle);  // no product is on its way when the CTAs give their memory back
         mbar_settle(idle, 0);
         if (ok) mbar_settle_ring(empty, kStages, it);
-    } else if (warp == 1 && lane == 0) {
-        mbar_settle(idle, 0);
-        if (!*static_cast<volatile int*>(&s_failed)) mbar_settle_ring(empty, kStages, (tiles - first + step - 1) / step * nk);
     } else if (warp >= 2) {
         const int quarter = warp & 3;
         const uint32_t lead_drained = cluster_addr(drained, 0);
@@ -945,6 +942,13 @@ __global__ void __launch_bounds__(kI8Threads, 1) __cluster_dims__(2, 1, 1)
     __syncwarp();
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
+    // What the other CTA has committed here: not before the last tile has been taken out, however long that took.
+    if (rank != 0 && warp == 1) {  // a barrier a lane
+        const int j = (tiles - first + step - 1) / step * nk - lane;  // of the ring, from its last turn back
+        if (lane == 0) mbar_settle(idle, 0);
+        else if (lane <= kStages && j >= 0 && !*static_cast<volatile int*>(&s_failed)) mbar_settle(empty + 8 * (j % kStages), (j / kStages) & 1);
+    }
+    __syncwarp();
     cluster_meet();  // neither CTA's memory goes while the other may reach it
     if (warp == 1) {
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");

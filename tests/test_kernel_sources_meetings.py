@@ -31,3 +31,15 @@ def test_no_kernel_lets_the_next_launch_start_before_it_holds_its_tensor_memory(
             ahead = kernel[:kernel.index("pdl_trigger();")]
             assert "tcgen05.alloc" in ahead or re.search(r"static_assert\(k\w+Registers == 64 \* 1024,", ahead), path.name
     assert found >= 8
+
+
+def test_a_bounded_wait_for_the_last_commits_begins_when_the_work_is_over():
+    """The second CTA of a pair waits for the commits of the first before it gives its memory back. That wait is bounded by two
+    seconds, which a large product may take itself: it begins behind the barrier that all warps come to with their work done."""
+    code = re.sub(r"//.*", "", (CSRC / "phonon_i8.cuh").read_text())
+    kernel = code[code.index("i8_pair_kernel("):]
+    over = kernel.rindex("__syncthreads();")
+    settle = [m.start() for m in re.finditer(r"mbar_settle\(idle, 0\);", kernel)]
+    assert len(settle) == 2
+    ahead, behind = kernel[:settle[0]], kernel[over:settle[1]]
+    assert ahead.rstrip().endswith("commit(idle);") and settle[1] > over and "rank != 0" in behind
