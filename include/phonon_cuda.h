@@ -624,16 +624,19 @@ int phonon_cuda_i8_product_device(int device, const PhononCudaI8Product *args, i
  * (p - window, p], or [0, p] where window is 0. Rows of no prompt, before
  * row_begin[0] or from row_begin[prompts] on, are left as they were. max_rows
  * bounds every prompt's rows. Sums and softmax statistics are fp32; bf16 rows:
- * weights are rounded to bf16 (an output's error stays near its own rounding);
- * fp32 rows: parts of a query, key or value below 2^-133 count as 0.
+ * weights are rounded to bf16 before they meet the values, their sum is of the
+ * unrounded ones (an output's error is by a fifth to a third more than its own
+ * rounding's; fp32 rows have none of it); fp32 rows: parts of a query, key or
+ * value below 2^-133 count as 0.
  * Enqueued on `cuda_stream` of `device`, like the cache's calls; status_dev
  * (device, [prompts], optional, zeroed by the caller) is raised for a prompt
  *   - whose rows lie outside [0, rows), are more than max_rows or begin before
  *     an earlier entry of row_begin (INVALID_ARGUMENT): its rows of out stay;
  *   - with a non-finite output (NON_FINITE): a row that sees a value which is
  *     not finite, whatever its weight, or whose own query (fp32: times the
- *     scale, beyond 2.3e38) or a score is not, but for scores of -infinity
- *     beside others, which are weights of 0. Finite values give finite
+ *     scale, beyond 2.3e38) or a score (bf16: q k before the scale, too) is
+ *     not, but for scores of -infinity beside others, which are weights of 0.
+ *     All of the row's elements of that head are NaN. Finite values give finite
  *     outputs, up to the type's largest. Other rows are what they are without
  *     it (near it, bits of values below 2^-60 may be lost);
  *   - where the kernel gave up a bounded wait (DEVICE_ERROR, about two

@@ -209,8 +209,8 @@ __device__ __forceinline__ bool i8_store(void* y, size_t at, float v) {  // whet
 // 64c + 16t, whose words count as the depths that the fragments' order asks
 // for, in the rows' operand alike, so that nothing is exchanged.
 //
-// 1 x 4096 x 4096 in 5.1 us (3.3 TB/s), 8 x 14336 x 4096 in 14.9 (4.0), from
-// DRAM; 16 x 4096 x 4096 and the pass that quantises its rows in 9.2 together
+// 1 x 4096 x 4096 in 5.1 us (3.3 TB/s), 16 in 5.8, 8 x 14336 x 4096 in 14.9
+// (4.0), 16 in 17.2, from DRAM; 16 x 4096 x 4096 and the pass that quantises its rows in 9.2 together
 // (10.3 without the weights' prefetch). What is left is a chain:
 // the start, two rounds of loads, the sums' meeting. All loads of a warp ahead
 // of the first product took 6.6 us where two rounds took 6.2 (16 rows).
@@ -297,12 +297,14 @@ __device__ __forceinline__ void mbar_settle_ring(uint32_t bars, int stages, int 
 // channels in its shared memory and the products read both, so that a CTA's
 // copies are 32 KB for what takes 48 KB alone.
 //
-// 8192 x 16384 x 4096: 380 us, 2.9 * 10^15 operations a second (9 tenths of
-// twice the measured bf16 rate), bound by the tensor cores under the power
-// limit; 1024 x 4096 x 4096 18.7 us and 512 x 4096 x 4096 15.2, one wave each:
-// 0.35 to 0.43 us for 128 bytes of depth, which is what the copies from the L2
-// take (192 channels a pair, with 28 KB a stage, took 0.41: dropped). Tiles of
-// 128 x 256 by one CTA read a fifth more from the L2: dropped, too.
+// 8192 x 16384 x 4096, bound by the tensor cores under the power limit: 363 us
+// where a captured graph has a few of them (3.0 * 10^15 operations a second, 92 %
+// of twice the measured bf16 rate), 418 in a long loop of calls (2.6; 95 % of
+// twice the sustained rate). 1024 x 4096 x 4096 17.7 us and 512 x 4096 x 4096
+// 14.3, one wave each: 0.35 to 0.45 us for 128 bytes of depth, which is what the
+// copies from the L2 take (192 channels a pair, with 28 KB a stage, took 0.41
+// where 256 took 0.43: dropped). Tiles of 128 x 256 by one CTA read a fifth more
+// from the L2: dropped, too.
 constexpr int kI8Threads = 320;
 constexpr int kI8Staging = 8 * 32 * 64;  // bytes: 32 rows of 64 for each of warps 2-9
 
@@ -386,9 +388,9 @@ __device__ __forceinline__ void i8_store_words(const I8Params& p, uint32_t stagi
 // row stride; `taken` is called once they have left TMEM. scale, bias: the
 // tile's channels'; xs: the row's. failed: NaN. Rows that are a multiple of 16
 // bytes apart go 64 bytes at a time; others 128, a row a store, since what they
-// cost is the instructions of every store (1001 x 5003 x 2064, bf16: 21.7 us;
+// cost is the instructions of every store (1001 x 5003 x 2064, bf16: 21.4 us;
 // two rows a store, with their alignment seen to there, 30.5; 5008 channels
-// 20.5).
+// 20.0).
 template <bool kBf16, typename Taken>
 __device__ __forceinline__ void i8_take(const I8Params& p, uint32_t tmem, uint32_t staging, int row0, int n0, int c0, int c1,
                                         const float* scale, const float* bias, float xs, bool failed, const Taken& taken) {
@@ -656,8 +658,8 @@ __device__ __forceinline__ void cluster_meet() {
 // Few tiles: the depth of one is split over the CTAs of a cluster, whose sums
 // meet in shared memory (integers: the result does not depend on the split).
 // Bound by the weights' way to few CTAs and then by the meeting (3.3 us with 64
-// channels a tile, 4.5 with 128): 512 x 512 x 2048 in 7.3 us (a CTA a tile:
-// 8.1), 32 and 128 x 4096 x 4096 in 9.5 and 11.9 (13.7, 13.9).
+// channels a tile, 4.5 with 128): 512 x 512 x 2048 in 7.1 us (a CTA a tile:
+// 8.2), 32 and 128 x 4096 x 4096 in 9.2 and 11.6 (13.4, 13.7).
 template <int kN>
 __host__ __device__ constexpr int i8_split_stages() { return kN == 128 ? 6 : 8; }
 

@@ -152,6 +152,15 @@ __device__ __forceinline__ void prompt_put_rows(void* out, long long own, uint32
 //   warps 0-7  S to registers, its maximum, the weights 2^(s - M) as bf16 back
 //              over S (the A operand of P v), the sum of weights in fp32
 //
+// Weights are rounded to bf16, as the matrix instruction wants them beside bf16
+// values. It shows: an output's error against 64 bits is 1.95e-3 (prompts of up
+// to 512) to 2.2e-3 (of 8191, or a window of 250) of the outputs' norm, where
+// rounding the output alone makes 1.62e-3 to 1.66e-3. Two slices a weight bring
+// it down to that and take 13 % (64 dims, short) to 30 % (128 dims, long) more
+// time; the sum of the rounded weights in place of the exact ones makes no
+// difference that shows (1.97e-3 and 1.95e-3 in a model of 2000 positions) and
+// takes 4 % more with 128 dims. Rows in fp32 lose nothing.
+//
 // O stays in TMEM. M follows the maximum only where that would make weights
 // above 2^8: the tile's own warps then multiply O by 2^(M - M'), which they may
 // since S of a turn comes behind P v of the turn before in the tensor cores'
@@ -170,9 +179,11 @@ __device__ __forceinline__ void prompt_put_rows(void* out, long long own, uint32
 // what the second adds is kept small: more of it, behind branches that are not
 // taken, took calls with 128 dims 5 % longer.)
 //
-// Measured: prompts of 8191 and 7500, 32 heads on 8 x 128, 885 us, 1.2 PFLOP/s
-// of the products that rows see (73 % of the measured matrix rate); 4 of 4096,
-// 16 heads of 128 280 us, of 64 213 (0.98 and 0.65 PFLOP/s). With 128 dims
+// Measured: prompts of 8191 and 7500, 32 heads on 8 x 128: 880 us where a
+// captured graph has a few of them, 1.2 PFLOP/s of the products that rows see (73
+// % of the measured matrix rate), 1030 in a long loop of calls, under the power
+// limit (1.03; 74 % of the sustained rate). 4 of 4096 in a graph: 16 heads of 128
+// 265 to 300 us, of 64 212 (1.0 and 0.65 PFLOP/s). With 128 dims
 // matrix and exponential units are each busy half of the time, and the two
 // tiles' turns do not fill each other's gaps; with 64 the exponentials are the
 // most. 64 prompts of up to 512 take 40 us and 16 with a window of 250 61, bound
@@ -648,9 +659,10 @@ __global__ void __launch_bounds__(kPromptThreads, PromptShape<D>::kCtas)
 // Values that are not finite, sums that leave fp32's range: as for bf16 rows; of keys that are not, or would
 // not be as bf16, the careful CTA computes the scores one by one.
 //
-// Measured: 2 prompts of 4096, 16 heads of 128, 700 us, 196 TFLOP/s of the
-// products that rows see, 1.2 PFLOP/s of slices (72 % of the measured matrix
-// rate); of 64 366 us; 4 of 1024 to 2048, 8 x 64, 90 us. Long prompts are bound
+// Measured, in a graph: 2 prompts of 4096, 16 heads of 128, 710 to 820 us by the
+// power limit, 168 to 194 TFLOP/s of the products that rows see, 1.0 to 1.16
+// PFLOP/s of slices (71 % of the measured matrix rate); of 64 400 us; 4 of 1024
+// to 2048, 8 x 64, 90 us (97 among a user's calls). Long prompts are bound
 // by the tensor cores; short ones by a CTA's start, end and chain of turns
 // (one of 128: 9 us). Errors stay at or below those of the plain form in fp32
 // (0.1 to 0.5e-6 of the output's norm against 0.1 to 1.2e-6).

@@ -107,3 +107,23 @@ def test_large_values_of_many_long_prompts(cuda_ok, dim, heads, kvh, bf16):
     assert status == [0] * 10
     want, lim = formula(q, k, v, begin, tol=bf16)
     assert ((out.double() - want).abs() <= lim).all()
+
+
+@pytest.mark.parametrize("dim", [32, 64, 128])
+def test_keys_beyond_the_largest_bf16(cuda_ok, dim):
+    """fp32 keys beyond the largest bf16, beside queries so small that every score is a number: weights as of any others, values
+    large and small."""
+    rng = np.random.default_rng(dim + 3)
+    begin = begins([150, 70])
+    packed, q, k, v = rows_of(rng, begin[-1], 4, 2, dim, False)
+    q[..., 0] = torch.tensor(rng.uniform(-1e-37, 1e-37, q.shape[:2]), dtype=torch.float32, device="cuda")
+    k[20, 0, 0], k[90, 1, 0], k[160, 0, 0] = 3.4e38, -3.395e38, most(False)
+    v[30, 1] = 3.2e38
+    out, status = attend(q, k, v, begin, False)
+    assert status == [0, 0]
+    want, lim = formula(q, k, v, begin, tol=False)
+    # 3.395e38 is nearer to the largest bf16 than to the next power of two, so that it is one of three slices like any other key.
+    # Of a query, parts below 2^-133 count as 0: up to 2^-133 * 3.395e38 = 0.0312 of the scores beside that key, and
+    # expm1(2 * 0.0312) of a row's weights relative to one another.
+    lim[90:150, 2:] += np.expm1(2 * 2.0 ** -133 * 3.395e38) * formula(q, k, v.abs(), begin)[90:150, 2:]
+    assert ((out.double() - want).abs() <= lim).all()
