@@ -626,8 +626,9 @@ int phonon_cuda_i8_product_device(int device, const PhononCudaI8Product *args, i
  * bounds every prompt's rows. Sums and softmax statistics are fp32; bf16 rows:
  * weights are rounded to bf16 before they meet the values, their sum is of the
  * unrounded ones (an output's error is by a fifth to a third more than its own
- * rounding's; fp32 rows have none of it); fp32 rows: parts of a query, key or
- * value below 2^-133 count as 0.
+ * rounding's; fp32 rows have none of it). Weights below 2^-126 of a row's
+ * largest count as 0, and so do, of fp32 rows, parts of a query, key or value
+ * below 2^-133.
  * Enqueued on `cuda_stream` of `device`, like the cache's calls; status_dev
  * (device, [prompts], optional, zeroed by the caller) is raised for a prompt
  *   - whose rows lie outside [0, rows), are more than max_rows or begin before
